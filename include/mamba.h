@@ -107,6 +107,8 @@ const char *mamba_last_error(void);
  * projection GEMM (the model's forward projections, mamba_linear above 512
  * rows, mamba_gated_mlp_up by default).  Bit 5: the same for
  * the decode state update's bulk-copy waits (mamba_ssm_step, mamba_step).
+ * Bit 6: a wait of mamba_gated_recurrence or its backward pass for the
+ * sequence tile before it exceeded the same bound.
  * Waits for the device; clear != 0 resets them. */
 unsigned mamba_device_status(int clear);
 
@@ -357,6 +359,72 @@ int mamba_ssm_step(const void *x, int64_t x_row_stride, const void *delta,
                    const void *z, int64_t z_row_stride, void *y, int64_t y_row_stride,
                    float *state, int batch, int dim, int dstate, int x_dtype,
                    int delta_dtype, int bc_dtype, void *stream);
+
+/* Gated linear recurrence over [batch, seqlen, dim] (no reference
+ * counterpart; a sibling of the selective scan with one state per channel
+ * and gates that come from projections).  Per (b, t, d):
+ *   s = sigmoid(r),  a = exp(-c * softplus(lambda[d]) * s),
+ *   h_t = a * h_{t-1} + sqrt(1 - a^2) * sigmoid(i) * x,
+ * with h_{-1} = initial_state (zeros when NULL).
+ * x, r, i, h share `dtype` (MAMBA_F32 or MAMBA_F16); strides in elements,
+ * {batch, time}, channel stride 1; lambda, the states and every sum are
+ * FP32.  1 - a^2 is evaluated without cancellation for decays close to 1.
+ * lengths (NULL: every row has seqlen tokens): row b ends after
+ * lengths[b] tokens (values outside [0, seqlen] are clamped); later
+ * positions are neither read nor written, and final_state is the state
+ * after the row's last token (the initial state for an empty row).
+ * resets, [batch, seqlen] bytes (NULL: none): where nonzero, h_{t-1} counts
+ * as zero at that token, so several documents can share a row.
+ * Outputs must not overlap inputs or each other.  The kernels run on the
+ * device that is current in the calling thread. */
+typedef struct MambaRecurrenceArgs {
+    const void *x;
+    const void *r;
+    const void *i;
+    const float *lambda;        /* [dim] */
+    const float *initial_state; /* [batch, dim] or NULL (zeros) */
+    const int32_t *lengths;     /* [batch] or NULL */
+    const uint8_t *resets;      /* [batch, seqlen] or NULL */
+    void *h;                    /* forward: written; backward: the forward's output */
+    float *final_state;         /* [batch, dim] or NULL (forward only) */
+    int32_t batch, seqlen, dim, dtype;
+    float c;                    /* > 0 */
+    int64_t x_stride[2], r_stride[2], i_stride[2], h_stride[2];
+} MambaRecurrenceArgs;
+
+/* Gradients of the recurrence.  dh: gradient of h; dfinal_state: gradient
+ * of final_state or NULL (zeros).  Written: dx, dr, di (dtype, positions
+ * behind a row's length left as they were), dlambda [dim] FP32 (the sum over
+ * batch and time, overwritten, the same bits on every call) and
+ * dinitial_state [batch, dim] FP32 or NULL.  h_{t-1} is read from the
+ * forward's output, i.e. in `dtype`. */
+typedef struct MambaRecurrenceGrads {
+    const void *dh;
+    const float *dfinal_state;
+    void *dx;
+    void *dr;
+    void *di;
+    float *dlambda;
+    float *dinitial_state;
+    int64_t dh_stride[2], dx_stride[2], dr_stride[2], di_stride[2];
+} MambaRecurrenceGrads;
+
+/* Scratch bytes of one call (backward != 0: of the backward pass); 0 when
+ * it needs none or the args are invalid.  16-byte aligned device memory.
+ * Calls (or captured graphs) that share a workspace must not overlap on the
+ * GPU; nothing in it carries over from one call to the next. */
+size_t mamba_gated_recurrence_workspace(const MambaRecurrenceArgs *a, int backward);
+int mamba_gated_recurrence(const MambaRecurrenceArgs *a, void *workspace, size_t workspace_bytes, void *stream);
+int mamba_gated_recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads *g, void *workspace,
+                                    size_t workspace_bytes, void *stream);
+
+/* One token of the gated recurrence (decode): rows of the given row strides
+ * (channel stride 1), state_in and state_out FP32 [batch, dim] (state_out
+ * may be state_in).  Writes h (dtype) and state_out. */
+int mamba_gated_recurrence_step(const void *x, int64_t x_row_stride, const void *r, int64_t r_row_stride,
+                                const void *i, int64_t i_row_stride, const float *lambda, const float *state_in,
+                                float *state_out, void *h, int64_t h_row_stride, int batch, int dim, float c,
+                                int dtype, void *stream);
 
 /* RMSNorm (rmsnorm.metal:11-81): y = x * rsqrt(mean(x^2) + eps) * w.
  * x [rows, cols] of in_dtype, y [rows, cols] of out_dtype, w FP32 [cols]

@@ -45,6 +45,15 @@ int causal_conv1d_step(const void *x, int64_t xrs, const float *w, const float *
                        int64_t yrs, float *state, int batch, int D, int K, int silu, int dtype,
                        cudaStream_t st);
 
+// recurrence.cu
+size_t recurrence_workspace_bytes(const MambaRecurrenceArgs *a, bool backward);
+int recurrence_forward(const MambaRecurrenceArgs *a, void *ws, size_t ws_bytes, cudaStream_t st);
+int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads *g, void *ws, size_t ws_bytes,
+                        cudaStream_t st);
+int recurrence_step(const void *x, int64_t xrs, const void *r, int64_t rrs, const void *i, int64_t irs,
+                    const float *lambda, const float *state_in, float *state_out, void *h, int64_t hrs, int batch,
+                    int dim, float c, int dtype, cudaStream_t st);
+
 // norm.cu
 int rmsnorm(const void *x, const float *w, void *y, int64_t rows, int cols, float eps, int in_dt,
             int out_dt, cudaStream_t st);

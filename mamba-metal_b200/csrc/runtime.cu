@@ -1464,6 +1464,32 @@ int mamba_rmsnorm(const void *x, const float *w, void *y, int64_t rows, int cols
                                                                                                         : 0;
 }
 
+size_t mamba_gated_recurrence_workspace(const MambaRecurrenceArgs *a, int backward) {
+    return mb::recurrence_workspace_bytes(a, backward != 0);
+}
+
+int mamba_gated_recurrence(const MambaRecurrenceArgs *a, void *workspace, size_t workspace_bytes, void *stream) {
+    mb::clear_error();
+    return mb::recurrence_forward(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)) ? -1 : 0;
+}
+
+int mamba_gated_recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads *g, void *workspace,
+                                    size_t workspace_bytes, void *stream) {
+    mb::clear_error();
+    return mb::recurrence_backward(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)) ? -1 : 0;
+}
+
+int mamba_gated_recurrence_step(const void *x, int64_t x_row_stride, const void *r, int64_t r_row_stride,
+                                const void *i, int64_t i_row_stride, const float *lambda, const float *state_in,
+                                float *state_out, void *h, int64_t h_row_stride, int batch, int dim, float c,
+                                int dtype, void *stream) {
+    mb::clear_error();
+    return mb::recurrence_step(x, x_row_stride, r, r_row_stride, i, i_row_stride, lambda, state_in, state_out, h,
+                               h_row_stride, batch, dim, c, dtype, static_cast<cudaStream_t>(stream))
+               ? -1
+               : 0;
+}
+
 int mamba_propagate_tile_carries(float *carries, int num_tiles, int64_t width, float *total, void *stream) {
     mb::clear_error();
     return mb::propagate_tile_carries(carries, num_tiles, width, total, static_cast<cudaStream_t>(stream)) ? -1 : 0;

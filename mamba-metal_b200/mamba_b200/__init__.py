@@ -16,6 +16,8 @@ Reference interface mirrored (SNAPKITTYWEST/mamba-metal):
   causal_conv1d, causal_conv1d_step, ssm_step, rmsnorm
                    (Sources/Kernels/causal_conv1d.metal, state_update.metal,
                    rmsnorm.metal)
+Without a counterpart in the reference: gated_recurrence (with its backward
+pass and single-token step).
 """
 import ctypes
 import os
@@ -69,6 +71,22 @@ class MambaScanArgs(ctypes.Structure):
                 ("C_stride", c_i64 * 3), ("z_stride", c_i64 * 3), ("y_stride", c_i64 * 3)]
 
 
+class MambaRecurrenceArgs(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("r", c_void_p), ("i", c_void_p), ("lambda_", c_void_p),
+                ("initial_state", c_void_p), ("lengths", c_void_p), ("resets", c_void_p), ("h", c_void_p),
+                ("final_state", c_void_p),
+                ("batch", ctypes.c_int32), ("seqlen", ctypes.c_int32), ("dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("c", c_float),
+                ("x_stride", c_i64 * 2), ("r_stride", c_i64 * 2), ("i_stride", c_i64 * 2), ("h_stride", c_i64 * 2)]
+
+
+class MambaRecurrenceGrads(ctypes.Structure):
+    _fields_ = [("dh", c_void_p), ("dfinal_state", c_void_p), ("dx", c_void_p), ("dr", c_void_p), ("di", c_void_p),
+                ("dlambda", c_void_p), ("dinitial_state", c_void_p),
+                ("dh_stride", c_i64 * 2), ("dx_stride", c_i64 * 2), ("dr_stride", c_i64 * 2),
+                ("di_stride", c_i64 * 2)]
+
+
 # Every symbol include/mamba.h declares, with its ctypes prototype.
 _PROTOTYPES = {
     "mamba_create": (c_void_p, [ctypes.POINTER(MambaConfig)]),
@@ -120,6 +138,12 @@ _PROTOTYPES = {
                                c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "mamba_rmsnorm": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, c_float, c_int, c_int,
                               c_void_p]),
+    "mamba_gated_recurrence_workspace": (c_size, [ctypes.POINTER(MambaRecurrenceArgs), c_int]),
+    "mamba_gated_recurrence": (c_int, [ctypes.POINTER(MambaRecurrenceArgs), c_void_p, c_size, c_void_p]),
+    "mamba_gated_recurrence_backward": (c_int, [ctypes.POINTER(MambaRecurrenceArgs),
+                                                ctypes.POINTER(MambaRecurrenceGrads), c_void_p, c_size, c_void_p]),
+    "mamba_gated_recurrence_step": (c_int, [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_void_p,
+                                            c_void_p, c_void_p, c_i64, c_int, c_int, c_float, c_int, c_void_p]),
     "mamba_propagate_tile_carries": (c_int, [c_void_p, c_int, c_i64, c_void_p, c_void_p]),
     "mamba_gated_silu_mul": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, c_void_p]),
     "mamba_gated_mlp_up": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, c_int, c_void_p]),
@@ -576,6 +600,188 @@ def rmsnorm(x, w=None, eps=1e-5, out_dtype=None, y=None, stream=None):
     _check(lib().mamba_rmsnorm(_ptr(x), _ptr(w), _ptr(y), rows, cols, eps, _dt(x), _dt(y),
                                _stream(stream)), "mamba_rmsnorm")
     return y
+
+
+def _require(cond, msg):
+    """Argument checks of the tensor-level helpers: MambaError, like the library's own refusals."""
+    if not cond:
+        raise MambaError(msg)
+
+
+def _check_tensor(t, name, what, shape, dtype, device, strided=False):
+    """t is a tensor of this shape, dtype and device, contiguous or (strided) with channel stride 1."""
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device:
+        raise MambaError("%s: %s must be %s %s on %s, got %s %s on %s"
+                         % (what, name, dtype, tuple(shape), device, t.dtype, tuple(t.shape), t.device))
+    if strided:
+        _require(t.shape[-1] <= 1 or t.stride(-1) == 1, "%s: %s needs channel stride 1" % (what, name))
+    else:
+        _require(t.is_contiguous(), "%s: %s must be contiguous" % (what, name))
+
+
+def _stream_of(t, stream):
+    """The stream handle of a call on t's device: the caller's, else that device's current stream."""
+    if stream is None:
+        return _torch().cuda.current_stream(t.device).cuda_stream
+    return _stream(stream)
+
+
+class _on_device:
+    """Makes a tensor's device current for a library call (no CUDA call when it already is)."""
+
+    def __init__(self, t):
+        torch = _torch()
+        _require(t.is_cuda, "tensors must be on a CUDA device")
+        self._dev = t.device.index
+        self._prev = torch.cuda.current_device()
+
+    def __enter__(self):
+        if self._prev != self._dev:
+            _torch().cuda.set_device(self._dev)
+
+    def __exit__(self, *exc):
+        if self._prev != self._dev:
+            _torch().cuda.set_device(self._prev)
+
+
+def _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets):
+    torch = _torch()
+    _require(x.dim() == 3, "%s: x must be [batch, seqlen, dim]" % what)
+    bsz, L, dim = x.shape
+    dev = x.device
+    _require(x.dtype in (torch.float16, torch.float32), "%s: x must be float16 or float32" % what)
+    _check_tensor(x, "x", what, x.shape, x.dtype, dev, True)
+    _check_tensor(r, "r", what, x.shape, x.dtype, dev, True)
+    _check_tensor(i, "i", what, x.shape, x.dtype, dev, True)
+    _check_tensor(lam, "lam", what, (dim,), torch.float32, dev)
+    if initial_state is not None:
+        _check_tensor(initial_state, "initial_state", what, (bsz, dim), torch.float32, dev)
+    if lengths is not None:
+        _check_tensor(lengths, "lengths", what, (bsz,), torch.int32, dev)
+    if resets is not None:
+        if resets.dtype == torch.bool:
+            resets = resets.view(torch.uint8)
+        _check_tensor(resets, "resets", what, (bsz, L), torch.uint8, dev)
+    a = MambaRecurrenceArgs()
+    a.x, a.r, a.i, a.lambda_ = x.data_ptr(), r.data_ptr(), i.data_ptr(), lam.data_ptr()
+    a.initial_state, a.lengths, a.resets = _ptr(initial_state), _ptr(lengths), _ptr(resets)
+    a.batch, a.seqlen, a.dim, a.dtype, a.c = bsz, L, dim, _dt(x), c
+    a.x_stride[:] = x.stride()[:2]
+    a.r_stride[:] = r.stride()[:2]
+    a.i_stride[:] = i.stride()[:2]
+    return a
+
+
+def _recurrence_out(name, what, out, x, lengths):
+    """An output like x; fresh ones are zeroed when rows end early, since
+    positions behind a row's end are not written."""
+    torch = _torch()
+    if out is None:
+        make = torch.empty if lengths is None else torch.zeros
+        return make(x.shape, dtype=x.dtype, device=x.device)
+    _check_tensor(out, name, what, x.shape, x.dtype, x.device, True)
+    return out
+
+
+def _recurrence_workspace(what, a, backward, workspace, x):
+    need = lib().mamba_gated_recurrence_workspace(ctypes.byref(a), int(backward))
+    if need and workspace is None:
+        workspace = _torch().empty(need, dtype=_torch().uint8, device=x.device)
+    if workspace is None:
+        return None, None, 0
+    _require(workspace.is_contiguous() and workspace.device == x.device,
+             "%s: workspace must be contiguous and on the tensors' device" % what)
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def gated_recurrence(x, r, i, lam, c=8.0, initial_state=None, lengths=None, resets=None,
+                     return_final_state=False, h=None, workspace=None, stream=None):
+    """Gated linear recurrence (mamba_gated_recurrence):
+    h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t,
+    a_t = exp(-c softplus(lam) sigmoid(r_t)).
+
+    x, r, i: [batch, L, dim] views, F16 or F32, channel stride 1; lam FP32
+    [dim]; initial_state FP32 [batch, dim]; lengths int32 [batch] (a padded
+    batch: positions behind a row's end are left as they were, zero in a
+    fresh h); resets uint8 or bool [batch, L] (the state counts as zero
+    before a marked token).  Returns h (x's dtype) and, if asked, the FP32
+    state after each row's last token."""
+    torch = _torch()
+    what = "gated_recurrence"
+    a = _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets)
+    h = _recurrence_out("h", what, h, x, lengths)
+    a.h = h.data_ptr()
+    a.h_stride[:] = h.stride()[:2]
+    hN = torch.empty((a.batch, a.dim), dtype=torch.float32, device=x.device) if return_final_state else None
+    a.final_state = _ptr(hN)
+    with _on_device(x):
+        ws, ws_ptr, ws_len = _recurrence_workspace(what, a, False, workspace, x)
+        _check(lib().mamba_gated_recurrence(ctypes.byref(a), ws_ptr, ws_len, _stream_of(x, stream)),
+               "mamba_gated_recurrence")
+    return (h, hN) if return_final_state else h
+
+
+def gated_recurrence_backward(dh, x, r, i, lam, h, c=8.0, initial_state=None, lengths=None, resets=None,
+                              dfinal_state=None, dx=None, dr=None, di=None, workspace=None, stream=None):
+    """Gradients of gated_recurrence (mamba_gated_recurrence_backward): dh is
+    the gradient of h, dfinal_state (FP32 [batch, dim] or None) that of the
+    final state; h is the forward's output.  Returns (dx, dr, di, dlam,
+    dinitial_state); dlam and dinitial_state are FP32."""
+    torch = _torch()
+    what = "gated_recurrence_backward"
+    a = _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets)
+    _check_tensor(h, "h", what, x.shape, x.dtype, x.device, True)
+    _check_tensor(dh, "dh", what, x.shape, x.dtype, x.device, True)
+    a.h = h.data_ptr()
+    a.h_stride[:] = h.stride()[:2]
+    if dfinal_state is not None:
+        _check_tensor(dfinal_state, "dfinal_state", what, (a.batch, a.dim), torch.float32, x.device)
+    dx, dr, di = (_recurrence_out(n, what, t, x, lengths) for n, t in (("dx", dx), ("dr", dr), ("di", di)))
+    dlam = torch.empty((a.dim,), dtype=torch.float32, device=x.device)
+    dh0 = torch.empty((a.batch, a.dim), dtype=torch.float32, device=x.device)
+    g = MambaRecurrenceGrads()
+    g.dh, g.dfinal_state, g.dx, g.dr, g.di = dh.data_ptr(), _ptr(dfinal_state), _ptr(dx), _ptr(dr), _ptr(di)
+    g.dlambda, g.dinitial_state = dlam.data_ptr(), dh0.data_ptr()
+    g.dh_stride[:] = dh.stride()[:2]
+    g.dx_stride[:] = dx.stride()[:2]
+    g.dr_stride[:] = dr.stride()[:2]
+    g.di_stride[:] = di.stride()[:2]
+    with _on_device(x):
+        ws, ws_ptr, ws_len = _recurrence_workspace(what, a, True, workspace, x)
+        _check(lib().mamba_gated_recurrence_backward(ctypes.byref(a), ctypes.byref(g), ws_ptr, ws_len,
+                                                     _stream_of(x, stream)), "mamba_gated_recurrence_backward")
+    return dx, dr, di, dlam, dh0
+
+
+def gated_recurrence_step(x, r, i, lam, state, c=8.0, state_out=None, h=None, stream=None):
+    """One token of the gated recurrence (mamba_gated_recurrence_step): x, r,
+    i [batch, dim] (row stride any, channel stride 1), state FP32 [batch,
+    dim].  state_out may be the state itself (update in place); by default
+    the state is left alone.  Returns (h, state_out)."""
+    torch = _torch()
+    what = "gated_recurrence_step"
+    _require(x.dim() == 2, "%s: x must be [batch, dim]" % what)
+    _require(x.dtype in (torch.float16, torch.float32), "%s: x must be float16 or float32" % what)
+    bsz, dim = x.shape
+    dev = x.device
+    for name, t in (("x", x), ("r", r), ("i", i)):
+        _check_tensor(t, name, what, x.shape, x.dtype, dev, True)
+    _check_tensor(lam, "lam", what, (dim,), torch.float32, dev)
+    _check_tensor(state, "state", what, x.shape, torch.float32, dev)
+    if state_out is None:
+        state_out = torch.empty((bsz, dim), dtype=torch.float32, device=dev)
+    else:
+        _check_tensor(state_out, "state_out", what, x.shape, torch.float32, dev)
+    if h is None:
+        h = torch.empty((bsz, dim), dtype=x.dtype, device=dev)
+    else:
+        _check_tensor(h, "h", what, x.shape, x.dtype, dev, True)
+    with _on_device(x):
+        _check(lib().mamba_gated_recurrence_step(x.data_ptr(), x.stride(0), r.data_ptr(), r.stride(0), i.data_ptr(),
+                                                 i.stride(0), lam.data_ptr(), state.data_ptr(), state_out.data_ptr(),
+                                                 h.data_ptr(), h.stride(0), bsz, dim, c, _dt(x),
+                                                 _stream_of(x, stream)), "mamba_gated_recurrence_step")
+    return h, state_out
 
 
 def propagate_tile_carries(carries, total=None, stream=None):

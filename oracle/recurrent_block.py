@@ -1,0 +1,76 @@
+"""The recurrent-block operators in FP64 numpy, from their definitions:
+gated linear recurrence (forward, backward), block norm (forward, backward),
+row quantisation and the 8-bit linear layer.
+
+Beside each result the functions give a magnitude: the sum of the absolute
+values of the terms that the result adds up, which is what rounding errors
+of a lower-precision evaluation scale with."""
+import numpy as np
+
+
+def sigmoid(v):
+    e = np.exp(-np.abs(v))
+    return np.where(v >= 0, 1.0, e) / (1 + e)
+
+
+def softplus(v):
+    return np.maximum(v, 0) + np.log1p(np.exp(-np.abs(v)))
+
+
+def _gates(r, i, lam, c):
+    y = c * softplus(lam) * sigmoid(r)
+    return y, np.exp(-y), np.sqrt(-np.expm1(-2 * y)), sigmoid(i)
+
+
+def gated_recurrence(x, r, i, lam, c, h0=None, lengths=None, resets=None):
+    """Returns (h, final state, magnitude of h); positions behind a row's end are zero."""
+    x, r, i, lam = (np.asarray(v, np.float64) for v in (x, r, i, lam))
+    B, L, D = x.shape
+    n = np.full(B, L) if lengths is None else np.clip(lengths, 0, L)
+    h = np.zeros((B, D)) if h0 is None else np.asarray(h0, np.float64).copy()
+    m = np.abs(h)
+    out, mag = np.zeros((B, L, D)), np.zeros((B, L, D))
+    for t in range(L):
+        live = (t < n)[:, None]
+        rt, it, xt = (np.where(live, v[:, t], 0.0) for v in (r, i, x))
+        _, a, beta, si = _gates(rt, it, lam, c)
+        if resets is not None:
+            a = np.where(resets[:, t, None] != 0, 0.0, a)
+        b = beta * si * xt
+        h, m = np.where(live, a * h + b, h), np.where(live, a * m + np.abs(b), m)
+        out[:, t], mag[:, t] = np.where(live, h, 0), np.where(live, m, 0)
+    return out, h, mag
+
+
+def gated_recurrence_backward(dh, x, r, i, lam, h, c, h0=None, lengths=None, resets=None, dfinal=None):
+    """Returns dicts (gradients, magnitudes) with keys dx, dr, di, dlam, dh0; h_{t-1} is taken from h."""
+    dh, x, r, i, lam, h = (np.asarray(v, np.float64) for v in (dh, x, r, i, lam, h))
+    B, L, D = x.shape
+    n = np.full(B, L) if lengths is None else np.clip(lengths, 0, L)
+    C = np.zeros((B, D)) if dfinal is None else np.asarray(dfinal, np.float64).copy()
+    Cm = np.abs(C)
+    g = {k: np.zeros((B, L, D)) for k in ("dx", "dr", "di")}
+    mag = {k: np.zeros((B, L, D)) for k in ("dx", "dr", "di")}
+    dsp, dspm = np.zeros(D), np.zeros(D)
+    first = np.zeros((B, D)) if h0 is None else np.asarray(h0, np.float64)
+    for t in range(L - 1, -1, -1):
+        live = (t < n)[:, None]
+        rt, it, xt, dht = (np.where(live, v[:, t], 0.0) for v in (r, i, x, dh))
+        y, a, beta, si = _gates(rt, it, lam, c)
+        keep = np.ones((B, 1)) if resets is None else (resets[:, t, None] == 0).astype(float)
+        prev = np.where(live & (keep > 0), h[:, t - 1] if t else first, 0.0)
+        G, Gm = dht + C, np.abs(dht) + Cm
+        dbeta_dy = np.where(beta > 0, a * a / np.where(beta > 0, beta, 1.0), 0.0)
+        t1, t2 = si * xt * dbeta_dy, a * prev
+        s = sigmoid(rt)
+        dy_dr = c * softplus(lam) * s * sigmoid(-rt)
+        for k, v, vm in (("dx", G * beta * si, Gm * beta * si),
+                         ("di", G * beta * xt * si * sigmoid(-it), Gm * np.abs(beta * xt * si * sigmoid(-it))),
+                         ("dr", G * (t1 - t2) * dy_dr, Gm * (np.abs(t1) + np.abs(t2)) * dy_dr)):
+            g[k][:, t], mag[k][:, t] = np.where(live, v, 0), np.where(live, vm, 0)
+        dsp += np.where(live, G * (t1 - t2) * s, 0).sum(0)
+        dspm += np.where(live, Gm * (np.abs(t1) + np.abs(t2)) * s, 0).sum(0)
+        C, Cm = np.where(live, keep * a * G, C), np.where(live, keep * a * Gm, Cm)
+    g["dlam"], mag["dlam"] = c * sigmoid(lam) * dsp, c * sigmoid(lam) * dspm
+    g["dh0"], mag["dh0"] = C, Cm
+    return g, mag

@@ -1,0 +1,346 @@
+"""GPU parity of the gated linear recurrence (forward, backward, step) against
+the FP64 oracle on the same (rounded) inputs.
+
+Tolerance, per element: |gpu - ref| <= u |ref| + d * mag + tiny, where u is the
+output type's half step (2^-11 FP16, 2^-24 FP32), tiny half of FP16's smallest
+step, and mag the largest magnitude (sum of absolute terms) in the tensor.
+d bounds the FP32 evaluation: per token ~16 roundings of 2^-24 in the gates
+and one in the running sum, which stays for at most 1/(1 - a) <= 2000 tokens
+of these inputs: d = 2^-24 (16 + min(L, 2000)); FP16 tensors add 1e-5 for the
+short series and the approximate exponentials."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import mamba_b200 as mb
+from oracle import recurrent_block as rb
+
+pytestmark = pytest.mark.gpu
+C = 8.0
+
+
+def _case(seed, B, L, D, dtype, ragged=False, resets=False, h0=True):
+    rng = np.random.default_rng(seed)
+    np_t = np.float16 if dtype == torch.float16 else np.float32
+    v = {k: rng.standard_normal((B, L, D)).astype(np_t) for k in ("x", "r", "i", "dh")}
+    decay = rng.uniform(0.9, 0.999, D)
+    v["lam"] = np.log(np.expm1(-np.log(decay) / C)).astype(np.float32)
+    v["h0"] = rng.standard_normal((B, D)).astype(np.float32) if h0 else None
+    v["dfinal"] = rng.standard_normal((B, D)).astype(np.float32) if h0 else None
+    v["lengths"] = v["resets"] = None
+    if ragged:
+        v["lengths"] = rng.integers(0, L + 1, B).astype(np.int32)
+        v["lengths"][-1] = 0
+        v["lengths"][0] = L
+    if resets:
+        v["resets"] = (rng.random((B, L)) < 0.1).astype(np.uint8)
+    return v
+
+
+def _dev(v):
+    return {k: None if a is None else torch.from_numpy(np.ascontiguousarray(a)).cuda() for k, a in v.items()}
+
+
+def _tol(dtype, L):
+    d = 2.0 ** -24 * (16 + min(L, 2000))
+    return (2.0 ** -11, d + 1e-5) if dtype == torch.float16 else (2.0 ** -24, d)
+
+
+def _close(got, ref, mag, u, d, name=""):
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all(), name
+    if not got.size:
+        return
+    err = np.abs(got - ref) - (u * np.abs(ref) + d * mag.max() + 2.0 ** -25)
+    assert err.max() <= 0, (name, err.max(), np.unravel_index(err.argmax(), err.shape))
+
+
+def _forward(t, **kw):
+    return mb.gated_recurrence(t["x"], t["r"], t["i"], t["lam"], c=C, initial_state=t["h0"], lengths=t["lengths"],
+                               resets=t["resets"], return_final_state=True, **kw)
+
+
+def _backward(t, h, **kw):
+    return mb.gated_recurrence_backward(t["dh"], t["x"], t["r"], t["i"], t["lam"], h, c=C, initial_state=t["h0"],
+                                        lengths=t["lengths"], resets=t["resets"], dfinal_state=t["dfinal"], **kw)
+
+
+def _check_forward(v, h, hN, dtype):
+    u, d = _tol(dtype, v["x"].shape[1])
+    ref, fin, mag = rb.gated_recurrence(v["x"], v["r"], v["i"], v["lam"], C, v["h0"], v["lengths"], v["resets"])
+    scale = np.concatenate([mag.ravel(), np.abs(fin).ravel()])
+    _close(h, ref, scale, u, d, "h")
+    _close(hN, fin, scale, 2.0 ** -24, d, "final state")
+
+
+def _check_backward(v, h, grads, dtype):
+    L = v["x"].shape[1]
+    u, d = _tol(dtype, L)
+    ref, mag = rb.gated_recurrence_backward(v["dh"], v["x"], v["r"], v["i"], v["lam"], h, C, v["h0"], v["lengths"],
+                                            v["resets"], v["dfinal"])
+    for got, k in zip(grads, ("dx", "dr", "di", "dlam", "dh0")):
+        scale = mag[k] if mag[k].size else np.zeros(1)
+        _close(got, ref[k], scale, u if k in ("dx", "dr", "di") else 2.0 ** -24, d, k)
+
+
+SHAPES = [(1, 1, 1), (2, 1, 64), (1, 7, 3), (3, 64, 64), (2, 65, 130), (2, 129, 66), (1, 257, 1001), (2, 300, 256),
+          (1, 2000, 96), (5, 17, 33), (2, 513, 72)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("ragged,resets,h0", [(False, False, False), (False, False, True), (True, False, True),
+                                              (False, True, True), (True, True, False)])
+@pytest.mark.parametrize("B,L,D", SHAPES)
+def test_forward_and_backward(cuda, B, L, D, ragged, resets, h0, dtype):
+    v = _case(B * 1000 + L + D, B, L, D, dtype, ragged, resets, h0)
+    t = _dev(v)
+    h, hN = _forward(t)
+    grads = _backward(t, h)
+    torch.cuda.synchronize()
+    assert mb.device_status() == 0
+    _check_forward(v, h, hN, dtype)
+    _check_backward(v, h.cpu().numpy(), grads, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("offset", [0, 1, 3])
+def test_strided_views(cuda, dtype, offset):
+    """x, r, i as column blocks of one wide projection whose rows are not
+    aligned to more than an element, time-major outputs, and a batch read
+    through a transposed view."""
+    B, L, D = 3, 150, 70
+    v = _case(5, B, L, D, dtype)
+    t = _dev(v)
+    wide = torch.full((L, B, 3 * D + 9), float("nan"), dtype=dtype, device="cuda")
+    views = {}
+    for k, name in enumerate(("x", "r", "i")):
+        views[name] = wide[:, :, offset + k * (D + 1):offset + k * (D + 1) + D].transpose(0, 1)
+        views[name].copy_(t[name])
+        t[name] = views[name]
+    out = torch.full((L, B, D + 5), float("nan"), dtype=dtype, device="cuda")
+    ho = out[:, :, offset:offset + D].transpose(0, 1)
+    h, hN = _forward(t, h=ho)
+    outs = [torch.full_like(out, float("nan")) for _ in range(3)]
+    grads = _backward(t, h, **{n: o[:, :, offset:offset + D].transpose(0, 1) for n, o in zip(("dx", "dr", "di"), outs)})
+    torch.cuda.synchronize()
+    assert h.data_ptr() == ho.data_ptr()
+    _check_forward(v, h, hN, dtype)
+    _check_backward(v, h.cpu().numpy(), grads, dtype)
+    for o in [out] + outs:  # nothing outside the views
+        assert o[:, :, :offset].isnan().all() and o[:, :, offset + D:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_padding_is_neither_read_nor_written(cuda, dtype):
+    B, L, D = 4, 200, 64
+    v = _case(9, B, L, D, dtype, ragged=True)
+    t = _dev(v)
+    for b, n in enumerate(v["lengths"]):
+        for k in ("x", "r", "i", "dh"):
+            t[k][b, n:] = float("nan") if b % 2 else float("inf")
+    mark = 7.0
+    h = torch.full((B, L, D), mark, dtype=dtype, device="cuda")
+    h, hN = _forward(t, h=h)
+    outs = [torch.full_like(h, mark) for _ in range(3)]
+    h_in = h.clone()
+    for b, n in enumerate(v["lengths"]):
+        h_in[b, n:] = float("nan")
+    grads = _backward(t, h_in, dx=outs[0], dr=outs[1], di=outs[2])
+    torch.cuda.synchronize()
+    for o in [h] + outs:
+        for b, n in enumerate(v["lengths"]):
+            assert (o[b, n:] == mark).all()
+            o[b, n:] = 0
+    _check_forward(v, h, hN, dtype)
+    _check_backward(v, h.cpu().numpy(), grads, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_lengths_outside_the_range_are_clamped(cuda, dtype):
+    v = _case(4, 3, 40, 32, dtype)
+    v["lengths"] = np.array([1000, -5, 40], np.int32)
+    t = _dev(v)
+    h, hN = _forward(t)
+    grads = _backward(t, h)
+    _check_forward(v, h, hN, dtype)
+    _check_backward(v, h.cpu().numpy(), grads, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_extreme_gates(cuda, dtype):
+    """Gates that close or open completely, decays of 0 and 1: finite, and
+    equal to the formulas' limits."""
+    B, L, D = 2, 70, 40
+    v = _case(2, B, L, D, dtype)
+    big = np.float32(60000.0) if dtype == torch.float16 else np.float32(3e38)
+    v["r"][:, ::3] = -big
+    v["r"][:, 1::7] = big
+    v["i"][:, ::5] = big
+    v["i"][:, 2::5] = -big
+    v["r"][:, 5::11] = -12.0
+    v["lam"][:8] = [-90, -40, -25, -15, 10, 40, 100, 0]
+    v["x"][:, ::13] = 0
+    t = _dev(v)
+    h, hN = _forward(t)
+    grads = _backward(t, h)
+    torch.cuda.synchronize()
+    _check_forward(v, h, hN, dtype)
+    _check_backward(v, h.cpu().numpy(), grads, dtype)
+
+
+def test_gradients_against_differences(cuda):
+    """FP32 gradients against central differences of the FP64 forward."""
+    v = _case(8, 2, 12, 6, torch.float32, ragged=True, resets=True)
+    v["lengths"] = np.array([12, 7], np.int32)
+    t = _dev(v)
+    h, _ = _forward(t)
+    grads = dict(zip(("x", "r", "i", "lam", "h0"), _backward(t, h)))
+    w = {k: v[k].astype(np.float64) for k in grads}
+
+    def loss():
+        hh, fin, _ = rb.gated_recurrence(w["x"], w["r"], w["i"], w["lam"], C, w["h0"], v["lengths"], v["resets"])
+        return (hh * v["dh"]).sum() + (fin * v["dfinal"]).sum()
+
+    for k, g in grads.items():
+        num = np.zeros_like(w[k])
+        for j in np.ndindex(num.shape):
+            keep = w[k][j]
+            w[k][j] = keep + 1e-5
+            up = loss()
+            w[k][j] = keep - 1e-5
+            num[j] = (up - loss()) / 2e-5
+            w[k][j] = keep
+        # FP32 rounding of the gradients (~2^-24 * 40 of the largest) + differences (1e-8)
+        assert np.abs(g.double().cpu().numpy() - num).max() < 1e-5 * max(1.0, np.abs(num).max()), k
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_empty_sizes(cuda, dtype):
+    t = _dev(_case(1, 3, 5, 8, dtype))
+    for k in ("x", "r", "i", "dh"):
+        t[k] = t[k][:, :0]
+    h, hN = _forward(t)
+    assert h.shape == (3, 0, 8) and torch.equal(hN, t["h0"])
+    dx, dr, di, dlam, dh0 = _backward(t, h)
+    assert dx.shape == (3, 0, 8) and torch.equal(dh0, t["dfinal"]) and not dlam.any()
+    t = _dev(_case(1, 3, 5, 8, dtype))
+    t = {k: a[:0] if a is not None and k not in ("lam",) else a for k, a in t.items()}
+    h, hN = _forward(t)
+    dlam = _backward(t, h)[3]
+    assert h.shape[0] == 0 and not dlam.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("B,L,D", [(2, 1500, 200), (8, 700, 1024)])
+def test_repeated_calls_give_the_same_bits(cuda, dtype, B, L, D):
+    t = _dev(_case(6, B, L, D, dtype))
+    first = None
+    for _ in range(5):
+        h, hN = _forward(t)
+        out = [h, hN] + list(_backward(t, h))
+        if first is None:
+            first = out
+        assert all(torch.equal(a, b) for a, b in zip(first, out))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_pieces_of_a_sequence_join(cuda, dtype):
+    """Prefill in two calls through the state, then single tokens: the same
+    function as one call over the whole sequence."""
+    B, L, D = 3, 90, 136
+    v = _case(12, B, L, D, dtype)
+    t = _dev(v)
+    whole, hN = _forward(t)
+    part = {k: a[:, :60] if k in ("x", "r", "i") else a for k, a in t.items()}
+    h1, s = _forward(part)
+    hs = [h1]
+    for k in range(60, L):
+        hk, s = mb.gated_recurrence_step(t["x"][:, k], t["r"][:, k], t["i"][:, k], t["lam"], s, c=C)
+        hs.append(hk[:, None])
+    h = torch.cat(hs, 1)
+    _check_forward(v, h, s, dtype)
+    _check_forward(v, whole, hN, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("B,D", [(1, 1), (1, 64), (7, 33), (256, 640), (3, 1001), (64, 1028)])
+def test_step(cuda, dtype, B, D):
+    v = _case(B + D, B, 1, D, dtype)
+    t = _dev(v)
+    keep = t["h0"].clone()
+    x, r, i = (t[k][:, 0] for k in ("x", "r", "i"))
+    h, s = mb.gated_recurrence_step(x, r, i, t["lam"], t["h0"], c=C)
+    assert torch.equal(t["h0"], keep)
+    _check_forward(v, h[:, None], s, dtype)
+    # in place, from the column blocks of one wide projection
+    wide = torch.zeros((B, 3 * D + 3), dtype=dtype, device="cuda")
+    views = [wide[:, 1 + k * (D + 1):1 + k * (D + 1) + D] for k in range(3)]
+    for w, a in zip(views, (x, r, i)):
+        w.copy_(a)
+    h2, s2 = mb.gated_recurrence_step(*views, t["lam"], keep, c=C, state_out=keep)
+    assert s2.data_ptr() == keep.data_ptr()
+    assert torch.equal(h2, h) and torch.equal(keep, s)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_streams_graphs_and_a_shared_workspace(cuda, dtype):
+    """On a side stream, two differently sized calls in turn on one workspace,
+    and a captured forward + backward replayed on new inputs."""
+    cases = [_case(20, 2, 700, 96, dtype), _case(21, 1, 1111, 40, dtype, resets=True)]
+    ts = [_dev(v) for v in cases]
+    need = 0
+    for t in ts:
+        a = mb._recurrence_args("t", t["x"], t["r"], t["i"], t["lam"], C, None, None, None)
+        need = max([need] + [mb.lib().mamba_gated_recurrence_workspace(ctypes.byref(a), k) for k in (0, 1)])
+    ws = torch.full((max(need, 16),), 0xAB, dtype=torch.uint8, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    results = []
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            for t in ts:
+                h, hN = _forward(t, workspace=ws)
+                results.append((h, hN, _backward(t, h, workspace=ws)))
+    side.synchronize()
+    for k, (h, hN, grads) in enumerate(results):
+        _check_forward(cases[k % 2], h, hN, dtype)
+        _check_backward(cases[k % 2], h.cpu().numpy(), grads, dtype)
+
+    t = ts[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h, hN = _forward(t)
+        grads = _backward(t, h)
+    for seed in (30, 31):
+        v = _case(seed, 2, 700, 96, dtype)
+        for k, a in _dev(v).items():
+            if a is not None:
+                t[k].copy_(a)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_forward(v, h, hN, dtype)
+        _check_backward(v, h.cpu().numpy(), grads, dtype)
+    assert mb.device_status() == 0
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """Rows that start more than 2^31 elements apart."""
+    L, D, gap = 40, 64, (1 << 31) + 64
+    free = torch.cuda.mem_get_info()[0]
+    if free < 3 * 2 * (gap + L * D):
+        pytest.skip("needs 13 GB of free device memory")
+    v = _case(3, 2, L, D, torch.float16)
+    t = _dev(v)
+    big = torch.zeros(gap + L * D, dtype=torch.float16, device="cuda")
+    out = torch.zeros(gap + L * D, dtype=torch.float16, device="cuda")
+    view = lambda buf: buf.as_strided((2, L, D), (gap, D, 1))  # noqa: E731
+    view(big).copy_(t["x"])
+    t["x"] = view(big)
+    h, hN = _forward(t, h=view(out))
+    _check_forward(v, h, hN, torch.float16)
+    t["h_big"] = h
+    out2 = torch.zeros(gap + L * D, dtype=torch.float16, device="cuda")
+    grads = _backward(t, h, dx=view(out2))
+    _check_backward(v, h.cpu().numpy(), grads, torch.float16)
