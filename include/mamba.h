@@ -432,6 +432,60 @@ int mamba_gated_recurrence_step(const void *x, int64_t x_row_stride, const void 
 int mamba_rmsnorm(const void *x, const float *w, void *y, int64_t rows, int cols, float eps,
                   int in_dtype, int out_dtype, void *stream);
 
+/* The join between two blocks of a residual stack (no reference counterpart
+ * as one op: rmsnorm_f32/_f16, rmsnorm.metal:11-81, on both sides of the
+ * residual add and the gate): the norm behind a block with its gate, the
+ * scaled residual add, and the norm before the next block.  Per row:
+ *   n = y * rsqrt(mean(y^2) + eps) * w_post [* SiLU(z)]
+ *   residual_out = residual_scale * residual + n
+ *   out = residual_out * rsqrt(mean(residual_out^2) + eps) * w_pre
+ * y, z, out [rows, cols] of `dtype` (MAMBA_F32 or MAMBA_F16), y and z with
+ * row strides in elements (channel stride 1), out contiguous; the residual
+ * stream and all sums FP32, contiguous.  NULL: z (no gate), a weight (ones),
+ * out (no second norm), rstd_* (not kept).  residual_out may be residual
+ * itself; otherwise outputs must not overlap inputs or each other.
+ * cols <= 16384. */
+typedef struct MambaBlockNormArgs {
+    const void *y;
+    const void *z;
+    const float *residual;
+    const float *w_post; /* [cols] */
+    const float *w_pre;  /* [cols] */
+    float *residual_out; /* forward: written; backward: the forward's output */
+    void *out;
+    float *rstd_post; /* [rows], 1 / sqrt(mean(y^2) + eps): kept for the backward pass */
+    float *rstd_pre;  /* [rows], the same of residual_out */
+    int64_t rows;
+    int32_t cols, dtype;
+    float residual_scale, eps;
+    int64_t y_stride, z_stride;
+} MambaBlockNormArgs;
+
+/* Gradients of the block norm.  dresidual_out (FP32) and dout (dtype) are
+ * the gradients of the two outputs; one of them may be NULL (zeros).
+ * Written: dresidual (FP32; may be dresidual_out itself), dy and dz (dtype,
+ * row strides in elements; dz only with a gate), and the column sums dw_post
+ * and dw_pre (FP32, overwritten, the same bits on every call; NULL: not
+ * wanted; dw_pre is zero without dout).  The call reads y, z, the weights,
+ * residual_out and rstd_* of `a` (not residual or out). */
+typedef struct MambaBlockNormGrads {
+    const float *dresidual_out;
+    const void *dout;
+    float *dresidual;
+    void *dy;
+    void *dz;
+    float *dw_post;
+    float *dw_pre;
+    int64_t dy_stride, dz_stride;
+} MambaBlockNormGrads;
+
+int mamba_block_norm(const MambaBlockNormArgs *a, void *stream);
+/* Scratch bytes of the backward pass (0 for invalid args), 16-byte aligned
+ * device memory; calls that share it must not overlap on the GPU. */
+size_t mamba_block_norm_workspace(const MambaBlockNormArgs *a);
+int mamba_block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *g, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
 /* Exclusive propagation of per-tile affine carries: the job of
  * propagate_tile_carries_f32 (prefix_scan.metal:19-40), with the pair layout
  * that kernel documents and its indexing fixed.  carries FP32

@@ -58,6 +58,12 @@ int recurrence_step(const void *x, int64_t xrs, const void *r, int64_t rrs, cons
 int rmsnorm(const void *x, const float *w, void *y, int64_t rows, int cols, float eps, int in_dt,
             int out_dt, cudaStream_t st);
 
+// block_norm.cu
+size_t block_norm_workspace_bytes(const MambaBlockNormArgs *a);
+int block_norm(const MambaBlockNormArgs *a, cudaStream_t st);
+int block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *g, void *ws, size_t ws_bytes,
+                        cudaStream_t st);
+
 // ssm_step.cu
 int ssm_step(const void *x, int64_t xrs, const void *delta, int64_t drs, const float *dt_bias,
              const void *B, const void *C, int64_t bcrs, const float *A, const float *Dskip,

@@ -1490,6 +1490,19 @@ int mamba_gated_recurrence_step(const void *x, int64_t x_row_stride, const void 
                : 0;
 }
 
+int mamba_block_norm(const MambaBlockNormArgs *a, void *stream) {
+    mb::clear_error();
+    return mb::block_norm(a, static_cast<cudaStream_t>(stream)) ? -1 : 0;
+}
+
+size_t mamba_block_norm_workspace(const MambaBlockNormArgs *a) { return mb::block_norm_workspace_bytes(a); }
+
+int mamba_block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *g, void *workspace,
+                              size_t workspace_bytes, void *stream) {
+    mb::clear_error();
+    return mb::block_norm_backward(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)) ? -1 : 0;
+}
+
 int mamba_propagate_tile_carries(float *carries, int num_tiles, int64_t width, float *total, void *stream) {
     mb::clear_error();
     return mb::propagate_tile_carries(carries, num_tiles, width, total, static_cast<cudaStream_t>(stream)) ? -1 : 0;

@@ -17,7 +17,7 @@ Reference interface mirrored (SNAPKITTYWEST/mamba-metal):
                    (Sources/Kernels/causal_conv1d.metal, state_update.metal,
                    rmsnorm.metal)
 Without a counterpart in the reference: gated_recurrence (with its backward
-pass and single-token step).
+pass and single-token step), block_norm (with its backward pass).
 """
 import ctypes
 import os
@@ -87,6 +87,19 @@ class MambaRecurrenceGrads(ctypes.Structure):
                 ("di_stride", c_i64 * 2)]
 
 
+class MambaBlockNormArgs(ctypes.Structure):
+    _fields_ = [("y", c_void_p), ("z", c_void_p), ("residual", c_void_p), ("w_post", c_void_p),
+                ("w_pre", c_void_p), ("residual_out", c_void_p), ("out", c_void_p), ("rstd_post", c_void_p),
+                ("rstd_pre", c_void_p), ("rows", c_i64), ("cols", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("residual_scale", c_float), ("eps", c_float), ("y_stride", c_i64), ("z_stride", c_i64)]
+
+
+class MambaBlockNormGrads(ctypes.Structure):
+    _fields_ = [("dresidual_out", c_void_p), ("dout", c_void_p), ("dresidual", c_void_p), ("dy", c_void_p),
+                ("dz", c_void_p), ("dw_post", c_void_p), ("dw_pre", c_void_p), ("dy_stride", c_i64),
+                ("dz_stride", c_i64)]
+
+
 # Every symbol include/mamba.h declares, with its ctypes prototype.
 _PROTOTYPES = {
     "mamba_create": (c_void_p, [ctypes.POINTER(MambaConfig)]),
@@ -144,6 +157,10 @@ _PROTOTYPES = {
                                                 ctypes.POINTER(MambaRecurrenceGrads), c_void_p, c_size, c_void_p]),
     "mamba_gated_recurrence_step": (c_int, [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_void_p,
                                             c_void_p, c_void_p, c_i64, c_int, c_int, c_float, c_int, c_void_p]),
+    "mamba_block_norm": (c_int, [ctypes.POINTER(MambaBlockNormArgs), c_void_p]),
+    "mamba_block_norm_workspace": (c_size, [ctypes.POINTER(MambaBlockNormArgs)]),
+    "mamba_block_norm_backward": (c_int, [ctypes.POINTER(MambaBlockNormArgs), ctypes.POINTER(MambaBlockNormGrads),
+                                          c_void_p, c_size, c_void_p]),
     "mamba_propagate_tile_carries": (c_int, [c_void_p, c_int, c_i64, c_void_p, c_void_p]),
     "mamba_gated_silu_mul": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, c_void_p]),
     "mamba_gated_mlp_up": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, c_int, c_void_p]),
@@ -782,6 +799,115 @@ def gated_recurrence_step(x, r, i, lam, state, c=8.0, state_out=None, h=None, st
                                                  h.data_ptr(), h.stride(0), bsz, dim, c, _dt(x),
                                                  _stream_of(x, stream)), "mamba_gated_recurrence_step")
     return h, state_out
+
+
+def _block_norm_args(what, y, w_post, z, w_pre, residual_scale, eps):
+    torch = _torch()
+    _require(y.dim() == 2, "%s: y must be [rows, cols]" % what)
+    _require(y.dtype in (torch.float16, torch.float32), "%s: y must be float16 or float32" % what)
+    rows, cols = y.shape
+    dev = y.device
+    _check_tensor(y, "y", what, y.shape, y.dtype, dev, True)
+    if z is not None:
+        _check_tensor(z, "z", what, y.shape, y.dtype, dev, True)
+    for name, w in (("w_post", w_post), ("w_pre", w_pre)):
+        if w is not None:
+            _check_tensor(w, name, what, (cols,), torch.float32, dev)
+    a = MambaBlockNormArgs()
+    a.y, a.z, a.w_post, a.w_pre = y.data_ptr(), _ptr(z), _ptr(w_post), _ptr(w_pre)
+    a.rows, a.cols, a.dtype, a.residual_scale, a.eps = rows, cols, _dt(y), residual_scale, eps
+    a.y_stride, a.z_stride = y.stride(0), z.stride(0) if z is not None else 0
+    return a
+
+
+def block_norm(y, residual, w_post=None, z=None, w_pre=None, residual_scale=1.0, eps=1e-5, second_norm=True,
+               return_rstd=False, residual_out=None, out=None, stream=None):
+    """The join between two blocks (mamba_block_norm):
+    residual_out = residual_scale * residual + rmsnorm(y) * w_post [* SiLU(z)]
+    out = rmsnorm(residual_out) * w_pre
+
+    y, z: [rows, cols] F16 or F32 (row stride any, channel stride 1);
+    residual FP32 contiguous (residual_out may be the same tensor); weights
+    FP32 [cols] or None (ones).  Returns (residual_out, out), out None with
+    second_norm=False, and with return_rstd also the two FP32 [rows] factors
+    that block_norm_backward reads."""
+    torch = _torch()
+    what = "block_norm"
+    a = _block_norm_args(what, y, w_post, z, w_pre, residual_scale, eps)
+    dev = y.device
+    _check_tensor(residual, "residual", what, y.shape, torch.float32, dev)
+    if residual_out is None:
+        residual_out = torch.empty(y.shape, dtype=torch.float32, device=dev)
+    else:
+        _check_tensor(residual_out, "residual_out", what, y.shape, torch.float32, dev)
+    if not second_norm:
+        out = None
+    elif out is None:
+        out = torch.empty(y.shape, dtype=y.dtype, device=dev)
+    else:
+        _check_tensor(out, "out", what, y.shape, y.dtype, dev)
+    a.residual, a.residual_out, a.out = residual.data_ptr(), residual_out.data_ptr(), _ptr(out)
+    rstd_post = rstd_pre = None
+    if return_rstd:
+        rstd_post = torch.empty((a.rows,), dtype=torch.float32, device=dev)
+        rstd_pre = torch.empty((a.rows,), dtype=torch.float32, device=dev) if second_norm else None
+        a.rstd_post, a.rstd_pre = rstd_post.data_ptr(), _ptr(rstd_pre)
+    with _on_device(y):
+        _check(lib().mamba_block_norm(ctypes.byref(a), _stream_of(y, stream)), "mamba_block_norm")
+    return (residual_out, out, rstd_post, rstd_pre) if return_rstd else (residual_out, out)
+
+
+def block_norm_backward(dresidual_out, dout, y, residual_out, rstd_post, rstd_pre, w_post=None, z=None, w_pre=None,
+                        residual_scale=1.0, dresidual=None, dy=None, dz=None, workspace=None, stream=None):
+    """Gradients of block_norm (mamba_block_norm_backward): dresidual_out
+    (FP32) and dout (y's dtype) are the gradients of its two outputs (either
+    may be None), residual_out and rstd_* what it returned.  dresidual may be
+    dresidual_out.  Returns (dy, dresidual, dw_post, dw_pre, dz); the sums
+    dw_post and dw_pre are FP32 [cols], dz is None without a gate."""
+    torch = _torch()
+    what = "block_norm_backward"
+    a = _block_norm_args(what, y, w_post, z, w_pre, residual_scale, 1.0)  # eps is inside rstd_*
+    dev = y.device
+    _check_tensor(residual_out, "residual_out", what, y.shape, torch.float32, dev)
+    _check_tensor(rstd_post, "rstd_post", what, (a.rows,), torch.float32, dev)
+    a.residual_out, a.rstd_post = residual_out.data_ptr(), rstd_post.data_ptr()
+    if dresidual_out is not None:
+        _check_tensor(dresidual_out, "dresidual_out", what, y.shape, torch.float32, dev)
+    if dout is not None:
+        _check_tensor(dout, "dout", what, y.shape, y.dtype, dev)
+        _require(rstd_pre is not None, "%s: dout needs rstd_pre" % what)
+        _check_tensor(rstd_pre, "rstd_pre", what, (a.rows,), torch.float32, dev)
+        a.rstd_pre = rstd_pre.data_ptr()
+    if dresidual is None:
+        dresidual = torch.empty(y.shape, dtype=torch.float32, device=dev)
+    else:
+        _check_tensor(dresidual, "dresidual", what, y.shape, torch.float32, dev)
+    if dy is None:
+        dy = torch.empty(y.shape, dtype=y.dtype, device=dev)
+    else:
+        _check_tensor(dy, "dy", what, y.shape, y.dtype, dev, True)
+    if z is None:
+        dz = None
+    elif dz is None:
+        dz = torch.empty(y.shape, dtype=y.dtype, device=dev)
+    else:
+        _check_tensor(dz, "dz", what, y.shape, y.dtype, dev, True)
+    dw_post = torch.empty((a.cols,), dtype=torch.float32, device=dev)
+    dw_pre = torch.empty((a.cols,), dtype=torch.float32, device=dev)
+    g = MambaBlockNormGrads()
+    g.dresidual_out, g.dout, g.dresidual = _ptr(dresidual_out), _ptr(dout), dresidual.data_ptr()
+    g.dy, g.dz, g.dw_post, g.dw_pre = dy.data_ptr(), _ptr(dz), dw_post.data_ptr(), dw_pre.data_ptr()
+    g.dy_stride, g.dz_stride = dy.stride(0), dz.stride(0) if dz is not None else 0
+    with _on_device(y):
+        need = lib().mamba_block_norm_workspace(ctypes.byref(a))
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        _require(workspace.is_contiguous() and workspace.device == dev,
+                 "%s: workspace must be contiguous and on the tensors' device" % what)
+        _check(lib().mamba_block_norm_backward(ctypes.byref(a), ctypes.byref(g), workspace.data_ptr(),
+                                               workspace.numel() * workspace.element_size(), _stream_of(y, stream)),
+               "mamba_block_norm_backward")
+    return dy, dresidual, dw_post, dw_pre, dz
 
 
 def propagate_tile_carries(carries, total=None, stream=None):

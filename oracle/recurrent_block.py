@@ -74,3 +74,54 @@ def gated_recurrence_backward(dh, x, r, i, lam, h, c, h0=None, lengths=None, res
     g["dlam"], mag["dlam"] = c * sigmoid(lam) * dsp, c * sigmoid(lam) * dspm
     g["dh0"], mag["dh0"] = C, Cm
     return g, mag
+
+
+def _silu(z):
+    s = sigmoid(z)
+    return z * s, s * (1 + z * sigmoid(-z))
+
+
+def block_norm(y, residual, w_post, z, w_pre, rho, eps):
+    """Returns (residual_out, out, rstd_post, rstd_pre) and the magnitudes of the first two."""
+    y, residual = np.asarray(y, np.float64), np.asarray(residual, np.float64)
+    wq = np.ones(y.shape[1]) if w_post is None else np.asarray(w_post, np.float64)
+    wp = np.ones(y.shape[1]) if w_pre is None else np.asarray(w_pre, np.float64)
+    g = 1.0 if z is None else _silu(np.asarray(z, np.float64))[0]
+    rs = 1 / np.sqrt((y * y).mean(1) + eps)
+    n = y * rs[:, None] * wq * g
+    r1 = rho * residual + n
+    rp = 1 / np.sqrt((r1 * r1).mean(1) + eps)
+    mag = np.abs(rho * residual) + np.abs(n)
+    return (r1, r1 * rp[:, None] * wp, rs, rp), (mag, mag * rp[:, None] * np.abs(wp))
+
+
+def block_norm_backward(dres_out, dout, y, res_out, rstd_post, rstd_pre, w_post, z, w_pre, rho):
+    """Returns dicts (gradients, magnitudes) with keys dy, dresidual, dw_post, dw_pre, dz (with a gate)."""
+    y, r1 = np.asarray(y, np.float64), np.asarray(res_out, np.float64)
+    wq = np.ones(y.shape[1]) if w_post is None else np.asarray(w_post, np.float64)
+    wp = np.ones(y.shape[1]) if w_pre is None else np.asarray(w_pre, np.float64)
+    rs = np.asarray(rstd_post, np.float64)[:, None]
+    R = np.zeros(y.shape) if dres_out is None else np.asarray(dres_out, np.float64)
+    Rm, g, mag = np.abs(R), {}, {}
+    g["dw_pre"], mag["dw_pre"] = np.zeros(y.shape[1]), np.zeros(y.shape[1])
+    if dout is not None:
+        d, rp = np.asarray(dout, np.float64), np.asarray(rstd_pre, np.float64)[:, None]
+        m, u = r1 * rp, d * wp
+        R = R + rp * (u - m * (u * m).mean(1, keepdims=True))
+        Rm = Rm + rp * (np.abs(u) + np.abs(m) * np.abs(u * m).mean(1, keepdims=True))
+        g["dw_pre"], mag["dw_pre"] = (d * m).sum(0), np.abs(d * m).sum(0)
+    gate, dgate = (1.0, 0.0) if z is None else _silu(np.asarray(z, np.float64))
+    n = y * rs
+    v, vm = R * wq * gate, Rm * np.abs(wq * gate)
+    g["dresidual"], mag["dresidual"] = rho * R, abs(rho) * Rm
+    g["dw_post"], mag["dw_post"] = (R * n * gate).sum(0), (Rm * np.abs(n * gate)).sum(0)
+    g["dy"] = rs * (v - n * (v * n).mean(1, keepdims=True))
+    mag["dy"] = rs * (vm + np.abs(n) * (vm * np.abs(n)).mean(1, keepdims=True))
+    if z is not None:
+        # SiLU'(z) = s + s z (1 - s) cancels near z = -1.278, so its two terms
+        # count: an error e of either sigmoid is e s (1 + |z| (1 - s)) there,
+        # however small the sum is.
+        zz = np.asarray(z, np.float64)
+        terms = sigmoid(zz) * (1 + np.abs(zz) * sigmoid(-zz))
+        g["dz"], mag["dz"] = R * wq * n * dgate, Rm * np.abs(wq * n) * terms
+    return g, mag
