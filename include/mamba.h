@@ -524,6 +524,32 @@ size_t mamba_linear_workspace(int64_t rows, int n, int k);
 int mamba_linear(const void *x, int64_t ldx, const void *w, const float *bias, void *y, int64_t ldy, int64_t rows,
                  int n, int k, int mode, void *workspace, size_t workspace_bytes, void *stream);
 
+/* Symmetric 8-bit quantisation of rows (no reference counterpart):
+ *   scale[t] = max_c |x[t, c]| / 127,   q[t, c] = round(x[t, c] / scale[t])
+ * with the FP32 quotient rounded once, ties of the exact x / scale to even
+ * and q within -127..127.  A row of zeros has scale 0; a row that holds an
+ * infinity or NaN has scale NaN and q 0, so that products with it are NaN.
+ * x [rows, cols] of dtype (MAMBA_F32 or MAMBA_F16) with row stride ldx, q
+ * with row stride ldq >= cols (elements; columns beyond cols are left as
+ * they were), scale FP32 [rows].  Activations per token, and weights [n, k]
+ * per output channel.  For mamba_linear_i8's tensor-core kernels give q a
+ * 16-byte aligned start and an ldq that is a multiple of 16.  0 / -1. */
+int mamba_quantize_rows(const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int64_t rows, int cols,
+                        int dtype, void *stream);
+
+/* Linear layer in 8-bit integers: with v = x_scale[t] * w_scale[n] *
+ * sum_k x[t, k] w[n, k] + bias[n],
+ *   mode 0: y (FP16) = v,   mode 1: y (FP32) += v,   mode 2: y (FP32) = v
+ * (the modes of mamba_linear).  x [rows, k] and w [n, k] int8 with row
+ * strides ldx and ldw, x_scale FP32 [rows], w_scale FP32 [n], bias FP32 [n]
+ * or NULL, y row stride ldy.  The sums are exact 32-bit integers, which
+ * bounds k to 131071; any value of int8 may occur.  16-byte aligned x and w
+ * with row strides that are multiples of 16 run on the tensor cores, others
+ * on a slower kernel with the same result.  No workspace.  0 / -1. */
+int mamba_linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw,
+                    const float *w_scale, const float *bias, void *y, int64_t ldy, int64_t rows, int n, int k,
+                    int mode, void *stream);
+
 /* in_proj with the causal conv fused into its epilogue (the first three
  * steps of the layer graph after RMSNorm, MambaRuntime.cpp:94-96:
  * linear_f16, projection.metal:32-49, then causal_conv1d_f16 + SiLU,

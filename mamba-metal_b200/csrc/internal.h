@@ -101,6 +101,12 @@ int linear_tc(const void *x, int64_t ldx, const void *w, const float *bias, void
               int K, int mode, void *ws, size_t ws_bytes, cudaStream_t st);
 unsigned linear_error_flags(bool clear);
 
+// linear_i8.cu
+int quantize_rows(const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int64_t rows, int cols, int dtype,
+                  cudaStream_t st);
+int linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw, const float *w_scale,
+              const float *bias, void *y, int64_t ldy, int64_t rows, int n, int k, int mode, cudaStream_t st);
+
 // init.cu
 uint64_t fill_key(uint64_t seed, int layer, int tag);
 int fill_random(void *out, int dtype, int64_t n, uint64_t key, int dist, float p0, float p1,

@@ -1519,6 +1519,22 @@ int mamba_linear(const void *x, int64_t ldx, const void *w, const float *bias, v
                : 0;
 }
 
+int mamba_quantize_rows(const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int64_t rows, int cols,
+                        int dtype, void *stream) {
+    mb::clear_error();
+    return mb::quantize_rows(x, ldx, q, ldq, scale, rows, cols, dtype, static_cast<cudaStream_t>(stream)) ? -1 : 0;
+}
+
+int mamba_linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw,
+                    const float *w_scale, const float *bias, void *y, int64_t ldy, int64_t rows, int n, int k,
+                    int mode, void *stream) {
+    mb::clear_error();
+    return mb::linear_i8(x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, rows, n, k, mode,
+                         static_cast<cudaStream_t>(stream))
+               ? -1
+               : 0;
+}
+
 int mamba_in_proj_conv(const void *x, const void *w_in, const float *conv_w, const float *conv_b, void *u, void *z,
                        int64_t z_row_stride, int batch, int seqlen, int d_model, int d_inner, int d_conv,
                        void *stream) {

@@ -17,7 +17,8 @@ Reference interface mirrored (SNAPKITTYWEST/mamba-metal):
                    (Sources/Kernels/causal_conv1d.metal, state_update.metal,
                    rmsnorm.metal)
 Without a counterpart in the reference: gated_recurrence (with its backward
-pass and single-token step), block_norm (with its backward pass).
+pass and single-token step), block_norm (with its backward pass),
+quantize_rows and linear_i8 (8-bit linear layer).
 """
 import ctypes
 import os
@@ -166,6 +167,9 @@ _PROTOTYPES = {
     "mamba_gated_mlp_up": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, c_int, c_void_p]),
     "mamba_in_proj_conv": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_int, c_int,
                                    c_int, c_int, c_int, c_void_p]),
+    "mamba_quantize_rows": (c_int, [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_int, c_int, c_void_p]),
+    "mamba_linear_i8": (c_int, [c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_i64,
+                                c_i64, c_int, c_int, c_int, c_void_p]),
     "mamba_linear_workspace": (c_size, [c_i64, c_int, c_int]),
     "mamba_selftest_bounded_wait": (c_int, [ctypes.c_uint, c_void_p]),
     "mamba_linear": (c_int, [c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_int, c_int, c_int,
@@ -942,6 +946,60 @@ def linear(x, w, bias=None, y=None, mode=0, workspace=None, stream=None):
     ws_ptr, ws_len = (_ptr(workspace), workspace.numel()) if workspace is not None else (None, 0)
     _check(lib().mamba_linear(_ptr(x), x.stride(0), _ptr(w), _ptr(bias), _ptr(y), y.stride(0), rows, n, k, mode,
                               ws_ptr, ws_len, _stream(stream)), "mamba_linear")
+    return y
+
+
+def quantize_rows(x, q=None, scale=None, stream=None):
+    """Symmetric 8-bit rows (mamba_quantize_rows): x [rows, cols] F16 or F32
+    (row stride any, channel stride 1) -> (q int8 [rows, cols], scale FP32
+    [rows]) with x ~ q * scale.  A fresh q is a view of rows padded to a
+    multiple of 16 bytes, the layout linear_i8's fast kernels read."""
+    torch = _torch()
+    what = "quantize_rows"
+    _require(x.dim() == 2, "%s: x must be [rows, cols]" % what)
+    _require(x.dtype in (torch.float16, torch.float32), "%s: x must be float16 or float32" % what)
+    rows, cols = x.shape
+    _check_tensor(x, "x", what, x.shape, x.dtype, x.device, True)
+    if q is None:
+        q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :cols]
+    else:
+        _check_tensor(q, "q", what, x.shape, torch.int8, x.device, True)
+    if scale is None:
+        scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    else:
+        _check_tensor(scale, "scale", what, (rows,), torch.float32, x.device)
+    with _on_device(x):
+        _check(lib().mamba_quantize_rows(x.data_ptr(), x.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr(), rows,
+                                         cols, _dt(x), _stream_of(x, stream)), "mamba_quantize_rows")
+    return q, scale
+
+
+def linear_i8(x, x_scale, w, w_scale, bias=None, y=None, mode=0, stream=None):
+    """Linear layer in 8-bit integers (mamba_linear_i8): x int8 [rows, k] and
+    w int8 [n, k] as quantize_rows gives them (row stride any, channel stride
+    1), x_scale FP32 [rows], w_scale FP32 [n], bias FP32 [n].  mode 0 -> y
+    FP16, 1 -> y FP32 += result, 2 -> y FP32 = result."""
+    torch = _torch()
+    what = "linear_i8"
+    _require(x.dim() == 2 and w.dim() == 2, "%s: x and w must be matrices" % what)
+    _require(mode in (0, 1, 2), "%s: mode must be 0, 1 or 2" % what)
+    (rows, k), n, dev = x.shape, w.shape[0], x.device
+    _check_tensor(x, "x", what, (rows, k), torch.int8, dev, True)
+    _check_tensor(w, "w", what, (n, k), torch.int8, dev, True)
+    _check_tensor(x_scale, "x_scale", what, (rows,), torch.float32, dev)
+    _check_tensor(w_scale, "w_scale", what, (n,), torch.float32, dev)
+    if bias is not None:
+        _check_tensor(bias, "bias", what, (n,), torch.float32, dev)
+    out = torch.float16 if mode == 0 else torch.float32
+    if y is None:
+        _require(mode != 1, "%s: mode 1 adds into a given y" % what)
+        y = torch.empty((rows, n), dtype=out, device=dev)
+    else:
+        _check_tensor(y, "y", what, (rows, n), out, dev, True)
+    with _on_device(x):
+        _check(lib().mamba_linear_i8(x.data_ptr(), x.stride(0), x_scale.data_ptr(), w.data_ptr(), w.stride(0),
+                                     w_scale.data_ptr(), _ptr(bias), y.data_ptr(), y.stride(0), rows, n, k, mode,
+                                     _stream_of(x, stream)), "mamba_linear_i8")
     return y
 
 

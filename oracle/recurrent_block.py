@@ -125,3 +125,24 @@ def block_norm_backward(dres_out, dout, y, res_out, rstd_post, rstd_pre, w_post,
         terms = sigmoid(zz) * (1 + np.abs(zz) * sigmoid(-zz))
         g["dz"], mag["dz"] = R * wq * n * dgate, Rm * np.abs(wq * n) * terms
     return g, mag
+
+
+def quantize_rows(x):
+    """(q int8, scale FP32).  Both quotients are exact enough in 64 bits to
+    round like the exact ones: max / 127 to 32 bits (53 >= 2 * 24 + 2), and
+    x / scale to a whole number (24-bit operands)."""
+    x = np.asarray(x)
+    with np.errstate(invalid="ignore"):
+        amax = np.abs(x.astype(np.float64)).max(1, initial=0)
+        scale = (amax / 127).astype(np.float32)
+        scale[~np.isfinite(amax)] = np.nan
+        div = np.where((scale == 0) | np.isnan(scale), np.inf, scale.astype(np.float64))
+        q = np.nan_to_num(np.rint(x.astype(np.float64) / div[:, None]), nan=0.0)
+    return np.clip(q, -127, 127).astype(np.int8), scale
+
+
+def linear_i8(x, xs, w, ws, bias=None):
+    """Returns the FP64 result and its magnitude."""
+    v = (x.astype(np.float64) @ w.astype(np.float64).T) * xs.astype(np.float64)[:, None] * ws.astype(np.float64)
+    b = 0.0 if bias is None else bias.astype(np.float64)
+    return v + b, np.abs(v) + np.abs(b)
