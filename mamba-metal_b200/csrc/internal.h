@@ -53,6 +53,7 @@ int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads
 int recurrence_step(const void *x, int64_t xrs, const void *r, int64_t rrs, const void *i, int64_t irs,
                     const float *lambda, const float *state_in, float *state_out, void *h, int64_t hrs, int batch,
                     int dim, float c, int dtype, cudaStream_t st);
+unsigned recurrence_error_flags(bool clear);
 
 // norm.cu
 int rmsnorm(const void *x, const float *w, void *y, int64_t rows, int cols, float eps, int in_dt,

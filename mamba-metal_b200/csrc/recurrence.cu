@@ -15,7 +15,13 @@
 #include "internal.h"
 #include "scan_math.cuh"
 
+#include "tma.cuh"
+
+#include <algorithm>
+
 namespace mb {
+
+__device__ unsigned int g_recurrence_error = 0;
 
 namespace {
 
@@ -58,6 +64,19 @@ __device__ __forceinline__ float sqrt_gate(float m) {
 // softplus(lambda): per channel, so the accurate form for both types.
 __device__ __forceinline__ float softplus_channel(float l) { return fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))); }
 
+// beta = sqrt(m) and q = y / beta; q -> sqrt(y / 2) -> 0 as the gate closes.
+template <bool PRECISE>
+__device__ __forceinline__ void root_gate(float m, float y, float &beta, float &q) {
+    if (PRECISE) {
+        beta = sqrtf(m);
+        q = beta <= 1e-18f ? 0.f : __fdiv_rn(y, beta);
+    } else {
+        const float r = rsqrtf(m);
+        beta = m <= 1e-36f ? 0.f : m * r;  // a NaN stays one
+        q = m <= 1e-36f ? 0.f : y * r;
+    }
+}
+
 struct Decay {
     float s, om, y, a;
 };
@@ -86,7 +105,7 @@ struct BwdParams {
     const void *dh;
     const float *dhN;
     void *dx, *dr, *di;
-    float *dlambda, *dh0, *part;
+    float *dh0, *part;
     int64_t sdh[2], sdx[2], sdr[2], sdi[2];
 };
 
@@ -96,83 +115,499 @@ __device__ __forceinline__ int row_length(const FwdParams &p, int b) {
 
 constexpr int kThreads = 128;
 
-// One thread per (row, channel), walking time.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) recurrence_fwd_kernel(const FwdParams p) {
+// ---- tiles of a sequence ----------------------------------------------------
+// A CTA of W warps owns one tile of the time axis, W * S tokens of 32 * VEC
+// channels; warp w holds S consecutive tokens in registers.  The recurrence is
+// affine in the state that enters a span, h_out = P h_in + H, so
+//   1. each warp reduces its S tokens to (P, H), and the warps' maps are
+//      composed through shared memory into the tile's,
+//   2. the state entering the tile comes from the tiles before it, and
+//   3. each warp walks its S tokens again, from registers, and writes h.
+// Every tensor is read and written once, for any split of the time axis.
+//
+// Step 2 crosses CTAs.  Tiles are handed out by an atomic ticket, time-major
+// (all rows' and channels' first tiles, then all second ones), so every tile
+// before a running one is running or done and waiting for it ends.  Tiles form
+// groups of kGroup: a tile publishes its map to the later tiles of its group,
+// and the group's last tile publishes the state leaving the group.  So the
+// serial chain over a long sequence has one hop per group, each tile composes
+// the same maps in the same order on every run (a scheme that takes whatever
+// state is ready first would not), and results repeat bit for bit.
+// A published value is one machine word that says itself whether it is there:
+// the workspace starts as all ones bits (a NaN that no published value has).
+constexpr int kGroup = 8;
+constexpr unsigned kErrRecurrenceTimeout = 64u;
+constexpr uint32_t kEmpty = 0xffffffffu;
+
+__device__ __forceinline__ float published(float v) {  // never the empty pattern
+    return __float_as_uint(v) == kEmpty ? __uint_as_float(0x7fffffffu) : v;
+}
+__device__ __forceinline__ void put_map(float2 *slot, float P, float H) {
+    const uint64_t w = (uint64_t)__float_as_uint(H) << 32 | __float_as_uint(published(P));
+    asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(slot), "l"(w) : "memory");
+}
+__device__ __forceinline__ void put_state(float *slot, float h) {
+    asm volatile("st.relaxed.gpu.global.b32 [%0], %1;" ::"l"(slot), "r"(__float_as_uint(published(h))) : "memory");
+}
+__device__ __forceinline__ uint64_t get_map(const float2 *slot) {
+    uint64_t w;
+    asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(w) : "l"(slot) : "memory");
+    return w;
+}
+__device__ __forceinline__ uint32_t get_state(const float *slot) {
+    uint32_t w;
+    asm volatile("ld.relaxed.gpu.global.b32 %0, [%1];" : "=r"(w) : "l"(slot) : "memory");
+    return w;
+}
+
+// Bounded wait (2 s, or at once after another CTA's wait ran out).
+struct Waiting {
+    uint64_t t0 = 0;
+    int spins = 0;
+    __device__ __forceinline__ bool again() {
+        if ((++spins & 63) == 0) {
+            const uint64_t now = global_timer_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > 2000000000ull || *(volatile unsigned int *)&g_recurrence_error) {
+                atomicOr(&g_recurrence_error, kErrRecurrenceTimeout);
+                return false;
+            }
+        }
+        return true;
+    }
+};
+
+template <int VEC>
+__device__ __forceinline__ void wait_maps(const float2 *slot, float2 (&m)[VEC]) {
+    Waiting wt;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+        uint64_t w = get_map(slot + k);
+        while ((uint32_t)w == kEmpty && wt.again()) w = get_map(slot + k);
+        m[k] = make_float2(__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32)));
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void wait_states(const float *slot, float (&h)[VEC]) {
+    Waiting wt;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+        uint32_t w = get_state(slot + k);
+        while (w == kEmpty && wt.again()) w = get_state(slot + k);
+        h[k] = __uint_as_float(w);
+    }
+}
+
+struct Chains {
+    unsigned int *ticket;
+    float2 *maps;    // [chains, tiles, channels of a tile]
+    float *states;   // [chains, groups, channels of a tile]
+    int blocks;      // channel blocks of a row
+    int chains;      // rows * blocks
+    int tiles;
+};
+
+// This CTA's chain and its place in it, in the order the state runs.
+__device__ __forceinline__ void take_tile(const Chains &c, int &chain, int &k) {
+    __shared__ unsigned int id;
+    unsigned int v = blockIdx.x;
+    if (c.tiles > 1) {
+        if (threadIdx.x == 0) id = atomicAdd(c.ticket, 1u) + 1u;  // starts as all ones bits
+        __syncthreads();
+        v = id;
+    }
+    k = (int)(v / (unsigned)c.chains);
+    chain = (int)(v - (unsigned)k * (unsigned)c.chains);
+}
+
+// The state entering tile k of a chain: `first` (the chain's initial state) or
+// the state leaving the group before, then the group's tiles before k in
+// order.  Warp w publishes nothing and waits for the maps of tiles w, w + W, ...
+// of the group; the maps meet in shared memory.  Returns the state in every
+// warp.  Call after the tile's own map is published; syncs the CTA.
+template <int VEC, int W>
+__device__ __forceinline__ void entering_state(const Chains &c, int chain, int k, const float (&first)[VEC],
+                                               float2 (*gm)[VEC * 32], float *gs, float (&h)[VEC]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cw = VEC * 32;
+    const int g = k / kGroup, j = k % kGroup;
+#pragma unroll
+    for (int q = 0; q < (kGroup + W - 1) / W; ++q) {
+        const int tile = warp + q * W;
+        if (tile < j) {
+            float2 m[VEC];
+            wait_maps<VEC>(c.maps + ((int64_t)chain * c.tiles + g * kGroup + tile) * cw + lane * VEC, m);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) gm[tile][e * 32 + lane] = m[e];
+        } else if (tile == kGroup - 1 && g > 0) {
+            float s[VEC];
+            const int groups = (c.tiles + kGroup - 1) / kGroup;
+            wait_states<VEC>(c.states + ((int64_t)chain * groups + g - 1) * cw + lane * VEC, s);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) gs[e * 32 + lane] = s[e];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) h[e] = g > 0 ? gs[e * 32 + lane] : first[e];
+    for (int t = 0; t < j; ++t)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float2 m = gm[t][e * 32 + lane];
+            h[e] = fmaf(m.x, h[e], m.y);
+        }
+}
+
+// VEC consecutive elements, as loaded and as FP32.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+    T v[VEC];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T *p) {
+    return *reinterpret_cast<const Pack<T, VEC> *>(p);
+}
+
+// Tokens of this warp that exist, and which of them cut the state.
+__device__ __forceinline__ uint32_t cut_mask(const FwdParams &p, int b, int t0, int cnt) {
+    if (!p.resets) return 0;
+    const int lane = threadIdx.x & 31;
+    const bool z = lane < cnt && p.resets[(int64_t)b * p.L + t0 + lane] != 0;
+    return __ballot_sync(0xffffffffu, z);
+}
+
+template <typename T, int VEC, int S, int W>
+__global__ void __launch_bounds__(32 * W, 512 / (32 * W)) recurrence_fwd_kernel(const FwdParams p, const Chains ch) {
     constexpr bool PRECISE = sizeof(T) == 4;
-    const int d = blockIdx.x * kThreads + threadIdx.x, b = blockIdx.y;
-    if (d >= p.D) return;
+    constexpr int cw = 32 * VEC;
+    __shared__ float2 wm[W][cw], gm[kGroup][cw];
+    __shared__ float gs[cw];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int chain, k;
+    take_tile(ch, chain, k);
+    const int b = chain / ch.blocks, d = (chain - b * ch.blocks) * cw + lane * VEC;
     const int n = row_length(p, b);
-    const float csp = p.c * softplus_channel(p.lambda[d]);
-    const T *x = static_cast<const T *>(p.x) + b * p.sx[0] + d;
-    const T *r = static_cast<const T *>(p.r) + b * p.sr[0] + d;
-    const T *gi = static_cast<const T *>(p.i) + b * p.si[0] + d;
-    T *ho = static_cast<T *>(p.h) + b * p.sh[0] + d;
-    float h = p.h0 ? p.h0[(int64_t)b * p.D + d] : 0.f;
-    for (int t = 0; t < n; ++t) {
-        const Decay g = decay<PRECISE>(ld_f32(r + t * p.sr[1]), csp);
-        float si, om;
-        sigmoid2<PRECISE>(ld_f32(gi + t * p.si[1]), si, om);
-        const float bt = sqrt_gate<PRECISE>(one_minus_a2<PRECISE>(g.y, g.a)) * si * ld_f32(x + t * p.sx[1]);
-        if (p.resets && p.resets[(int64_t)b * p.L + t]) h = 0.f;
-        h = fmaf(g.a, h, bt);
-        ho[t * p.sh[1]] = cvt_out<T>(h);
+    const int tile0 = k * (S * W);
+    if (k > 0 && tile0 >= n) return;  // behind the row's end: no later tile of the row has work either
+    const bool in = d < p.D;
+    const int t0 = tile0 + warp * S;
+    const int cnt = in ? min(max(n - t0, 0), S) : 0;
+
+    float a[S][VEC], bt[S][VEC];
+    {
+        Pack<T, VEC> x[S], r[S], gi[S];
+        const T *px = static_cast<const T *>(p.x) + b * p.sx[0] + t0 * p.sx[1] + d;
+        const T *pr = static_cast<const T *>(p.r) + b * p.sr[0] + t0 * p.sr[1] + d;
+        const T *pi = static_cast<const T *>(p.i) + b * p.si[0] + t0 * p.si[1] + d;
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+            if (j < cnt) {
+                r[j] = load_pack<T, VEC>(pr + j * p.sr[1]);
+                gi[j] = load_pack<T, VEC>(pi + j * p.si[1]);
+                x[j] = load_pack<T, VEC>(px + j * p.sx[1]);
+            }
+        float csp[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) csp[e] = in ? p.c * softplus_channel(p.lambda[d + e]) : 0.f;
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (j < cnt) {
+                    const Decay g = decay<PRECISE>(cvt_f32(r[j].v[e]), csp[e]);
+                    float si, om;
+                    sigmoid2<PRECISE>(cvt_f32(gi[j].v[e]), si, om);
+                    a[j][e] = g.a;
+                    bt[j][e] = sqrt_gate<PRECISE>(one_minus_a2<PRECISE>(g.y, g.a)) * si * cvt_f32(x[j].v[e]);
+                } else {
+                    a[j][e] = 1.f;
+                    bt[j][e] = 0.f;
+                }
+            }
+        }
     }
-    if (p.hN) p.hN[(int64_t)b * p.D + d] = h;
+    const uint32_t cut = cut_mask(p, b, t0, min(max(n - t0, 0), S));
+    if (cut)
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+            if (cut >> j & 1)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) a[j][e] = 0.f;
+
+    // this warp's map, then the tile's (in warp 0) and its publication
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        float P = 1.f, H = 0.f;
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+            H = fmaf(a[j][e], H, bt[j][e]);
+            P *= a[j][e];
+        }
+        wm[warp][e * 32 + lane] = make_float2(P, H);
+    }
+    __syncthreads();
+    const bool more = k + 1 < ch.tiles && (k + 1) * (S * W) < n;  // a later tile waits for this one
+    if (warp == 0 && more && k % kGroup != kGroup - 1) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            float2 m = make_float2(1.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float2 q = wm[w][e * 32 + lane];
+                m.y = fmaf(q.x, m.y, q.y);
+                m.x *= q.x;
+            }
+            put_map(ch.maps + ((int64_t)chain * ch.tiles + k) * cw + lane * VEC + e, m.x, m.y);
+        }
+    }
+    float h[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) h[e] = in && p.h0 && k < kGroup ? p.h0[(int64_t)b * p.D + d + e] : 0.f;
+    if (k > 0) {
+        float first[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) first[e] = h[e];
+        entering_state<VEC, W>(ch, chain, k, first, gm, gs, h);
+    }
+    float hw[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        hw[e] = h[e];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w == warp) hw[e] = h[e];
+            const float2 q = wm[w][e * 32 + lane];
+            h[e] = fmaf(q.x, h[e], q.y);
+        }
+    }
+    if (warp == 0) {
+        if (more) {
+            if (k % kGroup == kGroup - 1) {
+                const int groups = (ch.tiles + kGroup - 1) / kGroup;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    put_state(ch.states + ((int64_t)chain * groups + k / kGroup) * cw + lane * VEC + e, h[e]);
+            }
+        } else if (in && p.hN) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) p.hN[(int64_t)b * p.D + d + e] = h[e];
+        }
+    }
+    T *ph = static_cast<T *>(p.h) + b * p.sh[0] + t0 * p.sh[1] + d;
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+        if (j < cnt) {
+            Pack<T, VEC> o;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                hw[e] = fmaf(a[j][e], hw[e], bt[j][e]);
+                o.v[e] = cvt_out<T>(hw[e]);
+            }
+            *reinterpret_cast<Pack<T, VEC> *>(ph + j * p.sh[1]) = o;
+        }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) recurrence_bwd_kernel(const BwdParams p) {
+// Backward: the same tiles and chains with time reversed; what runs along a
+// chain is C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.
+template <typename T, int VEC, int S, int W>
+__global__ void __launch_bounds__(32 * W, 512 / (32 * W)) recurrence_bwd_kernel(const BwdParams p, const Chains ch) {
     constexpr bool PRECISE = sizeof(T) == 4;
+    constexpr int cw = 32 * VEC;
+    __shared__ float2 wm[W][cw], gm[kGroup][cw];
+    __shared__ float gs[cw];
     const FwdParams &f = p.f;
-    const int d = blockIdx.x * kThreads + threadIdx.x, b = blockIdx.y;
-    if (d >= f.D) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int chain, k;
+    take_tile(ch, chain, k);
+    const int b = chain / ch.blocks, d = (chain - b * ch.blocks) * cw + lane * VEC;
     const int n = row_length(f, b);
-    const float csp = f.c * softplus_channel(f.lambda[d]);
-    const T *x = static_cast<const T *>(f.x) + b * f.sx[0] + d;
-    const T *r = static_cast<const T *>(f.r) + b * f.sr[0] + d;
-    const T *gi = static_cast<const T *>(f.i) + b * f.si[0] + d;
-    const T *h = static_cast<const T *>(f.h) + b * f.sh[0] + d;
-    const T *dh = static_cast<const T *>(p.dh) + b * p.sdh[0] + d;
-    T *dx = static_cast<T *>(p.dx) + b * p.sdx[0] + d;
-    T *dr = static_cast<T *>(p.dr) + b * p.sdr[0] + d;
-    T *di = static_cast<T *>(p.di) + b * p.sdi[0] + d;
-    float C = p.dhN ? p.dhN[(int64_t)b * f.D + d] : 0.f, sum = 0.f;
-    for (int t = n - 1; t >= 0; --t) {
-        const Decay g = decay<PRECISE>(ld_f32(r + t * f.sr[1]), csp);
-        float si, om;
-        sigmoid2<PRECISE>(ld_f32(gi + t * f.si[1]), si, om);
-        const float m = one_minus_a2<PRECISE>(g.y, g.a), beta = sqrt_gate<PRECISE>(m);
-        const float q = beta > 1e-18f ? g.y / beta : 0.f;
-        const bool keep = !(f.resets && f.resets[(int64_t)b * f.L + t]);
-        float prev = t ? ld_f32(h + (t - 1) * f.sh[1]) : (f.h0 ? f.h0[(int64_t)b * f.D + d] : 0.f);
-        if (!keep) prev = 0.f;
-        const float G = ld_f32(dh + t * p.sdh[1]) + C, xv = ld_f32(x + t * f.sx[1]);
-        const float gx = G * beta * si;
-        const float E = G * (si * xv * g.a * g.a * q - g.y * g.a * prev);
-        dx[t * p.sdx[1]] = cvt_out<T>(gx);
-        di[t * p.sdi[1]] = cvt_out<T>(gx * xv * om);
-        dr[t * p.sdr[1]] = cvt_out<T>(E * g.om);
-        sum += E;
-        C = keep ? g.a * G : 0.f;
+    const bool in = d < f.D;
+    const int row_tiles = max((n + S * W - 1) / (S * W), 1);
+    float *part = p.part + ((int64_t)b * ch.tiles + k) * f.D + d;
+    if (k >= row_tiles) {  // behind the row's end
+        if (warp == 0 && in)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) part[e] = 0.f;
+        return;
     }
-    if (p.dh0) p.dh0[(int64_t)b * f.D + d] = C;
-    p.part[(int64_t)b * f.D + d] = sum;
+    const int t0 = (row_tiles - 1 - k) * (S * W) + (W - 1 - warp) * S;  // warp 0 holds the tile's last tokens
+    const int cnt = in ? min(max(n - t0, 0), S) : 0;
+
+    Pack<T, VEC> x[S], gi[S], hp[S], dh[S];
+    float a[S][VEC], y[S][VEC], om[S][VEC];
+    {
+        Pack<T, VEC> r[S];
+        const T *pr = static_cast<const T *>(f.r) + b * f.sr[0] + t0 * f.sr[1] + d;
+        const T *pg = static_cast<const T *>(p.dh) + b * p.sdh[0] + t0 * p.sdh[1] + d;
+        const T *px = static_cast<const T *>(f.x) + b * f.sx[0] + t0 * f.sx[1] + d;
+        const T *pi = static_cast<const T *>(f.i) + b * f.si[0] + t0 * f.si[1] + d;
+        const T *ph = static_cast<const T *>(f.h) + b * f.sh[0] + (t0 - 1) * f.sh[1] + d;
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+            if (j < cnt) {
+                r[j] = load_pack<T, VEC>(pr + j * f.sr[1]);
+                dh[j] = load_pack<T, VEC>(pg + j * p.sdh[1]);
+            }
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+            if (j < cnt) {
+                x[j] = load_pack<T, VEC>(px + j * f.sx[1]);
+                gi[j] = load_pack<T, VEC>(pi + j * f.si[1]);
+                if (t0 + j > 0) hp[j] = load_pack<T, VEC>(ph + j * f.sh[1]);
+            }
+        float csp[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) csp[e] = in ? f.c * softplus_channel(f.lambda[d + e]) : 0.f;
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (j < cnt) {
+                    const Decay g = decay<PRECISE>(cvt_f32(r[j].v[e]), csp[e]);
+                    a[j][e] = g.a;
+                    y[j][e] = g.y;
+                    om[j][e] = g.om;
+                } else {
+                    a[j][e] = 1.f;
+                    y[j][e] = om[j][e] = 0.f;
+                }
+            }
+    }
+    const uint32_t cut = cut_mask(f, b, t0, min(max(n - t0, 0), S));
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        float P = 1.f, H = 0.f;
+#pragma unroll
+        for (int j = S - 1; j >= 0; --j) {
+            const float g = (j < cnt ? cvt_f32(dh[j].v[e]) : 0.f) + H;
+            const float ak = cut >> j & 1 ? 0.f : a[j][e];
+            H = ak * g;
+            P *= ak;
+        }
+        wm[warp][e * 32 + lane] = make_float2(P, H);
+    }
+    __syncthreads();
+    const bool more = k + 1 < row_tiles;
+    if (warp == 0 && more && k % kGroup != kGroup - 1) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            float2 m = make_float2(1.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float2 q = wm[w][e * 32 + lane];
+                m.y = fmaf(q.x, m.y, q.y);
+                m.x *= q.x;
+            }
+            put_map(ch.maps + ((int64_t)chain * ch.tiles + k) * cw + lane * VEC + e, m.x, m.y);
+        }
+    }
+    float C[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) C[e] = in && p.dhN && k < kGroup ? p.dhN[(int64_t)b * f.D + d + e] : 0.f;
+    if (k > 0) {
+        float first[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) first[e] = C[e];
+        entering_state<VEC, W>(ch, chain, k, first, gm, gs, C);
+    }
+    float cv[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        cv[e] = C[e];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w == warp) cv[e] = C[e];
+            const float2 q = wm[w][e * 32 + lane];
+            C[e] = fmaf(q.x, C[e], q.y);
+        }
+    }
+    if (warp == 0) {
+        if (more) {
+            if (k % kGroup == kGroup - 1) {
+                const int groups = (ch.tiles + kGroup - 1) / kGroup;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    put_state(ch.states + ((int64_t)chain * groups + k / kGroup) * cw + lane * VEC + e, C[e]);
+            }
+        } else if (in && p.dh0) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) p.dh0[(int64_t)b * f.D + d + e] = C[e];
+        }
+    }
+    T *qx = static_cast<T *>(p.dx) + b * p.sdx[0] + t0 * p.sdx[1] + d;
+    T *qr = static_cast<T *>(p.dr) + b * p.sdr[0] + t0 * p.sdr[1] + d;
+    T *qi = static_cast<T *>(p.di) + b * p.sdi[0] + t0 * p.sdi[1] + d;
+    float sum[VEC] = {};
+#pragma unroll
+    for (int j = S - 1; j >= 0; --j) {
+        if (j < cnt) {
+            Pack<T, VEC> ox, orr, oi;
+            const bool keep = !(cut >> j & 1);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float av = a[j][e], yv = y[j][e], xv = cvt_f32(x[j].v[e]);
+                const float G = cvt_f32(dh[j].v[e]) + cv[e];
+                const float ca = keep ? av : 0.f;
+                cv[e] = ca * G;
+                float si, omi;
+                sigmoid2<PRECISE>(cvt_f32(gi[j].v[e]), si, omi);
+                const float m = one_minus_a2<PRECISE>(yv, av);
+                float beta, q;
+                root_gate<PRECISE>(m, yv, beta, q);
+                float prev;
+                if (t0 + j > 0)
+                    prev = cvt_f32(hp[j].v[e]);
+                else
+                    prev = f.h0 ? f.h0[(int64_t)b * f.D + d + e] : 0.f;
+                if (!keep) prev = 0.f;
+                const float gx = G * beta * si;
+                const float E = G * (si * xv * av * av * q - yv * av * prev);
+                sum[e] += E;
+                ox.v[e] = cvt_out<T>(gx);
+                oi.v[e] = cvt_out<T>(gx * xv * omi);
+                orr.v[e] = cvt_out<T>(E * om[j][e]);
+            }
+            *reinterpret_cast<Pack<T, VEC> *>(qx + j * p.sdx[1]) = ox;
+            *reinterpret_cast<Pack<T, VEC> *>(qi + j * p.sdi[1]) = oi;
+            *reinterpret_cast<Pack<T, VEC> *>(qr + j * p.sdr[1]) = orr;
+        }
+    }
+    // the tile's sum of E per channel, warps in order
+    __syncthreads();  // wm is free again
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) wm[warp][e * 32 + lane].x = sum[e];
+    __syncthreads();
+    if (warp == 0 && in)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) s += wm[w][e * 32 + lane].x;
+            part[e] = s;
+        }
 }
 
-// dlambda[d] = sigmoid(lambda)/softplus(lambda) * sum of the partial sums of
-// E, added in row order.  The quotient tends to 1 for very negative lambda.
-__global__ void __launch_bounds__(kThreads)
+// dlambda[d] = sigmoid(lambda)/softplus(lambda) * sum of the tiles' sums of E,
+// in a fixed order: warp w adds rows w, w + 16, ..., then the warps in order.
+// The quotient tends to 1 for very negative lambda.
+constexpr int kSumWarps = 16;
+__global__ void __launch_bounds__(32 * kSumWarps)
     recurrence_dlambda_kernel(const float *__restrict__ part, const float *__restrict__ lambda,
                               float *__restrict__ dlambda, int64_t rows, int D) {
-    const int d = blockIdx.x * kThreads + threadIdx.x;
-    if (d >= D) return;
+    __shared__ float sm[kSumWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = blockIdx.x * 32 + lane;
     float s = 0.f;
-    for (int64_t k = 0; k < rows; ++k) s += part[k * D + d];
-    float sg, om;
-    const float l = lambda[d];
-    sigmoid2<true>(l, sg, om);
-    dlambda[d] = s * (l < -20.f ? 1.f : sg / softplus_channel(l));
+    if (d < D)
+        for (int64_t k = warp; k < rows; k += kSumWarps) s += part[k * D + d];
+    sm[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && d < D) {
+#pragma unroll
+        for (int w = 1; w < kSumWarps; ++w) s += sm[w][lane];
+        float sg, om;
+        const float l = lambda[d];
+        sigmoid2<true>(l, sg, om);
+        dlambda[d] = s * (l < -20.f ? 1.f : sg / softplus_channel(l));
+    }
 }
 
 template <typename T>
@@ -194,6 +629,12 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Every row starts at a multiple of VEC elements' bytes.
+template <typename T, int VEC>
+bool vector_rows(const void *p, const int64_t *s) {
+    return aligned_to(p, sizeof(T) * VEC) && s[0] % VEC == 0 && s[1] % VEC == 0;
+}
 
 // Rows of an output must not overlap one another.
 bool output_rows_disjoint(const int64_t *s, int B, int L, int D) {
@@ -245,23 +686,107 @@ FwdParams fwd_params(const MambaRecurrenceArgs *a) {
     return p;
 }
 
+// Channels a thread holds (1 serves any alignment and channel count).
+constexpr int kFwdVec = 4, kBwdVec = 2;
+constexpr int kFwdTile = 32, kBwdTile = 32;  // tokens of a tile (S * W)
+
+// The chains of a call and where its workspace holds what.
+struct Plan {
+    Chains ch;
+    size_t bytes, part_bytes;
+};
+bool plan_chains(const MambaRecurrenceArgs *a, bool backward, int vec, Plan &pl) {
+    const int tile = backward ? kBwdTile : kFwdTile, cw = 32 * vec;
+    Chains &c = pl.ch;
+    c = Chains{};
+    const int64_t blocks = ceil_div64(a->dim, cw), tiles = std::max<int64_t>(1, ceil_div64(a->seqlen, tile));
+    if (blocks * a->batch * tiles > 0x7fffffffLL) return false;
+    c.blocks = (int)blocks;
+    c.chains = (int)blocks * a->batch;
+    c.tiles = (int)tiles;
+    pl.bytes = 0;
+    if (tiles > 1)
+        pl.bytes = 256 + (size_t)c.chains * cw * (tiles * sizeof(float2) + ceil_div64(tiles, kGroup) * sizeof(float));
+    pl.part_bytes = backward ? ((size_t)a->batch * tiles * a->dim * sizeof(float) + 15) / 16 * 16 : 0;
+    return true;
+}
+void place_chains(Plan &pl, void *ws) {
+    uint8_t *base = static_cast<uint8_t *>(ws) + pl.part_bytes;
+    pl.ch.ticket = reinterpret_cast<unsigned int *>(base);
+    pl.ch.maps = reinterpret_cast<float2 *>(base + 256);
+}
+
 }  // namespace
 
+// The largest of the variants that the alignment could choose, so that the
+// size does not depend on pointers.
 size_t recurrence_workspace_bytes(const MambaRecurrenceArgs *a, bool backward) {
-    if (!a || a->batch <= 0 || a->seqlen < 0 || a->dim <= 0 || !backward) return 0;
-    return (size_t)a->batch * a->dim * sizeof(float);
+    if (!a || a->batch <= 0 || a->seqlen < 0 || a->dim <= 0) return 0;
+    size_t need = 0;
+    for (int vec : {1, backward ? kBwdVec : kFwdVec}) {
+        Plan pl;
+        if (!plan_chains(a, backward, vec, pl)) return 0;
+        need = std::max(need, pl.bytes + pl.part_bytes);
+    }
+    return need;
 }
+
+namespace {
+
+template <typename T>
+int launch_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
+    const FwdParams p = fwd_params(a);
+    constexpr int V = kFwdVec;
+    const bool vec = a->dim % V == 0 && vector_rows<T, V>(a->x, a->x_stride) && vector_rows<T, V>(a->r, a->r_stride) &&
+                     vector_rows<T, V>(a->i, a->i_stride) && vector_rows<T, V>(a->h, a->h_stride);
+    Plan pl;
+    MB_CHECK_ARG(plan_chains(a, false, vec ? V : 1, pl), "gated_recurrence: too many tiles");
+    place_chains(pl, ws);
+    Chains &c = pl.ch;
+    c.states = reinterpret_cast<float *>(c.maps + (int64_t)c.chains * c.tiles * 32 * (vec ? V : 1));
+    if (pl.bytes) MB_CUDA_TRY(cudaMemsetAsync(c.ticket, 0xff, pl.bytes, st));
+    const unsigned grid = (unsigned)(c.chains * c.tiles);
+    if (vec)
+        recurrence_fwd_kernel<T, V, 8, 4><<<grid, 128, 0, st>>>(p, c);
+    else
+        recurrence_fwd_kernel<T, 1, 8, 4><<<grid, 128, 0, st>>>(p, c);
+    return launch_status("gated_recurrence kernel");
+}
+
+template <typename T>
+int launch_backward(const MambaRecurrenceArgs *a, const BwdParams &p, const MambaRecurrenceGrads *g, void *ws,
+                    cudaStream_t st) {
+    constexpr int V = kBwdVec;
+    const bool vec = a->dim % V == 0 && vector_rows<T, V>(a->x, a->x_stride) && vector_rows<T, V>(a->r, a->r_stride) &&
+                     vector_rows<T, V>(a->i, a->i_stride) && vector_rows<T, V>(a->h, a->h_stride) &&
+                     vector_rows<T, V>(g->dh, g->dh_stride) && vector_rows<T, V>(g->dx, g->dx_stride) &&
+                     vector_rows<T, V>(g->dr, g->dr_stride) && vector_rows<T, V>(g->di, g->di_stride);
+    Plan pl;
+    MB_CHECK_ARG(plan_chains(a, true, vec ? V : 1, pl), "gated_recurrence_backward: too many tiles");
+    place_chains(pl, ws);
+    Chains &c = pl.ch;
+    c.states = reinterpret_cast<float *>(c.maps + (int64_t)c.chains * c.tiles * 32 * (vec ? V : 1));
+    if (pl.bytes) MB_CUDA_TRY(cudaMemsetAsync(c.ticket, 0xff, pl.bytes, st));
+    const unsigned grid = (unsigned)(c.chains * c.tiles);
+    if (vec)
+        recurrence_bwd_kernel<T, V, 8, 4><<<grid, 128, 0, st>>>(p, c);
+    else
+        recurrence_bwd_kernel<T, 1, 8, 4><<<grid, 128, 0, st>>>(p, c);
+    if (launch_status("gated_recurrence_backward kernel")) return -1;
+    recurrence_dlambda_kernel<<<(unsigned)ceil_div(a->dim, 32), 32 * kSumWarps, 0, st>>>(
+        p.part, a->lambda, g->dlambda, (int64_t)a->batch * c.tiles, a->dim);
+    return launch_status("gated_recurrence_backward sum kernel");
+}
+
+}  // namespace
 
 int recurrence_forward(const MambaRecurrenceArgs *a, void *ws, size_t ws_bytes, cudaStream_t st) {
     if (check_args(a, false)) return -1;
     if (a->batch == 0 || a->dim == 0) return 0;
-    const FwdParams p = fwd_params(a);
-    const dim3 grid((unsigned)ceil_div(a->dim, kThreads), (unsigned)a->batch);
-    if (a->dtype == MAMBA_F16)
-        recurrence_fwd_kernel<__half><<<grid, kThreads, 0, st>>>(p);
-    else
-        recurrence_fwd_kernel<float><<<grid, kThreads, 0, st>>>(p);
-    return launch_status("gated_recurrence kernel");
+    const size_t need = recurrence_workspace_bytes(a, false);
+    MB_CHECK_ARG(need == 0 || (ws && ws_bytes >= need && aligned_to(ws, 16)),
+                 "gated_recurrence: workspace too small or not 16-byte aligned");
+    return a->dtype == MAMBA_F16 ? launch_forward<__half>(a, ws, st) : launch_forward<float>(a, ws, st);
 }
 
 int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads *g, void *ws, size_t ws_bytes,
@@ -283,7 +808,8 @@ int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads
                      output_rows_disjoint(g->dr_stride, a->batch, a->seqlen, a->dim) &&
                      output_rows_disjoint(g->di_stride, a->batch, a->seqlen, a->dim),
                  "gated_recurrence_backward: rows of a gradient overlap (strides)");
-    MB_CHECK_ARG(ws && ws_bytes >= recurrence_workspace_bytes(a, true) && aligned_to(ws, 16),
+    const size_t need = recurrence_workspace_bytes(a, true);
+    MB_CHECK_ARG(ws && need && ws_bytes >= need && aligned_to(ws, 16),
                  "gated_recurrence_backward: workspace too small or not 16-byte aligned");
     BwdParams p{};
     p.f = fwd_params(a);
@@ -292,7 +818,6 @@ int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads
     p.dx = g->dx;
     p.dr = g->dr;
     p.di = g->di;
-    p.dlambda = g->dlambda;
     p.dh0 = g->dinitial_state;
     p.part = static_cast<float *>(ws);
     for (int k = 0; k < 2; ++k) {
@@ -301,15 +826,17 @@ int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads
         p.sdr[k] = g->dr_stride[k];
         p.sdi[k] = g->di_stride[k];
     }
-    const dim3 grid((unsigned)ceil_div(a->dim, kThreads), (unsigned)a->batch);
-    if (a->dtype == MAMBA_F16)
-        recurrence_bwd_kernel<__half><<<grid, kThreads, 0, st>>>(p);
-    else
-        recurrence_bwd_kernel<float><<<grid, kThreads, 0, st>>>(p);
-    if (launch_status("gated_recurrence_backward kernel")) return -1;
-    recurrence_dlambda_kernel<<<(unsigned)ceil_div(a->dim, kThreads), kThreads, 0, st>>>(p.part, a->lambda,
-                                                                                          g->dlambda, a->batch, a->dim);
-    return launch_status("gated_recurrence_backward sum kernel");
+    return a->dtype == MAMBA_F16 ? launch_backward<__half>(a, p, g, ws, st) : launch_backward<float>(a, p, g, ws, st);
+}
+
+unsigned recurrence_error_flags(bool clear) {
+    unsigned v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_recurrence_error, sizeof(v)) != cudaSuccess) return ~0u;
+    if (clear && v) {
+        const unsigned z = 0;
+        cudaMemcpyToSymbol(g_recurrence_error, &z, sizeof(z));
+    }
+    return v;
 }
 
 int recurrence_step(const void *x, int64_t xrs, const void *r, int64_t rrs, const void *i, int64_t irs,

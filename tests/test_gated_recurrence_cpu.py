@@ -73,6 +73,19 @@ def test_forward_refusals(change, text):
     assert text in mb.last_error()
 
 
+def test_forward_workspace_refusals():
+    L = mb.lib()
+    a = _args(L=5000)
+    need = L.mamba_gated_recurrence_workspace(ctypes.byref(a), 0)
+    assert need > 0
+    for ws, n in ((None, need), (4096, need - 1), (4104, need)):
+        assert _forward(a, ws, n) == -1 and "workspace" in mb.last_error()
+    a = _args(B=60000, L=2 ** 31 - 1, D=2 ** 20)
+    for s in (a.x_stride, a.r_stride, a.i_stride, a.h_stride):
+        s[0], s[1] = 2 ** 52, 2 ** 20
+    assert _forward(a, 4096, 2 ** 62) == -1 and "too many tiles" in mb.last_error()
+
+
 def test_overlapping_output_rows_refused():
     a = _args()
     a.h_stride[1] = 7
