@@ -180,22 +180,34 @@ struct Waiting {
 template <int VEC>
 __device__ __forceinline__ void wait_maps(const float2 *slot, float2 (&m)[VEC]) {
     Waiting wt;
+    bool ready;
+    do {
+        uint64_t w[VEC];
+        ready = true;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-        uint64_t w = get_map(slot + k);
-        while ((uint32_t)w == kEmpty && wt.again()) w = get_map(slot + k);
-        m[k] = make_float2(__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32)));
-    }
+        for (int k = 0; k < VEC; ++k) w[k] = get_map(slot + k);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            ready &= (uint32_t)w[k] != kEmpty;
+            m[k] = make_float2(__uint_as_float((uint32_t)w[k]), __uint_as_float((uint32_t)(w[k] >> 32)));
+        }
+    } while (!ready && wt.again());
 }
 template <int VEC>
 __device__ __forceinline__ void wait_states(const float *slot, float (&h)[VEC]) {
     Waiting wt;
+    bool ready;
+    do {
+        uint32_t w[VEC];
+        ready = true;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-        uint32_t w = get_state(slot + k);
-        while (w == kEmpty && wt.again()) w = get_state(slot + k);
-        h[k] = __uint_as_float(w);
-    }
+        for (int k = 0; k < VEC; ++k) w[k] = get_state(slot + k);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            ready &= w[k] != kEmpty;
+            h[k] = __uint_as_float(w[k]);
+        }
+    } while (!ready && wt.again());
 }
 
 struct Chains {
@@ -207,54 +219,95 @@ struct Chains {
     int tiles;
 };
 
-// This CTA's chain and its place in it, in the order the state runs.
-__device__ __forceinline__ void take_tile(const Chains &c, int &chain, int &k) {
-    __shared__ unsigned int id;
-    unsigned int v = blockIdx.x;
-    if (c.tiles > 1) {
-        if (threadIdx.x == 0) id = atomicAdd(c.ticket, 1u) + 1u;  // starts as all ones bits
-        __syncthreads();
-        v = id;
+// Hands out tickets one ahead: next() gives the ticket drawn by the call
+// before it (or at the start) and draws another, whose latency then hides
+// behind a tile's work.  Each call syncs the CTA.
+struct Tickets {
+    unsigned int *counter, *shared;  // shared: two places, used in turn
+    unsigned int ahead = 0, turn = 0;
+    __device__ __forceinline__ Tickets(unsigned int *c, unsigned int *s) : counter(c), shared(s) {
+        if (threadIdx.x == 0) ahead = atomicAdd(counter, 1u) + 1u;  // the counter starts as all ones bits
     }
-    k = (int)(v / (unsigned)c.chains);
-    chain = (int)(v - (unsigned)k * (unsigned)c.chains);
-}
+    __device__ __forceinline__ unsigned int next() {
+        turn ^= 1;
+        if (threadIdx.x == 0) shared[turn] = ahead;
+        __syncthreads();
+        const unsigned int v = shared[turn];
+        if (threadIdx.x == 0) ahead = atomicAdd(counter, 1u) + 1u;
+        return v;
+    }
+};
 
-// The state entering tile k of a chain: `first` (the chain's initial state) or
-// the state leaving the group before, then the group's tiles before k in
-// order.  Warp w publishes nothing and waits for the maps of tiles w, w + W, ...
-// of the group; the maps meet in shared memory.  Returns the state in every
-// warp.  Call after the tile's own map is published; syncs the CTA.
+// The map from the state at the start of tile k's group to the state entering
+// this warp's tokens (m), for the last warp also to the state leaving the
+// tile (end).  Warps wait for the maps of the group's earlier tiles between
+// them; `wm` holds the maps of this tile's warps.  Syncs the CTA.
 template <int VEC, int W>
-__device__ __forceinline__ void entering_state(const Chains &c, int chain, int k, const float (&first)[VEC],
-                                               float2 (*gm)[VEC * 32], float *gs, float (&h)[VEC]) {
+__device__ __forceinline__ void prefix_maps(const Chains &c, int chain, int k, const float2 (*wm)[VEC * 32],
+                                            float2 (*gm)[VEC * 32], float2 (&m)[VEC], float2 (&end)[VEC]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cw = VEC * 32;
     const int g = k / kGroup, j = k % kGroup;
 #pragma unroll
-    for (int q = 0; q < (kGroup + W - 1) / W; ++q) {
+    for (int q = 0; q < (kGroup - 1 + W - 1) / W; ++q) {
         const int tile = warp + q * W;
         if (tile < j) {
-            float2 m[VEC];
-            wait_maps<VEC>(c.maps + ((int64_t)chain * c.tiles + g * kGroup + tile) * cw + lane * VEC, m);
+            float2 t[VEC];
+            wait_maps<VEC>(c.maps + ((int64_t)chain * c.tiles + g * kGroup + tile) * cw + lane * VEC, t);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) gm[tile][e * 32 + lane] = m[e];
-        } else if (tile == kGroup - 1 && g > 0) {
-            float s[VEC];
-            const int groups = (c.tiles + kGroup - 1) / kGroup;
-            wait_states<VEC>(c.states + ((int64_t)chain * groups + g - 1) * cw + lane * VEC, s);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) gs[e * 32 + lane] = s[e];
+            for (int e = 0; e < VEC; ++e) gm[tile][e * 32 + lane] = t[e];
         }
     }
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) h[e] = g > 0 ? gs[e * 32 + lane] : first[e];
+    for (int e = 0; e < VEC; ++e) m[e] = make_float2(1.f, 0.f);
+    auto then = [&](float2 &f, const float2 &q) {
+        f.y = fmaf(q.x, f.y, q.y);
+        f.x *= q.x;
+    };
     for (int t = 0; t < j; ++t)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float2 m = gm[t][e * 32 + lane];
-            h[e] = fmaf(m.x, h[e], m.y);
+        for (int e = 0; e < VEC; ++e) then(m[e], gm[t][e * 32 + lane]);
+    for (int w = 0; w < warp; ++w)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) then(m[e], wm[w][e * 32 + lane]);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        end[e] = m[e];
+        then(end[e], wm[warp][e * 32 + lane]);
+    }
+}
+
+// The state at the start of tile k's group: `first`, or what the group before
+// left.  Every warp waits for itself, so that the group's last warp can pass
+// the state on without another barrier.
+template <int VEC>
+__device__ __forceinline__ void group_state(const Chains &c, int chain, int k, float (&s)[VEC]) {
+    const int lane = threadIdx.x & 31, g = k / kGroup, groups = (c.tiles + kGroup - 1) / kGroup;
+    if (g > 0) wait_states<VEC>(c.states + ((int64_t)chain * groups + g - 1) * (VEC * 32) + lane * VEC, s);
+}
+template <int VEC>
+__device__ __forceinline__ void leave_group(const Chains &c, int chain, int k, const float (&h)[VEC]) {
+    const int lane = threadIdx.x & 31, groups = (c.tiles + kGroup - 1) / kGroup;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+        put_state(c.states + ((int64_t)chain * groups + k / kGroup) * (VEC * 32) + lane * VEC + e, h[e]);
+}
+
+// The tile's own map (warp maps in order), published for the group's later tiles.
+template <int VEC, int W>
+__device__ __forceinline__ void publish_map(const Chains &c, int chain, int k, const float2 (*wm)[VEC * 32]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        float2 m = make_float2(1.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float2 q = wm[w][e * 32 + lane];
+            m.y = fmaf(q.x, m.y, q.y);
+            m.x *= q.x;
         }
+        put_map(c.maps + ((int64_t)chain * c.tiles + k) * (VEC * 32) + lane * VEC + e, m.x, m.y);
+    }
 }
 
 // VEC consecutive elements, as loaded and as FP32.
@@ -267,7 +320,7 @@ __device__ __forceinline__ Pack<T, VEC> load_pack(const T *p) {
     return *reinterpret_cast<const Pack<T, VEC> *>(p);
 }
 
-// Tokens of this warp that exist, and which of them cut the state.
+// Which of this warp's tokens cut the state.
 __device__ __forceinline__ uint32_t cut_mask(const FwdParams &p, int b, int t0, int cnt) {
     if (!p.resets) return 0;
     const int lane = threadIdx.x & 31;
@@ -275,315 +328,337 @@ __device__ __forceinline__ uint32_t cut_mask(const FwdParams &p, int b, int t0, 
     return __ballot_sync(0xffffffffu, z);
 }
 
-template <typename T, int VEC, int S, int W>
-__global__ void __launch_bounds__(32 * W, 512 / (32 * W)) recurrence_fwd_kernel(const FwdParams p, const Chains ch) {
-    constexpr bool PRECISE = sizeof(T) == 4;
-    constexpr int cw = 32 * VEC;
-    __shared__ float2 wm[W][cw], gm[kGroup][cw];
-    __shared__ float gs[cw];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int chain, k;
-    take_tile(ch, chain, k);
-    const int b = chain / ch.blocks, d = (chain - b * ch.blocks) * cw + lane * VEC;
-    const int n = row_length(p, b);
-    const int tile0 = k * (S * W);
-    if (k > 0 && tile0 >= n) return;  // behind the row's end: no later tile of the row has work either
-    const bool in = d < p.D;
-    const int t0 = tile0 + warp * S;
-    const int cnt = in ? min(max(n - t0, 0), S) : 0;
-
-    float a[S][VEC], bt[S][VEC];
-    {
-        Pack<T, VEC> x[S], r[S], gi[S];
-        const T *px = static_cast<const T *>(p.x) + b * p.sx[0] + t0 * p.sx[1] + d;
-        const T *pr = static_cast<const T *>(p.r) + b * p.sr[0] + t0 * p.sr[1] + d;
-        const T *pi = static_cast<const T *>(p.i) + b * p.si[0] + t0 * p.si[1] + d;
-#pragma unroll
-        for (int j = 0; j < S; ++j)
-            if (j < cnt) {
-                r[j] = load_pack<T, VEC>(pr + j * p.sr[1]);
-                gi[j] = load_pack<T, VEC>(pi + j * p.si[1]);
-                x[j] = load_pack<T, VEC>(px + j * p.sx[1]);
-            }
-        float csp[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) csp[e] = in ? p.c * softplus_channel(p.lambda[d + e]) : 0.f;
-#pragma unroll
-        for (int j = 0; j < S; ++j) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                if (j < cnt) {
-                    const Decay g = decay<PRECISE>(cvt_f32(r[j].v[e]), csp[e]);
-                    float si, om;
-                    sigmoid2<PRECISE>(cvt_f32(gi[j].v[e]), si, om);
-                    a[j][e] = g.a;
-                    bt[j][e] = sqrt_gate<PRECISE>(one_minus_a2<PRECISE>(g.y, g.a)) * si * cvt_f32(x[j].v[e]);
-                } else {
-                    a[j][e] = 1.f;
-                    bt[j][e] = 0.f;
-                }
-            }
-        }
-    }
-    const uint32_t cut = cut_mask(p, b, t0, min(max(n - t0, 0), S));
-    if (cut)
-#pragma unroll
-        for (int j = 0; j < S; ++j)
-            if (cut >> j & 1)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) a[j][e] = 0.f;
-
-    // this warp's map, then the tile's (in warp 0) and its publication
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        float P = 1.f, H = 0.f;
-#pragma unroll
-        for (int j = 0; j < S; ++j) {
-            H = fmaf(a[j][e], H, bt[j][e]);
-            P *= a[j][e];
-        }
-        wm[warp][e * 32 + lane] = make_float2(P, H);
-    }
-    __syncthreads();
-    const bool more = k + 1 < ch.tiles && (k + 1) * (S * W) < n;  // a later tile waits for this one
-    if (warp == 0 && more && k % kGroup != kGroup - 1) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            float2 m = make_float2(1.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float2 q = wm[w][e * 32 + lane];
-                m.y = fmaf(q.x, m.y, q.y);
-                m.x *= q.x;
-            }
-            put_map(ch.maps + ((int64_t)chain * ch.tiles + k) * cw + lane * VEC + e, m.x, m.y);
-        }
-    }
-    float h[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) h[e] = in && p.h0 && k < kGroup ? p.h0[(int64_t)b * p.D + d + e] : 0.f;
-    if (k > 0) {
-        float first[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) first[e] = h[e];
-        entering_state<VEC, W>(ch, chain, k, first, gm, gs, h);
-    }
-    float hw[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        hw[e] = h[e];
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (w == warp) hw[e] = h[e];
-            const float2 q = wm[w][e * 32 + lane];
-            h[e] = fmaf(q.x, h[e], q.y);
-        }
-    }
-    if (warp == 0) {
-        if (more) {
-            if (k % kGroup == kGroup - 1) {
-                const int groups = (ch.tiles + kGroup - 1) / kGroup;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    put_state(ch.states + ((int64_t)chain * groups + k / kGroup) * cw + lane * VEC + e, h[e]);
-            }
-        } else if (in && p.hN) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) p.hN[(int64_t)b * p.D + d + e] = h[e];
-        }
-    }
-    T *ph = static_cast<T *>(p.h) + b * p.sh[0] + t0 * p.sh[1] + d;
-#pragma unroll
-    for (int j = 0; j < S; ++j)
-        if (j < cnt) {
-            Pack<T, VEC> o;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                hw[e] = fmaf(a[j][e], hw[e], bt[j][e]);
-                o.v[e] = cvt_out<T>(hw[e]);
-            }
-            *reinterpret_cast<Pack<T, VEC> *>(ph + j * p.sh[1]) = o;
-        }
+// Copies VEC elements to this thread's own place in shared memory,
+// asynchronously where they make at least the 4 bytes cp.async takes.
+template <typename T, int VEC>
+__device__ __forceinline__ void copy_pack(Pack<T, VEC> *dst, const T *src) {
+    if constexpr (sizeof(T) * VEC >= 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src),
+                     "n"((int)(sizeof(T) * VEC))
+                     : "memory");
+    else
+        *dst = load_pack<T, VEC>(src);
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Backward: the same tiles and chains with time reversed; what runs along a
-// chain is C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.
-template <typename T, int VEC, int S, int W>
-__global__ void __launch_bounds__(32 * W, 512 / (32 * W)) recurrence_bwd_kernel(const BwdParams p, const Chains ch) {
-    constexpr bool PRECISE = sizeof(T) == 4;
-    constexpr int cw = 32 * VEC;
-    __shared__ float2 wm[W][cw], gm[kGroup][cw];
-    __shared__ float gs[cw];
-    const FwdParams &f = p.f;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int chain, k;
-    take_tile(ch, chain, k);
-    const int b = chain / ch.blocks, d = (chain - b * ch.blocks) * cw + lane * VEC;
-    const int n = row_length(f, b);
-    const bool in = d < f.D;
-    const int row_tiles = max((n + S * W - 1) / (S * W), 1);
-    float *part = p.part + ((int64_t)b * ch.tiles + k) * f.D + d;
-    if (k >= row_tiles) {  // behind the row's end
-        if (warp == 0 && in)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) part[e] = 0.f;
-        return;
-    }
-    const int t0 = (row_tiles - 1 - k) * (S * W) + (W - 1 - warp) * S;  // warp 0 holds the tile's last tokens
-    const int cnt = in ? min(max(n - t0, 0), S) : 0;
+template <bool PRECISE>
+__device__ __forceinline__ float channel_softplus(float l) {
+    return PRECISE ? softplus_channel(l) : softplus_fast(l);
+}
 
-    Pack<T, VEC> x[S], gi[S], hp[S], dh[S];
-    float a[S][VEC], y[S][VEC], om[S][VEC];
-    {
-        Pack<T, VEC> r[S];
-        const T *pr = static_cast<const T *>(f.r) + b * f.sr[0] + t0 * f.sr[1] + d;
-        const T *pg = static_cast<const T *>(p.dh) + b * p.sdh[0] + t0 * p.sdh[1] + d;
-        const T *px = static_cast<const T *>(f.x) + b * f.sx[0] + t0 * f.sx[1] + d;
-        const T *pi = static_cast<const T *>(f.i) + b * f.si[0] + t0 * f.si[1] + d;
-        const T *ph = static_cast<const T *>(f.h) + b * f.sh[0] + (t0 - 1) * f.sh[1] + d;
+// Which tile a ticket stands for: time-major, all chains' k-th tiles together.
+struct Tile {
+    int chain, k, b, d, n, t0, cnt;
+    bool live, in;
+};
+
+// ---- forward --------------------------------------------------------------------
+// Persistent CTAs: the copies of the next tile's x, r and i into shared memory
+// run while the current tile is computed and waits for its state.  A thread
+// reads back only what it copied itself, so no barrier guards the buffers.
+template <typename T, int VEC, int S, int W>
+struct FwdSmem {
+    Pack<T, VEC> in[2][3][S][32 * W];
+    float2 wm[W][32 * VEC], gm[kGroup][32 * VEC];
+    unsigned int ticket[2];
+};
+
+template <typename T, int VEC, int S, int W, int CTAS>
+__global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdParams p, const Chains ch) {
+    constexpr bool PRECISE = sizeof(T) == 4;
+    constexpr int cw = 32 * VEC, TT = S * W;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    auto &sm = *reinterpret_cast<FwdSmem<T, VEC, S, W> *>(smem_raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const unsigned total = (unsigned)ch.chains * (unsigned)ch.tiles;
+
+    auto place = [&](unsigned v) {
+        Tile t;
+        t.k = (int)(v / (unsigned)ch.chains);
+        t.chain = (int)(v - (unsigned)t.k * (unsigned)ch.chains);
+        t.b = t.chain / ch.blocks;
+        t.d = (t.chain - t.b * ch.blocks) * cw + lane * VEC;
+        t.n = row_length(p, t.b);
+        t.t0 = t.k * TT + warp * S;
+        t.live = t.k == 0 || t.k * TT < t.n;  // else behind the row's end
+        t.in = t.d < p.D;
+        t.cnt = t.in ? min(max(t.n - t.t0, 0), S) : 0;
+        return t;
+    };
+    auto fetch = [&](const Tile &t, int buf) {
+        const T *px = static_cast<const T *>(p.x) + t.b * p.sx[0] + t.t0 * p.sx[1] + t.d;
+        const T *pr = static_cast<const T *>(p.r) + t.b * p.sr[0] + t.t0 * p.sr[1] + t.d;
+        const T *pi = static_cast<const T *>(p.i) + t.b * p.si[0] + t.t0 * p.si[1] + t.d;
 #pragma unroll
         for (int j = 0; j < S; ++j)
-            if (j < cnt) {
-                r[j] = load_pack<T, VEC>(pr + j * f.sr[1]);
-                dh[j] = load_pack<T, VEC>(pg + j * p.sdh[1]);
+            if (j < t.cnt) {
+                copy_pack<T, VEC>(&sm.in[buf][0][j][tid], pr + j * p.sr[1]);
+                copy_pack<T, VEC>(&sm.in[buf][1][j][tid], pi + j * p.si[1]);
+                copy_pack<T, VEC>(&sm.in[buf][2][j][tid], px + j * p.sx[1]);
             }
+    };
+
+    Tickets tickets(ch.ticket, sm.ticket);
+    unsigned v = tickets.next();
+    if (v >= total) return;
+    Tile t = place(v);
+    fetch(t, 0);
+    copy_commit();
+    for (int buf = 0;; buf ^= 1) {
+        const unsigned vn = tickets.next();  // its barrier also frees sm.wm and sm.gm
+        Tile tn{};
+        if (vn < total) {
+            tn = place(vn);
+            fetch(tn, buf ^ 1);
+        }
+        copy_commit();
+        copy_wait<1>();
+        if (t.live) {
+            float a[S][VEC], bt[S][VEC], csp[VEC];
 #pragma unroll
-        for (int j = 0; j < S; ++j)
-            if (j < cnt) {
-                x[j] = load_pack<T, VEC>(px + j * f.sx[1]);
-                gi[j] = load_pack<T, VEC>(pi + j * f.si[1]);
-                if (t0 + j > 0) hp[j] = load_pack<T, VEC>(ph + j * f.sh[1]);
+            for (int e = 0; e < VEC; ++e) csp[e] = t.in ? p.c * channel_softplus<PRECISE>(p.lambda[t.d + e]) : 0.f;
+#pragma unroll
+            for (int j = 0; j < S; ++j) {
+                const Pack<T, VEC> r = sm.in[buf][0][j][tid], gi = sm.in[buf][1][j][tid], x = sm.in[buf][2][j][tid];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const Decay g = decay<PRECISE>(cvt_f32(r.v[e]), csp[e]);
+                    float si, om;
+                    sigmoid2<PRECISE>(cvt_f32(gi.v[e]), si, om);
+                    const float bv = sqrt_gate<PRECISE>(one_minus_a2<PRECISE>(g.y, g.a)) * si * cvt_f32(x.v[e]);
+                    a[j][e] = j < t.cnt ? g.a : 1.f;  // what the buffer holds behind the end does not count
+                    bt[j][e] = j < t.cnt ? bv : 0.f;
+                }
             }
-        float csp[VEC];
+            const uint32_t cut = cut_mask(p, t.b, t.t0, min(max(t.n - t.t0, 0), S));
+            if (cut)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) csp[e] = in ? f.c * softplus_channel(f.lambda[d + e]) : 0.f;
+                for (int j = 0; j < S; ++j)
+                    if (cut >> j & 1)
 #pragma unroll
-        for (int j = 0; j < S; ++j)
+                        for (int e = 0; e < VEC; ++e) a[j][e] = 0.f;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                if (j < cnt) {
-                    const Decay g = decay<PRECISE>(cvt_f32(r[j].v[e]), csp[e]);
+                float P = 1.f, H = 0.f;
+#pragma unroll
+                for (int j = 0; j < S; ++j) {
+                    H = fmaf(a[j][e], H, bt[j][e]);
+                    P *= a[j][e];
+                }
+                sm.wm[warp][e * 32 + lane] = make_float2(P, H);
+            }
+            __syncthreads();
+            const bool more = (t.k + 1) * TT < t.n;  // a later tile waits for this one
+            const bool last = t.k % kGroup == kGroup - 1;
+            if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t.chain, t.k, sm.wm);
+            float2 m[VEC], end[VEC];
+            prefix_maps<VEC, W>(ch, t.chain, t.k, sm.wm, sm.gm, m, end);
+            float s[VEC], h[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                s[e] = t.in && p.h0 && t.k < kGroup ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
+            group_state<VEC>(ch, t.chain, t.k, s);
+            if (warp == W - 1 && (last || !more)) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) h[e] = fmaf(end[e].x, s[e], end[e].y);
+                if (more)
+                    leave_group<VEC>(ch, t.chain, t.k, h);
+                else if (t.in && p.hN)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) p.hN[(int64_t)t.b * p.D + t.d + e] = h[e];
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) h[e] = fmaf(m[e].x, s[e], m[e].y);
+            T *ph = static_cast<T *>(p.h) + t.b * p.sh[0] + t.t0 * p.sh[1] + t.d;
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                if (j < t.cnt) {
+                    Pack<T, VEC> o;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        h[e] = fmaf(a[j][e], h[e], bt[j][e]);
+                        o.v[e] = cvt_out<T>(h[e]);
+                    }
+                    *reinterpret_cast<Pack<T, VEC> *>(ph + j * p.sh[1]) = o;
+                }
+        }
+        if (vn >= total) break;
+        t = tn;
+    }
+}
+
+// ---- backward -------------------------------------------------------------------
+// The same tiles and chains with time reversed; what runs along a chain is
+// C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.
+template <typename T, int VEC, int S, int W>
+struct BwdSmem {
+    Pack<T, VEC> in[2][5][S][32 * W];
+    float2 wm[W][32 * VEC], gm[kGroup][32 * VEC];
+    float sums[W][32 * VEC];
+    unsigned int ticket[2];
+};
+
+template <typename T, int VEC, int S, int W, int CTAS>
+__global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdParams p, const Chains ch) {
+    constexpr bool PRECISE = sizeof(T) == 4;
+    constexpr int cw = 32 * VEC, TT = S * W;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    auto &sm = *reinterpret_cast<BwdSmem<T, VEC, S, W> *>(smem_raw);
+    const FwdParams &f = p.f;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const unsigned total = (unsigned)ch.chains * (unsigned)ch.tiles;
+
+    auto place = [&](unsigned v) {
+        Tile t;
+        t.k = (int)(v / (unsigned)ch.chains);
+        t.chain = (int)(v - (unsigned)t.k * (unsigned)ch.chains);
+        t.b = t.chain / ch.blocks;
+        t.d = (t.chain - t.b * ch.blocks) * cw + lane * VEC;
+        t.n = row_length(f, t.b);
+        const int row_tiles = max((t.n + TT - 1) / TT, 1);
+        t.live = t.k < row_tiles;
+        t.t0 = (row_tiles - 1 - t.k) * TT + (W - 1 - warp) * S;  // warp 0 holds the tile's last tokens
+        t.in = t.d < f.D;
+        t.cnt = t.in && t.live ? min(max(t.n - t.t0, 0), S) : 0;
+        return t;
+    };
+    auto fetch = [&](const Tile &t, int buf) {
+        const T *pr = static_cast<const T *>(f.r) + t.b * f.sr[0] + t.t0 * f.sr[1] + t.d;
+        const T *pg = static_cast<const T *>(p.dh) + t.b * p.sdh[0] + t.t0 * p.sdh[1] + t.d;
+        const T *px = static_cast<const T *>(f.x) + t.b * f.sx[0] + t.t0 * f.sx[1] + t.d;
+        const T *pi = static_cast<const T *>(f.i) + t.b * f.si[0] + t.t0 * f.si[1] + t.d;
+        const T *ph = static_cast<const T *>(f.h) + t.b * f.sh[0] + (t.t0 - 1) * f.sh[1] + t.d;
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+            if (j < t.cnt) {
+                copy_pack<T, VEC>(&sm.in[buf][0][j][tid], pr + j * f.sr[1]);
+                copy_pack<T, VEC>(&sm.in[buf][1][j][tid], pg + j * p.sdh[1]);
+                copy_pack<T, VEC>(&sm.in[buf][2][j][tid], px + j * f.sx[1]);
+                copy_pack<T, VEC>(&sm.in[buf][3][j][tid], pi + j * f.si[1]);
+                if (t.t0 + j > 0) copy_pack<T, VEC>(&sm.in[buf][4][j][tid], ph + j * f.sh[1]);
+            }
+    };
+
+    Tickets tickets(ch.ticket, sm.ticket);
+    unsigned v = tickets.next();
+    if (v >= total) return;
+    Tile t = place(v);
+    fetch(t, 0);
+    copy_commit();
+    for (int buf = 0;; buf ^= 1) {
+        const unsigned vn = tickets.next();  // its barrier also frees sm.wm and sm.gm
+        Tile tn{};
+        if (vn < total) {
+            tn = place(vn);
+            fetch(tn, buf ^ 1);
+        }
+        copy_commit();
+        copy_wait<1>();
+        float *part = p.part + ((int64_t)t.b * ch.tiles + t.k) * f.D + t.d;
+        if (t.live) {
+            float a[S][VEC], y[S][VEC], om[S][VEC], csp[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) csp[e] = t.in ? f.c * channel_softplus<PRECISE>(f.lambda[t.d + e]) : 0.f;
+            const uint32_t cut = cut_mask(f, t.b, t.t0, min(max(t.n - t.t0, 0), S));
+            float2 own[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) own[e] = make_float2(1.f, 0.f);
+#pragma unroll
+            for (int j = S - 1; j >= 0; --j) {
+                const Pack<T, VEC> r = sm.in[buf][0][j][tid], dh = sm.in[buf][1][j][tid];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const Decay g = decay<PRECISE>(cvt_f32(r.v[e]), csp[e]);
                     a[j][e] = g.a;
                     y[j][e] = g.y;
                     om[j][e] = g.om;
-                } else {
-                    a[j][e] = 1.f;
-                    y[j][e] = om[j][e] = 0.f;
+                    if (j < t.cnt) {  // what the buffer holds behind the end does not count
+                        const float ak = cut >> j & 1 ? 0.f : g.a;
+                        own[e].y = ak * (cvt_f32(dh.v[e]) + own[e].y);
+                        own[e].x *= ak;
+                    }
                 }
             }
-    }
-    const uint32_t cut = cut_mask(f, b, t0, min(max(n - t0, 0), S));
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        float P = 1.f, H = 0.f;
+            for (int e = 0; e < VEC; ++e) sm.wm[warp][e * 32 + lane] = own[e];
+            __syncthreads();
+            const bool more = t.t0 - (W - 1 - warp) * S > 0;  // an earlier tile waits for this one
+            const bool last = t.k % kGroup == kGroup - 1;
+            if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t.chain, t.k, sm.wm);
+            float2 m[VEC], end[VEC];
+            prefix_maps<VEC, W>(ch, t.chain, t.k, sm.wm, sm.gm, m, end);
+            float s[VEC], C[VEC];
 #pragma unroll
-        for (int j = S - 1; j >= 0; --j) {
-            const float g = (j < cnt ? cvt_f32(dh[j].v[e]) : 0.f) + H;
-            const float ak = cut >> j & 1 ? 0.f : a[j][e];
-            H = ak * g;
-            P *= ak;
-        }
-        wm[warp][e * 32 + lane] = make_float2(P, H);
-    }
-    __syncthreads();
-    const bool more = k + 1 < row_tiles;
-    if (warp == 0 && more && k % kGroup != kGroup - 1) {
+            for (int e = 0; e < VEC; ++e)
+                s[e] = t.in && p.dhN && t.k < kGroup ? p.dhN[(int64_t)t.b * f.D + t.d + e] : 0.f;
+            group_state<VEC>(ch, t.chain, t.k, s);
+            if (warp == W - 1 && (last || !more)) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            float2 m = make_float2(1.f, 0.f);
+                for (int e = 0; e < VEC; ++e) C[e] = fmaf(end[e].x, s[e], end[e].y);
+                if (more)
+                    leave_group<VEC>(ch, t.chain, t.k, C);
+                else if (t.in && p.dh0)
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float2 q = wm[w][e * 32 + lane];
-                m.y = fmaf(q.x, m.y, q.y);
-                m.x *= q.x;
+                    for (int e = 0; e < VEC; ++e) p.dh0[(int64_t)t.b * f.D + t.d + e] = C[e];
             }
-            put_map(ch.maps + ((int64_t)chain * ch.tiles + k) * cw + lane * VEC + e, m.x, m.y);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) C[e] = fmaf(m[e].x, s[e], m[e].y);
+            T *qx = static_cast<T *>(p.dx) + t.b * p.sdx[0] + t.t0 * p.sdx[1] + t.d;
+            T *qr = static_cast<T *>(p.dr) + t.b * p.sdr[0] + t.t0 * p.sdr[1] + t.d;
+            T *qi = static_cast<T *>(p.di) + t.b * p.sdi[0] + t.t0 * p.sdi[1] + t.d;
+            float sum[VEC] = {};
+#pragma unroll
+            for (int j = S - 1; j >= 0; --j)
+                if (j < t.cnt) {
+                    const Pack<T, VEC> dh = sm.in[buf][1][j][tid], x = sm.in[buf][2][j][tid],
+                                       gi = sm.in[buf][3][j][tid], hp = sm.in[buf][4][j][tid];
+                    Pack<T, VEC> ox, orr, oi;
+                    const bool keep = !(cut >> j & 1);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float av = a[j][e], yv = y[j][e], xv = cvt_f32(x.v[e]);
+                        const float G = cvt_f32(dh.v[e]) + C[e];
+                        C[e] = (keep ? av : 0.f) * G;
+                        float si, omi, beta, q;
+                        sigmoid2<PRECISE>(cvt_f32(gi.v[e]), si, omi);
+                        root_gate<PRECISE>(one_minus_a2<PRECISE>(yv, av), yv, beta, q);
+                        float prev = cvt_f32(hp.v[e]);
+                        if (t.t0 + j == 0) prev = f.h0 ? f.h0[(int64_t)t.b * f.D + t.d + e] : 0.f;
+                        if (!keep) prev = 0.f;
+                        const float gx = G * beta * si;
+                        const float E = G * (si * xv * av * av * q - yv * av * prev);
+                        sum[e] += E;
+                        ox.v[e] = cvt_out<T>(gx);
+                        oi.v[e] = cvt_out<T>(gx * xv * omi);
+                        orr.v[e] = cvt_out<T>(E * om[j][e]);
+                    }
+                    *reinterpret_cast<Pack<T, VEC> *>(qx + j * p.sdx[1]) = ox;
+                    *reinterpret_cast<Pack<T, VEC> *>(qi + j * p.sdi[1]) = oi;
+                    *reinterpret_cast<Pack<T, VEC> *>(qr + j * p.sdr[1]) = orr;
+                }
+            // the tile's sum of E per channel, warps in order
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sm.sums[warp][e * 32 + lane] = sum[e];
+            __syncthreads();
+            if (warp == 0 && t.in)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    float v = 0.f;
+#pragma unroll
+                    for (int w = 0; w < W; ++w) v += sm.sums[w][e * 32 + lane];
+                    part[e] = v;
+                }
+        } else if (warp == 0 && t.in) {  // behind the row's end
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) part[e] = 0.f;
         }
+        if (vn >= total) break;
+        t = tn;
     }
-    float C[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) C[e] = in && p.dhN && k < kGroup ? p.dhN[(int64_t)b * f.D + d + e] : 0.f;
-    if (k > 0) {
-        float first[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) first[e] = C[e];
-        entering_state<VEC, W>(ch, chain, k, first, gm, gs, C);
-    }
-    float cv[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        cv[e] = C[e];
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (w == warp) cv[e] = C[e];
-            const float2 q = wm[w][e * 32 + lane];
-            C[e] = fmaf(q.x, C[e], q.y);
-        }
-    }
-    if (warp == 0) {
-        if (more) {
-            if (k % kGroup == kGroup - 1) {
-                const int groups = (ch.tiles + kGroup - 1) / kGroup;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    put_state(ch.states + ((int64_t)chain * groups + k / kGroup) * cw + lane * VEC + e, C[e]);
-            }
-        } else if (in && p.dh0) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) p.dh0[(int64_t)b * f.D + d + e] = C[e];
-        }
-    }
-    T *qx = static_cast<T *>(p.dx) + b * p.sdx[0] + t0 * p.sdx[1] + d;
-    T *qr = static_cast<T *>(p.dr) + b * p.sdr[0] + t0 * p.sdr[1] + d;
-    T *qi = static_cast<T *>(p.di) + b * p.sdi[0] + t0 * p.sdi[1] + d;
-    float sum[VEC] = {};
-#pragma unroll
-    for (int j = S - 1; j >= 0; --j) {
-        if (j < cnt) {
-            Pack<T, VEC> ox, orr, oi;
-            const bool keep = !(cut >> j & 1);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float av = a[j][e], yv = y[j][e], xv = cvt_f32(x[j].v[e]);
-                const float G = cvt_f32(dh[j].v[e]) + cv[e];
-                const float ca = keep ? av : 0.f;
-                cv[e] = ca * G;
-                float si, omi;
-                sigmoid2<PRECISE>(cvt_f32(gi[j].v[e]), si, omi);
-                const float m = one_minus_a2<PRECISE>(yv, av);
-                float beta, q;
-                root_gate<PRECISE>(m, yv, beta, q);
-                float prev;
-                if (t0 + j > 0)
-                    prev = cvt_f32(hp[j].v[e]);
-                else
-                    prev = f.h0 ? f.h0[(int64_t)b * f.D + d + e] : 0.f;
-                if (!keep) prev = 0.f;
-                const float gx = G * beta * si;
-                const float E = G * (si * xv * av * av * q - yv * av * prev);
-                sum[e] += E;
-                ox.v[e] = cvt_out<T>(gx);
-                oi.v[e] = cvt_out<T>(gx * xv * omi);
-                orr.v[e] = cvt_out<T>(E * om[j][e]);
-            }
-            *reinterpret_cast<Pack<T, VEC> *>(qx + j * p.sdx[1]) = ox;
-            *reinterpret_cast<Pack<T, VEC> *>(qi + j * p.sdi[1]) = oi;
-            *reinterpret_cast<Pack<T, VEC> *>(qr + j * p.sdr[1]) = orr;
-        }
-    }
-    // the tile's sum of E per channel, warps in order
-    __syncthreads();  // wm is free again
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) wm[warp][e * 32 + lane].x = sum[e];
-    __syncthreads();
-    if (warp == 0 && in)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            float s = 0.f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) s += wm[w][e * 32 + lane].x;
-            part[e] = s;
-        }
 }
 
 // dlambda[d] = sigmoid(lambda)/softplus(lambda) * sum of the tiles' sums of E,
@@ -686,9 +761,12 @@ FwdParams fwd_params(const MambaRecurrenceArgs *a) {
     return p;
 }
 
-// Channels a thread holds (1 serves any alignment and channel count).
-constexpr int kFwdVec = 4, kBwdVec = 2;
-constexpr int kFwdTile = 32, kBwdTile = 32;  // tokens of a tile (S * W)
+// Tile shapes: channels a thread holds (1 serves any alignment and channel
+// count), tokens a warp holds, warps and CTAs per SM.
+constexpr int kFwdS = 8, kFwdW = 4, kFwdCtas = 4;
+constexpr int kBwdS = 8, kBwdW = 4, kBwdCtas = 4;
+constexpr int fwd_vec(int dtype) { return dtype == MAMBA_F16 ? 4 : 2; }
+constexpr int bwd_vec(int dtype) { return dtype == MAMBA_F16 ? 2 : 1; }
 
 // The chains of a call and where its workspace holds what.
 struct Plan {
@@ -696,7 +774,7 @@ struct Plan {
     size_t bytes, part_bytes;
 };
 bool plan_chains(const MambaRecurrenceArgs *a, bool backward, int vec, Plan &pl) {
-    const int tile = backward ? kBwdTile : kFwdTile, cw = 32 * vec;
+    const int tile = backward ? kBwdS * kBwdW : kFwdS * kFwdW, cw = 32 * vec;
     Chains &c = pl.ch;
     c = Chains{};
     const int64_t blocks = ceil_div64(a->dim, cw), tiles = std::max<int64_t>(1, ceil_div64(a->seqlen, tile));
@@ -704,16 +782,10 @@ bool plan_chains(const MambaRecurrenceArgs *a, bool backward, int vec, Plan &pl)
     c.blocks = (int)blocks;
     c.chains = (int)blocks * a->batch;
     c.tiles = (int)tiles;
-    pl.bytes = 0;
-    if (tiles > 1)
-        pl.bytes = 256 + (size_t)c.chains * cw * (tiles * sizeof(float2) + ceil_div64(tiles, kGroup) * sizeof(float));
+    pl.bytes = 256 + (size_t)c.chains * cw * (tiles * sizeof(float2) + ceil_div64(tiles, kGroup) * sizeof(float));
+    if (tiles == 1) pl.bytes = 256;
     pl.part_bytes = backward ? ((size_t)a->batch * tiles * a->dim * sizeof(float) + 15) / 16 * 16 : 0;
     return true;
-}
-void place_chains(Plan &pl, void *ws) {
-    uint8_t *base = static_cast<uint8_t *>(ws) + pl.part_bytes;
-    pl.ch.ticket = reinterpret_cast<unsigned int *>(base);
-    pl.ch.maps = reinterpret_cast<float2 *>(base + 256);
 }
 
 }  // namespace
@@ -723,7 +795,7 @@ void place_chains(Plan &pl, void *ws) {
 size_t recurrence_workspace_bytes(const MambaRecurrenceArgs *a, bool backward) {
     if (!a || a->batch <= 0 || a->seqlen < 0 || a->dim <= 0) return 0;
     size_t need = 0;
-    for (int vec : {1, backward ? kBwdVec : kFwdVec}) {
+    for (int vec : {1, backward ? bwd_vec(a->dtype) : fwd_vec(a->dtype)}) {
         Plan pl;
         if (!plan_chains(a, backward, vec, pl)) return 0;
         need = std::max(need, pl.bytes + pl.part_bytes);
@@ -733,48 +805,58 @@ size_t recurrence_workspace_bytes(const MambaRecurrenceArgs *a, bool backward) {
 
 namespace {
 
-template <typename T>
-int launch_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
-    const FwdParams p = fwd_params(a);
-    constexpr int V = kFwdVec;
-    const bool vec = a->dim % V == 0 && vector_rows<T, V>(a->x, a->x_stride) && vector_rows<T, V>(a->r, a->r_stride) &&
-                     vector_rows<T, V>(a->i, a->i_stride) && vector_rows<T, V>(a->h, a->h_stride);
-    Plan pl;
-    MB_CHECK_ARG(plan_chains(a, false, vec ? V : 1, pl), "gated_recurrence: too many tiles");
-    place_chains(pl, ws);
+// Launches one variant: the workspace's part from the ticket on set to all
+// ones bits, then persistent CTAs.
+template <int VEC, typename Kernel, typename Params>
+int launch_tiles(Kernel kernel, const Params &p, Plan &pl, int threads, int ctas, size_t smem, void *ws,
+                 cudaStream_t st, const char *what) {
     Chains &c = pl.ch;
-    c.states = reinterpret_cast<float *>(c.maps + (int64_t)c.chains * c.tiles * 32 * (vec ? V : 1));
-    if (pl.bytes) MB_CUDA_TRY(cudaMemsetAsync(c.ticket, 0xff, pl.bytes, st));
-    const unsigned grid = (unsigned)(c.chains * c.tiles);
-    if (vec)
-        recurrence_fwd_kernel<T, V, 8, 4><<<grid, 128, 0, st>>>(p, c);
-    else
-        recurrence_fwd_kernel<T, 1, 8, 4><<<grid, 128, 0, st>>>(p, c);
-    return launch_status("gated_recurrence kernel");
+    uint8_t *base = static_cast<uint8_t *>(ws) + pl.part_bytes;
+    c.ticket = reinterpret_cast<unsigned int *>(base);
+    c.maps = reinterpret_cast<float2 *>(base + 256);
+    c.states = reinterpret_cast<float *>(c.maps + (int64_t)c.chains * c.tiles * 32 * VEC);
+    MB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    MB_CUDA_TRY(cudaMemsetAsync(base, 0xff, pl.bytes, st));
+    const int64_t total = (int64_t)c.chains * c.tiles, most = (int64_t)ctas * device_sm_count();
+    kernel<<<(unsigned)std::min(total, most), threads, smem, st>>>(p, c);
+    return launch_status(what);
 }
 
+template <typename T, int VEC>
+int launch_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
+    Plan pl;
+    MB_CHECK_ARG(plan_chains(a, false, VEC, pl), "gated_recurrence: too many tiles");
+    return launch_tiles<VEC>(recurrence_fwd_kernel<T, VEC, kFwdS, kFwdW, kFwdCtas>, fwd_params(a), pl, 32 * kFwdW,
+                             kFwdCtas, sizeof(FwdSmem<T, VEC, kFwdS, kFwdW>), ws, st, "gated_recurrence kernel");
+}
 template <typename T>
-int launch_backward(const MambaRecurrenceArgs *a, const BwdParams &p, const MambaRecurrenceGrads *g, void *ws,
+int choose_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
+    constexpr int V = fwd_vec(sizeof(T) == 2 ? MAMBA_F16 : MAMBA_F32);
+    const bool vec = a->dim % V == 0 && vector_rows<T, V>(a->x, a->x_stride) && vector_rows<T, V>(a->r, a->r_stride) &&
+                     vector_rows<T, V>(a->i, a->i_stride) && vector_rows<T, V>(a->h, a->h_stride);
+    return vec ? launch_forward<T, V>(a, ws, st) : launch_forward<T, 1>(a, ws, st);
+}
+
+template <typename T, int VEC>
+int launch_backward(const MambaRecurrenceArgs *a, BwdParams &p, void *ws, cudaStream_t st, int &tiles) {
+    Plan pl;
+    MB_CHECK_ARG(plan_chains(a, true, VEC, pl), "gated_recurrence_backward: too many tiles");
+    tiles = pl.ch.tiles;
+    return launch_tiles<VEC>(recurrence_bwd_kernel<T, VEC, kBwdS, kBwdW, kBwdCtas>, p, pl, 32 * kBwdW, kBwdCtas,
+                             sizeof(BwdSmem<T, VEC, kBwdS, kBwdW>), ws, st, "gated_recurrence_backward kernel");
+}
+template <typename T>
+int choose_backward(const MambaRecurrenceArgs *a, BwdParams &p, const MambaRecurrenceGrads *g, void *ws,
                     cudaStream_t st) {
-    constexpr int V = kBwdVec;
+    constexpr int V = bwd_vec(sizeof(T) == 2 ? MAMBA_F16 : MAMBA_F32);
     const bool vec = a->dim % V == 0 && vector_rows<T, V>(a->x, a->x_stride) && vector_rows<T, V>(a->r, a->r_stride) &&
                      vector_rows<T, V>(a->i, a->i_stride) && vector_rows<T, V>(a->h, a->h_stride) &&
                      vector_rows<T, V>(g->dh, g->dh_stride) && vector_rows<T, V>(g->dx, g->dx_stride) &&
                      vector_rows<T, V>(g->dr, g->dr_stride) && vector_rows<T, V>(g->di, g->di_stride);
-    Plan pl;
-    MB_CHECK_ARG(plan_chains(a, true, vec ? V : 1, pl), "gated_recurrence_backward: too many tiles");
-    place_chains(pl, ws);
-    Chains &c = pl.ch;
-    c.states = reinterpret_cast<float *>(c.maps + (int64_t)c.chains * c.tiles * 32 * (vec ? V : 1));
-    if (pl.bytes) MB_CUDA_TRY(cudaMemsetAsync(c.ticket, 0xff, pl.bytes, st));
-    const unsigned grid = (unsigned)(c.chains * c.tiles);
-    if (vec)
-        recurrence_bwd_kernel<T, V, 8, 4><<<grid, 128, 0, st>>>(p, c);
-    else
-        recurrence_bwd_kernel<T, 1, 8, 4><<<grid, 128, 0, st>>>(p, c);
-    if (launch_status("gated_recurrence_backward kernel")) return -1;
+    int tiles = 0;
+    if (vec ? launch_backward<T, V>(a, p, ws, st, tiles) : launch_backward<T, 1>(a, p, ws, st, tiles)) return -1;
     recurrence_dlambda_kernel<<<(unsigned)ceil_div(a->dim, 32), 32 * kSumWarps, 0, st>>>(
-        p.part, a->lambda, g->dlambda, (int64_t)a->batch * c.tiles, a->dim);
+        p.part, a->lambda, g->dlambda, (int64_t)a->batch * tiles, a->dim);
     return launch_status("gated_recurrence_backward sum kernel");
 }
 
@@ -784,9 +866,10 @@ int recurrence_forward(const MambaRecurrenceArgs *a, void *ws, size_t ws_bytes, 
     if (check_args(a, false)) return -1;
     if (a->batch == 0 || a->dim == 0) return 0;
     const size_t need = recurrence_workspace_bytes(a, false);
-    MB_CHECK_ARG(need == 0 || (ws && ws_bytes >= need && aligned_to(ws, 16)),
+    MB_CHECK_ARG(need, "gated_recurrence: too many tiles");
+    MB_CHECK_ARG(ws && ws_bytes >= need && aligned_to(ws, 16),
                  "gated_recurrence: workspace too small or not 16-byte aligned");
-    return a->dtype == MAMBA_F16 ? launch_forward<__half>(a, ws, st) : launch_forward<float>(a, ws, st);
+    return a->dtype == MAMBA_F16 ? choose_forward<__half>(a, ws, st) : choose_forward<float>(a, ws, st);
 }
 
 int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads *g, void *ws, size_t ws_bytes,
@@ -809,7 +892,8 @@ int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads
                      output_rows_disjoint(g->di_stride, a->batch, a->seqlen, a->dim),
                  "gated_recurrence_backward: rows of a gradient overlap (strides)");
     const size_t need = recurrence_workspace_bytes(a, true);
-    MB_CHECK_ARG(ws && need && ws_bytes >= need && aligned_to(ws, 16),
+    MB_CHECK_ARG(need, "gated_recurrence_backward: too many tiles");
+    MB_CHECK_ARG(ws && ws_bytes >= need && aligned_to(ws, 16),
                  "gated_recurrence_backward: workspace too small or not 16-byte aligned");
     BwdParams p{};
     p.f = fwd_params(a);
@@ -826,7 +910,7 @@ int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads
         p.sdr[k] = g->dr_stride[k];
         p.sdi[k] = g->di_stride[k];
     }
-    return a->dtype == MAMBA_F16 ? launch_backward<__half>(a, p, g, ws, st) : launch_backward<float>(a, p, g, ws, st);
+    return a->dtype == MAMBA_F16 ? choose_backward<__half>(a, p, g, ws, st) : choose_backward<float>(a, p, g, ws, st);
 }
 
 unsigned recurrence_error_flags(bool clear) {
