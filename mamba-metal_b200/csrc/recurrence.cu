@@ -14,7 +14,6 @@
 #include "common.cuh"
 #include "internal.h"
 #include "scan_math.cuh"
-
 #include "tma.cuh"
 
 #include <algorithm>
@@ -25,68 +24,109 @@ __device__ unsigned int g_recurrence_error = 0;
 
 namespace {
 
-// Gates of one element.  FP16 tensors: single-instruction exponentials and
-// reciprocals (relative error ~2^-22, far below FP16's 2^-11 rounding).
-// FP32 tensors: the CUDA math library's FP32 functions.
-template <bool PRECISE>
-__device__ __forceinline__ float exp_neg(float v) {  // exp(-v)
-    return PRECISE ? expf(-v) : ex2_approx(-v * kLog2e);
-}
-
-// sigmoid(v) and 1 - sigmoid(v), each without cancellation.
-template <bool PRECISE>
-__device__ __forceinline__ void sigmoid2(float v, float &s, float &om) {
-    const float e = exp_neg<PRECISE>(fabsf(v));
-    const float t = PRECISE ? __fdiv_rn(1.f, 1.f + e) : rcp_approx(1.f + e);
-    const float u = e * t;
-    s = v >= 0.f ? t : u;
-    om = v >= 0.f ? u : t;
-}
-
-// 1 - a^2 = -expm1(-2y) for a = exp(-y).  FP16 tensors: below y = 0.03 the
-// series 2y - 2y^2 + 4/3 y^3 (relative error < y^3/3 = 9e-6), above it
-// fma(-a, a, 1), whose absolute error of ~4e-7 is then below 7e-6 of it.
-template <bool PRECISE>
-__device__ __forceinline__ float one_minus_a2(float y, float a) {
-    if (PRECISE) return -expm1f(-2.f * y);
-    const float series = 2.f * y * fmaf(y, fmaf(y, 2.f / 3.f, -1.f), 1.f);
-    return y < 0.03f ? series : fmaf(-a, a, 1.f);
-}
-
-template <bool PRECISE>
-__device__ __forceinline__ float sqrt_gate(float m) {
-    if (PRECISE) return sqrtf(m);
+// ---- gates ------------------------------------------------------------------
+// Two elements at a time in packed FP32 (one issue slot per pair and
+// operation); what is left per element are the special-function operations,
+// five forward and six backward.  Approximate exponentials, reciprocals and
+// roots have relative errors of 2^-22 or less.  PRECISE (FP32 tensors) adds
+// what their rounding needs: the exponent's product with log2(e) in two parts
+// and a longer series; for FP16 tensors the rounding to 2^-11 hides both.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN operand stays one
     float r;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(m));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float rsqrt_approx(float v) {
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
 
-// softplus(lambda): per channel, so the accurate form for both types.
-__device__ __forceinline__ float softplus_channel(float l) { return fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))); }
-
-// beta = sqrt(m) and q = y / beta; q -> sqrt(y / 2) -> 0 as the gate closes.
+// exp(-v), v above -120 and, PRECISE, below 1e30.
 template <bool PRECISE>
-__device__ __forceinline__ void root_gate(float m, float y, float &beta, float &q) {
-    if (PRECISE) {
-        beta = sqrtf(m);
-        q = beta <= 1e-18f ? 0.f : __fdiv_rn(y, beta);
-    } else {
-        const float r = rsqrtf(m);
-        beta = m <= 1e-36f ? 0.f : m * r;  // a NaN stays one
-        q = m <= 1e-36f ? 0.f : y * r;
+__device__ __forceinline__ float2 exp_neg(float2 v) {
+    const float2 t = __fmul2_rn(v, both(kLog2e));
+    float2 e = make_float2(ex2_approx(-t.x), ex2_approx(-t.y));
+    if (PRECISE) {  // 2^-(v log2 e) = 2^-t (1 + ln 2 d), d = t - v log2 e with log2 e in two parts
+        float2 d = __ffma2_rn(v, both(-kLog2e), t);
+        d = __ffma2_rn(v, both(-1.92596303e-8f), d);
+        e = __ffma2_rn(e, __fmul2_rn(d, both(kLn2)), e);
     }
+    return e;
 }
 
-struct Decay {
-    float s, om, y, a;
-};
+// A gate's preactivation, held where exp(-v) and its products stay finite:
+// sigmoid(-80) = 2e-35 and sigmoid(150) = 1 stand for what lies beyond.
 template <bool PRECISE>
-__device__ __forceinline__ Decay decay(float r, float csp) {
-    Decay d;
-    sigmoid2<PRECISE>(r, d.s, d.om);
-    d.y = csp * d.s;
-    d.a = exp_neg<PRECISE>(d.y);
-    return d;
+__device__ __forceinline__ float2 clamp_gate(float2 v) {
+    v = make_float2(max_nan(v.x, -80.f), max_nan(v.y, -80.f));
+    if (PRECISE) v = make_float2(min_nan(v.x, 150.f), min_nan(v.y, 150.f));
+    return v;
+}
+
+// 1 - a^2 for a = exp(-y), without cancellation for y near 0: a series in
+// z = 2y below a border, (1 - a)(1 + a) above it, where a's error of 2^-22
+// has lost its weight.  PRECISE: Taylor to z^7 below y = 1/4 (relative
+// error < (1/2)^8 / 9! = 1e-8; above, 2^-22 / (1 - e^-1/2) * e^-1/2).  Else to
+// z^2 below y = 0.03 (error < y^3 / 3 = 9e-6; above, 7e-6).
+template <bool PRECISE>
+__device__ __forceinline__ float2 one_minus_a2(float2 y, float2 a) {
+    const float2 z = __fadd2_rn(y, y);
+    float2 q;
+    if (PRECISE) {
+        q = __ffma2_rn(z, both(-1.f / 40320), both(1.f / 5040));
+        q = __ffma2_rn(z, q, both(-1.f / 720));
+        q = __ffma2_rn(z, q, both(1.f / 120));
+        q = __ffma2_rn(z, q, both(-1.f / 24));
+        q = __ffma2_rn(z, q, both(1.f / 6));
+    } else {
+        q = both(1.f / 6);
+    }
+    q = __ffma2_rn(z, q, both(-0.5f));
+    q = __ffma2_rn(z, q, both(1.f));
+    q = __fmul2_rn(z, q);
+    const float2 d = __ffma2_rn(a, both(-1.f), both(1.f)), w = __ffma2_rn(a, d, d);
+    constexpr float border = PRECISE ? 0.25f : 0.03f;
+    return make_float2(y.x < border ? q.x : w.x, y.y < border ? q.y : w.y);
+}
+
+// 1 / sqrt(m), finite for m = 0 (m * the result is then 0, as it should be).
+__device__ __forceinline__ float2 rsqrt_pos(float2 m) {
+    return make_float2(rsqrt_approx(max_nan(m.x, 1e-37f)), rsqrt_approx(max_nan(m.y, 1e-37f)));
+}
+
+// sigmoid(r) and the decay y = csp sigmoid(r), a = exp(-y).
+template <bool PRECISE>
+__device__ __forceinline__ void decay(float2 r, float2 csp, float2 &e, float2 &s, float2 &y, float2 &a) {
+    e = exp_neg<PRECISE>(clamp_gate<PRECISE>(r));
+    const float2 q = __fadd2_rn(e, both(1.f));
+    s = make_float2(rcp_approx(q.x), rcp_approx(q.y));
+    y = __fmul2_rn(csp, s);
+    a = exp_neg<PRECISE>(y);
+}
+
+// Forward: a and b = sqrt(1 - a^2) sigmoid(i) x.  With q = 1 + exp(-i) and
+// m = 1 - a^2, sqrt(m) / q = m / sqrt(m q^2): one root for both.
+template <bool PRECISE>
+__device__ __forceinline__ void forward_gates(float2 r, float2 i, float2 x, float2 csp, float2 &a, float2 &b) {
+    float2 e, s, y;
+    decay<PRECISE>(r, csp, e, s, y, a);
+    const float2 m = one_minus_a2<PRECISE>(y, a);
+    const float2 q = __fadd2_rn(exp_neg<PRECISE>(clamp_gate<PRECISE>(i)), both(1.f));
+    const float2 w = rsqrt_pos(__fmul2_rn(__fmul2_rn(m, q), q));
+    b = __fmul2_rn(__fmul2_rn(m, w), x);
+}
+
+// softplus(lambda): per channel.
+template <bool PRECISE>
+__device__ __forceinline__ float channel_softplus(float l) {
+    return PRECISE ? fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))) : softplus_fast(l);
 }
 
 struct FwdParams {
@@ -177,8 +217,58 @@ struct Waiting {
     }
 };
 
+// VEC consecutive elements.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+    T v[VEC];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T *p) {
+    return *reinterpret_cast<const Pack<T, VEC> *>(p);
+}
+
+// Affine maps h -> P h + H of a thread's channels.
 template <int VEC>
-__device__ __forceinline__ void wait_maps(const float2 *slot, float2 (&m)[VEC]) {
+struct Maps {
+    Pack<float, VEC> P, H;
+    __device__ __forceinline__ void identity() {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            P.v[e] = 1.f;
+            H.v[e] = 0.f;
+        }
+    }
+    // then q, later in time
+    __device__ __forceinline__ void then(const Pack<float, VEC> &qP, const Pack<float, VEC> &qH) {
+        if constexpr (VEC == 1) {
+            H.v[0] = fmaf(qP.v[0], H.v[0], qH.v[0]);
+            P.v[0] *= qP.v[0];
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 2) {
+                const float2 p = make_float2(qP.v[e], qP.v[e + 1]);
+                const float2 h = __ffma2_rn(p, make_float2(H.v[e], H.v[e + 1]), make_float2(qH.v[e], qH.v[e + 1]));
+                const float2 n = __fmul2_rn(p, make_float2(P.v[e], P.v[e + 1]));
+                H.v[e] = h.x;
+                H.v[e + 1] = h.y;
+                P.v[e] = n.x;
+                P.v[e + 1] = n.y;
+            }
+        }
+    }
+    __device__ __forceinline__ void apply(const float (&s)[VEC], float (&h)[VEC]) const {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[e] = fmaf(P.v[e], s[e], H.v[e]);
+    }
+};
+// A CTA's maps in shared memory, by warp or by tile of the group.
+template <int VEC, int N>
+struct MapRows {
+    Pack<float, VEC> P[N][32], H[N][32];
+};
+
+template <int VEC>
+__device__ __forceinline__ void wait_maps(const float2 *slot, Pack<float, VEC> &P, Pack<float, VEC> &H) {
     Waiting wt;
     bool ready;
     do {
@@ -189,7 +279,8 @@ __device__ __forceinline__ void wait_maps(const float2 *slot, float2 (&m)[VEC]) 
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
             ready &= (uint32_t)w[k] != kEmpty;
-            m[k] = make_float2(__uint_as_float((uint32_t)w[k]), __uint_as_float((uint32_t)(w[k] >> 32)));
+            P.v[k] = __uint_as_float((uint32_t)w[k]);
+            H.v[k] = __uint_as_float((uint32_t)(w[k] >> 32));
         }
     } while (!ready && wt.again());
 }
@@ -210,13 +301,27 @@ __device__ __forceinline__ void wait_states(const float *slot, float (&h)[VEC]) 
     } while (!ready && wt.again());
 }
 
+// v / d by a product with floor(2^32 / d): at most one below the quotient.
+struct Divisor {
+    unsigned d, m;
+    __device__ __forceinline__ unsigned divide(unsigned v, unsigned &rest) const {
+        unsigned q = __umulhi(v, m);
+        rest = v - q * d;
+        if (rest >= d) {
+            ++q;
+            rest -= d;
+        }
+        return q;
+    }
+};
+
 struct Chains {
     unsigned int *ticket;
     float2 *maps;    // [chains, tiles, channels of a tile]
     float *states;   // [chains, groups, channels of a tile]
-    int blocks;      // channel blocks of a row
-    int chains;      // rows * blocks
-    int tiles;
+    Divisor blocks;  // channel blocks of a row
+    Divisor chains;  // rows * blocks
+    int tiles, groups;
 };
 
 // Hands out tickets one ahead: next() gives the ticket drawn by the call
@@ -238,86 +343,77 @@ struct Tickets {
     }
 };
 
+// What a ticket stands for: time-major, all chains' k-th tiles together.
+struct Tile {
+    int chain, k, b, d, n, t0, cnt;
+    bool live, in;
+};
+template <int VEC>
+__device__ __forceinline__ Tile place_tile(const Chains &c, const FwdParams &p, unsigned v) {
+    Tile t;
+    unsigned chain, block;
+    t.k = (int)c.chains.divide(v, chain);
+    t.chain = (int)chain;
+    t.b = (int)c.blocks.divide(chain, block);
+    t.d = ((int)block * 32 + (threadIdx.x & 31)) * VEC;
+    t.in = t.d < p.D;
+    t.n = row_length(p, t.b);
+    return t;
+}
+
 // The map from the state at the start of tile k's group to the state entering
-// this warp's tokens (m), for the last warp also to the state leaving the
-// tile (end).  Warps wait for the maps of the group's earlier tiles between
-// them; `wm` holds the maps of this tile's warps.  Syncs the CTA.
+// this warp's tokens.  Warps wait for the maps of the group's earlier tiles
+// between them; `wm` holds the maps of this tile's warps.  Syncs the CTA.
 template <int VEC, int W>
-__device__ __forceinline__ void prefix_maps(const Chains &c, int chain, int k, const float2 (*wm)[VEC * 32],
-                                            float2 (*gm)[VEC * 32], float2 (&m)[VEC], float2 (&end)[VEC]) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cw = VEC * 32;
-    const int g = k / kGroup, j = k % kGroup;
+__device__ __forceinline__ Maps<VEC> prefix_maps(const Chains &c, const Tile &t, const MapRows<VEC, W> &wm,
+                                                 MapRows<VEC, kGroup - 1> &gm) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int j = t.k % kGroup;
 #pragma unroll
     for (int q = 0; q < (kGroup - 1 + W - 1) / W; ++q) {
         const int tile = warp + q * W;
         if (tile < j) {
-            float2 t[VEC];
-            wait_maps<VEC>(c.maps + ((int64_t)chain * c.tiles + g * kGroup + tile) * cw + lane * VEC, t);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) gm[tile][e * 32 + lane] = t[e];
+            Pack<float, VEC> P, H;
+            wait_maps<VEC>(c.maps + ((int64_t)t.chain * c.tiles + t.k - j + tile) * (32 * VEC) + lane * VEC, P, H);
+            gm.P[tile][lane] = P;
+            gm.H[tile][lane] = H;
         }
     }
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) m[e] = make_float2(1.f, 0.f);
-    auto then = [&](float2 &f, const float2 &q) {
-        f.y = fmaf(q.x, f.y, q.y);
-        f.x *= q.x;
-    };
-    for (int t = 0; t < j; ++t)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) then(m[e], gm[t][e * 32 + lane]);
-    for (int w = 0; w < warp; ++w)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) then(m[e], wm[w][e * 32 + lane]);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        end[e] = m[e];
-        then(end[e], wm[warp][e * 32 + lane]);
-    }
+    Maps<VEC> m;
+    m.identity();
+    for (int q = 0; q < j; ++q) m.then(gm.P[q][lane], gm.H[q][lane]);
+    for (int w = 0; w < warp; ++w) m.then(wm.P[w][lane], wm.H[w][lane]);
+    return m;
 }
 
-// The state at the start of tile k's group: `first`, or what the group before
-// left.  Every warp waits for itself, so that the group's last warp can pass
-// the state on without another barrier.
+// The state at the start of tile k's group, where a group went before it.
+// Every warp waits for itself, so that the group's last warp can pass the
+// state on without another barrier.
 template <int VEC>
-__device__ __forceinline__ void group_state(const Chains &c, int chain, int k, float (&s)[VEC]) {
-    const int lane = threadIdx.x & 31, g = k / kGroup, groups = (c.tiles + kGroup - 1) / kGroup;
-    if (g > 0) wait_states<VEC>(c.states + ((int64_t)chain * groups + g - 1) * (VEC * 32) + lane * VEC, s);
+__device__ __forceinline__ void group_state(const Chains &c, const Tile &t, float (&s)[VEC]) {
+    const int g = t.k / kGroup;
+    if (g > 0)
+        wait_states<VEC>(c.states + ((int64_t)t.chain * c.groups + g - 1) * (32 * VEC) + (threadIdx.x & 31) * VEC, s);
 }
 template <int VEC>
-__device__ __forceinline__ void leave_group(const Chains &c, int chain, int k, const float (&h)[VEC]) {
-    const int lane = threadIdx.x & 31, groups = (c.tiles + kGroup - 1) / kGroup;
+__device__ __forceinline__ void leave_group(const Chains &c, const Tile &t, const float (&h)[VEC]) {
+    float *slot = c.states + ((int64_t)t.chain * c.groups + t.k / kGroup) * (32 * VEC) + (threadIdx.x & 31) * VEC;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-        put_state(c.states + ((int64_t)chain * groups + k / kGroup) * (VEC * 32) + lane * VEC + e, h[e]);
+    for (int e = 0; e < VEC; ++e) put_state(slot + e, h[e]);
 }
 
 // The tile's own map (warp maps in order), published for the group's later tiles.
 template <int VEC, int W>
-__device__ __forceinline__ void publish_map(const Chains &c, int chain, int k, const float2 (*wm)[VEC * 32]) {
+__device__ __forceinline__ void publish_map(const Chains &c, const Tile &t, const MapRows<VEC, W> &wm) {
     const int lane = threadIdx.x & 31;
+    Maps<VEC> m;
+    m.identity();
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        float2 m = make_float2(1.f, 0.f);
+    for (int w = 0; w < W; ++w) m.then(wm.P[w][lane], wm.H[w][lane]);
+    float2 *slot = c.maps + ((int64_t)t.chain * c.tiles + t.k) * (32 * VEC) + lane * VEC;
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float2 q = wm[w][e * 32 + lane];
-            m.y = fmaf(q.x, m.y, q.y);
-            m.x *= q.x;
-        }
-        put_map(c.maps + ((int64_t)chain * c.tiles + k) * (VEC * 32) + lane * VEC + e, m.x, m.y);
-    }
-}
-
-// VEC consecutive elements, as loaded and as FP32.
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
-    T v[VEC];
-};
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> load_pack(const T *p) {
-    return *reinterpret_cast<const Pack<T, VEC> *>(p);
+    for (int e = 0; e < VEC; ++e) put_map(slot + e, m.P.v[e], m.H.v[e]);
 }
 
 // Which of this warp's tokens cut the state.
@@ -345,134 +441,139 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <bool PRECISE>
-__device__ __forceinline__ float channel_softplus(float l) {
-    return PRECISE ? softplus_channel(l) : softplus_fast(l);
+// A thread's S x VEC elements in pairs: along the channels, or along time
+// where it has one channel.  Element (token j, channel e) is number j * VEC + e.
+template <typename T, int VEC, int S>
+__device__ __forceinline__ float2 pair_of(const Pack<T, VEC> (&in)[S], int q) {
+    const int k = 2 * q;
+    return make_float2(cvt_f32(in[k / VEC].v[k % VEC]), cvt_f32(in[(k + 1) / VEC].v[(k + 1) % VEC]));
 }
-
-// Which tile a ticket stands for: time-major, all chains' k-th tiles together.
-struct Tile {
-    int chain, k, b, d, n, t0, cnt;
-    bool live, in;
-};
+template <int VEC>
+__device__ __forceinline__ float2 channel_pair(const float (&v)[VEC], int q) {
+    return make_float2(v[(2 * q) % VEC], v[(2 * q + 1) % VEC]);
+}
+__device__ __forceinline__ float &half_of(float2 &v, int k) { return k & 1 ? v.y : v.x; }
 
 // ---- forward --------------------------------------------------------------------
-// Persistent CTAs: the copies of the next tile's x, r and i into shared memory
-// run while the current tile is computed and waits for its state.  A thread
-// reads back only what it copied itself, so no barrier guards the buffers.
+// Persistent CTAs: once a tile's gates are computed, the copies of the next
+// tile's x, r and i into shared memory start, and run while this tile waits
+// for its state and writes h.  A thread reads back only what it copied
+// itself, so no barrier guards the buffer.
 template <typename T, int VEC, int S, int W>
 struct FwdSmem {
-    Pack<T, VEC> in[2][3][S][32 * W];
-    float2 wm[W][32 * VEC], gm[kGroup][32 * VEC];
+    Pack<T, VEC> in[3][S][32 * W];
+    MapRows<VEC, W> wm;
+    MapRows<VEC, kGroup - 1> gm;
     unsigned int ticket[2];
 };
 
 template <typename T, int VEC, int S, int W, int CTAS>
 __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdParams p, const Chains ch) {
     constexpr bool PRECISE = sizeof(T) == 4;
-    constexpr int cw = 32 * VEC, TT = S * W;
+    constexpr int TT = S * W, NP = S * VEC / 2;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     auto &sm = *reinterpret_cast<FwdSmem<T, VEC, S, W> *>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const unsigned total = (unsigned)ch.chains * (unsigned)ch.tiles;
+    const unsigned total = ch.chains.d * (unsigned)ch.tiles;
 
     auto place = [&](unsigned v) {
-        Tile t;
-        t.k = (int)(v / (unsigned)ch.chains);
-        t.chain = (int)(v - (unsigned)t.k * (unsigned)ch.chains);
-        t.b = t.chain / ch.blocks;
-        t.d = (t.chain - t.b * ch.blocks) * cw + lane * VEC;
-        t.n = row_length(p, t.b);
+        Tile t = place_tile<VEC>(ch, p, v);
         t.t0 = t.k * TT + warp * S;
         t.live = t.k == 0 || t.k * TT < t.n;  // else behind the row's end
-        t.in = t.d < p.D;
         t.cnt = t.in ? min(max(t.n - t.t0, 0), S) : 0;
         return t;
     };
-    auto fetch = [&](const Tile &t, int buf) {
+    auto fetch = [&](const Tile &t) {
         const T *px = static_cast<const T *>(p.x) + t.b * p.sx[0] + t.t0 * p.sx[1] + t.d;
         const T *pr = static_cast<const T *>(p.r) + t.b * p.sr[0] + t.t0 * p.sr[1] + t.d;
         const T *pi = static_cast<const T *>(p.i) + t.b * p.si[0] + t.t0 * p.si[1] + t.d;
 #pragma unroll
         for (int j = 0; j < S; ++j)
             if (j < t.cnt) {
-                copy_pack<T, VEC>(&sm.in[buf][0][j][tid], pr + j * p.sr[1]);
-                copy_pack<T, VEC>(&sm.in[buf][1][j][tid], pi + j * p.si[1]);
-                copy_pack<T, VEC>(&sm.in[buf][2][j][tid], px + j * p.sx[1]);
+                copy_pack<T, VEC>(&sm.in[0][j][tid], pr + j * p.sr[1]);
+                copy_pack<T, VEC>(&sm.in[1][j][tid], pi + j * p.si[1]);
+                copy_pack<T, VEC>(&sm.in[2][j][tid], px + j * p.sx[1]);
             }
+        copy_commit();
     };
 
     Tickets tickets(ch.ticket, sm.ticket);
     unsigned v = tickets.next();
     if (v >= total) return;
     Tile t = place(v);
-    fetch(t, 0);
-    copy_commit();
-    for (int buf = 0;; buf ^= 1) {
+    fetch(t);
+    for (;;) {
         const unsigned vn = tickets.next();  // its barrier also frees sm.wm and sm.gm
         Tile tn{};
-        if (vn < total) {
-            tn = place(vn);
-            fetch(tn, buf ^ 1);
-        }
-        copy_commit();
-        copy_wait<1>();
+        if (vn < total) tn = place(vn);
+        copy_wait<0>();
+        float2 a[NP], b[NP];
         if (t.live) {
-            float a[S][VEC], bt[S][VEC], csp[VEC];
+            float csp[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) csp[e] = t.in ? p.c * channel_softplus<PRECISE>(p.lambda[t.d + e]) : 0.f;
+            Pack<T, VEC> r[S], gi[S], x[S];
 #pragma unroll
             for (int j = 0; j < S; ++j) {
-                const Pack<T, VEC> r = sm.in[buf][0][j][tid], gi = sm.in[buf][1][j][tid], x = sm.in[buf][2][j][tid];
+                r[j] = sm.in[0][j][tid];
+                gi[j] = sm.in[1][j][tid];
+                x[j] = sm.in[2][j][tid];
+            }
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const Decay g = decay<PRECISE>(cvt_f32(r.v[e]), csp[e]);
-                    float si, om;
-                    sigmoid2<PRECISE>(cvt_f32(gi.v[e]), si, om);
-                    const float bv = sqrt_gate<PRECISE>(one_minus_a2<PRECISE>(g.y, g.a)) * si * cvt_f32(x.v[e]);
-                    a[j][e] = j < t.cnt ? g.a : 1.f;  // what the buffer holds behind the end does not count
-                    bt[j][e] = j < t.cnt ? bv : 0.f;
-                }
+            for (int q = 0; q < NP; ++q)
+                forward_gates<PRECISE>(pair_of<T, VEC, S>(r, q), pair_of<T, VEC, S>(gi, q), pair_of<T, VEC, S>(x, q),
+                                       channel_pair<VEC>(csp, q), a[q], b[q]);
+        }
+        if (vn < total) fetch(tn);
+        if (t.live) {
+            if (t.cnt < S) {  // what the buffer holds behind the end does not count
+#pragma unroll
+                for (int k = 0; k < S * VEC; ++k)
+                    if (k / VEC >= t.cnt) {
+                        half_of(a[k / 2], k) = 1.f;
+                        half_of(b[k / 2], k) = 0.f;
+                    }
             }
             const uint32_t cut = cut_mask(p, t.b, t.t0, min(max(t.n - t.t0, 0), S));
             if (cut)
 #pragma unroll
-                for (int j = 0; j < S; ++j)
-                    if (cut >> j & 1)
+                for (int k = 0; k < S * VEC; ++k)
+                    if (cut >> (k / VEC) & 1) half_of(a[k / 2], k) = 0.f;
+            Maps<VEC> own;
+            own.identity();
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) a[j][e] = 0.f;
+            for (int j = 0; j < S; ++j) {
+                Pack<float, VEC> P, H;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                float P = 1.f, H = 0.f;
-#pragma unroll
-                for (int j = 0; j < S; ++j) {
-                    H = fmaf(a[j][e], H, bt[j][e]);
-                    P *= a[j][e];
+                for (int e = 0; e < VEC; ++e) {
+                    P.v[e] = half_of(a[(j * VEC + e) / 2], j * VEC + e);
+                    H.v[e] = half_of(b[(j * VEC + e) / 2], j * VEC + e);
                 }
-                sm.wm[warp][e * 32 + lane] = make_float2(P, H);
+                own.then(P, H);
             }
+            sm.wm.P[warp][lane] = own.P;
+            sm.wm.H[warp][lane] = own.H;
             __syncthreads();
             const bool more = (t.k + 1) * TT < t.n;  // a later tile waits for this one
             const bool last = t.k % kGroup == kGroup - 1;
-            if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t.chain, t.k, sm.wm);
-            float2 m[VEC], end[VEC];
-            prefix_maps<VEC, W>(ch, t.chain, t.k, sm.wm, sm.gm, m, end);
+            if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, sm.wm);
+            Maps<VEC> m = prefix_maps<VEC, W>(ch, t, sm.wm, sm.gm);
             float s[VEC], h[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
                 s[e] = t.in && p.h0 && t.k < kGroup ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
-            group_state<VEC>(ch, t.chain, t.k, s);
+            group_state<VEC>(ch, t, s);
             if (warp == W - 1 && (last || !more)) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) h[e] = fmaf(end[e].x, s[e], end[e].y);
+                Maps<VEC> end = m;
+                end.then(own.P, own.H);
+                end.apply(s, h);
                 if (more)
-                    leave_group<VEC>(ch, t.chain, t.k, h);
+                    leave_group<VEC>(ch, t, h);
                 else if (t.in && p.hN)
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) p.hN[(int64_t)t.b * p.D + t.d + e] = h[e];
             }
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) h[e] = fmaf(m[e].x, s[e], m[e].y);
+            m.apply(s, h);
             T *ph = static_cast<T *>(p.h) + t.b * p.sh[0] + t.t0 * p.sh[1] + t.d;
 #pragma unroll
             for (int j = 0; j < S; ++j)
@@ -480,7 +581,8 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
                     Pack<T, VEC> o;
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
-                        h[e] = fmaf(a[j][e], h[e], bt[j][e]);
+                        const int k = j * VEC + e;
+                        h[e] = fmaf(half_of(a[k / 2], k), h[e], half_of(b[k / 2], k));
                         o.v[e] = cvt_out<T>(h[e]);
                     }
                     *reinterpret_cast<Pack<T, VEC> *>(ph + j * p.sh[1]) = o;
@@ -493,36 +595,32 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
 
 // ---- backward -------------------------------------------------------------------
 // The same tiles and chains with time reversed; what runs along a chain is
-// C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.
+// C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.  x, i
+// and h are needed after the wait, so two buffers take turns.
 template <typename T, int VEC, int S, int W>
 struct BwdSmem {
     Pack<T, VEC> in[2][5][S][32 * W];
-    float2 wm[W][32 * VEC], gm[kGroup][32 * VEC];
-    float sums[W][32 * VEC];
+    MapRows<VEC, W> wm;
+    MapRows<VEC, kGroup - 1> gm;
+    Pack<float, VEC> sums[W][32];
     unsigned int ticket[2];
 };
 
 template <typename T, int VEC, int S, int W, int CTAS>
 __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdParams p, const Chains ch) {
     constexpr bool PRECISE = sizeof(T) == 4;
-    constexpr int cw = 32 * VEC, TT = S * W;
+    constexpr int TT = S * W, NP = S * VEC / 2;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     auto &sm = *reinterpret_cast<BwdSmem<T, VEC, S, W> *>(smem_raw);
     const FwdParams &f = p.f;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const unsigned total = (unsigned)ch.chains * (unsigned)ch.tiles;
+    const unsigned total = ch.chains.d * (unsigned)ch.tiles;
 
     auto place = [&](unsigned v) {
-        Tile t;
-        t.k = (int)(v / (unsigned)ch.chains);
-        t.chain = (int)(v - (unsigned)t.k * (unsigned)ch.chains);
-        t.b = t.chain / ch.blocks;
-        t.d = (t.chain - t.b * ch.blocks) * cw + lane * VEC;
-        t.n = row_length(f, t.b);
+        Tile t = place_tile<VEC>(ch, f, v);
         const int row_tiles = max((t.n + TT - 1) / TT, 1);
         t.live = t.k < row_tiles;
         t.t0 = (row_tiles - 1 - t.k) * TT + (W - 1 - warp) * S;  // warp 0 holds the tile's last tokens
-        t.in = t.d < f.D;
         t.cnt = t.in && t.live ? min(max(t.n - t.t0, 0), S) : 0;
         return t;
     };
@@ -550,7 +648,7 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
     fetch(t, 0);
     copy_commit();
     for (int buf = 0;; buf ^= 1) {
-        const unsigned vn = tickets.next();  // its barrier also frees sm.wm and sm.gm
+        const unsigned vn = tickets.next();  // its barrier also frees sm.wm, sm.gm and sm.sums
         Tile tn{};
         if (vn < total) {
             tn = place(vn);
@@ -560,97 +658,150 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
         copy_wait<1>();
         float *part = p.part + ((int64_t)t.b * ch.tiles + t.k) * f.D + t.d;
         if (t.live) {
-            float a[S][VEC], y[S][VEC], om[S][VEC], csp[VEC];
+            float2 a[NP], sg[NP], om[PRECISE ? NP : 1];
+            float csp[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) csp[e] = t.in ? f.c * channel_softplus<PRECISE>(f.lambda[t.d + e]) : 0.f;
-            const uint32_t cut = cut_mask(f, t.b, t.t0, min(max(t.n - t.t0, 0), S));
-            float2 own[VEC];
+            Pack<T, VEC> dh[S];
+            {
+                Pack<T, VEC> r[S];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) own[e] = make_float2(1.f, 0.f);
+                for (int j = 0; j < S; ++j) {
+                    r[j] = sm.in[buf][0][j][tid];
+                    dh[j] = sm.in[buf][1][j][tid];
+                }
 #pragma unroll
-            for (int j = S - 1; j >= 0; --j) {
-                const Pack<T, VEC> r = sm.in[buf][0][j][tid], dh = sm.in[buf][1][j][tid];
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const Decay g = decay<PRECISE>(cvt_f32(r.v[e]), csp[e]);
-                    a[j][e] = g.a;
-                    y[j][e] = g.y;
-                    om[j][e] = g.om;
-                    if (j < t.cnt) {  // what the buffer holds behind the end does not count
-                        const float ak = cut >> j & 1 ? 0.f : g.a;
-                        own[e].y = ak * (cvt_f32(dh.v[e]) + own[e].y);
-                        own[e].x *= ak;
-                    }
+                for (int q = 0; q < NP; ++q) {
+                    float2 e, y;
+                    decay<PRECISE>(pair_of<T, VEC, S>(r, q), channel_pair<VEC>(csp, q), e, sg[q], y, a[q]);
+                    if (PRECISE) om[q] = __fmul2_rn(e, sg[q]);
                 }
             }
+            const uint32_t cut = cut_mask(f, t.b, t.t0, min(max(t.n - t.t0, 0), S));
+            Maps<VEC> own;
+            own.identity();
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) sm.wm[warp][e * 32 + lane] = own[e];
+            for (int j = S - 1; j >= 0; --j)
+                if (j < t.cnt) {  // what the buffer holds behind the end does not count
+                    Pack<float, VEC> P, H;
+                    const float keep = cut >> j & 1 ? 0.f : 1.f;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const int k = j * VEC + e;
+                        P.v[e] = half_of(a[k / 2], k) * keep;
+                        H.v[e] = P.v[e] * cvt_f32(dh[j].v[e]);
+                    }
+                    own.then(P, H);
+                }
+            sm.wm.P[warp][lane] = own.P;
+            sm.wm.H[warp][lane] = own.H;
             __syncthreads();
             const bool more = t.t0 - (W - 1 - warp) * S > 0;  // an earlier tile waits for this one
             const bool last = t.k % kGroup == kGroup - 1;
-            if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t.chain, t.k, sm.wm);
-            float2 m[VEC], end[VEC];
-            prefix_maps<VEC, W>(ch, t.chain, t.k, sm.wm, sm.gm, m, end);
+            if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, sm.wm);
+            Maps<VEC> m = prefix_maps<VEC, W>(ch, t, sm.wm, sm.gm);
             float s[VEC], C[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
                 s[e] = t.in && p.dhN && t.k < kGroup ? p.dhN[(int64_t)t.b * f.D + t.d + e] : 0.f;
-            group_state<VEC>(ch, t.chain, t.k, s);
+            group_state<VEC>(ch, t, s);
             if (warp == W - 1 && (last || !more)) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) C[e] = fmaf(end[e].x, s[e], end[e].y);
+                Maps<VEC> end = m;
+                end.then(own.P, own.H);
+                end.apply(s, C);
                 if (more)
-                    leave_group<VEC>(ch, t.chain, t.k, C);
+                    leave_group<VEC>(ch, t, C);
                 else if (t.in && p.dh0)
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) p.dh0[(int64_t)t.b * f.D + t.d + e] = C[e];
             }
+            m.apply(s, C);
+
+            // G = dh + C of every element, then everything else in pairs
+            float2 G[NP];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) C[e] = fmaf(m[e].x, s[e], m[e].y);
+            for (int j = S - 1; j >= 0; --j) {
+                const float keep = cut >> j & 1 ? 0.f : 1.f;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const int k = j * VEC + e;
+                    const float g = cvt_f32(dh[j].v[e]) + C[e];
+                    half_of(G[k / 2], k) = g;
+                    if (j < t.cnt) C[e] = half_of(a[k / 2], k) * keep * g;
+                }
+            }
             T *qx = static_cast<T *>(p.dx) + t.b * p.sdx[0] + t.t0 * p.sdx[1] + t.d;
             T *qr = static_cast<T *>(p.dr) + t.b * p.sdr[0] + t.t0 * p.sdr[1] + t.d;
             T *qi = static_cast<T *>(p.di) + t.b * p.sdi[0] + t.t0 * p.sdi[1] + t.d;
             float sum[VEC] = {};
+            constexpr int TP = VEC == 1 ? 2 : 1;  // tokens whose pairs are computed together
 #pragma unroll
-            for (int j = S - 1; j >= 0; --j)
-                if (j < t.cnt) {
-                    const Pack<T, VEC> dh = sm.in[buf][1][j][tid], x = sm.in[buf][2][j][tid],
-                                       gi = sm.in[buf][3][j][tid], hp = sm.in[buf][4][j][tid];
-                    Pack<T, VEC> ox, orr, oi;
-                    const bool keep = !(cut >> j & 1);
+            for (int j0 = S - TP; j0 >= 0; j0 -= TP) {
+                if (j0 >= t.cnt) continue;
+                Pack<T, VEC> x[TP], gi[TP], hp[TP], ox[TP], orr[TP], oi[TP];
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float av = a[j][e], yv = y[j][e], xv = cvt_f32(x.v[e]);
-                        const float G = cvt_f32(dh.v[e]) + C[e];
-                        C[e] = (keep ? av : 0.f) * G;
-                        float si, omi, beta, q;
-                        sigmoid2<PRECISE>(cvt_f32(gi.v[e]), si, omi);
-                        root_gate<PRECISE>(one_minus_a2<PRECISE>(yv, av), yv, beta, q);
-                        float prev = cvt_f32(hp.v[e]);
-                        if (t.t0 + j == 0) prev = f.h0 ? f.h0[(int64_t)t.b * f.D + t.d + e] : 0.f;
-                        if (!keep) prev = 0.f;
-                        const float gx = G * beta * si;
-                        const float E = G * (si * xv * av * av * q - yv * av * prev);
-                        sum[e] += E;
-                        ox.v[e] = cvt_out<T>(gx);
-                        oi.v[e] = cvt_out<T>(gx * xv * omi);
-                        orr.v[e] = cvt_out<T>(E * om[j][e]);
-                    }
-                    *reinterpret_cast<Pack<T, VEC> *>(qx + j * p.sdx[1]) = ox;
-                    *reinterpret_cast<Pack<T, VEC> *>(qi + j * p.sdi[1]) = oi;
-                    *reinterpret_cast<Pack<T, VEC> *>(qr + j * p.sdr[1]) = orr;
+                for (int u = 0; u < TP; ++u) {
+                    x[u] = sm.in[buf][2][j0 + u][tid];
+                    gi[u] = sm.in[buf][3][j0 + u][tid];
+                    hp[u] = sm.in[buf][4][j0 + u][tid];
                 }
+#pragma unroll
+                for (int u = 0; u < TP; ++u) {
+                    if (t.t0 + j0 + u == 0 || (cut >> (j0 + u) & 1))  // the initial state, or none
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) hp[u].v[e] = cvt_out<T>(0.f);
+                }
+#pragma unroll
+                for (int z = 0; z < TP * VEC / 2; ++z) {
+                    const int q = j0 * VEC / 2 + z;
+                    const float2 xv = pair_of<T, VEC, TP>(x, z), av = a[q], y = __fmul2_rn(channel_pair<VEC>(csp, z), sg[q]);
+                    float2 prev = pair_of<T, VEC, TP>(hp, z);
+                    if (t.t0 + j0 == 0 && f.h0 && !(cut >> j0 & 1)) {  // h_{-1}, in FP32
+                        prev.x = f.h0[(int64_t)t.b * f.D + t.d + (2 * z) % VEC];
+                        if (VEC > 1) prev.y = f.h0[(int64_t)t.b * f.D + t.d + (2 * z + 1) % VEC];
+                    }
+                    const float2 ei = exp_neg<PRECISE>(clamp_gate<PRECISE>(pair_of<T, VEC, TP>(gi, z)));
+                    const float2 qi = __fadd2_rn(ei, both(1.f));
+                    const float2 si = make_float2(rcp_approx(qi.x), rcp_approx(qi.y));
+                    const float2 m2 = one_minus_a2<PRECISE>(y, av), w = rsqrt_pos(m2);
+                    const float2 gs2 = __fmul2_rn(G[q], si);                      // G sigmoid(i)
+                    const float2 gx = __fmul2_rn(gs2, __fmul2_rn(m2, w));         // * sqrt(m)
+                    const float2 gi2 = __fmul2_rn(__fmul2_rn(gx, xv), __fmul2_rn(ei, si));
+                    // E = a (G si x a (y / sqrt(m)) - y G h_{t-1}); y / sqrt(m) first, it tends to 0
+                    const float2 u1 = __fmul2_rn(__fmul2_rn(gs2, xv), __fmul2_rn(av, __fmul2_rn(y, w)));
+                    const float2 u2 = __ffma2_rn(__fmul2_rn(__fmul2_rn(y, both(-1.f)), G[q]), prev, u1);
+                    const float2 E = __fmul2_rn(av, u2);
+                    const float2 os = PRECISE ? om[PRECISE ? q : 0] : __ffma2_rn(sg[q], both(-1.f), both(1.f));
+                    const float2 gr = __fmul2_rn(E, os);
+#pragma unroll
+                    for (int hlf = 0; hlf < 2; ++hlf) {
+                        const int k = 2 * z + hlf, u = k / VEC, e = k % VEC;
+                        ox[u].v[e] = cvt_out<T>(hlf ? gx.y : gx.x);
+                        oi[u].v[e] = cvt_out<T>(hlf ? gi2.y : gi2.x);
+                        orr[u].v[e] = cvt_out<T>(hlf ? gr.y : gr.x);
+                        if (j0 + u < t.cnt) sum[e] += hlf ? E.y : E.x;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < TP; ++u)
+                    if (j0 + u < t.cnt) {
+                        const int j = j0 + u;
+                        *reinterpret_cast<Pack<T, VEC> *>(qx + j * p.sdx[1]) = ox[u];
+                        *reinterpret_cast<Pack<T, VEC> *>(qi + j * p.sdi[1]) = oi[u];
+                        *reinterpret_cast<Pack<T, VEC> *>(qr + j * p.sdr[1]) = orr[u];
+                    }
+            }
             // the tile's sum of E per channel, warps in order
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) sm.sums[warp][e * 32 + lane] = sum[e];
+            for (int e = 0; e < VEC; ++e) sm.sums[warp][lane].v[e] = sum[e];
             __syncthreads();
             if (warp == 0 && t.in)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    float v = 0.f;
+                    float z = 0.f;
 #pragma unroll
-                    for (int w = 0; w < W; ++w) v += sm.sums[w][e * 32 + lane];
-                    part[e] = v;
+                    for (int w = 0; w < W; ++w) z += sm.sums[w][lane].v[e];
+                    part[e] = z;
                 }
         } else if (warp == 0 && t.in) {  // behind the row's end
 #pragma unroll
@@ -678,29 +829,55 @@ __global__ void __launch_bounds__(32 * kSumWarps)
     if (warp == 0 && d < D) {
 #pragma unroll
         for (int w = 1; w < kSumWarps; ++w) s += sm[w][lane];
-        float sg, om;
         const float l = lambda[d];
-        sigmoid2<true>(l, sg, om);
-        dlambda[d] = s * (l < -20.f ? 1.f : sg / softplus_channel(l));
+        dlambda[d] = s * (l < -20.f ? 1.f : 1.f / (1.f + expf(-l)) / channel_softplus<true>(l));
     }
 }
 
+// ---- single token -----------------------------------------------------------------
+// A thread serves VEC channels of `rows` batch rows, so that its softplus of
+// lambda serves them all and several rows' loads are in flight.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    recurrence_step_kernel(const T *__restrict__ x, int64_t xrs, const T *__restrict__ r, int64_t rrs,
-                           const T *__restrict__ gi, int64_t irs, const float *__restrict__ lambda,
-                           const float *s_in, float *s_out, T *__restrict__ h, int64_t hrs, int D, float c) {
+struct StepParams {
+    const T *x, *r, *i;
+    T *h;
+    const float *lambda, *s_in;
+    float *s_out;
+    int64_t xrs, rrs, irs, hrs;
+    int B, D, rows;
+    float c;
+};
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) recurrence_step_kernel(const StepParams<T> p) {
     constexpr bool PRECISE = sizeof(T) == 4;
-    const int d = blockIdx.x * kThreads + threadIdx.x;
-    const int64_t b = blockIdx.y;
-    if (d >= D) return;
-    const Decay g = decay<PRECISE>(ld_f32(r + b * rrs + d), c * softplus_channel(lambda[d]));
-    float si, om;
-    sigmoid2<PRECISE>(ld_f32(gi + b * irs + d), si, om);
-    const float bt = sqrt_gate<PRECISE>(one_minus_a2<PRECISE>(g.y, g.a)) * si * ld_f32(x + b * xrs + d);
-    const float v = fmaf(g.a, s_in[b * D + d], bt);
-    s_out[b * D + d] = v;
-    h[b * hrs + d] = cvt_out<T>(v);
+    const int d = (blockIdx.x * kThreads + threadIdx.x) * VEC;
+    if (d >= p.D) return;
+    float csp[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) csp[e] = p.c * channel_softplus<PRECISE>(p.lambda[d + e]);
+    const int64_t b0 = (int64_t)blockIdx.y * p.rows, b1 = min(b0 + p.rows, (int64_t)p.B);
+#pragma unroll 4
+    for (int64_t b = b0; b < b1; ++b) {
+        const Pack<T, VEC> x[1] = {load_pack<T, VEC>(p.x + b * p.xrs + d)}, r[1] = {load_pack<T, VEC>(p.r + b * p.rrs + d)},
+                           gi[1] = {load_pack<T, VEC>(p.i + b * p.irs + d)};
+        Pack<float, VEC> s = load_pack<float, VEC>(p.s_in + b * p.D + d);
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) {
+            const int f = VEC == 1 ? 0 : e + 1;
+            float2 a, bt;
+            forward_gates<PRECISE>(make_float2(cvt_f32(r[0].v[e]), cvt_f32(r[0].v[f])),
+                                   make_float2(cvt_f32(gi[0].v[e]), cvt_f32(gi[0].v[f])),
+                                   make_float2(cvt_f32(x[0].v[e]), cvt_f32(x[0].v[f])), make_float2(csp[e], csp[f]), a,
+                                   bt);
+            s.v[e] = fmaf(a.x, s.v[e], bt.x);
+            if (VEC > 1) s.v[f] = fmaf(a.y, s.v[f], bt.y);
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o.v[e] = cvt_out<T>(s.v[e]);
+        *reinterpret_cast<Pack<float, VEC> *>(p.s_out + b * p.D + d) = s;
+        *reinterpret_cast<Pack<T, VEC> *>(p.h + b * p.hrs + d) = o;
+    }
 }
 
 bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -763,10 +940,14 @@ FwdParams fwd_params(const MambaRecurrenceArgs *a) {
 
 // Tile shapes: channels a thread holds (1 serves any alignment and channel
 // count), tokens a warp holds, warps and CTAs per SM.
-constexpr int kFwdS = 8, kFwdW = 4, kFwdCtas = 4;
-constexpr int kBwdS = 8, kBwdW = 4, kBwdCtas = 4;
-constexpr int fwd_vec(int dtype) { return dtype == MAMBA_F16 ? 4 : 2; }
-constexpr int bwd_vec(int dtype) { return dtype == MAMBA_F16 ? 2 : 1; }
+template <typename T>
+struct FwdShape {
+    static constexpr int VEC = sizeof(T) == 2 ? 4 : 2, S = 8, W = 4, CTAS = sizeof(T) == 2 ? 4 : 5;
+};
+template <typename T>
+struct BwdShape {
+    static constexpr int VEC = sizeof(T) == 2 ? 4 : 2, S = 4, W = 8, CTAS = 2;
+};
 
 // The chains of a call and where its workspace holds what.
 struct Plan {
@@ -774,15 +955,22 @@ struct Plan {
     size_t bytes, part_bytes;
 };
 bool plan_chains(const MambaRecurrenceArgs *a, bool backward, int vec, Plan &pl) {
-    const int tile = backward ? kBwdS * kBwdW : kFwdS * kFwdW, cw = 32 * vec;
+    const bool half = a->dtype == MAMBA_F16;
+    const int tile = backward ? (half ? BwdShape<__half>::S * BwdShape<__half>::W : BwdShape<float>::S * BwdShape<float>::W)
+                              : (half ? FwdShape<__half>::S * FwdShape<__half>::W : FwdShape<float>::S * FwdShape<float>::W);
+    const int cw = 32 * vec;
     Chains &c = pl.ch;
     c = Chains{};
     const int64_t blocks = ceil_div64(a->dim, cw), tiles = std::max<int64_t>(1, ceil_div64(a->seqlen, tile));
     if (blocks * a->batch * tiles > 0x7fffffffLL) return false;
-    c.blocks = (int)blocks;
-    c.chains = (int)blocks * a->batch;
+    auto divisor = [](int64_t d) {
+        return Divisor{(unsigned)d, d == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / (unsigned long long)d)};
+    };
+    c.blocks = divisor(blocks);
+    c.chains = divisor(blocks * a->batch);
     c.tiles = (int)tiles;
-    pl.bytes = 256 + (size_t)c.chains * cw * (tiles * sizeof(float2) + ceil_div64(tiles, kGroup) * sizeof(float));
+    c.groups = (int)ceil_div64(tiles, kGroup);
+    pl.bytes = 256 + (size_t)c.chains.d * cw * (tiles * sizeof(float2) + c.groups * sizeof(float));
     if (tiles == 1) pl.bytes = 256;
     pl.part_bytes = backward ? ((size_t)a->batch * tiles * a->dim * sizeof(float) + 15) / 16 * 16 : 0;
     return true;
@@ -790,12 +978,12 @@ bool plan_chains(const MambaRecurrenceArgs *a, bool backward, int vec, Plan &pl)
 
 }  // namespace
 
-// The largest of the variants that the alignment could choose, so that the
-// size does not depend on pointers.
+// The largest of what any channel width needs, so that the size does not
+// depend on pointers.
 size_t recurrence_workspace_bytes(const MambaRecurrenceArgs *a, bool backward) {
     if (!a || a->batch <= 0 || a->seqlen < 0 || a->dim <= 0) return 0;
     size_t need = 0;
-    for (int vec : {1, backward ? bwd_vec(a->dtype) : fwd_vec(a->dtype)}) {
+    for (int vec : {1, 2, 4}) {
         Plan pl;
         if (!plan_chains(a, backward, vec, pl)) return 0;
         need = std::max(need, pl.bytes + pl.part_bytes);
@@ -814,10 +1002,10 @@ int launch_tiles(Kernel kernel, const Params &p, Plan &pl, int threads, int ctas
     uint8_t *base = static_cast<uint8_t *>(ws) + pl.part_bytes;
     c.ticket = reinterpret_cast<unsigned int *>(base);
     c.maps = reinterpret_cast<float2 *>(base + 256);
-    c.states = reinterpret_cast<float *>(c.maps + (int64_t)c.chains * c.tiles * 32 * VEC);
+    c.states = reinterpret_cast<float *>(c.maps + (int64_t)c.chains.d * c.tiles * 32 * VEC);
     MB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     MB_CUDA_TRY(cudaMemsetAsync(base, 0xff, pl.bytes, st));
-    const int64_t total = (int64_t)c.chains * c.tiles, most = (int64_t)ctas * device_sm_count();
+    const int64_t total = (int64_t)c.chains.d * c.tiles, most = (int64_t)ctas * device_sm_count();
     kernel<<<(unsigned)std::min(total, most), threads, smem, st>>>(p, c);
     return launch_status(what);
 }
@@ -826,12 +1014,13 @@ template <typename T, int VEC>
 int launch_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
     Plan pl;
     MB_CHECK_ARG(plan_chains(a, false, VEC, pl), "gated_recurrence: too many tiles");
-    return launch_tiles<VEC>(recurrence_fwd_kernel<T, VEC, kFwdS, kFwdW, kFwdCtas>, fwd_params(a), pl, 32 * kFwdW,
-                             kFwdCtas, sizeof(FwdSmem<T, VEC, kFwdS, kFwdW>), ws, st, "gated_recurrence kernel");
+    using F = FwdShape<T>;
+    return launch_tiles<VEC>(recurrence_fwd_kernel<T, VEC, F::S, F::W, F::CTAS>, fwd_params(a), pl, 32 * F::W, F::CTAS,
+                             sizeof(FwdSmem<T, VEC, F::S, F::W>), ws, st, "gated_recurrence kernel");
 }
 template <typename T>
 int choose_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
-    constexpr int V = fwd_vec(sizeof(T) == 2 ? MAMBA_F16 : MAMBA_F32);
+    constexpr int V = FwdShape<T>::VEC;
     const bool vec = a->dim % V == 0 && vector_rows<T, V>(a->x, a->x_stride) && vector_rows<T, V>(a->r, a->r_stride) &&
                      vector_rows<T, V>(a->i, a->i_stride) && vector_rows<T, V>(a->h, a->h_stride);
     return vec ? launch_forward<T, V>(a, ws, st) : launch_forward<T, 1>(a, ws, st);
@@ -842,13 +1031,14 @@ int launch_backward(const MambaRecurrenceArgs *a, BwdParams &p, void *ws, cudaSt
     Plan pl;
     MB_CHECK_ARG(plan_chains(a, true, VEC, pl), "gated_recurrence_backward: too many tiles");
     tiles = pl.ch.tiles;
-    return launch_tiles<VEC>(recurrence_bwd_kernel<T, VEC, kBwdS, kBwdW, kBwdCtas>, p, pl, 32 * kBwdW, kBwdCtas,
-                             sizeof(BwdSmem<T, VEC, kBwdS, kBwdW>), ws, st, "gated_recurrence_backward kernel");
+    using F = BwdShape<T>;
+    return launch_tiles<VEC>(recurrence_bwd_kernel<T, VEC, F::S, F::W, F::CTAS>, p, pl, 32 * F::W, F::CTAS,
+                             sizeof(BwdSmem<T, VEC, F::S, F::W>), ws, st, "gated_recurrence_backward kernel");
 }
 template <typename T>
 int choose_backward(const MambaRecurrenceArgs *a, BwdParams &p, const MambaRecurrenceGrads *g, void *ws,
                     cudaStream_t st) {
-    constexpr int V = bwd_vec(sizeof(T) == 2 ? MAMBA_F16 : MAMBA_F32);
+    constexpr int V = BwdShape<T>::VEC;
     const bool vec = a->dim % V == 0 && vector_rows<T, V>(a->x, a->x_stride) && vector_rows<T, V>(a->r, a->r_stride) &&
                      vector_rows<T, V>(a->i, a->i_stride) && vector_rows<T, V>(a->h, a->h_stride) &&
                      vector_rows<T, V>(g->dh, g->dh_stride) && vector_rows<T, V>(g->dx, g->dx_stride) &&
@@ -937,15 +1127,26 @@ int recurrence_step(const void *x, int64_t xrs, const void *r, int64_t rrs, cons
                      aligned_to(lambda, 4) && aligned_to(state_in, 4) && aligned_to(state_out, 4),
                  "gated_recurrence_step: pointers must be aligned to their element type");
     MB_CHECK_ARG(batch == 1 || hrs >= dim, "gated_recurrence_step: rows of h overlap (stride)");
-    const dim3 grid((unsigned)ceil_div(dim, kThreads), (unsigned)batch);
+    auto run = [&](auto zero) {
+        using T = decltype(zero);
+        StepParams<T> p{static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(i),
+                        static_cast<T *>(h), lambda, state_in, state_out, xrs, rrs, irs, hrs, batch, dim, 1, c};
+        const bool vec = dim % 4 == 0 && xrs % 4 == 0 && rrs % 4 == 0 && irs % 4 == 0 && hrs % 4 == 0 &&
+                         aligned_to(x, 4 * es) && aligned_to(r, 4 * es) && aligned_to(i, 4 * es) &&
+                         aligned_to(h, 4 * es) && aligned_to(state_in, 16) && aligned_to(state_out, 16);
+        const int blocks = ceil_div(dim, kThreads * (vec ? 4 : 1));
+        // several rows per thread once one row each would fill the GPU four times over
+        p.rows = (int64_t)blocks * batch >= 16LL * device_sm_count() ? 4 : 1;
+        const dim3 grid((unsigned)blocks, (unsigned)ceil_div(batch, p.rows));
+        if (vec)
+            recurrence_step_kernel<T, 4><<<grid, kThreads, 0, st>>>(p);
+        else
+            recurrence_step_kernel<T, 1><<<grid, kThreads, 0, st>>>(p);
+    };
     if (dtype == MAMBA_F16)
-        recurrence_step_kernel<__half><<<grid, kThreads, 0, st>>>(
-            static_cast<const __half *>(x), xrs, static_cast<const __half *>(r), rrs, static_cast<const __half *>(i),
-            irs, lambda, state_in, state_out, static_cast<__half *>(h), hrs, dim, c);
+        run(__half());
     else
-        recurrence_step_kernel<float><<<grid, kThreads, 0, st>>>(
-            static_cast<const float *>(x), xrs, static_cast<const float *>(r), rrs, static_cast<const float *>(i), irs,
-            lambda, state_in, state_out, static_cast<float *>(h), hrs, dim, c);
+        run(0.f);
     return launch_status("gated_recurrence_step kernel");
 }
 
