@@ -108,7 +108,8 @@ const char *mamba_last_error(void);
  * rows, mamba_gated_mlp_up by default).  Bit 5: the same for
  * the decode state update's bulk-copy waits (mamba_ssm_step, mamba_step).
  * Bit 6: a wait of mamba_gated_recurrence or its backward pass for the
- * sequence tile before it exceeded the same bound.
+ * sequence tile before it exceeded the same bound.  Bit 7: the same as bit 4
+ * for mamba_linear_i8's tensor-core kernel.
  * Waits for the device; clear != 0 resets them. */
 unsigned mamba_device_status(int clear);
 

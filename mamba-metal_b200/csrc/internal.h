@@ -107,6 +107,7 @@ int quantize_rows(const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *sca
                   cudaStream_t st);
 int linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw, const float *w_scale,
               const float *bias, void *y, int64_t ldy, int64_t rows, int n, int k, int mode, cudaStream_t st);
+unsigned linear_i8_error_flags(bool clear);
 
 // init.cu
 uint64_t fill_key(uint64_t seed, int layer, int tag);

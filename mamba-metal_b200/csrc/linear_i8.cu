@@ -6,10 +6,16 @@
 // so the result does not depend on how K is split.
 #include "common.cuh"
 #include "internal.h"
+#include "tma.cuh"
+#include "umma.cuh"
 
 #include <algorithm>
+#include <mutex>
+#include <vector>
 
 namespace mb {
+
+__device__ unsigned int g_linear_i8_error = 0;
 
 namespace {
 
@@ -172,6 +178,365 @@ __device__ __forceinline__ void emit_i8(const I8Params &p, int64_t t, int n, int
         static_cast<float *>(p.y)[t * p.ldy + n] = v;
 }
 
+// ---- tensor cores -----------------------------------------------------------------
+// A persistent kernel of CTA pairs (clusters of two, cta_group::2), the shape
+// of the FP16 projection GEMM: a pair owns 256 tokens x BN channels; per 128
+// bytes of K each CTA loads its 128 rows of x and BN / 2 rows of w by TMA
+// (128-byte swizzle) into a ring of stages, one thread of the even CTA issues
+// tcgen05.mma.kind::i8 over both CTAs' operands, and the 32-bit sums land in
+// both CTAs' TMEM, two accumulators in turn.  Eight epilogue warps scale the
+// sums (warp w: TMEM lanes of quarter w % 4, every other chunk of 32 columns)
+// and send them out through swizzled shared-memory boxes by bulk tensor stores
+// (adds for mode 1), or element by element where y's rows are not 16-byte
+// aligned.
+//
+// BN decides how decode-sized calls fill the GPU (choose_bn): a pair reads 256
+// tokens and BN channels per byte of K, so few rows want just as many column
+// tiles as there are pairs.
+// Every mbarrier wait is bounded (2 s); on timeout the role stops, bit 7 of the
+// device status is set, and both CTAs still reach the final cluster barrier.
+constexpr int kBK = 128, kUK = 32;          // bytes of K per stage and per MMA
+constexpr int kStages = 5, kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
+constexpr int kStageX = 128 * kBK, kStageW = 128 * kBK, kStageBytes = kStageX + kStageW;
+constexpr int kAccCols = 256;
+constexpr int kBox = 32 * 128;              // 32 rows x 128 bytes
+constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * 2 * kBox + 1024 /* alignment */ + 256 /* barriers */;
+static_assert(kSmemBytes <= 232448, "shared memory");
+constexpr unsigned kErrLinearI8Timeout = 128u;
+
+struct PairParams {
+    I8Params g;
+    int BN, m_tiles, n_tiles, kblocks;
+    uint32_t idesc, tx_bytes;
+    bool boxes;  // y's rows allow bulk tensor stores
+};
+
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
+    int ok = 0;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait_bounded(bar, parity) ? 1 : 0;
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+// 32 columns of one row, without a bulk store: 16 bytes at a time where the
+// row is aligned and the columns exist.
+__device__ __forceinline__ void store_row(const I8Params &g, int64_t row, int c0, const float (&f)[32], bool aligned) {
+    if (g.mode == 0) {
+        __half *o = static_cast<__half *>(g.y) + row * g.ldy + c0;
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+            if (aligned && c0 + j + 8 <= g.n) {
+                uint32_t w[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const __half2 h = __floats2half2_rn(f[j + 2 * q], f[j + 2 * q + 1]);
+                    w[q] = *reinterpret_cast<const uint32_t *>(&h);
+                }
+                *reinterpret_cast<uint4 *>(o + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (c0 + j + q < g.n) o[j + q] = __float2half_rn(f[j + q]);
+            }
+        }
+    } else {
+        float *o = static_cast<float *>(g.y) + row * g.ldy + c0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (c0 + j < g.n) o[j] = g.mode == 1 ? o[j] + f[j] : f[j];
+    }
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_i8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                          const __grid_constant__ CUtensorMap map_y, const PairParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *epi = smem + kStages * kStageBytes;
+    uint64_t *full = reinterpret_cast<uint64_t *>(epi + kEpiWarps * 2 * kBox);
+    uint64_t *empty = full + kStages, *tfull = empty + kStages, *tempty = tfull + 2, *drain = tempty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    const uint32_t rank = cluster_ctarank();
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles = p.m_tiles * p.n_tiles;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], 2 * kEpiWarps);
+        }
+        mbar_init(drain, 1);
+        fence_mbar_init();
+        prefetch_tensormap(&map_x);
+        prefetch_tensormap(&map_w);
+        prefetch_tensormap(&map_y);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 2 * kAccCols);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint32_t full0 = mapa_shared(smem_u32(&full[0]), 0);
+            uint32_t it = 0;
+            for (int tile = pair; tile < tiles && ok; tile += npairs) {
+                const int mt = tile / p.n_tiles, nt = tile % p.n_tiles;
+                const int xrow = mt * 256 + (int)rank * 128, wrow = nt * p.BN + (int)rank * (p.BN >> 1);
+                for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+                    const uint32_t s = it % kStages, ph = (it / kStages) & 1;
+                    if (!mbar_wait_bounded(&empty[s], ph ^ 1)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], p.tx_bytes);
+                    uint8_t *a = smem + s * kStageBytes;
+                    tma_load_2d_pair(a, &map_x, full0 + s * 8, kb * kBK, xrow);
+                    tma_load_2d_pair(a + kStageX, &map_w, full0 + s * 8, kb * kBK, wrow);
+                }
+            }
+            if (rank == 0) {  // every copy of both CTAs has landed before the even CTA leaves
+                const uint32_t first = it > (uint32_t)kStages ? it - kStages : 0;
+                for (uint32_t j = first; j < it; ++j)
+                    if (!mbar_wait_bounded_cluster(&full[j % kStages], (j / kStages) & 1)) ok = false;
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            uint32_t it = 0, tcount = 0;
+            for (int tile = pair; tile < tiles && ok; tile += npairs, ++tcount) {
+                const uint32_t b = tcount & 1, tph = (tcount >> 1) & 1;
+                if (!mbar_wait_bounded_cluster(&tempty[b], tph ^ 1)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem + b * kAccCols;
+                for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+                    const uint32_t s = it % kStages, ph = (it / kStages) & 1;
+                    if (!mbar_wait_bounded_cluster(&full[s], ph)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a_addr = smem_u32(smem + s * kStageBytes), b_addr = a_addr + kStageX;
+#pragma unroll
+                    for (int k = 0; k < kBK / kUK; ++k)
+                        umma_i8_pair(d_tmem, smem_desc_sw128(a_addr + k * kUK), smem_desc_sw128(b_addr + k * kUK),
+                                     p.idesc, (kb | k) != 0);
+                    umma_commit_pair(&empty[s], 0x3);
+                }
+                if (!ok) break;
+                umma_commit_pair(&tfull[b], 0x3);
+            }
+            umma_commit_pair(drain, 0x1);  // every issued MMA completes before TMEM may be freed
+            if (!mbar_wait_bounded(drain, 0)) ok = false;
+        }
+    } else {
+        const int quarter = warp & 3, egroup = (warp - 2) >> 2;
+        uint8_t *boxes = epi + (warp - 2) * 2 * kBox;
+        const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
+        const I8Params &g = p.g;
+        const int cstep = g.mode == 0 ? 64 : 32;  // columns of one 128-byte box row
+        uint32_t tcount = 0, nbox = 0;
+        for (int tile = pair; tile < tiles; tile += npairs, ++tcount) {
+            const uint32_t b = tcount & 1, tph = (tcount >> 1) & 1;
+            const int mt = tile / p.n_tiles, nt = tile % p.n_tiles;
+            const int64_t row0 = (int64_t)mt * 256 + rank * 128 + quarter * 32, row = row0 + lane;
+            const float xs = row < g.rows ? g.xs[row] : 0.f;
+            if (!warp_wait(&tfull[b], tph)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16) + b * kAccCols;
+            for (int c = egroup * cstep; c < p.BN; c += 2 * cstep) {
+                const int col = nt * p.BN + c;
+                if (col >= g.n || row0 >= g.rows) break;  // the same for the whole warp
+                uint8_t *box = boxes + (nbox & 1) * kBox;
+                // an FP16 box takes 64 columns: of a BN that is an odd multiple of 32 the last 32
+                // go out without one, since the box's other half would be the next tile's
+                const bool boxed = p.boxes && (g.mode != 0 || c + 32 < p.BN);
+                if (boxed) {  // the bulk store that last read this box has finished reading it
+                    if (lane == 0) bulk_wait_group_read<1>();
+                    __syncwarp();
+                }
+                for (int hlf = 0; hlf < (g.mode == 0 ? 2 : 1); ++hlf) {
+                    const int c0 = col + 32 * hlf;
+                    if (c + 32 * hlf >= p.BN) break;  // BN is a multiple of 32
+                    uint32_t v[32];
+                    tmem_ld_32x32b_x32(tl + c + 32 * hlf, v);
+                    tmem_wait_ld();
+                    float f[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const int cc = min(c0 + j, g.n - 1);
+                        f[j] = (float)(int)v[j] * xs * __ldg(g.ws + cc);
+                        if (g.bias) f[j] += __ldg(g.bias + cc);
+                    }
+                    if (!boxed) {
+                        if (row < g.rows) store_row(g, row, c0, f, p.boxes);
+                        continue;
+                    }
+                    // row `lane` of a 32-row box with the TMA 128-byte swizzle: chunk j at j ^ (row % 8)
+                    if (g.mode == 0) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const __half2 h = __floats2half2_rn(f[8 * j + 2 * q], f[8 * j + 2 * q + 1]);
+                                w[q] = *reinterpret_cast<const uint32_t *>(&h);
+                            }
+                            *reinterpret_cast<uint4 *>(box + lane * 128 + (((4 * hlf + j) ^ (lane & 7)) << 4)) =
+                                make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<float4 *>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                                make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                    }
+                }
+                if (!boxed) continue;
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    if (g.mode == 1)
+                        tma_reduce_add_2d(&map_y, box, col, (int)row0);
+                    else
+                        tma_store_2d(&map_y, box, col, (int)row0);
+                    bulk_commit_group();
+                }
+                ++nbox;
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (rank == 0)
+                    mbar_arrive(&tempty[b]);
+                else
+                    mbar_arrive_cluster(tempty0 + b * 8);
+            }
+        }
+        if (lane == 0) bulk_wait_group_all();
+        __syncwarp();
+    }
+    if (!ok) atomicOr(&g_linear_i8_error, kErrLinearI8Timeout);
+    tc_fence_before();
+    cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 2 * kAccCols);
+    }
+}
+
+// 2-D map over row-major rows with 128-byte-swizzled boxes of 128 bytes x
+// box_rows; loads outside the matrix read zeros, stores outside are dropped.
+bool encode_rows(CUtensorMap *m, CUtensorMapDataType t, int esize, const void *ptr, int64_t rows, int64_t cols,
+                 int64_t ld, int box_rows) {
+    auto enc = tensor_map_encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(ld * esize)};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / esize), (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    return enc(m, t, 2, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+cudaLaunchConfig_t pair_launch(int pairs, cudaLaunchAttribute *attr, cudaStream_t st) {
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = 2;
+    attr->val.clusterDim.y = 1;
+    attr->val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(2 * pairs, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cfg;
+}
+
+// CTA pairs that fit on the current device at once (asked once per device),
+// -1 on an error, 0 on a device without these tensor cores.
+int device_pairs() {
+    static std::mutex mu;
+    static std::vector<int> cache;
+    int dev = 0;
+    MB_CUDA_TRY(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lk(mu);
+    if ((int)cache.size() <= dev) cache.resize(dev + 1, -1);
+    if (cache[dev] < 0) {
+        int major = 0, n = 0;
+        MB_CUDA_TRY(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
+        if (major == 10) {
+            MB_CUDA_TRY(cudaFuncSetAttribute(linear_i8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             kSmemBytes));
+            cudaLaunchAttribute attr{};
+            cudaLaunchConfig_t cfg = pair_launch(148, &attr, nullptr);
+            MB_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, linear_i8_pair_kernel, &cfg));
+        }
+        cache[dev] = n;
+    }
+    return cache[dev];
+}
+
+// Columns per tile: the multiple of 32 with the least rounds of tiles over the
+// pairs, each round costing what a CTA loads per byte of K (128 rows of x and
+// BN / 2 of w).
+int choose_bn(int64_t m_tiles, int n, int pairs) {
+    int best = 256;
+    int64_t cost = INT64_MAX;
+    for (int bn = 256; bn >= 32; bn -= 32) {
+        const int64_t rounds = ceil_div64(m_tiles * ceil_div(n, bn), pairs), c = rounds * (128 + bn / 2);
+        if (c < cost) {
+            cost = c;
+            best = bn;
+        }
+    }
+    return best;
+}
+
+int launch_pairs(const I8Params &g, int pairs, cudaStream_t st) {
+    PairParams p{};
+    p.g = g;
+    p.m_tiles = (int)ceil_div64(g.rows, 256);
+    p.BN = choose_bn(p.m_tiles, g.n, pairs);
+    const int64_t tiles = (int64_t)p.m_tiles * ceil_div(g.n, p.BN);
+    MB_CHECK_ARG(tiles <= 0x7fffffff, "linear_i8: too many tiles");
+    p.n_tiles = ceil_div(g.n, p.BN);
+    p.kblocks = ceil_div(g.k, kBK);
+    p.idesc = idesc_s8_s32acc(256, p.BN);
+    p.tx_bytes = (uint32_t)(2 * (kStageX + (p.BN / 2) * kBK));
+    const int es = g.mode == 0 ? 2 : 4;
+    p.boxes = aligned_to(g.y, 16) && (g.ldy * es) % 16 == 0;
+    CUtensorMap mx, mw, my;
+    bool enc = encode_rows(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.x, g.rows, g.k, g.ldx, 128) &&
+               encode_rows(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.w, g.n, g.k, g.ldw, p.BN / 2);
+    if (enc && p.boxes)
+        enc = encode_rows(&my, es == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, es, g.y,
+                          g.rows, g.n, g.ldy, 32);
+    else
+        my = mx;
+    MB_CHECK_ARG(enc, "linear_i8: tensor map encoding failed");
+    cudaLaunchAttribute attr{};
+    const cudaLaunchConfig_t cfg = pair_launch((int)std::min<int64_t>(tiles, pairs), &attr, st);
+    MB_CUDA_TRY(cudaLaunchKernelEx(&cfg, linear_i8_pair_kernel, mx, mw, my, p));
+    return launch_status("linear_i8 (tcgen05, CTA pairs) kernel");
+}
+
 // Any strides and alignment: 64 x 64 outputs per CTA, 64 bytes of K staged at
 // a time by single bytes, 4 x 4 outputs per thread by dp4a.
 constexpr int kDT = 64, kDPitch = 68;
@@ -246,7 +611,6 @@ int linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *
                      aligned_to(y, mode == 0 ? 2 : 4),
                  "linear_i8: pointers must be aligned to their element type");
     MB_CHECK_ARG((rows == 1 || (ldx >= k && ldy >= n)) && (n == 1 || ldw >= k), "linear_i8: a row stride is below its row");
-    MB_CHECK_ARG(rows <= 65535LL * kDT, "linear_i8: too many rows");
     I8Params p{};
     p.x = x;
     p.w = w;
@@ -261,8 +625,25 @@ int linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *
     p.n = n;
     p.k = k;
     p.mode = mode;
+    if (k > 0 && aligned_to(x, 16) && aligned_to(w, 16) && ldx % 16 == 0 && ldw % 16 == 0 && ldx >= k && ldw >= k &&
+        rows <= 0x7fffffff - 256) {
+        const int pairs = device_pairs();
+        if (pairs < 0) return -1;
+        if (pairs > 0) return launch_pairs(p, pairs, st);
+    }
+    MB_CHECK_ARG(rows <= 65535LL * kDT, "linear_i8: too many rows");
     linear_i8_dp4a_kernel<<<dim3((unsigned)ceil_div(n, kDT), (unsigned)ceil_div64(rows, kDT)), 256, 0, st>>>(p);
     return launch_status("linear_i8 kernel");
+}
+
+unsigned linear_i8_error_flags(bool clear) {
+    unsigned v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_linear_i8_error, sizeof(v)) != cudaSuccess) return ~0u;
+    if (clear && v) {
+        const unsigned z = 0;
+        cudaMemcpyToSymbol(g_linear_i8_error, &z, sizeof(z));
+    }
+    return v;
 }
 
 }  // namespace mb
