@@ -17,6 +17,9 @@
 #include "tma.cuh"
 
 #include <algorithm>
+#include <mutex>
+#include <utility>
+#include <vector>
 
 namespace mb {
 
@@ -993,6 +996,21 @@ size_t recurrence_workspace_bytes(const MambaRecurrenceArgs *a, bool backward) {
 
 namespace {
 
+// Opts a kernel into its shared memory, once per device.
+template <typename Kernel>
+int allow_smem(Kernel kernel, size_t bytes) {
+    static std::mutex mu;
+    static std::vector<std::pair<const void *, int>> done;
+    int dev = 0;
+    MB_CUDA_TRY(cudaGetDevice(&dev));
+    const std::pair<const void *, int> key(reinterpret_cast<const void *>(kernel), dev);
+    std::lock_guard<std::mutex> lk(mu);
+    if (std::find(done.begin(), done.end(), key) != done.end()) return 0;
+    MB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    done.push_back(key);
+    return 0;
+}
+
 // Launches one variant: the workspace's part from the ticket on set to all
 // ones bits, then persistent CTAs.
 template <int VEC, typename Kernel, typename Params>
@@ -1003,7 +1021,7 @@ int launch_tiles(Kernel kernel, const Params &p, Plan &pl, int threads, int ctas
     c.ticket = reinterpret_cast<unsigned int *>(base);
     c.maps = reinterpret_cast<float2 *>(base + 256);
     c.states = reinterpret_cast<float *>(c.maps + (int64_t)c.chains.d * c.tiles * 32 * VEC);
-    MB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (allow_smem(kernel, smem)) return -1;
     MB_CUDA_TRY(cudaMemsetAsync(base, 0xff, pl.bytes, st));
     const int64_t total = (int64_t)c.chains.d * c.tiles, most = (int64_t)ctas * device_sm_count();
     kernel<<<(unsigned)std::min(total, most), threads, smem, st>>>(p, c);

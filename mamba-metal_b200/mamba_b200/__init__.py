@@ -21,6 +21,7 @@ pass and single-token step), block_norm (with its backward pass),
 quantize_rows and linear_i8 (8-bit linear layer).
 """
 import ctypes
+import functools
 import os
 import struct
 
@@ -429,9 +430,15 @@ class State:
 # ---------------------------------------------------------------------------
 # Kernel-level helpers on torch CUDA tensors
 # ---------------------------------------------------------------------------
+_torch_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def _dt(t):
@@ -631,92 +638,119 @@ def _require(cond, msg):
 
 def _check_tensor(t, name, what, shape, dtype, device, strided=False):
     """t is a tensor of this shape, dtype and device, contiguous or (strided) with channel stride 1."""
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device:
+    if t.is_contiguous() and t.shape == shape and t.dtype is dtype and t.device == device:
+        return
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
         raise MambaError("%s: %s must be %s %s on %s, got %s %s on %s"
                          % (what, name, dtype, tuple(shape), device, t.dtype, tuple(t.shape), t.device))
-    if strided:
-        _require(t.shape[-1] <= 1 or t.stride(-1) == 1, "%s: %s needs channel stride 1" % (what, name))
-    else:
-        _require(t.is_contiguous(), "%s: %s must be contiguous" % (what, name))
+    if not strided:
+        raise MambaError("%s: %s must be contiguous" % (what, name))
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise MambaError("%s: %s needs channel stride 1" % (what, name))
 
 
-def _stream_of(t, stream):
-    """The stream handle of a call on t's device: the caller's, else that device's current stream."""
-    if stream is None:
-        return _torch().cuda.current_stream(t.device).cuda_stream
-    return _stream(stream)
+def _check_float(t, name, what):
+    torch = _torch()
+    if t.dtype is not torch.float16 and t.dtype is not torch.float32:
+        raise MambaError("%s: %s must be float16 or float32" % (what, name))
 
 
-class _on_device:
-    """Makes a tensor's device current for a library call (no CUDA call when it already is)."""
-
-    def __init__(self, t):
+def _on_stream(fn):
+    """Adds the `stream` argument (a torch stream or a handle; default: the
+    current one).  The whole helper runs with that stream current, so that
+    what it allocates and fills belongs to the stream its kernels run on."""
+    @functools.wraps(fn)
+    def helper(t, *args, stream=None, **kw):
+        if stream is None:
+            return fn(t, *args, **kw)
         torch = _torch()
-        _require(t.is_cuda, "tensors must be on a CUDA device")
-        self._dev = t.device.index
-        self._prev = torch.cuda.current_device()
-
-    def __enter__(self):
-        if self._prev != self._dev:
-            _torch().cuda.set_device(self._dev)
-
-    def __exit__(self, *exc):
-        if self._prev != self._dev:
-            _torch().cuda.set_device(self._prev)
+        if not t.is_cuda:
+            raise MambaError("%s: tensors must be on a CUDA device" % fn.__name__)
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(stream, device=t.device) if stream \
+                else torch.cuda.default_stream(t.device)
+        with torch.cuda.stream(stream):
+            return fn(t, *args, **kw)
+    return helper
 
 
-def _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets):
+def _call(fn, what, t, *args):
+    """fn(*args, stream) on t's device and its current stream.  The device is
+    made current only where it is not."""
+    torch = _torch()
+    if not t.is_cuda:
+        raise MambaError("%s: tensors must be on a CUDA device" % what)
+    dev = t.device.index
+    stream = torch._C._cuda_getCurrentRawStream(dev)  # without building a Stream object (2 us)
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    _check(rc, what)
+
+
+# The argument structs are packed in one go (setting their fields one by one
+# costs several microseconds, more than the launch).
+_RECURRENCE_ARGS = struct.Struct("@9P4if4x8q")
+_RECURRENCE_GRADS = struct.Struct("@7P8q")
+_BLOCK_NORM_ARGS = struct.Struct("@9Pq2i2f2q")
+_BLOCK_NORM_GRADS = struct.Struct("@7P2q")
+
+
+def _ptr0(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets, h=None, final_state=None):
     torch = _torch()
     _require(x.dim() == 3, "%s: x must be [batch, seqlen, dim]" % what)
-    bsz, L, dim = x.shape
-    dev = x.device
-    _require(x.dtype in (torch.float16, torch.float32), "%s: x must be float16 or float32" % what)
-    _check_tensor(x, "x", what, x.shape, x.dtype, dev, True)
-    _check_tensor(r, "r", what, x.shape, x.dtype, dev, True)
-    _check_tensor(i, "i", what, x.shape, x.dtype, dev, True)
+    _check_float(x, "x", what)
+    shape, dt, dev = x.shape, x.dtype, x.device
+    bsz, L, dim = shape
+    _check_tensor(x, "x", what, shape, dt, dev, True)
+    _check_tensor(r, "r", what, shape, dt, dev, True)
+    _check_tensor(i, "i", what, shape, dt, dev, True)
     _check_tensor(lam, "lam", what, (dim,), torch.float32, dev)
     if initial_state is not None:
         _check_tensor(initial_state, "initial_state", what, (bsz, dim), torch.float32, dev)
     if lengths is not None:
         _check_tensor(lengths, "lengths", what, (bsz,), torch.int32, dev)
     if resets is not None:
-        if resets.dtype == torch.bool:
+        if resets.dtype is torch.bool:
             resets = resets.view(torch.uint8)
         _check_tensor(resets, "resets", what, (bsz, L), torch.uint8, dev)
-    a = MambaRecurrenceArgs()
-    a.x, a.r, a.i, a.lambda_ = x.data_ptr(), r.data_ptr(), i.data_ptr(), lam.data_ptr()
-    a.initial_state, a.lengths, a.resets = _ptr(initial_state), _ptr(lengths), _ptr(resets)
-    a.batch, a.seqlen, a.dim, a.dtype, a.c = bsz, L, dim, _dt(x), c
-    a.x_stride[:] = x.stride()[:2]
-    a.r_stride[:] = r.stride()[:2]
-    a.i_stride[:] = i.stride()[:2]
-    return a
+    sx, sr, si = x.stride(), r.stride(), i.stride()
+    sh = sx if h is None else h.stride()
+    return MambaRecurrenceArgs.from_buffer_copy(_RECURRENCE_ARGS.pack(
+        x.data_ptr(), r.data_ptr(), i.data_ptr(), lam.data_ptr(), _ptr0(initial_state), _ptr0(lengths), _ptr0(resets),
+        _ptr0(h), _ptr0(final_state), bsz, L, dim, F16 if dt is torch.float16 else F32, c, sx[0], sx[1], sr[0], sr[1],
+        si[0], si[1], sh[0], sh[1]))
 
 
 def _recurrence_out(name, what, out, x, lengths):
     """An output like x; fresh ones are zeroed when rows end early, since
     positions behind a row's end are not written."""
-    torch = _torch()
     if out is None:
-        make = torch.empty if lengths is None else torch.zeros
-        return make(x.shape, dtype=x.dtype, device=x.device)
+        return x.new_empty(x.shape) if lengths is None else x.new_zeros(x.shape)
     _check_tensor(out, name, what, x.shape, x.dtype, x.device, True)
     return out
 
 
-def _recurrence_workspace(what, a, backward, workspace, x):
-    need = lib().mamba_gated_recurrence_workspace(ctypes.byref(a), int(backward))
-    if need and workspace is None:
-        workspace = _torch().empty(need, dtype=_torch().uint8, device=x.device)
+def _workspace(what, need, workspace, x):
+    """(pointer, bytes) of the caller's workspace or a fresh one, and the tensor that owns it."""
     if workspace is None:
-        return None, None, 0
+        if not need:
+            return 0, 0, None
+        workspace = _torch().empty(need, dtype=_torch().uint8, device=x.device)
     _require(workspace.is_contiguous() and workspace.device == x.device,
              "%s: workspace must be contiguous and on the tensors' device" % what)
-    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
+@_on_stream
 def gated_recurrence(x, r, i, lam, c=8.0, initial_state=None, lengths=None, resets=None,
-                     return_final_state=False, h=None, workspace=None, stream=None):
+                     return_final_state=False, h=None, workspace=None):
     """Gated linear recurrence (mamba_gated_recurrence):
     h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t,
     a_t = exp(-c softplus(lam) sigmoid(r_t)).
@@ -727,105 +761,96 @@ def gated_recurrence(x, r, i, lam, c=8.0, initial_state=None, lengths=None, rese
     fresh h); resets uint8 or bool [batch, L] (the state counts as zero
     before a marked token).  Returns h (x's dtype) and, if asked, the FP32
     state after each row's last token."""
-    torch = _torch()
-    what = "gated_recurrence"
-    a = _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets)
+    what = "mamba_gated_recurrence"
     h = _recurrence_out("h", what, h, x, lengths)
-    a.h = h.data_ptr()
-    a.h_stride[:] = h.stride()[:2]
-    hN = torch.empty((a.batch, a.dim), dtype=torch.float32, device=x.device) if return_final_state else None
-    a.final_state = _ptr(hN)
-    with _on_device(x):
-        ws, ws_ptr, ws_len = _recurrence_workspace(what, a, False, workspace, x)
-        _check(lib().mamba_gated_recurrence(ctypes.byref(a), ws_ptr, ws_len, _stream_of(x, stream)),
-               "mamba_gated_recurrence")
+    hN = lam.new_empty((x.shape[0], x.shape[-1])) if return_final_state else None
+    a = _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets, h, hN)
+    need = lib().mamba_gated_recurrence_workspace(a, 0)
+    ws, ws_len, owner = _workspace(what, need, workspace, x)
+    _call(lib().mamba_gated_recurrence, what, x, a, ws, ws_len)
     return (h, hN) if return_final_state else h
 
 
+@_on_stream
 def gated_recurrence_backward(dh, x, r, i, lam, h, c=8.0, initial_state=None, lengths=None, resets=None,
-                              dfinal_state=None, dx=None, dr=None, di=None, workspace=None, stream=None):
+                              dfinal_state=None, dx=None, dr=None, di=None, workspace=None):
     """Gradients of gated_recurrence (mamba_gated_recurrence_backward): dh is
     the gradient of h, dfinal_state (FP32 [batch, dim] or None) that of the
     final state; h is the forward's output.  Returns (dx, dr, di, dlam,
     dinitial_state); dlam and dinitial_state are FP32."""
-    torch = _torch()
-    what = "gated_recurrence_backward"
-    a = _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets)
+    what = "mamba_gated_recurrence_backward"
     _check_tensor(h, "h", what, x.shape, x.dtype, x.device, True)
     _check_tensor(dh, "dh", what, x.shape, x.dtype, x.device, True)
-    a.h = h.data_ptr()
-    a.h_stride[:] = h.stride()[:2]
+    a = _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets, h)
     if dfinal_state is not None:
-        _check_tensor(dfinal_state, "dfinal_state", what, (a.batch, a.dim), torch.float32, x.device)
-    dx, dr, di = (_recurrence_out(n, what, t, x, lengths) for n, t in (("dx", dx), ("dr", dr), ("di", di)))
-    dlam = torch.empty((a.dim,), dtype=torch.float32, device=x.device)
-    dh0 = torch.empty((a.batch, a.dim), dtype=torch.float32, device=x.device)
-    g = MambaRecurrenceGrads()
-    g.dh, g.dfinal_state, g.dx, g.dr, g.di = dh.data_ptr(), _ptr(dfinal_state), _ptr(dx), _ptr(dr), _ptr(di)
-    g.dlambda, g.dinitial_state = dlam.data_ptr(), dh0.data_ptr()
-    g.dh_stride[:] = dh.stride()[:2]
-    g.dx_stride[:] = dx.stride()[:2]
-    g.dr_stride[:] = dr.stride()[:2]
-    g.di_stride[:] = di.stride()[:2]
-    with _on_device(x):
-        ws, ws_ptr, ws_len = _recurrence_workspace(what, a, True, workspace, x)
-        _check(lib().mamba_gated_recurrence_backward(ctypes.byref(a), ctypes.byref(g), ws_ptr, ws_len,
-                                                     _stream_of(x, stream)), "mamba_gated_recurrence_backward")
+        _check_tensor(dfinal_state, "dfinal_state", what, (a.batch, a.dim), lam.dtype, x.device)
+    dx = _recurrence_out("dx", what, dx, x, lengths)
+    dr = _recurrence_out("dr", what, dr, x, lengths)
+    di = _recurrence_out("di", what, di, x, lengths)
+    dlam = lam.new_empty(lam.shape)
+    dh0 = lam.new_empty((a.batch, a.dim))
+    sg, sx, sr, si = dh.stride(), dx.stride(), dr.stride(), di.stride()
+    g = MambaRecurrenceGrads.from_buffer_copy(_RECURRENCE_GRADS.pack(
+        dh.data_ptr(), _ptr0(dfinal_state), dx.data_ptr(), dr.data_ptr(), di.data_ptr(), dlam.data_ptr(),
+        dh0.data_ptr(), sg[0], sg[1], sx[0], sx[1], sr[0], sr[1], si[0], si[1]))
+    need = lib().mamba_gated_recurrence_workspace(a, 1)
+    ws, ws_len, owner = _workspace(what, need, workspace, x)
+    _call(lib().mamba_gated_recurrence_backward, what, x, a, g, ws, ws_len)
     return dx, dr, di, dlam, dh0
 
 
-def gated_recurrence_step(x, r, i, lam, state, c=8.0, state_out=None, h=None, stream=None):
+@_on_stream
+def gated_recurrence_step(x, r, i, lam, state, c=8.0, state_out=None, h=None):
     """One token of the gated recurrence (mamba_gated_recurrence_step): x, r,
     i [batch, dim] (row stride any, channel stride 1), state FP32 [batch,
     dim].  state_out may be the state itself (update in place); by default
     the state is left alone.  Returns (h, state_out)."""
     torch = _torch()
-    what = "gated_recurrence_step"
+    what = "mamba_gated_recurrence_step"
     _require(x.dim() == 2, "%s: x must be [batch, dim]" % what)
-    _require(x.dtype in (torch.float16, torch.float32), "%s: x must be float16 or float32" % what)
-    bsz, dim = x.shape
-    dev = x.device
-    for name, t in (("x", x), ("r", r), ("i", i)):
-        _check_tensor(t, name, what, x.shape, x.dtype, dev, True)
-    _check_tensor(lam, "lam", what, (dim,), torch.float32, dev)
-    _check_tensor(state, "state", what, x.shape, torch.float32, dev)
+    _check_float(x, "x", what)
+    shape, dt, dev = x.shape, x.dtype, x.device
+    _check_tensor(x, "x", what, shape, dt, dev, True)
+    _check_tensor(r, "r", what, shape, dt, dev, True)
+    _check_tensor(i, "i", what, shape, dt, dev, True)
+    _check_tensor(lam, "lam", what, shape[1:], torch.float32, dev)
+    _check_tensor(state, "state", what, shape, torch.float32, dev)
     if state_out is None:
-        state_out = torch.empty((bsz, dim), dtype=torch.float32, device=dev)
+        state_out = torch.empty_like(state)
     else:
-        _check_tensor(state_out, "state_out", what, x.shape, torch.float32, dev)
+        _check_tensor(state_out, "state_out", what, shape, torch.float32, dev)
     if h is None:
-        h = torch.empty((bsz, dim), dtype=x.dtype, device=dev)
+        h = x.new_empty(shape)
     else:
-        _check_tensor(h, "h", what, x.shape, x.dtype, dev, True)
-    with _on_device(x):
-        _check(lib().mamba_gated_recurrence_step(x.data_ptr(), x.stride(0), r.data_ptr(), r.stride(0), i.data_ptr(),
-                                                 i.stride(0), lam.data_ptr(), state.data_ptr(), state_out.data_ptr(),
-                                                 h.data_ptr(), h.stride(0), bsz, dim, c, _dt(x),
-                                                 _stream_of(x, stream)), "mamba_gated_recurrence_step")
+        _check_tensor(h, "h", what, shape, dt, dev, True)
+    _call(lib().mamba_gated_recurrence_step, what, x, x.data_ptr(), x.stride(0), r.data_ptr(), r.stride(0),
+          i.data_ptr(), i.stride(0), lam.data_ptr(), state.data_ptr(), state_out.data_ptr(), h.data_ptr(), h.stride(0),
+          shape[0], shape[1], c, F16 if dt is torch.float16 else F32)
     return h, state_out
 
 
-def _block_norm_args(what, y, w_post, z, w_pre, residual_scale, eps):
+def _block_norm_args(what, y, w_post, z, w_pre, residual_scale, eps, residual=None, residual_out=None, out=None,
+                     rstd_post=None, rstd_pre=None):
     torch = _torch()
     _require(y.dim() == 2, "%s: y must be [rows, cols]" % what)
-    _require(y.dtype in (torch.float16, torch.float32), "%s: y must be float16 or float32" % what)
-    rows, cols = y.shape
-    dev = y.device
-    _check_tensor(y, "y", what, y.shape, y.dtype, dev, True)
+    _check_float(y, "y", what)
+    shape, dt, dev = y.shape, y.dtype, y.device
+    _check_tensor(y, "y", what, shape, dt, dev, True)
     if z is not None:
-        _check_tensor(z, "z", what, y.shape, y.dtype, dev, True)
-    for name, w in (("w_post", w_post), ("w_pre", w_pre)):
-        if w is not None:
-            _check_tensor(w, name, what, (cols,), torch.float32, dev)
-    a = MambaBlockNormArgs()
-    a.y, a.z, a.w_post, a.w_pre = y.data_ptr(), _ptr(z), _ptr(w_post), _ptr(w_pre)
-    a.rows, a.cols, a.dtype, a.residual_scale, a.eps = rows, cols, _dt(y), residual_scale, eps
-    a.y_stride, a.z_stride = y.stride(0), z.stride(0) if z is not None else 0
-    return a
+        _check_tensor(z, "z", what, shape, dt, dev, True)
+    if w_post is not None:
+        _check_tensor(w_post, "w_post", what, shape[1:], torch.float32, dev)
+    if w_pre is not None:
+        _check_tensor(w_pre, "w_pre", what, shape[1:], torch.float32, dev)
+    return MambaBlockNormArgs.from_buffer_copy(_BLOCK_NORM_ARGS.pack(
+        y.data_ptr(), _ptr0(z), _ptr0(residual), _ptr0(w_post), _ptr0(w_pre), _ptr0(residual_out), _ptr0(out),
+        _ptr0(rstd_post), _ptr0(rstd_pre), shape[0], shape[1], F16 if dt is torch.float16 else F32, residual_scale,
+        eps, y.stride(0), 0 if z is None else z.stride(0)))
 
 
+@_on_stream
 def block_norm(y, residual, w_post=None, z=None, w_pre=None, residual_scale=1.0, eps=1e-5, second_norm=True,
-               return_rstd=False, residual_out=None, out=None, stream=None):
+               return_rstd=False, residual_out=None, out=None):
     """The join between two blocks (mamba_block_norm):
     residual_out = residual_scale * residual + rmsnorm(y) * w_post [* SiLU(z)]
     out = rmsnorm(residual_out) * w_pre
@@ -836,81 +861,72 @@ def block_norm(y, residual, w_post=None, z=None, w_pre=None, residual_scale=1.0,
     second_norm=False, and with return_rstd also the two FP32 [rows] factors
     that block_norm_backward reads."""
     torch = _torch()
-    what = "block_norm"
-    a = _block_norm_args(what, y, w_post, z, w_pre, residual_scale, eps)
-    dev = y.device
-    _check_tensor(residual, "residual", what, y.shape, torch.float32, dev)
+    what = "mamba_block_norm"
+    shape, dev = y.shape, y.device
+    _check_tensor(residual, "residual", what, shape, torch.float32, dev)
     if residual_out is None:
-        residual_out = torch.empty(y.shape, dtype=torch.float32, device=dev)
+        residual_out = torch.empty_like(residual)
     else:
-        _check_tensor(residual_out, "residual_out", what, y.shape, torch.float32, dev)
+        _check_tensor(residual_out, "residual_out", what, shape, torch.float32, dev)
     if not second_norm:
         out = None
     elif out is None:
-        out = torch.empty(y.shape, dtype=y.dtype, device=dev)
+        out = y.new_empty(shape)
     else:
-        _check_tensor(out, "out", what, y.shape, y.dtype, dev)
-    a.residual, a.residual_out, a.out = residual.data_ptr(), residual_out.data_ptr(), _ptr(out)
+        _check_tensor(out, "out", what, shape, y.dtype, dev)
     rstd_post = rstd_pre = None
     if return_rstd:
-        rstd_post = torch.empty((a.rows,), dtype=torch.float32, device=dev)
-        rstd_pre = torch.empty((a.rows,), dtype=torch.float32, device=dev) if second_norm else None
-        a.rstd_post, a.rstd_pre = rstd_post.data_ptr(), _ptr(rstd_pre)
-    with _on_device(y):
-        _check(lib().mamba_block_norm(ctypes.byref(a), _stream_of(y, stream)), "mamba_block_norm")
+        rstd_post = residual.new_empty(shape[:1])
+        rstd_pre = residual.new_empty(shape[:1]) if second_norm else None
+    a = _block_norm_args(what, y, w_post, z, w_pre, residual_scale, eps, residual, residual_out, out, rstd_post,
+                         rstd_pre)
+    _call(lib().mamba_block_norm, what, y, a)
     return (residual_out, out, rstd_post, rstd_pre) if return_rstd else (residual_out, out)
 
 
+@_on_stream
 def block_norm_backward(dresidual_out, dout, y, residual_out, rstd_post, rstd_pre, w_post=None, z=None, w_pre=None,
-                        residual_scale=1.0, dresidual=None, dy=None, dz=None, workspace=None, stream=None):
+                        residual_scale=1.0, dresidual=None, dy=None, dz=None, workspace=None):
     """Gradients of block_norm (mamba_block_norm_backward): dresidual_out
     (FP32) and dout (y's dtype) are the gradients of its two outputs (either
     may be None), residual_out and rstd_* what it returned.  dresidual may be
     dresidual_out.  Returns (dy, dresidual, dw_post, dw_pre, dz); the sums
     dw_post and dw_pre are FP32 [cols], dz is None without a gate."""
     torch = _torch()
-    what = "block_norm_backward"
-    a = _block_norm_args(what, y, w_post, z, w_pre, residual_scale, 1.0)  # eps is inside rstd_*
-    dev = y.device
-    _check_tensor(residual_out, "residual_out", what, y.shape, torch.float32, dev)
-    _check_tensor(rstd_post, "rstd_post", what, (a.rows,), torch.float32, dev)
-    a.residual_out, a.rstd_post = residual_out.data_ptr(), rstd_post.data_ptr()
+    what = "mamba_block_norm_backward"
+    shape, dev = y.shape, y.device
+    _check_tensor(residual_out, "residual_out", what, shape, torch.float32, dev)
+    _check_tensor(rstd_post, "rstd_post", what, shape[:1], torch.float32, dev)
     if dresidual_out is not None:
-        _check_tensor(dresidual_out, "dresidual_out", what, y.shape, torch.float32, dev)
+        _check_tensor(dresidual_out, "dresidual_out", what, shape, torch.float32, dev)
     if dout is not None:
-        _check_tensor(dout, "dout", what, y.shape, y.dtype, dev)
+        _check_tensor(dout, "dout", what, shape, y.dtype, dev)
         _require(rstd_pre is not None, "%s: dout needs rstd_pre" % what)
-        _check_tensor(rstd_pre, "rstd_pre", what, (a.rows,), torch.float32, dev)
-        a.rstd_pre = rstd_pre.data_ptr()
+        _check_tensor(rstd_pre, "rstd_pre", what, shape[:1], torch.float32, dev)
+    # eps is inside rstd_*
+    a = _block_norm_args(what, y, w_post, z, w_pre, residual_scale, 1.0, None, residual_out, None, rstd_post,
+                         rstd_pre if dout is not None else None)
     if dresidual is None:
-        dresidual = torch.empty(y.shape, dtype=torch.float32, device=dev)
+        dresidual = torch.empty_like(residual_out)
     else:
-        _check_tensor(dresidual, "dresidual", what, y.shape, torch.float32, dev)
+        _check_tensor(dresidual, "dresidual", what, shape, torch.float32, dev)
     if dy is None:
-        dy = torch.empty(y.shape, dtype=y.dtype, device=dev)
+        dy = y.new_empty(shape)
     else:
-        _check_tensor(dy, "dy", what, y.shape, y.dtype, dev, True)
+        _check_tensor(dy, "dy", what, shape, y.dtype, dev, True)
     if z is None:
         dz = None
     elif dz is None:
-        dz = torch.empty(y.shape, dtype=y.dtype, device=dev)
+        dz = y.new_empty(shape)
     else:
-        _check_tensor(dz, "dz", what, y.shape, y.dtype, dev, True)
-    dw_post = torch.empty((a.cols,), dtype=torch.float32, device=dev)
-    dw_pre = torch.empty((a.cols,), dtype=torch.float32, device=dev)
-    g = MambaBlockNormGrads()
-    g.dresidual_out, g.dout, g.dresidual = _ptr(dresidual_out), _ptr(dout), dresidual.data_ptr()
-    g.dy, g.dz, g.dw_post, g.dw_pre = dy.data_ptr(), _ptr(dz), dw_post.data_ptr(), dw_pre.data_ptr()
-    g.dy_stride, g.dz_stride = dy.stride(0), dz.stride(0) if dz is not None else 0
-    with _on_device(y):
-        need = lib().mamba_block_norm_workspace(ctypes.byref(a))
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        _require(workspace.is_contiguous() and workspace.device == dev,
-                 "%s: workspace must be contiguous and on the tensors' device" % what)
-        _check(lib().mamba_block_norm_backward(ctypes.byref(a), ctypes.byref(g), workspace.data_ptr(),
-                                               workspace.numel() * workspace.element_size(), _stream_of(y, stream)),
-               "mamba_block_norm_backward")
+        _check_tensor(dz, "dz", what, shape, y.dtype, dev, True)
+    dw_post = residual_out.new_empty(shape[1:])
+    dw_pre = residual_out.new_empty(shape[1:])
+    g = MambaBlockNormGrads.from_buffer_copy(_BLOCK_NORM_GRADS.pack(
+        _ptr0(dresidual_out), _ptr0(dout), dresidual.data_ptr(), dy.data_ptr(), _ptr0(dz), dw_post.data_ptr(),
+        dw_pre.data_ptr(), dy.stride(0), 0 if dz is None else dz.stride(0)))
+    ws, ws_len, owner = _workspace(what, lib().mamba_block_norm_workspace(a), workspace, y)
+    _call(lib().mamba_block_norm_backward, what, y, a, g, ws, ws_len)
     return dy, dresidual, dw_post, dw_pre, dz
 
 
@@ -949,57 +965,59 @@ def linear(x, w, bias=None, y=None, mode=0, workspace=None, stream=None):
     return y
 
 
-def quantize_rows(x, q=None, scale=None, stream=None):
+@_on_stream
+def quantize_rows(x, q=None, scale=None):
     """Symmetric 8-bit rows (mamba_quantize_rows): x [rows, cols] F16 or F32
     (row stride any, channel stride 1) -> (q int8 [rows, cols], scale FP32
     [rows]) with x ~ q * scale.  A fresh q is a view of rows padded to a
     multiple of 16 bytes, the layout linear_i8's fast kernels read."""
     torch = _torch()
-    what = "quantize_rows"
+    what = "mamba_quantize_rows"
     _require(x.dim() == 2, "%s: x must be [rows, cols]" % what)
-    _require(x.dtype in (torch.float16, torch.float32), "%s: x must be float16 or float32" % what)
-    rows, cols = x.shape
-    _check_tensor(x, "x", what, x.shape, x.dtype, x.device, True)
+    _check_float(x, "x", what)
+    shape, dt, dev = x.shape, x.dtype, x.device
+    rows, cols = shape
+    _check_tensor(x, "x", what, shape, dt, dev, True)
     if q is None:
-        q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :cols]
+        q = x.new_empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8)
+        if cols % 16:
+            q = q[:, :cols]
     else:
-        _check_tensor(q, "q", what, x.shape, torch.int8, x.device, True)
+        _check_tensor(q, "q", what, shape, torch.int8, dev, True)
     if scale is None:
-        scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
+        scale = x.new_empty((rows,), dtype=torch.float32)
     else:
-        _check_tensor(scale, "scale", what, (rows,), torch.float32, x.device)
-    with _on_device(x):
-        _check(lib().mamba_quantize_rows(x.data_ptr(), x.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr(), rows,
-                                         cols, _dt(x), _stream_of(x, stream)), "mamba_quantize_rows")
+        _check_tensor(scale, "scale", what, shape[:1], torch.float32, dev)
+    _call(lib().mamba_quantize_rows, what, x, x.data_ptr(), x.stride(0), q.data_ptr(), q.stride(0),
+          scale.data_ptr(), rows, cols, F16 if dt is torch.float16 else F32)
     return q, scale
 
 
-def linear_i8(x, x_scale, w, w_scale, bias=None, y=None, mode=0, stream=None):
+@_on_stream
+def linear_i8(x, x_scale, w, w_scale, bias=None, y=None, mode=0):
     """Linear layer in 8-bit integers (mamba_linear_i8): x int8 [rows, k] and
     w int8 [n, k] as quantize_rows gives them (row stride any, channel stride
     1), x_scale FP32 [rows], w_scale FP32 [n], bias FP32 [n].  mode 0 -> y
     FP16, 1 -> y FP32 += result, 2 -> y FP32 = result."""
     torch = _torch()
-    what = "linear_i8"
+    what = "mamba_linear_i8"
     _require(x.dim() == 2 and w.dim() == 2, "%s: x and w must be matrices" % what)
     _require(mode in (0, 1, 2), "%s: mode must be 0, 1 or 2" % what)
     (rows, k), n, dev = x.shape, w.shape[0], x.device
-    _check_tensor(x, "x", what, (rows, k), torch.int8, dev, True)
+    _check_tensor(x, "x", what, x.shape, torch.int8, dev, True)
     _check_tensor(w, "w", what, (n, k), torch.int8, dev, True)
     _check_tensor(x_scale, "x_scale", what, (rows,), torch.float32, dev)
     _check_tensor(w_scale, "w_scale", what, (n,), torch.float32, dev)
     if bias is not None:
         _check_tensor(bias, "bias", what, (n,), torch.float32, dev)
-    out = torch.float16 if mode == 0 else torch.float32
     if y is None:
         _require(mode != 1, "%s: mode 1 adds into a given y" % what)
-        y = torch.empty((rows, n), dtype=out, device=dev)
+        y = x.new_empty((rows, n), dtype=torch.float16 if mode == 0 else torch.float32)
     else:
-        _check_tensor(y, "y", what, (rows, n), out, dev, True)
-    with _on_device(x):
-        _check(lib().mamba_linear_i8(x.data_ptr(), x.stride(0), x_scale.data_ptr(), w.data_ptr(), w.stride(0),
-                                     w_scale.data_ptr(), _ptr(bias), y.data_ptr(), y.stride(0), rows, n, k, mode,
-                                     _stream_of(x, stream)), "mamba_linear_i8")
+        _check_tensor(y, "y", what, (rows, n), torch.float16 if mode == 0 else torch.float32, dev, True)
+    _call(lib().mamba_linear_i8, what, x, x.data_ptr(), x.stride(0), x_scale.data_ptr(), w.data_ptr(),
+          w.stride(0), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr(), y.stride(0), rows, n,
+          k, mode)
     return y
 
 

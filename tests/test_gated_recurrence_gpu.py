@@ -344,3 +344,24 @@ def test_offsets_beyond_32_bits(cuda):
     out2 = torch.zeros(gap + L * D, dtype=torch.float16, device="cuda")
     grads = _backward(t, h, dx=view(out2))
     _check_backward(v, h.cpu().numpy(), grads, torch.float16)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_stream_argument(cuda, dtype):
+    """On a given stream (object or handle), what the helper allocates and
+    zeroes belongs to that stream: back-to-back calls from a busy current
+    stream do not disturb each other's scratch."""
+    v = _case(40, 4, 900, 128, dtype, ragged=True)
+    t = _dev(v)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    outs = []
+    for k in range(6):
+        s = side if k % 2 else side.cuda_stream
+        h, hN = _forward(t, stream=s)
+        outs.append((h, hN, _backward(t, h, stream=s)))
+        torch.full((1 << 22,), float("nan"), device="cuda")  # reuses whatever the current stream was given back
+    torch.cuda.synchronize()
+    for h, hN, grads in outs:
+        _check_forward(v, h, hN, dtype)
+        _check_backward(v, h.cpu().numpy(), grads, dtype)
