@@ -66,9 +66,9 @@ __device__ __forceinline__ float2 exp_neg(float2 v) {
 
 // A gate's preactivation, held where exp(-v) and its products stay finite:
 // sigmoid(-80) = 2e-35 and sigmoid(150) = 1 stand for what lies beyond.
-template <bool PRECISE>
+template <bool PRECISE, bool BELOW = true>
 __device__ __forceinline__ float2 clamp_gate(float2 v) {
-    v = make_float2(max_nan(v.x, -80.f), max_nan(v.y, -80.f));
+    if (BELOW) v = make_float2(max_nan(v.x, -80.f), max_nan(v.y, -80.f));
     if (PRECISE) v = make_float2(min_nan(v.x, 150.f), min_nan(v.y, 150.f));
     return v;
 }
@@ -107,7 +107,8 @@ __device__ __forceinline__ float2 rsqrt_pos(float2 m) {
 // sigmoid(r) and the decay y = csp sigmoid(r), a = exp(-y).
 template <bool PRECISE>
 __device__ __forceinline__ void decay(float2 r, float2 csp, float2 &e, float2 &s, float2 &y, float2 &a) {
-    e = exp_neg<PRECISE>(clamp_gate<PRECISE>(r));
+    // without PRECISE, exp(-r) = infinity just gives s = 0
+    e = exp_neg<PRECISE>(clamp_gate<PRECISE, PRECISE>(r));
     const float2 q = __fadd2_rn(e, both(1.f));
     s = make_float2(rcp_approx(q.x), rcp_approx(q.y));
     y = __fmul2_rn(csp, s);
@@ -126,11 +127,8 @@ __device__ __forceinline__ void forward_gates(float2 r, float2 i, float2 x, floa
     b = __fmul2_rn(__fmul2_rn(m, w), x);
 }
 
-// softplus(lambda): per channel.
-template <bool PRECISE>
-__device__ __forceinline__ float channel_softplus(float l) {
-    return PRECISE ? fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))) : softplus_fast(l);
-}
+// softplus(lambda), once per channel and call.
+__device__ __forceinline__ float channel_softplus(float l) { return fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))); }
 
 struct FwdParams {
     const void *x, *r, *i;
@@ -171,14 +169,14 @@ constexpr int kThreads = 128;
 // Step 2 crosses CTAs.  Tiles are handed out by an atomic ticket, time-major
 // (all rows' and channels' first tiles, then all second ones), so every tile
 // before a running one is running or done and waiting for it ends.  Tiles form
-// groups of kGroup: a tile publishes its map to the later tiles of its group,
-// and the group's last tile publishes the state leaving the group.  So the
-// serial chain over a long sequence has one hop per group, each tile composes
-// the same maps in the same order on every run (a scheme that takes whatever
-// state is ready first would not), and results repeat bit for bit.
+// groups: a tile publishes its map to the later tiles of its group, and the
+// group's last tile publishes the state leaving the group.  So the serial
+// chain over a long sequence has one hop per group, each tile composes the
+// same maps in the same order on every run (a scheme that takes whatever state
+// is ready first would not), and results repeat bit for bit.
 // A published value is one machine word that says itself whether it is there:
 // the workspace starts as all ones bits (a NaN that no published value has).
-constexpr int kGroup = 8;
+constexpr int max_group_shift(int vec) { return vec == 4 ? 3 : 4; }  // what shared memory has room for
 constexpr unsigned kErrRecurrenceTimeout = 64u;
 constexpr uint32_t kEmpty = 0xffffffffu;
 
@@ -271,6 +269,9 @@ struct MapRows {
 };
 
 template <int VEC>
+using GroupRows = MapRows<VEC, (1 << max_group_shift(VEC)) - 1>;
+
+template <int VEC>
 __device__ __forceinline__ void wait_maps(const float2 *slot, Pack<float, VEC> &P, Pack<float, VEC> &H) {
     Waiting wt;
     bool ready;
@@ -320,11 +321,12 @@ struct Divisor {
 
 struct Chains {
     unsigned int *ticket;
-    float2 *maps;    // [chains, tiles, channels of a tile]
-    float *states;   // [chains, groups, channels of a tile]
-    Divisor blocks;  // channel blocks of a row
-    Divisor chains;  // rows * blocks
-    int tiles, groups;
+    float2 *maps;      // [chains, tiles, channels of a tile]
+    float *states;     // [chains, groups, channels of a tile]
+    const float *csp;  // [dim] c * softplus(lambda)
+    Divisor blocks;    // channel blocks of a row
+    Divisor chains;    // rows * blocks
+    int tiles, groups, group, group_shift;  // tiles of a chain, in groups of `group` = 1 << group_shift
 };
 
 // Hands out tickets one ahead: next() gives the ticket drawn by the call
@@ -348,7 +350,7 @@ struct Tickets {
 
 // What a ticket stands for: time-major, all chains' k-th tiles together.
 struct Tile {
-    int chain, k, b, d, n, t0, cnt;
+    int chain, k, g, j, b, d, n, t0, cnt;  // tile k of its chain is tile j of group g
     bool live, in;
 };
 template <int VEC>
@@ -357,6 +359,8 @@ __device__ __forceinline__ Tile place_tile(const Chains &c, const FwdParams &p, 
     unsigned chain, block;
     t.k = (int)c.chains.divide(v, chain);
     t.chain = (int)chain;
+    t.g = t.k >> c.group_shift;
+    t.j = t.k - (t.g << c.group_shift);
     t.b = (int)c.blocks.divide(chain, block);
     t.d = ((int)block * 32 + (threadIdx.x & 31)) * VEC;
     t.in = t.d < p.D;
@@ -369,18 +373,14 @@ __device__ __forceinline__ Tile place_tile(const Chains &c, const FwdParams &p, 
 // between them; `wm` holds the maps of this tile's warps.  Syncs the CTA.
 template <int VEC, int W>
 __device__ __forceinline__ Maps<VEC> prefix_maps(const Chains &c, const Tile &t, const MapRows<VEC, W> &wm,
-                                                 MapRows<VEC, kGroup - 1> &gm) {
+                                                 GroupRows<VEC> &gm) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int j = t.k % kGroup;
-#pragma unroll
-    for (int q = 0; q < (kGroup - 1 + W - 1) / W; ++q) {
-        const int tile = warp + q * W;
-        if (tile < j) {
-            Pack<float, VEC> P, H;
-            wait_maps<VEC>(c.maps + ((int64_t)t.chain * c.tiles + t.k - j + tile) * (32 * VEC) + lane * VEC, P, H);
-            gm.P[tile][lane] = P;
-            gm.H[tile][lane] = H;
-        }
+    const int j = t.j;
+    for (int tile = warp; tile < j; tile += W) {
+        Pack<float, VEC> P, H;
+        wait_maps<VEC>(c.maps + ((int64_t)t.chain * c.tiles + t.k - j + tile) * (32 * VEC) + lane * VEC, P, H);
+        gm.P[tile][lane] = P;
+        gm.H[tile][lane] = H;
     }
     __syncthreads();
     Maps<VEC> m;
@@ -395,13 +395,12 @@ __device__ __forceinline__ Maps<VEC> prefix_maps(const Chains &c, const Tile &t,
 // state on without another barrier.
 template <int VEC>
 __device__ __forceinline__ void group_state(const Chains &c, const Tile &t, float (&s)[VEC]) {
-    const int g = t.k / kGroup;
-    if (g > 0)
-        wait_states<VEC>(c.states + ((int64_t)t.chain * c.groups + g - 1) * (32 * VEC) + (threadIdx.x & 31) * VEC, s);
+    if (t.g > 0)
+        wait_states<VEC>(c.states + ((int64_t)t.chain * c.groups + t.g - 1) * (32 * VEC) + (threadIdx.x & 31) * VEC, s);
 }
 template <int VEC>
 __device__ __forceinline__ void leave_group(const Chains &c, const Tile &t, const float (&h)[VEC]) {
-    float *slot = c.states + ((int64_t)t.chain * c.groups + t.k / kGroup) * (32 * VEC) + (threadIdx.x & 31) * VEC;
+    float *slot = c.states + ((int64_t)t.chain * c.groups + t.g) * (32 * VEC) + (threadIdx.x & 31) * VEC;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) put_state(slot + e, h[e]);
 }
@@ -466,7 +465,7 @@ template <typename T, int VEC, int S, int W>
 struct FwdSmem {
     Pack<T, VEC> in[3][S][32 * W];
     MapRows<VEC, W> wm;
-    MapRows<VEC, kGroup - 1> gm;
+    GroupRows<VEC> gm;
     unsigned int ticket[2];
 };
 
@@ -514,7 +513,7 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
         if (t.live) {
             float csp[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) csp[e] = t.in ? p.c * channel_softplus<PRECISE>(p.lambda[t.d + e]) : 0.f;
+            for (int e = 0; e < VEC; ++e) csp[e] = t.in ? ch.csp[t.d + e] : 0.f;
             Pack<T, VEC> r[S], gi[S], x[S];
 #pragma unroll
             for (int j = 0; j < S; ++j) {
@@ -558,13 +557,13 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
             sm.wm.H[warp][lane] = own.H;
             __syncthreads();
             const bool more = (t.k + 1) * TT < t.n;  // a later tile waits for this one
-            const bool last = t.k % kGroup == kGroup - 1;
+            const bool last = t.j == ch.group - 1;
             if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, sm.wm);
             Maps<VEC> m = prefix_maps<VEC, W>(ch, t, sm.wm, sm.gm);
             float s[VEC], h[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
-                s[e] = t.in && p.h0 && t.k < kGroup ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
+                s[e] = t.in && p.h0 && t.g == 0 ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
             group_state<VEC>(ch, t, s);
             if (warp == W - 1 && (last || !more)) {
                 Maps<VEC> end = m;
@@ -598,13 +597,16 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
 
 // ---- backward -------------------------------------------------------------------
 // The same tiles and chains with time reversed; what runs along a chain is
-// C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.  x, i
-// and h are needed after the wait, so two buffers take turns.
+// C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.  The
+// next tile's copies start as soon as a buffer is read for the last time: those
+// of r and dh once the tile's map is computed, the others' behind the
+// gradients.  Across the wait a thread keeps sigmoid(r) and dh; the decay is
+// computed again (one exponential) rather than held.
 template <typename T, int VEC, int S, int W>
 struct BwdSmem {
-    Pack<T, VEC> in[2][5][S][32 * W];
+    Pack<T, VEC> in[5][S][32 * W];
     MapRows<VEC, W> wm;
-    MapRows<VEC, kGroup - 1> gm;
+    GroupRows<VEC> gm;
     Pack<float, VEC> sums[W][32];
     unsigned int ticket[2];
 };
@@ -627,86 +629,98 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
         t.cnt = t.in && t.live ? min(max(t.n - t.t0, 0), S) : 0;
         return t;
     };
-    auto fetch = [&](const Tile &t, int buf) {
+    // each commits one group of copies, also where there is nothing to copy
+    auto fetch_first = [&](const Tile &t, bool any) {
         const T *pr = static_cast<const T *>(f.r) + t.b * f.sr[0] + t.t0 * f.sr[1] + t.d;
         const T *pg = static_cast<const T *>(p.dh) + t.b * p.sdh[0] + t.t0 * p.sdh[1] + t.d;
+        if (any)
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                if (j < t.cnt) {
+                    copy_pack<T, VEC>(&sm.in[0][j][tid], pr + j * f.sr[1]);
+                    copy_pack<T, VEC>(&sm.in[1][j][tid], pg + j * p.sdh[1]);
+                }
+        copy_commit();
+    };
+    auto fetch_rest = [&](const Tile &t, bool any) {
         const T *px = static_cast<const T *>(f.x) + t.b * f.sx[0] + t.t0 * f.sx[1] + t.d;
         const T *pi = static_cast<const T *>(f.i) + t.b * f.si[0] + t.t0 * f.si[1] + t.d;
         const T *ph = static_cast<const T *>(f.h) + t.b * f.sh[0] + (t.t0 - 1) * f.sh[1] + t.d;
+        if (any)
 #pragma unroll
-        for (int j = 0; j < S; ++j)
-            if (j < t.cnt) {
-                copy_pack<T, VEC>(&sm.in[buf][0][j][tid], pr + j * f.sr[1]);
-                copy_pack<T, VEC>(&sm.in[buf][1][j][tid], pg + j * p.sdh[1]);
-                copy_pack<T, VEC>(&sm.in[buf][2][j][tid], px + j * f.sx[1]);
-                copy_pack<T, VEC>(&sm.in[buf][3][j][tid], pi + j * f.si[1]);
-                if (t.t0 + j > 0) copy_pack<T, VEC>(&sm.in[buf][4][j][tid], ph + j * f.sh[1]);
-            }
+            for (int j = 0; j < S; ++j)
+                if (j < t.cnt) {
+                    copy_pack<T, VEC>(&sm.in[2][j][tid], px + j * f.sx[1]);
+                    copy_pack<T, VEC>(&sm.in[3][j][tid], pi + j * f.si[1]);
+                    if (t.t0 + j > 0) copy_pack<T, VEC>(&sm.in[4][j][tid], ph + j * f.sh[1]);
+                }
+        copy_commit();
     };
 
     Tickets tickets(ch.ticket, sm.ticket);
     unsigned v = tickets.next();
     if (v >= total) return;
     Tile t = place(v);
-    fetch(t, 0);
-    copy_commit();
-    for (int buf = 0;; buf ^= 1) {
+    fetch_first(t, true);
+    fetch_rest(t, true);
+    for (;;) {
         const unsigned vn = tickets.next();  // its barrier also frees sm.wm, sm.gm and sm.sums
         Tile tn{};
-        if (vn < total) {
-            tn = place(vn);
-            fetch(tn, buf ^ 1);
-        }
-        copy_commit();
-        copy_wait<1>();
+        if (vn < total) tn = place(vn);
+        copy_wait<1>();  // r and dh are there
         float *part = p.part + ((int64_t)t.b * ch.tiles + t.k) * f.D + t.d;
         if (t.live) {
-            float2 a[NP], sg[NP], om[PRECISE ? NP : 1];
+            float2 sg[NP], om[PRECISE ? NP : 1];
             float csp[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) csp[e] = t.in ? f.c * channel_softplus<PRECISE>(f.lambda[t.d + e]) : 0.f;
-            Pack<T, VEC> dh[S];
-            {
-                Pack<T, VEC> r[S];
-#pragma unroll
-                for (int j = 0; j < S; ++j) {
-                    r[j] = sm.in[buf][0][j][tid];
-                    dh[j] = sm.in[buf][1][j][tid];
-                }
-#pragma unroll
-                for (int q = 0; q < NP; ++q) {
-                    float2 e, y;
-                    decay<PRECISE>(pair_of<T, VEC, S>(r, q), channel_pair<VEC>(csp, q), e, sg[q], y, a[q]);
-                    if (PRECISE) om[q] = __fmul2_rn(e, sg[q]);
-                }
-            }
+            for (int e = 0; e < VEC; ++e) csp[e] = t.in ? ch.csp[t.d + e] : 0.f;
             const uint32_t cut = cut_mask(f, t.b, t.t0, min(max(t.n - t.t0, 0), S));
+            Pack<T, VEC> dh[S];
             Maps<VEC> own;
             own.identity();
+            constexpr int TP = VEC == 1 ? 2 : 1;  // tokens whose pairs are computed together
 #pragma unroll
-            for (int j = S - 1; j >= 0; --j)
-                if (j < t.cnt) {  // what the buffer holds behind the end does not count
-                    Pack<float, VEC> P, H;
-                    const float keep = cut >> j & 1 ? 0.f : 1.f;
+            for (int j0 = S - TP; j0 >= 0; j0 -= TP) {
+                float2 a[TP * VEC / 2];
+                Pack<T, VEC> r[TP];
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const int k = j * VEC + e;
-                        P.v[e] = half_of(a[k / 2], k) * keep;
-                        H.v[e] = P.v[e] * cvt_f32(dh[j].v[e]);
-                    }
-                    own.then(P, H);
+                for (int u = 0; u < TP; ++u) {
+                    r[u] = sm.in[0][j0 + u][tid];
+                    dh[j0 + u] = sm.in[1][j0 + u][tid];
                 }
+#pragma unroll
+                for (int z = 0; z < TP * VEC / 2; ++z) {
+                    const int q = j0 * VEC / 2 + z;
+                    float2 e, y;
+                    decay<PRECISE>(pair_of<T, VEC, TP>(r, z), channel_pair<VEC>(csp, z), e, sg[q], y, a[z]);
+                    if (PRECISE) om[q] = __fmul2_rn(e, sg[q]);
+                }
+#pragma unroll
+                for (int u = TP - 1; u >= 0; --u)
+                    if (j0 + u < t.cnt) {  // what the buffer holds behind the end does not count
+                        Pack<float, VEC> P, H;
+                        const float keep = cut >> (j0 + u) & 1 ? 0.f : 1.f;
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) {
+                            const int k = u * VEC + e;
+                            P.v[e] = half_of(a[k / 2], k) * keep;
+                            H.v[e] = P.v[e] * cvt_f32(dh[j0 + u].v[e]);
+                        }
+                        own.then(P, H);
+                    }
+            }
+            fetch_first(tn, vn < total);
             sm.wm.P[warp][lane] = own.P;
             sm.wm.H[warp][lane] = own.H;
             __syncthreads();
             const bool more = t.t0 - (W - 1 - warp) * S > 0;  // an earlier tile waits for this one
-            const bool last = t.k % kGroup == kGroup - 1;
+            const bool last = t.j == ch.group - 1;
             if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, sm.wm);
             Maps<VEC> m = prefix_maps<VEC, W>(ch, t, sm.wm, sm.gm);
             float s[VEC], C[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
-                s[e] = t.in && p.dhN && t.k < kGroup ? p.dhN[(int64_t)t.b * f.D + t.d + e] : 0.f;
+                s[e] = t.in && p.dhN && t.g == 0 ? p.dhN[(int64_t)t.b * f.D + t.d + e] : 0.f;
             group_state<VEC>(ch, t, s);
             if (warp == W - 1 && (last || !more)) {
                 Maps<VEC> end = m;
@@ -720,33 +734,37 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
             }
             m.apply(s, C);
 
-            // G = dh + C of every element, then everything else in pairs
-            float2 G[NP];
-#pragma unroll
-            for (int j = S - 1; j >= 0; --j) {
-                const float keep = cut >> j & 1 ? 0.f : 1.f;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int k = j * VEC + e;
-                    const float g = cvt_f32(dh[j].v[e]) + C[e];
-                    half_of(G[k / 2], k) = g;
-                    if (j < t.cnt) C[e] = half_of(a[k / 2], k) * keep * g;
-                }
-            }
+            copy_wait<1>();  // x, i and h are there
             T *qx = static_cast<T *>(p.dx) + t.b * p.sdx[0] + t.t0 * p.sdx[1] + t.d;
             T *qr = static_cast<T *>(p.dr) + t.b * p.sdr[0] + t.t0 * p.sdr[1] + t.d;
             T *qi = static_cast<T *>(p.di) + t.b * p.sdi[0] + t.t0 * p.sdi[1] + t.d;
             float sum[VEC] = {};
-            constexpr int TP = VEC == 1 ? 2 : 1;  // tokens whose pairs are computed together
 #pragma unroll
             for (int j0 = S - TP; j0 >= 0; j0 -= TP) {
                 if (j0 >= t.cnt) continue;
                 Pack<T, VEC> x[TP], gi[TP], hp[TP], ox[TP], orr[TP], oi[TP];
+                float2 a[TP * VEC / 2], y[TP * VEC / 2], G[TP * VEC / 2];  // G = dh + C
+#pragma unroll
+                for (int z = 0; z < TP * VEC / 2; ++z) {
+                    y[z] = __fmul2_rn(channel_pair<VEC>(csp, z), sg[j0 * VEC / 2 + z]);
+                    a[z] = exp_neg<PRECISE>(y[z]);
+                }
+#pragma unroll
+                for (int u = TP - 1; u >= 0; --u) {
+                    const float keep = cut >> (j0 + u) & 1 ? 0.f : 1.f;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const int k = u * VEC + e;
+                        const float g = cvt_f32(dh[j0 + u].v[e]) + C[e];
+                        half_of(G[k / 2], k) = g;
+                        if (j0 + u < t.cnt) C[e] = half_of(a[k / 2], k) * keep * g;
+                    }
+                }
 #pragma unroll
                 for (int u = 0; u < TP; ++u) {
-                    x[u] = sm.in[buf][2][j0 + u][tid];
-                    gi[u] = sm.in[buf][3][j0 + u][tid];
-                    hp[u] = sm.in[buf][4][j0 + u][tid];
+                    x[u] = sm.in[2][j0 + u][tid];
+                    gi[u] = sm.in[3][j0 + u][tid];
+                    hp[u] = sm.in[4][j0 + u][tid];
                 }
 #pragma unroll
                 for (int u = 0; u < TP; ++u) {
@@ -757,7 +775,7 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
 #pragma unroll
                 for (int z = 0; z < TP * VEC / 2; ++z) {
                     const int q = j0 * VEC / 2 + z;
-                    const float2 xv = pair_of<T, VEC, TP>(x, z), av = a[q], y = __fmul2_rn(channel_pair<VEC>(csp, z), sg[q]);
+                    const float2 xv = pair_of<T, VEC, TP>(x, z), av = a[z];
                     float2 prev = pair_of<T, VEC, TP>(hp, z);
                     if (t.t0 + j0 == 0 && f.h0 && !(cut >> j0 & 1)) {  // h_{-1}, in FP32
                         prev.x = f.h0[(int64_t)t.b * f.D + t.d + (2 * z) % VEC];
@@ -766,13 +784,13 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                     const float2 ei = exp_neg<PRECISE>(clamp_gate<PRECISE>(pair_of<T, VEC, TP>(gi, z)));
                     const float2 qi = __fadd2_rn(ei, both(1.f));
                     const float2 si = make_float2(rcp_approx(qi.x), rcp_approx(qi.y));
-                    const float2 m2 = one_minus_a2<PRECISE>(y, av), w = rsqrt_pos(m2);
-                    const float2 gs2 = __fmul2_rn(G[q], si);                      // G sigmoid(i)
+                    const float2 m2 = one_minus_a2<PRECISE>(y[z], av), w = rsqrt_pos(m2);
+                    const float2 gs2 = __fmul2_rn(G[z], si);                      // G sigmoid(i)
                     const float2 gx = __fmul2_rn(gs2, __fmul2_rn(m2, w));         // * sqrt(m)
                     const float2 gi2 = __fmul2_rn(__fmul2_rn(gx, xv), __fmul2_rn(ei, si));
                     // E = a (G si x a (y / sqrt(m)) - y G h_{t-1}); y / sqrt(m) first, it tends to 0
-                    const float2 u1 = __fmul2_rn(__fmul2_rn(gs2, xv), __fmul2_rn(av, __fmul2_rn(y, w)));
-                    const float2 u2 = __ffma2_rn(__fmul2_rn(__fmul2_rn(y, both(-1.f)), G[q]), prev, u1);
+                    const float2 u1 = __fmul2_rn(__fmul2_rn(gs2, xv), __fmul2_rn(av, __fmul2_rn(y[z], w)));
+                    const float2 u2 = __ffma2_rn(__fmul2_rn(__fmul2_rn(y[z], both(-1.f)), G[z]), prev, u1);
                     const float2 E = __fmul2_rn(av, u2);
                     const float2 os = PRECISE ? om[PRECISE ? q : 0] : __ffma2_rn(sg[q], both(-1.f), both(1.f));
                     const float2 gr = __fmul2_rn(E, os);
@@ -794,6 +812,7 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                         *reinterpret_cast<Pack<T, VEC> *>(qr + j * p.sdr[1]) = orr[u];
                     }
             }
+            fetch_rest(tn, vn < total);
             // the tile's sum of E per channel, warps in order
 #pragma unroll
             for (int e = 0; e < VEC; ++e) sm.sums[warp][lane].v[e] = sum[e];
@@ -806,9 +825,12 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                     for (int w = 0; w < W; ++w) z += sm.sums[w][lane].v[e];
                     part[e] = z;
                 }
-        } else if (warp == 0 && t.in) {  // behind the row's end
+        } else {  // behind the row's end
+            if (warp == 0 && t.in)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) part[e] = 0.f;
+                for (int e = 0; e < VEC; ++e) part[e] = 0.f;
+            fetch_first(tn, vn < total);
+            fetch_rest(tn, vn < total);
         }
         if (vn >= total) break;
         t = tn;
@@ -833,7 +855,7 @@ __global__ void __launch_bounds__(32 * kSumWarps)
 #pragma unroll
         for (int w = 1; w < kSumWarps; ++w) s += sm[w][lane];
         const float l = lambda[d];
-        dlambda[d] = s * (l < -20.f ? 1.f : 1.f / (1.f + expf(-l)) / channel_softplus<true>(l));
+        dlambda[d] = s * (l < -20.f ? 1.f : 1.f / (1.f + expf(-l)) / channel_softplus(l));
     }
 }
 
@@ -857,7 +879,7 @@ __global__ void __launch_bounds__(kThreads) recurrence_step_kernel(const StepPar
     if (d >= p.D) return;
     float csp[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) csp[e] = p.c * channel_softplus<PRECISE>(p.lambda[d + e]);
+    for (int e = 0; e < VEC; ++e) csp[e] = p.c * channel_softplus(p.lambda[d + e]);
     const int64_t b0 = (int64_t)blockIdx.y * p.rows, b1 = min(b0 + p.rows, (int64_t)p.B);
 #pragma unroll 4
     for (int64_t b = b0; b < b1; ++b) {
@@ -949,13 +971,13 @@ struct FwdShape {
 };
 template <typename T>
 struct BwdShape {
-    static constexpr int VEC = sizeof(T) == 2 ? 4 : 2, S = 4, W = 8, CTAS = 2;
+    static constexpr int VEC = sizeof(T) == 2 ? 4 : 2, S = 8, W = 4, CTAS = 4;
 };
 
 // The chains of a call and where its workspace holds what.
 struct Plan {
     Chains ch;
-    size_t bytes, part_bytes;
+    size_t bytes, csp_bytes, part_bytes, ones_bytes;
 };
 bool plan_chains(const MambaRecurrenceArgs *a, bool backward, int vec, Plan &pl) {
     const bool half = a->dtype == MAMBA_F16;
@@ -972,10 +994,17 @@ bool plan_chains(const MambaRecurrenceArgs *a, bool backward, int vec, Plan &pl)
     c.blocks = divisor(blocks);
     c.chains = divisor(blocks * a->batch);
     c.tiles = (int)tiles;
-    c.groups = (int)ceil_div64(tiles, kGroup);
-    pl.bytes = 256 + (size_t)c.chains.d * cw * (tiles * sizeof(float2) + c.groups * sizeof(float));
-    if (tiles == 1) pl.bytes = 256;
-    pl.part_bytes = backward ? ((size_t)a->batch * tiles * a->dim * sizeof(float) + 15) / 16 * 16 : 0;
+    c.group_shift = std::min(max_group_shift(vec), tiles <= 128 ? 2 : tiles <= 1024 ? 3 : 4);
+    c.group = 1 << c.group_shift;
+    c.groups = ceil_div((int)tiles, c.group);
+    // csp, the backward's partial sums, then what starts as all ones bits:
+    // the ticket, the maps and the states (a multiple of 16 bytes: cw is 32 at least)
+    auto up = [](size_t v) { return (v + 15) / 16 * 16; };
+    pl.csp_bytes = up((size_t)a->dim * sizeof(float));
+    pl.part_bytes = backward ? up((size_t)a->batch * tiles * a->dim * sizeof(float)) : 0;
+    pl.ones_bytes = 256;
+    if (tiles > 1) pl.ones_bytes += (size_t)c.chains.d * cw * (tiles * sizeof(float2) + c.groups * sizeof(float));
+    pl.bytes = pl.csp_bytes + pl.part_bytes + pl.ones_bytes;
     return true;
 }
 
@@ -989,7 +1018,7 @@ size_t recurrence_workspace_bytes(const MambaRecurrenceArgs *a, bool backward) {
     for (int vec : {1, 2, 4}) {
         Plan pl;
         if (!plan_chains(a, backward, vec, pl)) return 0;
-        need = std::max(need, pl.bytes + pl.part_bytes);
+        need = std::max(need, pl.bytes);
     }
     return need;
 }
@@ -1011,20 +1040,35 @@ int allow_smem(Kernel kernel, size_t bytes) {
     return 0;
 }
 
-// Launches one variant: the workspace's part from the ticket on set to all
-// ones bits, then persistent CTAs.
+// Prepares the workspace: c * softplus(lambda) per channel, and all ones bits
+// from the ticket on.
+__global__ void __launch_bounds__(256)
+    recurrence_init_kernel(const float *__restrict__ lambda, float c, int D, float *__restrict__ csp,
+                           uint4 *__restrict__ ones, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, stride = (int64_t)gridDim.x * 256;
+    for (int64_t d = i; d < D; d += stride) csp[d] = c * channel_softplus(lambda[d]);
+    for (int64_t k = i; k < n; k += stride) ones[k] = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
+}
+
+// Launches one variant: the workspace's preparation, then persistent CTAs.
 template <int VEC, typename Kernel, typename Params>
-int launch_tiles(Kernel kernel, const Params &p, Plan &pl, int threads, int ctas, size_t smem, void *ws,
-                 cudaStream_t st, const char *what) {
+int launch_tiles(Kernel kernel, const Params &p, const FwdParams &f, Plan &pl, int threads, int ctas, size_t smem,
+                 void *ws, cudaStream_t st, const char *what) {
     Chains &c = pl.ch;
-    uint8_t *base = static_cast<uint8_t *>(ws) + pl.part_bytes;
+    uint8_t *base = static_cast<uint8_t *>(ws);
+    float *csp = reinterpret_cast<float *>(base);
+    base += pl.csp_bytes + pl.part_bytes;
+    c.csp = csp;
     c.ticket = reinterpret_cast<unsigned int *>(base);
     c.maps = reinterpret_cast<float2 *>(base + 256);
     c.states = reinterpret_cast<float *>(c.maps + (int64_t)c.chains.d * c.tiles * 32 * VEC);
     if (allow_smem(kernel, smem)) return -1;
-    MB_CUDA_TRY(cudaMemsetAsync(base, 0xff, pl.bytes, st));
-    const int64_t total = (int64_t)c.chains.d * c.tiles, most = (int64_t)ctas * device_sm_count();
-    kernel<<<(unsigned)std::min(total, most), threads, smem, st>>>(p, c);
+    const int64_t ones = (int64_t)pl.ones_bytes / 16, sms = device_sm_count();
+    const int64_t init = std::min<int64_t>(8 * sms, std::max<int64_t>(ceil_div64(ones, 1024), ceil_div64(f.D, 256)));
+    recurrence_init_kernel<<<(unsigned)init, 256, 0, st>>>(f.lambda, f.c, f.D, csp, reinterpret_cast<uint4 *>(base),
+                                                           ones);
+    if (launch_status(what)) return -1;
+    kernel<<<(unsigned)std::min((int64_t)c.chains.d * c.tiles, ctas * sms), threads, smem, st>>>(p, c);
     return launch_status(what);
 }
 
@@ -1033,7 +1077,8 @@ int launch_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
     Plan pl;
     MB_CHECK_ARG(plan_chains(a, false, VEC, pl), "gated_recurrence: too many tiles");
     using F = FwdShape<T>;
-    return launch_tiles<VEC>(recurrence_fwd_kernel<T, VEC, F::S, F::W, F::CTAS>, fwd_params(a), pl, 32 * F::W, F::CTAS,
+    const FwdParams p = fwd_params(a);
+    return launch_tiles<VEC>(recurrence_fwd_kernel<T, VEC, F::S, F::W, F::CTAS>, p, p, pl, 32 * F::W, F::CTAS,
                              sizeof(FwdSmem<T, VEC, F::S, F::W>), ws, st, "gated_recurrence kernel");
 }
 template <typename T>
@@ -1049,8 +1094,9 @@ int launch_backward(const MambaRecurrenceArgs *a, BwdParams &p, void *ws, cudaSt
     Plan pl;
     MB_CHECK_ARG(plan_chains(a, true, VEC, pl), "gated_recurrence_backward: too many tiles");
     tiles = pl.ch.tiles;
+    p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + pl.csp_bytes);
     using F = BwdShape<T>;
-    return launch_tiles<VEC>(recurrence_bwd_kernel<T, VEC, F::S, F::W, F::CTAS>, p, pl, 32 * F::W, F::CTAS,
+    return launch_tiles<VEC>(recurrence_bwd_kernel<T, VEC, F::S, F::W, F::CTAS>, p, p.f, pl, 32 * F::W, F::CTAS,
                              sizeof(BwdSmem<T, VEC, F::S, F::W>), ws, st, "gated_recurrence_backward kernel");
 }
 template <typename T>
@@ -1111,7 +1157,6 @@ int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads
     p.dr = g->dr;
     p.di = g->di;
     p.dh0 = g->dinitial_state;
-    p.part = static_cast<float *>(ws);
     for (int k = 0; k < 2; ++k) {
         p.sdh[k] = g->dh_stride[k];
         p.sdx[k] = g->dx_stride[k];
