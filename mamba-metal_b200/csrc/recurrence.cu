@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -74,10 +75,13 @@ __device__ __forceinline__ float2 clamp_gate(float2 v) {
 }
 
 // 1 - a^2 for a = exp(-y), without cancellation for y near 0: a series in
-// z = 2y below a border, (1 - a)(1 + a) above it, where a's error of 2^-22
-// has lost its weight.  PRECISE: Taylor to z^7 below y = 1/4 (relative
-// error < (1/2)^8 / 9! = 1e-8; above, 2^-22 / (1 - e^-1/2) * e^-1/2).  Else to
-// z^2 below y = 0.03 (error < y^3 / 3 = 9e-6; above, 7e-6).
+// z = 2y for small y, (1 - a)(1 + a) where a's error of 2^-22 has lost its
+// weight.  PRECISE: Taylor to z^8 below y = 1/4 (relative error < (1/2)^8 / 9! =
+// 1e-8; above, 2^-22 e^-1/2 / (1 - e^-1/2)).  Else z - z^2/2 + z^3/6, which is
+// z^4/24 too large, and the other form with 2.4e-7 added to its first factor,
+// which makes it too large also where a's rounding works against it: the
+// smaller of the two is right to 2.5e-5 everywhere (worst where they meet, near
+// z = 0.06) and to z^3/24 below.
 template <bool PRECISE>
 __device__ __forceinline__ float2 one_minus_a2(float2 y, float2 a) {
     const float2 z = __fadd2_rn(y, y);
@@ -94,15 +98,13 @@ __device__ __forceinline__ float2 one_minus_a2(float2 y, float2 a) {
     q = __ffma2_rn(z, q, both(-0.5f));
     q = __ffma2_rn(z, q, both(1.f));
     q = __fmul2_rn(z, q);
-    const float2 d = __ffma2_rn(a, both(-1.f), both(1.f)), w = __ffma2_rn(a, d, d);
-    constexpr float border = PRECISE ? 0.25f : 0.03f;
-    return make_float2(y.x < border ? q.x : w.x, y.y < border ? q.y : w.y);
+    const float2 d = __ffma2_rn(a, both(-1.f), both(PRECISE ? 1.f : 1.f + 2.4e-7f)), w = __ffma2_rn(a, d, d);
+    if (!PRECISE) return make_float2(fminf(q.x, w.x), fminf(q.y, w.y));
+    return make_float2(y.x < 0.25f ? q.x : w.x, y.y < 0.25f ? q.y : w.y);
 }
 
-// 1 / sqrt(m), finite for m = 0 (m * the result is then 0, as it should be).
-__device__ __forceinline__ float2 rsqrt_pos(float2 m) {
-    return make_float2(rsqrt_approx(max_nan(m.x, 1e-37f)), rsqrt_approx(max_nan(m.y, 1e-37f)));
-}
+// 1 / sqrt(m + 1e-37): finite for m = 0, where m times it is 0 as it should be.
+constexpr float kTiny = 1e-37f;
 
 // sigmoid(r) and the decay y = csp sigmoid(r), a = exp(-y).
 template <bool PRECISE>
@@ -123,8 +125,8 @@ __device__ __forceinline__ void forward_gates(float2 r, float2 i, float2 x, floa
     decay<PRECISE>(r, csp, e, s, y, a);
     const float2 m = one_minus_a2<PRECISE>(y, a);
     const float2 q = __fadd2_rn(exp_neg<PRECISE>(clamp_gate<PRECISE>(i)), both(1.f));
-    const float2 w = rsqrt_pos(__fmul2_rn(__fmul2_rn(m, q), q));
-    b = __fmul2_rn(__fmul2_rn(m, w), x);
+    const float2 t = __ffma2_rn(__fmul2_rn(m, q), q, both(kTiny));
+    b = __fmul2_rn(__fmul2_rn(m, make_float2(rsqrt_approx(t.x), rsqrt_approx(t.y))), x);
 }
 
 // softplus(lambda), once per channel and call.
@@ -269,9 +271,6 @@ struct MapRows {
 };
 
 template <int VEC>
-using GroupRows = MapRows<VEC, (1 << max_group_shift(VEC)) - 1>;
-
-template <int VEC>
 __device__ __forceinline__ void wait_maps(const float2 *slot, Pack<float, VEC> &P, Pack<float, VEC> &H) {
     Waiting wt;
     bool ready;
@@ -336,7 +335,7 @@ struct Tickets {
     unsigned int *counter, *shared;  // shared: two places, used in turn
     unsigned int ahead = 0, turn = 0;
     __device__ __forceinline__ Tickets(unsigned int *c, unsigned int *s) : counter(c), shared(s) {
-        if (threadIdx.x == 0) ahead = atomicAdd(counter, 1u) + 1u;  // the counter starts as all ones bits
+        if (c && threadIdx.x == 0) ahead = atomicAdd(counter, 1u) + 1u;  // the counter starts as all ones bits
     }
     __device__ __forceinline__ unsigned int next() {
         turn ^= 1;
@@ -373,7 +372,7 @@ __device__ __forceinline__ Tile place_tile(const Chains &c, const FwdParams &p, 
 // between them; `wm` holds the maps of this tile's warps.  Syncs the CTA.
 template <int VEC, int W>
 __device__ __forceinline__ Maps<VEC> prefix_maps(const Chains &c, const Tile &t, const MapRows<VEC, W> &wm,
-                                                 GroupRows<VEC> &gm) {
+                                                 MapRows<VEC, (1 << max_group_shift(VEC)) - 1> &gm) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int j = t.j;
     for (int tile = warp; tile < j; tile += W) {
@@ -416,6 +415,22 @@ __device__ __forceinline__ void publish_map(const Chains &c, const Tile &t, cons
     float2 *slot = c.maps + ((int64_t)t.chain * c.tiles + t.k) * (32 * VEC) + lane * VEC;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) put_map(slot + e, m.P.v[e], m.H.v[e]);
+}
+
+// WALK: the state entering this warp's tokens (h) and the state leaving the
+// tile (s) from the state entering it (s), through the maps of the tile's warps.
+template <int VEC, int W>
+__device__ __forceinline__ void walk_state(const MapRows<VEC, W> &wm, float (&s)[VEC], float (&h)[VEC]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const Pack<float, VEC> P = wm.P[w][lane], H = wm.H[w][lane];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            if (w == warp) h[e] = s[e];
+            s[e] = fmaf(P.v[e], s[e], H.v[e]);
+        }
+    }
 }
 
 // Which of this warp's tokens cut the state.
@@ -461,20 +476,24 @@ __device__ __forceinline__ float &half_of(float2 &v, int k) { return k & 1 ? v.y
 // tile's x, r and i into shared memory start, and run while this tile waits
 // for its state and writes h.  A thread reads back only what it copied
 // itself, so no barrier guards the buffer.
-template <typename T, int VEC, int S, int W>
+//
+// With enough chains to fill the GPU (walks()), a CTA walks one chain from its
+// first tile to its last instead (WALK): no tickets, nothing published, the
+// state stays in registers.
+template <typename T, int VEC, int S, int W, bool WALK>
 struct FwdSmem {
     Pack<T, VEC> in[3][S][32 * W];
-    MapRows<VEC, W> wm;
-    GroupRows<VEC> gm;
+    MapRows<VEC, W> wm[WALK ? 2 : 1];
+    MapRows<VEC, WALK ? 1 : (1 << max_group_shift(VEC)) - 1> gm;
     unsigned int ticket[2];
 };
 
-template <typename T, int VEC, int S, int W, int CTAS>
+template <typename T, int VEC, int S, int W, int CTAS, bool WALK>
 __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdParams p, const Chains ch) {
     constexpr bool PRECISE = sizeof(T) == 4;
     constexpr int TT = S * W, NP = S * VEC / 2;
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    auto &sm = *reinterpret_cast<FwdSmem<T, VEC, S, W> *>(smem_raw);
+    auto &sm = *reinterpret_cast<FwdSmem<T, VEC, S, W, WALK> *>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned total = ch.chains.d * (unsigned)ch.tiles;
 
@@ -499,21 +518,38 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
         copy_commit();
     };
 
-    Tickets tickets(ch.ticket, sm.ticket);
-    unsigned v = tickets.next();
+    Tickets tickets(WALK ? nullptr : ch.ticket, sm.ticket);
+    unsigned v = WALK ? blockIdx.x : tickets.next();
     if (v >= total) return;
     Tile t = place(v);
     fetch(t);
+    float csp[VEC], s[VEC];
+    if (WALK) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            csp[e] = t.in ? p.c * channel_softplus(p.lambda[t.d + e]) : 0.f;
+            s[e] = t.in && p.h0 ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
+        }
+    }
     for (;;) {
-        const unsigned vn = tickets.next();  // its barrier also frees sm.wm and sm.gm
-        Tile tn{};
-        if (vn < total) tn = place(vn);
+        Tile tn = t;
+        bool next;
+        if (WALK) {
+            ++tn.k;
+            tn.t0 += TT;
+            tn.cnt = t.in ? min(max(t.n - tn.t0, 0), S) : 0;
+            next = tn.k * TT < t.n;
+        } else {
+            v = tickets.next();  // its barrier also frees sm.wm and sm.gm
+            next = v < total;
+            if (next) tn = place(v);
+        }
         copy_wait<0>();
         float2 a[NP], b[NP];
         if (t.live) {
-            float csp[VEC];
+            if (!WALK)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) csp[e] = t.in ? ch.csp[t.d + e] : 0.f;
+                for (int e = 0; e < VEC; ++e) csp[e] = t.in ? ch.csp[t.d + e] : 0.f;
             Pack<T, VEC> r[S], gi[S], x[S];
 #pragma unroll
             for (int j = 0; j < S; ++j) {
@@ -526,7 +562,7 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
                 forward_gates<PRECISE>(pair_of<T, VEC, S>(r, q), pair_of<T, VEC, S>(gi, q), pair_of<T, VEC, S>(x, q),
                                        channel_pair<VEC>(csp, q), a[q], b[q]);
         }
-        if (vn < total) fetch(tn);
+        if (next) fetch(tn);
         if (t.live) {
             if (t.cnt < S) {  // what the buffer holds behind the end does not count
 #pragma unroll
@@ -553,44 +589,58 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
                 }
                 own.then(P, H);
             }
-            sm.wm.P[warp][lane] = own.P;
-            sm.wm.H[warp][lane] = own.H;
+            float h[VEC];
+            auto &wm = sm.wm[WALK ? t.k & 1 : 0];
+            wm.P[warp][lane] = own.P;
+            wm.H[warp][lane] = own.H;
             __syncthreads();
-            const bool more = (t.k + 1) * TT < t.n;  // a later tile waits for this one
-            const bool last = t.j == ch.group - 1;
-            if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, sm.wm);
-            Maps<VEC> m = prefix_maps<VEC, W>(ch, t, sm.wm, sm.gm);
-            float s[VEC], h[VEC];
+            if constexpr (WALK) {
+                walk_state<VEC, W>(wm, s, h);
+                if (!next && warp == 0 && t.in && p.hN)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                s[e] = t.in && p.h0 && t.g == 0 ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
-            group_state<VEC>(ch, t, s);
-            if (warp == W - 1 && (last || !more)) {
-                Maps<VEC> end = m;
-                end.then(own.P, own.H);
-                end.apply(s, h);
-                if (more)
-                    leave_group<VEC>(ch, t, h);
-                else if (t.in && p.hN)
+                    for (int e = 0; e < VEC; ++e) p.hN[(int64_t)t.b * p.D + t.d + e] = s[e];
+            } else {
+                const bool more = (t.k + 1) * TT < t.n;  // a later tile waits for this one
+                const bool last = t.j == ch.group - 1;
+                if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, wm);
+                Maps<VEC> m = prefix_maps<VEC, W>(ch, t, wm, sm.gm);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) p.hN[(int64_t)t.b * p.D + t.d + e] = h[e];
+                for (int e = 0; e < VEC; ++e)
+                    s[e] = t.in && p.h0 && t.g == 0 ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
+                group_state<VEC>(ch, t, s);
+                if (warp == W - 1 && (last || !more)) {
+                    Maps<VEC> end = m;
+                    end.then(own.P, own.H);
+                    end.apply(s, h);
+                    if (more)
+                        leave_group<VEC>(ch, t, h);
+                    else if (t.in && p.hN)
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) p.hN[(int64_t)t.b * p.D + t.d + e] = h[e];
+                }
+                m.apply(s, h);
             }
-            m.apply(s, h);
             T *ph = static_cast<T *>(p.h) + t.b * p.sh[0] + t.t0 * p.sh[1] + t.d;
 #pragma unroll
             for (int j = 0; j < S; ++j)
                 if (j < t.cnt) {
                     Pack<T, VEC> o;
+                    if constexpr (VEC == 1) {
+                        h[0] = fmaf(half_of(a[j / 2], j), h[0], half_of(b[j / 2], j));
+                        o.v[0] = cvt_out<T>(h[0]);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const int k = j * VEC + e;
-                        h[e] = fmaf(half_of(a[k / 2], k), h[e], half_of(b[k / 2], k));
-                        o.v[e] = cvt_out<T>(h[e]);
+                        for (int e = 0; e < VEC; e += 2) {
+                            const int q = (j * VEC + e) / 2;
+                            const float2 n = __ffma2_rn(a[q], make_float2(h[e], h[e + 1]), b[q]);
+                            o.v[e] = cvt_out<T>(h[e] = n.x);
+                            o.v[e + 1] = cvt_out<T>(h[e + 1] = n.y);
+                        }
                     }
                     *reinterpret_cast<Pack<T, VEC> *>(ph + j * p.sh[1]) = o;
                 }
         }
-        if (vn >= total) break;
+        if (!next) break;
         t = tn;
     }
 }
@@ -602,21 +652,21 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
 // of r and dh once the tile's map is computed, the others' behind the
 // gradients.  Across the wait a thread keeps sigmoid(r) and dh; the decay is
 // computed again (one exponential) rather than held.
-template <typename T, int VEC, int S, int W>
+template <typename T, int VEC, int S, int W, bool WALK>
 struct BwdSmem {
     Pack<T, VEC> in[5][S][32 * W];
-    MapRows<VEC, W> wm;
-    GroupRows<VEC> gm;
+    MapRows<VEC, W> wm[WALK ? 2 : 1];
+    MapRows<VEC, WALK ? 1 : (1 << max_group_shift(VEC)) - 1> gm;
     Pack<float, VEC> sums[W][32];
     unsigned int ticket[2];
 };
 
-template <typename T, int VEC, int S, int W, int CTAS>
+template <typename T, int VEC, int S, int W, int CTAS, bool WALK>
 __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdParams p, const Chains ch) {
     constexpr bool PRECISE = sizeof(T) == 4;
     constexpr int TT = S * W, NP = S * VEC / 2;
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    auto &sm = *reinterpret_cast<BwdSmem<T, VEC, S, W> *>(smem_raw);
+    auto &sm = *reinterpret_cast<BwdSmem<T, VEC, S, W, WALK> *>(smem_raw);
     const FwdParams &f = p.f;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned total = ch.chains.d * (unsigned)ch.tiles;
@@ -657,23 +707,44 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
         copy_commit();
     };
 
-    Tickets tickets(ch.ticket, sm.ticket);
-    unsigned v = tickets.next();
+    Tickets tickets(WALK ? nullptr : ch.ticket, sm.ticket);
+    unsigned v = WALK ? blockIdx.x : tickets.next();
     if (v >= total) return;
     Tile t = place(v);
     fetch_first(t, true);
     fetch_rest(t, true);
+    float csp[VEC], s[VEC], sum[VEC] = {};
+    if (WALK) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            csp[e] = t.in ? f.c * channel_softplus(f.lambda[t.d + e]) : 0.f;
+            s[e] = t.in && p.dhN ? p.dhN[(int64_t)t.b * f.D + t.d + e] : 0.f;
+        }
+    }
     for (;;) {
-        const unsigned vn = tickets.next();  // its barrier also frees sm.wm, sm.gm and sm.sums
-        Tile tn{};
-        if (vn < total) tn = place(vn);
+        Tile tn = t;
+        bool next;
+        if (WALK) {
+            ++tn.k;
+            tn.t0 -= TT;
+            tn.cnt = t.in ? S : 0;  // only the last tokens' tile can be short
+            next = tn.t0 - (W - 1 - warp) * S >= 0;
+        } else {
+            v = tickets.next();  // its barrier also frees sm.wm, sm.gm and sm.sums
+            next = v < total;
+            if (next) tn = place(v);
+        }
         copy_wait<1>();  // r and dh are there
-        float *part = p.part + ((int64_t)t.b * ch.tiles + t.k) * f.D + t.d;
+        // WALK: one row of sums per chain, else one per tile
+        float *part = p.part + (WALK ? (int64_t)t.b : (int64_t)t.b * ch.tiles + t.k) * f.D + t.d;
         if (t.live) {
             float2 sg[NP], om[PRECISE ? NP : 1];
-            float csp[VEC];
+            if (!WALK)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) csp[e] = t.in ? ch.csp[t.d + e] : 0.f;
+                for (int e = 0; e < VEC; ++e) {
+                    csp[e] = t.in ? ch.csp[t.d + e] : 0.f;
+                    sum[e] = 0.f;
+                }
             const uint32_t cut = cut_mask(f, t.b, t.t0, min(max(t.n - t.t0, 0), S));
             Pack<T, VEC> dh[S];
             Maps<VEC> own;
@@ -698,47 +769,66 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
 #pragma unroll
                 for (int u = TP - 1; u >= 0; --u)
                     if (j0 + u < t.cnt) {  // what the buffer holds behind the end does not count
-                        Pack<float, VEC> P, H;
-                        const float keep = cut >> (j0 + u) & 1 ? 0.f : 1.f;
+                        const Pack<T, VEC> &g = dh[j0 + u];
+                        if (cut >> (j0 + u) & 1) {  // nothing passes
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            const int k = u * VEC + e;
-                            P.v[e] = half_of(a[k / 2], k) * keep;
-                            H.v[e] = P.v[e] * cvt_f32(dh[j0 + u].v[e]);
+                            for (int e = 0; e < VEC; ++e) own.P.v[e] = own.H.v[e] = 0.f;
+                        } else if constexpr (VEC == 1) {
+                            const float av = half_of(a[0], u);
+                            own.H.v[0] = av * (own.H.v[0] + cvt_f32(g.v[0]));
+                            own.P.v[0] *= av;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < VEC; e += 2) {
+                                const float2 av = a[e / 2];
+                                const float2 h = __fmul2_rn(
+                                    av, __fadd2_rn(make_float2(own.H.v[e], own.H.v[e + 1]),
+                                                   make_float2(cvt_f32(g.v[e]), cvt_f32(g.v[e + 1]))));
+                                const float2 P = __fmul2_rn(av, make_float2(own.P.v[e], own.P.v[e + 1]));
+                                own.H.v[e] = h.x;
+                                own.H.v[e + 1] = h.y;
+                                own.P.v[e] = P.x;
+                                own.P.v[e + 1] = P.y;
+                            }
                         }
-                        own.then(P, H);
                     }
             }
-            fetch_first(tn, vn < total);
-            sm.wm.P[warp][lane] = own.P;
-            sm.wm.H[warp][lane] = own.H;
+            fetch_first(tn, next);
+            float C[VEC];
+            auto &wm = sm.wm[WALK ? t.k & 1 : 0];
+            wm.P[warp][lane] = own.P;
+            wm.H[warp][lane] = own.H;
             __syncthreads();
-            const bool more = t.t0 - (W - 1 - warp) * S > 0;  // an earlier tile waits for this one
-            const bool last = t.j == ch.group - 1;
-            if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, sm.wm);
-            Maps<VEC> m = prefix_maps<VEC, W>(ch, t, sm.wm, sm.gm);
-            float s[VEC], C[VEC];
+            if constexpr (WALK) {
+                walk_state<VEC, W>(wm, s, C);
+                if (!next && warp == 0 && t.in && p.dh0)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                s[e] = t.in && p.dhN && t.g == 0 ? p.dhN[(int64_t)t.b * f.D + t.d + e] : 0.f;
-            group_state<VEC>(ch, t, s);
-            if (warp == W - 1 && (last || !more)) {
-                Maps<VEC> end = m;
-                end.then(own.P, own.H);
-                end.apply(s, C);
-                if (more)
-                    leave_group<VEC>(ch, t, C);
-                else if (t.in && p.dh0)
+                    for (int e = 0; e < VEC; ++e) p.dh0[(int64_t)t.b * f.D + t.d + e] = s[e];
+            } else {
+                const bool more = t.t0 - (W - 1 - warp) * S > 0;  // an earlier tile waits for this one
+                const bool last = t.j == ch.group - 1;
+                if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, wm);
+                Maps<VEC> m = prefix_maps<VEC, W>(ch, t, wm, sm.gm);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) p.dh0[(int64_t)t.b * f.D + t.d + e] = C[e];
+                for (int e = 0; e < VEC; ++e)
+                    s[e] = t.in && p.dhN && t.g == 0 ? p.dhN[(int64_t)t.b * f.D + t.d + e] : 0.f;
+                group_state<VEC>(ch, t, s);
+                if (warp == W - 1 && (last || !more)) {
+                    Maps<VEC> end = m;
+                    end.then(own.P, own.H);
+                    end.apply(s, C);
+                    if (more)
+                        leave_group<VEC>(ch, t, C);
+                    else if (t.in && p.dh0)
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) p.dh0[(int64_t)t.b * f.D + t.d + e] = C[e];
+                }
+                m.apply(s, C);
             }
-            m.apply(s, C);
-
             copy_wait<1>();  // x, i and h are there
             T *qx = static_cast<T *>(p.dx) + t.b * p.sdx[0] + t.t0 * p.sdx[1] + t.d;
             T *qr = static_cast<T *>(p.dr) + t.b * p.sdr[0] + t.t0 * p.sdr[1] + t.d;
             T *qi = static_cast<T *>(p.di) + t.b * p.sdi[0] + t.t0 * p.sdi[1] + t.d;
-            float sum[VEC] = {};
 #pragma unroll
             for (int j0 = S - TP; j0 >= 0; j0 -= TP) {
                 if (j0 >= t.cnt) continue;
@@ -749,16 +839,26 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                     y[z] = __fmul2_rn(channel_pair<VEC>(csp, z), sg[j0 * VEC / 2 + z]);
                     a[z] = exp_neg<PRECISE>(y[z]);
                 }
+                if constexpr (VEC == 1) {
 #pragma unroll
-                for (int u = TP - 1; u >= 0; --u) {
-                    const float keep = cut >> (j0 + u) & 1 ? 0.f : 1.f;
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const int k = u * VEC + e;
-                        const float g = cvt_f32(dh[j0 + u].v[e]) + C[e];
-                        half_of(G[k / 2], k) = g;
-                        if (j0 + u < t.cnt) C[e] = half_of(a[k / 2], k) * keep * g;
+                    for (int u = TP - 1; u >= 0; --u) {
+                        const float g = cvt_f32(dh[j0 + u].v[0]) + C[0];
+                        half_of(G[0], u) = g;
+                        if (j0 + u < t.cnt) C[0] = cut >> (j0 + u) & 1 ? 0.f : half_of(a[0], u) * g;
                     }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; e += 2) {
+                        const Pack<T, VEC> &g = dh[j0];
+                        G[e / 2] = __fadd2_rn(make_float2(cvt_f32(g.v[e]), cvt_f32(g.v[e + 1])),
+                                              make_float2(C[e], C[e + 1]));
+                        const float2 n = __fmul2_rn(a[e / 2], G[e / 2]);
+                        C[e] = n.x;
+                        C[e + 1] = n.y;
+                    }
+                    if (cut >> j0 & 1)
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) C[e] = 0.f;
                 }
 #pragma unroll
                 for (int u = 0; u < TP; ++u) {
@@ -784,7 +884,8 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                     const float2 ei = exp_neg<PRECISE>(clamp_gate<PRECISE>(pair_of<T, VEC, TP>(gi, z)));
                     const float2 qi = __fadd2_rn(ei, both(1.f));
                     const float2 si = make_float2(rcp_approx(qi.x), rcp_approx(qi.y));
-                    const float2 m2 = one_minus_a2<PRECISE>(y[z], av), w = rsqrt_pos(m2);
+                    const float2 m2 = one_minus_a2<PRECISE>(y[z], av), m1 = __fadd2_rn(m2, both(kTiny));
+                    const float2 w = make_float2(rsqrt_approx(m1.x), rsqrt_approx(m1.y));
                     const float2 gs2 = __fmul2_rn(G[z], si);                      // G sigmoid(i)
                     const float2 gx = __fmul2_rn(gs2, __fmul2_rn(m2, w));         // * sqrt(m)
                     const float2 gi2 = __fmul2_rn(__fmul2_rn(gx, xv), __fmul2_rn(ei, si));
@@ -800,39 +901,41 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                         ox[u].v[e] = cvt_out<T>(hlf ? gx.y : gx.x);
                         oi[u].v[e] = cvt_out<T>(hlf ? gi2.y : gi2.x);
                         orr[u].v[e] = cvt_out<T>(hlf ? gr.y : gr.x);
-                        if (j0 + u < t.cnt) sum[e] += hlf ? E.y : E.x;
+                        if (VEC > 1 || j0 + u < t.cnt) sum[e] += hlf ? E.y : E.x;
                     }
                 }
 #pragma unroll
                 for (int u = 0; u < TP; ++u)
-                    if (j0 + u < t.cnt) {
+                    if (VEC > 1 || j0 + u < t.cnt) {
                         const int j = j0 + u;
                         *reinterpret_cast<Pack<T, VEC> *>(qx + j * p.sdx[1]) = ox[u];
                         *reinterpret_cast<Pack<T, VEC> *>(qi + j * p.sdi[1]) = oi[u];
                         *reinterpret_cast<Pack<T, VEC> *>(qr + j * p.sdr[1]) = orr[u];
                     }
             }
-            fetch_rest(tn, vn < total);
-            // the tile's sum of E per channel, warps in order
+            fetch_rest(tn, next);
+            // the sum of E per channel, warps in order
+            if (!WALK || !next) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) sm.sums[warp][lane].v[e] = sum[e];
-            __syncthreads();
-            if (warp == 0 && t.in)
+                for (int e = 0; e < VEC; ++e) sm.sums[warp][lane].v[e] = sum[e];
+                __syncthreads();
+                if (warp == 0 && t.in)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    float z = 0.f;
+                    for (int e = 0; e < VEC; ++e) {
+                        float z = 0.f;
 #pragma unroll
-                    for (int w = 0; w < W; ++w) z += sm.sums[w][lane].v[e];
-                    part[e] = z;
-                }
+                        for (int w = 0; w < W; ++w) z += sm.sums[w][lane].v[e];
+                        part[e] = z;
+                    }
+            }
         } else {  // behind the row's end
             if (warp == 0 && t.in)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) part[e] = 0.f;
-            fetch_first(tn, vn < total);
-            fetch_rest(tn, vn < total);
+            fetch_first(tn, next);
+            fetch_rest(tn, next);
         }
-        if (vn >= total) break;
+        if (!next) break;
         t = tn;
     }
 }
@@ -965,13 +1068,26 @@ FwdParams fwd_params(const MambaRecurrenceArgs *a) {
 
 // Tile shapes: channels a thread holds (1 serves any alignment and channel
 // count), tokens a warp holds, warps and CTAs per SM.
-template <typename T>
-struct FwdShape {
-    static constexpr int VEC = sizeof(T) == 2 ? 4 : 2, S = 8, W = 4, CTAS = sizeof(T) == 2 ? 4 : 5;
+template <int VEC_, int S_, int W_, int CTAS_>
+struct Shape {
+    static constexpr int VEC = VEC_, S = S_, W = W_, CTAS = CTAS_, tile = S_ * W_;
 };
-template <typename T>
-struct BwdShape {
-    static constexpr int VEC = sizeof(T) == 2 ? 4 : 2, S = 8, W = 4, CTAS = 4;
+template <typename T> struct Shapes;
+template <> struct Shapes<__half> {
+    using Fwd = Shape<4, 8, 4, 4>;
+    using FwdOne = Shape<1, 8, 4, 4>;
+    using FwdWalk = Shape<4, 8, 8, 2>;
+    using Bwd = Shape<4, 4, 4, 4>;
+    using BwdOne = Shape<1, 8, 4, 4>;
+    using BwdWalk = Shape<4, 4, 8, 2>;
+};
+template <> struct Shapes<float> {
+    using Fwd = Shape<2, 8, 4, 5>;
+    using FwdOne = Shape<1, 8, 4, 5>;
+    using FwdWalk = Shape<2, 8, 4, 5>;
+    using Bwd = Shape<2, 8, 4, 4>;
+    using BwdOne = Shape<1, 8, 4, 4>;
+    using BwdWalk = Shape<2, 8, 4, 4>;
 };
 
 // The chains of a call and where its workspace holds what.
@@ -979,14 +1095,12 @@ struct Plan {
     Chains ch;
     size_t bytes, csp_bytes, part_bytes, ones_bytes;
 };
-bool plan_chains(const MambaRecurrenceArgs *a, bool backward, int vec, Plan &pl) {
-    const bool half = a->dtype == MAMBA_F16;
-    const int tile = backward ? (half ? BwdShape<__half>::S * BwdShape<__half>::W : BwdShape<float>::S * BwdShape<float>::W)
-                              : (half ? FwdShape<__half>::S * FwdShape<__half>::W : FwdShape<float>::S * FwdShape<float>::W);
-    const int cw = 32 * vec;
+template <typename Sh>
+bool plan_chains(const MambaRecurrenceArgs *a, bool backward, Plan &pl) {
+    const int cw = 32 * Sh::VEC;
     Chains &c = pl.ch;
     c = Chains{};
-    const int64_t blocks = ceil_div64(a->dim, cw), tiles = std::max<int64_t>(1, ceil_div64(a->seqlen, tile));
+    const int64_t blocks = ceil_div64(a->dim, cw), tiles = std::max<int64_t>(1, ceil_div64(a->seqlen, Sh::tile));
     if (blocks * a->batch * tiles > 0x7fffffffLL) return false;
     auto divisor = [](int64_t d) {
         return Divisor{(unsigned)d, d == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / (unsigned long long)d)};
@@ -994,7 +1108,7 @@ bool plan_chains(const MambaRecurrenceArgs *a, bool backward, int vec, Plan &pl)
     c.blocks = divisor(blocks);
     c.chains = divisor(blocks * a->batch);
     c.tiles = (int)tiles;
-    c.group_shift = std::min(max_group_shift(vec), tiles <= 128 ? 2 : tiles <= 1024 ? 3 : 4);
+    c.group_shift = std::min(max_group_shift(Sh::VEC), tiles <= 128 ? 2 : tiles <= 1024 ? 3 : 4);
     c.group = 1 << c.group_shift;
     c.groups = ceil_div((int)tiles, c.group);
     // csp, the backward's partial sums, then what starts as all ones bits:
@@ -1007,20 +1121,22 @@ bool plan_chains(const MambaRecurrenceArgs *a, bool backward, int vec, Plan &pl)
     pl.bytes = pl.csp_bytes + pl.part_bytes + pl.ones_bytes;
     return true;
 }
+template <typename T>
+size_t workspace_bytes(const MambaRecurrenceArgs *a, bool backward) {
+    using S = Shapes<T>;
+    Plan p, q;
+    if (!(backward ? plan_chains<typename S::Bwd>(a, true, p) : plan_chains<typename S::Fwd>(a, false, p))) return 0;
+    if (!(backward ? plan_chains<typename S::BwdOne>(a, true, q) : plan_chains<typename S::FwdOne>(a, false, q)))
+        return 0;
+    return std::max(p.bytes, q.bytes);
+}
 
 }  // namespace
 
-// The largest of what any channel width needs, so that the size does not
-// depend on pointers.
+// What either channel width needs, so that the size does not depend on pointers.
 size_t recurrence_workspace_bytes(const MambaRecurrenceArgs *a, bool backward) {
     if (!a || a->batch <= 0 || a->seqlen < 0 || a->dim <= 0) return 0;
-    size_t need = 0;
-    for (int vec : {1, 2, 4}) {
-        Plan pl;
-        if (!plan_chains(a, backward, vec, pl)) return 0;
-        need = std::max(need, pl.bytes);
-    }
-    return need;
+    return a->dtype == MAMBA_F16 ? workspace_bytes<__half>(a, backward) : workspace_bytes<float>(a, backward);
 }
 
 namespace {
@@ -1050,67 +1166,106 @@ __global__ void __launch_bounds__(256)
     for (int64_t k = i; k < n; k += stride) ones[k] = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
 }
 
-// Launches one variant: the workspace's preparation, then persistent CTAs.
-template <int VEC, typename Kernel, typename Params>
-int launch_tiles(Kernel kernel, const Params &p, const FwdParams &f, Plan &pl, int threads, int ctas, size_t smem,
-                 void *ws, cudaStream_t st, const char *what) {
+// Launches one variant.  Tickets: the workspace's preparation, then as many
+// persistent CTAs as fit; walking: one CTA per chain, no preparation.
+template <typename Sh, bool WALK, typename Kernel, typename Params>
+int launch_tiles(Kernel kernel, const Params &p, const FwdParams &f, Plan &pl, size_t smem, void *ws, cudaStream_t st,
+                 const char *what) {
     Chains &c = pl.ch;
-    uint8_t *base = static_cast<uint8_t *>(ws);
-    float *csp = reinterpret_cast<float *>(base);
-    base += pl.csp_bytes + pl.part_bytes;
-    c.csp = csp;
-    c.ticket = reinterpret_cast<unsigned int *>(base);
-    c.maps = reinterpret_cast<float2 *>(base + 256);
-    c.states = reinterpret_cast<float *>(c.maps + (int64_t)c.chains.d * c.tiles * 32 * VEC);
     if (allow_smem(kernel, smem)) return -1;
-    const int64_t ones = (int64_t)pl.ones_bytes / 16, sms = device_sm_count();
-    const int64_t init = std::min<int64_t>(8 * sms, std::max<int64_t>(ceil_div64(ones, 1024), ceil_div64(f.D, 256)));
-    recurrence_init_kernel<<<(unsigned)init, 256, 0, st>>>(f.lambda, f.c, f.D, csp, reinterpret_cast<uint4 *>(base),
-                                                           ones);
-    if (launch_status(what)) return -1;
-    kernel<<<(unsigned)std::min((int64_t)c.chains.d * c.tiles, ctas * sms), threads, smem, st>>>(p, c);
+    const int64_t sms = device_sm_count();
+    int64_t grid = c.chains.d;
+    if (!WALK) {
+        uint8_t *base = static_cast<uint8_t *>(ws);
+        float *csp = reinterpret_cast<float *>(base);
+        base += pl.csp_bytes + pl.part_bytes;
+        c.csp = csp;
+        c.ticket = reinterpret_cast<unsigned int *>(base);
+        c.maps = reinterpret_cast<float2 *>(base + 256);
+        c.states = reinterpret_cast<float *>(c.maps + (int64_t)c.chains.d * c.tiles * 32 * Sh::VEC);
+        const int64_t ones = (int64_t)pl.ones_bytes / 16;
+        const int64_t init = std::min<int64_t>(8 * sms, std::max<int64_t>(ceil_div64(ones, 1024), ceil_div64(f.D, 256)));
+        recurrence_init_kernel<<<(unsigned)init, 256, 0, st>>>(f.lambda, f.c, f.D, csp, reinterpret_cast<uint4 *>(base),
+                                                               ones);
+        if (launch_status(what)) return -1;
+        grid = std::min(grid * c.tiles, Sh::CTAS * sms);
+    }
+    kernel<<<(unsigned)grid, 32 * Sh::W, smem, st>>>(p, c);
     return launch_status(what);
 }
 
-template <typename T, int VEC>
-int launch_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
-    Plan pl;
-    MB_CHECK_ARG(plan_chains(a, false, VEC, pl), "gated_recurrence: too many tiles");
-    using F = FwdShape<T>;
+// Whether CTAs should walk whole chains: where the chains fill the resident
+// CTAs of `Sh` in nearly whole rounds, walking spares the hand-over of states
+// between CTAs; with fewer chains it would leave SMs empty.
+template <typename Sh>
+bool walks(const Plan &pl) {
+    const int64_t slots = (int64_t)Sh::CTAS * device_sm_count(), chains = pl.ch.chains.d;
+    return chains * 10 >= ceil_div64(chains, slots) * slots * 6 || pl.ch.tiles == 1;
+}
+
+template <typename T, typename Sh, bool WALK>
+int launch_forward(const MambaRecurrenceArgs *a, Plan &pl, void *ws, cudaStream_t st) {
     const FwdParams p = fwd_params(a);
-    return launch_tiles<VEC>(recurrence_fwd_kernel<T, VEC, F::S, F::W, F::CTAS>, p, p, pl, 32 * F::W, F::CTAS,
-                             sizeof(FwdSmem<T, VEC, F::S, F::W>), ws, st, "gated_recurrence kernel");
+    return launch_tiles<Sh, WALK>(recurrence_fwd_kernel<T, Sh::VEC, Sh::S, Sh::W, Sh::CTAS, WALK>, p, p, pl,
+                                  sizeof(FwdSmem<T, Sh::VEC, Sh::S, Sh::W, WALK>), ws, st, "gated_recurrence kernel");
 }
 template <typename T>
 int choose_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
-    constexpr int V = FwdShape<T>::VEC;
-    const bool vec = a->dim % V == 0 && vector_rows<T, V>(a->x, a->x_stride) && vector_rows<T, V>(a->r, a->r_stride) &&
-                     vector_rows<T, V>(a->i, a->i_stride) && vector_rows<T, V>(a->h, a->h_stride);
-    return vec ? launch_forward<T, V>(a, ws, st) : launch_forward<T, 1>(a, ws, st);
+    using S = Shapes<T>;
+    constexpr int V = S::Fwd::VEC;
+    auto vec = [&](auto v) {
+        constexpr int N = decltype(v)::value;
+        return a->dim % N == 0 && vector_rows<T, N>(a->x, a->x_stride) && vector_rows<T, N>(a->r, a->r_stride) &&
+               vector_rows<T, N>(a->i, a->i_stride) && vector_rows<T, N>(a->h, a->h_stride);
+    };
+    Plan pl;
+    const char *many = "gated_recurrence: too many tiles";
+    MB_CHECK_ARG(plan_chains<typename S::FwdWalk>(a, false, pl), many);
+    if (vec(std::integral_constant<int, S::FwdWalk::VEC>()) && walks<typename S::FwdWalk>(pl))
+        return launch_forward<T, typename S::FwdWalk, true>(a, pl, ws, st);
+    if (vec(std::integral_constant<int, V>())) {
+        MB_CHECK_ARG(plan_chains<typename S::Fwd>(a, false, pl), many);
+        return launch_forward<T, typename S::Fwd, false>(a, pl, ws, st);
+    }
+    MB_CHECK_ARG(plan_chains<typename S::FwdOne>(a, false, pl), many);
+    return launch_forward<T, typename S::FwdOne, false>(a, pl, ws, st);
 }
 
-template <typename T, int VEC>
-int launch_backward(const MambaRecurrenceArgs *a, BwdParams &p, void *ws, cudaStream_t st, int &tiles) {
-    Plan pl;
-    MB_CHECK_ARG(plan_chains(a, true, VEC, pl), "gated_recurrence_backward: too many tiles");
-    tiles = pl.ch.tiles;
+template <typename T, typename Sh, bool WALK>
+int launch_backward(const MambaRecurrenceArgs *a, BwdParams &p, Plan &pl, void *ws, cudaStream_t st) {
     p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + pl.csp_bytes);
-    using F = BwdShape<T>;
-    return launch_tiles<VEC>(recurrence_bwd_kernel<T, VEC, F::S, F::W, F::CTAS>, p, p.f, pl, 32 * F::W, F::CTAS,
-                             sizeof(BwdSmem<T, VEC, F::S, F::W>), ws, st, "gated_recurrence_backward kernel");
+    return launch_tiles<Sh, WALK>(recurrence_bwd_kernel<T, Sh::VEC, Sh::S, Sh::W, Sh::CTAS, WALK>, p, p.f, pl,
+                                  sizeof(BwdSmem<T, Sh::VEC, Sh::S, Sh::W, WALK>), ws, st,
+                                  "gated_recurrence_backward kernel");
 }
 template <typename T>
 int choose_backward(const MambaRecurrenceArgs *a, BwdParams &p, const MambaRecurrenceGrads *g, void *ws,
                     cudaStream_t st) {
-    constexpr int V = BwdShape<T>::VEC;
-    const bool vec = a->dim % V == 0 && vector_rows<T, V>(a->x, a->x_stride) && vector_rows<T, V>(a->r, a->r_stride) &&
-                     vector_rows<T, V>(a->i, a->i_stride) && vector_rows<T, V>(a->h, a->h_stride) &&
-                     vector_rows<T, V>(g->dh, g->dh_stride) && vector_rows<T, V>(g->dx, g->dx_stride) &&
-                     vector_rows<T, V>(g->dr, g->dr_stride) && vector_rows<T, V>(g->di, g->di_stride);
-    int tiles = 0;
-    if (vec ? launch_backward<T, V>(a, p, ws, st, tiles) : launch_backward<T, 1>(a, p, ws, st, tiles)) return -1;
-    recurrence_dlambda_kernel<<<(unsigned)ceil_div(a->dim, 32), 32 * kSumWarps, 0, st>>>(
-        p.part, a->lambda, g->dlambda, (int64_t)a->batch * tiles, a->dim);
+    using S = Shapes<T>;
+    auto vec = [&](auto v) {
+        constexpr int N = decltype(v)::value;
+        return a->dim % N == 0 && vector_rows<T, N>(a->x, a->x_stride) && vector_rows<T, N>(a->r, a->r_stride) &&
+               vector_rows<T, N>(a->i, a->i_stride) && vector_rows<T, N>(a->h, a->h_stride) &&
+               vector_rows<T, N>(g->dh, g->dh_stride) && vector_rows<T, N>(g->dx, g->dx_stride) &&
+               vector_rows<T, N>(g->dr, g->dr_stride) && vector_rows<T, N>(g->di, g->di_stride);
+    };
+    Plan pl;
+    const char *many = "gated_recurrence_backward: too many tiles";
+    int64_t rows = a->batch;
+    MB_CHECK_ARG(plan_chains<typename S::BwdWalk>(a, true, pl), many);
+    if (vec(std::integral_constant<int, S::BwdWalk::VEC>()) && walks<typename S::BwdWalk>(pl)) {
+        if (launch_backward<T, typename S::BwdWalk, true>(a, p, pl, ws, st)) return -1;
+    } else if (vec(std::integral_constant<int, S::Bwd::VEC>())) {
+        MB_CHECK_ARG(plan_chains<typename S::Bwd>(a, true, pl), many);
+        if (launch_backward<T, typename S::Bwd, false>(a, p, pl, ws, st)) return -1;
+        rows *= pl.ch.tiles;
+    } else {
+        MB_CHECK_ARG(plan_chains<typename S::BwdOne>(a, true, pl), many);
+        if (launch_backward<T, typename S::BwdOne, false>(a, p, pl, ws, st)) return -1;
+        rows *= pl.ch.tiles;
+    }
+    recurrence_dlambda_kernel<<<(unsigned)ceil_div(a->dim, 32), 32 * kSumWarps, 0, st>>>(p.part, a->lambda,
+                                                                                         g->dlambda, rows, a->dim);
     return launch_status("gated_recurrence_backward sum kernel");
 }
 

@@ -86,7 +86,8 @@ def _check_backward(v, h, grads, dtype):
 
 
 SHAPES = [(1, 1, 1), (2, 1, 64), (1, 7, 3), (3, 64, 64), (2, 65, 130), (2, 129, 66), (1, 257, 1001), (2, 300, 256),
-          (1, 2000, 96), (5, 17, 33), (2, 513, 72)]
+          (1, 2000, 96), (5, 17, 33), (2, 513, 72),
+          (24, 140, 1000)]  # the last: enough rows and channels for CTAs to walk whole rows
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
@@ -233,7 +234,7 @@ def test_empty_sizes(cuda, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
-@pytest.mark.parametrize("B,L,D", [(2, 1500, 200), (8, 700, 1024)])
+@pytest.mark.parametrize("B,L,D", [(2, 1500, 200), (8, 700, 1024), (40, 200, 640)])
 def test_repeated_calls_give_the_same_bits(cuda, dtype, B, L, D):
     t = _dev(_case(6, B, L, D, dtype))
     first = None
