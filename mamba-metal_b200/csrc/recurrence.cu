@@ -141,6 +141,7 @@ struct FwdParams {
     float *hN;
     int B, L, D;
     float c;
+    unsigned row_first;  // per tensor map: see fetch_box
     int64_t sx[2], sr[2], si[2], sh[2];
 };
 struct BwdParams {
@@ -441,16 +442,41 @@ __device__ __forceinline__ uint32_t cut_mask(const FwdParams &p, int b, int t0, 
     return __ballot_sync(0xffffffffu, z);
 }
 
-// Copies VEC elements to this thread's own place in shared memory,
-// asynchronously where they make at least the 4 bytes cp.async takes.
-template <typename T, int VEC>
-__device__ __forceinline__ void copy_pack(Pack<T, VEC> *dst, const T *src) {
-    if constexpr (sizeof(T) * VEC >= 4)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src),
-                     "n"((int)(sizeof(T) * VEC))
+// ---- a tile's inputs in shared memory -----------------------------------------------
+// N tensors of TT tokens x 32 * VEC channels, NB buffers in turn.  With TMA
+// (16-byte aligned rows) one thread fetches a tile by one bulk tensor copy per
+// tensor, completing on the buffer's mbarrier: no other thread spends an
+// instruction on addresses.  Elsewhere each thread copies the elements that it
+// will read itself.
+template <typename T, int VEC, int TT, int N, int NB>
+struct TileIn {
+    alignas(128) Pack<T, VEC> v[NB][N][TT][32];
+    alignas(16) uint64_t full[NB];
+};
+struct TileMaps {
+    CUtensorMap m[5];
+};
+// Order of a tensor map's outer two dimensions: time then row, or row then
+// time (the larger stride last).
+__device__ __forceinline__ void fetch_box(void *dst, const CUtensorMap *map, uint64_t *bar, int d, int t, int b,
+                                          bool row_first) {
+    tma_load_3d(dst, map, bar, d, row_first ? b : t, row_first ? t : b);
+}
+
+// Waits for buffer `buf` in its `use`-th use.  A wait that runs out is
+// reported; the CTA goes on (with wrong values), so nothing else waits for it.
+__device__ __forceinline__ void await_box(uint64_t *bar, uint32_t use) {
+    if (!mbar_wait_bounded(bar, use & 1)) atomicOr(&g_recurrence_error, kErrRecurrenceTimeout);
+}
+
+// Copies one element (at least 4 bytes asynchronously, 2 bytes at once).
+template <typename T>
+__device__ __forceinline__ void copy_one(Pack<T, 1> *dst, const T *src) {
+    if constexpr (sizeof(T) >= 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"((int)sizeof(T))
                      : "memory");
     else
-        *dst = load_pack<T, VEC>(src);
+        dst->v[0] = *src;
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -472,31 +498,36 @@ __device__ __forceinline__ float2 channel_pair(const float (&v)[VEC], int q) {
 __device__ __forceinline__ float &half_of(float2 &v, int k) { return k & 1 ? v.y : v.x; }
 
 // ---- forward --------------------------------------------------------------------
-// Persistent CTAs: once a tile's gates are computed, the copies of the next
-// tile's x, r and i into shared memory start, and run while this tile waits
-// for its state and writes h.  A thread reads back only what it copied
-// itself, so no barrier guards the buffer.
-//
-// With enough chains to fill the GPU (walks()), a CTA walks one chain from its
-// first tile to its last instead (WALK): no tickets, nothing published, the
-// state stays in registers.
+// Persistent CTAs take tiles by ticket; the next tile's inputs are fetched once
+// every warp has this tile's in registers, while it waits for its state and
+// writes h.  With enough chains to fill the GPU
+// (walks()), a CTA walks one chain from its first tile to its last instead
+// (WALK): no tickets, nothing published, the state stays in registers.
 template <typename T, int VEC, int S, int W, bool WALK>
 struct FwdSmem {
-    Pack<T, VEC> in[3][S][32 * W];
+    TileIn<T, VEC, S * W, 3, 1> in;
     MapRows<VEC, W> wm[WALK ? 2 : 1];
     MapRows<VEC, WALK ? 1 : (1 << max_group_shift(VEC)) - 1> gm;
     unsigned int ticket[2];
 };
 
-template <typename T, int VEC, int S, int W, int CTAS, bool WALK>
-__global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdParams p, const Chains ch) {
+template <typename T, int VEC, int S, int W, int CTAS, bool TMA, bool WALK>
+__global__ void __launch_bounds__(32 * W, CTAS)
+    recurrence_fwd_kernel(const FwdParams p, const Chains ch, const __grid_constant__ TileMaps maps) {
     constexpr bool PRECISE = sizeof(T) == 4;
     constexpr int TT = S * W, NP = S * VEC / 2;
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+    extern __shared__ __align__(128) uint8_t smem_raw[];
     auto &sm = *reinterpret_cast<FwdSmem<T, VEC, S, W, WALK> *>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned total = ch.chains.d * (unsigned)ch.tiles;
 
+    if (TMA) {
+        if (tid == 0) {
+            mbar_init(&sm.in.full[0], 1);
+            fence_mbar_init();
+        }
+        __syncthreads();
+    }
     auto place = [&](unsigned v) {
         Tile t = place_tile<VEC>(ch, p, v);
         t.t0 = t.k * TT + warp * S;
@@ -505,17 +536,30 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
         return t;
     };
     auto fetch = [&](const Tile &t) {
-        const T *px = static_cast<const T *>(p.x) + t.b * p.sx[0] + t.t0 * p.sx[1] + t.d;
-        const T *pr = static_cast<const T *>(p.r) + t.b * p.sr[0] + t.t0 * p.sr[1] + t.d;
-        const T *pi = static_cast<const T *>(p.i) + t.b * p.si[0] + t.t0 * p.si[1] + t.d;
-#pragma unroll
-        for (int j = 0; j < S; ++j)
-            if (j < t.cnt) {
-                copy_pack<T, VEC>(&sm.in[0][j][tid], pr + j * p.sr[1]);
-                copy_pack<T, VEC>(&sm.in[1][j][tid], pi + j * p.si[1]);
-                copy_pack<T, VEC>(&sm.in[2][j][tid], px + j * p.sx[1]);
+        if constexpr (TMA) {
+            if (tid == 0) {
+                uint64_t *bar = &sm.in.full[0];
+                mbar_arrive_expect_tx(bar, 3 * TT * 32 * VEC * sizeof(T));
+                const int d0 = t.d, t0 = t.t0;  // of thread 0: the tile's first channel and token
+                fetch_box(sm.in.v[0][0], &maps.m[0], bar, d0, t0, t.b, p.row_first & 1);
+                fetch_box(sm.in.v[0][1], &maps.m[1], bar, d0, t0, t.b, p.row_first & 2);
+                fetch_box(sm.in.v[0][2], &maps.m[2], bar, d0, t0, t.b, p.row_first & 4);
             }
-        copy_commit();
+        } else {
+            const T *px = static_cast<const T *>(p.x) + t.b * p.sx[0] + t.t0 * p.sx[1] + t.d;
+            const T *pr = static_cast<const T *>(p.r) + t.b * p.sr[0] + t.t0 * p.sr[1] + t.d;
+            const T *pi = static_cast<const T *>(p.i) + t.b * p.si[0] + t.t0 * p.si[1] + t.d;
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                if (j < t.cnt) {
+                    if constexpr (VEC == 1) {
+                        copy_one<T>(&sm.in.v[0][0][warp * S + j][lane], pr + j * p.sr[1]);
+                        copy_one<T>(&sm.in.v[0][1][warp * S + j][lane], pi + j * p.si[1]);
+                        copy_one<T>(&sm.in.v[0][2][warp * S + j][lane], px + j * p.sx[1]);
+                    }
+                }
+            copy_commit();
+        }
     };
 
     Tickets tickets(WALK ? nullptr : ch.ticket, sm.ticket);
@@ -531,7 +575,7 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
             s[e] = t.in && p.h0 ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
         }
     }
-    for (;;) {
+    for (uint32_t it = 0;; ++it) {
         Tile tn = t;
         bool next;
         if (WALK) {
@@ -544,26 +588,28 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
             next = v < total;
             if (next) tn = place(v);
         }
-        copy_wait<0>();
-        float2 a[NP], b[NP];
+        if constexpr (TMA)
+            await_box(&sm.in.full[0], it);
+        else
+            copy_wait<0>();
         if (t.live) {
             if (!WALK)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) csp[e] = t.in ? ch.csp[t.d + e] : 0.f;
-            Pack<T, VEC> r[S], gi[S], x[S];
+            float2 a[NP], b[NP];
+            {
+                Pack<T, VEC> r[S], gi[S], x[S];
 #pragma unroll
-            for (int j = 0; j < S; ++j) {
-                r[j] = sm.in[0][j][tid];
-                gi[j] = sm.in[1][j][tid];
-                x[j] = sm.in[2][j][tid];
+                for (int j = 0; j < S; ++j) {
+                    r[j] = sm.in.v[0][0][warp * S + j][lane];
+                    gi[j] = sm.in.v[0][1][warp * S + j][lane];
+                    x[j] = sm.in.v[0][2][warp * S + j][lane];
+                }
+#pragma unroll
+                for (int q = 0; q < NP; ++q)
+                    forward_gates<PRECISE>(pair_of<T, VEC, S>(r, q), pair_of<T, VEC, S>(gi, q),
+                                           pair_of<T, VEC, S>(x, q), channel_pair<VEC>(csp, q), a[q], b[q]);
             }
-#pragma unroll
-            for (int q = 0; q < NP; ++q)
-                forward_gates<PRECISE>(pair_of<T, VEC, S>(r, q), pair_of<T, VEC, S>(gi, q), pair_of<T, VEC, S>(x, q),
-                                       channel_pair<VEC>(csp, q), a[q], b[q]);
-        }
-        if (next) fetch(tn);
-        if (t.live) {
             if (t.cnt < S) {  // what the buffer holds behind the end does not count
 #pragma unroll
                 for (int k = 0; k < S * VEC; ++k)
@@ -594,6 +640,7 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
             wm.P[warp][lane] = own.P;
             wm.H[warp][lane] = own.H;
             __syncthreads();
+            if (next) fetch(tn);  // every warp has read the buffer
             if constexpr (WALK) {
                 walk_state<VEC, W>(wm, s, h);
                 if (!next && warp == 0 && t.in && p.hN)
@@ -639,6 +686,8 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
                     }
                     *reinterpret_cast<Pack<T, VEC> *>(ph + j * p.sh[1]) = o;
                 }
+        } else if (next) {
+            fetch(tn);
         }
         if (!next) break;
         t = tn;
@@ -647,72 +696,86 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_fwd_kernel(const FwdP
 
 // ---- backward -------------------------------------------------------------------
 // The same tiles and chains with time reversed; what runs along a chain is
-// C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.  The
-// next tile's copies start as soon as a buffer is read for the last time: those
-// of r and dh once the tile's map is computed, the others' behind the
-// gradients.  Across the wait a thread keeps sigmoid(r) and dh; the decay is
-// computed again (one exponential) rather than held.
+// C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.  Across
+// the wait a thread keeps sigmoid(r) and dh; the decay is computed again (one
+// exponential) rather than held.
 template <typename T, int VEC, int S, int W, bool WALK>
 struct BwdSmem {
-    Pack<T, VEC> in[5][S][32 * W];
+    TileIn<T, VEC, S * W, 5, 2> in;
     MapRows<VEC, W> wm[WALK ? 2 : 1];
     MapRows<VEC, WALK ? 1 : (1 << max_group_shift(VEC)) - 1> gm;
     Pack<float, VEC> sums[W][32];
     unsigned int ticket[2];
 };
 
-template <typename T, int VEC, int S, int W, int CTAS, bool WALK>
-__global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdParams p, const Chains ch) {
+template <typename T, int VEC, int S, int W, int CTAS, bool TMA, bool WALK>
+__global__ void __launch_bounds__(32 * W, CTAS)
+    recurrence_bwd_kernel(const BwdParams p, const Chains ch, const __grid_constant__ TileMaps maps) {
     constexpr bool PRECISE = sizeof(T) == 4;
     constexpr int TT = S * W, NP = S * VEC / 2;
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+    extern __shared__ __align__(128) uint8_t smem_raw[];
     auto &sm = *reinterpret_cast<BwdSmem<T, VEC, S, W, WALK> *>(smem_raw);
     const FwdParams &f = p.f;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned total = ch.chains.d * (unsigned)ch.tiles;
+    const int trow = (W - 1 - warp) * S;  // this warp's first token in the tile: warp 0 holds the last ones
 
+    if (TMA) {
+        if (tid == 0) {
+            mbar_init(&sm.in.full[0], 1);
+            mbar_init(&sm.in.full[1], 1);
+            fence_mbar_init();
+        }
+        __syncthreads();
+    }
     auto place = [&](unsigned v) {
         Tile t = place_tile<VEC>(ch, f, v);
         const int row_tiles = max((t.n + TT - 1) / TT, 1);
         t.live = t.k < row_tiles;
-        t.t0 = (row_tiles - 1 - t.k) * TT + (W - 1 - warp) * S;  // warp 0 holds the tile's last tokens
+        t.t0 = (row_tiles - 1 - t.k) * TT + trow;
         t.cnt = t.in && t.live ? min(max(t.n - t.t0, 0), S) : 0;
         return t;
     };
-    // each commits one group of copies, also where there is nothing to copy
-    auto fetch_first = [&](const Tile &t, bool any) {
-        const T *pr = static_cast<const T *>(f.r) + t.b * f.sr[0] + t.t0 * f.sr[1] + t.d;
-        const T *pg = static_cast<const T *>(p.dh) + t.b * p.sdh[0] + t.t0 * p.sdh[1] + t.d;
-        if (any)
+    auto fetch = [&](const Tile &t, int buf) {
+        if constexpr (TMA) {
+            if (tid == 0) {
+                uint64_t *bar = &sm.in.full[buf];
+                mbar_arrive_expect_tx(bar, 5 * TT * 32 * VEC * sizeof(T));
+                // A dead tile lies before time 0: its copies read zeros.
+                const int d0 = t.d, t0 = t.t0 - trow;
+                fetch_box(sm.in.v[buf][0], &maps.m[0], bar, d0, t0, t.b, f.row_first & 1);
+                fetch_box(sm.in.v[buf][1], &maps.m[1], bar, d0, t0, t.b, f.row_first & 2);
+                fetch_box(sm.in.v[buf][2], &maps.m[2], bar, d0, t0, t.b, f.row_first & 4);
+                fetch_box(sm.in.v[buf][3], &maps.m[3], bar, d0, t0, t.b, f.row_first & 8);
+                fetch_box(sm.in.v[buf][4], &maps.m[4], bar, d0, t0 - 1, t.b, f.row_first & 16);
+            }
+        } else {
+            const T *pr = static_cast<const T *>(f.r) + t.b * f.sr[0] + t.t0 * f.sr[1] + t.d;
+            const T *pg = static_cast<const T *>(p.dh) + t.b * p.sdh[0] + t.t0 * p.sdh[1] + t.d;
+            const T *px = static_cast<const T *>(f.x) + t.b * f.sx[0] + t.t0 * f.sx[1] + t.d;
+            const T *pi = static_cast<const T *>(f.i) + t.b * f.si[0] + t.t0 * f.si[1] + t.d;
+            const T *ph = static_cast<const T *>(f.h) + t.b * f.sh[0] + (t.t0 - 1) * f.sh[1] + t.d;
 #pragma unroll
             for (int j = 0; j < S; ++j)
                 if (j < t.cnt) {
-                    copy_pack<T, VEC>(&sm.in[0][j][tid], pr + j * f.sr[1]);
-                    copy_pack<T, VEC>(&sm.in[1][j][tid], pg + j * p.sdh[1]);
+                    const int row = trow + j;
+                    if constexpr (VEC == 1) {
+                        copy_one<T>(&sm.in.v[buf][0][row][lane], pr + j * f.sr[1]);
+                        copy_one<T>(&sm.in.v[buf][1][row][lane], px + j * f.sx[1]);
+                        copy_one<T>(&sm.in.v[buf][2][row][lane], pi + j * f.si[1]);
+                        copy_one<T>(&sm.in.v[buf][3][row][lane], pg + j * p.sdh[1]);
+                        if (t.t0 + j > 0) copy_one<T>(&sm.in.v[buf][4][row][lane], ph + j * f.sh[1]);
+                    }
                 }
-        copy_commit();
-    };
-    auto fetch_rest = [&](const Tile &t, bool any) {
-        const T *px = static_cast<const T *>(f.x) + t.b * f.sx[0] + t.t0 * f.sx[1] + t.d;
-        const T *pi = static_cast<const T *>(f.i) + t.b * f.si[0] + t.t0 * f.si[1] + t.d;
-        const T *ph = static_cast<const T *>(f.h) + t.b * f.sh[0] + (t.t0 - 1) * f.sh[1] + t.d;
-        if (any)
-#pragma unroll
-            for (int j = 0; j < S; ++j)
-                if (j < t.cnt) {
-                    copy_pack<T, VEC>(&sm.in[2][j][tid], px + j * f.sx[1]);
-                    copy_pack<T, VEC>(&sm.in[3][j][tid], pi + j * f.si[1]);
-                    if (t.t0 + j > 0) copy_pack<T, VEC>(&sm.in[4][j][tid], ph + j * f.sh[1]);
-                }
-        copy_commit();
+        }
     };
 
     Tickets tickets(WALK ? nullptr : ch.ticket, sm.ticket);
     unsigned v = WALK ? blockIdx.x : tickets.next();
     if (v >= total) return;
     Tile t = place(v);
-    fetch_first(t, true);
-    fetch_rest(t, true);
+    fetch(t, 0);
+    if (!TMA) copy_commit();
     float csp[VEC], s[VEC], sum[VEC] = {};
     if (WALK) {
 #pragma unroll
@@ -721,20 +784,24 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
             s[e] = t.in && p.dhN ? p.dhN[(int64_t)t.b * f.D + t.d + e] : 0.f;
         }
     }
-    for (;;) {
+    for (uint32_t it = 0;; ++it) {
+        const int buf = it & 1;
         Tile tn = t;
         bool next;
         if (WALK) {
             ++tn.k;
             tn.t0 -= TT;
             tn.cnt = t.in ? S : 0;  // only the last tokens' tile can be short
-            next = tn.t0 - (W - 1 - warp) * S >= 0;
+            next = tn.t0 - trow >= 0;
         } else {
             v = tickets.next();  // its barrier also frees sm.wm, sm.gm and sm.sums
             next = v < total;
             if (next) tn = place(v);
         }
-        copy_wait<1>();  // r and dh are there
+        if constexpr (TMA)
+            await_box(&sm.in.full[buf], it >> 1);
+        else
+            copy_wait<0>();
         // WALK: one row of sums per chain, else one per tile
         float *part = p.part + (WALK ? (int64_t)t.b : (int64_t)t.b * ch.tiles + t.k) * f.D + t.d;
         if (t.live) {
@@ -756,8 +823,8 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                 Pack<T, VEC> r[TP];
 #pragma unroll
                 for (int u = 0; u < TP; ++u) {
-                    r[u] = sm.in[0][j0 + u][tid];
-                    dh[j0 + u] = sm.in[1][j0 + u][tid];
+                    r[u] = sm.in.v[buf][0][trow + j0 + u][lane];
+                    dh[j0 + u] = sm.in.v[buf][3][trow + j0 + u][lane];
                 }
 #pragma unroll
                 for (int z = 0; z < TP * VEC / 2; ++z) {
@@ -793,19 +860,21 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                         }
                     }
             }
-            fetch_first(tn, next);
             float C[VEC];
             auto &wm = sm.wm[WALK ? t.k & 1 : 0];
             wm.P[warp][lane] = own.P;
             wm.H[warp][lane] = own.H;
             __syncthreads();
+            // Every warp is done with the tile before, so the other buffer is free.
+            if (next) fetch(tn, buf ^ 1);
+            if (!TMA) copy_commit();
             if constexpr (WALK) {
                 walk_state<VEC, W>(wm, s, C);
                 if (!next && warp == 0 && t.in && p.dh0)
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) p.dh0[(int64_t)t.b * f.D + t.d + e] = s[e];
             } else {
-                const bool more = t.t0 - (W - 1 - warp) * S > 0;  // an earlier tile waits for this one
+                const bool more = t.t0 - trow > 0;  // an earlier tile waits for this one
                 const bool last = t.j == ch.group - 1;
                 if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, wm);
                 Maps<VEC> m = prefix_maps<VEC, W>(ch, t, wm, sm.gm);
@@ -825,7 +894,7 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                 }
                 m.apply(s, C);
             }
-            copy_wait<1>();  // x, i and h are there
+
             T *qx = static_cast<T *>(p.dx) + t.b * p.sdx[0] + t.t0 * p.sdx[1] + t.d;
             T *qr = static_cast<T *>(p.dr) + t.b * p.sdr[0] + t.t0 * p.sdr[1] + t.d;
             T *qi = static_cast<T *>(p.di) + t.b * p.sdi[0] + t.t0 * p.sdi[1] + t.d;
@@ -862,19 +931,15 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                 }
 #pragma unroll
                 for (int u = 0; u < TP; ++u) {
-                    x[u] = sm.in[2][j0 + u][tid];
-                    gi[u] = sm.in[3][j0 + u][tid];
-                    hp[u] = sm.in[4][j0 + u][tid];
-                }
-#pragma unroll
-                for (int u = 0; u < TP; ++u) {
+                    x[u] = sm.in.v[buf][1][trow + j0 + u][lane];
+                    gi[u] = sm.in.v[buf][2][trow + j0 + u][lane];
+                    hp[u] = sm.in.v[buf][4][trow + j0 + u][lane];
                     if (t.t0 + j0 + u == 0 || (cut >> (j0 + u) & 1))  // the initial state, or none
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) hp[u].v[e] = cvt_out<T>(0.f);
                 }
 #pragma unroll
                 for (int z = 0; z < TP * VEC / 2; ++z) {
-                    const int q = j0 * VEC / 2 + z;
                     const float2 xv = pair_of<T, VEC, TP>(x, z), av = a[z];
                     float2 prev = pair_of<T, VEC, TP>(hp, z);
                     if (t.t0 + j0 == 0 && f.h0 && !(cut >> j0 & 1)) {  // h_{-1}, in FP32
@@ -882,17 +947,18 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                         if (VEC > 1) prev.y = f.h0[(int64_t)t.b * f.D + t.d + (2 * z + 1) % VEC];
                     }
                     const float2 ei = exp_neg<PRECISE>(clamp_gate<PRECISE>(pair_of<T, VEC, TP>(gi, z)));
-                    const float2 qi = __fadd2_rn(ei, both(1.f));
-                    const float2 si = make_float2(rcp_approx(qi.x), rcp_approx(qi.y));
+                    const float2 qi1 = __fadd2_rn(ei, both(1.f));
+                    const float2 si = make_float2(rcp_approx(qi1.x), rcp_approx(qi1.y));
                     const float2 m2 = one_minus_a2<PRECISE>(y[z], av), m1 = __fadd2_rn(m2, both(kTiny));
                     const float2 w = make_float2(rsqrt_approx(m1.x), rsqrt_approx(m1.y));
-                    const float2 gs2 = __fmul2_rn(G[z], si);                      // G sigmoid(i)
-                    const float2 gx = __fmul2_rn(gs2, __fmul2_rn(m2, w));         // * sqrt(m)
+                    const float2 gs2 = __fmul2_rn(G[z], si);               // G sigmoid(i)
+                    const float2 gx = __fmul2_rn(gs2, __fmul2_rn(m2, w));  // * sqrt(m)
                     const float2 gi2 = __fmul2_rn(__fmul2_rn(gx, xv), __fmul2_rn(ei, si));
                     // E = a (G si x a (y / sqrt(m)) - y G h_{t-1}); y / sqrt(m) first, it tends to 0
                     const float2 u1 = __fmul2_rn(__fmul2_rn(gs2, xv), __fmul2_rn(av, __fmul2_rn(y[z], w)));
                     const float2 u2 = __ffma2_rn(__fmul2_rn(__fmul2_rn(y[z], both(-1.f)), G[z]), prev, u1);
                     const float2 E = __fmul2_rn(av, u2);
+                    const int q = j0 * VEC / 2 + z;
                     const float2 os = PRECISE ? om[PRECISE ? q : 0] : __ffma2_rn(sg[q], both(-1.f), both(1.f));
                     const float2 gr = __fmul2_rn(E, os);
 #pragma unroll
@@ -913,7 +979,6 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
                         *reinterpret_cast<Pack<T, VEC> *>(qr + j * p.sdr[1]) = orr[u];
                     }
             }
-            fetch_rest(tn, next);
             // the sum of E per channel, warps in order
             if (!WALK || !next) {
 #pragma unroll
@@ -932,8 +997,8 @@ __global__ void __launch_bounds__(32 * W, CTAS) recurrence_bwd_kernel(const BwdP
             if (warp == 0 && t.in)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) part[e] = 0.f;
-            fetch_first(tn, next);
-            fetch_rest(tn, next);
+            if (next) fetch(tn, buf ^ 1);
+            if (!TMA) copy_commit();
         }
         if (!next) break;
         t = tn;
@@ -1066,28 +1131,29 @@ FwdParams fwd_params(const MambaRecurrenceArgs *a) {
     return p;
 }
 
-// Tile shapes: channels a thread holds (1 serves any alignment and channel
-// count), tokens a warp holds, warps and CTAs per SM.
-template <int VEC_, int S_, int W_, int CTAS_>
+// Tile shapes: channels a thread holds, tokens a warp holds, warps, CTAs per SM.
+// The ...One shapes, without tensor maps, serve any alignment and strides.
+template <int VEC_, int S_, int W_, int CTAS_, bool TMA_ = true>
 struct Shape {
     static constexpr int VEC = VEC_, S = S_, W = W_, CTAS = CTAS_, tile = S_ * W_;
+    static constexpr bool TMA = TMA_;
 };
 template <typename T> struct Shapes;
 template <> struct Shapes<__half> {
     using Fwd = Shape<4, 8, 4, 4>;
-    using FwdOne = Shape<1, 8, 4, 4>;
-    using FwdWalk = Shape<4, 8, 8, 2>;
+    using FwdOne = Shape<1, 8, 4, 4, false>;
+    using FwdWalk = Shape<2, 16, 4, 4>;
     using Bwd = Shape<4, 4, 4, 4>;
-    using BwdOne = Shape<1, 8, 4, 4>;
-    using BwdWalk = Shape<4, 4, 8, 2>;
+    using BwdOne = Shape<1, 8, 4, 4, false>;
+    using BwdWalk = Shape<2, 8, 4, 4>;
 };
 template <> struct Shapes<float> {
     using Fwd = Shape<2, 8, 4, 5>;
-    using FwdOne = Shape<1, 8, 4, 5>;
+    using FwdOne = Shape<1, 8, 4, 5, false>;
     using FwdWalk = Shape<2, 8, 4, 5>;
-    using Bwd = Shape<2, 8, 4, 4>;
-    using BwdOne = Shape<1, 8, 4, 4>;
-    using BwdWalk = Shape<2, 8, 4, 4>;
+    using Bwd = Shape<1, 8, 4, 4>;
+    using BwdOne = Shape<1, 8, 4, 4, false>;
+    using BwdWalk = Shape<1, 8, 4, 4>;
 };
 
 // The chains of a call and where its workspace holds what.
@@ -1169,8 +1235,8 @@ __global__ void __launch_bounds__(256)
 // Launches one variant.  Tickets: the workspace's preparation, then as many
 // persistent CTAs as fit; walking: one CTA per chain, no preparation.
 template <typename Sh, bool WALK, typename Kernel, typename Params>
-int launch_tiles(Kernel kernel, const Params &p, const FwdParams &f, Plan &pl, size_t smem, void *ws, cudaStream_t st,
-                 const char *what) {
+int launch_tiles(Kernel kernel, const Params &p, const FwdParams &f, Plan &pl, const TileMaps &maps, size_t smem,
+                 void *ws, cudaStream_t st, const char *what) {
     Chains &c = pl.ch;
     if (allow_smem(kernel, smem)) return -1;
     const int64_t sms = device_sm_count();
@@ -1190,7 +1256,7 @@ int launch_tiles(Kernel kernel, const Params &p, const FwdParams &f, Plan &pl, s
         if (launch_status(what)) return -1;
         grid = std::min(grid * c.tiles, Sh::CTAS * sms);
     }
-    kernel<<<(unsigned)grid, 32 * Sh::W, smem, st>>>(p, c);
+    kernel<<<(unsigned)grid, 32 * Sh::W, smem, st>>>(p, c, maps);
     return launch_status(what);
 }
 
@@ -1203,65 +1269,106 @@ bool walks(const Plan &pl) {
     return chains * 10 >= ceil_div64(chains, slots) * slots * 6 || pl.ch.tiles == 1;
 }
 
+// Tensor map of [batch, seqlen, dim] with boxes of `tokens` x `chans`; false
+// where the hardware cannot describe it (the caller then takes the kernels
+// without tensor maps).  The outer dimension with the larger stride comes last.
+template <typename T>
+bool encode_tile(CUtensorMap *m, const void *ptr, const int64_t *s, int B, int L, int D, int chans, int tokens,
+                 unsigned bit, unsigned &row_first) {
+    constexpr int64_t es = sizeof(T);
+    if (!ptr || !aligned_to(ptr, 16)) return false;
+    // a dimension of one element has no stride of its own
+    const int64_t row = ((int64_t)D * es + 15) / 16 * 16;
+    int64_t st = L > 1 ? s[1] * es : row, sb = B > 1 ? s[0] * es : st * std::max(L, 1);
+    const bool swap = B > 1 && L > 1 && sb < st;
+    if (B > 1 && L == 1) st = row;
+    const int64_t s1 = swap ? sb : st, s2 = swap ? st : std::max(sb, s1);
+    if (s1 < D * es || s1 % 16 || s2 % 16 || s1 >= (1ll << 40) || s2 >= (1ll << 40)) return false;
+    if (B > 1 && !swap && sb != s2) return false;
+    auto enc = tensor_map_encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)(swap ? B : L), (cuuint64_t)(swap ? L : B)};
+    const cuuint64_t strides[2] = {(cuuint64_t)s1, (cuuint64_t)s2};
+    const cuuint32_t box[3] = {(cuuint32_t)chans, (cuuint32_t)(swap ? 1 : tokens), (cuuint32_t)(swap ? tokens : 1)};
+    const cuuint32_t one[3] = {1, 1, 1};
+    if (swap) row_first |= bit;
+    return enc(m, es == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3,
+               const_cast<void *>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, typename Sh, bool WALK>
-int launch_forward(const MambaRecurrenceArgs *a, Plan &pl, void *ws, cudaStream_t st) {
-    const FwdParams p = fwd_params(a);
-    return launch_tiles<Sh, WALK>(recurrence_fwd_kernel<T, Sh::VEC, Sh::S, Sh::W, Sh::CTAS, WALK>, p, p, pl,
+int launch_forward(const FwdParams &p, Plan &pl, const TileMaps &maps, void *ws, cudaStream_t st) {
+    return launch_tiles<Sh, WALK>(recurrence_fwd_kernel<T, Sh::VEC, Sh::S, Sh::W, Sh::CTAS, Sh::TMA, WALK>, p, p, pl, maps,
                                   sizeof(FwdSmem<T, Sh::VEC, Sh::S, Sh::W, WALK>), ws, st, "gated_recurrence kernel");
+}
+// The forward's tensors (x, r, i first: the order of the kernel's buffers).
+template <typename T, typename Sh>
+bool forward_maps(FwdParams &p, TileMaps &maps) {
+    p.row_first = 0;
+    if (p.D % Sh::VEC || p.L == 0) return false;
+    auto enc = [&](int k, const void *ptr, const int64_t *s) {
+        return encode_tile<T>(&maps.m[k], ptr, s, p.B, p.L, p.D, 32 * Sh::VEC, Sh::tile, 1u << k, p.row_first);
+    };
+    return enc(0, p.r, p.sr) && enc(1, p.i, p.si) && enc(2, p.x, p.sx) && vector_rows<T, Sh::VEC>(p.h, p.sh);
 }
 template <typename T>
 int choose_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
     using S = Shapes<T>;
-    constexpr int V = S::Fwd::VEC;
-    auto vec = [&](auto v) {
-        constexpr int N = decltype(v)::value;
-        return a->dim % N == 0 && vector_rows<T, N>(a->x, a->x_stride) && vector_rows<T, N>(a->r, a->r_stride) &&
-               vector_rows<T, N>(a->i, a->i_stride) && vector_rows<T, N>(a->h, a->h_stride);
-    };
+    FwdParams p = fwd_params(a);
+    TileMaps maps;
     Plan pl;
     const char *many = "gated_recurrence: too many tiles";
     MB_CHECK_ARG(plan_chains<typename S::FwdWalk>(a, false, pl), many);
-    if (vec(std::integral_constant<int, S::FwdWalk::VEC>()) && walks<typename S::FwdWalk>(pl))
-        return launch_forward<T, typename S::FwdWalk, true>(a, pl, ws, st);
-    if (vec(std::integral_constant<int, V>())) {
+    if (walks<typename S::FwdWalk>(pl) && forward_maps<T, typename S::FwdWalk>(p, maps))
+        return launch_forward<T, typename S::FwdWalk, true>(p, pl, maps, ws, st);
+    if (forward_maps<T, typename S::Fwd>(p, maps)) {
         MB_CHECK_ARG(plan_chains<typename S::Fwd>(a, false, pl), many);
-        return launch_forward<T, typename S::Fwd, false>(a, pl, ws, st);
+        return launch_forward<T, typename S::Fwd, false>(p, pl, maps, ws, st);
     }
     MB_CHECK_ARG(plan_chains<typename S::FwdOne>(a, false, pl), many);
-    return launch_forward<T, typename S::FwdOne, false>(a, pl, ws, st);
+    return launch_forward<T, typename S::FwdOne, false>(p, pl, maps, ws, st);
 }
 
 template <typename T, typename Sh, bool WALK>
-int launch_backward(const MambaRecurrenceArgs *a, BwdParams &p, Plan &pl, void *ws, cudaStream_t st) {
+int launch_backward(BwdParams &p, Plan &pl, const TileMaps &maps, void *ws, cudaStream_t st) {
     p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + pl.csp_bytes);
-    return launch_tiles<Sh, WALK>(recurrence_bwd_kernel<T, Sh::VEC, Sh::S, Sh::W, Sh::CTAS, WALK>, p, p.f, pl,
+    return launch_tiles<Sh, WALK>(recurrence_bwd_kernel<T, Sh::VEC, Sh::S, Sh::W, Sh::CTAS, Sh::TMA, WALK>, p, p.f, pl, maps,
                                   sizeof(BwdSmem<T, Sh::VEC, Sh::S, Sh::W, WALK>), ws, st,
                                   "gated_recurrence_backward kernel");
+}
+// The backward's tensors (r, x, i, dh, h: the order of the kernel's buffers).
+template <typename T, typename Sh>
+bool backward_maps(BwdParams &p, TileMaps &maps) {
+    FwdParams &f = p.f;
+    f.row_first = 0;
+    if (f.D % Sh::VEC || f.L == 0) return false;
+    auto enc = [&](int k, const void *ptr, const int64_t *s) {
+        return encode_tile<T>(&maps.m[k], ptr, s, f.B, f.L, f.D, 32 * Sh::VEC, Sh::tile, 1u << k, f.row_first);
+    };
+    return enc(0, f.r, f.sr) && enc(1, f.x, f.sx) && enc(2, f.i, f.si) && enc(3, p.dh, p.sdh) && enc(4, f.h, f.sh) &&
+           vector_rows<T, Sh::VEC>(p.dx, p.sdx) && vector_rows<T, Sh::VEC>(p.dr, p.sdr) &&
+           vector_rows<T, Sh::VEC>(p.di, p.sdi);
 }
 template <typename T>
 int choose_backward(const MambaRecurrenceArgs *a, BwdParams &p, const MambaRecurrenceGrads *g, void *ws,
                     cudaStream_t st) {
     using S = Shapes<T>;
-    auto vec = [&](auto v) {
-        constexpr int N = decltype(v)::value;
-        return a->dim % N == 0 && vector_rows<T, N>(a->x, a->x_stride) && vector_rows<T, N>(a->r, a->r_stride) &&
-               vector_rows<T, N>(a->i, a->i_stride) && vector_rows<T, N>(a->h, a->h_stride) &&
-               vector_rows<T, N>(g->dh, g->dh_stride) && vector_rows<T, N>(g->dx, g->dx_stride) &&
-               vector_rows<T, N>(g->dr, g->dr_stride) && vector_rows<T, N>(g->di, g->di_stride);
-    };
+    TileMaps maps;
     Plan pl;
     const char *many = "gated_recurrence_backward: too many tiles";
     int64_t rows = a->batch;
     MB_CHECK_ARG(plan_chains<typename S::BwdWalk>(a, true, pl), many);
-    if (vec(std::integral_constant<int, S::BwdWalk::VEC>()) && walks<typename S::BwdWalk>(pl)) {
-        if (launch_backward<T, typename S::BwdWalk, true>(a, p, pl, ws, st)) return -1;
-    } else if (vec(std::integral_constant<int, S::Bwd::VEC>())) {
+    if (walks<typename S::BwdWalk>(pl) && backward_maps<T, typename S::BwdWalk>(p, maps)) {
+        if (launch_backward<T, typename S::BwdWalk, true>(p, pl, maps, ws, st)) return -1;
+    } else if (backward_maps<T, typename S::Bwd>(p, maps)) {
         MB_CHECK_ARG(plan_chains<typename S::Bwd>(a, true, pl), many);
-        if (launch_backward<T, typename S::Bwd, false>(a, p, pl, ws, st)) return -1;
+        if (launch_backward<T, typename S::Bwd, false>(p, pl, maps, ws, st)) return -1;
         rows *= pl.ch.tiles;
     } else {
         MB_CHECK_ARG(plan_chains<typename S::BwdOne>(a, true, pl), many);
-        if (launch_backward<T, typename S::BwdOne, false>(a, p, pl, ws, st)) return -1;
+        if (launch_backward<T, typename S::BwdOne, false>(p, pl, maps, ws, st)) return -1;
         rows *= pl.ch.tiles;
     }
     recurrence_dlambda_kernel<<<(unsigned)ceil_div(a->dim, 32), 32 * kSumWarps, 0, st>>>(p.part, a->lambda,
