@@ -179,7 +179,7 @@ constexpr int kThreads = 128;
 // is ready first would not), and results repeat bit for bit.
 // A published value is one machine word that says itself whether it is there:
 // the workspace starts as all ones bits (a NaN that no published value has).
-constexpr int max_group_shift(int vec) { return vec == 4 ? 3 : 4; }  // what shared memory has room for
+constexpr int kMaxGroupShift = 4;
 constexpr unsigned kErrRecurrenceTimeout = 64u;
 constexpr uint32_t kEmpty = 0xffffffffu;
 
@@ -373,7 +373,7 @@ __device__ __forceinline__ Tile place_tile(const Chains &c, const FwdParams &p, 
 // between them; `wm` holds the maps of this tile's warps.  Syncs the CTA.
 template <int VEC, int W>
 __device__ __forceinline__ Maps<VEC> prefix_maps(const Chains &c, const Tile &t, const MapRows<VEC, W> &wm,
-                                                 MapRows<VEC, (1 << max_group_shift(VEC)) - 1> &gm) {
+                                                 MapRows<VEC, (1 << kMaxGroupShift) - 1> &gm) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int j = t.j;
     for (int tile = warp; tile < j; tile += W) {
@@ -469,14 +469,29 @@ __device__ __forceinline__ void await_box(uint64_t *bar, uint32_t use) {
     if (!mbar_wait_bounded(bar, use & 1)) atomicOr(&g_recurrence_error, kErrRecurrenceTimeout);
 }
 
-// Copies one element (at least 4 bytes asynchronously, 2 bytes at once).
+// Without TMA: FP32 elements are copied to shared memory asynchronously.  FP16
+// ones are too small for that; they wait in registers (held) and go to shared
+// memory when their tile's turn comes (put_held).
+template <typename T, int N, int S>
+struct Held {
+    T v[N][S];
+};
 template <typename T>
-__device__ __forceinline__ void copy_one(Pack<T, 1> *dst, const T *src) {
-    if constexpr (sizeof(T) >= 4)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"((int)sizeof(T))
-                     : "memory");
+__device__ __forceinline__ void copy_one(Pack<T, 1> *dst, T &held, const T *src) {
+    if constexpr (sizeof(T) == 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
     else
-        dst->v[0] = *src;
+        held = *src;
+}
+template <typename T, int N, int S, int TT>
+__device__ __forceinline__ void put_held(Pack<T, 1> (&dst)[N][TT][32], const Held<T, N, S> &held, int row, int cnt) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                if (j < cnt) dst[k][row + j][threadIdx.x & 31].v[0] = held.v[k][j];
+    }
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -507,7 +522,7 @@ template <typename T, int VEC, int S, int W, bool WALK>
 struct FwdSmem {
     TileIn<T, VEC, S * W, 3, 1> in;
     MapRows<VEC, W> wm[WALK ? 2 : 1];
-    MapRows<VEC, WALK ? 1 : (1 << max_group_shift(VEC)) - 1> gm;
+    MapRows<VEC, WALK ? 1 : (1 << kMaxGroupShift) - 1> gm;
     unsigned int ticket[2];
 };
 
@@ -535,6 +550,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
         t.cnt = t.in ? min(max(t.n - t.t0, 0), S) : 0;
         return t;
     };
+    Held<T, 3, TMA ? 1 : S> held;
     auto fetch = [&](const Tile &t) {
         if constexpr (TMA) {
             if (tid == 0) {
@@ -553,9 +569,9 @@ __global__ void __launch_bounds__(32 * W, CTAS)
             for (int j = 0; j < S; ++j)
                 if (j < t.cnt) {
                     if constexpr (VEC == 1) {
-                        copy_one<T>(&sm.in.v[0][0][warp * S + j][lane], pr + j * p.sr[1]);
-                        copy_one<T>(&sm.in.v[0][1][warp * S + j][lane], pi + j * p.si[1]);
-                        copy_one<T>(&sm.in.v[0][2][warp * S + j][lane], px + j * p.sx[1]);
+                        copy_one<T>(&sm.in.v[0][0][warp * S + j][lane], held.v[0][j], pr + j * p.sr[1]);
+                        copy_one<T>(&sm.in.v[0][1][warp * S + j][lane], held.v[1][j], pi + j * p.si[1]);
+                        copy_one<T>(&sm.in.v[0][2][warp * S + j][lane], held.v[2][j], px + j * p.sx[1]);
                     }
                 }
             copy_commit();
@@ -588,10 +604,12 @@ __global__ void __launch_bounds__(32 * W, CTAS)
             next = v < total;
             if (next) tn = place(v);
         }
-        if constexpr (TMA)
+        if constexpr (TMA) {
             await_box(&sm.in.full[0], it);
-        else
+        } else {
             copy_wait<0>();
+            put_held(sm.in.v[0], held, warp * S, t.cnt);
+        }
         if (t.live) {
             if (!WALK)
 #pragma unroll
@@ -703,7 +721,7 @@ template <typename T, int VEC, int S, int W, bool WALK>
 struct BwdSmem {
     TileIn<T, VEC, S * W, 5, 2> in;
     MapRows<VEC, W> wm[WALK ? 2 : 1];
-    MapRows<VEC, WALK ? 1 : (1 << max_group_shift(VEC)) - 1> gm;
+    MapRows<VEC, WALK ? 1 : (1 << kMaxGroupShift) - 1> gm;
     Pack<float, VEC> sums[W][32];
     unsigned int ticket[2];
 };
@@ -736,6 +754,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
         t.cnt = t.in && t.live ? min(max(t.n - t.t0, 0), S) : 0;
         return t;
     };
+    Held<T, 5, TMA ? 1 : S> held;
     auto fetch = [&](const Tile &t, int buf) {
         if constexpr (TMA) {
             if (tid == 0) {
@@ -760,11 +779,11 @@ __global__ void __launch_bounds__(32 * W, CTAS)
                 if (j < t.cnt) {
                     const int row = trow + j;
                     if constexpr (VEC == 1) {
-                        copy_one<T>(&sm.in.v[buf][0][row][lane], pr + j * f.sr[1]);
-                        copy_one<T>(&sm.in.v[buf][1][row][lane], px + j * f.sx[1]);
-                        copy_one<T>(&sm.in.v[buf][2][row][lane], pi + j * f.si[1]);
-                        copy_one<T>(&sm.in.v[buf][3][row][lane], pg + j * p.sdh[1]);
-                        if (t.t0 + j > 0) copy_one<T>(&sm.in.v[buf][4][row][lane], ph + j * f.sh[1]);
+                        copy_one<T>(&sm.in.v[buf][0][row][lane], held.v[0][j], pr + j * f.sr[1]);
+                        copy_one<T>(&sm.in.v[buf][1][row][lane], held.v[1][j], px + j * f.sx[1]);
+                        copy_one<T>(&sm.in.v[buf][2][row][lane], held.v[2][j], pi + j * f.si[1]);
+                        copy_one<T>(&sm.in.v[buf][3][row][lane], held.v[3][j], pg + j * p.sdh[1]);
+                        if (t.t0 + j > 0) copy_one<T>(&sm.in.v[buf][4][row][lane], held.v[4][j], ph + j * f.sh[1]);
                     }
                 }
         }
@@ -798,10 +817,12 @@ __global__ void __launch_bounds__(32 * W, CTAS)
             next = v < total;
             if (next) tn = place(v);
         }
-        if constexpr (TMA)
+        if constexpr (TMA) {
             await_box(&sm.in.full[buf], it >> 1);
-        else
+        } else {
             copy_wait<0>();
+            put_held(sm.in.v[buf], held, trow, t.cnt);
+        }
         // WALK: one row of sums per chain, else one per tile
         float *part = p.part + (WALK ? (int64_t)t.b : (int64_t)t.b * ch.tiles + t.k) * f.D + t.d;
         if (t.live) {
@@ -1140,16 +1161,16 @@ struct Shape {
 };
 template <typename T> struct Shapes;
 template <> struct Shapes<__half> {
-    using Fwd = Shape<4, 8, 4, 4>;
-    using FwdOne = Shape<1, 8, 4, 4, false>;
+    using Fwd = Shape<2, 16, 4, 4>;
+    using FwdOne = Shape<1, 16, 4, 4, false>;
     using FwdWalk = Shape<2, 16, 4, 4>;
-    using Bwd = Shape<4, 4, 4, 4>;
-    using BwdOne = Shape<1, 8, 4, 4, false>;
+    using Bwd = Shape<2, 8, 4, 4>;
+    using BwdOne = Shape<1, 8, 4, 3, false>;
     using BwdWalk = Shape<2, 8, 4, 4>;
 };
 template <> struct Shapes<float> {
-    using Fwd = Shape<2, 8, 4, 5>;
-    using FwdOne = Shape<1, 8, 4, 5, false>;
+    using Fwd = Shape<1, 16, 8, 3>;
+    using FwdOne = Shape<1, 8, 4, 6, false>;
     using FwdWalk = Shape<2, 8, 4, 5>;
     using Bwd = Shape<1, 8, 4, 4>;
     using BwdOne = Shape<1, 8, 4, 4, false>;
@@ -1174,7 +1195,7 @@ bool plan_chains(const MambaRecurrenceArgs *a, bool backward, Plan &pl) {
     c.blocks = divisor(blocks);
     c.chains = divisor(blocks * a->batch);
     c.tiles = (int)tiles;
-    c.group_shift = std::min(max_group_shift(Sh::VEC), tiles <= 128 ? 2 : tiles <= 1024 ? 3 : 4);
+    c.group_shift = std::min(kMaxGroupShift, tiles <= 128 ? 2 : tiles <= 1024 ? 3 : 4);
     c.group = 1 << c.group_shift;
     c.groups = ceil_div((int)tiles, c.group);
     // csp, the backward's partial sums, then what starts as all ones bits:
@@ -1328,7 +1349,8 @@ int choose_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
         return launch_forward<T, typename S::Fwd, false>(p, pl, maps, ws, st);
     }
     MB_CHECK_ARG(plan_chains<typename S::FwdOne>(a, false, pl), many);
-    return launch_forward<T, typename S::FwdOne, false>(p, pl, maps, ws, st);
+    return walks<typename S::FwdOne>(pl) ? launch_forward<T, typename S::FwdOne, true>(p, pl, maps, ws, st)
+                                         : launch_forward<T, typename S::FwdOne, false>(p, pl, maps, ws, st);
 }
 
 template <typename T, typename Sh, bool WALK>
@@ -1368,8 +1390,11 @@ int choose_backward(const MambaRecurrenceArgs *a, BwdParams &p, const MambaRecur
         rows *= pl.ch.tiles;
     } else {
         MB_CHECK_ARG(plan_chains<typename S::BwdOne>(a, true, pl), many);
-        if (launch_backward<T, typename S::BwdOne, false>(p, pl, maps, ws, st)) return -1;
-        rows *= pl.ch.tiles;
+        const bool walk = walks<typename S::BwdOne>(pl);
+        if (walk ? launch_backward<T, typename S::BwdOne, true>(p, pl, maps, ws, st)
+                 : launch_backward<T, typename S::BwdOne, false>(p, pl, maps, ws, st))
+            return -1;
+        if (!walk) rows *= pl.ch.tiles;
     }
     recurrence_dlambda_kernel<<<(unsigned)ceil_div(a->dim, 32), 32 * kSumWarps, 0, st>>>(p.part, a->lambda,
                                                                                          g->dlambda, rows, a->dim);
