@@ -109,7 +109,8 @@ const char *mamba_last_error(void);
  * the decode state update's bulk-copy waits (mamba_ssm_step, mamba_step).
  * Bit 6: a wait of mamba_gated_recurrence or its backward pass for the
  * sequence tile before it exceeded the same bound.  Bit 7: the same as bit 4
- * for mamba_linear_i8's tensor-core kernel.
+ * for mamba_linear_i8's tensor-core kernel.  Bit 8: the same for the row
+ * fetches of mamba_block_norm and its backward pass.
  * Waits for the device; clear != 0 resets them. */
 unsigned mamba_device_status(int clear);
 

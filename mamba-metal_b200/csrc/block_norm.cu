@@ -14,10 +14,16 @@
 #include "common.cuh"
 #include "internal.h"
 #include "scan_math.cuh"
+#include "tma.cuh"
 
 #include <algorithm>
+#include <mutex>
+#include <utility>
+#include <vector>
 
 namespace mb {
+
+__device__ unsigned int g_block_norm_error = 0;
 
 namespace {
 
@@ -53,7 +59,7 @@ __device__ __forceinline__ void silu_grad(float z, float &g, float &dg) {
 }
 
 constexpr int kMaxCols = 16384;
-constexpr int kMaxParts = 444;  // CTAs (and column-sum partials) of the backward pass
+constexpr int kDirectParts = 296;  // CTAs of the backward pass without a ring: few, so that their partial sums are
 
 // N consecutive elements as FP32; N = 8 by 16-byte accesses.
 template <int N>
@@ -137,17 +143,81 @@ __device__ __forceinline__ float block_sum(float v, float *sm, int &turn) {
     return v;
 }
 
+// With many rows (RING): persistent CTAs whose rows arrive through shared
+// memory.  One thread fetches each row by untiled bulk copies (one per tensor)
+// into a ring of `stages` rows, that far ahead, so that loads stay in flight
+// through a row's two sums and the threads spend no registers on them.  A
+// row's place is free again behind the first sum, when every thread has the
+// row in registers.
+constexpr unsigned kErrBlockNormTimeout = 256u;
+constexpr int kMaxStages = 4;
+constexpr int kRingBytes = 224 * 1024;                    // shared memory of an SM, with room for the static parts
+constexpr int kRingThreads = 1024, kRingBwdThreads = 768;  // resident threads per SM
+
+template <int N>
+struct RingRow {
+    const void *src[N];    // first row of each tensor
+    int64_t stride[N];     // bytes between rows
+    uint32_t bytes[N];     // bytes of a row, 0: tensor absent
+    uint32_t offset[N];    // within a stage
+    uint32_t stage, total; // bytes of a stage, bytes fetched per row
+    int stages;
+};
+
+template <int N>
+__device__ __forceinline__ void fetch_row(const RingRow<N> &r, uint8_t *ring, uint64_t *full, int64_t row, int s) {
+    mbar_arrive_expect_tx(&full[s], r.total);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        if (r.bytes[k])
+            bulk_load(ring + s * r.stage + r.offset[k], static_cast<const uint8_t *>(r.src[k]) + row * r.stride[k],
+                      r.bytes[k], &full[s]);
+}
+__device__ __forceinline__ void await_row(uint64_t *bar, uint32_t parity) {
+    if (!mbar_wait_bounded(bar, parity)) atomicOr(&g_block_norm_error, kErrBlockNormTimeout);
+}
+// Place s of the ring in use, and the parity of that use.
+struct RingPlace {
+    int s = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void step(int stages) {
+        if (++s == stages) {
+            s = 0;
+            parity ^= 1;
+        }
+    }
+};
+// Sets the ring up and fetches the first rows; rows first, first + step, ...
+template <int N>
+__device__ __forceinline__ void start_ring(const RingRow<N> &r, uint8_t *ring, uint64_t *full, int64_t rows) {
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < r.stages; ++s) mbar_init(&full[s], 1);
+        fence_mbar_init();
+        int64_t row = blockIdx.x;
+        for (int s = 0; s < r.stages && row < rows; ++s, row += gridDim.x) fetch_row<N>(r, ring, full, row, s);
+    }
+    __syncthreads();
+}
+
 // One CTA per row, the row in registers: thread t holds NV groups of VEC
 // channels, group j at channel (j * threads + t) * VEC.
-template <typename T, int VEC, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT) block_norm_kernel(const NormParams p) {
+template <typename T, int VEC, int NV, int MAXT, bool RING, int CTAS = 1>
+__global__ void __launch_bounds__(MAXT, CTAS) block_norm_kernel(const NormParams p, const RingRow<3> ring) {
     constexpr bool PRECISE = sizeof(T) == 4;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t full[kMaxStages];
     __shared__ float sm[64];
     int turn = 0;
     const float inv_cols = 1.f / (float)p.cols;
+    RingPlace at;
+    if (RING) start_ring<3>(ring, smem, full, p.rows);
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const T *y = static_cast<const T *>(p.y) + row * p.sy;
-        const T *z = p.z ? static_cast<const T *>(p.z) + row * p.sz : nullptr;
+        const uint8_t *place = smem + at.s * ring.stage;
+        const T *y = RING ? reinterpret_cast<const T *>(place) : static_cast<const T *>(p.y) + row * p.sy;
+        const T *z = RING ? reinterpret_cast<const T *>(place + ring.offset[1])
+                          : static_cast<const T *>(p.z) + row * p.sz;
+        const float *res = RING ? reinterpret_cast<const float *>(place + ring.offset[2]) : p.res + row * p.cols;
+        if (RING) await_row(&full[at.s], at.parity);
         float v[NV][VEC], gz[NV][VEC], r[NV][VEC];
         float ss = 0.f;
 #pragma unroll
@@ -155,13 +225,18 @@ __global__ void __launch_bounds__(MAXT) block_norm_kernel(const NormParams p) {
             const int c = (j * blockDim.x + threadIdx.x) * VEC;
             if (c < p.cols) {
                 load_n(y + c, v[j]);
-                if (z) load_n(z + c, gz[j]);
-                load_n(p.res + row * p.cols + c, r[j]);
+                if (p.z) load_n(z + c, gz[j]);
+                load_n(res + c, r[j]);
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) ss = fmaf(v[j][k], v[j][k], ss);
             }
         }
         const float rs = rsqrtf(block_sum(ss, sm, turn) * inv_cols + p.eps);
+        if (RING) {
+            const int64_t ahead = row + (int64_t)ring.stages * gridDim.x;
+            if (threadIdx.x == 0 && ahead < p.rows) fetch_row<3>(ring, smem, full, ahead, at.s);
+            at.step(ring.stages);
+        }
         float ss2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -172,7 +247,7 @@ __global__ void __launch_bounds__(MAXT) block_norm_kernel(const NormParams p) {
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
                     float n = v[j][k] * rs * w[k];
-                    if (z) {
+                    if (p.z) {
                         float g, dg;
                         silu_grad<PRECISE>(gz[j][k], g, dg);
                         n *= g;
@@ -203,19 +278,37 @@ __global__ void __launch_bounds__(MAXT) block_norm_kernel(const NormParams p) {
 
 // Backward: CTA k walks rows k, k + CTAs, ... and keeps the column sums of
 // its rows in registers; they leave as one partial row per CTA.
-template <typename T, int VEC, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT) block_norm_bwd_kernel(const NormGradParams p) {
+template <typename T, int VEC, int NV, int MAXT, bool RING, int CTAS = 1>
+__global__ void __launch_bounds__(MAXT, CTAS) block_norm_bwd_kernel(const NormGradParams p, const RingRow<5> ring) {
     constexpr bool PRECISE = sizeof(T) == 4;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t full[kMaxStages];
     __shared__ float sm[64];
     int turn = 0;
     const int cols = p.f.cols;
     const float inv_cols = 1.f / (float)cols;
     float acc_post[NV][VEC] = {}, acc_pre[NV][VEC] = {};
+    const bool first = p.dout != nullptr;  // the second norm's output has a gradient
+    RingPlace at;
+    if (RING) start_ring<5>(ring, smem, full, p.f.rows);
+    float rs_next = p.f.rstd_post[blockIdx.x], rp_next = first ? p.f.rstd_pre[blockIdx.x] : 0.f;  // grid <= rows
     for (int64_t row = blockIdx.x; row < p.f.rows; row += gridDim.x) {
-        const T *y = static_cast<const T *>(p.f.y) + row * p.f.sy;
-        const T *z = p.f.z ? static_cast<const T *>(p.f.z) + row * p.f.sz : nullptr;
-        const T *go = p.dout ? static_cast<const T *>(p.dout) + row * cols : nullptr;
-        const float rs = p.f.rstd_post[row], rp = go ? p.f.rstd_pre[row] : 0.f;
+        const uint8_t *place = smem + at.s * ring.stage;
+        const T *y = RING ? reinterpret_cast<const T *>(place) : static_cast<const T *>(p.f.y) + row * p.f.sy;
+        const T *z = RING ? reinterpret_cast<const T *>(place + ring.offset[1])
+                          : static_cast<const T *>(p.f.z) + row * p.f.sz;
+        const T *go = RING ? reinterpret_cast<const T *>(place + ring.offset[2])
+                           : static_cast<const T *>(p.dout) + row * cols;
+        const float *dro = RING ? reinterpret_cast<const float *>(place + ring.offset[3]) : p.dres_out + row * cols;
+        const float *r1 = RING ? reinterpret_cast<const float *>(place + ring.offset[4]) : p.f.res_out + row * cols;
+        // this row's factors were loaded a row ago, the next row's are on their way
+        const float rs = rs_next, rp = rp_next;
+        const int64_t after = row + gridDim.x;
+        if (after < p.f.rows) {
+            rs_next = p.f.rstd_post[after];
+            if (first) rp_next = p.f.rstd_pre[after];
+        }
+        if (RING) await_row(&full[at.s], at.parity);
         float R[NV][VEC], n[NV][VEC], gz[NV][VEC], d[NV][VEC], m[NV][VEC];
         float dot = 0.f;
 #pragma unroll
@@ -223,11 +316,11 @@ __global__ void __launch_bounds__(MAXT) block_norm_bwd_kernel(const NormGradPara
             const int c = (j * blockDim.x + threadIdx.x) * VEC;
             if (c < cols) {
                 load_n(y + c, n[j]);
-                if (z) load_n(z + c, gz[j]);
-                if (p.dres_out) load_n(p.dres_out + row * cols + c, R[j]);
-                if (go) {
+                if (p.f.z) load_n(z + c, gz[j]);
+                if (p.dres_out) load_n(dro + c, R[j]);
+                if (first) {
                     load_n(go + c, d[j]);
-                    load_n(p.f.res_out + row * cols + c, m[j]);
+                    load_n(r1 + c, m[j]);
                 }
             }
         }
@@ -241,7 +334,7 @@ __global__ void __launch_bounds__(MAXT) block_norm_bwd_kernel(const NormGradPara
                 for (int k = 0; k < VEC; ++k) {
                     n[j][k] *= rs;
                     if (!p.dres_out) R[j][k] = 0.f;
-                    if (go) {
+                    if (first) {
                         m[j][k] *= rp;
                         acc_pre[j][k] = fmaf(d[j][k], m[j][k], acc_pre[j][k]);
                         d[j][k] *= w[k];
@@ -250,7 +343,13 @@ __global__ void __launch_bounds__(MAXT) block_norm_bwd_kernel(const NormGradPara
                 }
             }
         }
-        const float mean = go ? block_sum(dot, sm, turn) * inv_cols : 0.f;
+        // (without dout the sum is 0, and its barrier still frees the ring's place)
+        const float mean = RING || first ? block_sum(dot, sm, turn) * inv_cols : 0.f;
+        if (RING) {
+            const int64_t ahead = row + (int64_t)ring.stages * gridDim.x;
+            if (threadIdx.x == 0 && ahead < p.f.rows) fetch_row<5>(ring, smem, full, ahead, at.s);
+            at.step(ring.stages);
+        }
         float dot2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -258,7 +357,7 @@ __global__ void __launch_bounds__(MAXT) block_norm_bwd_kernel(const NormGradPara
             if (c < cols) {
                 float w[VEC], o[VEC];
                 load_weight(p.f.w_post, c, w);
-                if (go) {
+                if (first) {
 #pragma unroll
                     for (int k = 0; k < VEC; ++k)
                         R[j][k] = fmaf(rp, fmaf(-m[j][k], mean, d[j][k]), R[j][k]);
@@ -269,14 +368,14 @@ __global__ void __launch_bounds__(MAXT) block_norm_bwd_kernel(const NormGradPara
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
                     float g = 1.f, dg = 0.f;
-                    if (z) silu_grad<PRECISE>(gz[j][k], g, dg);
+                    if (p.f.z) silu_grad<PRECISE>(gz[j][k], g, dg);
                     const float Rn = R[j][k] * n[j][k];
                     acc_post[j][k] = fmaf(Rn, g, acc_post[j][k]);
                     o[k] = Rn * w[k] * dg;
                     R[j][k] *= w[k] * g;
                     dot2 = fmaf(R[j][k], n[j][k], dot2);
                 }
-                if (z) store_n(static_cast<T *>(p.dz) + row * p.sdz + c, o);
+                if (p.f.z) store_n(static_cast<T *>(p.dz) + row * p.sdz + c, o);
             }
         }
         const float mean2 = block_sum(dot2, sm, turn) * inv_cols;
@@ -374,31 +473,130 @@ bool vector_rows(const MambaBlockNormArgs *a) {
 
 int threads_for(int cols, int per_thread) { return std::max(32, (ceil_div(cols, per_thread) + 31) / 32 * 32); }
 
+// Opts a kernel into the shared memory of its ring, once per device.
+template <typename Kernel>
+int allow_smem(Kernel kernel) {
+    static std::mutex mu;
+    static std::vector<std::pair<const void *, int>> done;
+    int dev = 0;
+    MB_CUDA_TRY(cudaGetDevice(&dev));
+    const std::pair<const void *, int> key(reinterpret_cast<const void *>(kernel), dev);
+    std::lock_guard<std::mutex> lk(mu);
+    if (std::find(done.begin(), done.end(), key) != done.end()) return 0;
+    MB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes));
+    done.push_back(key);
+    return 0;
+}
+
+// CTAs per SM that a ring kernel wants.
+int ring_ctas(int threads, int resident) { return std::max(1, std::min(32, resident / threads)); }
+// Rows of partial column sums of the backward pass at most.
+int64_t max_parts(int64_t rows, int cols) {
+    const int ctas = std::min(16, ring_ctas(threads_for(cols, cols <= 4096 ? 8 : 16), kRingBwdThreads));
+    return std::min<int64_t>(rows, std::max(kDirectParts, 148 * ctas));
+}
+
+// Lays a ring out and lowers the CTAs per SM until each has room for two rows
+// (one, if at most two CTAs share the SM).  False where a row is larger than that, or
+// where CTAs would get too few rows for a ring to pay.
+template <int N>
+bool plan_ring(RingRow<N> &r, int64_t rows, int &ctas_per_sm) {
+    uint32_t at = 0;
+    r.total = 0;
+    for (int k = 0; k < N; ++k) {
+        r.offset[k] = at;
+        at += (r.bytes[k] + 127) / 128 * 128;
+        r.total += r.bytes[k];
+    }
+    r.stage = at;
+    for (;; --ctas_per_sm) {
+        r.stages = (int)std::min<uint32_t>(kMaxStages, (uint32_t)(kRingBytes / ctas_per_sm - 2048) / std::max(at, 1u));
+        if (r.stages >= 2 || (r.stages == 1 && ctas_per_sm == 2) || ctas_per_sm == 1) break;
+    }
+    return r.stages >= 1 && rows >= 3LL * ctas_per_sm * device_sm_count();
+}
+
+template <typename T, int NV, int MAXT>
+int ring_fwd(const NormParams &p, const RingRow<3> &r, int ctas, int threads, cudaStream_t st) {
+    auto kernel = block_norm_kernel<T, 8, NV, MAXT, true>;
+    if (allow_smem(kernel)) return -1;
+    kernel<<<(unsigned)(ctas * device_sm_count()), threads, (size_t)r.stage * r.stages, st>>>(p, r);
+    return launch_status("block_norm kernel");
+}
 template <typename T>
 int launch_fwd(const NormParams &p, bool vec, cudaStream_t st) {
+    RingRow<3> r{};
+    if (vec && p.cols <= 8192) {
+        const uint32_t half = (uint32_t)(p.cols * sizeof(T));
+        r.src[0] = p.y;
+        r.src[1] = p.z;
+        r.src[2] = p.res;
+        r.stride[0] = p.sy * (int64_t)sizeof(T);
+        r.stride[1] = p.sz * (int64_t)sizeof(T);
+        r.stride[2] = p.cols * 4LL;
+        r.bytes[0] = half;
+        r.bytes[1] = p.z ? half : 0;
+        r.bytes[2] = (uint32_t)p.cols * 4;
+        const bool one = p.cols <= 4096;
+        const int threads = threads_for(p.cols, one ? 8 : 16);
+        int ctas = ring_ctas(threads, kRingThreads);
+        if (plan_ring<3>(r, p.rows, ctas))
+            return one ? ring_fwd<T, 1, 512>(p, r, ctas, threads, st) : ring_fwd<T, 2, 512>(p, r, ctas, threads, st);
+    }
     const unsigned grid = (unsigned)std::min<int64_t>(p.rows, 0x7fffffff);
     if (vec && p.cols <= 4096)
-        block_norm_kernel<T, 8, 1, 512><<<grid, threads_for(p.cols, 8), 0, st>>>(p);
+        block_norm_kernel<T, 8, 1, 512, false><<<grid, threads_for(p.cols, 8), 0, st>>>(p, r);
     else if (vec)
-        block_norm_kernel<T, 8, 2, 1024><<<grid, threads_for(p.cols, 16), 0, st>>>(p);
+        block_norm_kernel<T, 8, 2, 1024, false><<<grid, threads_for(p.cols, 16), 0, st>>>(p, r);
     else if (p.cols <= 4096)
-        block_norm_kernel<T, 1, 4, 1024><<<grid, threads_for(p.cols, 4), 0, st>>>(p);
+        block_norm_kernel<T, 1, 4, 1024, false><<<grid, threads_for(p.cols, 4), 0, st>>>(p, r);
     else
-        block_norm_kernel<T, 1, 16, 1024><<<grid, threads_for(p.cols, 16), 0, st>>>(p);
+        block_norm_kernel<T, 1, 16, 1024, false><<<grid, threads_for(p.cols, 16), 0, st>>>(p, r);
     return launch_status("block_norm kernel");
 }
 
+template <typename T, int NV, int MAXT, int CTAS>
+int ring_bwd(const NormGradParams &p, const RingRow<5> &r, unsigned grid, int threads, cudaStream_t st) {
+    auto kernel = block_norm_bwd_kernel<T, 8, NV, MAXT, true, CTAS>;
+    if (allow_smem(kernel)) return -1;
+    kernel<<<grid, threads, (size_t)r.stage * r.stages, st>>>(p, r);
+    return launch_status("block_norm_backward kernel");
+}
+// grid: CTAs to launch at most; set to those launched (rows of partial sums).
 template <typename T>
-int launch_bwd(const NormGradParams &p, bool vec, unsigned grid, cudaStream_t st) {
+int launch_bwd(const NormGradParams &p, bool vec, unsigned &grid, cudaStream_t st) {
     const int cols = p.f.cols;
+    RingRow<5> r{};
+    if (vec && cols <= 8192) {
+        const uint32_t half = (uint32_t)(cols * sizeof(T)), whole = (uint32_t)cols * 4;
+        const void *src[5] = {p.f.y, p.f.z, p.dout, p.dres_out, p.f.res_out};
+        const int64_t stride[5] = {p.f.sy * (int64_t)sizeof(T), p.f.sz * (int64_t)sizeof(T), half, whole, whole};
+        for (int k = 0; k < 5; ++k) {
+            r.src[k] = src[k];
+            r.stride[k] = stride[k];
+            r.bytes[k] = k < 3 ? half : whole;
+            if (!src[k] || (k == 4 && !p.dout)) r.bytes[k] = 0;
+        }
+        const bool one = cols <= 4096;
+        const int threads = threads_for(cols, one ? 8 : 16);
+        int ctas = std::min(16, ring_ctas(threads, kRingBwdThreads));
+        if (plan_ring<5>(r, p.f.rows, ctas)) {
+            grid = std::min(grid, (unsigned)(ctas * device_sm_count()));
+            if (!one) return ring_bwd<T, 2, 512, 1>(p, r, grid, threads, st);
+            // three CTAs fit by 80 registers a thread; with fewer, more registers are faster
+            return threads <= 256 && ctas >= 3 ? ring_bwd<T, 1, 256, 3>(p, r, grid, threads, st)
+                                             : ring_bwd<T, 1, 512, 1>(p, r, grid, threads, st);
+        }
+    }
+    grid = std::min(grid, (unsigned)kDirectParts);
     if (vec && cols <= 4096)
-        block_norm_bwd_kernel<T, 8, 1, 512><<<grid, threads_for(cols, 8), 0, st>>>(p);
+        block_norm_bwd_kernel<T, 8, 1, 512, false><<<grid, threads_for(cols, 8), 0, st>>>(p, r);
     else if (vec)
-        block_norm_bwd_kernel<T, 8, 2, 1024><<<grid, threads_for(cols, 16), 0, st>>>(p);
+        block_norm_bwd_kernel<T, 8, 2, 1024, false><<<grid, threads_for(cols, 16), 0, st>>>(p, r);
     else if (cols <= 4096)
-        block_norm_bwd_kernel<T, 1, 4, 1024><<<grid, threads_for(cols, 4), 0, st>>>(p);
+        block_norm_bwd_kernel<T, 1, 4, 1024, false><<<grid, threads_for(cols, 4), 0, st>>>(p, r);
     else
-        block_norm_bwd_kernel<T, 1, 16, 1024><<<grid, threads_for(cols, 16), 0, st>>>(p);
+        block_norm_bwd_kernel<T, 1, 16, 1024, false><<<grid, threads_for(cols, 16), 0, st>>>(p, r);
     return launch_status("block_norm_backward kernel");
 }
 
@@ -407,7 +605,7 @@ int launch_bwd(const NormGradParams &p, bool vec, unsigned grid, cudaStream_t st
 size_t block_norm_workspace_bytes(const MambaBlockNormArgs *a) {
     if (!a || a->rows <= 0 || a->cols <= 0 || a->cols > kMaxCols) return 0;
     // two sets of partial rows, each starting on a 16-byte boundary
-    return 2 * (((size_t)std::min<int64_t>(a->rows, kMaxParts) * a->cols + 3) / 4 * 4) * sizeof(float);
+    return 2 * (((size_t)max_parts(a->rows, a->cols) * a->cols + 3) / 4 * 4) * sizeof(float);
 }
 
 int block_norm(const MambaBlockNormArgs *a, cudaStream_t st) {
@@ -443,7 +641,7 @@ int block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *
                  "block_norm_backward: rows of a gradient overlap (strides)");
     MB_CHECK_ARG(ws && ws_bytes >= block_norm_workspace_bytes(a) && aligned_to(ws, 16),
                  "block_norm_backward: workspace too small or not 16-byte aligned");
-    const unsigned grid = (unsigned)std::min<int64_t>(a->rows, kMaxParts);
+    unsigned grid = (unsigned)max_parts(a->rows, a->cols);  // launch_bwd may take fewer
     NormGradParams p{};
     p.f = norm_params(a);
     p.dres_out = g->dresidual_out;
@@ -455,7 +653,7 @@ int block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *
     p.sdz = g->dz_stride;
     float *part = static_cast<float *>(ws);
     if (g->dw_post) p.part_post = part;
-    if (g->dw_pre) p.part_pre = part + ((int64_t)grid * a->cols + 3) / 4 * 4;
+    if (g->dw_pre) p.part_pre = part + ((int64_t)grid * a->cols + 3) / 4 * 4;  // grid is still the most
     const bool vec = vector_rows(a) && aligned_to(g->dout, 16) && aligned_to(g->dresidual_out, 16) &&
                      aligned_to(g->dresidual, 16) && aligned_to(g->dy, 16) && aligned_to(g->dz, 16) &&
                      (g->dy_stride * (int64_t)es) % 16 == 0 && (!a->z || (g->dz_stride * (int64_t)es) % 16 == 0);
@@ -464,6 +662,16 @@ int block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *
     block_norm_sum_kernel<<<dim3((unsigned)ceil_div(a->cols, 32), 2), kSumThreads, 0, st>>>(
         p.part_post, p.part_pre, g->dw_post, g->dw_pre, (int)grid, a->cols);
     return launch_status("block_norm_backward sum kernel");
+}
+
+unsigned block_norm_error_flags(bool clear) {
+    unsigned v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_block_norm_error, sizeof(v)) != cudaSuccess) return ~0u;
+    if (clear && v) {
+        const unsigned z = 0;
+        cudaMemcpyToSymbol(g_block_norm_error, &z, sizeof(z));
+    }
+    return v;
 }
 
 }  // namespace mb

@@ -64,6 +64,7 @@ size_t block_norm_workspace_bytes(const MambaBlockNormArgs *a);
 int block_norm(const MambaBlockNormArgs *a, cudaStream_t st);
 int block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *g, void *ws, size_t ws_bytes,
                         cudaStream_t st);
+unsigned block_norm_error_flags(bool clear);
 
 // ssm_step.cu
 int ssm_step(const void *x, int64_t xrs, const void *delta, int64_t drs, const float *dt_bias,

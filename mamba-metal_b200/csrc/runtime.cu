@@ -1238,9 +1238,11 @@ unsigned mamba_device_status(int clear) {
     const unsigned step = mb::step_error_flags(clear != 0);
     const unsigned rec = mb::recurrence_error_flags(clear != 0);
     const unsigned i8 = mb::linear_i8_error_flags(clear != 0);
-    return (scan == ~0u || gemm == ~0u || lin == ~0u || proj == ~0u || step == ~0u || rec == ~0u || i8 == ~0u)
+    const unsigned norm = mb::block_norm_error_flags(clear != 0);
+    return (scan == ~0u || gemm == ~0u || lin == ~0u || proj == ~0u || step == ~0u || rec == ~0u || i8 == ~0u ||
+            norm == ~0u)
                ? ~0u
-               : (scan | gemm | lin | proj | step | rec | i8);
+               : (scan | gemm | lin | proj | step | rec | i8 | norm);
 }
 
 int mamba_selftest_bounded_wait(unsigned limit_us, void *stream) {

@@ -91,7 +91,9 @@ def _check_backward(v, f, grads, dtype):
 
 
 SHAPES = [(1, 1), (1, 8), (3, 7), (2, 64), (5, 256), (4, 264), (130, 1000), (9, 1001), (700, 72), (300, 2048),
-          (64, 2560), (3, 4096), (3, 4099), (2, 8192), (2, 8200), (2, 16384), (2, 12001)]
+          (64, 2560), (3, 4096), (3, 4099), (2, 8192), (2, 8200), (2, 16384), (2, 12001),
+          # enough rows for persistent CTAs with rows fetched ahead: 1, 2, 8 and 16 warps, one and two rows of room
+          (14500, 72), (7300, 264), (2000, 2048), (1000, 4096), (950, 8192)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
