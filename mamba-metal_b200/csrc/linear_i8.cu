@@ -352,13 +352,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int mt = tile / p.n_tiles, nt = tile % p.n_tiles;
             const int64_t row0 = (int64_t)mt * 256 + rank * 128 + quarter * 32, row = row0 + lane;
             const float xs = row < g.rows ? g.xs[row] : 0.f;
+            // The scales and biases of this warp's columns, one column per lane and
+            // 32 columns, fetched before the sums are there and handed round by
+            // shuffle: chunk q of cstep columns starts at column (2 q + egroup) cstep.
+            float wsc[4], wbi[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int j = 32 * q, c = nt * p.BN + (2 * (j / cstep) + egroup) * cstep + j % cstep + lane;
+                wsc[q] = c < g.n ? __ldg(g.ws + c) : 0.f;
+                wbi[q] = g.bias && c < g.n ? __ldg(g.bias + c) : 0.f;
+            }
             if (!warp_wait(&tfull[b], tph)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
             const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16) + b * kAccCols;
-            for (int c = egroup * cstep; c < p.BN; c += 2 * cstep) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {  // chunks of 64 columns: only q = 0, 1
+                const int c = (2 * q + egroup) * cstep;
+                if (c >= p.BN) break;
                 const int col = nt * p.BN + c;
                 if (col >= g.n || row0 >= g.rows) break;  // the same for the whole warp
                 uint8_t *box = boxes + (nbox & 1) * kBox;
@@ -369,18 +382,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) bulk_wait_group_read<1>();
                     __syncwarp();
                 }
-                for (int hlf = 0; hlf < (g.mode == 0 ? 2 : 1); ++hlf) {
+#pragma unroll
+                for (int hlf = 0; hlf < 2; ++hlf) {
+                    if (hlf && g.mode != 0) break;
                     const int c0 = col + 32 * hlf;
                     if (c + 32 * hlf >= p.BN) break;  // BN is a multiple of 32
                     uint32_t v[32];
                     tmem_ld_32x32b_x32(tl + c + 32 * hlf, v);
                     tmem_wait_ld();
                     float f[32];
+                    const float wl = g.mode == 0 ? wsc[(2 * q + hlf) & 3] : wsc[q];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const int cc = min(c0 + j, g.n - 1);
-                        f[j] = (float)(int)v[j] * xs * __ldg(g.ws + cc);
-                        if (g.bias) f[j] += __ldg(g.bias + cc);
+                    for (int j = 0; j < 32; ++j)
+                        f[j] = (float)(int)v[j] * xs * __shfl_sync(0xffffffffu, wl, j);
+                    if (g.bias) {
+                        const float bl = g.mode == 0 ? wbi[(2 * q + hlf) & 3] : wbi[q];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) f[j] += __shfl_sync(0xffffffffu, bl, j);
                     }
                     if (!boxed) {
                         if (row < g.rows) store_row(g, row, c0, f, p.boxes);
