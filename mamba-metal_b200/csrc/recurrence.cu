@@ -74,56 +74,65 @@ __device__ __forceinline__ float2 clamp_gate(float2 v) {
     return v;
 }
 
-// 1 - a^2 for a = exp(-y), without cancellation for y near 0: a series in
-// z = 2y for small y, (1 - a)(1 + a) where a's error of 2^-22 has lost its
-// weight.  PRECISE: Taylor to z^8 below y = 1/4 (relative error < (1/2)^8 / 9! =
-// 1e-8; above, 2^-22 e^-1/2 / (1 - e^-1/2)).  Else z - z^2/2 + z^3/6, which is
-// z^4/24 too large, and the other form with 2.4e-7 added to its first factor,
-// which makes it too large also where a's rounding works against it: the
-// smaller of the two is right to 2.5e-5 everywhere (worst where they meet, near
-// z = 0.06) and to z^3/24 below.
+// a = exp(-y) and m = 1 - a^2, m without cancellation for y near 0.
+// PRECISE: below y = 1/2, d = 1 - a by its Taylor series to y^9 (relative
+// error < (1/2)^9 / 10! = 6e-10), a = 1 - d (rounded once, where the approximate
+// exponential would be off by up to four times that, which adds up over a
+// thousand tokens), m = d (2 - d).  Above, d = 1 - exp(-y): 2^-22 a / (1 - a) < 4e-7.
+// Else: a by the exponential; m by its Taylor series in z = 2y to z^5, which is
+// z^6/720 too large, and as (1 - a)(1 + a) with 2.4e-7 added to the first factor,
+// which makes it too large also where a's rounding works against it: the smaller
+// of the two is right to 4e-6 everywhere (worst where they meet, near z = 0.29),
+// and to z^5/720 below, without comparing and selecting.
 template <bool PRECISE>
-__device__ __forceinline__ float2 one_minus_a2(float2 y, float2 a) {
-    const float2 z = __fadd2_rn(y, y);
-    float2 q;
+__device__ __forceinline__ void decay_of(float2 y, float2 &a, float2 &m) {
+    const float2 e = exp_neg<PRECISE>(y);
     if (PRECISE) {
-        q = __ffma2_rn(z, both(-1.f / 40320), both(1.f / 5040));
-        q = __ffma2_rn(z, q, both(-1.f / 720));
-        q = __ffma2_rn(z, q, both(1.f / 120));
-        q = __ffma2_rn(z, q, both(-1.f / 24));
-        q = __ffma2_rn(z, q, both(1.f / 6));
+        float2 q = __ffma2_rn(y, both(1.f / 362880), both(-1.f / 40320));
+        q = __ffma2_rn(y, q, both(1.f / 5040));
+        q = __ffma2_rn(y, q, both(-1.f / 720));
+        q = __ffma2_rn(y, q, both(1.f / 120));
+        q = __ffma2_rn(y, q, both(-1.f / 24));
+        q = __ffma2_rn(y, q, both(1.f / 6));
+        q = __ffma2_rn(y, q, both(-0.5f));
+        q = __ffma2_rn(y, q, both(1.f));
+        const float2 s = __fmul2_rn(y, q), l = __ffma2_rn(e, both(-1.f), both(1.f));
+        const float2 d = make_float2(y.x < 0.5f ? s.x : l.x, y.y < 0.5f ? s.y : l.y);
+        const float2 r = __ffma2_rn(d, both(-1.f), both(1.f));
+        a = make_float2(y.x < 0.5f ? r.x : e.x, y.y < 0.5f ? r.y : e.y);
+        m = __fmul2_rn(d, __ffma2_rn(d, both(-1.f), both(2.f)));
     } else {
-        q = both(1.f / 6);
+        const float2 z = __fadd2_rn(y, y);
+        float2 q = __ffma2_rn(z, both(1.f / 120), both(-1.f / 24));
+        q = __ffma2_rn(z, q, both(1.f / 6));
+        q = __ffma2_rn(z, q, both(-0.5f));
+        q = __ffma2_rn(z, q, both(1.f));
+        q = __fmul2_rn(z, q);
+        const float2 d = __ffma2_rn(e, both(-1.f), both(1.f + 2.4e-7f)), w = __ffma2_rn(e, d, d);
+        a = e;
+        m = make_float2(fminf(q.x, w.x), fminf(q.y, w.y));
     }
-    q = __ffma2_rn(z, q, both(-0.5f));
-    q = __ffma2_rn(z, q, both(1.f));
-    q = __fmul2_rn(z, q);
-    const float2 d = __ffma2_rn(a, both(-1.f), both(PRECISE ? 1.f : 1.f + 2.4e-7f)), w = __ffma2_rn(a, d, d);
-    if (!PRECISE) return make_float2(fminf(q.x, w.x), fminf(q.y, w.y));
-    return make_float2(y.x < 0.25f ? q.x : w.x, y.y < 0.25f ? q.y : w.y);
 }
 
 // 1 / sqrt(m + 1e-37): finite for m = 0, where m times it is 0 as it should be.
 constexpr float kTiny = 1e-37f;
 
-// sigmoid(r) and the decay y = csp sigmoid(r), a = exp(-y).
+// sigmoid(r) and the decay y = csp sigmoid(r), a = exp(-y), m = 1 - a^2.
 template <bool PRECISE>
-__device__ __forceinline__ void decay(float2 r, float2 csp, float2 &e, float2 &s, float2 &y, float2 &a) {
+__device__ __forceinline__ void decay(float2 r, float2 csp, float2 &e, float2 &s, float2 &a, float2 &m) {
     // without PRECISE, exp(-r) = infinity just gives s = 0
     e = exp_neg<PRECISE>(clamp_gate<PRECISE, PRECISE>(r));
     const float2 q = __fadd2_rn(e, both(1.f));
     s = make_float2(rcp_approx(q.x), rcp_approx(q.y));
-    y = __fmul2_rn(csp, s);
-    a = exp_neg<PRECISE>(y);
+    decay_of<PRECISE>(__fmul2_rn(csp, s), a, m);
 }
 
 // Forward: a and b = sqrt(1 - a^2) sigmoid(i) x.  With q = 1 + exp(-i) and
 // m = 1 - a^2, sqrt(m) / q = m / sqrt(m q^2): one root for both.
 template <bool PRECISE>
 __device__ __forceinline__ void forward_gates(float2 r, float2 i, float2 x, float2 csp, float2 &a, float2 &b) {
-    float2 e, s, y;
-    decay<PRECISE>(r, csp, e, s, y, a);
-    const float2 m = one_minus_a2<PRECISE>(y, a);
+    float2 e, s, m;
+    decay<PRECISE>(r, csp, e, s, a, m);
     const float2 q = __fadd2_rn(exp_neg<PRECISE>(clamp_gate<PRECISE>(i)), both(1.f));
     const float2 t = __ffma2_rn(__fmul2_rn(m, q), q, both(kTiny));
     b = __fmul2_rn(__fmul2_rn(m, make_float2(rsqrt_approx(t.x), rsqrt_approx(t.y))), x);
@@ -850,8 +859,8 @@ __global__ void __launch_bounds__(32 * W, CTAS)
 #pragma unroll
                 for (int z = 0; z < TP * VEC / 2; ++z) {
                     const int q = j0 * VEC / 2 + z;
-                    float2 e, y;
-                    decay<PRECISE>(pair_of<T, VEC, TP>(r, z), channel_pair<VEC>(csp, z), e, sg[q], y, a[z]);
+                    float2 e, m;
+                    decay<PRECISE>(pair_of<T, VEC, TP>(r, z), channel_pair<VEC>(csp, z), e, sg[q], a[z], m);
                     if (PRECISE) om[q] = __fmul2_rn(e, sg[q]);
                 }
 #pragma unroll
@@ -923,11 +932,11 @@ __global__ void __launch_bounds__(32 * W, CTAS)
             for (int j0 = S - TP; j0 >= 0; j0 -= TP) {
                 if (j0 >= t.cnt) continue;
                 Pack<T, VEC> x[TP], gi[TP], hp[TP], ox[TP], orr[TP], oi[TP];
-                float2 a[TP * VEC / 2], y[TP * VEC / 2], G[TP * VEC / 2];  // G = dh + C
+                float2 a[TP * VEC / 2], m[TP * VEC / 2], y[TP * VEC / 2], G[TP * VEC / 2];  // G = dh + C
 #pragma unroll
                 for (int z = 0; z < TP * VEC / 2; ++z) {
                     y[z] = __fmul2_rn(channel_pair<VEC>(csp, z), sg[j0 * VEC / 2 + z]);
-                    a[z] = exp_neg<PRECISE>(y[z]);
+                    decay_of<PRECISE>(y[z], a[z], m[z]);
                 }
                 if constexpr (VEC == 1) {
 #pragma unroll
@@ -970,7 +979,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
                     const float2 ei = exp_neg<PRECISE>(clamp_gate<PRECISE>(pair_of<T, VEC, TP>(gi, z)));
                     const float2 qi1 = __fadd2_rn(ei, both(1.f));
                     const float2 si = make_float2(rcp_approx(qi1.x), rcp_approx(qi1.y));
-                    const float2 m2 = one_minus_a2<PRECISE>(y[z], av), m1 = __fadd2_rn(m2, both(kTiny));
+                    const float2 m2 = m[z], m1 = __fadd2_rn(m2, both(kTiny));
                     const float2 w = make_float2(rsqrt_approx(m1.x), rsqrt_approx(m1.y));
                     const float2 gs2 = __fmul2_rn(G[z], si);               // G sigmoid(i)
                     const float2 gx = __fmul2_rn(gs2, __fmul2_rn(m2, w));  // * sqrt(m)
