@@ -372,13 +372,15 @@ int mamba_ssm_step(const void *x, int64_t x_row_stride, const void *delta,
  * {batch, time}, channel stride 1; lambda, the states and every sum are
  * FP32.  1 - a^2 is evaluated without cancellation for decays close to 1.
  * lengths (NULL: every row has seqlen tokens): row b ends after
- * lengths[b] tokens (values outside [0, seqlen] are clamped); later
- * positions are neither read nor written, and final_state is the state
- * after the row's last token (the initial state for an empty row).
+ * lengths[b] tokens (values outside [0, seqlen] are clamped); what x, r and i
+ * hold at later positions has no effect, those of h are left as they were,
+ * and final_state is the state after the row's last token (the initial state
+ * for an empty row).
  * resets, [batch, seqlen] bytes (NULL: none): where nonzero, h_{t-1} counts
  * as zero at that token, so several documents can share a row.
- * Outputs must not overlap inputs or each other.  The kernels run on the
- * device that is current in the calling thread. */
+ * Outputs must not overlap inputs or each other (so final_state is not
+ * initial_state).  The kernels run on the device that is current in the
+ * calling thread. */
 typedef struct MambaRecurrenceArgs {
     const void *x;
     const void *r;

@@ -612,6 +612,9 @@ int block_norm(const MambaBlockNormArgs *a, cudaStream_t st) {
     if (check_args(a, "block_norm")) return -1;
     if (a->rows == 0 || a->cols == 0) return 0;
     MB_CHECK_ARG(a->residual, "block_norm: null pointer");
+    MB_CHECK_ARG(!a->out || (a->out != a->y && a->out != a->z && a->out != a->residual && a->out != a->residual_out),
+                 "block_norm: out needs memory of its own");
+    MB_CHECK_ARG(a->residual_out != a->y && a->residual_out != a->z, "block_norm: residual_out may not be y or z");
     const NormParams p = norm_params(a);
     const bool vec = vector_rows(a);
     return a->dtype == MAMBA_F16 ? launch_fwd<__half>(p, vec, st) : launch_fwd<float>(p, vec, st);
@@ -637,6 +640,14 @@ int block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *
     MB_CHECK_ARG(aligned_to(g->dout, es) && aligned_to(g->dy, es) && aligned_to(g->dz, es) &&
                      aligned_to(g->dresidual_out, 4) && aligned_to(g->dresidual, 4),
                  "block_norm_backward: pointers must be aligned to their element type");
+    const void *in[4] = {a->y, a->z, g->dout, a->residual_out};
+    for (const void *p : in)
+        MB_CHECK_ARG(p != g->dy && p != g->dresidual && (!p || p != g->dz),
+                     "block_norm_backward: a gradient may not be one of the inputs");
+    MB_CHECK_ARG(g->dy != g->dz && static_cast<void *>(g->dresidual) != g->dy &&
+                     static_cast<void *>(g->dresidual) != g->dz && g->dresidual_out != g->dy &&
+                     (!g->dz || g->dresidual_out != g->dz),
+                 "block_norm_backward: the gradients need memory of their own");
     MB_CHECK_ARG(a->rows == 1 || (g->dy_stride >= a->cols && (!a->z || g->dz_stride >= a->cols)),
                  "block_norm_backward: rows of a gradient overlap (strides)");
     MB_CHECK_ARG(ws && ws_bytes >= block_norm_workspace_bytes(a) && aligned_to(ws, 16),

@@ -636,14 +636,16 @@ int linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *
     p.ws = w_scale;
     p.bias = bias;
     p.y = y;
-    p.ldx = ldx;
-    p.ldw = ldw;
-    p.ldy = ldy;
+    // a single row has no stride of its own
+    const int64_t k16 = ((int64_t)k + 15) / 16 * 16, n16 = ((int64_t)n + 15) / 16 * 16;
+    p.ldx = ldx = rows == 1 ? k16 : ldx;
+    p.ldw = ldw = n == 1 ? k16 : ldw;
+    p.ldy = rows == 1 ? n16 : ldy;
     p.rows = rows;
     p.n = n;
     p.k = k;
     p.mode = mode;
-    if (k > 0 && aligned_to(x, 16) && aligned_to(w, 16) && ldx % 16 == 0 && ldw % 16 == 0 && ldx >= k && ldw >= k &&
+    if (k > 0 && aligned_to(x, 16) && aligned_to(w, 16) && ldx % 16 == 0 && ldw % 16 == 0 &&
         rows <= 0x7fffffff - 256) {
         const int pairs = device_pairs();
         if (pairs < 0) return -1;

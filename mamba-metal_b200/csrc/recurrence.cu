@@ -138,8 +138,10 @@ __device__ __forceinline__ void forward_gates(float2 r, float2 i, float2 x, floa
     b = __fmul2_rn(__fmul2_rn(m, make_float2(rsqrt_approx(t.x), rsqrt_approx(t.y))), x);
 }
 
-// softplus(lambda), once per channel and call.
+// softplus(lambda), and c times it (finite: 0 times it has to be 0), once per
+// channel and call.
 __device__ __forceinline__ float channel_softplus(float l) { return fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))); }
+__device__ __forceinline__ float channel_decay(float c, float l) { return min_nan(c * channel_softplus(l), 1e30f); }
 
 struct FwdParams {
     const void *x, *r, *i;
@@ -213,15 +215,19 @@ __device__ __forceinline__ uint32_t get_state(const float *slot) {
     return w;
 }
 
-// Bounded wait (2 s, or at once after another CTA's wait ran out).
+// Bounded wait: 2 s, or at once after a wait of this call ran out (`gave_up`, a
+// word of the call's workspace, is then no longer empty).
 struct Waiting {
+    uint32_t *gave_up;
     uint64_t t0 = 0;
     int spins = 0;
+    __device__ __forceinline__ explicit Waiting(uint32_t *g) : gave_up(g) {}
     __device__ __forceinline__ bool again() {
         if ((++spins & 63) == 0) {
             const uint64_t now = global_timer_ns();
             if (t0 == 0) t0 = now;
-            if (now - t0 > 2000000000ull || *(volatile unsigned int *)&g_recurrence_error) {
+            if (now - t0 > 2000000000ull || *(volatile uint32_t *)gave_up != kEmpty) {
+                *(volatile uint32_t *)gave_up = 0;
                 atomicOr(&g_recurrence_error, kErrRecurrenceTimeout);
                 return false;
             }
@@ -281,8 +287,9 @@ struct MapRows {
 };
 
 template <int VEC>
-__device__ __forceinline__ void wait_maps(const float2 *slot, Pack<float, VEC> &P, Pack<float, VEC> &H) {
-    Waiting wt;
+__device__ __forceinline__ void wait_maps(const float2 *slot, uint32_t *gave_up, Pack<float, VEC> &P,
+                                          Pack<float, VEC> &H) {
+    Waiting wt(gave_up);
     bool ready;
     do {
         uint64_t w[VEC];
@@ -298,8 +305,8 @@ __device__ __forceinline__ void wait_maps(const float2 *slot, Pack<float, VEC> &
     } while (!ready && wt.again());
 }
 template <int VEC>
-__device__ __forceinline__ void wait_states(const float *slot, float (&h)[VEC]) {
-    Waiting wt;
+__device__ __forceinline__ void wait_states(const float *slot, uint32_t *gave_up, float (&h)[VEC]) {
+    Waiting wt(gave_up);
     bool ready;
     do {
         uint32_t w[VEC];
@@ -329,7 +336,7 @@ struct Divisor {
 };
 
 struct Chains {
-    unsigned int *ticket;
+    unsigned int *ticket;  // and behind it the word of Waiting
     float2 *maps;      // [chains, tiles, channels of a tile]
     float *states;     // [chains, groups, channels of a tile]
     const float *csp;  // [dim] c * softplus(lambda)
@@ -387,7 +394,8 @@ __device__ __forceinline__ Maps<VEC> prefix_maps(const Chains &c, const Tile &t,
     const int j = t.j;
     for (int tile = warp; tile < j; tile += W) {
         Pack<float, VEC> P, H;
-        wait_maps<VEC>(c.maps + ((int64_t)t.chain * c.tiles + t.k - j + tile) * (32 * VEC) + lane * VEC, P, H);
+        wait_maps<VEC>(c.maps + ((int64_t)t.chain * c.tiles + t.k - j + tile) * (32 * VEC) + lane * VEC,
+                       c.ticket + 1, P, H);
         gm.P[tile][lane] = P;
         gm.H[tile][lane] = H;
     }
@@ -405,7 +413,8 @@ __device__ __forceinline__ Maps<VEC> prefix_maps(const Chains &c, const Tile &t,
 template <int VEC>
 __device__ __forceinline__ void group_state(const Chains &c, const Tile &t, float (&s)[VEC]) {
     if (t.g > 0)
-        wait_states<VEC>(c.states + ((int64_t)t.chain * c.groups + t.g - 1) * (32 * VEC) + (threadIdx.x & 31) * VEC, s);
+        wait_states<VEC>(c.states + ((int64_t)t.chain * c.groups + t.g - 1) * (32 * VEC) + (threadIdx.x & 31) * VEC,
+                         c.ticket + 1, s);
 }
 template <int VEC>
 __device__ __forceinline__ void leave_group(const Chains &c, const Tile &t, const float (&h)[VEC]) {
@@ -596,7 +605,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
     if (WALK) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            csp[e] = t.in ? p.c * channel_softplus(p.lambda[t.d + e]) : 0.f;
+            csp[e] = t.in ? channel_decay(p.c, p.lambda[t.d + e]) : 0.f;
             s[e] = t.in && p.h0 ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
         }
     }
@@ -808,7 +817,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
     if (WALK) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            csp[e] = t.in ? f.c * channel_softplus(f.lambda[t.d + e]) : 0.f;
+            csp[e] = t.in ? channel_decay(f.c, f.lambda[t.d + e]) : 0.f;
             s[e] = t.in && p.dhN ? p.dhN[(int64_t)t.b * f.D + t.d + e] : 0.f;
         }
     }
@@ -1077,7 +1086,7 @@ __global__ void __launch_bounds__(kThreads) recurrence_step_kernel(const StepPar
     if (d >= p.D) return;
     float csp[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) csp[e] = p.c * channel_softplus(p.lambda[d + e]);
+    for (int e = 0; e < VEC; ++e) csp[e] = channel_decay(p.c, p.lambda[d + e]);
     const int64_t b0 = (int64_t)blockIdx.y * p.rows, b1 = min(b0 + p.rows, (int64_t)p.B);
 #pragma unroll 4
     for (int64_t b = b0; b < b1; ++b) {
@@ -1124,7 +1133,6 @@ int check_args(const MambaRecurrenceArgs *a, bool backward) {
     MB_CHECK_ARG(a->batch >= 0 && a->seqlen >= 0 && a->dim >= 0, "gated_recurrence: negative size");
     MB_CHECK_ARG(a->dtype == MAMBA_F32 || a->dtype == MAMBA_F16, "gated_recurrence: bad dtype");
     MB_CHECK_ARG(a->c > 0.f && a->c <= 3.0e38f, "gated_recurrence: c must be positive and finite");
-    MB_CHECK_ARG(a->batch <= 65535, "gated_recurrence: batch above 65535");
     if (a->batch == 0 || a->dim == 0) return 0;
     MB_CHECK_ARG(a->lambda && (a->seqlen == 0 || (a->x && a->r && a->i && a->h)), "gated_recurrence: null pointer");
     const size_t es = dtype_size(a->dtype);
@@ -1132,6 +1140,10 @@ int check_args(const MambaRecurrenceArgs *a, bool backward) {
                      aligned_to(a->lambda, 4) && aligned_to(a->initial_state, 4) && aligned_to(a->final_state, 4) &&
                      aligned_to(a->lengths, 4),
                  "gated_recurrence: pointers must be aligned to their element type");
+    MB_CHECK_ARG(backward || a->seqlen == 0 || (a->h != a->x && a->h != a->r && a->h != a->i),
+                 "gated_recurrence: h may not be one of the inputs");
+    MB_CHECK_ARG(backward || !a->final_state || a->final_state != a->initial_state,
+                 "gated_recurrence: final_state may not be initial_state");
     MB_CHECK_ARG(backward || output_rows_disjoint(a->h_stride, a->batch, a->seqlen, a->dim),
                  "gated_recurrence: rows of h overlap (strides)");
     return 0;
@@ -1197,7 +1209,7 @@ bool plan_chains(const MambaRecurrenceArgs *a, bool backward, Plan &pl) {
     Chains &c = pl.ch;
     c = Chains{};
     const int64_t blocks = ceil_div64(a->dim, cw), tiles = std::max<int64_t>(1, ceil_div64(a->seqlen, Sh::tile));
-    if (blocks * a->batch * tiles > 0x7fffffffLL) return false;
+    if (blocks * a->batch > 0x7fffffffLL || blocks * a->batch * tiles > 0x7fffffffLL) return false;
     auto divisor = [](int64_t d) {
         return Divisor{(unsigned)d, d == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / (unsigned long long)d)};
     };
@@ -1258,7 +1270,7 @@ __global__ void __launch_bounds__(256)
     recurrence_init_kernel(const float *__restrict__ lambda, float c, int D, float *__restrict__ csp,
                            uint4 *__restrict__ ones, int64_t n) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, stride = (int64_t)gridDim.x * 256;
-    for (int64_t d = i; d < D; d += stride) csp[d] = c * channel_softplus(lambda[d]);
+    for (int64_t d = i; d < D; d += stride) csp[d] = channel_decay(c, lambda[d]);
     for (int64_t k = i; k < n; k += stride) ones[k] = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
 }
 
@@ -1437,6 +1449,16 @@ int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads
     MB_CHECK_ARG(aligned_to(g->dh, es) && aligned_to(g->dx, es) && aligned_to(g->dr, es) && aligned_to(g->di, es) &&
                      aligned_to(g->dfinal_state, 4) && aligned_to(g->dinitial_state, 4),
                  "gated_recurrence_backward: pointers must be aligned to their element type");
+    if (a->seqlen > 0) {
+        const void *in[5] = {a->x, a->r, a->i, a->h, g->dh};
+        for (const void *p : in)
+            MB_CHECK_ARG(p != g->dx && p != g->dr && p != g->di,
+                         "gated_recurrence_backward: a gradient may not be one of the inputs");
+        MB_CHECK_ARG(g->dx != g->dr && g->dx != g->di && g->dr != g->di,
+                     "gated_recurrence_backward: the gradients need memory of their own");
+    }
+    MB_CHECK_ARG(!g->dinitial_state || (g->dinitial_state != g->dfinal_state && g->dinitial_state != a->initial_state),
+                 "gated_recurrence_backward: dinitial_state may not be dfinal_state or initial_state");
     MB_CHECK_ARG(output_rows_disjoint(g->dx_stride, a->batch, a->seqlen, a->dim) &&
                      output_rows_disjoint(g->dr_stride, a->batch, a->seqlen, a->dim) &&
                      output_rows_disjoint(g->di_stride, a->batch, a->seqlen, a->dim),
@@ -1478,7 +1500,6 @@ int recurrence_step(const void *x, int64_t xrs, const void *r, int64_t rrs, cons
     MB_CHECK_ARG(batch >= 0 && dim >= 0, "gated_recurrence_step: negative size");
     MB_CHECK_ARG(dtype == MAMBA_F32 || dtype == MAMBA_F16, "gated_recurrence_step: bad dtype");
     MB_CHECK_ARG(c > 0.f && c <= 3.0e38f, "gated_recurrence_step: c must be positive and finite");
-    MB_CHECK_ARG(batch <= 65535, "gated_recurrence_step: batch above 65535");
     if (batch == 0 || dim == 0) return 0;
     MB_CHECK_ARG(x && r && i && lambda && state_in && state_out && h, "gated_recurrence_step: null pointer");
     const size_t es = dtype_size(dtype);
@@ -1486,6 +1507,7 @@ int recurrence_step(const void *x, int64_t xrs, const void *r, int64_t rrs, cons
                      aligned_to(lambda, 4) && aligned_to(state_in, 4) && aligned_to(state_out, 4),
                  "gated_recurrence_step: pointers must be aligned to their element type");
     MB_CHECK_ARG(batch == 1 || hrs >= dim, "gated_recurrence_step: rows of h overlap (stride)");
+    MB_CHECK_ARG(h != x && h != r && h != i, "gated_recurrence_step: h may not be one of the inputs");
     auto run = [&](auto zero) {
         using T = decltype(zero);
         StepParams<T> p{static_cast<const T *>(x), static_cast<const T *>(r), static_cast<const T *>(i),
@@ -1496,6 +1518,7 @@ int recurrence_step(const void *x, int64_t xrs, const void *r, int64_t rrs, cons
         const int blocks = ceil_div(dim, kThreads * (vec ? 4 : 1));
         // several rows per thread once one row each would fill the GPU four times over
         p.rows = (int64_t)blocks * batch >= 16LL * device_sm_count() ? 4 : 1;
+        p.rows = std::max(p.rows, ceil_div(batch, 65535));  // the grid's limit
         const dim3 grid((unsigned)blocks, (unsigned)ceil_div(batch, p.rows));
         if (vec)
             recurrence_step_kernel<T, 4><<<grid, kThreads, 0, st>>>(p);

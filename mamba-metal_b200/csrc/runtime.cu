@@ -1105,6 +1105,21 @@ static int init_random(Model &m, uint64_t seed) {
 // ============================================================================
 using mb::set_error;
 
+// Runs one entry point: 0 / -1, with no C++ exception (an allocation of host
+// memory that failed) crossing the C boundary.
+template <typename F>
+static int guarded(F &&f) {
+    try {
+        return f() ? -1 : 0;
+    } catch (...) {
+        try {
+            mb::set_error("out of host memory");
+        } catch (...) {
+        }
+        return -1;
+    }
+}
+
 extern "C" {
 
 MambaModel *mamba_create(const MambaConfig *cfg) {
@@ -1475,13 +1490,14 @@ size_t mamba_gated_recurrence_workspace(const MambaRecurrenceArgs *a, int backwa
 
 int mamba_gated_recurrence(const MambaRecurrenceArgs *a, void *workspace, size_t workspace_bytes, void *stream) {
     mb::clear_error();
-    return mb::recurrence_forward(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)) ? -1 : 0;
+    return guarded([&] { return mb::recurrence_forward(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)); });
 }
 
 int mamba_gated_recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads *g, void *workspace,
                                     size_t workspace_bytes, void *stream) {
     mb::clear_error();
-    return mb::recurrence_backward(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)) ? -1 : 0;
+    return guarded(
+        [&] { return mb::recurrence_backward(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)); });
 }
 
 int mamba_gated_recurrence_step(const void *x, int64_t x_row_stride, const void *r, int64_t r_row_stride,
@@ -1489,15 +1505,15 @@ int mamba_gated_recurrence_step(const void *x, int64_t x_row_stride, const void 
                                 float *state_out, void *h, int64_t h_row_stride, int batch, int dim, float c,
                                 int dtype, void *stream) {
     mb::clear_error();
-    return mb::recurrence_step(x, x_row_stride, r, r_row_stride, i, i_row_stride, lambda, state_in, state_out, h,
-                               h_row_stride, batch, dim, c, dtype, static_cast<cudaStream_t>(stream))
-               ? -1
-               : 0;
+    return guarded([&] {
+        return mb::recurrence_step(x, x_row_stride, r, r_row_stride, i, i_row_stride, lambda, state_in, state_out, h,
+                                   h_row_stride, batch, dim, c, dtype, static_cast<cudaStream_t>(stream));
+    });
 }
 
 int mamba_block_norm(const MambaBlockNormArgs *a, void *stream) {
     mb::clear_error();
-    return mb::block_norm(a, static_cast<cudaStream_t>(stream)) ? -1 : 0;
+    return guarded([&] { return mb::block_norm(a, static_cast<cudaStream_t>(stream)); });
 }
 
 size_t mamba_block_norm_workspace(const MambaBlockNormArgs *a) { return mb::block_norm_workspace_bytes(a); }
@@ -1505,7 +1521,8 @@ size_t mamba_block_norm_workspace(const MambaBlockNormArgs *a) { return mb::bloc
 int mamba_block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *g, void *workspace,
                               size_t workspace_bytes, void *stream) {
     mb::clear_error();
-    return mb::block_norm_backward(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)) ? -1 : 0;
+    return guarded(
+        [&] { return mb::block_norm_backward(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)); });
 }
 
 int mamba_propagate_tile_carries(float *carries, int num_tiles, int64_t width, float *total, void *stream) {
@@ -1527,17 +1544,18 @@ int mamba_linear(const void *x, int64_t ldx, const void *w, const float *bias, v
 int mamba_quantize_rows(const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int64_t rows, int cols,
                         int dtype, void *stream) {
     mb::clear_error();
-    return mb::quantize_rows(x, ldx, q, ldq, scale, rows, cols, dtype, static_cast<cudaStream_t>(stream)) ? -1 : 0;
+    return guarded(
+        [&] { return mb::quantize_rows(x, ldx, q, ldq, scale, rows, cols, dtype, static_cast<cudaStream_t>(stream)); });
 }
 
 int mamba_linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw,
                     const float *w_scale, const float *bias, void *y, int64_t ldy, int64_t rows, int n, int k,
                     int mode, void *stream) {
     mb::clear_error();
-    return mb::linear_i8(x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, rows, n, k, mode,
-                         static_cast<cudaStream_t>(stream))
-               ? -1
-               : 0;
+    return guarded([&] {
+        return mb::linear_i8(x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, rows, n, k, mode,
+                             static_cast<cudaStream_t>(stream));
+    });
 }
 
 int mamba_in_proj_conv(const void *x, const void *w_in, const float *conv_w, const float *conv_b, void *u, void *z,

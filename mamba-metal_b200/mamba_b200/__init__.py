@@ -660,17 +660,18 @@ def _on_stream(fn):
     current one).  The whole helper runs with that stream current, so that
     what it allocates and fills belongs to the stream its kernels run on."""
     @functools.wraps(fn)
-    def helper(t, *args, stream=None, **kw):
+    def helper(*args, stream=None, **kw):
         if stream is None:
-            return fn(t, *args, **kw)
+            return fn(*args, **kw)
         torch = _torch()
+        t = next(v for v in list(args) + list(kw.values()) if isinstance(v, torch.Tensor))
         if not t.is_cuda:
             raise MambaError("%s: tensors must be on a CUDA device" % fn.__name__)
         if not isinstance(stream, torch.cuda.Stream):
             stream = torch.cuda.ExternalStream(stream, device=t.device) if stream \
                 else torch.cuda.default_stream(t.device)
         with torch.cuda.stream(stream):
-            return fn(t, *args, **kw)
+            return fn(*args, **kw)
     return helper
 
 

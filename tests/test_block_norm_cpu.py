@@ -39,7 +39,8 @@ def test_oracle_gradients_match_differences(gate):
 
 def _args(**kw):
     a = mb.MambaBlockNormArgs()
-    a.y = a.residual = a.residual_out = a.out = a.rstd_post = a.rstd_pre = 4096  # never dereferenced
+    a.residual = a.residual_out = a.rstd_post = a.rstd_pre = 4096  # never dereferenced
+    a.y, a.out = 8192, 12288
     a.rows, a.cols, a.dtype, a.residual_scale, a.eps = 4, 8, mb.F32, 1.0, 1e-5
     a.y_stride = a.z_stride = 8
     for k, v in kw.items():
@@ -53,7 +54,8 @@ def _args(**kw):
     (dict(residual_scale=float("nan")), "residual_scale"), (dict(residual_scale=float("inf")), "residual_scale"),
     (dict(y=None), "null"), (dict(residual=None), "null"), (dict(residual_out=None), "null"),
     (dict(y=4098), "aligned"), (dict(z=4098), "aligned"), (dict(residual=4098), "aligned"), (dict(out=4098), "aligned"),
-    (dict(w_post=4098), "aligned"), (dict(w_pre=4098), "aligned"), (dict(rstd_post=4098), "aligned")])
+    (dict(w_post=4098), "aligned"), (dict(w_pre=4098), "aligned"), (dict(rstd_post=4098), "aligned"),
+    (dict(out=8192), "own"), (dict(out=4096), "own"), (dict(residual_out=8192), "residual_out")])
 def test_forward_refusals(change, text):
     assert mb.lib().mamba_block_norm(ctypes.byref(_args(**change)), None) == -1
     assert text in mb.last_error()
@@ -71,12 +73,15 @@ def test_empty_and_null():
     ({}, dict(dresidual=None), "null"), ({}, dict(dy=None), "null"), ({}, dict(dout=None, dresidual_out=None), "null"),
     (dict(rstd_post=None), {}, "null"), (dict(rstd_pre=None), {}, "rstd_pre"), (dict(z=4096), dict(dz=None), "dz"),
     ({}, dict(dy=4098), "aligned"), ({}, dict(dout=4098), "aligned"), ({}, dict(dw_pre=4098), "aligned"),
-    ({}, dict(dy_stride=7), "overlap"), (dict(z=4096), dict(dz=4096, dz_stride=7), "overlap"),
+    ({}, dict(dy_stride=7), "overlap"), (dict(z=28672), dict(dz=32768, dz_stride=7), "overlap"),
+    ({}, dict(dy=8192), "inputs"), ({}, dict(dresidual=4096), "inputs"), ({}, dict(dresidual=24576), "own"),
+    (dict(z=28672), dict(dz=24576), "own"), (dict(z=28672), dict(dz=28672), "inputs"),
     ({}, dict(ws=None), "workspace"), ({}, dict(short=1), "workspace"), ({}, dict(ws=4104), "workspace")])
 def test_backward_refusals(args, change, text):
     a = _args(**args)
     g = mb.MambaBlockNormGrads()
-    g.dresidual_out = g.dout = g.dresidual = g.dy = g.dw_post = g.dw_pre = 4096
+    g.dresidual_out = g.dresidual = g.dw_post = g.dw_pre = 16384
+    g.dout, g.dy = 20480, 24576
     g.dy_stride = g.dz_stride = 8
     ws, short = change.pop("ws", 4096), change.pop("short", 0)
     for k, v in change.items():

@@ -47,7 +47,8 @@ def test_oracle_gradients_match_differences(ragged):
 
 def _args(B=2, L=4, D=8, dtype=mb.F32, ptr=4096):
     a = mb.MambaRecurrenceArgs()
-    a.x = a.r = a.i = a.lambda_ = a.h = ptr  # never dereferenced: every call below is refused
+    a.x = a.r = a.i = a.lambda_ = ptr  # never dereferenced: every call below is refused
+    a.h = 2 * ptr
     a.batch, a.seqlen, a.dim, a.dtype, a.c = B, L, D, dtype, 8.0
     for s in (a.x_stride, a.r_stride, a.i_stride, a.h_stride):
         s[0], s[1] = L * D, D
@@ -64,7 +65,8 @@ def _forward(a, ws=None, n=0):
     (dict(c=float("nan")), "c must be"), (dict(c=float("inf")), "c must be"), (dict(x=None), "null"),
     (dict(r=None), "null"), (dict(i=None), "null"), (dict(h=None), "null"), (dict(lambda_=None), "null"),
     (dict(x=4098), "aligned"), (dict(lambda_=4098), "aligned"), (dict(initial_state=4098), "aligned"),
-    (dict(final_state=4098), "aligned"), (dict(lengths=4098), "aligned"), (dict(batch=70000), "65535")])
+    (dict(final_state=4098), "aligned"), (dict(lengths=4098), "aligned"), (dict(h=4096), "one of the inputs"),
+    (dict(initial_state=12288, final_state=12288), "may not be initial_state")])
 def test_forward_refusals(change, text):
     a = _args()
     for k, v in change.items():
@@ -80,6 +82,8 @@ def test_forward_workspace_refusals():
     assert need > 0
     for ws, n in ((None, need), (4096, need - 1), (4104, need)):
         assert _forward(a, ws, n) == -1 and "workspace" in mb.last_error()
+    a = _args(B=2 ** 31 - 1, L=2 ** 31 - 1, D=2 ** 31 - 1)  # the count of tiles exceeds 64 bits
+    assert _forward(a, 4096, 2 ** 62) == -1
     a = _args(B=60000, L=2 ** 31 - 1, D=2 ** 20)
     for s in (a.x_stride, a.r_stride, a.i_stride, a.h_stride):
         s[0], s[1] = 2 ** 52, 2 ** 20
@@ -112,7 +116,7 @@ def test_backward_refusals():
 
     def grads():
         g = mb.MambaRecurrenceGrads()
-        g.dh = g.dx = g.dr = g.di = g.dlambda = 4096
+        g.dh, g.dx, g.dr, g.di, g.dlambda = 4096, 16384, 20480, 24576, 28672
         for s in (g.dh_stride, g.dx_stride, g.dr_stride, g.di_stride):
             s[0], s[1] = 32, 8
         return g
@@ -124,6 +128,13 @@ def test_backward_refusals():
         g = grads()
         setattr(g, name, 4098)
         assert call(_args(), g) == -1, name
+    for name, other in (("dx", 4096), ("dr", 8192), ("di", 16384)):  # an input, h, another gradient
+        g = grads()
+        setattr(g, name, other)
+        assert call(_args(), g) == -1 and ("inputs" in mb.last_error() or "own" in mb.last_error())
+    g = grads()
+    g.dfinal_state = g.dinitial_state = 32768
+    assert call(_args(), g) == -1 and "dinitial_state" in mb.last_error()
     g = grads()
     g.dr_stride[1] = 4
     assert call(_args(), g) == -1 and "overlap" in mb.last_error()
@@ -136,10 +147,10 @@ def test_backward_refusals():
 
 @pytest.mark.parametrize("change,text", [
     (dict(dtype=2), "dtype"), (dict(batch=-1), "negative"), (dict(dim=-1), "negative"), (dict(c=0.0), "c must be"),
-    (dict(batch=70000), "65535"), (dict(x=None), "null"), (dict(state_out=None), "null"), (dict(h=None), "null"),
+    (dict(h=4096), "one of the inputs"), (dict(x=None), "null"), (dict(state_out=None), "null"), (dict(h=None), "null"),
     (dict(state_in=4098), "aligned"), (dict(hrs=7), "overlap")])
 def test_step_refusals(change, text):
-    v = dict(x=4096, xrs=8, r=4096, rrs=8, i=4096, irs=8, lam=4096, state_in=4096, state_out=4096, h=4096, hrs=8,
+    v = dict(x=4096, xrs=8, r=4096, rrs=8, i=4096, irs=8, lam=4096, state_in=4096, state_out=4096, h=8192, hrs=8,
              batch=2, dim=8, c=8.0, dtype=mb.F32, stream=None)
     v.update(change)
     assert mb.lib().mamba_gated_recurrence_step(*v.values()) == -1

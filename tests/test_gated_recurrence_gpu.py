@@ -366,3 +366,77 @@ def test_stream_argument(cuda, dtype):
     for h, hN, grads in outs:
         _check_forward(v, h, hN, dtype)
         _check_backward(v, h.cpu().numpy(), grads, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("order", ["batch", "time"])
+@pytest.mark.parametrize("B,L,D", [(3, 150, 72), (1, 300, 64), (24, 130, 1024), (5, 1, 64)])
+def test_aligned_views(cuda, B, L, D, order, dtype):
+    """Column blocks of a projection whose rows keep 16-byte alignment, with
+    batch or time outermost: the kernels that fetch tiles by tensor maps."""
+    v = _case(B + L + D, B, L, D, dtype, ragged=B > 1, resets=True)
+    t = _dev(v)
+    pitch = 3 * D + 16
+
+    def buf():
+        shape = (L, B, pitch) if order == "time" else (B, L, pitch)
+        w = torch.full(shape, float("nan"), dtype=dtype, device="cuda")
+        return w, (w.transpose(0, 1) if order == "time" else w)
+
+    wide, view = buf()
+    for k, name in enumerate(("x", "r", "i")):
+        part = view[:, :, 8 + k * D:8 + (k + 1) * D]
+        part.copy_(t[name])
+        t[name] = part
+    out, oview = buf()
+    for b, n in enumerate(v["lengths"] if v["lengths"] is not None else []):
+        oview[b, n:] = 0
+    h, hN = _forward(t, h=oview[:, :, 16:16 + D])
+    dwide, dview = buf()
+    dview[:, :, 8:8 + 3 * D] = 0
+    grads = _backward(t, h, **{n: dview[:, :, 8 + k * D:8 + (k + 1) * D] for k, n in enumerate(("dx", "dr", "di"))})
+    torch.cuda.synchronize()
+    assert mb.device_status() == 0
+    _check_forward(v, h, hN, dtype)
+    _check_backward(v, h.cpu().numpy(), grads, dtype)
+    assert dwide[..., :8].isnan().all() and dwide[..., 8 + 3 * D:].isnan().all()
+
+
+def test_many_rows(cuda):
+    """More batch rows than a grid dimension holds."""
+    B, L, D = 70000, 2, 8
+    v = _case(1, B, L, D, torch.float16, ragged=True)
+    t = _dev(v)
+    h, hN = _forward(t)
+    _check_forward(v, h, hN, torch.float16)
+    _check_backward(v, h.cpu().numpy(), _backward(t, h), torch.float16)
+    hs, s = mb.gated_recurrence_step(t["x"][:, 0], t["r"][:, 0], t["i"][:, 0], t["lam"], t["h0"], c=C)
+    v1 = dict(v, x=v["x"][:, :1], r=v["r"][:, :1], i=v["i"][:, :1], lengths=None)
+    _check_forward(v1, hs[:, None], s, torch.float16)
+
+
+def test_keywords_and_refusals(cuda):
+    t = _dev(_case(2, 2, 20, 16, torch.float32))
+    a = mb.gated_recurrence(x=t["x"], r=t["r"], i=t["i"], lam=t["lam"], stream=torch.cuda.current_stream())
+    assert torch.equal(a, mb.gated_recurrence(t["x"], t["r"], t["i"], t["lam"]))
+    with pytest.raises(mb.MambaError, match="inputs"):
+        mb.gated_recurrence(t["x"], t["r"], t["i"], t["lam"], h=t["x"])
+    with pytest.raises(mb.MambaError, match="workspace"):
+        mb.gated_recurrence(t["x"], t["r"], t["i"], t["lam"], workspace=torch.empty(8, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(mb.MambaError):
+        mb.gated_recurrence(t["x"], t["r"], t["i"], t["lam"], lengths=torch.ones(2, dtype=torch.int32))  # on the CPU
+
+
+def test_a_nan_stays_in_its_row_and_channel(cuda):
+    """Without a reset a NaN gate or input reaches every later state of its own
+    channel and no other; its gradient every earlier one."""
+    for dtype in (torch.float16, torch.float32):
+        for name in ("x", "r", "i"):
+            for B, L, D in ((2, 200, 64), (2, 200, 33), (40, 70, 640)):
+                t = _dev(_case(3, B, L, D, dtype))
+                ref = _forward(t)[0]
+                t[name][1, 50, 7] = float("nan")
+                h, hN = _forward(t)
+                assert h[1, 50:, 7].isnan().all() and hN[1, 7].isnan()
+                h[1, 50:, 7] = ref[1, 50:, 7]
+                assert torch.equal(h, ref)
