@@ -246,7 +246,18 @@ __device__ __forceinline__ Pack<T, VEC> load_pack(const T *p) {
     return *reinterpret_cast<const Pack<T, VEC> *>(p);
 }
 
-// Affine maps h -> P h + H of a thread's channels.
+// Affine maps h -> P h + H of a thread's channels.  A reset drops what enters
+// even where that is infinite or NaN, so it is not P = 0 but a set sign bit of P
+// (products of decays, which have none, keep it); CUTS: whether the call has
+// resets at all.  with_flag turns a run-time flag into such a template argument.
+template <typename F>
+__device__ __forceinline__ void with_flag(bool flag, F &&f) {
+    if (flag)
+        f(std::true_type());
+    else
+        f(std::false_type());
+}
+__device__ __forceinline__ bool is_cut(float P) { return __float_as_int(P) < 0; }
 template <int VEC>
 struct Maps {
     Pack<float, VEC> P, H;
@@ -257,7 +268,16 @@ struct Maps {
             H.v[e] = 0.f;
         }
     }
+    // a reset: nothing of the state passes
+    __device__ __forceinline__ void cut() {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            P.v[e] = -1.f;
+            H.v[e] = 0.f;
+        }
+    }
     // then q, later in time
+    template <bool CUTS = false>
     __device__ __forceinline__ void then(const Pack<float, VEC> &qP, const Pack<float, VEC> &qH) {
         if constexpr (VEC == 1) {
             H.v[0] = fmaf(qP.v[0], H.v[0], qH.v[0]);
@@ -274,10 +294,20 @@ struct Maps {
                 P.v[e + 1] = n.y;
             }
         }
-    }
-    __device__ __forceinline__ void apply(const float (&s)[VEC], float (&h)[VEC]) const {
+        if (CUTS)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) h[e] = fmaf(P.v[e], s[e], H.v[e]);
+            for (int e = 0; e < VEC; ++e)
+                if (is_cut(qP.v[e])) {
+                    P.v[e] = qP.v[e];
+                    H.v[e] = qH.v[e];
+                }
+    }
+    __device__ __forceinline__ void apply(const float (&s)[VEC], float (&h)[VEC], bool cuts) const {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            h[e] = fmaf(P.v[e], s[e], H.v[e]);
+            if (cuts && is_cut(P.v[e])) h[e] = H.v[e];
+        }
     }
 };
 // A CTA's maps in shared memory, by warp or by tile of the group.
@@ -389,7 +419,7 @@ __device__ __forceinline__ Tile place_tile(const Chains &c, const FwdParams &p, 
 // between them; `wm` holds the maps of this tile's warps.  Syncs the CTA.
 template <int VEC, int W>
 __device__ __forceinline__ Maps<VEC> prefix_maps(const Chains &c, const Tile &t, const MapRows<VEC, W> &wm,
-                                                 MapRows<VEC, (1 << kMaxGroupShift) - 1> &gm) {
+                                                 MapRows<VEC, (1 << kMaxGroupShift) - 1> &gm, bool cuts) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int j = t.j;
     for (int tile = warp; tile < j; tile += W) {
@@ -402,8 +432,11 @@ __device__ __forceinline__ Maps<VEC> prefix_maps(const Chains &c, const Tile &t,
     __syncthreads();
     Maps<VEC> m;
     m.identity();
-    for (int q = 0; q < j; ++q) m.then(gm.P[q][lane], gm.H[q][lane]);
-    for (int w = 0; w < warp; ++w) m.then(wm.P[w][lane], wm.H[w][lane]);
+    with_flag(cuts, [&](auto flag) {
+        constexpr bool CUTS = decltype(flag)::value;
+        for (int q = 0; q < j; ++q) m.template then<CUTS>(gm.P[q][lane], gm.H[q][lane]);
+        for (int w = 0; w < warp; ++w) m.template then<CUTS>(wm.P[w][lane], wm.H[w][lane]);
+    });
     return m;
 }
 
@@ -425,12 +458,14 @@ __device__ __forceinline__ void leave_group(const Chains &c, const Tile &t, cons
 
 // The tile's own map (warp maps in order), published for the group's later tiles.
 template <int VEC, int W>
-__device__ __forceinline__ void publish_map(const Chains &c, const Tile &t, const MapRows<VEC, W> &wm) {
+__device__ __forceinline__ void publish_map(const Chains &c, const Tile &t, const MapRows<VEC, W> &wm, bool cuts) {
     const int lane = threadIdx.x & 31;
     Maps<VEC> m;
     m.identity();
+    with_flag(cuts, [&](auto flag) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) m.then(wm.P[w][lane], wm.H[w][lane]);
+        for (int w = 0; w < W; ++w) m.template then<decltype(flag)::value>(wm.P[w][lane], wm.H[w][lane]);
+    });
     float2 *slot = c.maps + ((int64_t)t.chain * c.tiles + t.k) * (32 * VEC) + lane * VEC;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) put_map(slot + e, m.P.v[e], m.H.v[e]);
@@ -439,17 +474,20 @@ __device__ __forceinline__ void publish_map(const Chains &c, const Tile &t, cons
 // WALK: the state entering this warp's tokens (h) and the state leaving the
 // tile (s) from the state entering it (s), through the maps of the tile's warps.
 template <int VEC, int W>
-__device__ __forceinline__ void walk_state(const MapRows<VEC, W> &wm, float (&s)[VEC], float (&h)[VEC]) {
+__device__ __forceinline__ void walk_state(const MapRows<VEC, W> &wm, float (&s)[VEC], float (&h)[VEC], bool cuts) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    with_flag(cuts, [&](auto flag) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        const Pack<float, VEC> P = wm.P[w][lane], H = wm.H[w][lane];
+        for (int w = 0; w < W; ++w) {
+            const Pack<float, VEC> P = wm.P[w][lane], H = wm.H[w][lane];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            if (w == warp) h[e] = s[e];
-            s[e] = fmaf(P.v[e], s[e], H.v[e]);
+            for (int e = 0; e < VEC; ++e) {
+                if (w == warp) h[e] = s[e];
+                s[e] = fmaf(P.v[e], s[e], H.v[e]);
+                if (decltype(flag)::value && is_cut(P.v[e])) s[e] = H.v[e];
+            }
         }
-    }
+    });
 }
 
 // Which of this warp's tokens cut the state.
@@ -553,6 +591,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
     auto &sm = *reinterpret_cast<FwdSmem<T, VEC, S, W, WALK> *>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned total = ch.chains.d * (unsigned)ch.tiles;
+    const bool cuts = p.resets != nullptr;
 
     if (TMA) {
         if (tid == 0) {
@@ -655,22 +694,21 @@ __global__ void __launch_bounds__(32 * W, CTAS)
                     }
             }
             const uint32_t cut = cut_mask(p, t.b, t.t0, min(max(t.n - t.t0, 0), S));
-            if (cut)
-#pragma unroll
-                for (int k = 0; k < S * VEC; ++k)
-                    if (cut >> (k / VEC) & 1) half_of(a[k / 2], k) = 0.f;
             Maps<VEC> own;
             own.identity();
+            with_flag(cut != 0, [&](auto flag) {
 #pragma unroll
-            for (int j = 0; j < S; ++j) {
-                Pack<float, VEC> P, H;
+                for (int j = 0; j < S; ++j) {
+                    Pack<float, VEC> P, H;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    P.v[e] = half_of(a[(j * VEC + e) / 2], j * VEC + e);
-                    H.v[e] = half_of(b[(j * VEC + e) / 2], j * VEC + e);
+                    for (int e = 0; e < VEC; ++e) {
+                        P.v[e] = half_of(a[(j * VEC + e) / 2], j * VEC + e);
+                        H.v[e] = half_of(b[(j * VEC + e) / 2], j * VEC + e);
+                    }
+                    if (decltype(flag)::value && (cut >> j & 1)) own.cut();
+                    own.then(P, H);
                 }
-                own.then(P, H);
-            }
+            });
             float h[VEC];
             auto &wm = sm.wm[WALK ? t.k & 1 : 0];
             wm.P[warp][lane] = own.P;
@@ -678,50 +716,55 @@ __global__ void __launch_bounds__(32 * W, CTAS)
             __syncthreads();
             if (next) fetch(tn);  // every warp has read the buffer
             if constexpr (WALK) {
-                walk_state<VEC, W>(wm, s, h);
+                walk_state<VEC, W>(wm, s, h, cuts);
                 if (!next && warp == 0 && t.in && p.hN)
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) p.hN[(int64_t)t.b * p.D + t.d + e] = s[e];
             } else {
                 const bool more = (t.k + 1) * TT < t.n;  // a later tile waits for this one
                 const bool last = t.j == ch.group - 1;
-                if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, wm);
-                Maps<VEC> m = prefix_maps<VEC, W>(ch, t, wm, sm.gm);
+                if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, wm, cuts);
+                Maps<VEC> m = prefix_maps<VEC, W>(ch, t, wm, sm.gm, cuts);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e)
                     s[e] = t.in && p.h0 && t.g == 0 ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
                 group_state<VEC>(ch, t, s);
                 if (warp == W - 1 && (last || !more)) {
                     Maps<VEC> end = m;
-                    end.then(own.P, own.H);
-                    end.apply(s, h);
+                    with_flag(cuts, [&](auto flag) { end.template then<decltype(flag)::value>(own.P, own.H); });
+                    end.apply(s, h, cuts);
                     if (more)
                         leave_group<VEC>(ch, t, h);
                     else if (t.in && p.hN)
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) p.hN[(int64_t)t.b * p.D + t.d + e] = h[e];
                 }
-                m.apply(s, h);
+                m.apply(s, h, cuts);
             }
             T *ph = static_cast<T *>(p.h) + t.b * p.sh[0] + t.t0 * p.sh[1] + t.d;
+            with_flag(cut != 0, [&](auto flag) {
 #pragma unroll
-            for (int j = 0; j < S; ++j)
-                if (j < t.cnt) {
-                    Pack<T, VEC> o;
-                    if constexpr (VEC == 1) {
-                        h[0] = fmaf(half_of(a[j / 2], j), h[0], half_of(b[j / 2], j));
-                        o.v[0] = cvt_out<T>(h[0]);
-                    } else {
+                for (int j = 0; j < S; ++j)
+                    if (j < t.cnt) {
+                        Pack<T, VEC> o;
+                        if (decltype(flag)::value && (cut >> j & 1))
 #pragma unroll
-                        for (int e = 0; e < VEC; e += 2) {
-                            const int q = (j * VEC + e) / 2;
-                            const float2 n = __ffma2_rn(a[q], make_float2(h[e], h[e + 1]), b[q]);
-                            o.v[e] = cvt_out<T>(h[e] = n.x);
-                            o.v[e + 1] = cvt_out<T>(h[e + 1] = n.y);
+                            for (int e = 0; e < VEC; ++e) h[e] = 0.f;
+                        if constexpr (VEC == 1) {
+                            h[0] = fmaf(half_of(a[j / 2], j), h[0], half_of(b[j / 2], j));
+                            o.v[0] = cvt_out<T>(h[0]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < VEC; e += 2) {
+                                const int q = (j * VEC + e) / 2;
+                                const float2 n = __ffma2_rn(a[q], make_float2(h[e], h[e + 1]), b[q]);
+                                o.v[e] = cvt_out<T>(h[e] = n.x);
+                                o.v[e + 1] = cvt_out<T>(h[e + 1] = n.y);
+                            }
                         }
+                        *reinterpret_cast<Pack<T, VEC> *>(ph + j * p.sh[1]) = o;
                     }
-                    *reinterpret_cast<Pack<T, VEC> *>(ph + j * p.sh[1]) = o;
-                }
+            });
         } else if (next) {
             fetch(tn);
         }
@@ -754,6 +797,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
     const FwdParams &f = p.f;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned total = ch.chains.d * (unsigned)ch.tiles;
+    const bool cuts = f.resets != nullptr;
     const int trow = (W - 1 - warp) * S;  // this warp's first token in the tile: warp 0 holds the last ones
 
     if (TMA) {
@@ -876,9 +920,8 @@ __global__ void __launch_bounds__(32 * W, CTAS)
                 for (int u = TP - 1; u >= 0; --u)
                     if (j0 + u < t.cnt) {  // what the buffer holds behind the end does not count
                         const Pack<T, VEC> &g = dh[j0 + u];
-                        if (cut >> (j0 + u) & 1) {  // nothing passes
-#pragma unroll
-                            for (int e = 0; e < VEC; ++e) own.P.v[e] = own.H.v[e] = 0.f;
+                        if (cut >> (j0 + u) & 1) {
+                            own.cut();
                         } else if constexpr (VEC == 1) {
                             const float av = half_of(a[0], u);
                             own.H.v[0] = av * (own.H.v[0] + cvt_f32(g.v[0]));
@@ -908,30 +951,30 @@ __global__ void __launch_bounds__(32 * W, CTAS)
             if (next) fetch(tn, buf ^ 1);
             if (!TMA) copy_commit();
             if constexpr (WALK) {
-                walk_state<VEC, W>(wm, s, C);
+                walk_state<VEC, W>(wm, s, C, cuts);
                 if (!next && warp == 0 && t.in && p.dh0)
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) p.dh0[(int64_t)t.b * f.D + t.d + e] = s[e];
             } else {
                 const bool more = t.t0 - trow > 0;  // an earlier tile waits for this one
                 const bool last = t.j == ch.group - 1;
-                if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, wm);
-                Maps<VEC> m = prefix_maps<VEC, W>(ch, t, wm, sm.gm);
+                if (warp == 0 && more && !last) publish_map<VEC, W>(ch, t, wm, cuts);
+                Maps<VEC> m = prefix_maps<VEC, W>(ch, t, wm, sm.gm, cuts);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e)
                     s[e] = t.in && p.dhN && t.g == 0 ? p.dhN[(int64_t)t.b * f.D + t.d + e] : 0.f;
                 group_state<VEC>(ch, t, s);
                 if (warp == W - 1 && (last || !more)) {
                     Maps<VEC> end = m;
-                    end.then(own.P, own.H);
-                    end.apply(s, C);
+                    with_flag(cuts, [&](auto flag) { end.template then<decltype(flag)::value>(own.P, own.H); });
+                    end.apply(s, C, cuts);
                     if (more)
                         leave_group<VEC>(ch, t, C);
                     else if (t.in && p.dh0)
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) p.dh0[(int64_t)t.b * f.D + t.d + e] = C[e];
                 }
-                m.apply(s, C);
+                m.apply(s, C, cuts);
             }
 
             T *qx = static_cast<T *>(p.dx) + t.b * p.sdx[0] + t.t0 * p.sdx[1] + t.d;

@@ -440,3 +440,34 @@ def test_a_nan_stays_in_its_row_and_channel(cuda):
                 assert h[1, 50:, 7].isnan().all() and hN[1, 7].isnan()
                 h[1, 50:, 7] = ref[1, 50:, 7]
                 assert torch.equal(h, ref)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("B,L,D", [(2, 300, 64), (2, 300, 33), (40, 130, 640), (40, 70, 641)])
+def test_a_reset_stops_infinities_and_nan(cuda, B, L, D, dtype):
+    """Documents that share a row do not see each other, whatever the one
+    before holds: NaN and infinities stay before the reset going forward, and
+    behind it going backward."""
+    v = _case(5, B, L, D, dtype)
+    v["resets"] = np.zeros((B, L), np.uint8)
+    cuts = [0, 37, 64, 65, L - 3]
+    v["resets"][:, cuts] = 1
+    clean = _dev(v)
+    href, fref = _forward(clean)
+    gref = _backward(clean, href)
+    for bad in (float("nan"), float("inf")):
+        t = {k: None if a is None else a.clone() for k, a in clean.items()}
+        t["x"][0, 40:44] = bad       # the document from 37 to 63
+        t["h0"][1] = bad             # before a reset at the first token: unseen
+        h, hN = _forward(t)
+        assert not h[0, 44:64].isfinite().any()
+        h[0, 40:64] = href[0, 40:64]
+        assert torch.equal(h, href) and torch.equal(hN, fref)
+        t = {k: None if a is None else a.clone() for k, a in clean.items()}
+        t["dh"][0, 60:64] = bad
+        dx, dr, di, dlam, dh0 = _backward(t, href)
+        for got, ref in zip((dx, dr, di), gref):
+            assert not got[0, 40:60].isfinite().all()
+            got[0, 37:64] = ref[0, 37:64]
+            assert torch.equal(got, ref)
+        assert torch.equal(dh0, gref[4]) and not dh0.any()  # the first token resets
