@@ -217,33 +217,32 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
-// 32 columns of one row, without a bulk store: 16 bytes at a time where the
-// row is aligned and the columns exist.
-__device__ __forceinline__ void store_row(const I8Params &g, int64_t row, int c0, const float (&f)[32], bool aligned) {
-    if (g.mode == 0) {
-        __half *o = static_cast<__half *>(g.y) + row * g.ldy + c0;
+// 32 rows x 32 columns (a lane holds a row) without a bulk store: turned round
+// in a shared-memory box, so that a warp writes a row's 32 columns at once.
+__device__ __forceinline__ void store_block(const I8Params &g, uint8_t *box, int64_t row0, int c0,
+                                            const float (&f)[32]) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-            if (aligned && c0 + j + 8 <= g.n) {
-                uint32_t w[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const __half2 h = __floats2half2_rn(f[j + 2 * q], f[j + 2 * q + 1]);
-                    w[q] = *reinterpret_cast<const uint32_t *>(&h);
-                }
-                *reinterpret_cast<uint4 *>(o + j) = make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (c0 + j + q < g.n) o[j + q] = __float2half_rn(f[j + q]);
-            }
+    for (int j = 0; j < 8; ++j)  // 16-byte chunk j of a row at j ^ (row % 8): no bank conflicts either way
+        *reinterpret_cast<float4 *>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+            make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+    __syncwarp();
+    const int rows = (int)min((int64_t)32, g.rows - row0);
+    if (c0 + lane < g.n) {
+        const int64_t o0 = row0 * g.ldy + c0 + lane;
+#pragma unroll 8
+        for (int r = 0; r < rows; ++r) {
+            const float v =
+                *reinterpret_cast<const float *>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+            if (g.mode == 0)
+                static_cast<__half *>(g.y)[o0 + r * g.ldy] = __float2half_rn(v);
+            else if (g.mode == 1)
+                static_cast<float *>(g.y)[o0 + r * g.ldy] += v;
+            else
+                static_cast<float *>(g.y)[o0 + r * g.ldy] = v;
         }
-    } else {
-        float *o = static_cast<float *>(g.y) + row * g.ldy + c0;
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (c0 + j < g.n) o[j] = g.mode == 1 ? o[j] + f[j] : f[j];
     }
+    __syncwarp();
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -378,10 +377,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // an FP16 box takes 64 columns: of a BN that is an odd multiple of 32 the last 32
                 // go out without one, since the box's other half would be the next tile's
                 const bool boxed = p.boxes && (g.mode != 0 || c + 32 < p.BN);
-                if (boxed) {  // the bulk store that last read this box has finished reading it
-                    if (lane == 0) bulk_wait_group_read<1>();
-                    __syncwarp();
-                }
+                // the bulk store that last read this box has finished reading it
+                if (lane == 0) bulk_wait_group_read<1>();
+                __syncwarp();
 #pragma unroll
                 for (int hlf = 0; hlf < 2; ++hlf) {
                     if (hlf && g.mode != 0) break;
@@ -401,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int j = 0; j < 32; ++j) f[j] += __shfl_sync(0xffffffffu, bl, j);
                     }
                     if (!boxed) {
-                        if (row < g.rows) store_row(g, row, c0, f, p.boxes);
+                        store_block(g, box, row0, c0, f);
                         continue;
                     }
                     // row `lane` of a 32-row box with the TMA 128-byte swizzle: chunk j at j ^ (row % 8)

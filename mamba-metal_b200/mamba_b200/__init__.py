@@ -785,9 +785,13 @@ def gated_recurrence_backward(dh, x, r, i, lam, h, c=8.0, initial_state=None, le
     a = _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets, h)
     if dfinal_state is not None:
         _check_tensor(dfinal_state, "dfinal_state", what, (a.batch, a.dim), lam.dtype, x.device)
-    dx = _recurrence_out("dx", what, dx, x, lengths)
-    dr = _recurrence_out("dr", what, dr, x, lengths)
-    di = _recurrence_out("di", what, di, x, lengths)
+    if dx is None and dr is None and di is None:  # one allocation (and one fill) for the three
+        shape = (3,) + tuple(x.shape)
+        dx, dr, di = (x.new_empty(shape) if lengths is None else x.new_zeros(shape)).unbind(0)
+    else:
+        dx = _recurrence_out("dx", what, dx, x, lengths)
+        dr = _recurrence_out("dr", what, dr, x, lengths)
+        di = _recurrence_out("di", what, di, x, lengths)
     dlam = lam.new_empty(lam.shape)
     dh0 = lam.new_empty((a.batch, a.dim))
     sg, sx, sr, si = dh.stride(), dx.stride(), dr.stride(), di.stride()

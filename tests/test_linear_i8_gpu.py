@@ -15,6 +15,16 @@ from oracle import recurrent_block as rb
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(scope="module", autouse=True)
+def _leave_no_cached_memory():
+    """Later tests find the allocator as a fresh process has it: with large
+    cached blocks, tensors would no longer come from calls that synchronise."""
+    yield
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+
+
+
 def _dev(a):
     return None if a is None else torch.from_numpy(np.ascontiguousarray(a)).cuda()
 
