@@ -156,22 +156,35 @@ constexpr int kRingThreads = 1024, kRingBwdThreads = 768;  // resident threads p
 
 template <int N>
 struct RingRow {
-    const void *src[N];    // first row of each tensor
-    int64_t stride[N];     // bytes between rows
-    uint32_t bytes[N];     // bytes of a row, 0: tensor absent
-    uint32_t offset[N];    // within a stage
-    uint32_t stage, total; // bytes of a stage, bytes fetched per row
+    const void *src[N];  // first row of each tensor
+    int64_t stride[N];   // bytes between rows
+    uint32_t bytes[N];   // bytes of a row, 0: tensor absent
+    uint32_t offset[N];  // within a stage
+    uint32_t stage;      // bytes of a stage
     int stages;
+    // Bulk copies start and end on 16-byte boundaries: a row that does not is
+    // copied with the bytes around it (of its neighbours, or in the 16 bytes of
+    // memory that its first or last byte lies in) and starts this far behind
+    // its place.
+    __device__ __forceinline__ uint32_t shift(int k, int64_t row) const {
+        return (uint32_t)(reinterpret_cast<uintptr_t>(src[k]) + row * stride[k]) & 15u;
+    }
 };
 
 template <int N>
 __device__ __forceinline__ void fetch_row(const RingRow<N> &r, uint8_t *ring, uint64_t *full, int64_t row, int s) {
-    mbar_arrive_expect_tx(&full[s], r.total);
+    uint32_t bytes[N], total = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        bytes[k] = r.bytes[k] ? (r.shift(k, row) + r.bytes[k] + 15) / 16 * 16 : 0;
+        total += bytes[k];
+    }
+    mbar_arrive_expect_tx(&full[s], total);
 #pragma unroll
     for (int k = 0; k < N; ++k)
-        if (r.bytes[k])
-            bulk_load(ring + s * r.stage + r.offset[k], static_cast<const uint8_t *>(r.src[k]) + row * r.stride[k],
-                      r.bytes[k], &full[s]);
+        if (bytes[k])
+            bulk_load(ring + s * r.stage + r.offset[k],
+                      static_cast<const uint8_t *>(r.src[k]) + row * r.stride[k] - r.shift(k, row), bytes[k], &full[s]);
 }
 __device__ __forceinline__ void await_row(uint64_t *bar, uint32_t parity) {
     if (!mbar_wait_bounded(bar, parity)) atomicOr(&g_block_norm_error, kErrBlockNormTimeout);
@@ -213,10 +226,10 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_kernel(const NormParams
     if (RING) start_ring<3>(ring, smem, full, p.rows);
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const uint8_t *place = smem + at.s * ring.stage;
-        const T *y = RING ? reinterpret_cast<const T *>(place) : static_cast<const T *>(p.y) + row * p.sy;
-        const T *z = RING ? reinterpret_cast<const T *>(place + ring.offset[1])
-                          : static_cast<const T *>(p.z) + row * p.sz;
-        const float *res = RING ? reinterpret_cast<const float *>(place + ring.offset[2]) : p.res + row * p.cols;
+        auto at_place = [&](int k) { return place + ring.offset[k] + (VEC == 1 ? ring.shift(k, row) : 0u); };
+        const T *y = RING ? reinterpret_cast<const T *>(at_place(0)) : static_cast<const T *>(p.y) + row * p.sy;
+        const T *z = RING ? reinterpret_cast<const T *>(at_place(1)) : static_cast<const T *>(p.z) + row * p.sz;
+        const float *res = RING ? reinterpret_cast<const float *>(at_place(2)) : p.res + row * p.cols;
         if (RING) await_row(&full[at.s], at.parity);
         float v[NV][VEC], gz[NV][VEC], r[NV][VEC];
         float ss = 0.f;
@@ -294,13 +307,12 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_bwd_kernel(const NormGr
     float rs_next = p.f.rstd_post[blockIdx.x], rp_next = first ? p.f.rstd_pre[blockIdx.x] : 0.f;  // grid <= rows
     for (int64_t row = blockIdx.x; row < p.f.rows; row += gridDim.x) {
         const uint8_t *place = smem + at.s * ring.stage;
-        const T *y = RING ? reinterpret_cast<const T *>(place) : static_cast<const T *>(p.f.y) + row * p.f.sy;
-        const T *z = RING ? reinterpret_cast<const T *>(place + ring.offset[1])
-                          : static_cast<const T *>(p.f.z) + row * p.f.sz;
-        const T *go = RING ? reinterpret_cast<const T *>(place + ring.offset[2])
-                           : static_cast<const T *>(p.dout) + row * cols;
-        const float *dro = RING ? reinterpret_cast<const float *>(place + ring.offset[3]) : p.dres_out + row * cols;
-        const float *r1 = RING ? reinterpret_cast<const float *>(place + ring.offset[4]) : p.f.res_out + row * cols;
+        auto at_place = [&](int k) { return place + ring.offset[k] + (VEC == 1 ? ring.shift(k, row) : 0u); };
+        const T *y = RING ? reinterpret_cast<const T *>(at_place(0)) : static_cast<const T *>(p.f.y) + row * p.f.sy;
+        const T *z = RING ? reinterpret_cast<const T *>(at_place(1)) : static_cast<const T *>(p.f.z) + row * p.f.sz;
+        const T *go = RING ? reinterpret_cast<const T *>(at_place(2)) : static_cast<const T *>(p.dout) + row * cols;
+        const float *dro = RING ? reinterpret_cast<const float *>(at_place(3)) : p.dres_out + row * cols;
+        const float *r1 = RING ? reinterpret_cast<const float *>(at_place(4)) : p.f.res_out + row * cols;
         // this row's factors were loaded a row ago, the next row's are on their way
         const float rs = rs_next, rp = rp_next;
         const int64_t after = row + gridDim.x;
@@ -502,11 +514,9 @@ int64_t max_parts(int64_t rows, int cols) {
 template <int N>
 bool plan_ring(RingRow<N> &r, int64_t rows, int &ctas_per_sm) {
     uint32_t at = 0;
-    r.total = 0;
     for (int k = 0; k < N; ++k) {
         r.offset[k] = at;
-        at += (r.bytes[k] + 127) / 128 * 128;
-        r.total += r.bytes[k];
+        if (r.bytes[k]) at += (r.bytes[k] + 30 + 127) / 128 * 128;  // and what surrounds an unaligned row
     }
     r.stage = at;
     for (;; --ctas_per_sm) {
@@ -516,9 +526,9 @@ bool plan_ring(RingRow<N> &r, int64_t rows, int &ctas_per_sm) {
     return r.stages >= 1 && rows >= 3LL * ctas_per_sm * device_sm_count();
 }
 
-template <typename T, int NV, int MAXT>
+template <typename T, int VEC, int NV, int MAXT>
 int ring_fwd(const NormParams &p, const RingRow<3> &r, int ctas, int threads, cudaStream_t st) {
-    auto kernel = block_norm_kernel<T, 8, NV, MAXT, true>;
+    auto kernel = block_norm_kernel<T, VEC, NV, MAXT, true>;
     if (allow_smem(kernel)) return -1;
     kernel<<<(unsigned)(ctas * device_sm_count()), threads, (size_t)r.stage * r.stages, st>>>(p, r);
     return launch_status("block_norm kernel");
@@ -526,7 +536,7 @@ int ring_fwd(const NormParams &p, const RingRow<3> &r, int ctas, int threads, cu
 template <typename T>
 int launch_fwd(const NormParams &p, bool vec, cudaStream_t st) {
     RingRow<3> r{};
-    if (vec && p.cols <= 8192) {
+    if (p.cols <= 8192) {
         const uint32_t half = (uint32_t)(p.cols * sizeof(T));
         r.src[0] = p.y;
         r.src[1] = p.z;
@@ -540,8 +550,13 @@ int launch_fwd(const NormParams &p, bool vec, cudaStream_t st) {
         const bool one = p.cols <= 4096;
         const int threads = threads_for(p.cols, one ? 8 : 16);
         int ctas = ring_ctas(threads, kRingThreads);
-        if (plan_ring<3>(r, p.rows, ctas))
-            return one ? ring_fwd<T, 1, 512>(p, r, ctas, threads, st) : ring_fwd<T, 2, 512>(p, r, ctas, threads, st);
+        if (plan_ring<3>(r, p.rows, ctas)) {
+            if (vec)
+                return one ? ring_fwd<T, 8, 1, 512>(p, r, ctas, threads, st)
+                           : ring_fwd<T, 8, 2, 512>(p, r, ctas, threads, st);
+            return one ? ring_fwd<T, 1, 8, 512>(p, r, ctas, threads, st)
+                       : ring_fwd<T, 1, 16, 512>(p, r, ctas, threads, st);
+        }
     }
     const unsigned grid = (unsigned)std::min<int64_t>(p.rows, 0x7fffffff);
     if (vec && p.cols <= 4096)
@@ -555,9 +570,9 @@ int launch_fwd(const NormParams &p, bool vec, cudaStream_t st) {
     return launch_status("block_norm kernel");
 }
 
-template <typename T, int NV, int MAXT, int CTAS>
+template <typename T, int VEC, int NV, int MAXT, int CTAS>
 int ring_bwd(const NormGradParams &p, const RingRow<5> &r, unsigned grid, int threads, cudaStream_t st) {
-    auto kernel = block_norm_bwd_kernel<T, 8, NV, MAXT, true, CTAS>;
+    auto kernel = block_norm_bwd_kernel<T, VEC, NV, MAXT, true, CTAS>;
     if (allow_smem(kernel)) return -1;
     kernel<<<grid, threads, (size_t)r.stage * r.stages, st>>>(p, r);
     return launch_status("block_norm_backward kernel");
@@ -567,7 +582,7 @@ template <typename T>
 int launch_bwd(const NormGradParams &p, bool vec, unsigned &grid, cudaStream_t st) {
     const int cols = p.f.cols;
     RingRow<5> r{};
-    if (vec && cols <= 8192) {
+    if (cols <= 8192) {
         const uint32_t half = (uint32_t)(cols * sizeof(T)), whole = (uint32_t)cols * 4;
         const void *src[5] = {p.f.y, p.f.z, p.dout, p.dres_out, p.f.res_out};
         const int64_t stride[5] = {p.f.sy * (int64_t)sizeof(T), p.f.sz * (int64_t)sizeof(T), half, whole, whole};
@@ -582,10 +597,13 @@ int launch_bwd(const NormGradParams &p, bool vec, unsigned &grid, cudaStream_t s
         int ctas = std::min(16, ring_ctas(threads, kRingBwdThreads));
         if (plan_ring<5>(r, p.f.rows, ctas)) {
             grid = std::min(grid, (unsigned)(ctas * device_sm_count()));
-            if (!one) return ring_bwd<T, 2, 512, 1>(p, r, grid, threads, st);
+            if (!one)
+                return vec ? ring_bwd<T, 8, 2, 512, 1>(p, r, grid, threads, st)
+                           : ring_bwd<T, 1, 16, 512, 1>(p, r, grid, threads, st);
+            if (!vec) return ring_bwd<T, 1, 8, 512, 1>(p, r, grid, threads, st);
             // three CTAs fit by 80 registers a thread; with fewer, more registers are faster
-            return threads <= 256 && ctas >= 3 ? ring_bwd<T, 1, 256, 3>(p, r, grid, threads, st)
-                                             : ring_bwd<T, 1, 512, 1>(p, r, grid, threads, st);
+            return threads <= 256 && ctas >= 3 ? ring_bwd<T, 8, 1, 256, 3>(p, r, grid, threads, st)
+                                               : ring_bwd<T, 8, 1, 512, 1>(p, r, grid, threads, st);
         }
     }
     grid = std::min(grid, (unsigned)kDirectParts);

@@ -103,7 +103,9 @@ def _check_backward(v, f, grads, dtype):
 SHAPES = [(1, 1), (1, 8), (3, 7), (2, 64), (5, 256), (4, 264), (130, 1000), (9, 1001), (700, 72), (300, 2048),
           (64, 2560), (3, 4096), (3, 4099), (2, 8192), (2, 8200), (2, 16384), (2, 12001),
           # enough rows for persistent CTAs with rows fetched ahead: 1, 2, 8 and 16 warps, one and two rows of room
-          (14500, 72), (7300, 264), (2000, 2048), (1000, 4096), (950, 8192)]
+          (14500, 72), (7300, 264), (2000, 2048), (1000, 4096), (950, 8192),
+          # and of rows that start and end anywhere
+          (14500, 71), (3700, 513), (2000, 2045), (950, 7001)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
@@ -121,11 +123,10 @@ def test_forward_and_backward(cuda, T, D, gate, weights, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 @pytest.mark.parametrize("offset", [0, 1, 8])
-@pytest.mark.parametrize("D", [40, 136, 1000])
-def test_strided_views(cuda, dtype, offset, D):
+@pytest.mark.parametrize("T,D", [(21, 40), (21, 136), (21, 1000), (4000, 500)])
+def test_strided_views(cuda, dtype, offset, T, D):
     """y and the gate as column blocks of one projection, their gradients into
     column blocks of another."""
-    T = 21
     v = _case(6, T, D, dtype)
     t = _dev(v)
     pitch = 2 * D + 32
@@ -147,8 +148,9 @@ def test_strided_views(cuda, dtype, offset, D):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
-def test_in_place_and_missing_parts(cuda, dtype):
-    v = _case(7, 33, 520, dtype)
+@pytest.mark.parametrize("T,D", [(33, 520), (4000, 520), (4000, 523)])
+def test_in_place_and_missing_parts(cuda, T, D, dtype):
+    v = _case(7, T, D, dtype)
     t = _dev(v)
     f = _forward(t)
     res = t["res"].clone()
