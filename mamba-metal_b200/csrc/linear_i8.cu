@@ -20,38 +20,50 @@ __device__ unsigned int g_linear_i8_error = 0;
 namespace {
 
 // ---- row quantiser ----------------------------------------------------------
+// One read and one write of the row, which is held in registers as it was
+// loaded.  Bound by bytes as long as an element costs few instructions: the
+// largest magnitude is taken over packed FP16 bits, and the rounding stays in
+// the FMA pipe (a conversion instruction has a quarter of its rate).
 constexpr int kQThreads = 256;
-constexpr int kQRegs = 4;  // groups of VEC channels cached per thread
+template <int VEC>
+constexpr int kQRegs = VEC == 1 ? 16 : 8;  // groups of VEC channels a thread holds
 
-template <int N>
-__device__ __forceinline__ void load_n(const float *p, float (&v)[N]) {
-    if constexpr (N == 1) {
-        v[0] = *p;
+// VEC elements as loaded: 16 bytes, or one element.
+template <typename T, int VEC>
+struct Raw {
+    uint32_t w[VEC == 1 ? 1 : 4];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ Raw<T, VEC> load_raw(const T *p) {
+    Raw<T, VEC> r;
+    if constexpr (VEC == 1) {
+        if constexpr (sizeof(T) == 2)
+            r.w[0] = __half_as_ushort(*p);
+        else
+            r.w[0] = __float_as_uint(*p);
     } else {
-#pragma unroll
-        for (int k = 0; k < N; k += 4) {
-            const float4 q = *reinterpret_cast<const float4 *>(p + k);
-            v[k] = q.x;
-            v[k + 1] = q.y;
-            v[k + 2] = q.z;
-            v[k + 3] = q.w;
-        }
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        r.w[0] = v.x;
+        r.w[1] = v.y;
+        r.w[2] = v.z;
+        r.w[3] = v.w;
     }
+    return r;
 }
-template <int N>
-__device__ __forceinline__ void load_n(const __half *p, float (&v)[N]) {
-    if constexpr (N == 1) {
-        v[0] = __half2float(*p);
-    } else {
-        const uint4 raw = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+template <typename T, int VEC>
+__device__ __forceinline__ float element(const Raw<T, VEC> &r, int k) {
+    if constexpr (sizeof(T) == 2)
+        return __half2float(__ushort_as_half((unsigned short)(r.w[k / 2] >> (16 * (k & 1)))));
+    else
+        return __uint_as_float(r.w[k]);
+}
+// Largest magnitudes as bits, which are ordered like the values with infinity
+// and NaN above all numbers; FP16: of the two halves of a word each for itself.
+template <typename T, int VEC>
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, const Raw<T, VEC> &r) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
-            v[2 * k] = f.x;
-            v[2 * k + 1] = f.y;
-        }
-    }
+    for (uint32_t w : r.w) m = sizeof(T) == 2 ? __vmaxu2(m, w & 0x7fff7fffu) : max(m, w & 0x7fffffffu);
+    return m;
 }
 
 // round(x / s) with ties to even, of the exact quotient: the product with the
@@ -75,33 +87,48 @@ __device__ __forceinline__ int quantise(float x, float s, float inv, bool tiny) 
     return max(-127, min(127, q));
 }
 
+// Four elements, for a scale of 2^-100 or more: adding 1.5 * 2^23 rounds the
+// product with the reciprocal to an integer, which is then the sum's low byte
+// (|x| <= 127 s (1 + 2^-24), so it is 127 at most).  `off` is set where the
+// remainder says that quantise() has to look at a half.
+__device__ __forceinline__ uint32_t quantise4(const float (&x)[4], float s, float inv, float half, bool &off) {
+    const float magic = 12582912.f;
+    uint32_t t[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float v = fmaf(x[k], inv, magic);
+        off |= fabsf(fmaf(-(v - magic), s, x[k])) >= half;
+        t[k] = __float_as_uint(v);
+    }
+    return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+}
+
 template <typename T, int VEC, int TPR>
 __global__ void __launch_bounds__(kQThreads)
     quantize_rows_kernel(const T *__restrict__ x, int64_t ldx, int8_t *__restrict__ q, int64_t ldq,
                          float *__restrict__ scale, int64_t rows, int cols) {
+    constexpr int REGS = kQRegs<VEC>;
     __shared__ uint32_t sm[kQThreads / 32];
     const int tid = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * (kQThreads / TPR) + threadIdx.x / TPR;
     if (TPR == 32 && row >= rows) return;  // TPR 256: one row per CTA, always inside
     const T *xr = x + row * ldx;
     int8_t *qr = q + row * ldq;
-    float v[kQRegs][VEC];
-    uint32_t m = 0;  // largest |x| as bits: ordered like the values, infinity and NaN above all numbers
+    Raw<T, VEC> v[REGS];
+    uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < kQRegs; ++j) {
+    for (int j = 0; j < REGS; ++j) {
         const int64_t c = (int64_t)(j * TPR + tid) * VEC;
-        if (c < cols) {
-            load_n(xr + c, v[j]);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) m = max(m, __float_as_uint(v[j][k]) & 0x7fffffffu);
-        }
+        if (c < cols)
+            v[j] = load_raw<T, VEC>(xr + c);
+        else
+            v[j] = Raw<T, VEC>{};
     }
-    for (int64_t c = (int64_t)(kQRegs * TPR + tid) * VEC; c < cols; c += TPR * VEC) {
-        float u[VEC];
-        load_n(xr + c, u);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) m = max(m, __float_as_uint(u[k]) & 0x7fffffffu);
-    }
+    for (int j = 0; j < REGS; ++j) m = max_bits(m, v[j]);
+    for (int64_t c = (int64_t)(REGS * TPR + tid) * VEC; c < cols; c += TPR * VEC)
+        m = max_bits(m, load_raw<T, VEC>(xr + c));
+    if (sizeof(T) == 2) m = max(m >> 16, m & 0xffffu);
     m = __reduce_max_sync(0xffffffffu, m);
     if (TPR > 32) {
         if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
@@ -109,36 +136,45 @@ __global__ void __launch_bounds__(kQThreads)
 #pragma unroll
         for (int k = 0; k < kQThreads / 32; ++k) m = max(m, sm[k]);
     }
-    const bool bad = m >= 0x7f800000u;  // an infinity or NaN in the row: scale NaN, q 0
-    const float s = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(m), 127.f);
+    const float top = sizeof(T) == 2 ? __half2float(__ushort_as_half((unsigned short)m)) : __uint_as_float(m);
+    const bool bad = !(top < INFINITY);  // an infinity or NaN in the row: scale NaN, q 0
+    const float s = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(top, 127.f);
     const bool zero = bad || s == 0.f, tiny = s < 7.9e-31f;
-    const float inv = zero ? 0.f : __fdiv_rn(1.f, s);
+    const float inv = zero ? 0.f : __fdiv_rn(1.f, s), half = 0.5f * s;
     if (tid == 0) scale[row] = s;
-    auto emit = [&](int64_t c, const float (&u)[VEC]) {
-        int r[VEC];
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) r[k] = zero ? 0 : quantise(u[k], s, inv, tiny);
+    auto emit = [&](int64_t c, const Raw<T, VEC> &u) {
         if constexpr (VEC == 1) {
-            qr[c] = (int8_t)r[0];
+            qr[c] = (int8_t)(zero ? 0 : quantise(element(u, 0), s, inv, tiny));
         } else {
-            uint32_t w[2];
+            uint32_t w[VEC / 4];
+            bool off = zero || tiny;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                w[h] = (r[4 * h] & 0xff) | (r[4 * h + 1] & 0xff) << 8 | (r[4 * h + 2] & 0xff) << 16 |
-                       (uint32_t)r[4 * h + 3] << 24;
-            *reinterpret_cast<uint2 *>(qr + c) = make_uint2(w[0], w[1]);
+            for (int h = 0; h < VEC / 4; ++h) {
+                const float e[4] = {element(u, 4 * h), element(u, 4 * h + 1), element(u, 4 * h + 2),
+                                    element(u, 4 * h + 3)};
+                w[h] = quantise4(e, s, inv, half, off);
+            }
+            if (off) {
+#pragma unroll
+                for (int h = 0; h < VEC / 4; ++h) {
+                    w[h] = 0;
+                    for (int k = 0; k < 4 && !zero; ++k)
+                        w[h] |= (uint32_t)(quantise(element(u, 4 * h + k), s, inv, tiny) & 0xff) << (8 * k);
+                }
+            }
+            if constexpr (VEC == 8)
+                *reinterpret_cast<uint2 *>(qr + c) = make_uint2(w[0], w[1]);
+            else
+                *reinterpret_cast<uint32_t *>(qr + c) = w[0];
         }
     };
 #pragma unroll
-    for (int j = 0; j < kQRegs; ++j) {
+    for (int j = 0; j < REGS; ++j) {
         const int64_t c = (int64_t)(j * TPR + tid) * VEC;
         if (c < cols) emit(c, v[j]);
     }
-    for (int64_t c = (int64_t)(kQRegs * TPR + tid) * VEC; c < cols; c += TPR * VEC) {
-        float u[VEC];
-        load_n(xr + c, u);
-        emit(c, u);
-    }
+    for (int64_t c = (int64_t)(REGS * TPR + tid) * VEC; c < cols; c += TPR * VEC)
+        emit(c, load_raw<T, VEC>(xr + c));
 }
 
 bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -146,7 +182,7 @@ bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p)
 template <typename T, int VEC>
 int launch_quantize(const T *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int64_t rows, int cols,
                     cudaStream_t st) {
-    if (cols <= 32 * VEC * kQRegs && rows > 4LL * device_sm_count()) {
+    if (cols <= 32 * VEC * kQRegs<VEC> && rows > 4LL * device_sm_count()) {
         const int64_t grid = ceil_div64(rows, kQThreads / 32);
         MB_CHECK_ARG(grid <= 0x7fffffffLL, "quantize_rows: too many rows");
         quantize_rows_kernel<T, VEC, 32><<<(unsigned)grid, kQThreads, 0, st>>>(x, ldx, q, ldq, scale, rows, cols);
@@ -604,15 +640,16 @@ int quantize_rows(const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *sca
     MB_CHECK_ARG(scale && aligned_to(scale, 4) && (cols == 0 || (x && q)), "quantize_rows: null pointer");
     MB_CHECK_ARG(aligned_to(x, dtype_size(dtype)), "quantize_rows: pointers must be aligned to their element type");
     MB_CHECK_ARG(rows == 1 || ldq >= cols, "quantize_rows: rows of q overlap (stride)");
-    const bool vec = cols % 8 == 0 && aligned_to(x, 16) && (ldx * (int64_t)dtype_size(dtype)) % 16 == 0 &&
-                     aligned_to(q, 8) && ldq % 8 == 0;
+    const int wide = 16 / (int)dtype_size(dtype);  // elements of 16 bytes
+    const bool vec = cols % wide == 0 && aligned_to(x, 16) && (rows == 1 || (ldx % wide == 0 && ldq % wide == 0)) &&
+                     aligned_to(q, wide);
     if (dtype == MAMBA_F16) {
         auto *p = static_cast<const __half *>(x);
         return vec ? launch_quantize<__half, 8>(p, ldx, q, ldq, scale, rows, cols, st)
                    : launch_quantize<__half, 1>(p, ldx, q, ldq, scale, rows, cols, st);
     }
     auto *p = static_cast<const float *>(x);
-    return vec ? launch_quantize<float, 8>(p, ldx, q, ldq, scale, rows, cols, st)
+    return vec ? launch_quantize<float, 4>(p, ldx, q, ldq, scale, rows, cols, st)
                : launch_quantize<float, 1>(p, ldx, q, ldq, scale, rows, cols, st);
 }
 
