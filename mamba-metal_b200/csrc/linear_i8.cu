@@ -25,8 +25,11 @@ namespace {
 // largest magnitude is taken over packed FP16 bits, and the rounding stays in
 // the FMA pipe (a conversion instruction has a quarter of its rate).
 constexpr int kQThreads = 256;
+// Groups of VEC channels a thread holds.  FP16 rows: 4 (65536 x 512 takes 33
+// us, with 8 it takes 43; 16384 x 2048 takes 29 with either); FP32 rows: 8
+// (16384 x 8192 takes 109 us, with 4 it takes 119).
 template <int VEC>
-constexpr int kQRegs = VEC == 1 ? 16 : 8;  // groups of VEC channels a thread holds
+constexpr int kQRegs = VEC == 8 ? 4 : 8;
 
 // VEC elements as loaded: 16 bytes, or one element.
 template <typename T, int VEC>
@@ -111,7 +114,8 @@ __global__ void __launch_bounds__(kQThreads)
     __shared__ uint32_t sm[kQThreads / 32];
     const int tid = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * (kQThreads / TPR) + threadIdx.x / TPR;
-    if (TPR == 32 && row >= rows) return;  // TPR 256: one row per CTA, always inside
+    if (TPR == 32 && row >= rows) return;
+    const bool in = row < rows;  // rows of a CTA share its barrier
     const T *xr = x + row * ldx;
     int8_t *qr = q + row * ldq;
     Raw<T, VEC> v[REGS];
@@ -119,14 +123,14 @@ __global__ void __launch_bounds__(kQThreads)
 #pragma unroll
     for (int j = 0; j < REGS; ++j) {
         const int64_t c = (int64_t)(j * TPR + tid) * VEC;
-        if (c < cols)
+        if (in && c < cols)
             v[j] = load_raw<T, VEC>(xr + c);
         else
             v[j] = Raw<T, VEC>{};
     }
 #pragma unroll
     for (int j = 0; j < REGS; ++j) m = max_bits(m, v[j]);
-    for (int64_t c = (int64_t)(REGS * TPR + tid) * VEC; c < cols; c += TPR * VEC)
+    for (int64_t c = (int64_t)(REGS * TPR + tid) * VEC; in && c < cols; c += TPR * VEC)
         m = max_bits(m, load_raw<T, VEC>(xr + c));
     if (sizeof(T) == 2) m = max(m >> 16, m & 0xffffu);
     m = __reduce_max_sync(0xffffffffu, m);
@@ -134,7 +138,8 @@ __global__ void __launch_bounds__(kQThreads)
         if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kQThreads / 32; ++k) m = max(m, sm[k]);
+        for (int k = 0; k < TPR / 32; ++k) m = max(m, sm[threadIdx.x / TPR * (TPR / 32) + k]);
+        if (!in) return;
     }
     const float top = sizeof(T) == 2 ? __half2float(__ushort_as_half((unsigned short)m)) : __uint_as_float(m);
     const bool bad = !(top < INFINITY);  // an infinity or NaN in the row: scale NaN, q 0
@@ -179,18 +184,18 @@ __global__ void __launch_bounds__(kQThreads)
 
 bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-template <typename T, int VEC>
+template <typename T, int VEC, int TPR>
 int launch_quantize(const T *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int64_t rows, int cols,
                     cudaStream_t st) {
-    if (cols <= 32 * VEC * kQRegs<VEC> && rows > 4LL * device_sm_count()) {
-        const int64_t grid = ceil_div64(rows, kQThreads / 32);
-        MB_CHECK_ARG(grid <= 0x7fffffffLL, "quantize_rows: too many rows");
-        quantize_rows_kernel<T, VEC, 32><<<(unsigned)grid, kQThreads, 0, st>>>(x, ldx, q, ldq, scale, rows, cols);
-    } else {
-        MB_CHECK_ARG(rows <= 0x7fffffffLL, "quantize_rows: too many rows");
-        quantize_rows_kernel<T, VEC, kQThreads><<<(unsigned)rows, kQThreads, 0, st>>>(x, ldx, q, ldq, scale, rows,
-                                                                                      cols);
-    }
+    const int64_t grid = ceil_div64(rows, kQThreads / TPR);
+    // The fewest threads a row that hold it, while every SM still gets a CTA:
+    // 16384 x 2560 FP16 takes 39 us, with a whole CTA a row 62; 1024 x 2048
+    // takes 10, with four CTAs per SM asked for 12.
+    if constexpr (TPR < kQThreads)
+        if (cols > TPR * VEC * kQRegs<VEC> || grid <= device_sm_count())
+            return launch_quantize<T, VEC, 2 * TPR>(x, ldx, q, ldq, scale, rows, cols, st);
+    MB_CHECK_ARG(grid <= 0x7fffffffLL, "quantize_rows: too many rows");
+    quantize_rows_kernel<T, VEC, TPR><<<(unsigned)grid, kQThreads, 0, st>>>(x, ldx, q, ldq, scale, rows, cols);
     return launch_status("quantize_rows kernel");
 }
 
@@ -645,12 +650,12 @@ int quantize_rows(const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *sca
                      aligned_to(q, wide);
     if (dtype == MAMBA_F16) {
         auto *p = static_cast<const __half *>(x);
-        return vec ? launch_quantize<__half, 8>(p, ldx, q, ldq, scale, rows, cols, st)
-                   : launch_quantize<__half, 1>(p, ldx, q, ldq, scale, rows, cols, st);
+        return vec ? launch_quantize<__half, 8, 32>(p, ldx, q, ldq, scale, rows, cols, st)
+                   : launch_quantize<__half, 1, 32>(p, ldx, q, ldq, scale, rows, cols, st);
     }
     auto *p = static_cast<const float *>(x);
-    return vec ? launch_quantize<float, 4>(p, ldx, q, ldq, scale, rows, cols, st)
-               : launch_quantize<float, 1>(p, ldx, q, ldq, scale, rows, cols, st);
+    return vec ? launch_quantize<float, 4, 32>(p, ldx, q, ldq, scale, rows, cols, st)
+               : launch_quantize<float, 1, 32>(p, ldx, q, ldq, scale, rows, cols, st);
 }
 
 int linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw, const float *w_scale,
