@@ -536,8 +536,9 @@ int mamba_linear(const void *x, int64_t ldx, const void *w, const float *bias, v
  * x [rows, cols] of dtype (MAMBA_F32 or MAMBA_F16) with row stride ldx, q
  * with row stride ldq >= cols (elements; columns beyond cols are left as
  * they were), scale FP32 [rows].  Activations per token, and weights [n, k]
- * per output channel.  For mamba_linear_i8's tensor-core kernels give q a
- * 16-byte aligned start and an ldq that is a multiple of 16.  0 / -1. */
+ * per output channel.  q may not start where x or scale does.  For
+ * mamba_linear_i8's tensor-core kernels give q a 16-byte aligned start and an
+ * ldq that is a multiple of 16.  0 / -1. */
 int mamba_quantize_rows(const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int64_t rows, int cols,
                         int dtype, void *stream);
 
@@ -547,7 +548,8 @@ int mamba_quantize_rows(const void *x, int64_t ldx, int8_t *q, int64_t ldq, floa
  * (the modes of mamba_linear).  x [rows, k] and w [n, k] int8 with row
  * strides ldx and ldw, x_scale FP32 [rows], w_scale FP32 [n], bias FP32 [n]
  * or NULL, y row stride ldy.  The sums are exact 32-bit integers, which
- * bounds k to 131071; any value of int8 may occur.  16-byte aligned x and w
+ * bounds k to 131071; any value of int8 may occur.  y may not be one of the
+ * inputs.  16-byte aligned x and w
  * with row strides that are multiples of 16 run on the tensor cores, others
  * on a slower kernel with the same result.  No workspace.  0 / -1. */
 int mamba_linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw,

@@ -33,6 +33,16 @@ def test_linear_refusals(change, text):
     assert text in mb.last_error()
 
 
+def test_outputs_that_are_inputs_are_refused():
+    L = mb.lib()
+    for q, scale in ((4096, 8192), (8192, 8192)):  # x itself, scale itself
+        assert L.mamba_quantize_rows(4096, 8, q, 8, scale, 4, 8, mb.F32, None) == -1
+        assert "memory of its own" in mb.last_error()
+    for y in (4096, 8192, 12288, 16384, 20480):
+        assert L.mamba_linear_i8(4096, 16, 8192, 12288, 16, 16384, 20480, y, 8, 4, 8, 16, 2, None) == -1
+        assert "one of the inputs" in mb.last_error()
+
+
 def test_empty_calls():
     assert mb.lib().mamba_quantize_rows(None, 0, None, 0, None, 0, 8, mb.F32, None) == 0
     assert mb.lib().mamba_linear_i8(None, 0, None, None, 0, None, None, None, 0, 0, 8, 8, 0, None) == 0

@@ -56,6 +56,31 @@ def test_quantize_rows(cuda, rows, cols, dtype):
     assert torch.equal(q.cpu(), torch.from_numpy(rq))
 
 
+# Numbers of rows and channels on both sides of each choice of threads a row
+# (32 to 256), with rows left over in the last block, vector and single loads.
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("rows,cols", [(1205, 512), (1184, 512), (1203, 1024), (1203, 1032), (601, 2048), (599, 2056),
+                                       (301, 4096), (299, 4104), (150, 8192), (3, 9000), (1205, 250), (601, 501),
+                                       (301, 1001), (299, 1031), (150, 2051)])
+def test_quantize_exact_halves(cuda, rows, cols, dtype):
+    """Every half is met, exactly and one place above and below, for a
+    scale that is a power of two, 3, or any number: equal whole numbers."""
+    rng = np.random.default_rng(7 * rows + cols)
+    # all but the scale's channel at halves; 3 (k + 1/2) and 127 * 3 are FP16 numbers too
+    k = (rng.integers(-126, 127, (rows, cols)) + 0.5) * np.where(np.arange(rows) % 2, 3.0, 2.0 ** -6)[:, None]
+    x = k.astype(dtype)
+    near = rng.integers(0, 3, (rows, cols))
+    x = np.where(near == 0, x, np.where(near == 1, np.nextafter(x, dtype(np.inf)), np.nextafter(x, dtype(-np.inf))))
+    top = rng.integers(0, cols, rows)
+    x[np.arange(rows), top] = (127 * np.where(np.arange(rows) % 2, 3.0, 2.0 ** -6)).astype(dtype)
+    x[::5] = (rng.standard_normal((len(x[::5]), cols))).astype(dtype)  # any scale
+    x = x.astype(dtype)
+    q, s = mb.quantize_rows(_dev(x))
+    rq, rs = rb.quantize_rows(x)
+    assert torch.equal(s.cpu(), torch.from_numpy(rs))
+    assert torch.equal(q.cpu(), torch.from_numpy(rq))
+
+
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
 def test_quantize_strides_and_padding(cuda, dtype):
     rng = np.random.default_rng(0)
