@@ -574,6 +574,10 @@ __device__ __forceinline__ float &half_of(float2 &v, int k) { return k & 1 ? v.y
 // writes h.  With enough chains to fill the GPU
 // (walks()), a CTA walks one chain from its first tile to its last instead
 // (WALK): no tickets, nothing published, the state stays in registers.
+// Bound by bytes for many warps (64 x 512 x 4096 FP16: 214 us, 5.0 TB/s), by
+// latency below: 8 x 4096 x 4096 (512 chains, 12.5 warps an SM) 246 to 252 us
+// with the special-function unit 59% and issue 48% busy; 1 x 131072 x 2048 FP32
+// 813 us (5.3 TB/s, issue 62%).
 template <typename T, int VEC, int S, int W, bool WALK>
 struct FwdSmem {
     TileIn<T, VEC, S * W, 3, 1> in;
@@ -777,7 +781,8 @@ __global__ void __launch_bounds__(32 * W, CTAS)
 // The same tiles and chains with time reversed; what runs along a chain is
 // C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.  Across
 // the wait a thread keeps sigmoid(r) and dh; the decay is computed again (one
-// exponential) rather than held.
+// exponential) rather than held.  8 x 2048 x 4096 FP16 takes 272 to 284 us (3.8
+// to 3.9 TB/s, issue 53% at 12.5 warps an SM), 8 x 1024 x 4096 FP32 193 (5.6).
 template <typename T, int VEC, int S, int W, bool WALK>
 struct BwdSmem {
     TileIn<T, VEC, S * W, 5, 2> in;
@@ -1111,7 +1116,9 @@ __global__ void __launch_bounds__(32 * kSumWarps)
 
 // ---- single token -----------------------------------------------------------------
 // A thread serves VEC channels of `rows` batch rows, so that its softplus of
-// lambda serves them all and several rows' loads are in flight.
+// lambda serves them all and several rows' loads are in flight.  Bound by bytes
+// for large batches, by latency for small ones (256 x 5120 FP16: 4.8 us in a
+// kernel trace, where the bytes would take 3.2).
 template <typename T>
 struct StepParams {
     const T *x, *r, *i;
@@ -1223,6 +1230,8 @@ struct Shape {
     static constexpr int VEC = VEC_, S = S_, W = W_, CTAS = CTAS_, tile = S_ * W_;
     static constexpr bool TMA = TMA_;
 };
+// FP16 walking, 8 x 4096 x 4096: 251 us; 8 warps a CTA 267 to 277; one channel a
+// thread 262.  Backward 8 x 2048 x 4096: 285, 8 warps 325 to 335.
 template <typename T> struct Shapes;
 template <> struct Shapes<__half> {
     using Fwd = Shape<2, 16, 4, 4>;
@@ -1259,6 +1268,9 @@ bool plan_chains(const MambaRecurrenceArgs *a, bool backward, Plan &pl) {
     c.blocks = divisor(blocks);
     c.chains = divisor(blocks * a->batch);
     c.tiles = (int)tiles;
+    // A chain's latency is its groups' hand-overs plus a group's length of maps to
+    // compose.  Groups of 4 everywhere: 1 x 524288 x 64 FP16 971 us instead of 309;
+    // short chains take the same time with any (1 x 16384 x 4096 166 to 172 us).
     c.group_shift = std::min(kMaxGroupShift, tiles <= 128 ? 2 : tiles <= 1024 ? 3 : 4);
     c.group = 1 << c.group_shift;
     c.groups = ceil_div((int)tiles, c.group);
@@ -1347,7 +1359,11 @@ int launch_tiles(Kernel kernel, const Params &p, const FwdParams &f, Plan &pl, c
 
 // Whether CTAs should walk whole chains: where the chains fill the resident
 // CTAs of `Sh` in nearly whole rounds, walking spares the hand-over of states
-// between CTAs; with fewer chains it would leave SMs empty.
+// between CTAs; with fewer chains it would leave SMs empty.  FP16, by ticket and
+// walking: 8 x 4096 x 4096 262 and 251 us, 64 x 512 x 4096 277 and 214, 4 x 4096
+// x 2048 87 and 138, 1 x 16384 x 4096 172 and 488; backward 8 x 2048 x 4096 331
+// and 282, 4 x 2048 x 2048 114 and 158.  0.6 lies where the two meet: at 0.54
+// (16 x 2048 x 2560) forward 167 and 176, backward (16 x 1024 x 2560) 220 and 204.
 template <typename Sh>
 bool walks(const Plan &pl) {
     const int64_t slots = (int64_t)Sh::CTAS * device_sm_count(), chains = pl.ch.chains.d;
@@ -1357,6 +1373,9 @@ bool walks(const Plan &pl) {
 // Tensor map of [batch, seqlen, dim] with boxes of `tokens` x `chans`; false
 // where the hardware cannot describe it (the caller then takes the kernels
 // without tensor maps).  The outer dimension with the larger stride comes last.
+// Aligned tensors with tensor copies and with each thread's own: 8 x 4096 x 4096
+// FP16 246 and 549 us, backward 8 x 2048 x 4096 272 and 412, 8 x 2048 x 4096
+// FP32 186 and 309, backward 8 x 1024 x 4096 193 and 283.
 template <typename T>
 bool encode_tile(CUtensorMap *m, const void *ptr, const int64_t *s, int B, int L, int D, int chans, int tokens,
                  unsigned bit, unsigned &row_first) {
@@ -1559,7 +1578,8 @@ int recurrence_step(const void *x, int64_t xrs, const void *r, int64_t rrs, cons
                          aligned_to(x, 4 * es) && aligned_to(r, 4 * es) && aligned_to(i, 4 * es) &&
                          aligned_to(h, 4 * es) && aligned_to(state_in, 16) && aligned_to(state_out, 16);
         const int blocks = ceil_div(dim, kThreads * (vec ? 4 : 1));
-        // several rows per thread once one row each would fill the GPU four times over
+        // several rows per thread once one row each would fill the GPU four times over:
+        // 4096 x 5120 FP16 61 us (5.5 TB/s), with one row each 76; 1024 x 5120 23 and 25
         p.rows = (int64_t)blocks * batch >= 16LL * device_sm_count() ? 4 : 1;
         p.rows = std::max(p.rows, ceil_div(batch, 65535));  // the grid's limit
         const dim3 grid((unsigned)blocks, (unsigned)ceil_div(batch, p.rows));
