@@ -612,7 +612,12 @@ __global__ void __launch_bounds__(32 * W, CTAS)
         return t;
     };
     Held<T, 3, TMA ? 1 : S> held;
+    // Tiles behind their row's end are neither fetched nor waited for: every warp
+    // has passed the barrier's last phase (and the CTA barrier behind it) before
+    // the next one is armed, however many such tiles lie between.
+    uint32_t uses = 0;
     auto fetch = [&](const Tile &t) {
+        if (!t.live) return;
         if constexpr (TMA) {
             if (tid == 0) {
                 uint64_t *bar = &sm.in.full[0];
@@ -652,7 +657,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
             s[e] = t.in && p.h0 ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
         }
     }
-    for (uint32_t it = 0;; ++it) {
+    for (;;) {
         Tile tn = t;
         bool next;
         if (WALK) {
@@ -665,13 +670,13 @@ __global__ void __launch_bounds__(32 * W, CTAS)
             next = v < total;
             if (next) tn = place(v);
         }
-        if constexpr (TMA) {
-            await_box(&sm.in.full[0], it);
-        } else {
-            copy_wait<0>();
-            put_held(sm.in.v[0], held, warp * S, t.cnt);
-        }
         if (t.live) {
+            if constexpr (TMA) {
+                await_box(&sm.in.full[0], uses++);
+            } else {
+                copy_wait<0>();
+                put_held(sm.in.v[0], held, warp * S, t.cnt);
+            }
             if (!WALK)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) csp[e] = t.in ? ch.csp[t.d + e] : 0.f;
