@@ -126,13 +126,18 @@ __device__ __forceinline__ void load_weight(const float *w, int c, float (&v)[N]
     }
 }
 
-// Sum over the CTA, the same bits in every thread.  `sm` holds two sets of
-// 32 partials used in turn, so one barrier per sum suffices: a set is
-// overwritten only after the barrier of the sum in between.
+// Sum over the CTA, the same bits in every thread, and a barrier: what a thread
+// read from shared memory before it is read when any thread returns (shuffles
+// alone do not order memory).  `sm` holds two sets of 32 partials used in turn,
+// so one barrier per sum suffices: a set is overwritten only after the barrier
+// of the sum in between.
 __device__ __forceinline__ float block_sum(float v, float *sm, int &turn) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (blockDim.x == 32) return v;
+    if (blockDim.x == 32) {
+        __syncwarp();
+        return v;
+    }
     float *s = sm + 32 * turn;
     turn ^= 1;
     if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
