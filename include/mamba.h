@@ -378,6 +378,8 @@ int mamba_ssm_step(const void *x, int64_t x_row_stride, const void *delta,
  * for an empty row).
  * resets, [batch, seqlen] bytes (NULL: none): where nonzero, h_{t-1} counts
  * as zero at that token, so several documents can share a row.
+ * seqlen <= 2^31 - 257, and batch x (tiles of the sequence and channels)
+ * < 2^31.
  * Outputs must not overlap inputs or each other (so final_state is not
  * initial_state).  The kernels run on the device that is current in the
  * calling thread. */

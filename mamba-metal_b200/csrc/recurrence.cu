@@ -1255,6 +1255,9 @@ template <> struct Shapes<float> {
     using BwdWalk = Shape<1, 8, 4, 4>;
 };
 
+// Token positions are 32-bit numbers, up to two tiles behind the sequence's end.
+constexpr int kMaxSeqlen = 0x7fffffff - 256;
+
 // The chains of a call and where its workspace holds what.
 struct Plan {
     Chains ch;
@@ -1267,6 +1270,7 @@ bool plan_chains(const MambaRecurrenceArgs *a, bool backward, Plan &pl) {
     c = Chains{};
     const int64_t blocks = ceil_div64(a->dim, cw), tiles = std::max<int64_t>(1, ceil_div64(a->seqlen, Sh::tile));
     if (blocks * a->batch > 0x7fffffffLL || blocks * a->batch * tiles > 0x7fffffffLL) return false;
+    if (a->seqlen > kMaxSeqlen) return false;
     auto divisor = [](int64_t d) {
         return Divisor{(unsigned)d, d == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / (unsigned long long)d)};
     };
@@ -1428,7 +1432,7 @@ int choose_forward(const MambaRecurrenceArgs *a, void *ws, cudaStream_t st) {
     FwdParams p = fwd_params(a);
     TileMaps maps;
     Plan pl;
-    const char *many = "gated_recurrence: too many tiles";
+    const char *many = "gated_recurrence: too many tiles or tokens";
     MB_CHECK_ARG(plan_chains<typename S::FwdWalk>(a, false, pl), many);
     if (walks<typename S::FwdWalk>(pl) && forward_maps<T, typename S::FwdWalk>(p, maps))
         return launch_forward<T, typename S::FwdWalk, true>(p, pl, maps, ws, st);
@@ -1467,7 +1471,7 @@ int choose_backward(const MambaRecurrenceArgs *a, BwdParams &p, const MambaRecur
     using S = Shapes<T>;
     TileMaps maps;
     Plan pl;
-    const char *many = "gated_recurrence_backward: too many tiles";
+    const char *many = "gated_recurrence_backward: too many tiles or tokens";
     int64_t rows = a->batch;
     MB_CHECK_ARG(plan_chains<typename S::BwdWalk>(a, true, pl), many);
     if (walks<typename S::BwdWalk>(pl) && backward_maps<T, typename S::BwdWalk>(p, maps)) {
@@ -1495,7 +1499,7 @@ int recurrence_forward(const MambaRecurrenceArgs *a, void *ws, size_t ws_bytes, 
     if (check_args(a, false)) return -1;
     if (a->batch == 0 || a->dim == 0) return 0;
     const size_t need = recurrence_workspace_bytes(a, false);
-    MB_CHECK_ARG(need, "gated_recurrence: too many tiles");
+    MB_CHECK_ARG(need, "gated_recurrence: too many tiles or tokens");
     MB_CHECK_ARG(ws && ws_bytes >= need && aligned_to(ws, 16),
                  "gated_recurrence: workspace too small or not 16-byte aligned");
     return a->dtype == MAMBA_F16 ? choose_forward<__half>(a, ws, st) : choose_forward<float>(a, ws, st);
@@ -1531,7 +1535,7 @@ int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads
                      output_rows_disjoint(g->di_stride, a->batch, a->seqlen, a->dim),
                  "gated_recurrence_backward: rows of a gradient overlap (strides)");
     const size_t need = recurrence_workspace_bytes(a, true);
-    MB_CHECK_ARG(need, "gated_recurrence_backward: too many tiles");
+    MB_CHECK_ARG(need, "gated_recurrence_backward: too many tiles or tokens");
     MB_CHECK_ARG(ws && ws_bytes >= need && aligned_to(ws, 16),
                  "gated_recurrence_backward: workspace too small or not 16-byte aligned");
     BwdParams p{};
