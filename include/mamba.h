@@ -158,12 +158,15 @@ int mamba_save_weights(MambaModel *m, void *blob, size_t size);
 
 /* Device-pointer forward: input/output are DEVICE FP32 [batch, seq_len,
  * d_model] on the model's device (may alias).  Enqueued on `stream` (NULL =
- * the model's stream); does not synchronize. */
+ * the model's stream; its own one first waits for the work given so far to
+ * the legacy default stream, one set by mamba_set_stream does not); does not
+ * synchronize. */
 int mamba_forward_device(MambaModel *m, const float *input, float *output, int batch,
                          int seq_len, void *stream);
 
 /* Device-pointer decode step: token/out DEVICE FP32 [batch, d_model].
- * Enqueued on `stream` (NULL = the model's stream); does not synchronize. */
+ * Enqueued on `stream` (NULL as for mamba_forward_device); does not
+ * synchronize. */
 int mamba_step_device(MambaModel *m, MambaStateHandle *s, const float *token, float *out,
                       void *stream);
 

@@ -269,6 +269,7 @@ struct Model {
     int64_t step_rows = 0;
     // caller-provided stream (mamba_set_stream) and tracing
     cudaStream_t user_stream = nullptr;
+    cudaEvent_t given = nullptr;  // what the default stream was given before a call
     Profiler prof;
     // decode graph (MAMBA_STEP_GRAPH=0 disables)
     StepGraph step_graph;
@@ -283,6 +284,7 @@ struct Model {
         step_graph.reset();
         if (cublas) cublasDestroy(cublas);
         for (cudaEvent_t e : io_events) cudaEventDestroy(e);
+        if (given) cudaEventDestroy(given);
         if (h2d) cudaStreamDestroy(h2d);
         if (d2h) cudaStreamDestroy(d2h);
         if (stream) cudaStreamDestroy(stream);
@@ -322,6 +324,7 @@ struct Model {
         MB_CHECK_ARG(prop.major == 10, std::string("mamba_create: device '") + prop.name +
                                            "' is not sm_100 (compute capability 10.x required)");
         MB_CUDA_TRY(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking));
+        MB_CUDA_TRY(cudaEventCreateWithFlags(&given, cudaEventDisableTiming));
         if (const char *g = std::getenv("MAMBA_STEP_GRAPH")) use_graphs = std::atoi(g) != 0;
         if (const char *t = std::getenv("MAMBA_TC_LINEAR")) tc_linear = std::atoi(t) != 0;
         if (const char *h = std::getenv("MAMBA_HOST_CHUNKS")) host_chunks = std::max(0, std::atoi(h));
@@ -538,6 +541,16 @@ struct Model {
         ar.scan_ws_bytes = ws;
         ar.lin_ws = lws ? take(lws) : nullptr;
         ar.lin_ws_bytes = lws;
+        return 0;
+    }
+
+    // A device-pointer call without a stream of the caller runs on the model's
+    // own non-blocking stream, which nothing orders behind the work that made
+    // its inputs: it waits for what the default stream was given so far.
+    int follow_default(cudaStream_t st) {
+        if (st || user_stream) return 0;
+        MB_CUDA_TRY(cudaEventRecord(given, cudaStreamLegacy));
+        MB_CUDA_TRY(cudaStreamWaitEvent(stream, given, 0));
         return 0;
     }
 
@@ -1306,6 +1319,7 @@ int mamba_forward_device(MambaModel *m, const float *input, float *output, int b
         return -1;
     }
     mb::DeviceGuard g(m->rt->dev);
+    if (m->rt->follow_default(static_cast<cudaStream_t>(stream))) return -1;
     return m->rt->forward_device(input, output, batch, seq_len, static_cast<cudaStream_t>(stream)) ? -1 : 0;
 }
 
@@ -1316,6 +1330,7 @@ int mamba_step_device(MambaModel *m, MambaStateHandle *s, const float *token, fl
         return -1;
     }
     mb::DeviceGuard g(m->rt->dev);
+    if (m->rt->follow_default(static_cast<cudaStream_t>(stream))) return -1;
     return mb::step_device(*m->rt, *s, token, out, static_cast<cudaStream_t>(stream)) ? -1 : 0;
 }
 

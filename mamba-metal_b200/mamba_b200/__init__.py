@@ -350,6 +350,8 @@ class Model:
         _check(lib().mamba_forward(self._h, in_ptr, out_ptr, batch, L), "mamba_forward")
 
     def forward_device(self, in_ptr, out_ptr, batch, L, stream=0):
+        """Device FP32 [batch, L, d_model] pointers (mamba_forward_device) on a
+        stream handle; 0: the model's stream, behind the default stream's work so far."""
         _check(lib().mamba_forward_device(self._h, in_ptr, out_ptr, batch, L, stream),
                "mamba_forward_device")
 
@@ -408,6 +410,7 @@ class State:
         return out
 
     def step_device(self, in_ptr, out_ptr, stream=0):
+        """Device FP32 [batch, d_model] pointers (mamba_step_device); stream as in Model.forward_device."""
         _check(lib().mamba_step_device(self.model.handle, self._h, in_ptr, out_ptr, stream),
                "mamba_step_device")
 
