@@ -34,7 +34,9 @@ namespace {
 // five forward and six backward.  Approximate exponentials, reciprocals and
 // roots have relative errors of 2^-22 or less.  PRECISE (FP32 tensors) adds
 // what their rounding needs: the exponent's product with log2(e) in two parts
-// and a longer series; for FP16 tensors the rounding to 2^-11 hides both.
+// and a longer series.  For FP16 tensors the rounding to 2^-11 hides both: in
+// the gates, which count once, while the decay counts for as long as the FP32
+// state lives and is right to its last place for all (decay_of).
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN operand stays one
     float r;
@@ -74,20 +76,23 @@ __device__ __forceinline__ float2 clamp_gate(float2 v) {
     return v;
 }
 
-// a = exp(-y) and m = 1 - a^2, m without cancellation for y near 0.
-// PRECISE: below y = 1/2, d = 1 - a by its Taylor series to y^9 (relative
-// error < (1/2)^9 / 10! = 6e-10), a = 1 - d (rounded once, where the approximate
-// exponential would be off by up to four times that, which adds up over a
-// thousand tokens), m = d (2 - d).  Above, d = 1 - exp(-y): 2^-22 a / (1 - a) < 4e-7.
-// Else: a by the exponential; m by its Taylor series in z = 2y to z^5, which is
-// z^6/720 too large, and as (1 - a)(1 + a) with 2.4e-7 added to the first factor,
-// which makes it too large also where a's rounding works against it: the smaller
-// of the two is right to 4e-6 everywhere (worst where they meet, near z = 0.29),
-// and to z^5/720 below, without comparing and selecting.
+// a = exp(-y) and m = 1 - a^2, m without cancellation for y near 0 and a
+// rounded once there: an approximate exponential is off by up to 2^-23 and on
+// average by a quarter of 2^-24, which adds up over the tokens that an FP32
+// state lives.  So near 0 both come from d = 1 - a by its Taylor series, a = 1 -
+// d and m = d (2 - d).
+// PRECISE: below y = 1/2 the series to y^9 (relative error < (1/2)^9 / 10! =
+// 6e-10); above, d = 1 - exp(-y): 2^-22 a / (1 - a) < 4e-7.
+// Else: a series to y^5 and an exponential made 5 * 2^-24 too small, which is
+// more than it is ever off: both bound a from below, so the larger one is
+// right everywhere, without comparing and selecting.  Worst where they meet,
+// near y = 0.25: 6e-7 of a, 3e-6 of m.  With the plain exponential instead, up to 1.4 *
+// 2^-24 off near 1, 8 x 4096 x 4096 took 248 us, with the series 255; backward
+// 8 x 2048 x 4096 271 and 292.
 template <bool PRECISE>
 __device__ __forceinline__ void decay_of(float2 y, float2 &a, float2 &m) {
-    const float2 e = exp_neg<PRECISE>(y);
     if (PRECISE) {
+        const float2 e = exp_neg<PRECISE>(y);
         float2 q = __ffma2_rn(y, both(1.f / 362880), both(-1.f / 40320));
         q = __ffma2_rn(y, q, both(1.f / 5040));
         q = __ffma2_rn(y, q, both(-1.f / 720));
@@ -102,15 +107,16 @@ __device__ __forceinline__ void decay_of(float2 y, float2 &a, float2 &m) {
         a = make_float2(y.x < 0.5f ? r.x : e.x, y.y < 0.5f ? r.y : e.y);
         m = __fmul2_rn(d, __ffma2_rn(d, both(-1.f), both(2.f)));
     } else {
-        const float2 z = __fadd2_rn(y, y);
-        float2 q = __ffma2_rn(z, both(1.f / 120), both(-1.f / 24));
-        q = __ffma2_rn(z, q, both(1.f / 6));
-        q = __ffma2_rn(z, q, both(-0.5f));
-        q = __ffma2_rn(z, q, both(1.f));
-        q = __fmul2_rn(z, q);
-        const float2 d = __ffma2_rn(e, both(-1.f), both(1.f + 2.4e-7f)), w = __ffma2_rn(e, d, d);
-        a = e;
-        m = make_float2(fminf(q.x, w.x), fminf(q.y, w.y));
+        const float2 t = __ffma2_rn(y, both(-kLog2e), both(-5 * kLog2e / 16777216));
+        const float2 e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+        float2 q = __ffma2_rn(y, both(-1.f / 120), both(1.f / 24));
+        q = __ffma2_rn(y, q, both(-1.f / 6));
+        q = __ffma2_rn(y, q, both(0.5f));
+        q = __ffma2_rn(y, q, both(-1.f));
+        const float2 r = __ffma2_rn(y, q, both(1.f)), s = __fmul2_rn(y, q), l = __fadd2_rn(e, both(-1.f));
+        a = make_float2(fmaxf(r.x, e.x), fmaxf(r.y, e.y));
+        const float2 d = make_float2(fmaxf(s.x, l.x), fmaxf(s.y, l.y));  // a - 1
+        m = __fmul2_rn(d, __ffma2_rn(d, both(-1.f), both(-2.f)));
     }
 }
 

@@ -52,3 +52,102 @@ def test_mostly_empty_rows(cuda, B, L, D, dtype):
     fmag = np.where(lengths[keep, None] > 0, mag[np.arange(len(keep)), last], np.abs(h0[keep]))
     err = np.abs(first[1].double().cpu().numpy()[keep] - fin) - (d * fmag + 2.0 ** -25)
     assert err.max() <= 0
+
+
+def _last(mag, lengths=None):
+    return mag[:, -1] if lengths is None else mag[np.arange(len(lengths)), lengths - 1]
+
+
+def _check(got, ref, mag, u, d, tiny, name):
+    """|got - ref| <= u |ref| + d mag + tiny, every quantity of the element itself."""
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all(), name
+    err = np.abs(got - ref)
+    bad = err - (u * np.abs(ref) + d * mag + tiny)
+    assert bad.max() <= 0, (name, float(bad.max()), float((err / np.maximum(mag, 1e-300)).max()))
+
+
+def _slow(seed, B, L, D, dtype):
+    """Gates whose decays at r = 0 lie between 1 - 1e-2 and 1 - 1e-5."""
+    rng = np.random.default_rng(seed)
+    np_t = np.float16 if dtype == torch.float16 else np.float32
+    v = {k: rng.standard_normal((B, L, D)).astype(np_t) for k in ("x", "r", "i", "dh")}
+    y = 10.0 ** rng.uniform(-5, -2, D)
+    v["lam"] = np.log(np.expm1(2 * y / C)).astype(np.float32)
+    v["h0"], v["dfinal"] = (rng.standard_normal((B, D)).astype(np.float32) for _ in range(2))
+    return v
+
+
+def _slow_bound(dtype, L):
+    """Errors of an FP32 state that lives for up to L tokens, relative to its
+    terms.  Each token's gates: 16 roundings of 2^-24 (FP16 tensors: 1e-5 for
+    the short series and the approximate exponentials), of which those in the
+    decay's logarithm count once over the life of the state.  Along the
+    sequence: three roundings a token (the decay, the product of decays, the
+    sum), each at most 2^-24 of the state and as often up as down, since the
+    gates differ from token to token.  By Hoeffding's inequality their sum
+    exceeds 2^-24 sqrt(3 L) sqrt(2 ln(2 / p)) with probability p: 6.3 for the last factor is
+    p = 5e-9 an element."""
+    walk = 6.3 * 2.0 ** -24 * (3 * L) ** 0.5
+    return walk + (1e-5 if dtype == torch.float16 else 2.0 ** -24 * 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("B,L,D", [(1, 32768, 64), (1, 20000, 33), (64, 4096, 640)])
+def test_states_that_live_long(cuda, B, L, D, dtype):
+    """Decays up to 1 - 1e-5: what the approximation of the decay is off by adds
+    up over the state's life, in the FP32 states and in every gradient."""
+    rows = 1 if B > 1 else B  # the oracle follows one row of a batch
+    v = _slow(L, rows, L, D, dtype)
+    t = {k: torch.from_numpy(a).cuda() for k, a in v.items()}
+    t = {k: a if k == "lam" else a.repeat((B // rows,) + (1,) * (a.dim() - 1)) for k, a in t.items()}
+    h, hN = mb.gated_recurrence(t["x"], t["r"], t["i"], t["lam"], c=C, initial_state=t["h0"], return_final_state=True)
+    grads = mb.gated_recurrence_backward(t["dh"], t["x"], t["r"], t["i"], t["lam"], h, c=C, initial_state=t["h0"],
+                                         dfinal_state=t["dfinal"])
+    ref, fin, mag = rb.gated_recurrence(v["x"], v["r"], v["i"], v["lam"], C, v["h0"])
+    d, u = _slow_bound(dtype, L), 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -24
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    _check(hN[-rows:], fin, _last(mag), 0, d, 0, "final state")
+    _check(h[-rows:], ref, mag, u, d, tiny, "h")
+    g, gm = rb.gated_recurrence_backward(v["dh"], v["x"], v["r"], v["i"], v["lam"], h[-rows:].cpu().numpy(), C, v["h0"],
+                                         dfinal=v["dfinal"])
+    for got, k in zip(grads, ("dx", "dr", "di")):
+        # an error of the state's gradient and of the token's own gates
+        _check(got[-rows:], g[k], gm[k], u, d + (1e-5 if dtype == torch.float16 else 2.0 ** -24 * 16), tiny, k)
+    _check(grads[4][-rows:], g["dh0"], gm["dh0"], 0, d, 0, "dh0")
+    # sums over the tokens: at most L / 32 (a warp's share) + 64 additions after one another
+    _check(grads[3], B * g["dlam"], B * gm["dlam"], 0, 2 * d + 2.0 ** -24 * (L / 32 + 64 + B), 0, "dlam")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_many_single_tokens(cuda, dtype):
+    """Decoding: the FP32 state carried through 6000 calls."""
+    B, L, D = 2, 6000, 64
+    v = _slow(7, B, L, D, dtype)
+    t = {k: torch.from_numpy(a).cuda() for k, a in v.items()}
+    s = t["h0"].clone()
+    for k in range(L):
+        h, _ = mb.gated_recurrence_step(t["x"][:, k], t["r"][:, k], t["i"][:, k], t["lam"], s, c=C, state_out=s)
+    ref, fin, mag = rb.gated_recurrence(v["x"], v["r"], v["i"], v["lam"], C, v["h0"])
+    d, u = _slow_bound(dtype, L), 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -24
+    _check(s, fin, _last(mag), 0, d, 0, "state")
+    _check(h, ref[:, -1], mag[:, -1], u, d, 2.0 ** -25 if dtype == torch.float16 else 0.0, "h")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_the_decay_of_one_token(cuda, dtype):
+    """A state of 1 and no input leave the decay itself, for y = -ln a from 1e-6
+    to 10.  It is 1 - d with d by a series, rounded once (2^-25 below 1), while y is small:
+    y and d are off by eight roundings of 2^-24 and by 2^-21 for the gate's exponential and
+    reciprocal.  From y = 1/5 on the decay is the approximate exponential
+    itself or close to it: 2^-20."""
+    D = 1 << 18
+    y = 10.0 ** np.random.default_rng(1).uniform(-6, 1, D)
+    lam = np.log(np.expm1(2 * y / C)).astype(np.float32)
+    y = C * rb.softplus(lam.astype(np.float64)) / 2
+    z = torch.zeros((1, D), dtype=dtype, device="cuda")
+    one = torch.ones((1, D), device="cuda")
+    _, s = mb.gated_recurrence_step(z, z, z, torch.from_numpy(lam).cuda(), one, c=C)
+    bound = 2.0 ** -25 + y * (2.0 ** -21 + 8 * 2.0 ** -24) + np.where(y < 0.2, 0.0, 2.0 ** -20)
+    over = np.abs(s[0].double().cpu().numpy() - np.exp(-y)) - bound
+    assert over.max() <= 0, (float(over.max()), float(y[over.argmax()]))
