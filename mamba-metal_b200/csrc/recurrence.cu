@@ -67,13 +67,23 @@ __device__ __forceinline__ float2 exp_neg(float2 v) {
     return e;
 }
 
-// A gate's preactivation, held where exp(-v) and its products stay finite:
-// sigmoid(-80) = 2e-35 and sigmoid(150) = 1 stand for what lies beyond.
+// The decay gate's preactivation, held where exp(-v) is finite: sigmoid(-80) =
+// 2e-35 and sigmoid(150) = 1 stand for what lies beyond.
 template <bool PRECISE, bool BELOW = true>
 __device__ __forceinline__ float2 clamp_gate(float2 v) {
     if (BELOW) v = make_float2(max_nan(v.x, -80.f), max_nan(v.y, -80.f));
     if (PRECISE) v = make_float2(min_nan(v.x, 150.f), min_nan(v.y, 150.f));
     return v;
+}
+
+// E = exp(v) of the input gate, sigmoid(v) = E / (1 + E), 1 - sigmoid(v) = 1 / (1 +
+// E): right down to the smallest normal E, v held from above only (at `top`,
+// where E and its products stay finite).
+template <bool PRECISE>
+__device__ __forceinline__ float2 exp_gate(float2 v, float top) {
+    v = make_float2(max_nan(-v.x, -top), max_nan(-v.y, -top));
+    if (PRECISE) v = make_float2(min_nan(v.x, 150.f), min_nan(v.y, 150.f));
+    return exp_neg<PRECISE>(v);
 }
 
 // a = exp(-y) and m = 1 - a^2, m without cancellation for y near 0 and a
@@ -133,15 +143,18 @@ __device__ __forceinline__ void decay(float2 r, float2 csp, float2 &e, float2 &s
     decay_of<PRECISE>(__fmul2_rn(csp, s), a, m);
 }
 
-// Forward: a and b = sqrt(1 - a^2) sigmoid(i) x.  With q = 1 + exp(-i) and
-// m = 1 - a^2, sqrt(m) / q = m / sqrt(m q^2): one root for both.
+// Forward: a and b = sqrt(1 - a^2) sigmoid(i) x.  With E = exp(i), q = 1 + E and
+// m = 1 - a^2, sqrt(m) / q = m / sqrt(m q^2): one root for both.  sigmoid(20) is 1
+// to 2e-9, a fraction of a step of FP32, and q^2 finite.
 template <bool PRECISE>
 __device__ __forceinline__ void forward_gates(float2 r, float2 i, float2 x, float2 csp, float2 &a, float2 &b) {
     float2 e, s, m;
     decay<PRECISE>(r, csp, e, s, a, m);
-    const float2 q = __fadd2_rn(exp_neg<PRECISE>(clamp_gate<PRECISE>(i)), both(1.f));
+    const float2 E = exp_gate<PRECISE>(i, 20.f), q = __fadd2_rn(E, both(1.f));
     const float2 t = __ffma2_rn(__fmul2_rn(m, q), q, both(kTiny));
-    b = __fmul2_rn(__fmul2_rn(m, make_float2(rsqrt_approx(t.x), rsqrt_approx(t.y))), x);
+    const float2 w = __fmul2_rn(m, make_float2(rsqrt_approx(t.x), rsqrt_approx(t.y)));
+    // FP16: E x is finite.  FP32: w x is at most x.
+    b = PRECISE ? __fmul2_rn(__fmul2_rn(w, x), E) : __fmul2_rn(w, __fmul2_rn(E, x));
 }
 
 // softplus(lambda), and c times it (finite: 0 times it has to be 0), once per
@@ -1044,14 +1057,15 @@ __global__ void __launch_bounds__(32 * W, CTAS)
                         prev.x = f.h0[(int64_t)t.b * f.D + t.d + (2 * z) % VEC];
                         if (VEC > 1) prev.y = f.h0[(int64_t)t.b * f.D + t.d + (2 * z + 1) % VEC];
                     }
-                    const float2 ei = exp_neg<PRECISE>(clamp_gate<PRECISE>(pair_of<T, VEC, TP>(gi, z)));
+                    const float2 ei = exp_gate<PRECISE>(pair_of<T, VEC, TP>(gi, z), 80.f);
                     const float2 qi1 = __fadd2_rn(ei, both(1.f));
-                    const float2 si = make_float2(rcp_approx(qi1.x), rcp_approx(qi1.y));
+                    const float2 om1 = make_float2(rcp_approx(qi1.x), rcp_approx(qi1.y));  // 1 - sigmoid(i)
+                    const float2 si = __fmul2_rn(ei, om1);
                     const float2 m2 = m[z], m1 = __fadd2_rn(m2, both(kTiny));
                     const float2 w = make_float2(rsqrt_approx(m1.x), rsqrt_approx(m1.y));
                     const float2 gs2 = __fmul2_rn(G[z], si);               // G sigmoid(i)
                     const float2 gx = __fmul2_rn(gs2, __fmul2_rn(m2, w));  // * sqrt(m)
-                    const float2 gi2 = __fmul2_rn(__fmul2_rn(gx, xv), __fmul2_rn(ei, si));
+                    const float2 gi2 = __fmul2_rn(__fmul2_rn(gx, xv), om1);
                     // E = a (G si x a (y / sqrt(m)) - y G h_{t-1}); y / sqrt(m) first, it tends to 0
                     const float2 u1 = __fmul2_rn(__fmul2_rn(gs2, xv), __fmul2_rn(av, __fmul2_rn(y[z], w)));
                     const float2 u2 = __ffma2_rn(__fmul2_rn(__fmul2_rn(y[z], both(-1.f)), G[z]), prev, u1);

@@ -151,3 +151,29 @@ def test_the_decay_of_one_token(cuda, dtype):
     bound = 2.0 ** -25 + y * (2.0 ** -21 + 8 * 2.0 ** -24) + np.where(y < 0.2, 0.0, 2.0 ** -20)
     over = np.abs(s[0].double().cpu().numpy() - np.exp(-y)) - bound
     assert over.max() <= 0, (float(over.max()), float(y[over.argmax()]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("B,L,D", [(2, 130, 64), (40, 70, 640), (1, 300, 33)])
+def test_nearly_closed_input_gates(cuda, B, L, D, dtype):
+    """sigmoid(i) = exp(i) between 3e-20 and 1e-34: small, and not 0.  FP32
+    results element by element; of FP16 tensors the FP32 state."""
+    rng = np.random.default_rng(L)
+    np_t = np.float16 if dtype == torch.float16 else np.float32
+    x, r, dh = (rng.standard_normal((B, L, D)).astype(np_t) for _ in range(3))
+    i = rng.uniform(-78, -45, (B, L, D)).astype(np_t)
+    lam = rng.uniform(-5, -2, D).astype(np.float32)
+    tx, tr, ti, tl, tg = _dev(x, r, i, lam, dh)
+    h, hN = mb.gated_recurrence(tx, tr, ti, tl, c=C, return_final_state=True)
+    ref, fin, mag = rb.gated_recurrence(x, r, i, lam, C)
+    # the exponent's product with log2(e), up to 113, is rounded once (FP16 tensors): 113 * 2^-24 * 1.5 < 1.1e-5
+    d = 2.1e-5 if dtype == torch.float16 else 2.0 ** -24 * (16 + min(L, 2000))
+    _check(hN, fin, _last(mag), 0, d, 0, "final state")
+    s, _ = mb.gated_recurrence_step(tx[:, 0], tr[:, 0], ti[:, 0], tl, torch.zeros((B, D), device="cuda"), c=C)[::-1]
+    _check(s, ref[:, 0], mag[:, 0], 0, d, 0, "step")
+    if dtype == torch.float32:
+        _check(h, ref, mag, 2.0 ** -24, d, 0, "h")
+        grads = mb.gated_recurrence_backward(tg, tx, tr, ti, tl, h, c=C)
+        g, gm = rb.gated_recurrence_backward(dh, x, r, i, lam, h.cpu().numpy(), C)
+        for got, k in zip(grads, ("dx", "dr", "di")):
+            _check(got, g[k], gm[k], 2.0 ** -24, d, 0, k)
