@@ -1141,9 +1141,12 @@ __global__ void __launch_bounds__(32 * kSumWarps)
 
 // ---- single token -----------------------------------------------------------------
 // A thread serves VEC channels of `rows` batch rows, so that its softplus of
-// lambda serves them all and several rows' loads are in flight.  Bound by bytes
-// for large batches, by latency for small ones (256 x 5120 FP16: 4.8 us in a
-// kernel trace, where the bytes would take 3.2).
+// lambda serves them all, and loads two rows before it stores either (a store
+// may be to the loaded state, so the compiler keeps their order).  Bound by
+// bytes for large batches, by latency for small ones: 4096 x 5120 FP16 takes 58
+// us (5.8 TB/s), with one row loaded at a time 68, with four 59; 256 x 5120 12.3,
+// 13.3 and 12.3; 4096 x 5120 FP32 82 us each way.
+constexpr int kStepAhead = 2;
 template <typename T>
 struct StepParams {
     const T *x, *r, *i;
@@ -1163,27 +1166,37 @@ __global__ void __launch_bounds__(kThreads) recurrence_step_kernel(const StepPar
 #pragma unroll
     for (int e = 0; e < VEC; ++e) csp[e] = channel_decay(p.c, p.lambda[d + e]);
     const int64_t b0 = (int64_t)blockIdx.y * p.rows, b1 = min(b0 + p.rows, (int64_t)p.B);
-#pragma unroll 4
-    for (int64_t b = b0; b < b1; ++b) {
-        const Pack<T, VEC> x[1] = {load_pack<T, VEC>(p.x + b * p.xrs + d)}, r[1] = {load_pack<T, VEC>(p.r + b * p.rrs + d)},
-                           gi[1] = {load_pack<T, VEC>(p.i + b * p.irs + d)};
-        Pack<float, VEC> s = load_pack<float, VEC>(p.s_in + b * p.D + d);
-        Pack<T, VEC> o;
+    for (int64_t b = b0; b < b1; b += kStepAhead) {
+        Pack<T, VEC> x[kStepAhead], r[kStepAhead], gi[kStepAhead];
+        Pack<float, VEC> s[kStepAhead];
 #pragma unroll
-        for (int e = 0; e < VEC; e += 2) {
-            const int f = VEC == 1 ? 0 : e + 1;
-            float2 a, bt;
-            forward_gates<PRECISE>(make_float2(cvt_f32(r[0].v[e]), cvt_f32(r[0].v[f])),
-                                   make_float2(cvt_f32(gi[0].v[e]), cvt_f32(gi[0].v[f])),
-                                   make_float2(cvt_f32(x[0].v[e]), cvt_f32(x[0].v[f])), make_float2(csp[e], csp[f]), a,
-                                   bt);
-            s.v[e] = fmaf(a.x, s.v[e], bt.x);
-            if (VEC > 1) s.v[f] = fmaf(a.y, s.v[f], bt.y);
+        for (int k = 0; k < kStepAhead; ++k)
+            if (b + k < b1) {
+                x[k] = load_pack<T, VEC>(p.x + (b + k) * p.xrs + d);
+                r[k] = load_pack<T, VEC>(p.r + (b + k) * p.rrs + d);
+                gi[k] = load_pack<T, VEC>(p.i + (b + k) * p.irs + d);
+                s[k] = load_pack<float, VEC>(p.s_in + (b + k) * p.D + d);
+            }
+#pragma unroll
+        for (int k = 0; k < kStepAhead; ++k) {
+            if (b + k >= b1) break;
+            Pack<T, VEC> o;
+#pragma unroll
+            for (int e = 0; e < VEC; e += 2) {
+                const int f = VEC == 1 ? 0 : e + 1;
+                float2 a, bt;
+                forward_gates<PRECISE>(make_float2(cvt_f32(r[k].v[e]), cvt_f32(r[k].v[f])),
+                                       make_float2(cvt_f32(gi[k].v[e]), cvt_f32(gi[k].v[f])),
+                                       make_float2(cvt_f32(x[k].v[e]), cvt_f32(x[k].v[f])),
+                                       make_float2(csp[e], csp[f]), a, bt);
+                s[k].v[e] = fmaf(a.x, s[k].v[e], bt.x);
+                if (VEC > 1) s[k].v[f] = fmaf(a.y, s[k].v[f], bt.y);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o.v[e] = cvt_out<T>(s[k].v[e]);
+            *reinterpret_cast<Pack<float, VEC> *>(p.s_out + (b + k) * p.D + d) = s[k];
+            *reinterpret_cast<Pack<T, VEC> *>(p.h + (b + k) * p.hrs + d) = o;
         }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) o.v[e] = cvt_out<T>(s.v[e]);
-        *reinterpret_cast<Pack<float, VEC> *>(p.s_out + b * p.D + d) = s;
-        *reinterpret_cast<Pack<T, VEC> *>(p.h + b * p.hrs + d) = o;
     }
 }
 
@@ -1608,7 +1621,7 @@ int recurrence_step(const void *x, int64_t xrs, const void *r, int64_t rrs, cons
                          aligned_to(h, 4 * es) && aligned_to(state_in, 16) && aligned_to(state_out, 16);
         const int blocks = ceil_div(dim, kThreads * (vec ? 4 : 1));
         // several rows per thread once one row each would fill the GPU four times over:
-        // 4096 x 5120 FP16 61 us (5.5 TB/s), with one row each 76; 1024 x 5120 23 and 25
+        // 4096 x 5120 FP16 58 us, with one row each 80; 1024 x 5120 22 and 27; FP32 82 and 95
         p.rows = (int64_t)blocks * batch >= 16LL * device_sm_count() ? 4 : 1;
         p.rows = std::max(p.rows, ceil_div(batch, 65535));  // the grid's limit
         const dim3 grid((unsigned)blocks, (unsigned)ceil_div(batch, p.rows));

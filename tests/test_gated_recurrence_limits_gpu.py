@@ -177,3 +177,24 @@ def test_nearly_closed_input_gates(cuda, B, L, D, dtype):
         g, gm = rb.gated_recurrence_backward(dh, x, r, i, lam, h.cpu().numpy(), C)
         for got, k in zip(grads, ("dx", "dr", "di")):
             _check(got, g[k], gm[k], 2.0 ** -24, d, 0, k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("B,D", [(2371, 8), (2370, 7), (4099, 520), (65537, 4), (131071, 3), (327680, 1)])
+def test_steps_of_many_rows(cuda, B, D, dtype):
+    """Several rows a thread, loaded ahead of the stores: odd counts of rows, more
+    rows than a grid holds, and the state updated in place."""
+    rng = np.random.default_rng(B)
+    np_t = np.float16 if dtype == torch.float16 else np.float32
+    x, r, i = (rng.standard_normal((B, D)).astype(np_t) for _ in range(3))
+    lam = rng.uniform(-6, -2, D).astype(np.float32)
+    h0 = rng.standard_normal((B, D)).astype(np.float32)
+    tx, tr, ti, tl, s = _dev(x, r, i, lam, h0)
+    h, out = mb.gated_recurrence_step(tx, tr, ti, tl, s, c=C)
+    h2, _ = mb.gated_recurrence_step(tx, tr, ti, tl, s, c=C, state_out=s)
+    assert torch.equal(h, h2) and torch.equal(out, s)
+    ref, fin, mag = rb.gated_recurrence(x[:, None], r[:, None], i[:, None], lam, C, h0)
+    d = 2.0 ** -24 * 17 + (1e-5 if dtype == torch.float16 else 0.0)
+    _check(s, fin, mag[:, 0], 0, d, 0, "state")
+    u, tiny = (2.0 ** -11, 2.0 ** -25) if dtype == torch.float16 else (2.0 ** -24, 0.0)
+    _check(h, ref[:, 0], mag[:, 0], u, d, tiny, "h")
