@@ -133,13 +133,18 @@ __device__ __forceinline__ void decay_of(float2 y, float2 &a, float2 &m) {
 // 1 / sqrt(m + 1e-37): finite for m = 0, where m times it is 0 as it should be.
 constexpr float kTiny = 1e-37f;
 
-// sigmoid(r) and the decay y = csp sigmoid(r), a = exp(-y), m = 1 - a^2.
-template <bool PRECISE>
-__device__ __forceinline__ void decay(float2 r, float2 csp, float2 &e, float2 &s, float2 &a, float2 &m) {
-    // without PRECISE, exp(-r) = infinity just gives s = 0
-    e = exp_neg<PRECISE>(clamp_gate<PRECISE, PRECISE>(r));
+// 1 / (1 + e): sigmoid(v) for e = exp(-v).
+__device__ __forceinline__ float2 sigmoid_of(float2 e) {
     const float2 q = __fadd2_rn(e, both(1.f));
-    s = make_float2(rcp_approx(q.x), rcp_approx(q.y));
+    return make_float2(rcp_approx(q.x), rcp_approx(q.y));
+}
+
+// e = exp(-r), s = sigmoid(r) and the decay y = csp s, a = exp(-y), m = 1 - a^2.
+// FINITE: so is e, and 1 - s = e s; else infinity just gives s = 0.
+template <bool PRECISE, bool FINITE = PRECISE>
+__device__ __forceinline__ void decay(float2 r, float2 csp, float2 &e, float2 &s, float2 &a, float2 &m) {
+    e = exp_neg<PRECISE>(clamp_gate<PRECISE, FINITE>(r));
+    s = sigmoid_of(e);
     decay_of<PRECISE>(__fmul2_rn(csp, s), a, m);
 }
 
@@ -804,9 +809,10 @@ __global__ void __launch_bounds__(32 * W, CTAS)
 // ---- backward -------------------------------------------------------------------
 // The same tiles and chains with time reversed; what runs along a chain is
 // C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.  Across
-// the wait a thread keeps sigmoid(r) and dh; the decay is computed again (one
-// exponential) rather than held.  8 x 2048 x 4096 FP16 takes 272 to 284 us (3.8
-// to 3.9 TB/s, issue 53% at 12.5 warps an SM), 8 x 1024 x 4096 FP32 193 (5.6).
+// the wait a thread keeps dh and sigmoid(r), or exp(-r); the decay is computed
+// again (one exponential) rather than held.  8 x 2048 x 4096 FP16 takes 302 us
+// (3.6 TB/s), with 1 - sigmoid(r) as a difference, without its reciprocal, 292;
+// 8 x 1024 x 4096 FP32 193 (5.6).
 template <typename T, int VEC, int S, int W, bool WALK>
 struct BwdSmem {
     TileIn<T, VEC, S * W, 5, 2> in;
@@ -917,6 +923,9 @@ __global__ void __launch_bounds__(32 * W, CTAS)
         // WALK: one row of sums per chain, else one per tile
         float *part = p.part + (WALK ? (int64_t)t.b : (int64_t)t.b * ch.tiles + t.k) * f.D + t.d;
         if (t.live) {
+            // sigmoid(r) and 1 - sigmoid(r), or (FP16 tensors: fewer registers, one more
+            // reciprocal later) the exp(-r) that gives both.  The difference of 1 and an
+            // approximate sigmoid would lose dr of open gates: 1% at r = 12.
             float2 sg[NP], om[PRECISE ? NP : 1];
             if (!WALK)
 #pragma unroll
@@ -942,8 +951,11 @@ __global__ void __launch_bounds__(32 * W, CTAS)
                 for (int z = 0; z < TP * VEC / 2; ++z) {
                     const int q = j0 * VEC / 2 + z;
                     float2 e, m;
-                    decay<PRECISE>(pair_of<T, VEC, TP>(r, z), channel_pair<VEC>(csp, z), e, sg[q], a[z], m);
-                    if (PRECISE) om[q] = __fmul2_rn(e, sg[q]);
+                    decay<PRECISE, true>(pair_of<T, VEC, TP>(r, z), channel_pair<VEC>(csp, z), e, sg[q], a[z], m);
+                    if (PRECISE)
+                        om[q] = __fmul2_rn(e, sg[q]);
+                    else
+                        sg[q] = e;
                 }
 #pragma unroll
                 for (int u = TP - 1; u >= 0; --u)
@@ -1014,9 +1026,13 @@ __global__ void __launch_bounds__(32 * W, CTAS)
                 if (j0 >= t.cnt) continue;
                 Pack<T, VEC> x[TP], gi[TP], hp[TP], ox[TP], orr[TP], oi[TP];
                 float2 a[TP * VEC / 2], m[TP * VEC / 2], y[TP * VEC / 2], G[TP * VEC / 2];  // G = dh + C
+                float2 os[TP * VEC / 2];                                                    // 1 - sigmoid(r)
 #pragma unroll
                 for (int z = 0; z < TP * VEC / 2; ++z) {
-                    y[z] = __fmul2_rn(channel_pair<VEC>(csp, z), sg[j0 * VEC / 2 + z]);
+                    const int q = j0 * VEC / 2 + z;
+                    const float2 s = PRECISE ? sg[q] : sigmoid_of(sg[q]);
+                    os[z] = PRECISE ? om[PRECISE ? q : 0] : __fmul2_rn(sg[q], s);
+                    y[z] = __fmul2_rn(channel_pair<VEC>(csp, z), s);
                     decay_of<PRECISE>(y[z], a[z], m[z]);
                 }
                 if constexpr (VEC == 1) {
@@ -1070,9 +1086,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
                     const float2 u1 = __fmul2_rn(__fmul2_rn(gs2, xv), __fmul2_rn(av, __fmul2_rn(y[z], w)));
                     const float2 u2 = __ffma2_rn(__fmul2_rn(__fmul2_rn(y[z], both(-1.f)), G[z]), prev, u1);
                     const float2 E = __fmul2_rn(av, u2);
-                    const int q = j0 * VEC / 2 + z;
-                    const float2 os = PRECISE ? om[PRECISE ? q : 0] : __ffma2_rn(sg[q], both(-1.f), both(1.f));
-                    const float2 gr = __fmul2_rn(E, os);
+                    const float2 gr = __fmul2_rn(E, os[z]);
 #pragma unroll
                     for (int hlf = 0; hlf < 2; ++hlf) {
                         const int k = 2 * z + hlf, u = k / VEC, e = k % VEC;

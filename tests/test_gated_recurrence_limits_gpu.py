@@ -198,3 +198,24 @@ def test_steps_of_many_rows(cuda, B, D, dtype):
     _check(s, fin, mag[:, 0], 0, d, 0, "state")
     u, tiny = (2.0 ** -11, 2.0 ** -25) if dtype == torch.float16 else (2.0 ** -24, 0.0)
     _check(h, ref[:, 0], mag[:, 0], u, d, tiny, "h")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("B,L,D", [(2, 130, 64), (40, 70, 640), (1, 300, 33)])
+def test_gradients_of_nearly_open_gates(cuda, B, L, D, dtype):
+    """1 - sigmoid(r) = exp(-r) for r of 8 to 17, under a loss scale of 20000:
+    dr are ordinary numbers that a difference of 1 and the sigmoid would lose."""
+    rng = np.random.default_rng(L + 1)
+    np_t = np.float16 if dtype == torch.float16 else np.float32
+    x, i = (rng.standard_normal((B, L, D)).astype(np_t) for _ in range(2))
+    r = rng.uniform(8, 17, (B, L, D)).astype(np_t)
+    dh = (20000 * rng.uniform(-1, 1, (B, L, D))).astype(np_t)
+    lam = rng.uniform(-3, 0, D).astype(np.float32)  # y of 0.4 to 5.5
+    tx, tr, ti, tl, tg = _dev(x, r, i, lam, dh)
+    h = mb.gated_recurrence(tx, tr, ti, tl, c=C)
+    dr = mb.gated_recurrence_backward(tg, tx, tr, ti, tl, h, c=C)[1]
+    g, gm = rb.gated_recurrence_backward(dh, x, r, i, lam, h.cpu().numpy(), C)
+    # ~16 roundings in the gates, a state's gradient that lives for a few tokens; FP16 tensors 1e-5
+    # each for the decay and for the gates' approximate exponentials
+    d, u, tiny = (2.1e-5, 2.0 ** -11, 2.0 ** -25) if dtype == torch.float16 else (2.0 ** -24 * 64, 2.0 ** -24, 0.0)
+    _check(dr, g["dr"], gm["dr"], u, d, tiny, "dr")
