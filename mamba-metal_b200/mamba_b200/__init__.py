@@ -706,6 +706,20 @@ def _ptr0(t):
     return 0 if t is None else t.data_ptr()
 
 
+def _packed(what, cls, fmt, *values):
+    """An argument struct; sizes beyond its fields are a MambaError."""
+    try:
+        return cls.from_buffer_copy(fmt.pack(*values))
+    except struct.error:
+        raise MambaError("%s: a size does not fit 32 bits" % what) from None
+
+
+def _require_int32(what, *sizes):
+    """For sizes passed as ctypes c_int, which would cut them off."""
+    if max(sizes) > 0x7fffffff:
+        raise MambaError("%s: a size does not fit 32 bits" % what)
+
+
 def _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets, h=None, final_state=None):
     torch = _torch()
     _require(x.dim() == 3, "%s: x must be [batch, seqlen, dim]" % what)
@@ -726,10 +740,11 @@ def _recurrence_args(what, x, r, i, lam, c, initial_state, lengths, resets, h=No
         _check_tensor(resets, "resets", what, (bsz, L), torch.uint8, dev)
     sx, sr, si = x.stride(), r.stride(), i.stride()
     sh = sx if h is None else h.stride()
-    return MambaRecurrenceArgs.from_buffer_copy(_RECURRENCE_ARGS.pack(
+    return _packed(
+        what, MambaRecurrenceArgs, _RECURRENCE_ARGS,
         x.data_ptr(), r.data_ptr(), i.data_ptr(), lam.data_ptr(), _ptr0(initial_state), _ptr0(lengths), _ptr0(resets),
         _ptr0(h), _ptr0(final_state), bsz, L, dim, F16 if dt is torch.float16 else F32, c, sx[0], sx[1], sr[0], sr[1],
-        si[0], si[1], sh[0], sh[1]))
+        si[0], si[1], sh[0], sh[1])
 
 
 def _recurrence_out(name, what, out, x, lengths):
@@ -798,9 +813,10 @@ def gated_recurrence_backward(dh, x, r, i, lam, h, c=8.0, initial_state=None, le
     dlam = lam.new_empty(lam.shape)
     dh0 = lam.new_empty((a.batch, a.dim))
     sg, sx, sr, si = dh.stride(), dx.stride(), dr.stride(), di.stride()
-    g = MambaRecurrenceGrads.from_buffer_copy(_RECURRENCE_GRADS.pack(
+    g = _packed(
+        what, MambaRecurrenceGrads, _RECURRENCE_GRADS,
         dh.data_ptr(), _ptr0(dfinal_state), dx.data_ptr(), dr.data_ptr(), di.data_ptr(), dlam.data_ptr(),
-        dh0.data_ptr(), sg[0], sg[1], sx[0], sx[1], sr[0], sr[1], si[0], si[1]))
+        dh0.data_ptr(), sg[0], sg[1], sx[0], sx[1], sr[0], sr[1], si[0], si[1])
     need = lib().mamba_gated_recurrence_workspace(a, 1)
     ws, ws_len, owner = _workspace(what, need, workspace, x)
     _call(lib().mamba_gated_recurrence_backward, what, x, a, g, ws, ws_len)
@@ -821,6 +837,7 @@ def gated_recurrence_step(x, r, i, lam, state, c=8.0, state_out=None, h=None):
     _check_tensor(x, "x", what, shape, dt, dev, True)
     _check_tensor(r, "r", what, shape, dt, dev, True)
     _check_tensor(i, "i", what, shape, dt, dev, True)
+    _require_int32(what, *shape)
     _check_tensor(lam, "lam", what, shape[1:], torch.float32, dev)
     _check_tensor(state, "state", what, shape, torch.float32, dev)
     if state_out is None:
@@ -850,10 +867,11 @@ def _block_norm_args(what, y, w_post, z, w_pre, residual_scale, eps, residual=No
         _check_tensor(w_post, "w_post", what, shape[1:], torch.float32, dev)
     if w_pre is not None:
         _check_tensor(w_pre, "w_pre", what, shape[1:], torch.float32, dev)
-    return MambaBlockNormArgs.from_buffer_copy(_BLOCK_NORM_ARGS.pack(
+    return _packed(
+        what, MambaBlockNormArgs, _BLOCK_NORM_ARGS,
         y.data_ptr(), _ptr0(z), _ptr0(residual), _ptr0(w_post), _ptr0(w_pre), _ptr0(residual_out), _ptr0(out),
         _ptr0(rstd_post), _ptr0(rstd_pre), shape[0], shape[1], F16 if dt is torch.float16 else F32, residual_scale,
-        eps, y.stride(0), 0 if z is None else z.stride(0)))
+        eps, y.stride(0), 0 if z is None else z.stride(0))
 
 
 @_on_stream
@@ -930,9 +948,10 @@ def block_norm_backward(dresidual_out, dout, y, residual_out, rstd_post, rstd_pr
         _check_tensor(dz, "dz", what, shape, y.dtype, dev, True)
     dw_post = residual_out.new_empty(shape[1:])
     dw_pre = residual_out.new_empty(shape[1:])
-    g = MambaBlockNormGrads.from_buffer_copy(_BLOCK_NORM_GRADS.pack(
+    g = _packed(
+        what, MambaBlockNormGrads, _BLOCK_NORM_GRADS,
         _ptr0(dresidual_out), _ptr0(dout), dresidual.data_ptr(), dy.data_ptr(), _ptr0(dz), dw_post.data_ptr(),
-        dw_pre.data_ptr(), dy.stride(0), 0 if dz is None else dz.stride(0)))
+        dw_pre.data_ptr(), dy.stride(0), 0 if dz is None else dz.stride(0))
     ws, ws_len, owner = _workspace(what, lib().mamba_block_norm_workspace(a), workspace, y)
     _call(lib().mamba_block_norm_backward, what, y, a, g, ws, ws_len)
     return dy, dresidual, dw_post, dw_pre, dz
@@ -985,6 +1004,7 @@ def quantize_rows(x, q=None, scale=None):
     _check_float(x, "x", what)
     shape, dt, dev = x.shape, x.dtype, x.device
     rows, cols = shape
+    _require_int32(what, cols)
     _check_tensor(x, "x", what, shape, dt, dev, True)
     if q is None:
         q = x.new_empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8)
@@ -1012,6 +1032,7 @@ def linear_i8(x, x_scale, w, w_scale, bias=None, y=None, mode=0):
     _require(x.dim() == 2 and w.dim() == 2, "%s: x and w must be matrices" % what)
     _require(mode in (0, 1, 2), "%s: mode must be 0, 1 or 2" % what)
     (rows, k), n, dev = x.shape, w.shape[0], x.device
+    _require_int32(what, n, k)
     _check_tensor(x, "x", what, x.shape, torch.int8, dev, True)
     _check_tensor(w, "w", what, (n, k), torch.int8, dev, True)
     _check_tensor(x_scale, "x_scale", what, (rows,), torch.float32, dev)
