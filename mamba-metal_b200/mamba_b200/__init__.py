@@ -659,9 +659,10 @@ def _check_float(t, name, what):
 
 
 def _on_stream(fn):
-    """Adds the `stream` argument (a torch stream or a handle; default: the
-    current one).  The whole helper runs with that stream current, so that
-    what it allocates and fills belongs to the stream its kernels run on."""
+    """Adds the `stream` argument (a torch stream or a handle, of the tensors'
+    device; default: the current one).  The whole helper runs with that stream
+    current, so that what it allocates and fills belongs to the stream its
+    kernels run on."""
     @functools.wraps(fn)
     def helper(*args, stream=None, **kw):
         if stream is None:
@@ -673,6 +674,8 @@ def _on_stream(fn):
         if not isinstance(stream, torch.cuda.Stream):
             stream = torch.cuda.ExternalStream(stream, device=t.device) if stream \
                 else torch.cuda.default_stream(t.device)
+        if stream.device != t.device:
+            raise MambaError("%s: the stream's device is %s, the tensors' %s" % (fn.__name__, stream.device, t.device))
         with torch.cuda.stream(stream):
             return fn(*args, **kw)
     return helper

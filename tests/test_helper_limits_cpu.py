@@ -1,6 +1,9 @@
 """The tensor-level helpers of the recurrent-block operators, without a GPU:
 sizes that the C interface's 32-bit fields cannot hold are refused by the
 helper and not cut off.  Tensors on the meta device have shapes only."""
+import contextlib
+import types
+
 import pytest
 import torch
 
@@ -31,3 +34,25 @@ def test_sizes_beyond_32_bits(call):
     with pytest.raises(mb.MambaError, match="32 bits"):
         call()
 
+
+
+def test_a_stream_of_another_device(monkeypatch):
+    """The stream argument has to belong to the tensors' device: entering another
+    device's stream would leave the call on the tensors' device's current one."""
+    ran = []
+
+    class Tensor:
+        is_cuda, device = True, torch.device("cuda", 0)
+
+    class Stream:
+        def __init__(self, index):
+            self.device = torch.device("cuda", index)
+
+    cuda = types.SimpleNamespace(Stream=Stream, stream=lambda s: contextlib.nullcontext(ran.append(s)))
+    monkeypatch.setattr(mb, "_torch_module", types.SimpleNamespace(Tensor=Tensor, cuda=cuda))
+    helper = mb._on_stream(lambda t: "ran")
+    same = Stream(0)
+    assert helper(Tensor(), stream=same) == "ran" and ran == [same]
+    with pytest.raises(mb.MambaError, match="device"):
+        helper(Tensor(), stream=Stream(1))
+    assert ran == [same]
