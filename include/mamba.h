@@ -119,7 +119,9 @@ unsigned mamba_device_status(int clear);
  * barrier nothing completes, with a limit of limit_us microseconds
  * (1..1000000).  Returns 0 when the wait gave up on time and reported it
  * (bit 3 of mamba_device_status is then set; the context stays usable),
- * -1 otherwise. */
+ * -1 otherwise.  Waits of the gated recurrence, the 8-bit linear layer and
+ * the block norm run out the same way, each with that limit, and set bits 6,
+ * 7 and 8. */
 int mamba_selftest_bounded_wait(unsigned limit_us, void *stream);
 
 /* dt_rank used for a config: ceil(d_model / 16). */

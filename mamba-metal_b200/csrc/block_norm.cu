@@ -196,9 +196,6 @@ __device__ __forceinline__ void fetch_row(const RingRow<N> &r, uint8_t *ring, ui
             bulk_load(ring + s * r.stage + r.offset[k],
                       static_cast<const uint8_t *>(r.src[k]) + row * r.stride[k] - r.shift(k, row), bytes[k], &full[s]);
 }
-__device__ __forceinline__ void await_row(uint64_t *bar, uint32_t parity) {
-    if (!mbar_wait_bounded(bar, parity)) atomicOr(&g_block_norm_error, kErrBlockNormTimeout);
-}
 // Place s of the ring in use, and the parity of that use.
 struct RingPlace {
     int s = 0;
@@ -210,10 +207,19 @@ struct RingPlace {
         }
     }
 };
+// Waits for the row at a place.  A wait that runs out is reported; the CTA goes
+// on, with wrong values.
+constexpr uint64_t kWaitNs = 2000000000ull;
+__device__ __forceinline__ void await_row(uint64_t *full, const RingPlace &at, LostCopies *lost,
+                                          uint64_t limit_ns = kWaitNs) {
+    if (!await_copy(full, at.s, at.parity, lost, limit_ns)) atomicOr(&g_block_norm_error, kErrBlockNormTimeout);
+}
 // Sets the ring up and fetches the first rows; rows first, first + step, ...
 template <int N>
-__device__ __forceinline__ void start_ring(const RingRow<N> &r, uint8_t *ring, uint64_t *full, int64_t rows) {
+__device__ __forceinline__ void start_ring(const RingRow<N> &r, uint8_t *ring, uint64_t *full, LostCopies *lost,
+                                           int64_t rows) {
     if (threadIdx.x == 0) {
+        *lost = LostCopies{};
         for (int s = 0; s < r.stages; ++s) mbar_init(&full[s], 1);
         fence_mbar_init();
         int64_t row = blockIdx.x;
@@ -229,18 +235,19 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_kernel(const NormParams
     constexpr bool PRECISE = sizeof(T) == 4;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[kMaxStages];
+    __shared__ LostCopies lost;
     __shared__ float sm[64];
     int turn = 0;
     const float inv_cols = 1.f / (float)p.cols;
     RingPlace at;
-    if (RING) start_ring<3>(ring, smem, full, p.rows);
+    if (RING) start_ring<3>(ring, smem, full, &lost, p.rows);
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const uint8_t *place = smem + at.s * ring.stage;
         auto at_place = [&](int k) { return place + ring.offset[k] + (VEC == 1 ? ring.shift(k, row) : 0u); };
         const T *y = RING ? reinterpret_cast<const T *>(at_place(0)) : static_cast<const T *>(p.y) + row * p.sy;
         const T *z = RING ? reinterpret_cast<const T *>(at_place(1)) : static_cast<const T *>(p.z) + row * p.sz;
         const float *res = RING ? reinterpret_cast<const float *>(at_place(2)) : p.res + row * p.cols;
-        if (RING) await_row(&full[at.s], at.parity);
+        if (RING) await_row(full, at, &lost);
         float v[NV][VEC], gz[NV][VEC], r[NV][VEC];
         float ss = 0.f;
 #pragma unroll
@@ -257,7 +264,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_kernel(const NormParams
         const float rs = rsqrtf(block_sum(ss, sm, turn) * inv_cols + p.eps);
         if (RING) {
             const int64_t ahead = row + (int64_t)ring.stages * gridDim.x;
-            if (threadIdx.x == 0 && ahead < p.rows) fetch_row<3>(ring, smem, full, ahead, at.s);
+            if (threadIdx.x == 0 && ahead < p.rows && !lost.flag) fetch_row<3>(ring, smem, full, ahead, at.s);
             at.step(ring.stages);
         }
         float ss2 = 0.f;
@@ -297,6 +304,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_kernel(const NormParams
         }
         if (threadIdx.x == 0 && p.rstd_pre) p.rstd_pre[row] = rp;
     }
+    if (RING) drain_copies(full, ring.stages, &lost, kWaitNs);
 }
 
 // Backward: CTA k walks rows k, k + CTAs, ... and keeps the column sums of
@@ -306,6 +314,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_bwd_kernel(const NormGr
     constexpr bool PRECISE = sizeof(T) == 4;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[kMaxStages];
+    __shared__ LostCopies lost;
     __shared__ float sm[64];
     int turn = 0;
     const int cols = p.f.cols;
@@ -313,7 +322,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_bwd_kernel(const NormGr
     float acc_post[NV][VEC] = {}, acc_pre[NV][VEC] = {};
     const bool first = p.dout != nullptr;  // the second norm's output has a gradient
     RingPlace at;
-    if (RING) start_ring<5>(ring, smem, full, p.f.rows);
+    if (RING) start_ring<5>(ring, smem, full, &lost, p.f.rows);
     float rs_next = p.f.rstd_post[blockIdx.x], rp_next = first ? p.f.rstd_pre[blockIdx.x] : 0.f;  // grid <= rows
     for (int64_t row = blockIdx.x; row < p.f.rows; row += gridDim.x) {
         const uint8_t *place = smem + at.s * ring.stage;
@@ -330,7 +339,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_bwd_kernel(const NormGr
             rs_next = p.f.rstd_post[after];
             if (first) rp_next = p.f.rstd_pre[after];
         }
-        if (RING) await_row(&full[at.s], at.parity);
+        if (RING) await_row(full, at, &lost);
         float R[NV][VEC], n[NV][VEC], gz[NV][VEC], d[NV][VEC], m[NV][VEC];
         float dot = 0.f;
 #pragma unroll
@@ -369,7 +378,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_bwd_kernel(const NormGr
         const float mean = RING || first ? block_sum(dot, sm, turn) * inv_cols : 0.f;
         if (RING) {
             const int64_t ahead = row + (int64_t)ring.stages * gridDim.x;
-            if (threadIdx.x == 0 && ahead < p.f.rows) fetch_row<5>(ring, smem, full, ahead, at.s);
+            if (threadIdx.x == 0 && ahead < p.f.rows && !lost.flag) fetch_row<5>(ring, smem, full, ahead, at.s);
             at.step(ring.stages);
         }
         float dot2 = 0.f;
@@ -420,6 +429,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_bwd_kernel(const NormGr
             if (p.part_pre) store_n(p.part_pre + (int64_t)blockIdx.x * cols + c, acc_pre[j]);
         }
     }
+    if (RING) drain_copies(full, ring.stages, &lost, kWaitNs);
 }
 
 // Column sums of the partial rows, in a fixed order: warp w of a CTA adds
@@ -702,6 +712,30 @@ int block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *
     block_norm_sum_kernel<<<dim3((unsigned)ceil_div(a->cols, 32), 2), kSumThreads, 0, st>>>(
         p.part_post, p.part_pre, g->dw_post, g->dw_pre, (int)grid, a->cols);
     return launch_status("block_norm_backward sum kernel");
+}
+
+namespace {
+
+// A wait for a row that nothing fetches, through the kernels' own helper.
+__global__ void block_norm_wait_selftest_kernel(uint64_t limit_ns) {
+    __shared__ uint64_t full[2];
+    __shared__ LostCopies lost;
+    if (threadIdx.x != 0) return;
+    lost = LostCopies{};
+    for (int s = 0; s < 2; ++s) mbar_init(&full[s], 1);
+    fence_mbar_init();
+    RingPlace at;
+    await_row(full, at, &lost, limit_ns);
+    at.step(2);
+    await_row(full, at, &lost, limit_ns);  // at once
+    drain_copies(full, 2, &lost, limit_ns);
+}
+
+}  // namespace
+
+int block_norm_wait_selftest(uint64_t limit_ns, cudaStream_t st) {
+    block_norm_wait_selftest_kernel<<<1, 32, 0, st>>>(limit_ns);
+    return launch_status("block_norm wait self-test kernel");
 }
 
 unsigned block_norm_error_flags(bool clear) {

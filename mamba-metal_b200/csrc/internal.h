@@ -54,6 +54,7 @@ int recurrence_step(const void *x, int64_t xrs, const void *r, int64_t rrs, cons
                     const float *lambda, const float *state_in, float *state_out, void *h, int64_t hrs, int batch,
                     int dim, float c, int dtype, cudaStream_t st);
 unsigned recurrence_error_flags(bool clear);
+int recurrence_wait_selftest(uint64_t limit_ns, cudaStream_t st);
 
 // norm.cu
 int rmsnorm(const void *x, const float *w, void *y, int64_t rows, int cols, float eps, int in_dt,
@@ -65,6 +66,7 @@ int block_norm(const MambaBlockNormArgs *a, cudaStream_t st);
 int block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *g, void *ws, size_t ws_bytes,
                         cudaStream_t st);
 unsigned block_norm_error_flags(bool clear);
+int block_norm_wait_selftest(uint64_t limit_ns, cudaStream_t st);
 
 // ssm_step.cu
 int ssm_step(const void *x, int64_t xrs, const void *delta, int64_t drs, const float *dt_bias,
@@ -109,6 +111,7 @@ int quantize_rows(const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *sca
 int linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw, const float *w_scale,
               const float *bias, void *y, int64_t ldy, int64_t rows, int n, int k, int mode, cudaStream_t st);
 unsigned linear_i8_error_flags(bool clear);
+int linear_i8_wait_selftest(uint64_t limit_ns, cudaStream_t st);
 
 // init.cu
 uint64_t fill_key(uint64_t seed, int layer, int tag);

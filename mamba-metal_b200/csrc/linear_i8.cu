@@ -255,9 +255,9 @@ struct PairParams {
     bool boxes;  // y's rows allow bulk tensor stores
 };
 
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, uint64_t limit_ns = 2000000000ull) {
     int ok = 0;
-    if ((threadIdx.x & 31) == 0) ok = mbar_wait_bounded(bar, parity) ? 1 : 0;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait_bounded(bar, parity, limit_ns) ? 1 : 0;
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
@@ -703,6 +703,26 @@ int linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *
     MB_CHECK_ARG(rows <= 65535LL * kDT, "linear_i8: too many rows");
     linear_i8_dp4a_kernel<<<dim3((unsigned)ceil_div(n, kDT), (unsigned)ceil_div64(rows, kDT)), 256, 0, st>>>(p);
     return launch_status("linear_i8 kernel");
+}
+
+namespace {
+
+// A wait for sums that nothing computes, through the epilogue's own helper.
+__global__ void linear_i8_wait_selftest_kernel(uint64_t limit_ns) {
+    __shared__ uint64_t bar;
+    if (threadIdx.x == 0) {
+        mbar_init(&bar, 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
+    if (!warp_wait(&bar, 0, limit_ns)) atomicOr(&g_linear_i8_error, kErrLinearI8Timeout);
+}
+
+}  // namespace
+
+int linear_i8_wait_selftest(uint64_t limit_ns, cudaStream_t st) {
+    linear_i8_wait_selftest_kernel<<<1, 32, 0, st>>>(limit_ns);
+    return launch_status("linear_i8 wait self-test kernel");
 }
 
 unsigned linear_i8_error_flags(bool clear) {

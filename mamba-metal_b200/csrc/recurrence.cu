@@ -241,16 +241,17 @@ __device__ __forceinline__ uint32_t get_state(const float *slot) {
 
 // Bounded wait: 2 s, or at once after a wait of this call ran out (`gave_up`, a
 // word of the call's workspace, is then no longer empty).
+constexpr uint64_t kWaitNs = 2000000000ull;
 struct Waiting {
     uint32_t *gave_up;
-    uint64_t t0 = 0;
+    uint64_t limit_ns, t0 = 0;
     int spins = 0;
-    __device__ __forceinline__ explicit Waiting(uint32_t *g) : gave_up(g) {}
+    __device__ __forceinline__ Waiting(uint32_t *g, uint64_t limit) : gave_up(g), limit_ns(limit) {}
     __device__ __forceinline__ bool again() {
         if ((++spins & 63) == 0) {
             const uint64_t now = global_timer_ns();
             if (t0 == 0) t0 = now;
-            if (now - t0 > 2000000000ull || *(volatile uint32_t *)gave_up != kEmpty) {
+            if (now - t0 > limit_ns || *(volatile uint32_t *)gave_up != kEmpty) {
                 *(volatile uint32_t *)gave_up = 0;
                 atomicOr(&g_recurrence_error, kErrRecurrenceTimeout);
                 return false;
@@ -342,8 +343,8 @@ struct MapRows {
 
 template <int VEC>
 __device__ __forceinline__ void wait_maps(const float2 *slot, uint32_t *gave_up, Pack<float, VEC> &P,
-                                          Pack<float, VEC> &H) {
-    Waiting wt(gave_up);
+                                          Pack<float, VEC> &H, uint64_t limit_ns = kWaitNs) {
+    Waiting wt(gave_up, limit_ns);
     bool ready;
     do {
         uint64_t w[VEC];
@@ -359,8 +360,9 @@ __device__ __forceinline__ void wait_maps(const float2 *slot, uint32_t *gave_up,
     } while (!ready && wt.again());
 }
 template <int VEC>
-__device__ __forceinline__ void wait_states(const float *slot, uint32_t *gave_up, float (&h)[VEC]) {
-    Waiting wt(gave_up);
+__device__ __forceinline__ void wait_states(const float *slot, uint32_t *gave_up, float (&h)[VEC],
+                                            uint64_t limit_ns = kWaitNs) {
+    Waiting wt(gave_up, limit_ns);
     bool ready;
     do {
         uint32_t w[VEC];
@@ -532,6 +534,7 @@ template <typename T, int VEC, int TT, int N, int NB>
 struct TileIn {
     alignas(128) Pack<T, VEC> v[NB][N][TT][32];
     alignas(16) uint64_t full[NB];
+    LostCopies lost;
 };
 struct TileMaps {
     CUtensorMap m[5];
@@ -543,10 +546,11 @@ __device__ __forceinline__ void fetch_box(void *dst, const CUtensorMap *map, uin
     tma_load_3d(dst, map, bar, d, row_first ? b : t, row_first ? t : b);
 }
 
-// Waits for buffer `buf` in its `use`-th use.  A wait that runs out is
-// reported; the CTA goes on (with wrong values), so nothing else waits for it.
-__device__ __forceinline__ void await_box(uint64_t *bar, uint32_t use) {
-    if (!mbar_wait_bounded(bar, use & 1)) atomicOr(&g_recurrence_error, kErrRecurrenceTimeout);
+// Waits for buffer `buf` in its `use`-th use.  A wait that runs out is reported;
+// the CTA goes on, with wrong values.
+__device__ __forceinline__ void await_box(uint64_t *full, int buf, uint32_t use, LostCopies *lost,
+                                          uint64_t limit_ns = kWaitNs) {
+    if (!await_copy(full, buf, use & 1, lost, limit_ns)) atomicOr(&g_recurrence_error, kErrRecurrenceTimeout);
 }
 
 // Without TMA: FP32 elements are copied to shared memory asynchronously.  FP16
@@ -624,6 +628,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
     if (TMA) {
         if (tid == 0) {
             mbar_init(&sm.in.full[0], 1);
+            sm.in.lost = LostCopies{};
             fence_mbar_init();
         }
         __syncthreads();
@@ -643,7 +648,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
     auto fetch = [&](const Tile &t) {
         if (!t.live) return;
         if constexpr (TMA) {
-            if (tid == 0) {
+            if (tid == 0 && !sm.in.lost.flag) {
                 uint64_t *bar = &sm.in.full[0];
                 mbar_arrive_expect_tx(bar, 3 * TT * 32 * VEC * sizeof(T));
                 const int d0 = t.d, t0 = t.t0;  // of thread 0: the tile's first channel and token
@@ -696,7 +701,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
         }
         if (t.live) {
             if constexpr (TMA) {
-                await_box(&sm.in.full[0], uses++);
+                await_box(sm.in.full, 0, uses++, &sm.in.lost);
             } else {
                 copy_wait<0>();
                 put_held(sm.in.v[0], held, warp * S, t.cnt);
@@ -804,6 +809,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
         if (!next) break;
         t = tn;
     }
+    if (TMA) drain_copies(sm.in.full, 1, &sm.in.lost, kWaitNs);
 }
 
 // ---- backward -------------------------------------------------------------------
@@ -839,6 +845,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
         if (tid == 0) {
             mbar_init(&sm.in.full[0], 1);
             mbar_init(&sm.in.full[1], 1);
+            sm.in.lost = LostCopies{};
             fence_mbar_init();
         }
         __syncthreads();
@@ -854,7 +861,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
     Held<T, 5, TMA ? 1 : S> held;
     auto fetch = [&](const Tile &t, int buf) {
         if constexpr (TMA) {
-            if (tid == 0) {
+            if (tid == 0 && !sm.in.lost.flag) {
                 uint64_t *bar = &sm.in.full[buf];
                 mbar_arrive_expect_tx(bar, 5 * TT * 32 * VEC * sizeof(T));
                 // A dead tile lies before time 0: its copies read zeros.
@@ -915,7 +922,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
             if (next) tn = place(v);
         }
         if constexpr (TMA) {
-            await_box(&sm.in.full[buf], it >> 1);
+            await_box(sm.in.full, buf, it >> 1, &sm.in.lost);
         } else {
             copy_wait<0>();
             put_held(sm.in.v[buf], held, trow, t.cnt);
@@ -1129,6 +1136,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
         if (!next) break;
         t = tn;
     }
+    if (TMA) drain_copies(sm.in.full, 2, &sm.in.lost, kWaitNs);
 }
 
 // dlambda[d] = sigmoid(lambda)/softplus(lambda) * sum of the tiles' sums of E,
@@ -1600,6 +1608,33 @@ int recurrence_backward(const MambaRecurrenceArgs *a, const MambaRecurrenceGrads
         p.sdi[k] = g->di_stride[k];
     }
     return a->dtype == MAMBA_F16 ? choose_backward<__half>(a, p, g, ws, st) : choose_backward<float>(a, p, g, ws, st);
+}
+
+namespace {
+
+// Waits that nothing ends, through the kernels' own helpers: for a published
+// state and for a box.  The words outlive the call and stay as they are.
+__device__ uint32_t g_wait_selftest[2] = {kEmpty, kEmpty};
+__global__ void recurrence_wait_selftest_kernel(uint64_t limit_ns) {
+    __shared__ uint64_t full[1];
+    __shared__ LostCopies lost;
+    if (threadIdx.x != 0) return;
+    float h[1];
+    wait_states<1>(reinterpret_cast<const float *>(&g_wait_selftest[1]), &g_wait_selftest[0], h, limit_ns);
+    const bool reported = *(volatile uint32_t *)&g_wait_selftest[0] != kEmpty;
+    *(volatile uint32_t *)&g_wait_selftest[0] = kEmpty;
+    lost = LostCopies{};
+    mbar_init(&full[0], 1);
+    fence_mbar_init();
+    if (reported) await_box(full, 0, 0, &lost, limit_ns);
+    drain_copies(full, 1, &lost, limit_ns);
+}
+
+}  // namespace
+
+int recurrence_wait_selftest(uint64_t limit_ns, cudaStream_t st) {
+    recurrence_wait_selftest_kernel<<<1, 32, 0, st>>>(limit_ns);
+    return launch_status("gated_recurrence wait self-test kernel");
 }
 
 unsigned recurrence_error_flags(bool clear) {

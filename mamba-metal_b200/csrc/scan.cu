@@ -1548,8 +1548,11 @@ int bounded_wait_selftest(unsigned limit_us, cudaStream_t st) {
     int *flag = nullptr;
     MB_CUDA_TRY(cudaMallocAsync(&flag, sizeof(int), st));
     MB_CUDA_TRY(cudaMemsetAsync(flag, 0, sizeof(int), st));
-    bounded_wait_selftest_kernel<<<1, 32, 0, st>>>((uint64_t)limit_us * 1000ull, flag);
-    if (launch_status("bounded-wait selftest kernel")) return -1;
+    const uint64_t limit_ns = (uint64_t)limit_us * 1000ull;
+    bounded_wait_selftest_kernel<<<1, 32, 0, st>>>(limit_ns, flag);
+    if (launch_status("bounded-wait selftest kernel") || recurrence_wait_selftest(limit_ns, st) ||
+        linear_i8_wait_selftest(limit_ns, st) || block_norm_wait_selftest(limit_ns, st))
+        return -1;
     int h = 0;
     MB_CUDA_TRY(cudaMemcpyAsync(&h, flag, sizeof(int), cudaMemcpyDeviceToHost, st));
     MB_CUDA_TRY(cudaFreeAsync(flag, st));

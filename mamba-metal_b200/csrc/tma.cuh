@@ -62,6 +62,44 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity
     return true;
 }
 
+// A CTA whose threads all wait for the copies that thread 0 issues, over a few
+// places of shared memory in turn, and goes on after a wait that runs out, so
+// that its own barriers stay matched and nobody waits for it.  This word of
+// shared memory (0 to begin with) then says so: no thread waits again, thread 0 issues
+// no more copies, and gives those in flight a last chance to land (drain_copies,
+// at the end).  It costs no registers while nothing is lost.
+struct LostCopies {
+    uint32_t flag;   // a wait ran out
+    uint32_t place;  // 1 + 2 * the first place that thread 0 gave up + its parity
+};
+// False where this wait runs out: the caller reports it.
+__device__ __forceinline__ bool await_copy(uint64_t *bars, int place, uint32_t parity, volatile LostCopies *lost,
+                                           uint64_t limit_ns) {
+    if (mbar_try_wait(&bars[place], parity)) return true;
+    const uint64_t t0 = global_timer_ns();
+    while (!mbar_try_wait(&bars[place], parity)) {
+        const bool over = global_timer_ns() - t0 > limit_ns;
+        if (over || lost->flag) {
+            lost->flag = 1;
+            if (threadIdx.x == 0 && lost->place == 0) lost->place = 1 + 2 * place + parity;
+            return !over;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ void drain_copies(uint64_t *bars, int places, volatile LostCopies *lost, uint64_t limit_ns) {
+    if (threadIdx.x != 0 || lost->place == 0) return;
+    int at = (int)(lost->place - 1) >> 1;
+    uint32_t parity = (lost->place - 1) & 1;
+    for (int k = 0; k < places; ++k) {
+        mbar_wait_bounded(&bars[at], parity, limit_ns);
+        if (++at == places) {
+            at = 0;
+            parity ^= 1;
+        }
+    }
+}
+
 // 3-D tiled bulk tensor load global -> this CTA's shared memory, completing
 // on `bar` by transaction bytes.  Coordinates are element indices, innermost
 // first; the innermost coordinate is always a multiple of the 16-byte
