@@ -641,12 +641,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
         return t;
     };
     Held<T, 3, TMA ? 1 : S> held;
-    // Tiles behind their row's end are neither fetched nor waited for: every warp
-    // has passed the barrier's last phase (and the CTA barrier behind it) before
-    // the next one is armed, however many such tiles lie between.
-    uint32_t uses = 0;
     auto fetch = [&](const Tile &t) {
-        if (!t.live) return;
         if constexpr (TMA) {
             if (tid == 0 && !sm.in.lost.flag) {
                 uint64_t *bar = &sm.in.full[0];
@@ -686,7 +681,7 @@ __global__ void __launch_bounds__(32 * W, CTAS)
             s[e] = t.in && p.h0 ? p.h0[(int64_t)t.b * p.D + t.d + e] : 0.f;
         }
     }
-    for (;;) {
+    for (uint32_t it = 0;; ++it) {
         Tile tn = t;
         bool next;
         if (WALK) {
@@ -699,13 +694,13 @@ __global__ void __launch_bounds__(32 * W, CTAS)
             next = v < total;
             if (next) tn = place(v);
         }
+        if constexpr (TMA) {
+            await_box(sm.in.full, 0, it, &sm.in.lost);
+        } else {
+            copy_wait<0>();
+            put_held(sm.in.v[0], held, warp * S, t.cnt);
+        }
         if (t.live) {
-            if constexpr (TMA) {
-                await_box(sm.in.full, 0, uses++, &sm.in.lost);
-            } else {
-                copy_wait<0>();
-                put_held(sm.in.v[0], held, warp * S, t.cnt);
-            }
             if (!WALK)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) csp[e] = t.in ? ch.csp[t.d + e] : 0.f;
@@ -804,6 +799,10 @@ __global__ void __launch_bounds__(32 * W, CTAS)
                     }
             });
         } else if (next) {
+            // Behind the row's end there is nothing to compute, but every warp has to have
+            // seen this phase of the fetch barrier before the next one is armed: one that
+            // finds it two phases on takes the parity for the present one and stands.
+            __syncthreads();
             fetch(tn);
         }
         if (!next) break;
