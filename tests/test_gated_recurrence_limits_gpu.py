@@ -219,3 +219,79 @@ def test_gradients_of_nearly_open_gates(cuda, B, L, D, dtype):
     # each for the decay and for the gates' approximate exponentials
     d, u, tiny = (2.1e-5, 2.0 ** -11, 2.0 ** -25) if dtype == torch.float16 else (2.0 ** -24 * 64, 2.0 ** -24, 0.0)
     _check(dr, g["dr"], gm["dr"], u, d, tiny, "dr")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_calls_that_share_the_gpu(cuda, dtype):
+    """Forward and backward on two streams at once, each with tiles that wait for
+    one another, beside a replayed graph of a third call: every call as alone."""
+    cases = []
+    for seed, (B, L, D) in enumerate(((2, 6000, 256), (3, 5000, 320), (1, 9000, 128))):
+        v = _slow(50 + seed, B, L, D, dtype)
+        cases.append({k: torch.from_numpy(a).cuda() for k, a in v.items()})
+
+    def call(t):
+        h, hN = mb.gated_recurrence(t["x"], t["r"], t["i"], t["lam"], c=C, initial_state=t["h0"],
+                                    return_final_state=True)
+        return [h, hN, *mb.gated_recurrence_backward(t["dh"], t["x"], t["r"], t["i"], t["lam"], h, c=C,
+                                                     initial_state=t["h0"], dfinal_state=t["dfinal"])]
+
+    alone = [call(t) for t in cases]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = call(cases[2])
+    torch.cuda.synchronize()
+    mb.device_status(True)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        outs = []
+        for t, s in zip(cases[:2], streams):
+            with torch.cuda.stream(s):
+                outs.append(call(t))
+        with torch.cuda.stream(streams[2]):
+            graph.replay()
+        for t, s in zip(cases[:2], streams):
+            with torch.cuda.stream(s):
+                call(t)
+        torch.cuda.synchronize()
+        for got, want in zip(outs + [captured], alone):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert mb.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("ragged,resets", [(False, False), (True, True)])
+@pytest.mark.parametrize("B,L,D", [(1, 1, 1), (2, 65, 130), (1, 257, 1001), (3, 300, 256), (24, 140, 1000), (2, 900, 72)])
+def test_every_element_for_itself(cuda, B, L, D, ragged, resets, dtype):
+    """The parity cases with each element's own magnitude in the bound: small
+    states, closed gates and small gradients count as much as large ones."""
+    rng = np.random.default_rng(B + L + D)
+    np_t = np.float16 if dtype == torch.float16 else np.float32
+    x, r, i, dh = (rng.standard_normal((B, L, D)).astype(np_t) for _ in range(4))
+    scale = 10.0 ** rng.uniform(-3, 1, D)  # channels of different sizes
+    x, dh = (x * scale).astype(np_t), (dh / scale).astype(np_t)
+    lam = np.log(np.expm1(10.0 ** rng.uniform(-4, 0, D))).astype(np.float32)
+    h0, dfin = (rng.standard_normal((B, D)).astype(np.float32) for _ in range(2))
+    lengths = cuts = None
+    if ragged:
+        lengths = rng.integers(1, L + 1, B).astype(np.int32)
+        lengths[0] = L
+    if resets:
+        cuts = (rng.random((B, L)) < 0.05).astype(np.uint8)
+    tx, tr, ti, tl, tg, th, tf, tn, tc = _dev(x, r, i, lam, dh, h0, dfin, lengths, cuts)
+    kw = dict(c=C, initial_state=th, lengths=tn, resets=tc)
+    h, hN = mb.gated_recurrence(tx, tr, ti, tl, return_final_state=True, **kw)
+    grads = mb.gated_recurrence_backward(tg, tx, tr, ti, tl, h, dfinal_state=tf, **kw)
+    # gates: 16 roundings (FP16 tensors: 1e-5 for the series and the approximate exponentials);
+    # the state: three roundings a token at most, over its tokens
+    gates = 1e-5 if dtype == torch.float16 else 2.0 ** -24 * 16
+    d, u = gates + 2.0 ** -24 * 3 * L, 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -24
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
+    ref, fin, mag = rb.gated_recurrence(x, r, i, lam, C, h0, lengths, cuts)
+    _check(h, ref, mag, u, d, tiny, "h")
+    _check(hN, fin, _last(mag, lengths), 0, d, 2.0 ** -126, "final state")
+    g, gm = rb.gated_recurrence_backward(dh, x, r, i, lam, h.cpu().numpy(), C, h0, lengths, cuts, dfin)
+    for got, k in zip(grads, ("dx", "dr", "di")):
+        _check(got, g[k], gm[k], u, d + gates, tiny, k)
+    _check(grads[4], g["dh0"], gm["dh0"], 0, d, 2.0 ** -126, "dh0")
+    _check(grads[3], g["dlam"], gm["dlam"], 0, d + gates + 2.0 ** -24 * (L + 64 + B), 2.0 ** -126, "dlam")
