@@ -382,7 +382,12 @@ int mamba_ssm_step(const void *x, int64_t x_row_stride, const void *delta,
  * and final_state is the state after the row's last token (the initial state
  * for an empty row).
  * resets, [batch, seqlen] bytes (NULL: none): where nonzero, h_{t-1} counts
- * as zero at that token, so several documents can share a row.
+ * as zero at that token, so several documents can share a row.  A reset
+ * only cuts the state: its token still enters with sqrt(1 - a^2), not with
+ * weight 1 as some implementations of this layer let the first token of a
+ * document in, so weights trained that way give other results there.
+ * FP16 tensors: decays near 1 are rounded once, like those of FP32 tensors;
+ * the gates' exponentials and reciprocals are approximate (1e-5).
  * seqlen <= 2^31 - 257, and batch x (tiles of the sequence and channels)
  * < 2^31.
  * Outputs must not overlap inputs or each other (so final_state is not
@@ -455,7 +460,9 @@ int mamba_rmsnorm(const void *x, const float *w, void *y, int64_t rows, int cols
  * stream and all sums FP32, contiguous.  NULL: z (no gate), a weight (ones),
  * out (no second norm), rstd_* (not kept).  residual_out may be residual
  * itself; otherwise outputs must not overlap inputs or each other.
- * cols <= 16384. */
+ * Rows that are not 16-byte aligned may be read in aligned 16-byte pieces,
+ * together with the up to 15 bytes before and behind them; those bytes have
+ * no effect.  cols <= 16384. */
 typedef struct MambaBlockNormArgs {
     const void *y;
     const void *z;
@@ -558,7 +565,9 @@ int mamba_quantize_rows(const void *x, int64_t ldx, int8_t *q, int64_t ldq, floa
  * bounds k to 131071; any value of int8 may occur.  y may not be one of the
  * inputs.  16-byte aligned x and w
  * with row strides that are multiples of 16 run on the tensor cores, others
- * on a slower kernel with the same result.  No workspace.  0 / -1. */
+ * on a slower kernel (at most 4194240 rows) with the same result.  v is
+ * evaluated in FP32 as (sum * x_scale) * w_scale + bias: sum * x_scale has
+ * to be finite.  No workspace.  0 / -1. */
 int mamba_linear_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw,
                     const float *w_scale, const float *bias, void *y, int64_t ldy, int64_t rows, int n, int k,
                     int mode, void *stream);

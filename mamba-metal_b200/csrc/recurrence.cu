@@ -96,9 +96,9 @@ __device__ __forceinline__ float2 exp_gate(float2 v, float top) {
 // Else: a series to y^5 and an exponential made 5 * 2^-24 too small, which is
 // more than it is ever off: both bound a from below, so the larger one is
 // right everywhere, without comparing and selecting.  Worst where they meet,
-// near y = 0.25: 6e-7 of a, 3e-6 of m.  With the plain exponential instead, up to 1.4 *
-// 2^-24 off near 1, 8 x 4096 x 4096 took 248 us, with the series 255; backward
-// 8 x 2048 x 4096 271 and 292.
+// near y = 0.25: 6e-7 of a, 3e-6 of m.  With the plain exponential instead, up to
+// 1.4 * 2^-24 off near 1, 8 x 4096 x 4096 took 248 us, with the series 255;
+// backward 8 x 2048 x 4096 271 and 292.
 template <bool PRECISE>
 __device__ __forceinline__ void decay_of(float2 y, float2 &a, float2 &m) {
     if (PRECISE) {
@@ -602,10 +602,10 @@ __device__ __forceinline__ float &half_of(float2 &v, int k) { return k & 1 ? v.y
 // writes h.  With enough chains to fill the GPU
 // (walks()), a CTA walks one chain from its first tile to its last instead
 // (WALK): no tickets, nothing published, the state stays in registers.
-// Bound by bytes for many warps (64 x 512 x 4096 FP16: 214 us, 5.0 TB/s), by
-// latency below: 8 x 4096 x 4096 (512 chains, 12.5 warps an SM) 246 to 252 us
-// with the special-function unit 59% and issue 48% busy; 1 x 131072 x 2048 FP32
-// 813 us (5.3 TB/s, issue 62%).
+// Bound by bytes for many warps (64 x 512 x 4096 FP16: 219 us, 4.9 TB/s), by
+// latency below: 8 x 4096 x 4096 (512 chains, 12.5 warps an SM) 254 to 257 us
+// with the special-function unit 57% and issue 49% busy; 1 x 131072 x 2048 FP32
+// 806 us (5.3 TB/s).
 template <typename T, int VEC, int S, int W, bool WALK>
 struct FwdSmem {
     TileIn<T, VEC, S * W, 3, 1> in;
@@ -815,9 +815,10 @@ __global__ void __launch_bounds__(32 * W, CTAS)
 // The same tiles and chains with time reversed; what runs along a chain is
 // C_t = keep_t a_t G_t, the part of the gradient that reaches h_{t-1}.  Across
 // the wait a thread keeps dh and sigmoid(r), or exp(-r); the decay is computed
-// again (one exponential) rather than held.  8 x 2048 x 4096 FP16 takes 302 us
-// (3.6 TB/s), with 1 - sigmoid(r) as a difference, without its reciprocal, 292;
-// 8 x 1024 x 4096 FP32 193 (5.6).
+// again (one exponential) rather than held.  8 x 2048 x 4096 FP16 takes 306 us
+// (3.5 TB/s; issue 53% at 12.5 warps an SM, and time follows the count of
+// instructions), with 1 - sigmoid(r) as a difference, without its reciprocal,
+// 10 less; 8 x 1024 x 4096 FP32 194 (5.5).
 template <typename T, int VEC, int S, int W, bool WALK>
 struct BwdSmem {
     TileIn<T, VEC, S * W, 5, 2> in;
@@ -1289,8 +1290,8 @@ struct Shape {
     static constexpr int VEC = VEC_, S = S_, W = W_, CTAS = CTAS_, tile = S_ * W_;
     static constexpr bool TMA = TMA_;
 };
-// FP16 walking, 8 x 4096 x 4096: 251 us; 8 warps a CTA 267 to 277; one channel a
-// thread 262.  Backward 8 x 2048 x 4096: 285, 8 warps 325 to 335.
+// FP16 walking, 8 x 4096 x 4096: 257 us; 8 warps a CTA 314; one channel a thread
+// 286 to 293.  Backward 8 x 2048 x 4096: 308, 8 warps 306 to 308.
 template <typename T> struct Shapes;
 template <> struct Shapes<__half> {
     using Fwd = Shape<2, 16, 4, 4>;
@@ -1332,8 +1333,9 @@ bool plan_chains(const MambaRecurrenceArgs *a, bool backward, Plan &pl) {
     c.chains = divisor(blocks * a->batch);
     c.tiles = (int)tiles;
     // A chain's latency is its groups' hand-overs plus a group's length of maps to
-    // compose.  Groups of 4 everywhere: 1 x 524288 x 64 FP16 971 us instead of 309;
-    // short chains take the same time with any (1 x 16384 x 4096 166 to 172 us).
+    // compose.  Groups of 4 everywhere: 1 x 524288 x 64 FP16 931 us instead of 303;
+    // of 16 everywhere: 1 x 131072 x 2048 FP32 820 instead of 807, 1 x 16384 x 4096
+    // FP16 175 instead of 173.
     c.group_shift = std::min(kMaxGroupShift, tiles <= 128 ? 2 : tiles <= 1024 ? 3 : 4);
     c.group = 1 << c.group_shift;
     c.groups = ceil_div((int)tiles, c.group);
@@ -1423,10 +1425,10 @@ int launch_tiles(Kernel kernel, const Params &p, const FwdParams &f, Plan &pl, c
 // Whether CTAs should walk whole chains: where the chains fill the resident
 // CTAs of `Sh` in nearly whole rounds, walking spares the hand-over of states
 // between CTAs; with fewer chains it would leave SMs empty.  FP16, by ticket and
-// walking: 8 x 4096 x 4096 262 and 251 us, 64 x 512 x 4096 277 and 214, 4 x 4096
-// x 2048 87 and 138, 1 x 16384 x 4096 172 and 488; backward 8 x 2048 x 4096 331
-// and 282, 4 x 2048 x 2048 114 and 158.  0.6 lies where the two meet: at 0.54
-// (16 x 2048 x 2560) forward 167 and 176, backward (16 x 1024 x 2560) 220 and 204.
+// walking: 8 x 4096 x 4096 265 and 257 us, 64 x 512 x 4096 277 and 220, 4 x 4096
+// x 2048 87 and 148, 1 x 16384 x 4096 173 and 520; backward 8 x 2048 x 4096 340
+// and 308, 4 x 2048 x 2048 107 and 171.  0.6 lies where the two meet: at 0.54
+// (16 x 2048 x 2560) forward 171 and 184, backward (16 x 1024 x 2560) 220 and 222.
 template <typename Sh>
 bool walks(const Plan &pl) {
     const int64_t slots = (int64_t)Sh::CTAS * device_sm_count(), chains = pl.ch.chains.d;
@@ -1437,8 +1439,8 @@ bool walks(const Plan &pl) {
 // where the hardware cannot describe it (the caller then takes the kernels
 // without tensor maps).  The outer dimension with the larger stride comes last.
 // Aligned tensors with tensor copies and with each thread's own: 8 x 4096 x 4096
-// FP16 246 and 549 us, backward 8 x 2048 x 4096 272 and 412, 8 x 2048 x 4096
-// FP32 186 and 309, backward 8 x 1024 x 4096 193 and 283.
+// FP16 257 and 560 us, backward 8 x 2048 x 4096 308 and 430, 8 x 2048 x 4096
+// FP32 189 and 310, backward 8 x 1024 x 4096 196 and 286.
 template <typename T>
 bool encode_tile(CUtensorMap *m, const void *ptr, const int64_t *s, int B, int L, int D, int chans, int tokens,
                  unsigned bit, unsigned &row_first) {

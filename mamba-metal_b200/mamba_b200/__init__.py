@@ -18,7 +18,13 @@ Reference interface mirrored (SNAPKITTYWEST/mamba-metal):
                    rmsnorm.metal)
 Without a counterpart in the reference: gated_recurrence (with its backward
 pass and single-token step), block_norm (with its backward pass),
-quantize_rows and linear_i8 (8-bit linear layer).
+quantize_rows and linear_i8 (8-bit linear layer).  They take stream= (a torch
+stream or handle of the tensors' device) besides the arguments listed, and
+run, allocate and fill on it; a caller that uses their results on another
+stream has to wait for it.
+
+No helper is an autograd function: results of tensors that require gradients
+are detached, and gradients come from the ..._backward helpers.
 """
 import ctypes
 import functools
