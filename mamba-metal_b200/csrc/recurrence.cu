@@ -31,7 +31,7 @@ namespace {
 // ---- gates ------------------------------------------------------------------
 // Two elements at a time in packed FP32 (one issue slot per pair and
 // operation); what is left per element are the special-function operations,
-// five forward and six backward.  Approximate exponentials, reciprocals and
+// five forward and seven backward (FP16 tensors eight).  Approximate exponentials, reciprocals and
 // roots have relative errors of 2^-22 or less.  PRECISE (FP32 tensors) adds
 // what their rounding needs: the exponent's product with log2(e) in two parts
 // and a longer series.  For FP16 tensors the rounding to 2^-11 hides both: in

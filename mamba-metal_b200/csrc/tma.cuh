@@ -64,10 +64,10 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity
 
 // A CTA whose threads all wait for the copies that thread 0 issues, over a few
 // places of shared memory in turn, and goes on after a wait that runs out, so
-// that its own barriers stay matched and nobody waits for it.  This word of
-// shared memory (0 to begin with) then says so: no thread waits again, thread 0 issues
-// no more copies, and gives those in flight a last chance to land (drain_copies,
-// at the end).  It costs no registers while nothing is lost.
+// that its own barriers stay matched and nobody waits for it.  These words of
+// shared memory (0 to begin with) then say so: no thread waits again, thread 0
+// issues no more copies, and gives those in flight a last chance to land
+// (drain_copies, at the end).  They cost no registers while nothing is lost.
 struct LostCopies {
     uint32_t flag;   // a wait ran out
     uint32_t place;  // 1 + 2 * the first place that thread 0 gave up + its parity
