@@ -110,7 +110,7 @@ const char *mamba_last_error(void);
  * Bit 6: a wait of mamba_gated_recurrence or its backward pass for the
  * sequence tile before it exceeded the same bound.  Bit 7: the same as bit 4
  * for mamba_linear_i8's tensor-core kernel.  Bit 8: the same for the row
- * fetches of mamba_block_norm and its backward pass.
+ * fetches of mamba_block_norm, mamba_layer_norm and their backward passes.
  * Waits for the device; clear != 0 resets them. */
 unsigned mamba_device_status(int clear);
 
@@ -503,6 +503,110 @@ int mamba_block_norm(const MambaBlockNormArgs *a, void *stream);
 size_t mamba_block_norm_workspace(const MambaBlockNormArgs *a);
 int mamba_block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *g, void *workspace,
                               size_t workspace_bytes, void *stream);
+
+/* Layer norm (no reference counterpart; rmsnorm.metal:11-81 is the reference's
+ * norm).  Per row:
+ *   out = (x - mean) * rstd * w + b,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+ * x [rows, cols] of x_dtype, out of out_dtype (MAMBA_F32 or MAMBA_F16 each,
+ * e.g. an FP32 residual stream into FP16), row strides in elements, channel
+ * stride 1; w, b [cols] and all sums FP32.  NULL: w (ones), b (zeros), mean,
+ * rstd (not kept).  out must not overlap x.  Rows of x (and of dout below) may
+ * be read as those of mamba_block_norm are: with the bytes around them.
+ * cols <= 16384. */
+typedef struct MambaLayerNormArgs {
+    const void *x;
+    const float *w;
+    const float *b;
+    void *out;   /* forward only */
+    float *mean; /* [rows]: forward written, backward read */
+    float *rstd; /* [rows]: the same */
+    int64_t rows;
+    int32_t cols, x_dtype, out_dtype;
+    float eps; /* forward only */
+    int64_t x_stride, out_stride;
+} MambaLayerNormArgs;
+
+/* Gradients of the layer norm: dout (out_dtype) is that of out.  Written: dx
+ * (x_dtype), dw and db [cols] FP32 (overwritten, the same bits on every call;
+ * NULL: not wanted).  Reads x, w, mean and rstd of `a`.  dx must not overlap x
+ * or dout. */
+typedef struct MambaLayerNormGrads {
+    const void *dout;
+    void *dx;
+    float *dw;
+    float *db;
+    int64_t dout_stride, dx_stride;
+} MambaLayerNormGrads;
+
+int mamba_layer_norm(const MambaLayerNormArgs *a, void *stream);
+/* Scratch bytes of the backward pass (0 for invalid args), 16-byte aligned
+ * device memory; calls that share it must not overlap on the GPU. */
+size_t mamba_layer_norm_workspace(const MambaLayerNormArgs *a);
+int mamba_layer_norm_backward(const MambaLayerNormArgs *a, const MambaLayerNormGrads *g, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
+/* Embedding lookup (no reference counterpart; it makes the FP32 rows that
+ * mamba_forward_device takes from token ids):
+ *   out[t, :] = scale * table[ids[t], :]
+ * rounded once to out_dtype.  ids [tokens] of 4 or 8 bytes (signed); an id
+ * outside [0, vocab) gives a row of zeros.  table [vocab, dim] of table_dtype
+ * and out [tokens, dim] of out_dtype (MAMBA_F32 or MAMBA_F16 each), row
+ * strides in elements, channel stride 1.  tokens <= 2^30, vocab < 2^31. */
+typedef struct MambaEmbeddingArgs {
+    const void *ids;
+    const void *table; /* lookup only */
+    void *out;         /* lookup only */
+    int64_t tokens, vocab;
+    int32_t dim, id_bytes, table_dtype, out_dtype;
+    float scale;
+    int64_t table_stride, out_stride;
+} MambaEmbeddingArgs;
+
+int mamba_embedding(const MambaEmbeddingArgs *a, void *stream);
+
+/* Gradient of the table:
+ *   dtable[v, :] = scale * sum over t with ids[t] = v of dout[t, :]
+ * FP32 [vocab, dim] with row stride dtable_stride, summed in FP32 in an order
+ * that depends on ids alone (the same bits on every call); rows whose id does
+ * not occur are zero.  accumulate != 0: the sums are added to dtable instead,
+ * and rows whose id does not occur are left as they were.  ids outside
+ * [0, vocab) contribute nothing.  dout [tokens, dim] of a->out_dtype with row
+ * stride dout_stride.  Workspace: 16-byte aligned device memory; calls that
+ * share it must not overlap on the GPU. */
+size_t mamba_embedding_workspace(const MambaEmbeddingArgs *a);
+int mamba_embedding_backward(const MambaEmbeddingArgs *a, const void *dout, int64_t dout_stride, float *dtable,
+                             int64_t dtable_stride, int accumulate, void *workspace, size_t workspace_bytes,
+                             void *stream);
+
+/* Dropout from a counter-based generator, with an optional residual add (no
+ * reference counterpart):
+ *   out[i] = [residual[i] +] (word(i) >= p 2^32 ? x[i] / (1 - p) : 0)
+ * for element i = row * cols + col, where word(i) is number i % 4 of the
+ * Philox4x32-10 block (Salmon et al., SC 2011) of counter words {i / 4 low,
+ * high, offset low, high} and key {seed low, high}, and p 2^32 is rounded to a
+ * whole number.  The mask depends on (seed, offset, i) alone, whatever the
+ * strides, and is never stored: the backward pass is the same call on the
+ * gradient, without the residual.  Give each call of a program its own offset.
+ * state: device memory holding {seed, offset} as two uint64, or NULL; with it
+ * the seed is state[0] and the offset state[1] + offset, read when the kernel
+ * runs, so that a captured graph draws new numbers when it is replayed.
+ * x [rows, cols] of x_dtype, residual FP32, out of out_dtype, row strides in
+ * elements, channel stride 1.  A dropped element does not look at x (NaN
+ * included).  out may be x (same type and stride) or residual (out FP32, same
+ * stride).  0 <= p <= 1; rows x cols <= 2^40. */
+typedef struct MambaDropoutArgs {
+    const void *x;
+    const float *residual;
+    void *out;
+    const uint64_t *state;
+    int64_t rows, cols;
+    uint64_t seed, offset;
+    int32_t x_dtype, out_dtype;
+    float p;
+    int64_t x_stride, residual_stride, out_stride;
+} MambaDropoutArgs;
+
+int mamba_dropout(const MambaDropoutArgs *a, void *stream);
 
 /* Exclusive propagation of per-tile affine carries: the job of
  * propagate_tile_carries_f32 (prefix_scan.metal:19-40), with the pair layout

@@ -13,13 +13,10 @@
 // where means are over the row and sums over the rows.
 #include "common.cuh"
 #include "internal.h"
+#include "rows.cuh"
 #include "scan_math.cuh"
-#include "tma.cuh"
 
 #include <algorithm>
-#include <mutex>
-#include <utility>
-#include <vector>
 
 namespace mb {
 
@@ -58,96 +55,6 @@ __device__ __forceinline__ void silu_grad(float z, float &g, float &dg) {
     dg = s * fmaf(z, om, 1.f);
 }
 
-constexpr int kMaxCols = 16384;
-constexpr int kDirectParts = 296;  // CTAs of the backward pass without a ring: few, so that their partial sums are
-
-// N consecutive elements as FP32; N = 8 by 16-byte accesses.
-template <int N>
-__device__ __forceinline__ void load_n(const float *p, float (&v)[N]) {
-    if constexpr (N == 1) {
-        v[0] = *p;
-    } else {
-#pragma unroll
-        for (int k = 0; k < N; k += 4) {
-            const float4 q = *reinterpret_cast<const float4 *>(p + k);
-            v[k] = q.x;
-            v[k + 1] = q.y;
-            v[k + 2] = q.z;
-            v[k + 3] = q.w;
-        }
-    }
-}
-template <int N>
-__device__ __forceinline__ void load_n(const __half *p, float (&v)[N]) {
-    if constexpr (N == 1) {
-        v[0] = __half2float(*p);
-    } else {
-        const uint4 raw = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
-            v[2 * k] = f.x;
-            v[2 * k + 1] = f.y;
-        }
-    }
-}
-template <int N>
-__device__ __forceinline__ void store_n(float *p, const float (&v)[N]) {
-    if constexpr (N == 1) {
-        *p = v[0];
-    } else {
-#pragma unroll
-        for (int k = 0; k < N; k += 4)
-            *reinterpret_cast<float4 *>(p + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-    }
-}
-template <int N>
-__device__ __forceinline__ void store_n(__half *p, const float (&v)[N]) {
-    if constexpr (N == 1) {
-        *p = __float2half_rn(v[0]);
-    } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
-            w[k] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-}
-template <int N>
-__device__ __forceinline__ void load_weight(const float *w, int c, float (&v)[N]) {
-    if (w) {
-        load_n(w + c, v);
-    } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = 1.f;
-    }
-}
-
-// Sum over the CTA, the same bits in every thread, and a barrier: what a thread
-// read from shared memory before it is read when any thread returns (shuffles
-// alone do not order memory).  `sm` holds two sets of 32 partials used in turn,
-// so one barrier per sum suffices: a set is overwritten only after the barrier
-// of the sum in between.
-__device__ __forceinline__ float block_sum(float v, float *sm, int &turn) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (blockDim.x == 32) {
-        __syncwarp();
-        return v;
-    }
-    float *s = sm + 32 * turn;
-    turn ^= 1;
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = (threadIdx.x & 31) < (blockDim.x >> 5) ? s[threadIdx.x & 31] : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
 // With many rows (RING): persistent CTAs whose rows arrive through shared
 // memory.  One thread fetches each row by untiled bulk copies (one per tensor)
 // into a ring of `stages` rows, that far ahead, so that loads stay in flight
@@ -156,77 +63,11 @@ __device__ __forceinline__ float block_sum(float v, float *sm, int &turn) {
 // row in registers.  Bound by bytes.  32768 x 2048 FP16, with the ring and
 // without: forward 162 and 182 us (5.8 and 5.2 TB/s), backward 289 and 324;
 // 16384 x 4096 164 and 205; unaligned 32768 x 2047 332 and 535.
-constexpr unsigned kErrBlockNormTimeout = 256u;
-constexpr int kMaxStages = 4;
-constexpr int kRingBytes = 224 * 1024;                    // shared memory of an SM, with room for the static parts
 // Resident threads per SM.  32768 x 2048 FP16: forward 160 us, with 768 threads
 // 180, with 1280 207 (57 registers a thread, they no longer fit); backward 276,
 // with 512 336.
 constexpr int kRingThreads = 1024, kRingBwdThreads = 768;
 
-template <int N>
-struct RingRow {
-    const void *src[N];  // first row of each tensor
-    int64_t stride[N];   // bytes between rows
-    uint32_t bytes[N];   // bytes of a row, 0: tensor absent
-    uint32_t offset[N];  // within a stage
-    uint32_t stage;      // bytes of a stage
-    int stages;
-    // Bulk copies start and end on 16-byte boundaries: a row that does not is
-    // copied with the bytes around it (of its neighbours, or in the 16 bytes of
-    // memory that its first or last byte lies in) and starts this far behind
-    // its place.
-    __device__ __forceinline__ uint32_t shift(int k, int64_t row) const {
-        return (uint32_t)(reinterpret_cast<uintptr_t>(src[k]) + row * stride[k]) & 15u;
-    }
-};
-
-template <int N>
-__device__ __forceinline__ void fetch_row(const RingRow<N> &r, uint8_t *ring, uint64_t *full, int64_t row, int s) {
-    uint32_t bytes[N], total = 0;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        bytes[k] = r.bytes[k] ? (r.shift(k, row) + r.bytes[k] + 15) / 16 * 16 : 0;
-        total += bytes[k];
-    }
-    mbar_arrive_expect_tx(&full[s], total);
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-        if (bytes[k])
-            bulk_load(ring + s * r.stage + r.offset[k],
-                      static_cast<const uint8_t *>(r.src[k]) + row * r.stride[k] - r.shift(k, row), bytes[k], &full[s]);
-}
-// Place s of the ring in use, and the parity of that use.
-struct RingPlace {
-    int s = 0;
-    uint32_t parity = 0;
-    __device__ __forceinline__ void step(int stages) {
-        if (++s == stages) {
-            s = 0;
-            parity ^= 1;
-        }
-    }
-};
-// Waits for the row at a place.  A wait that runs out is reported; the CTA goes
-// on, with wrong values.
-constexpr uint64_t kWaitNs = 2000000000ull;
-__device__ __forceinline__ void await_row(uint64_t *full, const RingPlace &at, LostCopies *lost,
-                                          uint64_t limit_ns = kWaitNs) {
-    if (!await_copy(full, at.s, at.parity, lost, limit_ns)) atomicOr(&g_block_norm_error, kErrBlockNormTimeout);
-}
-// Sets the ring up and fetches the first rows; rows first, first + step, ...
-template <int N>
-__device__ __forceinline__ void start_ring(const RingRow<N> &r, uint8_t *ring, uint64_t *full, LostCopies *lost,
-                                           int64_t rows) {
-    if (threadIdx.x == 0) {
-        *lost = LostCopies{};
-        for (int s = 0; s < r.stages; ++s) mbar_init(&full[s], 1);
-        fence_mbar_init();
-        int64_t row = blockIdx.x;
-        for (int s = 0; s < r.stages && row < rows; ++s, row += gridDim.x) fetch_row<N>(r, ring, full, row, s);
-    }
-    __syncthreads();
-}
 
 // One CTA per row, the row in registers: thread t holds NV groups of VEC
 // channels, group j at channel (j * threads + t) * VEC.
@@ -247,7 +88,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_kernel(const NormParams
         const T *y = RING ? reinterpret_cast<const T *>(at_place(0)) : static_cast<const T *>(p.y) + row * p.sy;
         const T *z = RING ? reinterpret_cast<const T *>(at_place(1)) : static_cast<const T *>(p.z) + row * p.sz;
         const float *res = RING ? reinterpret_cast<const float *>(at_place(2)) : p.res + row * p.cols;
-        if (RING) await_row(full, at, &lost);
+        if (RING) await_row(full, at, &lost, &g_block_norm_error);
         float v[NV][VEC], gz[NV][VEC], r[NV][VEC];
         float ss = 0.f;
 #pragma unroll
@@ -339,7 +180,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_bwd_kernel(const NormGr
             rs_next = p.f.rstd_post[after];
             if (first) rp_next = p.f.rstd_pre[after];
         }
-        if (RING) await_row(full, at, &lost);
+        if (RING) await_row(full, at, &lost, &g_block_norm_error);
         float R[NV][VEC], n[NV][VEC], gz[NV][VEC], d[NV][VEC], m[NV][VEC];
         float dot = 0.f;
 #pragma unroll
@@ -432,32 +273,6 @@ __global__ void __launch_bounds__(MAXT, CTAS) block_norm_bwd_kernel(const NormGr
     if (RING) drain_copies(full, ring.stages, &lost, kWaitNs);
 }
 
-// Column sums of the partial rows, in a fixed order: warp w of a CTA adds
-// rows w, w + 8, ... of 32 columns, then the warps' sums are added in order.
-// blockIdx.y: 0 = dw_post, 1 = dw_pre.
-constexpr int kSumThreads = 256;
-__global__ void __launch_bounds__(kSumThreads)
-    block_norm_sum_kernel(const float *__restrict__ part_post, const float *__restrict__ part_pre,
-                          float *__restrict__ dw_post, float *__restrict__ dw_pre, int parts, int cols) {
-    __shared__ float sm[kSumThreads / 32][32];
-    const float *part = blockIdx.y ? part_pre : part_post;
-    float *dw = blockIdx.y ? dw_pre : dw_post;
-    if (!dw) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-    float s = 0.f;
-    if (c < cols)
-        for (int k = warp; k < parts; k += kSumThreads / 32) s += part[(int64_t)k * cols + c];
-    sm[warp][lane] = s;
-    __syncthreads();
-    if (warp == 0 && c < cols) {
-#pragma unroll
-        for (int k = 1; k < kSumThreads / 32; ++k) s += sm[k][lane];
-        dw[c] = s;
-    }
-}
-
-bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
 int check_args(const MambaBlockNormArgs *a, const char *what) {
     MB_CHECK_ARG(a, std::string(what) + ": null args");
     MB_CHECK_ARG(a->rows >= 0 && a->cols >= 0, std::string(what) + ": negative size");
@@ -503,48 +318,10 @@ bool vector_rows(const MambaBlockNormArgs *a) {
            aligned_to(a->w_pre, 16) && (a->y_stride * es) % 16 == 0 && (!a->z || (a->z_stride * es) % 16 == 0);
 }
 
-int threads_for(int cols, int per_thread) { return std::max(32, (ceil_div(cols, per_thread) + 31) / 32 * 32); }
-
-// Opts a kernel into the shared memory of its ring, once per device.
-template <typename Kernel>
-int allow_smem(Kernel kernel) {
-    static std::mutex mu;
-    static std::vector<std::pair<const void *, int>> done;
-    int dev = 0;
-    MB_CUDA_TRY(cudaGetDevice(&dev));
-    const std::pair<const void *, int> key(reinterpret_cast<const void *>(kernel), dev);
-    std::lock_guard<std::mutex> lk(mu);
-    if (std::find(done.begin(), done.end(), key) != done.end()) return 0;
-    MB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes));
-    done.push_back(key);
-    return 0;
-}
-
-// CTAs per SM that a ring kernel wants.
-int ring_ctas(int threads, int resident) { return std::max(1, std::min(32, resident / threads)); }
 // Rows of partial column sums of the backward pass at most.
 int64_t max_parts(int64_t rows, int cols) {
     const int ctas = std::min(16, ring_ctas(threads_for(cols, cols <= 4096 ? 8 : 16), kRingBwdThreads));
     return std::min<int64_t>(rows, std::max(kDirectParts, 148 * ctas));
-}
-
-// Lays a ring out and lowers the CTAs per SM until each has room for two rows
-// (one, if at most two CTAs share the SM).  False where a row is larger than that, or
-// where CTAs would get too few rows for a ring to pay: with one or two nothing
-// is ahead.  Asking for 2, 3 or 6 rows a CTA measures the same.
-template <int N>
-bool plan_ring(RingRow<N> &r, int64_t rows, int &ctas_per_sm) {
-    uint32_t at = 0;
-    for (int k = 0; k < N; ++k) {
-        r.offset[k] = at;
-        if (r.bytes[k]) at += (r.bytes[k] + 30 + 127) / 128 * 128;  // and what surrounds an unaligned row
-    }
-    r.stage = at;
-    for (;; --ctas_per_sm) {
-        r.stages = (int)std::min<uint32_t>(kMaxStages, (uint32_t)(kRingBytes / ctas_per_sm - 2048) / std::max(at, 1u));
-        if (r.stages >= 2 || (r.stages == 1 && ctas_per_sm == 2) || ctas_per_sm == 1) break;
-    }
-    return r.stages >= 1 && rows >= 3LL * ctas_per_sm * device_sm_count();
 }
 
 template <typename T, int VEC, int NV, int MAXT>
@@ -709,7 +486,7 @@ int block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *
                      (g->dy_stride * (int64_t)es) % 16 == 0 && (!a->z || (g->dz_stride * (int64_t)es) % 16 == 0);
     if (a->dtype == MAMBA_F16 ? launch_bwd<__half>(p, vec, grid, st) : launch_bwd<float>(p, vec, grid, st)) return -1;
     if (!g->dw_post && !g->dw_pre) return 0;
-    block_norm_sum_kernel<<<dim3((unsigned)ceil_div(a->cols, 32), 2), kSumThreads, 0, st>>>(
+    column_sum_kernel<<<dim3((unsigned)ceil_div(a->cols, 32), 2), kSumThreads, 0, st>>>(
         p.part_post, p.part_pre, g->dw_post, g->dw_pre, (int)grid, a->cols);
     return launch_status("block_norm_backward sum kernel");
 }
@@ -725,9 +502,9 @@ __global__ void block_norm_wait_selftest_kernel(uint64_t limit_ns) {
     for (int s = 0; s < 2; ++s) mbar_init(&full[s], 1);
     fence_mbar_init();
     RingPlace at;
-    await_row(full, at, &lost, limit_ns);
+    await_row(full, at, &lost, &g_block_norm_error, limit_ns);
     at.step(2);
-    await_row(full, at, &lost, limit_ns);  // at once
+    await_row(full, at, &lost, &g_block_norm_error, limit_ns);  // at once
     drain_copies(full, 2, &lost, limit_ns);
 }
 

@@ -68,6 +68,22 @@ int block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *
 unsigned block_norm_error_flags(bool clear);
 int block_norm_wait_selftest(uint64_t limit_ns, cudaStream_t st);
 
+// layer_norm.cu
+size_t layer_norm_workspace_bytes(const MambaLayerNormArgs *a);
+int layer_norm(const MambaLayerNormArgs *a, cudaStream_t st);
+int layer_norm_backward(const MambaLayerNormArgs *a, const MambaLayerNormGrads *g, void *ws, size_t ws_bytes,
+                        cudaStream_t st);
+unsigned layer_norm_error_flags(bool clear);
+
+// embedding.cu
+int embedding(const MambaEmbeddingArgs *a, cudaStream_t st);
+size_t embedding_workspace_bytes(const MambaEmbeddingArgs *a);
+int embedding_backward(const MambaEmbeddingArgs *a, const void *dout, int64_t dout_stride, float *dtable,
+                       int64_t dtable_stride, int accumulate, void *ws, size_t ws_bytes, cudaStream_t st);
+
+// dropout.cu
+int dropout(const MambaDropoutArgs *a, cudaStream_t st);
+
 // ssm_step.cu
 int ssm_step(const void *x, int64_t xrs, const void *delta, int64_t drs, const float *dt_bias,
              const void *B, const void *C, int64_t bcrs, const float *A, const float *Dskip,

@@ -1267,10 +1267,11 @@ unsigned mamba_device_status(int clear) {
     const unsigned rec = mb::recurrence_error_flags(clear != 0);
     const unsigned i8 = mb::linear_i8_error_flags(clear != 0);
     const unsigned norm = mb::block_norm_error_flags(clear != 0);
+    const unsigned ln = mb::layer_norm_error_flags(clear != 0);
     return (scan == ~0u || gemm == ~0u || lin == ~0u || proj == ~0u || step == ~0u || rec == ~0u || i8 == ~0u ||
-            norm == ~0u)
+            norm == ~0u || ln == ~0u)
                ? ~0u
-               : (scan | gemm | lin | proj | step | rec | i8 | norm);
+               : (scan | gemm | lin | proj | step | rec | i8 | norm | ln);
 }
 
 int mamba_selftest_bounded_wait(unsigned limit_us, void *stream) {
@@ -1538,6 +1539,42 @@ int mamba_block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormG
     mb::clear_error();
     return guarded(
         [&] { return mb::block_norm_backward(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)); });
+}
+
+int mamba_layer_norm(const MambaLayerNormArgs *a, void *stream) {
+    mb::clear_error();
+    return guarded([&] { return mb::layer_norm(a, static_cast<cudaStream_t>(stream)); });
+}
+
+size_t mamba_layer_norm_workspace(const MambaLayerNormArgs *a) { return mb::layer_norm_workspace_bytes(a); }
+
+int mamba_layer_norm_backward(const MambaLayerNormArgs *a, const MambaLayerNormGrads *g, void *workspace,
+                              size_t workspace_bytes, void *stream) {
+    mb::clear_error();
+    return guarded(
+        [&] { return mb::layer_norm_backward(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)); });
+}
+
+int mamba_embedding(const MambaEmbeddingArgs *a, void *stream) {
+    mb::clear_error();
+    return guarded([&] { return mb::embedding(a, static_cast<cudaStream_t>(stream)); });
+}
+
+size_t mamba_embedding_workspace(const MambaEmbeddingArgs *a) { return mb::embedding_workspace_bytes(a); }
+
+int mamba_embedding_backward(const MambaEmbeddingArgs *a, const void *dout, int64_t dout_stride, float *dtable,
+                             int64_t dtable_stride, int accumulate, void *workspace, size_t workspace_bytes,
+                             void *stream) {
+    mb::clear_error();
+    return guarded([&] {
+        return mb::embedding_backward(a, dout, dout_stride, dtable, dtable_stride, accumulate, workspace,
+                                      workspace_bytes, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int mamba_dropout(const MambaDropoutArgs *a, void *stream) {
+    mb::clear_error();
+    return guarded([&] { return mb::dropout(a, static_cast<cudaStream_t>(stream)); });
 }
 
 int mamba_propagate_tile_carries(float *carries, int num_tiles, int64_t width, float *total, void *stream) {

@@ -108,6 +108,30 @@ class MambaBlockNormGrads(ctypes.Structure):
                 ("dz_stride", c_i64)]
 
 
+class MambaLayerNormArgs(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("w", c_void_p), ("b", c_void_p), ("out", c_void_p), ("mean", c_void_p),
+                ("rstd", c_void_p), ("rows", c_i64), ("cols", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32), ("eps", c_float), ("x_stride", c_i64), ("out_stride", c_i64)]
+
+
+class MambaLayerNormGrads(ctypes.Structure):
+    _fields_ = [("dout", c_void_p), ("dx", c_void_p), ("dw", c_void_p), ("db", c_void_p), ("dout_stride", c_i64),
+                ("dx_stride", c_i64)]
+
+
+class MambaEmbeddingArgs(ctypes.Structure):
+    _fields_ = [("ids", c_void_p), ("table", c_void_p), ("out", c_void_p), ("tokens", c_i64), ("vocab", c_i64),
+                ("dim", ctypes.c_int32), ("id_bytes", ctypes.c_int32), ("table_dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32), ("scale", c_float), ("table_stride", c_i64), ("out_stride", c_i64)]
+
+
+class MambaDropoutArgs(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("residual", c_void_p), ("out", c_void_p), ("state", c_void_p), ("rows", c_i64),
+                ("cols", c_i64), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("x_dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32), ("p", c_float), ("x_stride", c_i64), ("residual_stride", c_i64),
+                ("out_stride", c_i64)]
+
+
 # Every symbol include/mamba.h declares, with its ctypes prototype.
 _PROTOTYPES = {
     "mamba_create": (c_void_p, [ctypes.POINTER(MambaConfig)]),
@@ -169,6 +193,15 @@ _PROTOTYPES = {
     "mamba_block_norm_workspace": (c_size, [ctypes.POINTER(MambaBlockNormArgs)]),
     "mamba_block_norm_backward": (c_int, [ctypes.POINTER(MambaBlockNormArgs), ctypes.POINTER(MambaBlockNormGrads),
                                           c_void_p, c_size, c_void_p]),
+    "mamba_layer_norm": (c_int, [ctypes.POINTER(MambaLayerNormArgs), c_void_p]),
+    "mamba_layer_norm_workspace": (c_size, [ctypes.POINTER(MambaLayerNormArgs)]),
+    "mamba_layer_norm_backward": (c_int, [ctypes.POINTER(MambaLayerNormArgs), ctypes.POINTER(MambaLayerNormGrads),
+                                          c_void_p, c_size, c_void_p]),
+    "mamba_embedding": (c_int, [ctypes.POINTER(MambaEmbeddingArgs), c_void_p]),
+    "mamba_embedding_workspace": (c_size, [ctypes.POINTER(MambaEmbeddingArgs)]),
+    "mamba_embedding_backward": (c_int, [ctypes.POINTER(MambaEmbeddingArgs), c_void_p, c_i64, c_void_p, c_i64, c_int,
+                                         c_void_p, c_size, c_void_p]),
+    "mamba_dropout": (c_int, [ctypes.POINTER(MambaDropoutArgs), c_void_p]),
     "mamba_propagate_tile_carries": (c_int, [c_void_p, c_int, c_i64, c_void_p, c_void_p]),
     "mamba_gated_silu_mul": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, c_void_p]),
     "mamba_gated_mlp_up": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, c_int, c_void_p]),
@@ -709,6 +742,10 @@ _RECURRENCE_ARGS = struct.Struct("@9P4if4x8q")
 _RECURRENCE_GRADS = struct.Struct("@7P8q")
 _BLOCK_NORM_ARGS = struct.Struct("@9Pq2i2f2q")
 _BLOCK_NORM_GRADS = struct.Struct("@7P2q")
+_LAYER_NORM_ARGS = struct.Struct("@6Pq3if2q")
+_LAYER_NORM_GRADS = struct.Struct("@4P2q")
+_EMBEDDING_ARGS = struct.Struct("@3P2q4if4x2q")
+_DROPOUT_ARGS = struct.Struct("@4P2q2Q2if4x3q")
 
 
 def _ptr0(t):
@@ -721,6 +758,8 @@ def _packed(what, cls, fmt, *values):
         return cls.from_buffer_copy(fmt.pack(*values))
     except struct.error:
         raise MambaError("%s: a size does not fit 32 bits" % what) from None
+    except OverflowError:
+        raise MambaError("%s: a number does not fit FP32" % what) from None
 
 
 def _require_int32(what, *sizes):
@@ -964,6 +1003,188 @@ def block_norm_backward(dresidual_out, dout, y, residual_out, rstd_post, rstd_pr
     ws, ws_len, owner = _workspace(what, lib().mamba_block_norm_workspace(a), workspace, y)
     _call(lib().mamba_block_norm_backward, what, y, a, g, ws, ws_len)
     return dy, dresidual, dw_post, dw_pre, dz
+
+
+def _float_dtype(dtype, name, what):
+    """The library's number of a torch dtype."""
+    torch = _torch()
+    if dtype is torch.float16:
+        return F16
+    if dtype is torch.float32:
+        return F32
+    raise MambaError("%s: %s must be float16 or float32" % (what, name))
+
+
+def _output(out, name, what, shape, dtype, like, strided=True):
+    """The caller's output after its checks, or a fresh one."""
+    if out is None:
+        return like.new_empty(shape, dtype=dtype)
+    _check_tensor(out, name, what, shape, dtype, like.device, strided)
+    return out
+
+
+def _layer_norm_args(what, x, w, b, mean, rstd, out_dtype, eps, out=None):
+    torch = _torch()
+    _require(x.dim() == 2, "%s: x must be [rows, cols]" % what)
+    x_dt = _float_dtype(x.dtype, "x", what)
+    shape, dev = x.shape, x.device
+    _check_tensor(x, "x", what, shape, x.dtype, dev, True)
+    if w is not None:
+        _check_tensor(w, "w", what, shape[1:], torch.float32, dev)
+    if b is not None:
+        _check_tensor(b, "b", what, shape[1:], torch.float32, dev)
+    return _packed(what, MambaLayerNormArgs, _LAYER_NORM_ARGS, x.data_ptr(), _ptr0(w), _ptr0(b), _ptr0(out),
+                   _ptr0(mean), _ptr0(rstd), shape[0], shape[1], x_dt, _float_dtype(out_dtype, "out", what), eps,
+                   x.stride(0), 0 if out is None else out.stride(0))
+
+
+@_on_stream
+def layer_norm(x, w=None, b=None, eps=1e-5, out_dtype=None, return_stats=False, out=None):
+    """Layer norm (mamba_layer_norm): (x - mean) * rstd * w + b over the rows
+    of x [rows, cols], F16 or F32 (row stride any, channel stride 1); w, b
+    FP32 [cols] or None; the result in out_dtype (default: x's).  Returns out,
+    and with return_stats also the FP32 [rows] mean and rstd that
+    layer_norm_backward reads."""
+    what = "mamba_layer_norm"
+    _require(x.dim() == 2, "%s: x must be [rows, cols]" % what)
+    if out_dtype is None:
+        out_dtype = x.dtype if out is None else out.dtype
+    _float_dtype(out_dtype, "out", what)
+    out = _output(out, "out", what, x.shape, out_dtype, x)
+    mean = rstd = None
+    if return_stats:
+        mean, rstd = x.new_empty((2, x.shape[0]), dtype=_torch().float32).unbind(0)
+    a = _layer_norm_args(what, x, w, b, mean, rstd, out_dtype, eps, out)
+    _call(lib().mamba_layer_norm, what, x, a)
+    return (out, mean, rstd) if return_stats else out
+
+
+@_on_stream
+def layer_norm_backward(dout, x, mean, rstd, w=None, dx=None, workspace=None):
+    """Gradients of layer_norm (mamba_layer_norm_backward): dout [rows, cols]
+    F16 or F32 is the gradient of its output, mean and rstd what it returned.
+    Returns (dx, dw, db): dx in x's dtype, the sums dw and db FP32 [cols]."""
+    torch = _torch()
+    what = "mamba_layer_norm_backward"
+    _check_tensor(dout, "dout", what, x.shape, dout.dtype, x.device, True)
+    _check_tensor(mean, "mean", what, x.shape[:1], torch.float32, x.device)
+    _check_tensor(rstd, "rstd", what, x.shape[:1], torch.float32, x.device)
+    a = _layer_norm_args(what, x, w, None, mean, rstd, dout.dtype, 1.0)  # eps is inside rstd
+    dx = _output(dx, "dx", what, x.shape, x.dtype, x)
+    dw, db = mean.new_empty((2, x.shape[1])).unbind(0)
+    g = _packed(what, MambaLayerNormGrads, _LAYER_NORM_GRADS, dout.data_ptr(), dx.data_ptr(), dw.data_ptr(),
+                db.data_ptr(), dout.stride(0), dx.stride(0))
+    ws, ws_len, owner = _workspace(what, lib().mamba_layer_norm_workspace(a), workspace, x)
+    _call(lib().mamba_layer_norm_backward, what, x, a, g, ws, ws_len)
+    return dx, dw, db
+
+
+def _embedding_args(what, tokens, vocab, dim, table_dtype, out_dtype, scale, table=None, out=None):
+    torch = _torch()
+    _require(tokens.dtype is torch.int32 or tokens.dtype is torch.int64, "%s: tokens must be int32 or int64" % what)
+    _require(tokens.is_contiguous(), "%s: tokens must be contiguous" % what)
+    return _packed(what, MambaEmbeddingArgs, _EMBEDDING_ARGS, tokens.data_ptr(), _ptr0(table), _ptr0(out),
+                   tokens.numel(), vocab, dim, tokens.element_size(), table_dtype, out_dtype, scale,
+                   0 if table is None else table.stride(0), 0 if out is None else out.stride(-2))
+
+
+@_on_stream
+def embedding(tokens, table, scale=1.0, out_dtype=None, out=None):
+    """Embedding lookup (mamba_embedding): scale * table[tokens] in out_dtype
+    (default: the table's); ids outside the table give rows of zeros.
+
+    tokens: int32 or int64, any shape, contiguous; table [vocab, dim] F16 or
+    F32 (row stride any, channel stride 1).  Returns [*tokens.shape, dim]; an
+    `out` of that shape must be contiguous, or [tokens, dim] rows of any
+    stride."""
+    what = "mamba_embedding"
+    _require(table.dim() == 2, "%s: table must be [vocab, dim]" % what)
+    t_dt = _float_dtype(table.dtype, "table", what)
+    _check_tensor(table, "table", what, table.shape, table.dtype, tokens.device, True)
+    vocab, dim = table.shape
+    if out_dtype is None:
+        out_dtype = table.dtype if out is None else out.dtype
+    o_dt = _float_dtype(out_dtype, "out", what)
+    shape = tuple(tokens.shape) + (dim,)
+    rows = _output(out, "out", what, shape, out_dtype, table, len(shape) == 2)
+    a = _embedding_args(what, tokens, vocab, dim, t_dt, o_dt, scale, table,
+                        rows if len(shape) == 2 else rows.view(-1, dim) if dim else rows.new_empty((0, 0)))
+    _call(lib().mamba_embedding, what, table, a)
+    return rows
+
+
+@_on_stream
+def embedding_backward(dout, tokens, vocab, scale=1.0, dtable=None, accumulate=False, workspace=None):
+    """Gradient of embedding's table (mamba_embedding_backward): dtable[v] =
+    scale * the sum of dout's rows whose token is v, FP32 [vocab, dim].
+
+    dout: [*tokens.shape, dim] F16 or F32, contiguous (or [tokens, dim] rows
+    of any stride).  accumulate: adds to a given dtable, whose other rows stay
+    as they are; otherwise they become zero."""
+    torch = _torch()
+    what = "mamba_embedding_backward"
+    o_dt = _float_dtype(dout.dtype, "dout", what)
+    _require(dout.dim() >= 1, "%s: dout must be [*tokens.shape, dim]" % what)
+    dim = dout.shape[-1]
+    _check_tensor(dout, "dout", what, tuple(tokens.shape) + (dim,), dout.dtype, tokens.device, dout.dim() == 2)
+    if dtable is None:
+        _require(not accumulate, "%s: accumulate adds into a given dtable" % what)
+        dtable = dout.new_empty((vocab, dim), dtype=torch.float32)
+    else:
+        _check_tensor(dtable, "dtable", what, (vocab, dim), torch.float32, dout.device, True)
+    a = _embedding_args(what, tokens, vocab, dim, F32, o_dt, scale)
+    ws, ws_len, owner = _workspace(what, lib().mamba_embedding_workspace(a), workspace, dout)
+    _call(lib().mamba_embedding_backward, what, dout, a, dout.data_ptr(), dout.stride(0) if dout.dim() == 2 else dim,
+          dtable.data_ptr(), dtable.stride(0), int(bool(accumulate)), ws, ws_len)
+    return dtable
+
+
+def _dropout(what, x, p, seed, offset, residual, out_dtype, out, state):
+    torch = _torch()
+    x_dt = _float_dtype(x.dtype, "x", what)
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else x.dtype if residual is None else torch.float32
+    o_dt = _float_dtype(out_dtype, "out", what)
+    shape, dev, rows2 = x.shape, x.device, x.dim() == 2
+    _check_tensor(x, "x", what, shape, x.dtype, dev, rows2)
+    if residual is not None:
+        _check_tensor(residual, "residual", what, shape, torch.float32, dev, rows2)
+    if state is not None:
+        _check_tensor(state, "state", what, (2,), torch.int64, dev)
+    _require(0 <= seed < 1 << 64 and 0 <= offset < 1 << 64, "%s: seed and offset must fit 64 bits" % what)
+    out = _output(out, "out", what, shape, out_dtype, x, rows2)
+    if rows2:
+        rows, cols = shape
+        sx, sr, so = x.stride(0), 0 if residual is None else residual.stride(0), out.stride(0)
+    else:
+        rows, cols = 1, x.numel()
+        sx = sr = so = cols
+    a = _packed(what, MambaDropoutArgs, _DROPOUT_ARGS, x.data_ptr(), _ptr0(residual), out.data_ptr(), _ptr0(state),
+                rows, cols, seed, offset, x_dt, o_dt, p, sx, sr, so)
+    _call(lib().mamba_dropout, what, x, a)
+    return out
+
+
+@_on_stream
+def dropout(x, p, seed=0, offset=0, residual=None, out_dtype=None, out=None, state=None):
+    """Dropout (mamba_dropout): [residual +] x / (1 - p) where a number drawn
+    for the element keeps it, else [residual +] 0.  The numbers are those of a
+    counter-based generator for (seed, offset, element): the same mask on
+    every call with these, never stored.
+
+    x: F16 or F32, contiguous of any shape, or [rows, cols] with rows of any
+    stride; residual FP32 of x's shape; out_dtype: x's, or F32 with a
+    residual.  out may be x or the residual.  state: int64 [2] CUDA tensor of
+    (seed, offset to add), read when the kernel runs (for captured graphs)."""
+    return _dropout("mamba_dropout", x, p, seed, offset, residual, out_dtype, out, state)
+
+
+@_on_stream
+def dropout_backward(dout, p, seed=0, offset=0, out_dtype=None, dx=None, state=None):
+    """Gradient of dropout's x: dout / (1 - p) where the forward call with this
+    p, seed, offset and state kept the element, else 0, in out_dtype (default:
+    dout's).  The residual's gradient is dout itself."""
+    return _dropout("mamba_dropout", dout, p, seed, offset, None, out_dtype, dx, state)
 
 
 def propagate_tile_carries(carries, total=None, stream=None):
