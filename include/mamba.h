@@ -251,6 +251,43 @@ size_t mamba_selective_scan_workspace(const MambaScanArgs *a);
 int mamba_selective_scan(const MambaScanArgs *a, void *workspace, size_t workspace_bytes,
                          void *stream);
 
+/* Gradients of the selective scan (of mamba_selective_scan with the same
+ * args; selective_scan_cpu.cpp:17-41).  The call reads x, delta, B, C, A, D,
+ * z, dt_bias and initial_state of `a` (not y, final_state or chunk_len; states
+ * and intermediate values are computed again).  dy: gradient of y (x's dtype);
+ * dfinal_state [batch, dim, dstate] FP32: gradient of the final state or NULL
+ * (zeros).  Written: dx, dz (x's dtype; dz only with a gate), ddelta (delta's
+ * dtype), dB and dC (the dtype of B and C, sums over channels rounded once),
+ * and FP32: dA [dim, dstate], dD and ddt_bias [dim] (sums over batch and time)
+ * and dinitial_state [batch, dim, dstate].  NULL: dB, dC, dA, dD, ddt_bias,
+ * dinitial_state (not wanted).  All sums are FP32 in a fixed order: the same
+ * bits on every call.  Strides in elements {batch, time, channel} ({batch,
+ * time, state} for dB and dC).  FP16 tensors: exponentials and reciprocals are
+ * approximate (2e-6).  Where |A| <= 1e-6 the gradients are those of the
+ * zero-order hold's limit.  States 16-byte aligned.  Outputs must not overlap
+ * inputs or each other.  batch * seqlen * ceil(dim / 128) <= 2^31. */
+typedef struct MambaScanGrads {
+    const void *dy;
+    const float *dfinal_state;
+    void *dx;
+    void *ddelta;
+    void *dz;
+    void *dB;
+    void *dC;
+    float *dA;
+    float *dD;
+    float *ddt_bias;
+    float *dinitial_state;
+    int64_t dy_stride[3], dx_stride[3], ddelta_stride[3], dz_stride[3], dB_stride[3], dC_stride[3];
+} MambaScanGrads;
+
+/* Scratch bytes of the call (0 for invalid args): 16-byte aligned device
+ * memory, about 8 bytes per token and channel (a state of 16 FP32 numbers
+ * every 8 tokens).  Calls that share it must not overlap on the GPU. */
+size_t mamba_selective_scan_backward_workspace(const MambaScanArgs *a);
+int mamba_selective_scan_backward(const MambaScanArgs *a, const MambaScanGrads *g, void *workspace,
+                                  size_t workspace_bytes, void *stream);
+
 /* The fused selective scan with the layer's dt_proj computed inside it
  * (linear_f16 of projection.metal:32-49 for dt_proj, MambaRuntime.cpp:98,
  * folded into selective_scan.metal:84-244): delta = dt_r @ w_dt^T with FP32
@@ -353,6 +390,26 @@ int mamba_causal_conv1d_step(const void *x_t, int64_t x_row_stride, const float 
                              const float *bias, void *y_t, int64_t y_row_stride,
                              float *conv_state, int batch, int dim, int K, int silu,
                              int dtype, void *stream);
+
+/* Gradients of the depthwise causal conv (of mamba_causal_conv1d with these x,
+ * w, bias and silu).  dy, x and dx share `dtype`; strides {batch, time,
+ * channel}; w [dim, K] and bias [dim] (or NULL) FP32, K in 1..8.  Written: dx,
+ * and FP32 dw [dim, K] and dbias [dim] (sums over batch and time in a fixed
+ * order; NULL: not wanted).  dx must not overlap dy or x.  Workspace: 16-byte
+ * aligned device memory; calls that share it must not overlap on the GPU. */
+typedef struct MambaConvGradArgs {
+    const void *dy;
+    const void *x;
+    const float *w;
+    const float *bias;
+    void *dx;
+    float *dw;
+    float *dbias;
+    int32_t batch, seqlen, dim, K, silu, dtype;
+    int64_t dy_stride[3], x_stride[3], dx_stride[3];
+} MambaConvGradArgs;
+size_t mamba_causal_conv1d_backward_workspace(const MambaConvGradArgs *a);
+int mamba_causal_conv1d_backward(const MambaConvGradArgs *a, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Single-token SSM update (state_update.metal:15-57, softplus always
  * applied as in selective_scan_cpu.cpp:20), with optional dt_bias and

@@ -44,17 +44,6 @@ struct NormGradParams {
     int64_t sdy, sdz;
 };
 
-// SiLU(z) and its derivative.  FP16 tensors: one approximate exponential and
-// reciprocal (relative error ~2^-22, far below FP16's 2^-11).
-template <bool PRECISE>
-__device__ __forceinline__ void silu_grad(float z, float &g, float &dg) {
-    const float e = PRECISE ? expf(-fabsf(z)) : ex2_approx(-fabsf(z) * kLog2e);
-    const float t = PRECISE ? __fdiv_rn(1.f, 1.f + e) : rcp_approx(1.f + e), u = e * t;
-    const float s = z >= 0.f ? t : u, om = z >= 0.f ? u : t;
-    g = z * s;
-    dg = s * fmaf(z, om, 1.f);
-}
-
 // With many rows (RING): persistent CTAs whose rows arrive through shared
 // memory.  One thread fetches each row by untiled bulk copies (one per tensor)
 // into a ring of `stages` rows, that far ahead, so that loads stay in flight

@@ -1,0 +1,300 @@
+// conv_bwd.cu -- gradients of the depthwise causal conv of conv.cu
+// (Sources/Kernels/causal_conv1d.metal:21-45 with the SiLU of
+// MambaRuntime.cpp:96).  With pre_t = sum_k w_k x_{t-K+1+k} + bias and
+// p_t = dy_t SiLU'(pre_t) (dy_t without the activation):
+//   dx_t = sum_k w_k p_{t+K-1-k},  dw_k = sum_t p_t x_{t-K+1+k},  dbias = sum_t p_t
+//
+// Bound by bytes: one pass over x and dy that writes dx.  A thread owns VEC
+// channels and a run of timesteps; the last K inputs and the last K p_t stay in
+// registers, so a run reads K - 1 rows before it (of x) and behind it (of
+// both) again.  The sums of dw and dbias leave as one partial row per run and
+// are added in a fixed order.
+#include <algorithm>
+
+#include "common.cuh"
+#include "internal.h"
+#include "scan_math.cuh"
+
+namespace mb {
+namespace {
+
+struct ConvGradParams {
+    const void *dy, *x;
+    const float *w, *bias;
+    void *dx;
+    float *part;  // [runs * batch][K + 1][dim]: K taps, then the bias
+    int64_t sdy[3], sx[3], sdx[3];
+    int batch, L, D, run, runs, blocks;
+    bool silu;
+};
+
+constexpr int kCbThreads = 128;
+constexpr int kCbRows = 4;  // rows of x and dy in flight
+
+template <typename T, int VEC> struct RowVec;
+template <typename T> struct RowVec<T, 1> {
+    using Raw = T;
+    static __device__ __forceinline__ void unpack(const T &r, float *f) { f[0] = cvt_f32<T>(r); }
+    static __device__ __forceinline__ T pack(const float *f) { return cvt_out<T>(f[0]); }
+    static __device__ __forceinline__ T zero() { return cvt_out<T>(0.f); }
+};
+template <> struct RowVec<__half, 4> {
+    using Raw = uint2;
+    static __device__ __forceinline__ void unpack(const uint2 &r, float *f) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&r.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&r.y));
+        f[0] = a.x;
+        f[1] = a.y;
+        f[2] = b.x;
+        f[3] = b.y;
+    }
+    static __device__ __forceinline__ uint2 pack(const float *f) {
+        const __half2 a = __floats2half2_rn(f[0], f[1]), b = __floats2half2_rn(f[2], f[3]);
+        return make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
+    static __device__ __forceinline__ uint2 zero() { return make_uint2(0u, 0u); }
+};
+template <> struct RowVec<float, 4> {
+    using Raw = float4;
+    static __device__ __forceinline__ void unpack(const float4 &r, float *f) {
+        f[0] = r.x;
+        f[1] = r.y;
+        f[2] = r.z;
+        f[3] = r.w;
+    }
+    static __device__ __forceinline__ float4 pack(const float *f) { return make_float4(f[0], f[1], f[2], f[3]); }
+    static __device__ __forceinline__ float4 zero() { return make_float4(0.f, 0.f, 0.f, 0.f); }
+};
+
+template <typename T, int K, int VEC>
+__global__ void __launch_bounds__(kCbThreads) conv1d_bwd_kernel(const ConvGradParams p) {
+    using Rv = RowVec<T, VEC>;
+    using Raw = typename Rv::Raw;
+    constexpr bool PRECISE = sizeof(T) == 4;
+    const int block = blockIdx.x % p.blocks, rest = blockIdx.x / p.blocks;
+    const int run = rest % p.runs, b = rest / p.runs;
+    const int d0 = (block * kCbThreads + threadIdx.x) * VEC;
+    if (d0 >= p.D) return;
+    const int t0 = run * p.run, t1 = min(p.L, t0 + p.run);
+    const T *x = static_cast<const T *>(p.x) + b * p.sx[0] + d0 * p.sx[2];
+    const T *dy = static_cast<const T *>(p.dy) + b * p.sdy[0] + d0 * p.sdy[2];
+    T *dx = static_cast<T *>(p.dx) + b * p.sdx[0] + d0 * p.sdx[2];
+    auto row = [&](const T *v, const int64_t *s, int t) {
+        return t < p.L ? *reinterpret_cast<const Raw *>(v + (int64_t)t * s[1]) : Rv::zero();
+    };
+    float w[K][VEC], bias[VEC];
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) w[k][c] = p.w[(int64_t)(d0 + c) * K + k];
+        bias[c] = p.bias ? p.bias[d0 + c] : 0.f;
+    }
+    float win[K][VEC] = {};  // x_{s-K+1} .. x_s
+    float pw[K][VEC] = {};   // p_{s-K+1} .. p_s
+    float dw[K][VEC] = {}, db[VEC] = {};
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+        const int t = t0 - K + 1 + k;
+        if (t >= 0) Rv::unpack(row(x, p.sx, t), win[k]);
+    }
+    Raw xr[kCbRows], yr[kCbRows];
+#pragma unroll
+    for (int r = 0; r < kCbRows; ++r) {
+        xr[r] = row(x, p.sx, t0 + r);
+        yr[r] = row(dy, p.sdy, t0 + r);
+    }
+    const int s1 = t1 + K - 1;  // rows behind the run complete its last gradients
+    for (int sb = t0; sb < s1; sb += kCbRows) {
+        Raw xc[kCbRows], yc[kCbRows];
+#pragma unroll
+        for (int r = 0; r < kCbRows; ++r) {
+            xc[r] = xr[r];
+            yc[r] = yr[r];
+        }
+        if (sb + kCbRows < s1) {
+#pragma unroll
+            for (int r = 0; r < kCbRows; ++r) {
+                xr[r] = row(x, p.sx, sb + kCbRows + r);
+                yr[r] = row(dy, p.sdy, sb + kCbRows + r);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kCbRows; ++r) {
+            const int s = sb + r;
+            Rv::unpack(xc[r], win[K - 1]);
+            Rv::unpack(yc[r], pw[K - 1]);
+            if (p.silu) {
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) {
+                    float pre = bias[c], g, slope;
+#pragma unroll
+                    for (int k = 0; k < K; ++k) pre = fmaf(win[k][c], w[k][c], pre);
+                    silu_grad<PRECISE>(pre, g, slope);
+                    pw[K - 1][c] *= slope;
+                }
+            }
+            if (s < t1) {
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) {
+#pragma unroll
+                    for (int k = 0; k < K; ++k) dw[k][c] = fmaf(pw[K - 1][c], win[k][c], dw[k][c]);
+                    db[c] += pw[K - 1][c];
+                }
+            }
+            const int t = s - K + 1;
+            if (t >= t0 && t < t1) {
+                float out[VEC];
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) {
+                    out[c] = 0.f;
+#pragma unroll
+                    for (int k = 0; k < K; ++k) out[c] = fmaf(w[k][c], pw[K - 1 - k][c], out[c]);
+                }
+                *reinterpret_cast<Raw *>(dx + (int64_t)t * p.sdx[1]) = Rv::pack(out);
+            }
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) {
+                    win[k][c] = win[k + 1][c];
+                    pw[k][c] = pw[k + 1][c];
+                }
+        }
+    }
+    float *part = p.part + (int64_t)rest * (K + 1) * p.D + d0;
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) part[(int64_t)k * p.D + c] = dw[k][c];
+        part[(int64_t)K * p.D + c] = db[c];
+    }
+}
+
+// dw and dbias from the partial rows, in a fixed order: warp v of a CTA adds
+// rows v, v + 8, ... of 32 channels and one tap, then the warps' sums are added
+// in order.
+constexpr int kCbSumThreads = 256;
+__global__ void __launch_bounds__(kCbSumThreads)
+    conv1d_bwd_sum_kernel(const float *__restrict__ part, float *__restrict__ dw, float *__restrict__ dbias, int parts,
+                          int K, int D) {
+    __shared__ float sm[kCbSumThreads / 32][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = blockIdx.x * 32 + lane, k = blockIdx.y;
+    if (k == K ? !dbias : !dw) return;
+    float s = 0.f;
+    if (d < D)
+        for (int i = warp; i < parts; i += kCbSumThreads / 32) s += part[((int64_t)i * (K + 1) + k) * D + d];
+    sm[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && d < D) {
+#pragma unroll
+        for (int v = 1; v < kCbSumThreads / 32; ++v) s += sm[v][lane];
+        if (k == K)
+            dbias[d] = s;
+        else
+            dw[(int64_t)d * K + k] = s;
+    }
+}
+
+// Timesteps per thread: 128, fewer where that leaves the GPU short of threads.
+int run_length(int64_t batch, int64_t L, int64_t D) {
+    int run = 128;
+    while (run > 16 && batch * ceil_div64(L, run) * ceil_div64(D, 4) < 148 * 1024) run /= 2;
+    return run;
+}
+
+template <typename T, int K>
+int launch_conv_bwd(ConvGradParams &p, bool vec, cudaStream_t st) {
+    p.blocks = ceil_div(p.D, kCbThreads * (vec ? 4 : 1));
+    const int64_t grid = (int64_t)p.blocks * p.runs * p.batch;
+    MB_CHECK_ARG(grid <= 0x7fffffff, "causal_conv1d_backward: too many elements");
+    if (vec)
+        conv1d_bwd_kernel<T, K, 4><<<(unsigned)grid, kCbThreads, 0, st>>>(p);
+    else
+        conv1d_bwd_kernel<T, K, 1><<<(unsigned)grid, kCbThreads, 0, st>>>(p);
+    return launch_status("causal_conv1d_backward kernel");
+}
+template <typename T>
+int launch_conv_bwd(ConvGradParams &p, int K, bool vec, cudaStream_t st) {
+    switch (K) {
+        case 1: return launch_conv_bwd<T, 1>(p, vec, st);
+        case 2: return launch_conv_bwd<T, 2>(p, vec, st);
+        case 3: return launch_conv_bwd<T, 3>(p, vec, st);
+        case 4: return launch_conv_bwd<T, 4>(p, vec, st);
+        case 5: return launch_conv_bwd<T, 5>(p, vec, st);
+        case 6: return launch_conv_bwd<T, 6>(p, vec, st);
+        case 7: return launch_conv_bwd<T, 7>(p, vec, st);
+        default: return launch_conv_bwd<T, 8>(p, vec, st);
+    }
+}
+
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Rows of 4 channels at a time: channels adjacent, every row start aligned.
+bool vector_rows(const void *v, const int64_t *s, int64_t es) {
+    return s[2] == 1 && aligned(v, (size_t)(4 * es)) && s[1] % 4 == 0 && s[0] % 4 == 0;
+}
+
+int check(const MambaConvGradArgs *a) {
+    MB_CHECK_ARG(a, "causal_conv1d_backward: null args");
+    MB_CHECK_ARG(a->batch >= 0 && a->seqlen >= 0 && a->dim >= 0, "causal_conv1d_backward: negative size");
+    MB_CHECK_ARG(a->K >= 1 && a->K <= 8, "causal_conv1d_backward: K must be in 1..8");
+    MB_CHECK_ARG(a->dtype == MAMBA_F32 || a->dtype == MAMBA_F16, "causal_conv1d_backward: bad dtype");
+    MB_CHECK_ARG(a->seqlen <= 0x7fffffff - 256, "causal_conv1d_backward: sequence too long");
+    return 0;
+}
+
+}  // namespace
+
+size_t causal_conv1d_backward_workspace_bytes(const MambaConvGradArgs *a) {
+    if (!a || a->batch <= 0 || a->seqlen <= 0 || a->dim <= 0 || a->K < 1 || a->K > 8) return 0;
+    return (size_t)a->batch * ceil_div64(a->seqlen, run_length(a->batch, a->seqlen, a->dim)) * (a->K + 1) * a->dim * 4;
+}
+
+int causal_conv1d_backward(const MambaConvGradArgs *a, void *ws, size_t ws_bytes, cudaStream_t st) {
+    if (check(a)) return -1;
+    if (a->dim == 0) return 0;
+    MB_CHECK_ARG(aligned(a->dw, 4) && aligned(a->dbias, 4),
+                 "causal_conv1d_backward: pointers must be aligned to their element type");
+    MB_CHECK_ARG(!a->dw || a->dw != a->dbias, "causal_conv1d_backward: dw and dbias need memory of their own");
+    if (a->batch == 0 || a->seqlen == 0) {
+        if (a->dw) MB_CUDA_TRY(cudaMemsetAsync(a->dw, 0, (size_t)a->dim * a->K * 4, st));
+        if (a->dbias) MB_CUDA_TRY(cudaMemsetAsync(a->dbias, 0, (size_t)a->dim * 4, st));
+        return 0;
+    }
+    const size_t es = dtype_size(a->dtype);
+    MB_CHECK_ARG(a->dy && a->x && a->w && a->dx, "causal_conv1d_backward: null pointer");
+    MB_CHECK_ARG(aligned(a->dy, es) && aligned(a->x, es) && aligned(a->dx, es) && aligned(a->w, 4) && aligned(a->bias, 4),
+                 "causal_conv1d_backward: pointers must be aligned to their element type");
+    MB_CHECK_ARG(a->dx != a->x && a->dx != a->dy, "causal_conv1d_backward: dx needs memory of its own");
+    MB_CHECK_ARG(ws && ws_bytes >= causal_conv1d_backward_workspace_bytes(a) && aligned(ws, 16),
+                 "causal_conv1d_backward: workspace too small or not 16-byte aligned");
+    ConvGradParams p{};
+    p.dy = a->dy;
+    p.x = a->x;
+    p.w = a->w;
+    p.bias = a->bias;
+    p.dx = a->dx;
+    p.part = static_cast<float *>(ws);
+    for (int k = 0; k < 3; ++k) {
+        p.sdy[k] = a->dy_stride[k];
+        p.sx[k] = a->x_stride[k];
+        p.sdx[k] = a->dx_stride[k];
+    }
+    p.batch = a->batch;
+    p.L = a->seqlen;
+    p.D = a->dim;
+    p.run = run_length(a->batch, a->seqlen, a->dim);
+    p.runs = ceil_div(p.L, p.run);
+    p.silu = a->silu != 0;
+    MB_CHECK_ARG((int64_t)p.runs * p.batch <= 0x7fffffff, "causal_conv1d_backward: too many elements");
+    const bool vec = p.D % 4 == 0 && vector_rows(a->x, p.sx, (int64_t)es) && vector_rows(a->dy, p.sdy, (int64_t)es) &&
+                     vector_rows(a->dx, p.sdx, (int64_t)es);
+    if (a->dtype == MAMBA_F16 ? launch_conv_bwd<__half>(p, a->K, vec, st) : launch_conv_bwd<float>(p, a->K, vec, st))
+        return -1;
+    if (!a->dw && !a->dbias) return 0;
+    conv1d_bwd_sum_kernel<<<dim3((unsigned)ceil_div(p.D, 32), (unsigned)(a->K + 1)), kCbSumThreads, 0, st>>>(
+        p.part, a->dw, a->dbias, p.runs * p.batch, a->K, p.D);
+    return launch_status("causal_conv1d_backward sum kernel");
+}
+
+}  // namespace mb

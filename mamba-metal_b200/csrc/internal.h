@@ -45,6 +45,15 @@ int causal_conv1d_step(const void *x, int64_t xrs, const float *w, const float *
                        int64_t yrs, float *state, int batch, int D, int K, int silu, int dtype,
                        cudaStream_t st);
 
+// conv_bwd.cu
+size_t causal_conv1d_backward_workspace_bytes(const MambaConvGradArgs *a);
+int causal_conv1d_backward(const MambaConvGradArgs *a, void *ws, size_t ws_bytes, cudaStream_t st);
+
+// scan_bwd.cu
+size_t selective_scan_backward_workspace_bytes(const MambaScanArgs *a);
+int selective_scan_backward(const MambaScanArgs *a, const MambaScanGrads *g, void *ws, size_t ws_bytes,
+                            cudaStream_t st);
+
 // recurrence.cu
 size_t recurrence_workspace_bytes(const MambaRecurrenceArgs *a, bool backward);
 int recurrence_forward(const MambaRecurrenceArgs *a, void *ws, size_t ws_bytes, cudaStream_t st);

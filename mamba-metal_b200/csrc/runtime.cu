@@ -1541,6 +1541,28 @@ int mamba_block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormG
         [&] { return mb::block_norm_backward(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)); });
 }
 
+size_t mamba_selective_scan_backward_workspace(const MambaScanArgs *a) {
+    return mb::selective_scan_backward_workspace_bytes(a);
+}
+
+int mamba_selective_scan_backward(const MambaScanArgs *a, const MambaScanGrads *g, void *workspace,
+                                  size_t workspace_bytes, void *stream) {
+    mb::clear_error();
+    return guarded([&] {
+        return mb::selective_scan_backward(a, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    });
+}
+
+size_t mamba_causal_conv1d_backward_workspace(const MambaConvGradArgs *a) {
+    return mb::causal_conv1d_backward_workspace_bytes(a);
+}
+
+int mamba_causal_conv1d_backward(const MambaConvGradArgs *a, void *workspace, size_t workspace_bytes, void *stream) {
+    mb::clear_error();
+    return guarded(
+        [&] { return mb::causal_conv1d_backward(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)); });
+}
+
 int mamba_layer_norm(const MambaLayerNormArgs *a, void *stream) {
     mb::clear_error();
     return guarded([&] { return mb::layer_norm(a, static_cast<cudaStream_t>(stream)); });

@@ -132,6 +132,21 @@ class MambaDropoutArgs(ctypes.Structure):
                 ("out_stride", c_i64)]
 
 
+class MambaScanGrads(ctypes.Structure):
+    _fields_ = [("dy", c_void_p), ("dfinal_state", c_void_p), ("dx", c_void_p), ("ddelta", c_void_p), ("dz", c_void_p),
+                ("dB", c_void_p), ("dC", c_void_p), ("dA", c_void_p), ("dD", c_void_p), ("ddt_bias", c_void_p),
+                ("dinitial_state", c_void_p), ("dy_stride", c_i64 * 3), ("dx_stride", c_i64 * 3),
+                ("ddelta_stride", c_i64 * 3), ("dz_stride", c_i64 * 3), ("dB_stride", c_i64 * 3),
+                ("dC_stride", c_i64 * 3)]
+
+
+class MambaConvGradArgs(ctypes.Structure):
+    _fields_ = [("dy", c_void_p), ("x", c_void_p), ("w", c_void_p), ("bias", c_void_p), ("dx", c_void_p),
+                ("dw", c_void_p), ("dbias", c_void_p), ("batch", ctypes.c_int32), ("seqlen", ctypes.c_int32),
+                ("dim", ctypes.c_int32), ("K", ctypes.c_int32), ("silu", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("dy_stride", c_i64 * 3), ("x_stride", c_i64 * 3), ("dx_stride", c_i64 * 3)]
+
+
 # Every symbol include/mamba.h declares, with its ctypes prototype.
 _PROTOTYPES = {
     "mamba_create": (c_void_p, [ctypes.POINTER(MambaConfig)]),
@@ -193,6 +208,11 @@ _PROTOTYPES = {
     "mamba_block_norm_workspace": (c_size, [ctypes.POINTER(MambaBlockNormArgs)]),
     "mamba_block_norm_backward": (c_int, [ctypes.POINTER(MambaBlockNormArgs), ctypes.POINTER(MambaBlockNormGrads),
                                           c_void_p, c_size, c_void_p]),
+    "mamba_selective_scan_backward_workspace": (c_size, [ctypes.POINTER(MambaScanArgs)]),
+    "mamba_selective_scan_backward": (c_int, [ctypes.POINTER(MambaScanArgs), ctypes.POINTER(MambaScanGrads), c_void_p,
+                                              c_size, c_void_p]),
+    "mamba_causal_conv1d_backward_workspace": (c_size, [ctypes.POINTER(MambaConvGradArgs)]),
+    "mamba_causal_conv1d_backward": (c_int, [ctypes.POINTER(MambaConvGradArgs), c_void_p, c_size, c_void_p]),
     "mamba_layer_norm": (c_int, [ctypes.POINTER(MambaLayerNormArgs), c_void_p]),
     "mamba_layer_norm_workspace": (c_size, [ctypes.POINTER(MambaLayerNormArgs)]),
     "mamba_layer_norm_backward": (c_int, [ctypes.POINTER(MambaLayerNormArgs), ctypes.POINTER(MambaLayerNormGrads),
@@ -742,6 +762,9 @@ _RECURRENCE_ARGS = struct.Struct("@9P4if4x8q")
 _RECURRENCE_GRADS = struct.Struct("@7P8q")
 _BLOCK_NORM_ARGS = struct.Struct("@9Pq2i2f2q")
 _BLOCK_NORM_GRADS = struct.Struct("@7P2q")
+_SCAN_ARGS = struct.Struct("@11P8i18q")
+_SCAN_GRADS = struct.Struct("@11P18q")
+_CONV_GRAD_ARGS = struct.Struct("@7P6i9q")
 _LAYER_NORM_ARGS = struct.Struct("@6Pq3if2q")
 _LAYER_NORM_GRADS = struct.Struct("@4P2q")
 _EMBEDDING_ARGS = struct.Struct("@3P2q4if4x2q")
@@ -1185,6 +1208,101 @@ def dropout_backward(dout, p, seed=0, offset=0, out_dtype=None, dx=None, state=N
     p, seed, offset and state kept the element, else 0, in out_dtype (default:
     dout's).  The residual's gradient is dout itself."""
     return _dropout("mamba_dropout", dout, p, seed, offset, None, out_dtype, dx, state)
+
+
+_NO_STRIDE = (0, 0, 0)
+
+
+@_on_stream
+def selective_scan_backward(dy, x, delta, A, B, C, D=None, z=None, dt_bias=None, initial_state=None,
+                            dfinal_state=None, dx=None, ddelta=None, dz=None, workspace=None):
+    """Gradients of selective_scan (mamba_selective_scan_backward) for the
+    gradient dy of its output and dfinal_state (FP32 [batch, dim, N] or None)
+    of its final state; the other arguments are the forward call's.
+
+    x, delta, z, dy: [batch, L, dim] views, B, C: [batch, L, N] views (any
+    strides; dy of x's dtype).  Returns (dx, ddelta, dA, dB, dC, dD, dz,
+    ddt_bias, dinitial_state): dx, dz in x's dtype, ddelta in delta's, dB, dC
+    in B's, the others FP32; None for an argument that was not given."""
+    torch = _torch()
+    what = "mamba_selective_scan_backward"
+    _require(x.dim() == 3 and A.dim() == 2, "%s: x must be [batch, L, dim] and A [dim, N]" % what)
+    x_dt, d_dt = _float_dtype(x.dtype, "x", what), _float_dtype(delta.dtype, "delta", what)
+    b_dt = _float_dtype(B.dtype, "B", what)
+    shape, dev, f32 = x.shape, x.device, torch.float32
+    (bsz, L, dim), N = shape, A.shape[1]
+
+    def view(t, name, shape, dtype):
+        if t is not None and (t.shape != shape or t.dtype is not dtype or t.device != dev):
+            raise MambaError("%s: %s must be %s %s on %s, got %s %s on %s"
+                             % (what, name, dtype, tuple(shape), dev, t.dtype, tuple(t.shape), t.device))
+
+    view(delta, "delta", shape, delta.dtype)
+    for t, name in ((dy, "dy"), (z, "z"), (dx, "dx"), (dz, "dz")):
+        view(t, name, shape, x.dtype)
+    view(ddelta, "ddelta", shape, delta.dtype)
+    view(B, "B", (bsz, L, N), B.dtype)
+    view(C, "C", (bsz, L, N), B.dtype)
+    _check_tensor(A, "A", what, (dim, N), f32, dev)
+    for t, name in ((D, "D"), (dt_bias, "dt_bias")):
+        if t is not None:
+            _check_tensor(t, name, what, (dim,), f32, dev)
+    for t, name in ((initial_state, "initial_state"), (dfinal_state, "dfinal_state")):
+        if t is not None:
+            _check_tensor(t, name, what, (bsz, dim, N), f32, dev)
+    _require(z is not None or dz is None, "%s: dz without a gate" % what)
+    dx = x.new_empty(shape) if dx is None else dx
+    ddelta = delta.new_empty(shape) if ddelta is None else ddelta
+    if z is not None and dz is None:
+        dz = x.new_empty(shape)
+    dB, dC = B.new_empty((bsz, L, N)), B.new_empty((bsz, L, N))
+    dA = torch.empty_like(A)
+    dD = None if D is None else torch.empty_like(D)
+    ddt_bias = None if dt_bias is None else torch.empty_like(dt_bias)
+    dh0 = None if initial_state is None else torch.empty_like(initial_state)
+    if dim == 0:
+        dB.zero_()
+        dC.zero_()
+        return dx, ddelta, dA, dB, dC, dD, dz, ddt_bias, dh0
+    sz, sdz = (_NO_STRIDE, _NO_STRIDE) if z is None else (z.stride(), dz.stride())
+    a = _packed(what, MambaScanArgs, _SCAN_ARGS, x.data_ptr(), delta.data_ptr(), B.data_ptr(), C.data_ptr(),
+                A.data_ptr(), _ptr0(D), 0, 0, _ptr0(z), _ptr0(dt_bias), _ptr0(initial_state), bsz, L, dim, N, x_dt, d_dt,
+                b_dt, 0, *x.stride(), *delta.stride(), *B.stride(), *C.stride(), *sz, *_NO_STRIDE)
+    g = _packed(what, MambaScanGrads, _SCAN_GRADS, dy.data_ptr(), _ptr0(dfinal_state), dx.data_ptr(),
+                ddelta.data_ptr(), _ptr0(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), _ptr0(dD), _ptr0(ddt_bias),
+                _ptr0(dh0), *dy.stride(), *dx.stride(), *ddelta.stride(), *sdz, *dB.stride(), *dC.stride())
+    ws, ws_len, owner = _workspace(what, lib().mamba_selective_scan_backward_workspace(a), workspace, x)
+    _call(lib().mamba_selective_scan_backward, what, x, a, g, ws, ws_len)
+    return dx, ddelta, dA, dB, dC, dD, dz, ddt_bias, dh0
+
+
+@_on_stream
+def causal_conv1d_backward(dy, x, w, bias=None, silu=True, dx=None, workspace=None):
+    """Gradients of causal_conv1d (mamba_causal_conv1d_backward) for the
+    gradient dy of its output; x, w, bias and silu are the forward call's.
+    dy, x: [batch, L, dim] views of one dtype (any strides); w FP32 [dim, K].
+    Returns (dx, dw, dbias): dx in x's dtype, dw and dbias FP32, dbias None
+    without a bias."""
+    torch = _torch()
+    what = "mamba_causal_conv1d_backward"
+    _require(x.dim() == 3 and w.dim() == 2, "%s: x must be [batch, L, dim] and w [dim, K]" % what)
+    dt = _float_dtype(x.dtype, "x", what)
+    shape, dev = x.shape, x.device
+    for t, name in ((dy, "dy"), (dx, "dx")):
+        if t is not None and (t.shape != shape or t.dtype is not x.dtype or t.device != dev):
+            raise MambaError("%s: %s must be like x" % (what, name))
+    _check_tensor(w, "w", what, (shape[2], w.shape[1]), torch.float32, dev)
+    if bias is not None:
+        _check_tensor(bias, "bias", what, shape[2:], torch.float32, dev)
+    dx = x.new_empty(shape) if dx is None else dx
+    dw = torch.empty_like(w)
+    dbias = None if bias is None else torch.empty_like(bias)
+    a = _packed(what, MambaConvGradArgs, _CONV_GRAD_ARGS, dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr0(bias),
+                dx.data_ptr(), dw.data_ptr(), _ptr0(dbias), *shape, w.shape[1], int(bool(silu)), dt, *dy.stride(),
+                *x.stride(), *dx.stride())
+    ws, ws_len, owner = _workspace(what, lib().mamba_causal_conv1d_backward_workspace(a), workspace, x)
+    _call(lib().mamba_causal_conv1d_backward, what, x, a, ws, ws_len)
+    return dx, dw, dbias
 
 
 def propagate_tile_carries(carries, total=None, stream=None):

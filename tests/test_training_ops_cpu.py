@@ -19,6 +19,9 @@ NEW_STRUCTS = {
     "MambaLayerNormGrads": (mb.MambaLayerNormGrads, mb._LAYER_NORM_GRADS),
     "MambaEmbeddingArgs": (mb.MambaEmbeddingArgs, mb._EMBEDDING_ARGS),
     "MambaDropoutArgs": (mb.MambaDropoutArgs, mb._DROPOUT_ARGS),
+    "MambaScanArgs": (mb.MambaScanArgs, mb._SCAN_ARGS),
+    "MambaScanGrads": (mb.MambaScanGrads, mb._SCAN_GRADS),
+    "MambaConvGradArgs": (mb.MambaConvGradArgs, mb._CONV_GRAD_ARGS),
 }
 
 
@@ -69,6 +72,53 @@ def test_embedding_gradient_matches_differences():
     ids, g = np.array([1, 3, -1, 1, 4, 0]), rng.standard_normal((6, 3))
     grad, _ = tr.embedding_backward(g, ids, 4, 1.5)
     _check_differences(v, lambda: (tr.embedding(ids, v["table"], 1.5) * g).sum(), {"d": grad}, (("table", "d"),))
+
+
+@pytest.mark.parametrize("silu", [False, True])
+def test_conv_gradients_match_differences(silu):
+    rng = np.random.default_rng(3)
+    v = {"x": rng.standard_normal((2, 5, 3)), "w": rng.standard_normal((3, 4)), "b": rng.standard_normal(3)}
+    g = rng.standard_normal((2, 5, 3))
+
+    def run():
+        back = np.concatenate([np.zeros((2, 3, 3)), v["x"]], 1)
+        pre = v["b"] + sum(back[:, k:k + 5] * v["w"][:, k] for k in range(4))
+        return ((pre / (1 + np.exp(-pre)) if silu else pre) * g).sum()
+
+    grads, _ = tr.conv_backward(g, v["x"], v["w"], v["b"], silu)
+    _check_differences(v, run, grads, (("x", "dx"), ("w", "dw"), ("b", "dbias")))
+
+
+@pytest.mark.parametrize("gate", [False, True])
+def test_scan_gradients_match_differences(gate):
+    rng = np.random.default_rng(4)
+    b, L, D, N = 2, 4, 3, 2
+    v = {k: rng.standard_normal((b, L, D)) for k in ("x", "delta", "z")}
+    v.update({k: rng.standard_normal((b, L, N)) for k in ("B", "C")})
+    v.update(A=-np.exp(rng.standard_normal((D, N))), D=rng.standard_normal(D), bias=rng.standard_normal(D),
+             h0=rng.standard_normal((b, D, N)))
+    v["A"][0, 0] = -1e-4  # where psi comes from its series
+    g, gf = rng.standard_normal((b, L, D)), rng.standard_normal((b, D, N))
+
+    def run():
+        dt = np.logaddexp(0, v["delta"] + v["bias"])
+        h, total = v["h0"], 0.0
+        for t in range(L):
+            d = dt[:, t, :, None]
+            h = np.exp(d * v["A"]) * h + np.expm1(d * v["A"]) / v["A"] * v["B"][:, t, None] * v["x"][:, t, :, None]
+            y = (h * v["C"][:, t, None]).sum(2) + v["D"] * v["x"][:, t]
+            if gate:
+                y = y * v["z"][:, t] / (1 + np.exp(-v["z"][:, t]))
+            total += (y * g[:, t]).sum()
+        return total + (h * gf).sum()
+
+    grads, _ = tr.scan_backward(g, v["x"], v["delta"], v["A"], v["B"], v["C"], v["D"], v["z"] if gate else None,
+                                v["bias"], v["h0"], gf)
+    names = [("x", "dx"), ("delta", "ddelta"), ("B", "dB"), ("C", "dC"), ("D", "dD"), ("bias", "ddt_bias"),
+             ("h0", "dh0")] + ([("z", "dz")] if gate else [])
+    _check_differences(v, run, grads, names)
+    # A's element near zero is moved by less than itself
+    _check_differences(v, run, grads, (("A", "dA"),), 1e-6)
 
 
 def test_generator_matches_published_numbers():
@@ -185,7 +235,70 @@ def test_dropout_refusals(change, text):
     _refused(mb.lib().mamba_dropout, text, P(_drop(**change)), None)
 
 
+def _conv(**kw):
+    a = mb.MambaConvGradArgs()
+    a.dy, a.x, a.w, a.bias, a.dx, a.dw, a.dbias = 4096, 8192, 12288, 16384, 20480, 24576, 28672
+    a.batch, a.seqlen, a.dim, a.K, a.silu, a.dtype = 2, 5, 8, 4, 1, mb.F32
+    for s in (a.dy_stride, a.x_stride, a.dx_stride):
+        s[:] = (40, 8, 1)
+    return _set(a, kw)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(batch=-1), "negative"), (dict(seqlen=-1), "negative"), (dict(dim=-1), "negative"), (dict(K=0), "1..8"),
+    (dict(K=9), "1..8"), (dict(dtype=2), "dtype"), (dict(seqlen=0x7fffffff), "long"), (dict(dy=None), "null"),
+    (dict(x=None), "null"), (dict(w=None), "null"), (dict(dx=None), "null"), (dict(x=8194), "aligned"),
+    (dict(dw=4098), "aligned"), (dict(bias=4098), "aligned"), (dict(dx=8192), "own"), (dict(dx=4096), "own"),
+    (dict(dw=28672), "own"), (dict(ws=None), "workspace"), (dict(ws=4104), "workspace"), (dict(short=1), "workspace")])
+def test_conv_backward_refusals(change, text):
+    change = dict(change)
+    ws, short = change.pop("ws", 4096), change.pop("short", 0)
+    need = mb.lib().mamba_causal_conv1d_backward_workspace(P(_conv()))
+    assert need > 0
+    _refused(mb.lib().mamba_causal_conv1d_backward, text, P(_conv(**change)), ws, need - short, None)
+
+
+def _scan(**kw):
+    a = mb.MambaScanArgs()
+    a.x, a.delta, a.B, a.C, a.A, a.D, a.z, a.dt_bias, a.initial_state = (4096 * k for k in range(1, 10))
+    a.batch, a.seqlen, a.dim, a.dstate = 2, 5, 8, 4
+    return _set(a, kw)
+
+
+@pytest.mark.parametrize("args,change,text", [
+    (dict(batch=-1), {}, "negative"), (dict(seqlen=-1), {}, "negative"), (dict(dim=-1), {}, "negative"),
+    (dict(dstate=0), {}, "1..16"), (dict(dstate=17), {}, "1..16"), (dict(x_dtype=2), {}, "dtypes"),
+    (dict(x_dtype=1), {}, None), (dict(delta_dtype=1), {}, "dtypes"), (dict(bc_dtype=1), {}, "dtypes"),
+    (dict(x_dtype=1, delta_dtype=1), {}, "dtypes"), (dict(seqlen=0x7fffffff), {}, "many"),
+    (dict(batch=1 << 16, seqlen=1 << 16), {}, "many"),
+    (dict(x=None), {}, "null"), (dict(delta=None), {}, "null"), (dict(A=None), {}, "null"), (dict(B=None), {}, "null"),
+    (dict(C=None), {}, "null"), ({}, dict(dy=None), "null"), ({}, dict(dx=None), "null"),
+    ({}, dict(ddelta=None), "null"), ({}, dict(dz=None), "dz"), (dict(x=4098), {}, "aligned"),
+    (dict(dt_bias=4098), {}, "aligned"), ({}, dict(dA=4098), "aligned"), ({}, dict(dB=4098), "aligned"),
+    (dict(initial_state=4100), {}, "16-byte"), ({}, dict(dfinal_state=4100), "16-byte"), ({}, dict(dx=4096), "inputs"),
+    ({}, dict(dB=4096 * 3), "inputs"), ({}, dict(dinitial_state=4096 * 9), "inputs"), ({}, dict(dz=4096 * 13), "own"),
+    ({}, dict(dD=4096 * 18), "own"), ({}, dict(ws=None), "workspace"), ({}, dict(ws=4104), "workspace"),
+    ({}, dict(short=1), "workspace")])
+def test_scan_backward_refusals(args, change, text):
+    g, change = mb.MambaScanGrads(), dict(change)
+    for k, (name, *_) in enumerate(mb.MambaScanGrads._fields_[:11]):
+        setattr(g, name, 4096 * (11 + k))
+    ws, short = change.pop("ws", 4096), change.pop("short", 0)
+    need = mb.lib().mamba_selective_scan_backward_workspace(P(_scan()))
+    assert need > 0
+    if text is None:  # FP16 rows with FP32 delta, B and C are supported
+        _set(g, dict(dx=None))
+        text = "null"
+    _refused(mb.lib().mamba_selective_scan_backward, text, P(_scan(**args)), P(_set(g, change)), ws, need - short, None)
+
+
 def test_empty_and_null():
+    assert mb.lib().mamba_selective_scan_backward(None, None, None, 0, None) == -1
+    assert mb.lib().mamba_selective_scan_backward(P(_scan()), None, None, 0, None) == -1
+    assert mb.lib().mamba_causal_conv1d_backward(None, None, 0, None) == -1
+    assert mb.lib().mamba_selective_scan_backward_workspace(None) == 0
+    assert mb.lib().mamba_causal_conv1d_backward_workspace(None) == 0
+    assert mb.lib().mamba_causal_conv1d_backward(P(_conv(dim=0)), None, 0, None) == 0
     L = mb.lib()
     for fn in (L.mamba_layer_norm, L.mamba_embedding, L.mamba_dropout):
         assert fn(None, None) == -1
@@ -223,7 +336,27 @@ def test_binding_refuses_wrong_tensors():
                  lambda: mb.dropout_backward(x, 0.1, dx=x.half(), out_dtype=torch.float32)):
         with pytest.raises(mb.MambaError):
             call()
+    v, A, bc, k = torch.zeros((2, 5, 8)), torch.zeros((8, 4)), torch.zeros((2, 5, 4)), torch.zeros((8, 3))
+    h = torch.zeros((2, 8, 4))
+    for call in (lambda: mb.causal_conv1d_backward(v, v[0], k), lambda: mb.causal_conv1d_backward(v[:1], v, k),
+                 lambda: mb.causal_conv1d_backward(v.half(), v, k), lambda: mb.causal_conv1d_backward(v, v, k[:7]),
+                 lambda: mb.causal_conv1d_backward(v, v, k, w[:7]), lambda: mb.causal_conv1d_backward(v, v, k.half()),
+                 lambda: mb.selective_scan_backward(v[:1], v, v, A, bc, bc),
+                 lambda: mb.selective_scan_backward(v.half(), v, v, A, bc, bc),
+                 lambda: mb.selective_scan_backward(v, v, v[:, :4], A, bc, bc),
+                 lambda: mb.selective_scan_backward(v, v, v, A[:7], bc, bc),
+                 lambda: mb.selective_scan_backward(v, v, v, A.half(), bc, bc),
+                 lambda: mb.selective_scan_backward(v, v, v, A, bc[:1], bc),
+                 lambda: mb.selective_scan_backward(v, v, v, A, bc, bc.half()),
+                 lambda: mb.selective_scan_backward(v, v, v, A, bc, bc, D=w[:7]),
+                 lambda: mb.selective_scan_backward(v, v, v, A, bc, bc, z=v[:1]),
+                 lambda: mb.selective_scan_backward(v, v, v, A, bc, bc, dz=v),
+                 lambda: mb.selective_scan_backward(v, v, v, A, bc, bc, initial_state=h[:1]),
+                 lambda: mb.selective_scan_backward(v, v, v, A, bc, bc, dfinal_state=h.half())):
+        with pytest.raises(mb.MambaError):
+            call()
     for call in (lambda: mb.layer_norm(x), lambda: mb.layer_norm_backward(x, x, one, one), lambda: mb.dropout(x, 0.1),
+                 lambda: mb.causal_conv1d_backward(v, v, k), lambda: mb.selective_scan_backward(v, v, v, A, bc, bc),
                  lambda: mb.embedding(ids, x), lambda: mb.embedding_backward(x, ids, 5)):
         with pytest.raises(mb.MambaError, match="CUDA"):
             call()
