@@ -264,8 +264,7 @@ int mamba_selective_scan(const MambaScanArgs *a, void *workspace, size_t workspa
  * bits on every call.  Strides in elements {batch, time, channel} ({batch,
  * time, state} for dB and dC).  FP16 tensors: exponentials and reciprocals are
  * approximate (2e-6).  Where |A| <= 1e-6 the gradients are those of the
- * zero-order hold's limit.  States 16-byte aligned.  Outputs must not overlap
- * inputs or each other.  batch * seqlen * ceil(dim / 128) <= 2^31. */
+ * zero-order hold's limit. Outputs must not overlap inputs or each other.  batch * seqlen * ceil(dim / 128) <= 2^31. */
 typedef struct MambaScanGrads {
     const void *dy;
     const float *dfinal_state;

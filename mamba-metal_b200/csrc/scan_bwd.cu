@@ -8,9 +8,12 @@
 //   dB = sum_d g phi x,            dC = sum_d q h_t
 //   ddelta = sigmoid(delta + dt_bias) sum_n g a (A h_{t-1} + w)
 //   dA = sum g (dt a h_{t-1} + w psi),   psi = (dt a - phi) / A
-// a - 1 is evaluated without cancellation (e), psi too, and everything is kept
-// as e: h_t = h + e (h + w / A), a g = g + e g, phi = e / A.  A state with
-// |A| < 1e-20 counts as 1e-20, where these are the limits.
+// a - 1 is evaluated without cancellation (e): phi = e / A, and with FP16 tensors
+// e takes the place of a too: h_t = h + e (h + w / A), a g = g + e g.  Of A the
+// kernels keep A2 = A log2(e) and K2 = 1 / A2, with B log2(e) in place of B, so
+// that w / A = w2 K2.  dA is summed as A dA = sum r dt ln 2 h_{t-1} + g w2 (dt a
+// - phi) / log2(e) with r = g a A2.  A state with |A| < 1e-20 counts as 1e-20,
+// where all of these are the limits.
 //
 // Three passes over time chunks:
 //   1. forward: the state before every 8th token (a checkpoint), from zero at
@@ -18,18 +21,20 @@
 //      (its end state H, the reverse carry G and the sum of dt),
 //   2. (several chunks) the state entering each chunk and the carry entering
 //      it from behind,
-//   3. backward, 8 tokens at a time: the states from the checkpoint on into
-//      shared memory, then the reverse steps over them.
-// A CTA holds 128 channels: a thread has 4 channels x 4 states, so a row's x,
-// dt and q are one 16-byte access for 4 channels, and the sums over channels
-// (dB, dC) and states (dx, ddelta, y) are half done before the first shuffle.
-// dB and dC leave as one partial row per block of 128 channels, dA, dD and
-// ddt_bias as one per chunk and batch; a last kernel adds them in order.
+//   3. backward, 8 tokens at a time: the states from the checkpoint on, kept in
+//      tensor memory, then the reverse steps over them.
+// A CTA holds 128 channels: a thread has 4 channels x 4 states, two channels to
+// each packed operation, so a row's x, dt and q are one 16-byte access for 4
+// channels, and the sums over channels (dB, dC) and states (dx, ddelta, y) are
+// half done before the first shuffle.  dB and dC leave as one partial row per
+// block of 128 channels, dA, dD and ddt_bias as one per chunk and batch; a last
+// kernel adds them in order.
 #include <algorithm>
 
 #include "common.cuh"
 #include "internal.h"
 #include "scan_math.cuh"
+#include "umma.cuh"
 
 namespace mb {
 namespace {
@@ -37,63 +42,101 @@ namespace {
 constexpr int kT = 8;        // tokens between checkpoints
 constexpr int kCh = 128;     // channels (and threads) per CTA
 constexpr int kN = 16;       // states, padded
+constexpr int kHalf = kT / 2;  // tokens that a thread stages, of two channels
 
 struct ScanGradParams {
     const void *x, *delta, *dy, *z, *B, *C;
     const float *A, *D, *dt_bias, *h0, *dfinal;
     void *dx, *ddelta, *dz;
     float *dh0;
-    float *ck;    // [batch][subs][dim][16] states before every 8th token
+    // States are kept as [dim / 4 rounded up][16 states][4 channels].
+    float *ck;    // [batch][subs][states] before every 8th token
     float *ck_dt; // [batch][subs][dim] sum of dt before it, since the chunk's start
-    float *H, *G; // [batch][chunks][dim][16]
+    float *H, *G; // [batch][chunks][states]
     float *S;     // [batch][chunks][dim]
     float *part_bc;  // [blocks][batch * L][32]
-    float *part_a;   // [batch * chunks][sums_of(dim)]: dA [dim][16], dD [dim], ddt_bias [dim]
+    float *part_a;   // [batch * chunks][sums_of(dim)]: dA [states], dD [dim], ddt_bias [dim]
     int batch, L, dim, N, chunk, chunks, subs, blocks;
+    int64_t per;     // floats of one set of states
+    bool pairs;      // two adjacent channels can be loaded and stored as one
     int64_t sx[3], sdelta[3], sdy[3], sz[3], sB[3], sC[3], sdx[3], sddelta[3], sdz[3];
 };
 
+__host__ __device__ __forceinline__ int64_t states_of(int dim) { return ((int64_t)dim + 3) / 4 * (4 * kN); }
 // Floats of a partial row of dA, dD and ddt_bias, a multiple of 4.
-__host__ __device__ __forceinline__ int64_t sums_of(int dim) { return ((int64_t)dim * (kN + 2) + 3) / 4 * 4; }
+__host__ __device__ __forceinline__ int64_t sums_of(int dim) { return states_of(dim) + (2 * (int64_t)dim + 3) / 4 * 4; }
 __device__ __forceinline__ float2 make2(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float4 zero4() { return make_float4(0.f, 0.f, 0.f, 0.f); }
-__device__ __forceinline__ float at4(const float4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ float2 lo2(const float4 &v) { return make_float2(v.x, v.y); }
+__device__ __forceinline__ float2 hi2(const float4 &v) { return make_float2(v.z, v.w); }
 
-// e^(dt A) - 1 for two states.  FP16 tensors (v = dt A log2(e)): one
-// approximate exponential less 1, or below 1/32 the series to v^4 (relative
-// error below 2e-6 at the border, 6e-8 relative to e^v - 1 = O(1) elsewhere).
-constexpr float kNear2 = 0.03125f * 1.4426950408889634f;
+// max and min that keep a NaN
+__device__ __forceinline__ float clamp_nan(float v, float lo, float hi) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(lo));
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(r), "f"(hi));
+    return r;
+}
+
+// e = 2^v - 1, and a = 2^v, for two states.
+// FP16 tensors: one approximate exponential less 1, or where |dt A| is below
+// 1/16 the series to the fourth power (relative errors below 2e-6 and 2e-7);
+// a is left to the caller as 1 + e.
+// FP32 tensors: v = j + f with j whole and |f| <= 1/2, 2^f - 1 = f q(f) with q
+// interpolating (2^f - 1) / f at the six Chebyshev nodes of [-1/2, 1/2]
+// (relative error 7e-8), a = 2^j (1 + f q), e = 2^j f q + (2^j - 1).
+constexpr float kNear = 0.0625f * 1.4426950408889634f;
 template <bool PRECISE>
-__device__ __forceinline__ float2 expm1_2(float dt, float dt2, float2 A) {
-    if (PRECISE) return make_float2(expm1f(dt * A.x), expm1f(dt * A.y));
+__device__ __forceinline__ void exp2m1_2(float2 v, float2 &e, float2 &a) {
+    if (PRECISE) {
+        v.x = clamp_nan(v.x, -125.f, 127.f);
+        v.y = clamp_nan(v.y, -125.f, 127.f);
+        const float2 t = __fadd2_rn(v, make2(12582912.f));  // j in the low bits
+        const float2 f = __ffma2_rn(__fadd2_rn(t, make2(-12582912.f)), make2(-1.f), v);
+        float2 s = __ffma2_rn(f, make2(1.545316336e-04f), make2(1.339086331e-03f));
+        s = __ffma2_rn(s, f, make2(9.618083015e-03f));
+        s = __ffma2_rn(s, f, make2(5.550356954e-02f));
+        s = __ffma2_rn(s, f, make2(2.402265072e-01f));
+        s = __ffma2_rn(s, f, make2(6.931471825e-01f));
+        s = __fmul2_rn(s, f);
+        const float2 m = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
+                                     __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
+        e = __ffma2_rn(m, s, __fadd2_rn(m, make2(-1.f)));
+        a = __ffma2_rn(m, s, m);
+        return;
+    }
     constexpr float c1 = 0.69314718055994531f, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
-    const float2 v = __fmul2_rn(make2(dt2), A);
     float2 far = make_float2(ex2_approx(v.x), ex2_approx(v.y));
     far = __fadd2_rn(far, make2(-1.f));
     float2 s = __ffma2_rn(v, make2(c4), make2(c3));
     s = __ffma2_rn(s, v, make2(c2));
     s = __ffma2_rn(s, v, make2(c1));
     s = __fmul2_rn(s, v);
-    return make_float2(fabsf(v.x) < kNear2 ? s.x : far.x, fabsf(v.y) < kNear2 ? s.y : far.y);
+    e = make_float2(fabsf(v.x) < kNear ? s.x : far.x, fabsf(v.y) < kNear ? s.y : far.y);
 }
 
-// psi = (dt a - phi) / A.  Where |dt A| is small, dt^2 (1/2 + v/3 + v^2/8 + ...).
+// a x.  FP16 tensors: x + e x, which is off by 2^-24 |x| where a is small.
 template <bool PRECISE>
-__device__ __forceinline__ float psi_1(float dt, float e, float phi, float A, float kI) {
-    const float v = dt * A;
-    const float far = (fmaf(dt, e, dt) - phi) * kI;
-    float s;
-    if (PRECISE) {
-        s = fmaf(v, 1.f / 840, 1.f / 144);
-        s = fmaf(s, v, 1.f / 30);
-        s = fmaf(s, v, 1.f / 8);
-    } else {
-        s = fmaf(v, 1.f / 30, 1.f / 8);
-    }
-    s = fmaf(s, v, 1.f / 3);
-    s = fmaf(s, v, 0.5f);
-    s *= dt * dt;
-    return fabsf(v) < (PRECISE ? 0.25f : 0.0625f) ? s : far;
+__device__ __forceinline__ float2 decay_2(float2 e, float2 a, float2 x) {
+    return PRECISE ? __fmul2_rn(a, x) : __ffma2_rn(e, x, x);
+}
+// h_t = a h + phi w = h + e (h + w / A).
+template <bool PRECISE>
+__device__ __forceinline__ float2 step_2(float2 e, float2 a, float2 w, float2 K2, float2 h) {
+    return PRECISE ? __ffma2_rn(__fmul2_rn(e, K2), w, __fmul2_rn(a, h)) : __ffma2_rn(e, __ffma2_rn(w, K2, h), h);
+}
+
+// (dt a - phi) / log2(e) from e, phi / log2(e) = e / A2 and dt ln 2.  The
+// difference cancels where |dt A| is small: there phi (x / (1 - e^-x) - 1) with
+// x = dt A, by x/2 + x^2/12 - x^4/720 + ... (the last term for FP32 only).
+template <bool PRECISE>
+__device__ __forceinline__ float2 bend_2(float2 v, float2 e, float2 phi, float2 dt_ln2) {
+    constexpr float c1 = 0.69314718055994531f, c2 = c1 * c1 / 12, c4 = -c1 * c1 * c1 * c1 / 720;
+    const float2 far = __ffma2_rn(phi, make2(-1.f), __ffma2_rn(dt_ln2, e, dt_ln2));
+    float2 s = __ffma2_rn(v, make2(c2), make2(c1 / 2));
+    if (PRECISE) s = __ffma2_rn(__fmul2_rn(__fmul2_rn(v, v), v), make2(c4), s);
+    s = __fmul2_rn(__fmul2_rn(s, v), phi);
+    constexpr float near = PRECISE ? 4 * kNear : kNear;
+    return make_float2(fabsf(v.x) < near ? s.x : far.x, fabsf(v.y) < near ? s.y : far.y);
 }
 
 template <bool PRECISE>
@@ -107,30 +150,66 @@ __device__ __forceinline__ float sigmoid_of(float v) {
     return v >= 0.f ? t : e * t;
 }
 
-// One thread's inputs of 8 tokens: channel `tid` of the block's rows, and two
-// of the 8 x 32 values of B and C.
+// Two channels of one row.
+template <typename T> struct Pair;
+template <> struct Pair<float> {
+    float2 v;
+    __device__ __forceinline__ float2 f32() const { return v; }
+    static __device__ __forceinline__ Pair of(float2 v) { return {v}; }
+    static __device__ __forceinline__ Pair zero() { return {make_float2(0.f, 0.f)}; }
+};
+template <> struct Pair<__half> {
+    __half2 v;
+    __device__ __forceinline__ float2 f32() const { return __half22float2(v); }
+    static __device__ __forceinline__ Pair of(float2 v) { return {__float22half2_rn(v)}; }
+    static __device__ __forceinline__ Pair zero() { return {__float2half2_rn(0.f)}; }
+};
+template <typename T>
+__device__ __forceinline__ Pair<T> load_pair(const T *p, int64_t sc, bool pairs, bool second) {
+    if (pairs) return *reinterpret_cast<const Pair<T> *>(p);
+    Pair<T> r = Pair<T>::zero();
+    r.v.x = p[0];
+    if (second) r.v.y = p[sc];
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_pair(T *p, int64_t sc, bool pairs, bool second, float2 v) {
+    const Pair<T> r = Pair<T>::of(v);
+    if (pairs) {
+        *reinterpret_cast<Pair<T> *>(p) = r;
+    } else {
+        p[0] = r.v.x;
+        if (second) p[sc] = r.v.y;
+    }
+}
+
+// One thread's inputs of 8 tokens: channels 2 (tid % 64) and the next of the
+// block, tokens 4 (tid / 64) .. + 3, and two of the 8 x 32 values of B and C.
+// What lies behind the last token or channel is zero.
 template <typename Tx, typename Td, typename Tb>
 struct RawRows {
-    Tx x[kT], dy[kT], z[kT];
-    Td delta[kT];
+    Pair<Tx> x[kHalf], dy[kHalf], z[kHalf];
+    Pair<Td> delta[kHalf];
     Tb bc[2];
-    // Tokens behind `end` and channels behind the last are left unread: stage() skips them too.
     __device__ __forceinline__ void load(const ScanGradParams &p, int b, int t0, int end, int c, bool grads) {
-        if (c < p.dim) {
-            const Tx *px = static_cast<const Tx *>(p.x) + b * p.sx[0] + c * p.sx[2];
-            const Td *pd = static_cast<const Td *>(p.delta) + b * p.sdelta[0] + c * p.sdelta[2];
-            const Tx *pg = static_cast<const Tx *>(p.dy) + b * p.sdy[0] + c * p.sdy[2];
-            const Tx *pz = static_cast<const Tx *>(p.z) + b * p.sz[0] + c * p.sz[2];
+        const bool second = c + 1 < p.dim;
 #pragma unroll
-            for (int k = 0; k < kT; ++k) {
-                const int64_t t = t0 + k;
-                if (t < end) {
-                    x[k] = px[t * p.sx[1]];
-                    delta[k] = pd[t * p.sdelta[1]];
-                    if (grads) {
-                        dy[k] = pg[t * p.sdy[1]];
-                        if (p.z) z[k] = pz[t * p.sz[1]];
-                    }
+        for (int k = 0; k < kHalf; ++k) {
+            const int64_t t = t0 + k + (threadIdx.x >> 6) * kHalf;
+            x[k] = dy[k] = z[k] = Pair<Tx>::zero();
+            delta[k] = Pair<Td>::zero();
+            if (t < end && c < p.dim) {
+                x[k] = load_pair(static_cast<const Tx *>(p.x) + b * p.sx[0] + t * p.sx[1] + c * p.sx[2], p.sx[2],
+                                 p.pairs, second);
+                delta[k] = load_pair(static_cast<const Td *>(p.delta) + b * p.sdelta[0] + t * p.sdelta[1] +
+                                         c * p.sdelta[2],
+                                     p.sdelta[2], p.pairs, second);
+                if (grads) {
+                    dy[k] = load_pair(static_cast<const Tx *>(p.dy) + b * p.sdy[0] + t * p.sdy[1] + c * p.sdy[2],
+                                      p.sdy[2], p.pairs, second);
+                    if (p.z)
+                        z[k] = load_pair(static_cast<const Tx *>(p.z) + b * p.sz[0] + t * p.sz[1] + c * p.sz[2],
+                                         p.sz[2], p.pairs, second);
                 }
             }
         }
@@ -138,57 +217,74 @@ struct RawRows {
         for (int k = 0; k < 2; ++k) {
             const int at = threadIdx.x + k * kCh, n = at & 15;
             const int64_t t = t0 + (at >> 5);
+            bc[k] = cvt_out<Tb>(0.f);
             if (t < end && n < p.N)
                 bc[k] = at & 16 ? static_cast<const Tb *>(p.C)[b * p.sC[0] + t * p.sC[1] + n * p.sC[2]]
                                 : static_cast<const Tb *>(p.B)[b * p.sB[0] + t * p.sB[1] + n * p.sB[2]];
         }
     }
-};
-
-// A, 1/A of a thread's 4 channels x 4 states.
-__device__ __forceinline__ void load_A(const ScanGradParams &p, int c4, int n4, float2 (&A)[4][2], float2 (&kI)[4][2]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
+    // B log2(e) and C, each value twice in a row: {B, B, C, C} per token and state.
+    __device__ __forceinline__ void stage_bc(float4 (&bc4)[kT][kN]) const {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
+            const int at = threadIdx.x + k * kCh;
+            const float v = cvt_f32<Tb>(bc[k]) * (at & 16 ? 1.f : kLog2e);
+            reinterpret_cast<float2 *>(&bc4[at >> 5][at & 15])[(at >> 4) & 1] = make2(v);
+        }
+    }
+};
+
+// A2 and K2 of a thread's 4 states x 4 channels.
+__device__ __forceinline__ void load_A(const ScanGradParams &p, int c4, int n4, float2 (&A2)[4][2], float2 (&K2)[4][2]) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
             float v[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int n = n4 + 2 * k + e;
-                v[e] = c4 + i < p.dim && n < p.N ? p.A[(int64_t)(c4 + i) * p.N + n] : 0.f;
+                const int c = c4 + 2 * h + e;
+                v[e] = c < p.dim && n4 + s < p.N ? p.A[(int64_t)c * p.N + n4 + s] : 0.f;
                 if (fabsf(v[e]) < 1e-20f) v[e] = 1e-20f;
+                v[e] *= kLog2e;
             }
-            A[i][k] = make_float2(v[0], v[1]);
-            kI[i][k] = make_float2(__frcp_rn(v[0]), __frcp_rn(v[1]));
+            A2[s][h] = make_float2(v[0], v[1]);
+            K2[s][h] = make_float2(__frcp_rn(v[0]), __frcp_rn(v[1]));
         }
 }
 
-// Four states of each of a thread's channels, from [dim][16] rows or [dim][N] ones.
-__device__ __forceinline__ void load_states(const float *rows, int dim, int N, int c4, int n4, float2 (&v)[4][2]) {
+// A thread's states from the caller's [dim][N] rows (zero without any).
+__device__ __forceinline__ void load_given(const ScanGradParams &p, const float *rows, int b, int c4, int n4,
+                                           float2 (&v)[4][2]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float4 q = zero4();
-        if (rows && c4 + i < dim) {
-            const float *r = rows + (int64_t)(c4 + i) * N;
-            if (N == kN) {
-                q = *reinterpret_cast<const float4 *>(r + n4);
-            } else {
-                q.x = n4 + 0 < N ? r[n4 + 0] : 0.f;
-                q.y = n4 + 1 < N ? r[n4 + 1] : 0.f;
-                q.z = n4 + 2 < N ? r[n4 + 2] : 0.f;
-                q.w = n4 + 3 < N ? r[n4 + 3] : 0.f;
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float q[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = c4 + 2 * h + e;
+                q[e] = rows && c < p.dim && n4 + s < p.N ? rows[((int64_t)b * p.dim + c) * p.N + n4 + s] : 0.f;
             }
+            v[s][h] = make_float2(q[0], q[1]);
         }
-        v[i][0] = make_float2(q.x, q.y);
-        v[i][1] = make_float2(q.z, q.w);
+}
+// A thread's states from and to the workspace.
+__device__ __forceinline__ void load_states(const float *set, int dim, int c4, int n4, float2 (&v)[4][2]) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c4 < dim) q = *reinterpret_cast<const float4 *>(set + (int64_t)c4 * kN + (n4 + s) * 4);
+        v[s][0] = lo2(q);
+        v[s][1] = hi2(q);
     }
 }
-__device__ __forceinline__ void store_states(float *rows, int dim, int c4, int n4, const float2 (&v)[4][2]) {
+__device__ __forceinline__ void store_states(float *set, int dim, int c4, int n4, const float2 (&v)[4][2]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (c4 + i < dim)
-            *reinterpret_cast<float4 *>(rows + (int64_t)(c4 + i) * kN + n4) =
-                make_float4(v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y);
+    for (int s = 0; s < 4; ++s)
+        if (c4 < dim)
+            *reinterpret_cast<float4 *>(set + (int64_t)c4 * kN + (n4 + s) * 4) =
+                make_float4(v[s][0].x, v[s][0].y, v[s][1].x, v[s][1].y);
 }
 
 struct Place {
@@ -208,90 +304,97 @@ template <typename Tx, typename Td, typename Tb, bool MULTI>
 __global__ void __launch_bounds__(kCh) scan_bwd_states_kernel(const ScanGradParams p) {
     constexpr bool PRECISE = sizeof(Tx) == 4;
     __shared__ __align__(16) float xs[2][kT][kCh], dts[2][kT][kCh], qs[MULTI ? 2 : 1][kT][MULTI ? kCh : 4];
-    __shared__ __align__(16) float bcs[2][kT][2 * kN];
+    __shared__ float4 bc4[2][kT][kN];
+    __shared__ float half_dt[2][kCh];  // sums of dt over the tokens of either half
     const Place at = place(p);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int c = at.block * kCh + tid;  // the channel this thread stages
+    const int l2 = (tid & 63) * 2, k0 = (tid >> 6) * kHalf, c2 = at.block * kCh + l2;  // what this thread stages
     const int l4 = warp * 32 + (lane >> 2) * 4, c4 = at.block * kCh + l4, n4 = (lane & 3) * 4;
     const int t_first = at.chunk * p.chunk, t_end = min(p.L, t_first + p.chunk);
-    const float bias = p.dt_bias && c < p.dim ? p.dt_bias[c] : 0.f;
-    float2 A[4][2], kI[4][2], h[4][2], P[4][2], G[4][2];
-    load_A(p, c4, n4, A, kI);
-    load_states(at.chunk == 0 && p.h0 ? p.h0 + (int64_t)at.b * p.dim * p.N : nullptr, p.dim, p.N, c4, n4, h);
+    float2 bias = make2(0.f);
+    if (p.dt_bias && c2 < p.dim) bias = make_float2(p.dt_bias[c2], c2 + 1 < p.dim ? p.dt_bias[c2 + 1] : 0.f);
+    float2 A2[4][2], K2[4][2], h[4][2], P[4][2], G[4][2];
+    load_A(p, c4, n4, A2, K2);
+    load_given(p, at.chunk == 0 ? p.h0 : nullptr, at.b, c4, n4, h);
     if (MULTI) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                P[i][k] = make2(1.f);
-                G[i][k] = make2(0.f);
+            for (int i = 0; i < 2; ++i) {
+                P[s][i] = make2(1.f);
+                G[s][i] = make2(0.f);
             }
     }
-    float sum_dt = 0.f;
+    float2 sum_dt = make2(0.f);  // of this thread's tokens
     RawRows<Tx, Td, Tb> raw;
-    raw.load(p, at.b, t_first, t_end, c, MULTI);
     int buf = 0;
     for (int t0 = t_first; t0 < t_end; t0 += kT, buf ^= 1) {
         const int64_t sub = (int64_t)at.b * p.subs + t0 / kT;
-        if (MULTI && c < p.dim) p.ck_dt[sub * p.dim + c] = sum_dt;
+        raw.load(p, at.b, t0, t_end, c2, MULTI);
+        store_states(p.ck + sub * p.per, p.dim, c4, n4, h);
+        if (MULTI) *reinterpret_cast<float2 *>(&half_dt[tid >> 6][l2]) = sum_dt;
 #pragma unroll
-        for (int k = 0; k < kT; ++k) {
-            const bool live = t0 + k < t_end && c < p.dim;
-            const float dt = live ? softplus_of<PRECISE>(cvt_f32<Td>(raw.delta[k]) + bias) : 0.f;
-            xs[buf][k][tid] = live ? cvt_f32<Tx>(raw.x[k]) : 0.f;
-            dts[buf][k][tid] = dt;
-            sum_dt += dt;
+        for (int k = 0; k < kHalf; ++k) {
+            const bool live = t0 + k0 + k < t_end;
+            const float2 d = raw.delta[k].f32();
+            float2 dt = make2(0.f);
+            if (live && c2 < p.dim) dt.x = softplus_of<PRECISE>(d.x + bias.x);
+            if (live && c2 + 1 < p.dim) dt.y = softplus_of<PRECISE>(d.y + bias.y);
+            *reinterpret_cast<float2 *>(&xs[buf][k0 + k][l2]) = raw.x[k].f32();
+            *reinterpret_cast<float2 *>(&dts[buf][k0 + k][l2]) = dt;
             if (MULTI) {
-                float q = live ? cvt_f32<Tx>(raw.dy[k]) : 0.f;
-                if (live && p.z) {
-                    float gate, slope;
-                    silu_grad<PRECISE>(cvt_f32<Tx>(raw.z[k]), gate, slope);
-                    q *= gate;
+                sum_dt = __fadd2_rn(sum_dt, dt);
+                float2 q = raw.dy[k].f32();
+                if (p.z) {
+                    const float2 z = raw.z[k].f32();
+                    float2 gate, slope;
+                    silu_grad<PRECISE>(z.x, gate.x, slope.x);
+                    silu_grad<PRECISE>(z.y, gate.y, slope.y);
+                    q = __fmul2_rn(q, gate);
                 }
-                qs[buf][k][tid] = q;
+                *reinterpret_cast<float2 *>(&qs[buf][k0 + k][l2]) = q;
             }
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int i = tid + k * kCh;
-            (&bcs[buf][0][0])[i] = t0 + (i >> 5) < t_end && (i & 15) < p.N ? cvt_f32<Tb>(raw.bc[k]) : 0.f;
-        }
+        raw.stage_bc(bc4[buf]);
         __syncthreads();  // the other buffer's readers are behind this barrier's predecessor
-        if (t0 + kT < t_end) raw.load(p, at.b, t0 + kT, t_end, c, MULTI);
-        store_states(p.ck + sub * p.dim * kN, p.dim, c4, n4, h);
+        if (MULTI && at.block * kCh + tid < p.dim)
+            p.ck_dt[sub * p.dim + at.block * kCh + tid] = half_dt[0][tid] + half_dt[1][tid];
 #pragma unroll
         for (int k = 0; k < kT; ++k) {
             const float4 x4 = *reinterpret_cast<const float4 *>(&xs[buf][k][l4]);
             const float4 d4 = *reinterpret_cast<const float4 *>(&dts[buf][k][l4]);
-            const float4 B4 = *reinterpret_cast<const float4 *>(&bcs[buf][k][n4]);
-            float4 q4 = zero4(), C4 = zero4();
+            const float2 x2[2] = {lo2(x4), hi2(x4)}, d2[2] = {lo2(d4), hi2(d4)};
+            float2 q2[2];
             if (MULTI) {
-                q4 = *reinterpret_cast<const float4 *>(&qs[buf][k][l4]);
-                C4 = *reinterpret_cast<const float4 *>(&bcs[buf][k][kN + n4]);
+                const float4 q4 = *reinterpret_cast<const float4 *>(&qs[buf][k][l4]);
+                q2[0] = lo2(q4);
+                q2[1] = hi2(q4);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float dt = at4(d4, i), dt2 = dt * kLog2e;
+            for (int s = 0; s < 4; ++s) {
+                const float4 bc = bc4[buf][k][n4 + s];
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const float2 Bp = s ? make_float2(B4.z, B4.w) : make_float2(B4.x, B4.y);
-                    const float2 e = expm1_2<PRECISE>(dt, dt2, A[i][s]);
-                    const float2 w = __fmul2_rn(make2(at4(x4, i)), Bp);
-                    h[i][s] = __ffma2_rn(e, __ffma2_rn(w, kI[i][s], h[i][s]), h[i][s]);
+                for (int i = 0; i < 2; ++i) {
+                    float2 e, a;
+                    exp2m1_2<PRECISE>(__fmul2_rn(d2[i], A2[s][i]), e, a);
+                    h[s][i] = step_2<PRECISE>(e, a, __fmul2_rn(x2[i], lo2(bc)), K2[s][i], h[s][i]);
                     if (MULTI) {
-                        const float2 Cp = s ? make_float2(C4.z, C4.w) : make_float2(C4.x, C4.y);
-                        P[i][s] = __ffma2_rn(P[i][s], e, P[i][s]);
-                        G[i][s] = __ffma2_rn(P[i][s], __fmul2_rn(Cp, make2(at4(q4, i))), G[i][s]);
+                        P[s][i] = decay_2<PRECISE>(e, a, P[s][i]);
+                        G[s][i] = __ffma2_rn(P[s][i], __fmul2_rn(hi2(bc), q2[i]), G[s][i]);
                     }
                 }
             }
         }
+        if (MULTI) __syncthreads();  // half_dt has one buffer
     }
     if (MULTI) {
         const int64_t chunk = (int64_t)at.b * p.chunks + at.chunk;
-        store_states(p.H + chunk * p.dim * kN, p.dim, c4, n4, h);
-        store_states(p.G + chunk * p.dim * kN, p.dim, c4, n4, G);
-        if (c < p.dim) p.S[chunk * p.dim + c] = sum_dt;
+        store_states(p.H + chunk * p.per, p.dim, c4, n4, h);
+        store_states(p.G + chunk * p.per, p.dim, c4, n4, G);
+        *reinterpret_cast<float2 *>(&half_dt[tid >> 6][l2]) = sum_dt;
+        __syncthreads();
+        if (at.block * kCh + tid < p.dim)
+            p.S[chunk * p.dim + at.block * kCh + tid] = half_dt[0][tid] + half_dt[1][tid];
     }
 }
 
@@ -300,36 +403,58 @@ __global__ void __launch_bounds__(kCh) scan_bwd_states_kernel(const ScanGradPara
 // so H there becomes 0), backward for the carry that enters it from behind
 // (into G).
 __global__ void __launch_bounds__(256) scan_bwd_carry_kernel(const ScanGradParams p) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = (int64_t)p.dim * kN;
-    if (i >= p.batch * per) return;
-    const int64_t b = i / per, at = i - b * per;
-    const int d = (int)(at / kN), n = (int)(at % kN);
-    float A = n < p.N ? p.A[(int64_t)d * p.N + n] : 0.f;
-    if (fabsf(A) < 1e-20f) A = 1e-20f;
-    float *H = p.H + b * p.chunks * per + at, *G = p.G + b * p.chunks * per + at;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= p.batch * p.per) return;
+    const int64_t b = i / p.per, at = i - b * p.per;
+    const int d = (int)(at / (4 * kN)) * 4 + (int)(at & 3), n = (int)(at % (4 * kN)) / 4;
+    if (d >= p.dim) return;
+    float A2 = n < p.N ? p.A[(int64_t)d * p.N + n] : 0.f;
+    if (fabsf(A2) < 1e-20f) A2 = 1e-20f;
+    A2 *= kLog2e;
+    float *H = p.H + b * p.chunks * p.per + at, *G = p.G + b * p.chunks * p.per + at;
     const float *S = p.S + b * p.chunks * p.dim + d;
+    // 8 chunks' loads at a time: they do not wait for the stores between them
+    constexpr int kAhead = 8;
     float h = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < p.chunks; ++k) {
-        const float end = H[k * per], P = expf(A * S[(int64_t)k * p.dim]);
-        H[k * per] = h;
-        h = k == 0 ? end : fmaf(P, h, end);
+    for (int k0 = 0; k0 < p.chunks; k0 += kAhead) {
+        float end[kAhead], sum[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (k0 + u < p.chunks) {
+                end[u] = H[(k0 + u) * p.per];
+                sum[u] = S[(int64_t)(k0 + u) * p.dim];
+            }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (k0 + u < p.chunks) {
+                H[(k0 + u) * p.per] = h;
+                h = k0 + u == 0 ? end[u] : fmaf(exp2f(A2 * sum[u]), h, end[u]);
+            }
     }
     float g = p.dfinal && n < p.N ? p.dfinal[(b * p.dim + d) * p.N + n] : 0.f;
-#pragma unroll 4
-    for (int k = p.chunks - 1; k >= 0; --k) {
-        const float own = G[k * per], P = expf(A * S[(int64_t)k * p.dim]);
-        G[k * per] = g;
-        g = fmaf(P, g, own);
+    for (int k0 = p.chunks - 1; k0 >= 0; k0 -= kAhead) {
+        float own[kAhead], sum[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (k0 - u >= 0) {
+                own[u] = G[(k0 - u) * p.per];
+                sum[u] = S[(int64_t)(k0 - u) * p.dim];
+            }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (k0 - u >= 0) {
+                G[(k0 - u) * p.per] = g;
+                g = fmaf(exp2f(A2 * sum[u]), g, own[u]);
+            }
     }
 }
 
 // Sum over the 4 lanes of a quad: lane j is left with v[j]'s.
-__device__ __forceinline__ float quad_sum(const float (&v)[4], int j) {
+__device__ __forceinline__ float quad_sum(const float2 (&v)[2], int j) {
     const bool hi = j & 2, odd = j & 1;
-    float a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
-    a += __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 2);
-    b += __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 2);
+    float a = hi ? v[1].x : v[0].x, b = hi ? v[1].y : v[0].y;
+    a += __shfl_xor_sync(0xffffffffu, hi ? v[0].x : v[1].x, 2);
+    b += __shfl_xor_sync(0xffffffffu, hi ? v[0].y : v[1].y, 2);
     return (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
 }
 // Sum over the 8 lanes with the same lane & 3: lane l is left with v[l >> 2]'s.
@@ -345,176 +470,215 @@ __device__ __forceinline__ float oct_sum(const float (&v)[8], int lane) {
     return (b2 ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, b2 ? b[0] : b[1], 4);
 }
 
-struct BwdSmem {
-    float4 states[kT][4][kCh];  // h before each token: [token][channel of the thread][thread]
-    float x[kT][kCh];           // x, later dx
-    float dt[kT][kCh];          // dt, later the gradient of dt
-    float q[kT][kCh];           // q, later sum_n C h + D x
-    float fz[kT][kCh];          // dy SiLU'(z)
-    float fd[kT][kCh];          // sigmoid(delta + dt_bias)
-    float bc[kT][2 * kN];
-    float red[kT][kCh / 32][2 * kN];  // dB, dC of each warp
-};
+// A thread's 16 values to and from its lane of tensor memory, 16 columns from
+// `at` on.  (These touch no other memory, so there is no memory clobber; the
+// load waits for itself.)
+__device__ __forceinline__ void tmem_put(uint32_t at, const float2 (&v)[4][2]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+        " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+        "f"(v[0][0].x), "f"(v[0][0].y), "f"(v[0][1].x), "f"(v[0][1].y), "f"(v[1][0].x), "f"(v[1][0].y),
+        "f"(v[1][1].x), "f"(v[1][1].y), "f"(v[2][0].x), "f"(v[2][0].y), "f"(v[2][1].x), "f"(v[2][1].y),
+        "f"(v[3][0].x), "f"(v[3][0].y), "f"(v[3][1].x), "f"(v[3][1].y));
+}
+__device__ __forceinline__ void tmem_get(uint32_t at, float2 (&v)[4][2]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32"
+        " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0][0].x), "=f"(v[0][0].y), "=f"(v[0][1].x), "=f"(v[0][1].y), "=f"(v[1][0].x), "=f"(v[1][0].y),
+          "=f"(v[1][1].x), "=f"(v[1][1].y), "=f"(v[2][0].x), "=f"(v[2][0].y), "=f"(v[2][1].x), "=f"(v[2][1].y),
+          "=f"(v[3][0].x), "=f"(v[3][0].y), "=f"(v[3][1].x), "=f"(v[3][1].y)
+        : "r"(at));
+}
 
-// Pass 3.
+// Pass 3.  The states before each of 8 tokens are 128 columns of tensor memory
+// (a thread's own lane), which leaves shared memory and registers for three
+// CTAs an SM.
+constexpr uint32_t kColumns = kT * kN;
 template <typename Tx, typename Td, typename Tb, bool MULTI>
-__global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p) {
+__global__ void __launch_bounds__(kCh, 3) scan_bwd_kernel(const ScanGradParams p) {
     constexpr bool PRECISE = sizeof(Tx) == 4;
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    BwdSmem &sm = *reinterpret_cast<BwdSmem *>(smem_raw);
+    __shared__ __align__(16) float xs[kT][kCh];   // x, later dx
+    __shared__ __align__(16) float dts[kT][kCh];  // dt, later the gradient of dt
+    __shared__ __align__(16) float qs[kT][kCh];   // q, later sum_n C h + D x
+    __shared__ __align__(16) float fz[kT][kCh];   // dy SiLU'(z)
+    __shared__ __align__(16) float fd[kT][kCh];   // sigmoid(delta + dt_bias)
+    __shared__ float4 bc4[kT][kN];
+    __shared__ float red[kT][kCh / 32][2 * kN];   // dB, dC of each warp
+    __shared__ uint32_t tmem_base;
     const Place at = place(p);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, j = lane & 3;
-    const int c = at.block * kCh + tid;
+    const int l2 = (tid & 63) * 2, k0 = (tid >> 6) * kHalf, c2 = at.block * kCh + l2;
     const int l4 = warp * 32 + (lane >> 2) * 4, c4 = at.block * kCh + l4, n4 = j * 4;
     const int t_first = at.chunk * p.chunk, t_end = min(p.L, t_first + p.chunk);
     const int64_t chunk = (int64_t)at.b * p.chunks + at.chunk;
-    const float bias = p.dt_bias && c < p.dim ? p.dt_bias[c] : 0.f;
-    float2 A[4][2], kI[4][2], g[4][2], dA[4][2];
-    load_A(p, c4, n4, A, kI);
-    if (MULTI)
-        load_states(p.G + chunk * p.dim * kN, p.dim, kN, c4, n4, g);
-    else
-        load_states(p.dfinal ? p.dfinal + (int64_t)at.b * p.dim * p.N : nullptr, p.dim, p.N, c4, n4, g);
-    float Dk[4];  // the skip's weights, in one lane of each quad
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        Dk[i] = j == 0 && p.D && c4 + i < p.dim ? p.D[c4 + i] : 0.f;
-        dA[i][0] = dA[i][1] = make2(0.f);
+    if (warp == 0) {
+        tmem_alloc(&tmem_base, kColumns);
+        tmem_relinquish();
+        tc_fence_before();
     }
-    float dD = 0.f, dbias = 0.f;
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base + ((uint32_t)(warp * 32) << 16);
+    float2 bias = make2(0.f);
+    if (p.dt_bias && c2 < p.dim) bias = make_float2(p.dt_bias[c2], c2 + 1 < p.dim ? p.dt_bias[c2 + 1] : 0.f);
+    float2 A2[4][2], K2[4][2], g[4][2], dA[4][2];
+    load_A(p, c4, n4, A2, K2);
+    if (MULTI)
+        load_states(p.G + chunk * p.per, p.dim, c4, n4, g);
+    else
+        load_given(p, p.dfinal, at.b, c4, n4, g);
+    float2 Dk[2];  // the skip's weights, in one lane of each quad
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = c4 + 2 * i;
+        Dk[i] = make_float2(j == 0 && p.D && c < p.dim ? p.D[c] : 0.f, j == 0 && p.D && c + 1 < p.dim ? p.D[c + 1] : 0.f);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) dA[s][0] = dA[s][1] = make2(0.f);
+    float2 dD = make2(0.f), dbias = make2(0.f);  // of this thread's tokens and channels
     RawRows<Tx, Td, Tb> raw;
     const int t_last = t_first + (t_end - 1 - t_first) / kT * kT;
-    raw.load(p, at.b, t_last, t_end, c, true);
+    raw.load(p, at.b, t_last, t_end, c2, true);
     for (int t0 = t_last; t0 >= t_first; t0 -= kT) {
         const int64_t sub = (int64_t)at.b * p.subs + t0 / kT;
         float2 h[4][2];
-        load_states(p.ck + sub * p.dim * kN, p.dim, kN, c4, n4, h);
+        load_states(p.ck + sub * p.per, p.dim, c4, n4, h);
 #pragma unroll
-        for (int k = 0; k < kT; ++k) {
-            const bool live = t0 + k < t_end && c < p.dim;
-            const float xv = live ? cvt_f32<Tx>(raw.x[k]) : 0.f, dy = live ? cvt_f32<Tx>(raw.dy[k]) : 0.f;
-            const float pre = live ? cvt_f32<Td>(raw.delta[k]) + bias : 0.f;
-            float q = dy, fz = 0.f;
+        for (int k = 0; k < kHalf; ++k) {
+            const bool live = t0 + k0 + k < t_end;
+            const float2 x = raw.x[k].f32(), dy = raw.dy[k].f32(), d = raw.delta[k].f32();
+            const float2 pre = __fadd2_rn(d, bias);
+            float2 dt = make2(0.f), q = dy, f = make2(0.f);
+            if (live && c2 < p.dim) dt.x = softplus_of<PRECISE>(pre.x);
+            if (live && c2 + 1 < p.dim) dt.y = softplus_of<PRECISE>(pre.y);
             if (p.z) {
-                float gate, slope;
-                silu_grad<PRECISE>(live ? cvt_f32<Tx>(raw.z[k]) : 0.f, gate, slope);
-                q = dy * gate;
-                fz = dy * slope;
+                const float2 z = raw.z[k].f32();
+                float2 gate, slope;
+                silu_grad<PRECISE>(z.x, gate.x, slope.x);
+                silu_grad<PRECISE>(z.y, gate.y, slope.y);
+                q = __fmul2_rn(dy, gate);
+                f = __fmul2_rn(dy, slope);
             }
-            sm.x[k][tid] = xv;
-            sm.dt[k][tid] = live ? softplus_of<PRECISE>(pre) : 0.f;
-            sm.q[k][tid] = q;
-            sm.fz[k][tid] = fz;
-            sm.fd[k][tid] = sigmoid_of<PRECISE>(pre);
-            dD = fmaf(q, xv, dD);
+            *reinterpret_cast<float2 *>(&xs[k0 + k][l2]) = x;
+            *reinterpret_cast<float2 *>(&dts[k0 + k][l2]) = dt;
+            *reinterpret_cast<float2 *>(&qs[k0 + k][l2]) = q;
+            *reinterpret_cast<float2 *>(&fz[k0 + k][l2]) = f;
+            *reinterpret_cast<float2 *>(&fd[k0 + k][l2]) =
+                make_float2(sigmoid_of<PRECISE>(pre.x), sigmoid_of<PRECISE>(pre.y));
+            dD = __ffma2_rn(q, x, dD);
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int i = tid + k * kCh;
-            (&sm.bc[0][0])[i] = t0 + (i >> 5) < t_end && (i & 15) < p.N ? cvt_f32<Tb>(raw.bc[k]) : 0.f;
-        }
+        raw.stage_bc(bc4);
         __syncthreads();
-        if (t0 > t_first) raw.load(p, at.b, t0 - kT, t_end, c, true);
         if (MULTI && at.chunk > 0) {
             // the checkpoint holds the states from zero at the chunk's start
             float2 in[4][2];
-            load_states(p.H + chunk * p.dim * kN, p.dim, kN, c4, n4, in);
+            load_states(p.H + chunk * p.per, p.dim, c4, n4, in);
+            float sum[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float s = c4 + i < p.dim ? p.ck_dt[sub * p.dim + c4 + i] : 0.f;
+            for (int i = 0; i < 4; ++i) sum[i] = c4 + i < p.dim ? p.ck_dt[sub * p.dim + c4 + i] : 0.f;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    h[i][k].x = fmaf(expf(A[i][k].x * s), in[i][k].x, h[i][k].x);
-                    h[i][k].y = fmaf(expf(A[i][k].y * s), in[i][k].y, h[i][k].y);
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    h[s][i].x = fmaf(exp2f(A2[s][i].x * sum[2 * i]), in[s][i].x, h[s][i].x);
+                    h[s][i].y = fmaf(exp2f(A2[s][i].y * sum[2 * i + 1]), in[s][i].y, h[s][i].y);
                 }
-            }
         }
 #pragma unroll
         for (int k = 0; k < kT; ++k) {
-            const float4 x4 = *reinterpret_cast<const float4 *>(&sm.x[k][l4]);
-            const float4 d4 = *reinterpret_cast<const float4 *>(&sm.dt[k][l4]);
-            const float4 B4 = *reinterpret_cast<const float4 *>(&sm.bc[k][n4]);
+            tmem_put(tmem + k * kN, h);
+            if (k + 1 == kT) break;
+            const float4 x4 = *reinterpret_cast<const float4 *>(&xs[k][l4]);
+            const float4 d4 = *reinterpret_cast<const float4 *>(&dts[k][l4]);
+            const float2 x2[2] = {lo2(x4), hi2(x4)}, d2[2] = {lo2(d4), hi2(d4)};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sm.states[k][i][tid] = make_float4(h[i][0].x, h[i][0].y, h[i][1].x, h[i][1].y);
-                if (k + 1 < kT) {
-                    const float dt = at4(d4, i), dt2 = dt * kLog2e;
+            for (int s = 0; s < 4; ++s) {
+                const float2 B2 = *reinterpret_cast<const float2 *>(&bc4[k][n4 + s]);
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const float2 Bp = s ? make_float2(B4.z, B4.w) : make_float2(B4.x, B4.y);
-                        const float2 e = expm1_2<PRECISE>(dt, dt2, A[i][s]);
-                        const float2 w = __fmul2_rn(make2(at4(x4, i)), Bp);
-                        h[i][s] = __ffma2_rn(e, __ffma2_rn(w, kI[i][s], h[i][s]), h[i][s]);
-                    }
+                for (int i = 0; i < 2; ++i) {
+                    float2 e, a;
+                    exp2m1_2<PRECISE>(__fmul2_rn(d2[i], A2[s][i]), e, a);
+                    h[s][i] = step_2<PRECISE>(e, a, __fmul2_rn(x2[i], B2), K2[s][i], h[s][i]);
                 }
             }
         }
+        tmem_wait_st();
 #pragma unroll 1
         for (int k = kT - 1; k >= 0; --k) {
-            const float4 x4 = *reinterpret_cast<const float4 *>(&sm.x[k][l4]);
-            const float4 d4 = *reinterpret_cast<const float4 *>(&sm.dt[k][l4]);
-            const float4 q4 = *reinterpret_cast<const float4 *>(&sm.q[k][l4]);
-            const float4 B4 = *reinterpret_cast<const float4 *>(&sm.bc[k][n4]);
-            const float4 C4 = *reinterpret_cast<const float4 *>(&sm.bc[k][kN + n4]);
-            float2 bc[4] = {make2(0.f), make2(0.f), make2(0.f), make2(0.f)};  // dB, dC over the 4 channels
-            float y[4], dx[4], dd[4];
+            const float4 x4 = *reinterpret_cast<const float4 *>(&xs[k][l4]);
+            const float4 d4 = *reinterpret_cast<const float4 *>(&dts[k][l4]);
+            const float4 q4 = *reinterpret_cast<const float4 *>(&qs[k][l4]);
+            const float2 x2[2] = {lo2(x4), hi2(x4)}, d2[2] = {lo2(d4), hi2(d4)}, q2[2] = {lo2(q4), hi2(q4)};
+            float2 hp[4][2], y[2], dx[2], dd[2], dt_ln2[2];
+            tmem_get(tmem + k * kN, hp);
+            float v8[8];  // dB of the 4 states, dC of them: sums over the 4 channels
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 hv = sm.states[k][i][tid];
-                const float dt = at4(d4, i), dt2 = dt * kLog2e, q = at4(q4, i), xv = at4(x4, i);
-                float2 y2 = make2(0.f), dx2 = make2(0.f), dd2 = make2(0.f);
+            for (int i = 0; i < 2; ++i) {
+                y[i] = __fmul2_rn(Dk[i], x2[i]);
+                dx[i] = __fmul2_rn(Dk[i], q2[i]);
+                dd[i] = make2(0.f);
+                dt_ln2[i] = __fmul2_rn(d2[i], make2(kLn2));
+            }
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const float2 Bp = s ? make_float2(B4.z, B4.w) : make_float2(B4.x, B4.y);
-                    const float2 Cp = s ? make_float2(C4.z, C4.w) : make_float2(C4.x, C4.y);
-                    const float2 hp = s ? make_float2(hv.z, hv.w) : make_float2(hv.x, hv.y);
-                    const float2 e = expm1_2<PRECISE>(dt, dt2, A[i][s]);
-                    const float2 w = __fmul2_rn(make2(xv), Bp);
-                    const float2 hw = __ffma2_rn(w, kI[i][s], hp);     // h_{t-1} + w / A
-                    const float2 ht = __ffma2_rn(e, hw, hp);
-                    y2 = __ffma2_rn(Cp, ht, y2);
-                    bc[2 + s] = __ffma2_rn(make2(q), ht, bc[2 + s]);
-                    const float2 gt = __ffma2_rn(Cp, make2(q), g[i][s]);
-                    const float2 phi = __fmul2_rn(e, kI[i][s]);
-                    const float2 gphi = __fmul2_rn(gt, phi);
-                    bc[s] = __ffma2_rn(gphi, make2(xv), bc[s]);
-                    dx2 = __ffma2_rn(gphi, Bp, dx2);
-                    const float2 ga = __ffma2_rn(gt, e, gt);
-                    g[i][s] = ga;
-                    dd2 = __ffma2_rn(__fmul2_rn(ga, hw), A[i][s], dd2);
-                    const float2 psi = make_float2(psi_1<PRECISE>(dt, e.x, phi.x, A[i][s].x, kI[i][s].x),
-                                                   psi_1<PRECISE>(dt, e.y, phi.y, A[i][s].y, kI[i][s].y));
-                    dA[i][s] = __ffma2_rn(__fmul2_rn(ga, make2(dt)), hp, dA[i][s]);
-                    dA[i][s] = __ffma2_rn(__fmul2_rn(gt, w), psi, dA[i][s]);
+            for (int s = 0; s < 4; ++s) {
+                const float4 bc = bc4[k][n4 + s];
+                const float2 B2 = lo2(bc), C2 = hi2(bc);
+                float2 dB, dC;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 v = __fmul2_rn(d2[i], A2[s][i]);
+                    float2 e, a;
+                    exp2m1_2<PRECISE>(v, e, a);
+                    const float2 w = __fmul2_rn(x2[i], B2);
+                    const float2 hw = __ffma2_rn(w, K2[s][i], hp[s][i]);  // h_{t-1} + B x / A
+                    const float2 ht = PRECISE ? step_2<PRECISE>(e, a, w, K2[s][i], hp[s][i])
+                                              : __ffma2_rn(e, hw, hp[s][i]);
+                    y[i] = __ffma2_rn(C2, ht, y[i]);
+                    dC = i ? __ffma2_rn(q2[i], ht, dC) : __fmul2_rn(q2[i], ht);
+                    const float2 gt = __ffma2_rn(C2, q2[i], g[s][i]);
+                    const float2 phi = __fmul2_rn(e, K2[s][i]), gphi = __fmul2_rn(gt, phi);
+                    const float2 ga = decay_2<PRECISE>(e, a, gt);
+                    g[s][i] = ga;
+                    dB = i ? __ffma2_rn(gphi, x2[i], dB) : __fmul2_rn(gphi, x2[i]);
+                    dx[i] = __ffma2_rn(gphi, B2, dx[i]);
+                    const float2 r = __fmul2_rn(ga, A2[s][i]);
+                    dd[i] = __ffma2_rn(r, hw, dd[i]);
+                    const float2 bend = bend_2<PRECISE>(v, e, phi, dt_ln2[i]);
+                    dA[s][i] = __ffma2_rn(__fmul2_rn(r, dt_ln2[i]), hp[s][i], dA[s][i]);
+                    dA[s][i] = __ffma2_rn(__fmul2_rn(gt, w), bend, dA[s][i]);
                 }
-                y[i] = fmaf(Dk[i], xv, y2.x + y2.y);
-                dx[i] = fmaf(Dk[i], q, dx2.x + dx2.y);
-                dd[i] = dd2.x + dd2.y;
+                v8[s] = dB.x + dB.y;
+                v8[4 + s] = dC.x + dC.y;
             }
             const float ys = quad_sum(y, j), dxs = quad_sum(dx, j), dds = quad_sum(dd, j);
-            const float v[8] = {bc[0].x, bc[0].y, bc[1].x, bc[1].y, bc[2].x, bc[2].y, bc[3].x, bc[3].y};
-            const float r = oct_sum(v, lane);
+            const float r = oct_sum(v8, lane);
             const int m = lane >> 2;  // dB of state n4 + m, or dC of n4 + m - 4
             __syncwarp();             // the quad has read this token's rows
-            sm.q[k][l4 + j] = ys;
-            sm.x[k][l4 + j] = dxs;
-            sm.dt[k][l4 + j] = dds;
-            sm.red[k][warp][(m & 4) * 4 + n4 + (m & 3)] = r;
+            qs[k][l4 + j] = ys;
+            xs[k][l4 + j] = dxs;
+            dts[k][l4 + j] = dds * kLn2;
+            red[k][warp][(m & 4) * 4 + n4 + (m & 3)] = m & 4 ? r : r * kLog2e;
         }
+        if (t0 > t_first) raw.load(p, at.b, t0 - kT, t_end, c2, true);
         __syncthreads();
-        if (c < p.dim) {
-            Tx *dx = static_cast<Tx *>(p.dx) + at.b * p.sdx[0] + c * p.sdx[2];
-            Td *dd = static_cast<Td *>(p.ddelta) + at.b * p.sddelta[0] + c * p.sddelta[2];
-            Tx *dz = static_cast<Tx *>(p.dz) + at.b * p.sdz[0] + c * p.sdz[2];
+        if (c2 < p.dim) {
+            const bool second = c2 + 1 < p.dim;
 #pragma unroll
-            for (int k = 0; k < kT; ++k) {
-                const int64_t t = t0 + k;
+            for (int k = 0; k < kHalf; ++k) {
+                const int64_t t = t0 + k0 + k;
                 if (t < t_end) {
-                    const float u = sm.dt[k][tid] * sm.fd[k][tid];
-                    dx[t * p.sdx[1]] = cvt_out<Tx>(sm.x[k][tid]);
-                    dd[t * p.sddelta[1]] = cvt_out<Td>(u);
-                    if (p.z) dz[t * p.sdz[1]] = cvt_out<Tx>(sm.q[k][tid] * sm.fz[k][tid]);
-                    dbias += u;
+                    auto pair = [&](const float (&v)[kT][kCh]) { return *reinterpret_cast<const float2 *>(&v[k0 + k][l2]); };
+                    const float2 u = __fmul2_rn(pair(dts), pair(fd));
+                    store_pair(static_cast<Tx *>(p.dx) + at.b * p.sdx[0] + t * p.sdx[1] + c2 * p.sdx[2], p.sdx[2],
+                               p.pairs, second, pair(xs));
+                    store_pair(static_cast<Td *>(p.ddelta) + at.b * p.sddelta[0] + t * p.sddelta[1] + c2 * p.sddelta[2],
+                               p.sddelta[2], p.pairs, second, u);
+                    if (p.z)
+                        store_pair(static_cast<Tx *>(p.dz) + at.b * p.sdz[0] + t * p.sdz[1] + c2 * p.sdz[2], p.sdz[2],
+                                   p.pairs, second, __fmul2_rn(pair(qs), pair(fz)));
+                    dbias = __fadd2_rn(dbias, u);
                 }
             }
         }
@@ -524,29 +688,38 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
             if (t0 + t < t_end) {
                 float s = 0.f;
 #pragma unroll
-                for (int v = 0; v < kCh / 32; ++v) s += sm.red[t][v][i & 31];
+                for (int v = 0; v < kCh / 32; ++v) s += red[t][v][i & 31];
                 p.part_bc[(((int64_t)at.block * p.batch + at.b) * p.L + t0 + t) * (2 * kN) + (i & 31)] = s;
             }
         }
         __syncthreads();
     }
     float *part = p.part_a + chunk * sums_of(p.dim);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) dA[s][i] = __fmul2_rn(__fmul2_rn(dA[s][i], K2[s][i]), make2(kLog2e));
     store_states(part, p.dim, c4, n4, dA);
-    if (c < p.dim) {
-        part[(int64_t)p.dim * 16 + c] = dD;
-        part[(int64_t)p.dim * 17 + c] = dbias;
+    // the two halves' sums of dD and ddt_bias
+    *reinterpret_cast<float2 *>(&xs[tid >> 6][l2]) = dD;
+    *reinterpret_cast<float2 *>(&dts[tid >> 6][l2]) = dbias;
+    __syncthreads();
+    if (at.block * kCh + tid < p.dim) {
+        part += states_of(p.dim) + at.block * kCh + tid;
+        part[0] = xs[0][tid] + xs[1][tid];
+        part[p.dim] = dts[0][tid] + dts[1][tid];
     }
     if (at.chunk == 0 && p.dh0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (c4 + i < p.dim) {
-                float *to = p.dh0 + ((int64_t)at.b * p.dim + c4 + i) * p.N;
-                const float v[4] = {g[i][0].x, g[i][0].y, g[i][1].x, g[i][1].y};
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (n4 + k < p.N) to[n4 + k] = v[k];
-            }
+            for (int i = 0; i < 4; ++i)
+                if (c4 + i < p.dim && n4 + s < p.N)
+                    p.dh0[((int64_t)at.b * p.dim + c4 + i) * p.N + n4 + s] = i & 1 ? g[s][i / 2].y : g[s][i / 2].x;
     }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem_base, kColumns);
 }
 
 struct ScanSumParams {
@@ -580,7 +753,8 @@ __global__ void __launch_bounds__(256) scan_bwd_sum_kernel(const ScanSumParams p
         return;
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t cols = (int64_t)p.dim * (kN + 2), row = sums_of(p.dim), col = (int64_t)(blockIdx.x - p.bc_ctas) * 32 + lane;
+    const int64_t states = states_of(p.dim), cols = states + 2 * (int64_t)p.dim, row = sums_of(p.dim);
+    const int64_t col = (int64_t)(blockIdx.x - p.bc_ctas) * 32 + lane;
     float s = 0.f;
     if (col < cols)
         for (int k = warp; k < p.parts; k += 8) s += p.part_a[k * row + col];
@@ -589,19 +763,19 @@ __global__ void __launch_bounds__(256) scan_bwd_sum_kernel(const ScanSumParams p
     if (warp != 0 || col >= cols) return;
 #pragma unroll
     for (int v = 1; v < 8; ++v) s += sm[v][lane];
-    if (col < (int64_t)p.dim * 16) {
-        const int64_t d = col / kN;
-        const int n = (int)(col % kN);
-        if (n < p.N && p.dA) p.dA[d * p.N + n] = s;
-    } else if (col < (int64_t)p.dim * 17) {
-        if (p.dD) p.dD[col - (int64_t)p.dim * 16] = s;
+    if (col < states) {
+        const int64_t d = col / (4 * kN) * 4 + (col & 3);
+        const int n = (int)(col % (4 * kN)) / 4;
+        if (d < p.dim && n < p.N && p.dA) p.dA[d * p.N + n] = s;
+    } else if (col < states + p.dim) {
+        if (p.dD) p.dD[col - states] = s;
     } else if (p.ddt_bias) {
-        p.ddt_bias[col - (int64_t)p.dim * 17] = s;
+        p.ddt_bias[col - states - p.dim] = s;
     }
 }
 
 // Tokens per chunk: as few chunks as fill the GPU several times over with CTAs
-// (two fit an SM), but at least 32 tokens each.
+// (three fit an SM), but at least 32 tokens each.
 int chunk_length(int64_t batch, int64_t L, int64_t dim) {
     const int64_t blocks = batch * ceil_div64(dim, kCh), want = ceil_div64(8 * 148, std::max<int64_t>(blocks, 1));
     int64_t chunk = ceil_div64(ceil_div64(L, std::max<int64_t>(want, 1)), kT) * kT;
@@ -628,10 +802,11 @@ Layout layout(const MambaScanArgs *a) {
         return v;
     };
     const bool multi = l.chunks > 1;
-    l.ck = take(b * l.subs * dim * kN);
+    const size_t per = (size_t)states_of(a->dim);
+    l.ck = take(b * l.subs * per);
     l.ck_dt = take(multi ? b * l.subs * dim : 0);
-    l.H = take(multi ? b * l.chunks * dim * kN : 0);
-    l.G = take(multi ? b * l.chunks * dim * kN : 0);
+    l.H = take(multi ? b * l.chunks * per : 0);
+    l.G = take(multi ? b * l.chunks * per : 0);
     l.S = take(multi ? b * l.chunks * dim : 0);
     l.bc = take(l.blocks * b * L * 2 * kN);
     l.a = take(b * l.chunks * (size_t)sums_of(a->dim));
@@ -647,20 +822,18 @@ int launch_passes(const ScanGradParams &p, cudaStream_t st) {
     scan_bwd_states_kernel<Tx, Td, Tb, MULTI><<<grid, kCh, 0, st>>>(p);
     if (launch_status("selective_scan_backward states kernel")) return -1;
     if (MULTI) {
-        const int64_t n = (int64_t)p.batch * p.dim * kN;
+        const int64_t n = (int64_t)p.batch * p.per;
         scan_bwd_carry_kernel<<<(unsigned)ceil_div64(n, 256), 256, 0, st>>>(p);
         if (launch_status("selective_scan_backward carry kernel")) return -1;
     }
-    auto kernel = scan_bwd_kernel<Tx, Td, Tb, MULTI>;
-    MB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BwdSmem)));
-    kernel<<<grid, kCh, sizeof(BwdSmem), st>>>(p);
+    scan_bwd_kernel<Tx, Td, Tb, MULTI><<<grid, kCh, 0, st>>>(p);
     return launch_status("selective_scan_backward kernel");
 }
 template <typename Tx, typename Td, typename Tb>
 int launch_all(const ScanGradParams &p, ScanSumParams &s, cudaStream_t st) {
     if (p.chunks > 1 ? launch_passes<Tx, Td, Tb, true>(p, st) : launch_passes<Tx, Td, Tb, false>(p, st)) return -1;
     s.bc_ctas = (unsigned)ceil_div64(s.rows * 32, 256);
-    const int64_t grid = (int64_t)s.bc_ctas + ceil_div64((int64_t)p.dim * (kN + 2), 32);
+    const int64_t grid = (int64_t)s.bc_ctas + ceil_div64(p.per + 2 * (int64_t)p.dim, 32);
     scan_bwd_sum_kernel<Tb><<<(unsigned)grid, 256, 0, st>>>(s);
     return launch_status("selective_scan_backward sum kernel");
 }
@@ -718,10 +891,8 @@ int selective_scan_backward(const MambaScanArgs *a, const MambaScanGrads *g, voi
     MB_CHECK_ARG(aligned(a->x, ex) && aligned(a->z, ex) && aligned(g->dy, ex) && aligned(g->dx, ex) &&
                      aligned(g->dz, ex) && aligned(a->delta, ed) && aligned(g->ddelta, ed) && aligned(a->B, eb) &&
                      aligned(a->C, eb) && aligned(g->dB, eb) && aligned(g->dC, eb) && aligned(a->A, 4) &&
-                     aligned(a->D, 4) && aligned(a->dt_bias, 4),
+                     aligned(a->D, 4) && aligned(a->dt_bias, 4) && aligned(a->initial_state, 4),
                  "selective_scan_backward: pointers must be aligned to their element type");
-    MB_CHECK_ARG((!a->initial_state || aligned(a->initial_state, 16)) && aligned(g->dfinal_state, 16),
-                 "selective_scan_backward: states must be 16-byte aligned");
     const void *in[] = {a->x, a->delta, a->z, a->B, a->C, g->dy, a->A, a->D, a->dt_bias, a->initial_state,
                         g->dfinal_state};
     const void *out[] = {g->dx, g->ddelta, a->z ? g->dz : nullptr, g->dB, g->dC, g->dA, g->dD, g->ddt_bias,
@@ -769,6 +940,7 @@ int selective_scan_backward(const MambaScanArgs *a, const MambaScanGrads *g, voi
     p.chunks = l.chunks;
     p.subs = l.subs;
     p.blocks = l.blocks;
+    p.per = states_of(p.dim);
     ScanSumParams s{};
     for (int k = 0; k < 3; ++k) {
         p.sx[k] = a->x_stride[k];
@@ -783,6 +955,13 @@ int selective_scan_backward(const MambaScanArgs *a, const MambaScanGrads *g, voi
         s.sdB[k] = g->dB_stride[k];
         s.sdC[k] = g->dC_stride[k];
     }
+    // two channels at a time: adjacent, and every row start aligned for both
+    auto even = [&](const void *v, const int64_t *st3, size_t es) {
+        return !v || (st3[2] == 1 && st3[1] % 2 == 0 && st3[0] % 2 == 0 && aligned(v, 2 * es));
+    };
+    p.pairs = p.dim % 2 == 0 && even(p.x, p.sx, ex) && even(p.delta, p.sdelta, ed) && even(p.dy, p.sdy, ex) &&
+              even(p.z, p.sz, ex) && even(p.dx, p.sdx, ex) && even(p.ddelta, p.sddelta, ed) &&
+              (!p.z || even(p.dz, p.sdz, ex));
     s.part_bc = p.part_bc;
     s.part_a = p.part_a;
     s.dB = g->dB;

@@ -275,7 +275,7 @@ def _scan(**kw):
     (dict(C=None), {}, "null"), ({}, dict(dy=None), "null"), ({}, dict(dx=None), "null"),
     ({}, dict(ddelta=None), "null"), ({}, dict(dz=None), "dz"), (dict(x=4098), {}, "aligned"),
     (dict(dt_bias=4098), {}, "aligned"), ({}, dict(dA=4098), "aligned"), ({}, dict(dB=4098), "aligned"),
-    (dict(initial_state=4100), {}, "16-byte"), ({}, dict(dfinal_state=4100), "16-byte"), ({}, dict(dx=4096), "inputs"),
+    (dict(initial_state=4098), {}, "aligned"), ({}, dict(dfinal_state=4098), "aligned"), ({}, dict(dx=4096), "inputs"),
     ({}, dict(dB=4096 * 3), "inputs"), ({}, dict(dinitial_state=4096 * 9), "inputs"), ({}, dict(dz=4096 * 13), "own"),
     ({}, dict(dD=4096 * 18), "own"), ({}, dict(ws=None), "workspace"), ({}, dict(ws=4104), "workspace"),
     ({}, dict(short=1), "workspace")])
