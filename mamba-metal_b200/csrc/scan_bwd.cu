@@ -51,13 +51,14 @@ struct ScanGradParams {
     float *dh0;
     // States are kept as [dim / 4 rounded up][16 states][4 channels].
     float *ck;    // [batch][subs][states] before every 8th token
-    float *ck_dt; // [batch][subs][dim] sum of dt before it, since the chunk's start
+    float *ck_dt; // [batch][subs][dim4] sum of dt before it, since the chunk's start
     float *H, *G; // [batch][chunks][states]
     float *S;     // [batch][chunks][dim]
     float *part_bc;  // [blocks][batch * L][32]
     float *part_a;   // [batch * chunks][sums_of(dim)]: dA [states], dD [dim], ddt_bias [dim]
     int batch, L, dim, N, chunk, chunks, subs, blocks;
     int64_t per;     // floats of one set of states
+    int dim4;        // dim to the next multiple of 4
     bool pairs;      // two adjacent channels can be loaded and stored as one
     int64_t sx[3], sdelta[3], sdy[3], sz[3], sB[3], sC[3], sdx[3], sddelta[3], sdz[3];
 };
@@ -65,6 +66,9 @@ struct ScanGradParams {
 __host__ __device__ __forceinline__ int64_t states_of(int dim) { return ((int64_t)dim + 3) / 4 * (4 * kN); }
 // Floats of a partial row of dA, dD and ddt_bias, a multiple of 4.
 __host__ __device__ __forceinline__ int64_t sums_of(int dim) { return states_of(dim) + (2 * (int64_t)dim + 3) / 4 * 4; }
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 make2(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 lo2(const float4 &v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ float2 hi2(const float4 &v) { return make_float2(v.z, v.w); }
@@ -90,39 +94,39 @@ __device__ __forceinline__ void exp2m1_2(float2 v, float2 &e, float2 &a) {
     if (PRECISE) {
         v.x = clamp_nan(v.x, -125.f, 127.f);
         v.y = clamp_nan(v.y, -125.f, 127.f);
-        const float2 t = __fadd2_rn(v, make2(12582912.f));  // j in the low bits
-        const float2 f = __ffma2_rn(__fadd2_rn(t, make2(-12582912.f)), make2(-1.f), v);
-        float2 s = __ffma2_rn(f, make2(1.545316336e-04f), make2(1.339086331e-03f));
-        s = __ffma2_rn(s, f, make2(9.618083015e-03f));
-        s = __ffma2_rn(s, f, make2(5.550356954e-02f));
-        s = __ffma2_rn(s, f, make2(2.402265072e-01f));
-        s = __ffma2_rn(s, f, make2(6.931471825e-01f));
-        s = __fmul2_rn(s, f);
+        const float2 t = fadd2(v, make2(12582912.f));  // j in the low bits
+        const float2 f = ffma2(fadd2(t, make2(-12582912.f)), make2(-1.f), v);
+        float2 s = ffma2(f, make2(1.545316336e-04f), make2(1.339086331e-03f));
+        s = ffma2(s, f, make2(9.618083015e-03f));
+        s = ffma2(s, f, make2(5.550356954e-02f));
+        s = ffma2(s, f, make2(2.402265072e-01f));
+        s = ffma2(s, f, make2(6.931471825e-01f));
+        s = fmul2(s, f);
         const float2 m = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
                                      __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
-        e = __ffma2_rn(m, s, __fadd2_rn(m, make2(-1.f)));
-        a = __ffma2_rn(m, s, m);
+        e = ffma2(m, s, fadd2(m, make2(-1.f)));
+        a = ffma2(m, s, m);
         return;
     }
     constexpr float c1 = 0.69314718055994531f, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
     float2 far = make_float2(ex2_approx(v.x), ex2_approx(v.y));
-    far = __fadd2_rn(far, make2(-1.f));
-    float2 s = __ffma2_rn(v, make2(c4), make2(c3));
-    s = __ffma2_rn(s, v, make2(c2));
-    s = __ffma2_rn(s, v, make2(c1));
-    s = __fmul2_rn(s, v);
+    far = fadd2(far, make2(-1.f));
+    float2 s = ffma2(v, make2(c4), make2(c3));
+    s = ffma2(s, v, make2(c2));
+    s = ffma2(s, v, make2(c1));
+    s = fmul2(s, v);
     e = make_float2(fabsf(v.x) < kNear ? s.x : far.x, fabsf(v.y) < kNear ? s.y : far.y);
 }
 
 // a x.  FP16 tensors: x + e x, which is off by 2^-24 |x| where a is small.
 template <bool PRECISE>
 __device__ __forceinline__ float2 decay_2(float2 e, float2 a, float2 x) {
-    return PRECISE ? __fmul2_rn(a, x) : __ffma2_rn(e, x, x);
+    return PRECISE ? fmul2(a, x) : ffma2(e, x, x);
 }
 // h_t = a h + phi w = h + e (h + w / A).
 template <bool PRECISE>
 __device__ __forceinline__ float2 step_2(float2 e, float2 a, float2 w, float2 K2, float2 h) {
-    return PRECISE ? __ffma2_rn(__fmul2_rn(e, K2), w, __fmul2_rn(a, h)) : __ffma2_rn(e, __ffma2_rn(w, K2, h), h);
+    return PRECISE ? ffma2(fmul2(e, K2), w, fmul2(a, h)) : ffma2(e, ffma2(w, K2, h), h);
 }
 
 // (dt a - phi) / log2(e) from e, phi / log2(e) = e / A2 and dt ln 2.  The
@@ -131,10 +135,10 @@ __device__ __forceinline__ float2 step_2(float2 e, float2 a, float2 w, float2 K2
 template <bool PRECISE>
 __device__ __forceinline__ float2 bend_2(float2 v, float2 e, float2 phi, float2 dt_ln2) {
     constexpr float c1 = 0.69314718055994531f, c2 = c1 * c1 / 12, c4 = -c1 * c1 * c1 * c1 / 720;
-    const float2 far = __ffma2_rn(phi, make2(-1.f), __ffma2_rn(dt_ln2, e, dt_ln2));
-    float2 s = __ffma2_rn(v, make2(c2), make2(c1 / 2));
-    if (PRECISE) s = __ffma2_rn(__fmul2_rn(__fmul2_rn(v, v), v), make2(c4), s);
-    s = __fmul2_rn(__fmul2_rn(s, v), phi);
+    const float2 far = ffma2(phi, make2(-1.f), ffma2(dt_ln2, e, dt_ln2));
+    float2 s = ffma2(v, make2(c2), make2(c1 / 2));
+    if (PRECISE) s = ffma2(fmul2(fmul2(v, v), v), make2(c4), s);
+    s = fmul2(fmul2(s, v), phi);
     constexpr float near = PRECISE ? 4 * kNear : kNear;
     return make_float2(fabsf(v.x) < near ? s.x : far.x, fabsf(v.y) < near ? s.y : far.y);
 }
@@ -223,13 +227,15 @@ struct RawRows {
                                 : static_cast<const Tb *>(p.B)[b * p.sB[0] + t * p.sB[1] + n * p.sB[2]];
         }
     }
-    // B log2(e) and C, each value twice in a row: {B, B, C, C} per token and state.
+    // B log2(e) and C, each value twice in a row: {B, B, C, C} per token and state,
+    // state n at n % 4 * 4 + n / 4, so that the four lanes of a quad, 4 states
+    // apart, read 64 bytes in a row (without that, two of them share banks).
     __device__ __forceinline__ void stage_bc(float4 (&bc4)[kT][kN]) const {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int at = threadIdx.x + k * kCh;
             const float v = cvt_f32<Tb>(bc[k]) * (at & 16 ? 1.f : kLog2e);
-            reinterpret_cast<float2 *>(&bc4[at >> 5][at & 15])[(at >> 4) & 1] = make2(v);
+            reinterpret_cast<float2 *>(&bc4[at >> 5][(at & 3) * 4 + ((at >> 2) & 3)])[(at >> 4) & 1] = make2(v);
         }
     }
 };
@@ -301,11 +307,11 @@ __device__ __forceinline__ Place place(const ScanGradParams &p) {
 
 // Pass 1.
 template <typename Tx, typename Td, typename Tb, bool MULTI>
-__global__ void __launch_bounds__(kCh) scan_bwd_states_kernel(const ScanGradParams p) {
+__global__ void __launch_bounds__(kCh, 4) scan_bwd_states_kernel(const ScanGradParams p) {
     constexpr bool PRECISE = sizeof(Tx) == 4;
     __shared__ __align__(16) float xs[2][kT][kCh], dts[2][kT][kCh], qs[MULTI ? 2 : 1][kT][MULTI ? kCh : 4];
     __shared__ float4 bc4[2][kT][kN];
-    __shared__ float half_dt[2][kCh];  // sums of dt over the tokens of either half
+    __shared__ __align__(16) float half_dt[2][2][kCh];  // sums of dt over the tokens of either half
     const Place at = place(p);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int l2 = (tid & 63) * 2, k0 = (tid >> 6) * kHalf, c2 = at.block * kCh + l2;  // what this thread stages
@@ -332,7 +338,7 @@ __global__ void __launch_bounds__(kCh) scan_bwd_states_kernel(const ScanGradPara
         const int64_t sub = (int64_t)at.b * p.subs + t0 / kT;
         raw.load(p, at.b, t0, t_end, c2, MULTI);
         store_states(p.ck + sub * p.per, p.dim, c4, n4, h);
-        if (MULTI) *reinterpret_cast<float2 *>(&half_dt[tid >> 6][l2]) = sum_dt;
+        if (MULTI) *reinterpret_cast<float2 *>(&half_dt[buf][tid >> 6][l2]) = sum_dt;
 #pragma unroll
         for (int k = 0; k < kHalf; ++k) {
             const bool live = t0 + k0 + k < t_end;
@@ -343,22 +349,22 @@ __global__ void __launch_bounds__(kCh) scan_bwd_states_kernel(const ScanGradPara
             *reinterpret_cast<float2 *>(&xs[buf][k0 + k][l2]) = raw.x[k].f32();
             *reinterpret_cast<float2 *>(&dts[buf][k0 + k][l2]) = dt;
             if (MULTI) {
-                sum_dt = __fadd2_rn(sum_dt, dt);
+                sum_dt = fadd2(sum_dt, dt);
                 float2 q = raw.dy[k].f32();
                 if (p.z) {
                     const float2 z = raw.z[k].f32();
                     float2 gate, slope;
                     silu_grad<PRECISE>(z.x, gate.x, slope.x);
                     silu_grad<PRECISE>(z.y, gate.y, slope.y);
-                    q = __fmul2_rn(q, gate);
+                    q = fmul2(q, gate);
                 }
                 *reinterpret_cast<float2 *>(&qs[buf][k0 + k][l2]) = q;
             }
         }
         raw.stage_bc(bc4[buf]);
         __syncthreads();  // the other buffer's readers are behind this barrier's predecessor
-        if (MULTI && at.block * kCh + tid < p.dim)
-            p.ck_dt[sub * p.dim + at.block * kCh + tid] = half_dt[0][tid] + half_dt[1][tid];
+        if (MULTI && at.block * kCh + tid < p.dim4)
+            p.ck_dt[sub * p.dim4 + at.block * kCh + tid] = half_dt[buf][0][tid] + half_dt[buf][1][tid];
 #pragma unroll
         for (int k = 0; k < kT; ++k) {
             const float4 x4 = *reinterpret_cast<const float4 *>(&xs[buf][k][l4]);
@@ -372,29 +378,28 @@ __global__ void __launch_bounds__(kCh) scan_bwd_states_kernel(const ScanGradPara
             }
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const float4 bc = bc4[buf][k][n4 + s];
+                const float4 bc = bc4[buf][k][s * 4 + (lane & 3)];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     float2 e, a;
-                    exp2m1_2<PRECISE>(__fmul2_rn(d2[i], A2[s][i]), e, a);
-                    h[s][i] = step_2<PRECISE>(e, a, __fmul2_rn(x2[i], lo2(bc)), K2[s][i], h[s][i]);
+                    exp2m1_2<PRECISE>(fmul2(d2[i], A2[s][i]), e, a);
+                    h[s][i] = step_2<PRECISE>(e, a, fmul2(x2[i], lo2(bc)), K2[s][i], h[s][i]);
                     if (MULTI) {
                         P[s][i] = decay_2<PRECISE>(e, a, P[s][i]);
-                        G[s][i] = __ffma2_rn(P[s][i], __fmul2_rn(hi2(bc), q2[i]), G[s][i]);
+                        G[s][i] = ffma2(P[s][i], fmul2(hi2(bc), q2[i]), G[s][i]);
                     }
                 }
             }
         }
-        if (MULTI) __syncthreads();  // half_dt has one buffer
     }
     if (MULTI) {
         const int64_t chunk = (int64_t)at.b * p.chunks + at.chunk;
         store_states(p.H + chunk * p.per, p.dim, c4, n4, h);
         store_states(p.G + chunk * p.per, p.dim, c4, n4, G);
-        *reinterpret_cast<float2 *>(&half_dt[tid >> 6][l2]) = sum_dt;
+        *reinterpret_cast<float2 *>(&half_dt[buf][tid >> 6][l2]) = sum_dt;
         __syncthreads();
         if (at.block * kCh + tid < p.dim)
-            p.S[chunk * p.dim + at.block * kCh + tid] = half_dt[0][tid] + half_dt[1][tid];
+            p.S[chunk * p.dim + at.block * kCh + tid] = half_dt[buf][0][tid] + half_dt[buf][1][tid];
     }
 }
 
@@ -493,12 +498,12 @@ __device__ __forceinline__ void tmem_get(uint32_t at, float2 (&v)[4][2]) {
 }
 
 // Pass 3.  The states before each of 8 tokens are 128 columns of tensor memory
-// (a thread's own lane), which leaves shared memory and registers for three
-// CTAs an SM.
-constexpr uint32_t kColumns = kT * kN;
+// (a thread's own lane), and with FP16 tensors the e of each token 128 more, so
+// that the reverse steps do not evaluate it again.
+constexpr uint32_t kColumns = 2 * kT * kN;
 template <typename Tx, typename Td, typename Tb, bool MULTI>
-__global__ void __launch_bounds__(kCh, 3) scan_bwd_kernel(const ScanGradParams p) {
-    constexpr bool PRECISE = sizeof(Tx) == 4;
+__global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p) {
+    constexpr bool PRECISE = sizeof(Tx) == 4, KEEP_E = !PRECISE;
     __shared__ __align__(16) float xs[kT][kCh];   // x, later dx
     __shared__ __align__(16) float dts[kT][kCh];  // dt, later the gradient of dt
     __shared__ __align__(16) float qs[kT][kCh];   // q, later sum_n C h + D x
@@ -506,6 +511,7 @@ __global__ void __launch_bounds__(kCh, 3) scan_bwd_kernel(const ScanGradParams p
     __shared__ __align__(16) float fd[kT][kCh];   // sigmoid(delta + dt_bias)
     __shared__ float4 bc4[kT][kN];
     __shared__ float red[kT][kCh / 32][2 * kN];   // dB, dC of each warp
+    __shared__ float4 entry[MULTI ? 4 : 1][MULTI ? kCh : 1];  // the states entering the chunk
     __shared__ uint32_t tmem_base;
     const Place at = place(p);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, j = lane & 3;
@@ -541,15 +547,28 @@ __global__ void __launch_bounds__(kCh, 3) scan_bwd_kernel(const ScanGradParams p
     RawRows<Tx, Td, Tb> raw;
     const int t_last = t_first + (t_end - 1 - t_first) / kT * kT;
     raw.load(p, at.b, t_last, t_end, c2, true);
-    for (int t0 = t_last; t0 >= t_first; t0 -= kT) {
-        const int64_t sub = (int64_t)at.b * p.subs + t0 / kT;
-        float2 h[4][2];
+    float2 h[4][2];
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto load_check = [&](int t) {
+        const int64_t sub = (int64_t)at.b * p.subs + t / kT;
         load_states(p.ck + sub * p.per, p.dim, c4, n4, h);
+        if (MULTI && at.chunk > 0 && c4 < p.dim) {
+            sum = *reinterpret_cast<const float4 *>(p.ck_dt + sub * p.dim4 + c4);
+        }
+    };
+    load_check(t_last);
+    if (MULTI) {
+        float2 in[4][2];
+        load_states(p.H + chunk * p.per, p.dim, c4, n4, in);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) entry[s][tid] = make_float4(in[s][0].x, in[s][0].y, in[s][1].x, in[s][1].y);
+    }
+    for (int t0 = t_last; t0 >= t_first; t0 -= kT) {
 #pragma unroll
         for (int k = 0; k < kHalf; ++k) {
             const bool live = t0 + k0 + k < t_end;
             const float2 x = raw.x[k].f32(), dy = raw.dy[k].f32(), d = raw.delta[k].f32();
-            const float2 pre = __fadd2_rn(d, bias);
+            const float2 pre = fadd2(d, bias);
             float2 dt = make2(0.f), q = dy, f = make2(0.f);
             if (live && c2 < p.dim) dt.x = softplus_of<PRECISE>(pre.x);
             if (live && c2 + 1 < p.dim) dt.y = softplus_of<PRECISE>(pre.y);
@@ -558,8 +577,8 @@ __global__ void __launch_bounds__(kCh, 3) scan_bwd_kernel(const ScanGradParams p
                 float2 gate, slope;
                 silu_grad<PRECISE>(z.x, gate.x, slope.x);
                 silu_grad<PRECISE>(z.y, gate.y, slope.y);
-                q = __fmul2_rn(dy, gate);
-                f = __fmul2_rn(dy, slope);
+                q = fmul2(dy, gate);
+                f = fmul2(dy, slope);
             }
             *reinterpret_cast<float2 *>(&xs[k0 + k][l2]) = x;
             *reinterpret_cast<float2 *>(&dts[k0 + k][l2]) = dt;
@@ -567,42 +586,45 @@ __global__ void __launch_bounds__(kCh, 3) scan_bwd_kernel(const ScanGradParams p
             *reinterpret_cast<float2 *>(&fz[k0 + k][l2]) = f;
             *reinterpret_cast<float2 *>(&fd[k0 + k][l2]) =
                 make_float2(sigmoid_of<PRECISE>(pre.x), sigmoid_of<PRECISE>(pre.y));
-            dD = __ffma2_rn(q, x, dD);
+            dD = ffma2(q, x, dD);
         }
         raw.stage_bc(bc4);
         __syncthreads();
         if (MULTI && at.chunk > 0) {
             // the checkpoint holds the states from zero at the chunk's start
-            float2 in[4][2];
-            load_states(p.H + chunk * p.per, p.dim, c4, n4, in);
-            float sum[4];
+            const float2 sum2[2] = {lo2(sum), hi2(sum)};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] = c4 + i < p.dim ? p.ck_dt[sub * p.dim + c4 + i] : 0.f;
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
+            for (int s = 0; s < 4; ++s) {
+                const float4 in = entry[s][tid];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    h[s][i].x = fmaf(exp2f(A2[s][i].x * sum[2 * i]), in[s][i].x, h[s][i].x);
-                    h[s][i].y = fmaf(exp2f(A2[s][i].y * sum[2 * i + 1]), in[s][i].y, h[s][i].y);
+                    const float2 v = fmul2(A2[s][i], sum2[i]);
+                    const float2 f = PRECISE ? make_float2(exp2f(v.x), exp2f(v.y))
+                                             : make_float2(ex2_approx(v.x), ex2_approx(v.y));
+                    h[s][i] = ffma2(f, i ? hi2(in) : lo2(in), h[s][i]);
                 }
+            }
         }
 #pragma unroll
         for (int k = 0; k < kT; ++k) {
             tmem_put(tmem + k * kN, h);
-            if (k + 1 == kT) break;
+            if (!KEEP_E && k + 1 == kT) break;
+            float2 ee[4][2];
             const float4 x4 = *reinterpret_cast<const float4 *>(&xs[k][l4]);
             const float4 d4 = *reinterpret_cast<const float4 *>(&dts[k][l4]);
             const float2 x2[2] = {lo2(x4), hi2(x4)}, d2[2] = {lo2(d4), hi2(d4)};
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const float2 B2 = *reinterpret_cast<const float2 *>(&bc4[k][n4 + s]);
+                const float2 B2 = *reinterpret_cast<const float2 *>(&bc4[k][s * 4 + j]);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     float2 e, a;
-                    exp2m1_2<PRECISE>(__fmul2_rn(d2[i], A2[s][i]), e, a);
-                    h[s][i] = step_2<PRECISE>(e, a, __fmul2_rn(x2[i], B2), K2[s][i], h[s][i]);
+                    exp2m1_2<PRECISE>(fmul2(d2[i], A2[s][i]), e, a);
+                    if (KEEP_E) ee[s][i] = e;
+                    h[s][i] = step_2<PRECISE>(e, a, fmul2(x2[i], B2), K2[s][i], h[s][i]);
                 }
             }
+            if (KEEP_E) tmem_put(tmem + (kT + k) * kN, ee);
         }
         tmem_wait_st();
 #pragma unroll 1
@@ -612,42 +634,47 @@ __global__ void __launch_bounds__(kCh, 3) scan_bwd_kernel(const ScanGradParams p
             const float4 q4 = *reinterpret_cast<const float4 *>(&qs[k][l4]);
             const float2 x2[2] = {lo2(x4), hi2(x4)}, d2[2] = {lo2(d4), hi2(d4)}, q2[2] = {lo2(q4), hi2(q4)};
             float2 hp[4][2], y[2], dx[2], dd[2], dt_ln2[2];
+            float2 ee[4][2];
             tmem_get(tmem + k * kN, hp);
+            if (KEEP_E) tmem_get(tmem + (kT + k) * kN, ee);
             float v8[8];  // dB of the 4 states, dC of them: sums over the 4 channels
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                y[i] = __fmul2_rn(Dk[i], x2[i]);
-                dx[i] = __fmul2_rn(Dk[i], q2[i]);
+                y[i] = fmul2(Dk[i], x2[i]);
+                dx[i] = fmul2(Dk[i], q2[i]);
                 dd[i] = make2(0.f);
-                dt_ln2[i] = __fmul2_rn(d2[i], make2(kLn2));
+                dt_ln2[i] = fmul2(d2[i], make2(kLn2));
             }
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const float4 bc = bc4[k][n4 + s];
+                const float4 bc = bc4[k][s * 4 + j];
                 const float2 B2 = lo2(bc), C2 = hi2(bc);
                 float2 dB, dC;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float2 v = __fmul2_rn(d2[i], A2[s][i]);
+                    const float2 v = fmul2(d2[i], A2[s][i]);
                     float2 e, a;
-                    exp2m1_2<PRECISE>(v, e, a);
-                    const float2 w = __fmul2_rn(x2[i], B2);
-                    const float2 hw = __ffma2_rn(w, K2[s][i], hp[s][i]);  // h_{t-1} + B x / A
+                    if (KEEP_E)
+                        e = ee[s][i];
+                    else
+                        exp2m1_2<PRECISE>(v, e, a);
+                    const float2 w = fmul2(x2[i], B2);
+                    const float2 hw = ffma2(w, K2[s][i], hp[s][i]);  // h_{t-1} + B x / A
                     const float2 ht = PRECISE ? step_2<PRECISE>(e, a, w, K2[s][i], hp[s][i])
-                                              : __ffma2_rn(e, hw, hp[s][i]);
-                    y[i] = __ffma2_rn(C2, ht, y[i]);
-                    dC = i ? __ffma2_rn(q2[i], ht, dC) : __fmul2_rn(q2[i], ht);
-                    const float2 gt = __ffma2_rn(C2, q2[i], g[s][i]);
-                    const float2 phi = __fmul2_rn(e, K2[s][i]), gphi = __fmul2_rn(gt, phi);
+                                              : ffma2(e, hw, hp[s][i]);
+                    y[i] = ffma2(C2, ht, y[i]);
+                    dC = i ? ffma2(q2[i], ht, dC) : fmul2(q2[i], ht);
+                    const float2 gt = ffma2(C2, q2[i], g[s][i]);
+                    const float2 phi = fmul2(e, K2[s][i]), gphi = fmul2(gt, phi);
                     const float2 ga = decay_2<PRECISE>(e, a, gt);
                     g[s][i] = ga;
-                    dB = i ? __ffma2_rn(gphi, x2[i], dB) : __fmul2_rn(gphi, x2[i]);
-                    dx[i] = __ffma2_rn(gphi, B2, dx[i]);
-                    const float2 r = __fmul2_rn(ga, A2[s][i]);
-                    dd[i] = __ffma2_rn(r, hw, dd[i]);
+                    dB = i ? ffma2(gphi, x2[i], dB) : fmul2(gphi, x2[i]);
+                    dx[i] = ffma2(gphi, B2, dx[i]);
+                    const float2 r = fmul2(ga, A2[s][i]);
+                    dd[i] = ffma2(r, hw, dd[i]);
                     const float2 bend = bend_2<PRECISE>(v, e, phi, dt_ln2[i]);
-                    dA[s][i] = __ffma2_rn(__fmul2_rn(r, dt_ln2[i]), hp[s][i], dA[s][i]);
-                    dA[s][i] = __ffma2_rn(__fmul2_rn(gt, w), bend, dA[s][i]);
+                    dA[s][i] = ffma2(fmul2(r, dt_ln2[i]), hp[s][i], dA[s][i]);
+                    dA[s][i] = ffma2(fmul2(gt, w), bend, dA[s][i]);
                 }
                 v8[s] = dB.x + dB.y;
                 v8[4 + s] = dC.x + dC.y;
@@ -661,7 +688,10 @@ __global__ void __launch_bounds__(kCh, 3) scan_bwd_kernel(const ScanGradParams p
             dts[k][l4 + j] = dds * kLn2;
             red[k][warp][(m & 4) * 4 + n4 + (m & 3)] = m & 4 ? r : r * kLog2e;
         }
-        if (t0 > t_first) raw.load(p, at.b, t0 - kT, t_end, c2, true);
+        if (t0 > t_first) {
+            raw.load(p, at.b, t0 - kT, t_end, c2, true);
+            load_check(t0 - kT);
+        }
         __syncthreads();
         if (c2 < p.dim) {
             const bool second = c2 + 1 < p.dim;
@@ -670,15 +700,15 @@ __global__ void __launch_bounds__(kCh, 3) scan_bwd_kernel(const ScanGradParams p
                 const int64_t t = t0 + k0 + k;
                 if (t < t_end) {
                     auto pair = [&](const float (&v)[kT][kCh]) { return *reinterpret_cast<const float2 *>(&v[k0 + k][l2]); };
-                    const float2 u = __fmul2_rn(pair(dts), pair(fd));
+                    const float2 u = fmul2(pair(dts), pair(fd));
                     store_pair(static_cast<Tx *>(p.dx) + at.b * p.sdx[0] + t * p.sdx[1] + c2 * p.sdx[2], p.sdx[2],
                                p.pairs, second, pair(xs));
                     store_pair(static_cast<Td *>(p.ddelta) + at.b * p.sddelta[0] + t * p.sddelta[1] + c2 * p.sddelta[2],
                                p.sddelta[2], p.pairs, second, u);
                     if (p.z)
                         store_pair(static_cast<Tx *>(p.dz) + at.b * p.sdz[0] + t * p.sdz[1] + c2 * p.sdz[2], p.sdz[2],
-                                   p.pairs, second, __fmul2_rn(pair(qs), pair(fz)));
-                    dbias = __fadd2_rn(dbias, u);
+                                   p.pairs, second, fmul2(pair(qs), pair(fz)));
+                    dbias = fadd2(dbias, u);
                 }
             }
         }
@@ -698,7 +728,7 @@ __global__ void __launch_bounds__(kCh, 3) scan_bwd_kernel(const ScanGradParams p
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) dA[s][i] = __fmul2_rn(__fmul2_rn(dA[s][i], K2[s][i]), make2(kLog2e));
+        for (int i = 0; i < 2; ++i) dA[s][i] = fmul2(fmul2(dA[s][i], K2[s][i]), make2(kLog2e));
     store_states(part, p.dim, c4, n4, dA);
     // the two halves' sums of dD and ddt_bias
     *reinterpret_cast<float2 *>(&xs[tid >> 6][l2]) = dD;
@@ -774,13 +804,24 @@ __global__ void __launch_bounds__(256) scan_bwd_sum_kernel(const ScanSumParams p
     }
 }
 
-// Tokens per chunk: as few chunks as fill the GPU several times over with CTAs
-// (three fit an SM), but at least 32 tokens each.
+// Tokens per chunk.  Passes 1 and 3 run 4 and 2 CTAs an SM, each as long as its
+// chunk and some tokens' worth of work around it, and pass 1 costs about 0.4 of
+// pass 3; several chunks add a tenth.  Taken: the number of chunks (of 16
+// tokens or more) for which the rounds of CTAs are shortest.
 int chunk_length(int64_t batch, int64_t L, int64_t dim) {
-    const int64_t blocks = batch * ceil_div64(dim, kCh), want = ceil_div64(8 * 148, std::max<int64_t>(blocks, 1));
-    int64_t chunk = ceil_div64(ceil_div64(L, std::max<int64_t>(want, 1)), kT) * kT;
-    chunk = std::max<int64_t>(chunk, 32);
-    return (int)std::min<int64_t>(chunk, ceil_div64(L, kT) * kT);
+    const int64_t ctas = batch * ceil_div64(dim, kCh), slots = 148 * 2;
+    int64_t best = 0;
+    double least = 0;
+    for (int64_t n = 1; n <= 128 && n <= ceil_div64(L, 16); ++n) {
+        const int64_t chunk = ceil_div64(ceil_div64(L, n), kT) * kT, all = ctas * ceil_div64(L, chunk);
+        const double cost = (ceil_div64(all, slots) + 0.8 * ceil_div64(all, 2 * slots)) * (double)(chunk + 8) *
+                            (chunk < L ? 1.1 : 1.0);
+        if (best == 0 || cost < least) {
+            best = chunk;
+            least = cost;
+        }
+    }
+    return (int)best;
 }
 
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
@@ -804,7 +845,7 @@ Layout layout(const MambaScanArgs *a) {
     const bool multi = l.chunks > 1;
     const size_t per = (size_t)states_of(a->dim);
     l.ck = take(b * l.subs * per);
-    l.ck_dt = take(multi ? b * l.subs * dim : 0);
+    l.ck_dt = take(multi ? b * l.subs * ((dim + 3) / 4 * 4) : 0);
     l.H = take(multi ? b * l.chunks * per : 0);
     l.G = take(multi ? b * l.chunks * per : 0);
     l.S = take(multi ? b * l.chunks * dim : 0);
@@ -941,6 +982,7 @@ int selective_scan_backward(const MambaScanArgs *a, const MambaScanGrads *g, voi
     p.subs = l.subs;
     p.blocks = l.blocks;
     p.per = states_of(p.dim);
+    p.dim4 = (p.dim + 3) / 4 * 4;
     ScanSumParams s{};
     for (int k = 0; k < 3; ++k) {
         p.sx[k] = a->x_stride[k];
