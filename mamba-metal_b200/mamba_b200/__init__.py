@@ -833,6 +833,7 @@ def _workspace(what, need, workspace, x):
         if not need:
             return 0, 0, None
         workspace = _torch().empty(need, dtype=_torch().uint8, device=x.device)
+        return workspace.data_ptr(), need, workspace
     _require(workspace.is_contiguous() and workspace.device == x.device,
              "%s: workspace must be contiguous and on the tensors' device" % what)
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
@@ -1030,35 +1031,46 @@ def block_norm_backward(dresidual_out, dout, y, residual_out, rstd_post, rstd_pr
 
 def _float_dtype(dtype, name, what):
     """The library's number of a torch dtype."""
-    torch = _torch()
-    if dtype is torch.float16:
+    if _torch().float16 is dtype:
         return F16
-    if dtype is torch.float32:
+    if _torch().float32 is dtype:
         return F32
     raise MambaError("%s: %s must be float16 or float32" % (what, name))
 
 
-def _output(out, name, what, shape, dtype, like, strided=True):
-    """The caller's output after its checks, or a fresh one."""
+def _fresh(like, dtype):
+    """A fresh output of like's shape: empty_like is the cheapest of torch's ways where the dtype is like's (2.4 us
+    against 5 of new_empty on a small call)."""
+    torch = _torch()
+    return torch.empty_like(like) if like.dtype is dtype else \
+        torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
+
+
+def _rows_output(out, name, what, like, dtype):
+    """The caller's output with like's shape after its checks, or a fresh one."""
     if out is None:
-        return like.new_empty(shape, dtype=dtype)
-    _check_tensor(out, name, what, shape, dtype, like.device, strided)
+        return _fresh(like, dtype)
+    _check_tensor(out, name, what, like.shape, dtype, like.device, True)
     return out
 
 
 def _layer_norm_args(what, x, w, b, mean, rstd, out_dtype, eps, out=None):
     torch = _torch()
-    _require(x.dim() == 2, "%s: x must be [rows, cols]" % what)
-    x_dt = _float_dtype(x.dtype, "x", what)
-    shape, dev = x.shape, x.device
-    _check_tensor(x, "x", what, shape, x.dtype, dev, True)
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    if len(shape) != 2:
+        raise MambaError("%s: x must be [rows, cols]" % what)
+    rows, cols = shape
+    x_dt = _float_dtype(dtype, "x", what)
+    if not x.is_contiguous():
+        _check_tensor(x, "x", what, shape, dtype, dev, True)
     if w is not None:
-        _check_tensor(w, "w", what, shape[1:], torch.float32, dev)
+        _check_tensor(w, "w", what, (cols,), torch.float32, dev)
     if b is not None:
-        _check_tensor(b, "b", what, shape[1:], torch.float32, dev)
+        _check_tensor(b, "b", what, (cols,), torch.float32, dev)
     return _packed(what, MambaLayerNormArgs, _LAYER_NORM_ARGS, x.data_ptr(), _ptr0(w), _ptr0(b), _ptr0(out),
-                   _ptr0(mean), _ptr0(rstd), shape[0], shape[1], x_dt, _float_dtype(out_dtype, "out", what), eps,
-                   x.stride(0), 0 if out is None else out.stride(0))
+                   _ptr0(mean), _ptr0(rstd), rows, cols, x_dt,
+                   x_dt if out_dtype is dtype else _float_dtype(out_dtype, "out", what), eps, x.stride(0),
+                   0 if out is None else out.stride(0))
 
 
 @_on_stream
@@ -1069,14 +1081,16 @@ def layer_norm(x, w=None, b=None, eps=1e-5, out_dtype=None, return_stats=False, 
     and with return_stats also the FP32 [rows] mean and rstd that
     layer_norm_backward reads."""
     what = "mamba_layer_norm"
-    _require(x.dim() == 2, "%s: x must be [rows, cols]" % what)
+    if x.dim() != 2:
+        raise MambaError("%s: x must be [rows, cols]" % what)
     if out_dtype is None:
         out_dtype = x.dtype if out is None else out.dtype
-    _float_dtype(out_dtype, "out", what)
-    out = _output(out, "out", what, x.shape, out_dtype, x)
+    out = _rows_output(out, "out", what, x, out_dtype)
     mean = rstd = None
     if return_stats:
-        mean, rstd = x.new_empty((2, x.shape[0]), dtype=_torch().float32).unbind(0)
+        torch = _torch()
+        mean = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
     a = _layer_norm_args(what, x, w, b, mean, rstd, out_dtype, eps, out)
     _call(lib().mamba_layer_norm, what, x, a)
     return (out, mean, rstd) if return_stats else out
@@ -1089,12 +1103,14 @@ def layer_norm_backward(dout, x, mean, rstd, w=None, dx=None, workspace=None):
     Returns (dx, dw, db): dx in x's dtype, the sums dw and db FP32 [cols]."""
     torch = _torch()
     what = "mamba_layer_norm_backward"
-    _check_tensor(dout, "dout", what, x.shape, dout.dtype, x.device, True)
-    _check_tensor(mean, "mean", what, x.shape[:1], torch.float32, x.device)
-    _check_tensor(rstd, "rstd", what, x.shape[:1], torch.float32, x.device)
     a = _layer_norm_args(what, x, w, None, mean, rstd, dout.dtype, 1.0)  # eps is inside rstd
-    dx = _output(dx, "dx", what, x.shape, x.dtype, x)
-    dw, db = mean.new_empty((2, x.shape[1])).unbind(0)
+    shape, dev = x.shape, x.device
+    _check_tensor(dout, "dout", what, shape, dout.dtype, dev, True)
+    _check_tensor(mean, "mean", what, shape[:1], torch.float32, dev)
+    _check_tensor(rstd, "rstd", what, shape[:1], torch.float32, dev)
+    dx = _rows_output(dx, "dx", what, x, x.dtype)
+    dw = torch.empty(a.cols, dtype=torch.float32, device=dev) if w is None else torch.empty_like(w)
+    db = torch.empty_like(dw)
     g = _packed(what, MambaLayerNormGrads, _LAYER_NORM_GRADS, dout.data_ptr(), dx.data_ptr(), dw.data_ptr(),
                 db.data_ptr(), dout.stride(0), dx.stride(0))
     ws, ws_len, owner = _workspace(what, lib().mamba_layer_norm_workspace(a), workspace, x)
@@ -1102,13 +1118,16 @@ def layer_norm_backward(dout, x, mean, rstd, w=None, dx=None, workspace=None):
     return dx, dw, db
 
 
-def _embedding_args(what, tokens, vocab, dim, table_dtype, out_dtype, scale, table=None, out=None):
+def _embedding_args(what, tokens, vocab, dim, table_dtype, out_dtype, scale, table=0, out=0, table_stride=0,
+                    out_stride=0):
     torch = _torch()
-    _require(tokens.dtype is torch.int32 or tokens.dtype is torch.int64, "%s: tokens must be int32 or int64" % what)
-    _require(tokens.is_contiguous(), "%s: tokens must be contiguous" % what)
-    return _packed(what, MambaEmbeddingArgs, _EMBEDDING_ARGS, tokens.data_ptr(), _ptr0(table), _ptr0(out),
-                   tokens.numel(), vocab, dim, tokens.element_size(), table_dtype, out_dtype, scale,
-                   0 if table is None else table.stride(0), 0 if out is None else out.stride(-2))
+    wide = tokens.dtype is torch.int64
+    if not wide and tokens.dtype is not torch.int32:
+        raise MambaError("%s: tokens must be int32 or int64" % what)
+    if not tokens.is_contiguous():
+        raise MambaError("%s: tokens must be contiguous" % what)
+    return _packed(what, MambaEmbeddingArgs, _EMBEDDING_ARGS, tokens.data_ptr(), table, out, tokens.numel(), vocab, dim,
+                   8 if wide else 4, table_dtype, out_dtype, scale, table_stride, out_stride)
 
 
 @_on_stream
@@ -1120,20 +1139,26 @@ def embedding(tokens, table, scale=1.0, out_dtype=None, out=None):
     F32 (row stride any, channel stride 1).  Returns [*tokens.shape, dim]; an
     `out` of that shape must be contiguous, or [tokens, dim] rows of any
     stride."""
+    torch = _torch()
     what = "mamba_embedding"
-    _require(table.dim() == 2, "%s: table must be [vocab, dim]" % what)
-    t_dt = _float_dtype(table.dtype, "table", what)
-    _check_tensor(table, "table", what, table.shape, table.dtype, tokens.device, True)
+    dtype, dev = table.dtype, tokens.device
+    if table.dim() != 2:
+        raise MambaError("%s: table must be [vocab, dim]" % what)
+    t_dt = _float_dtype(dtype, "table", what)
+    _check_tensor(table, "table", what, table.shape, dtype, dev, True)
     vocab, dim = table.shape
     if out_dtype is None:
-        out_dtype = table.dtype if out is None else out.dtype
-    o_dt = _float_dtype(out_dtype, "out", what)
-    shape = tuple(tokens.shape) + (dim,)
-    rows = _output(out, "out", what, shape, out_dtype, table, len(shape) == 2)
-    a = _embedding_args(what, tokens, vocab, dim, t_dt, o_dt, scale, table,
-                        rows if len(shape) == 2 else rows.view(-1, dim) if dim else rows.new_empty((0, 0)))
+        out_dtype = dtype if out is None else out.dtype
+    o_dt = t_dt if out_dtype is dtype else _float_dtype(out_dtype, "out", what)
+    shape = tokens.shape + (dim,)
+    if out is None:
+        out = torch.empty(*shape, dtype=out_dtype, device=dev)
+    else:
+        _check_tensor(out, "out", what, shape, out_dtype, dev, len(shape) == 2)
+    a = _embedding_args(what, tokens, vocab, dim, t_dt, o_dt, scale, table.data_ptr(), out.data_ptr(), table.stride(0),
+                        out.stride(0) if len(shape) == 2 else dim)
     _call(lib().mamba_embedding, what, table, a)
-    return rows
+    return out
 
 
 @_on_stream
@@ -1147,35 +1172,43 @@ def embedding_backward(dout, tokens, vocab, scale=1.0, dtable=None, accumulate=F
     torch = _torch()
     what = "mamba_embedding_backward"
     o_dt = _float_dtype(dout.dtype, "dout", what)
-    _require(dout.dim() >= 1, "%s: dout must be [*tokens.shape, dim]" % what)
-    dim = dout.shape[-1]
-    _check_tensor(dout, "dout", what, tuple(tokens.shape) + (dim,), dout.dtype, tokens.device, dout.dim() == 2)
-    if dtable is None:
-        _require(not accumulate, "%s: accumulate adds into a given dtable" % what)
-        dtable = dout.new_empty((vocab, dim), dtype=torch.float32)
-    else:
+    if dout.dim() < 1:
+        raise MambaError("%s: dout must be [*tokens.shape, dim]" % what)
+    dim, rows = dout.shape[-1], dout.dim() == 2
+    _check_tensor(dout, "dout", what, tokens.shape + (dim,), dout.dtype, tokens.device, rows)
+    if dtable is not None:
         _check_tensor(dtable, "dtable", what, (vocab, dim), torch.float32, dout.device, True)
+    elif accumulate:
+        raise MambaError("%s: accumulate adds into a given dtable" % what)
     a = _embedding_args(what, tokens, vocab, dim, F32, o_dt, scale)
+    if dtable is None:
+        dtable = torch.empty(vocab, dim, dtype=torch.float32, device=dout.device)
     ws, ws_len, owner = _workspace(what, lib().mamba_embedding_workspace(a), workspace, dout)
-    _call(lib().mamba_embedding_backward, what, dout, a, dout.data_ptr(), dout.stride(0) if dout.dim() == 2 else dim,
+    _call(lib().mamba_embedding_backward, what, dout, a, dout.data_ptr(), dout.stride(0) if rows else dim,
           dtable.data_ptr(), dtable.stride(0), int(bool(accumulate)), ws, ws_len)
     return dtable
 
 
 def _dropout(what, x, p, seed, offset, residual, out_dtype, out, state):
     torch = _torch()
-    x_dt = _float_dtype(x.dtype, "x", what)
+    dtype = x.dtype
+    x_dt = _float_dtype(dtype, "x", what)
     if out_dtype is None:
-        out_dtype = out.dtype if out is not None else x.dtype if residual is None else torch.float32
-    o_dt = _float_dtype(out_dtype, "out", what)
+        out_dtype = out.dtype if out is not None else dtype if residual is None else torch.float32
+    o_dt = x_dt if out_dtype is dtype else _float_dtype(out_dtype, "out", what)
     shape, dev, rows2 = x.shape, x.device, x.dim() == 2
-    _check_tensor(x, "x", what, shape, x.dtype, dev, rows2)
+    if not x.is_contiguous():
+        _check_tensor(x, "x", what, shape, dtype, dev, rows2)
     if residual is not None:
         _check_tensor(residual, "residual", what, shape, torch.float32, dev, rows2)
     if state is not None:
         _check_tensor(state, "state", what, (2,), torch.int64, dev)
-    _require(0 <= seed < 1 << 64 and 0 <= offset < 1 << 64, "%s: seed and offset must fit 64 bits" % what)
-    out = _output(out, "out", what, shape, out_dtype, x, rows2)
+    if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
+        raise MambaError("%s: seed and offset must fit 64 bits" % what)
+    if out is None:
+        out = _fresh(x, out_dtype)
+    else:
+        _check_tensor(out, "out", what, shape, out_dtype, dev, rows2)
     if rows2:
         rows, cols = shape
         sx, sr, so = x.stride(0), 0 if residual is None else residual.stride(0), out.stride(0)
@@ -1213,6 +1246,13 @@ def dropout_backward(dout, p, seed=0, offset=0, out_dtype=None, dx=None, state=N
 _NO_STRIDE = (0, 0, 0)
 
 
+def _check_view(t, name, what, shape, dtype, device):
+    """t is a tensor of this shape, dtype and device, with any strides."""
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
+        raise MambaError("%s: %s must be %s %s on %s, got %s %s on %s"
+                         % (what, name, dtype, tuple(shape), device, t.dtype, tuple(t.shape), t.device))
+
+
 @_on_stream
 def selective_scan_backward(dy, x, delta, A, B, C, D=None, z=None, dt_bias=None, initial_state=None,
                             dfinal_state=None, dx=None, ddelta=None, dz=None, workspace=None):
@@ -1226,45 +1266,54 @@ def selective_scan_backward(dy, x, delta, A, B, C, D=None, z=None, dt_bias=None,
     in B's, the others FP32; None for an argument that was not given."""
     torch = _torch()
     what = "mamba_selective_scan_backward"
-    _require(x.dim() == 3 and A.dim() == 2, "%s: x must be [batch, L, dim] and A [dim, N]" % what)
-    x_dt, d_dt = _float_dtype(x.dtype, "x", what), _float_dtype(delta.dtype, "delta", what)
-    b_dt = _float_dtype(B.dtype, "B", what)
-    shape, dev, f32 = x.shape, x.device, torch.float32
+    shape, dev, f32, dtype, d_dtype, b_dtype = x.shape, x.device, torch.float32, x.dtype, delta.dtype, B.dtype
+    if len(shape) != 3 or A.dim() != 2:
+        raise MambaError("%s: x must be [batch, L, dim] and A [dim, N]" % what)
+    x_dt, d_dt = _float_dtype(dtype, "x", what), _float_dtype(d_dtype, "delta", what)
+    b_dt = _float_dtype(b_dtype, "B", what)
     (bsz, L, dim), N = shape, A.shape[1]
-
-    def view(t, name, shape, dtype):
-        if t is not None and (t.shape != shape or t.dtype is not dtype or t.device != dev):
-            raise MambaError("%s: %s must be %s %s on %s, got %s %s on %s"
-                             % (what, name, dtype, tuple(shape), dev, t.dtype, tuple(t.shape), t.device))
-
-    view(delta, "delta", shape, delta.dtype)
-    for t, name in ((dy, "dy"), (z, "z"), (dx, "dx"), (dz, "dz")):
-        view(t, name, shape, x.dtype)
-    view(ddelta, "ddelta", shape, delta.dtype)
-    view(B, "B", (bsz, L, N), B.dtype)
-    view(C, "C", (bsz, L, N), B.dtype)
+    states, rows = (bsz, dim, N), (bsz, L, N)
+    like = torch.empty_like
+    _check_view(dy, "dy", what, shape, dtype, dev)
+    _check_view(delta, "delta", what, shape, d_dtype, dev)
+    _check_view(B, "B", what, rows, b_dtype, dev)
+    _check_view(C, "C", what, rows, b_dtype, dev)
     _check_tensor(A, "A", what, (dim, N), f32, dev)
-    for t, name in ((D, "D"), (dt_bias, "dt_bias")):
-        if t is not None:
-            _check_tensor(t, name, what, (dim,), f32, dev)
-    for t, name in ((initial_state, "initial_state"), (dfinal_state, "dfinal_state")):
-        if t is not None:
-            _check_tensor(t, name, what, (bsz, dim, N), f32, dev)
-    _require(z is not None or dz is None, "%s: dz without a gate" % what)
-    dx = x.new_empty(shape) if dx is None else dx
-    ddelta = delta.new_empty(shape) if ddelta is None else ddelta
-    if z is not None and dz is None:
-        dz = x.new_empty(shape)
-    dB, dC = B.new_empty((bsz, L, N)), B.new_empty((bsz, L, N))
-    dA = torch.empty_like(A)
-    dD = None if D is None else torch.empty_like(D)
-    ddt_bias = None if dt_bias is None else torch.empty_like(dt_bias)
-    dh0 = None if initial_state is None else torch.empty_like(initial_state)
+    dD = ddt_bias = dh0 = None
+    if D is not None:
+        _check_tensor(D, "D", what, (dim,), f32, dev)
+        dD = like(D)
+    if dt_bias is not None:
+        _check_tensor(dt_bias, "dt_bias", what, (dim,), f32, dev)
+        ddt_bias = like(dt_bias)
+    if initial_state is not None:
+        _check_tensor(initial_state, "initial_state", what, states, f32, dev)
+        dh0 = like(initial_state)
+    if dfinal_state is not None:
+        _check_tensor(dfinal_state, "dfinal_state", what, states, f32, dev)
+    sz = sdz = _NO_STRIDE
+    if z is not None:
+        _check_view(z, "z", what, shape, dtype, dev)
+        if dz is None:
+            dz = like(z)
+        else:
+            _check_view(dz, "dz", what, shape, dtype, dev)
+        sz, sdz = z.stride(), dz.stride()
+    elif dz is not None:
+        raise MambaError("%s: dz without a gate" % what)
+    if dx is None:
+        dx = like(x)
+    else:
+        _check_view(dx, "dx", what, shape, dtype, dev)
+    if ddelta is None:
+        ddelta = like(delta)
+    else:
+        _check_view(ddelta, "ddelta", what, shape, d_dtype, dev)
+    dB, dC, dA = like(B), like(C), like(A)
     if dim == 0:
         dB.zero_()
         dC.zero_()
         return dx, ddelta, dA, dB, dC, dD, dz, ddt_bias, dh0
-    sz, sdz = (_NO_STRIDE, _NO_STRIDE) if z is None else (z.stride(), dz.stride())
     a = _packed(what, MambaScanArgs, _SCAN_ARGS, x.data_ptr(), delta.data_ptr(), B.data_ptr(), C.data_ptr(),
                 A.data_ptr(), _ptr0(D), 0, 0, _ptr0(z), _ptr0(dt_bias), _ptr0(initial_state), bsz, L, dim, N, x_dt, d_dt,
                 b_dt, 0, *x.stride(), *delta.stride(), *B.stride(), *C.stride(), *sz, *_NO_STRIDE)
@@ -1285,21 +1334,25 @@ def causal_conv1d_backward(dy, x, w, bias=None, silu=True, dx=None, workspace=No
     without a bias."""
     torch = _torch()
     what = "mamba_causal_conv1d_backward"
-    _require(x.dim() == 3 and w.dim() == 2, "%s: x must be [batch, L, dim] and w [dim, K]" % what)
-    dt = _float_dtype(x.dtype, "x", what)
-    shape, dev = x.shape, x.device
-    for t, name in ((dy, "dy"), (dx, "dx")):
-        if t is not None and (t.shape != shape or t.dtype is not x.dtype or t.device != dev):
-            raise MambaError("%s: %s must be like x" % (what, name))
-    _check_tensor(w, "w", what, (shape[2], w.shape[1]), torch.float32, dev)
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    if len(shape) != 3 or w.dim() != 2:
+        raise MambaError("%s: x must be [batch, L, dim] and w [dim, K]" % what)
+    dt = _float_dtype(dtype, "x", what)
+    K = w.shape[1]
+    _check_view(dy, "dy", what, shape, dtype, dev)
+    _check_tensor(w, "w", what, (shape[2], K), torch.float32, dev)
+    dbias = None
     if bias is not None:
         _check_tensor(bias, "bias", what, shape[2:], torch.float32, dev)
-    dx = x.new_empty(shape) if dx is None else dx
+        dbias = torch.empty_like(bias)
+    if dx is None:
+        dx = torch.empty_like(x)
+    else:
+        _check_view(dx, "dx", what, shape, dtype, dev)
     dw = torch.empty_like(w)
-    dbias = None if bias is None else torch.empty_like(bias)
     a = _packed(what, MambaConvGradArgs, _CONV_GRAD_ARGS, dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr0(bias),
-                dx.data_ptr(), dw.data_ptr(), _ptr0(dbias), *shape, w.shape[1], int(bool(silu)), dt, *dy.stride(),
-                *x.stride(), *dx.stride())
+                dx.data_ptr(), dw.data_ptr(), _ptr0(dbias), *shape, K, 1 if silu else 0, dt, *dy.stride(), *x.stride(),
+                *dx.stride())
     ws, ws_len, owner = _workspace(what, lib().mamba_causal_conv1d_backward_workspace(a), workspace, x)
     _call(lib().mamba_causal_conv1d_backward, what, x, a, ws, ws_len)
     return dx, dw, dbias
