@@ -111,6 +111,7 @@ const char *mamba_last_error(void);
  * sequence tile before it exceeded the same bound.  Bit 7: the same as bit 4
  * for mamba_linear_i8's tensor-core kernel.  Bit 8: the same for the row
  * fetches of mamba_block_norm, mamba_layer_norm and their backward passes.
+ * Bit 9: the same for the row fetches of mamba_embedding_backward.
  * Waits for the device; clear != 0 resets them. */
 unsigned mamba_device_status(int clear);
 
@@ -627,7 +628,8 @@ int mamba_embedding(const MambaEmbeddingArgs *a, void *stream);
  * not occur are zero.  accumulate != 0: the sums are added to dtable instead,
  * and rows whose id does not occur are left as they were.  ids outside
  * [0, vocab) contribute nothing.  dout [tokens, dim] of a->out_dtype with row
- * stride dout_stride.  Workspace: 16-byte aligned device memory; calls that
+ * stride dout_stride; its rows may be read with the up to 15 bytes before and
+ * behind them, which have no effect.  Workspace: 16-byte aligned device memory; calls that
  * share it must not overlap on the GPU. */
 size_t mamba_embedding_workspace(const MambaEmbeddingArgs *a);
 int mamba_embedding_backward(const MambaEmbeddingArgs *a, const void *dout, int64_t dout_stride, float *dtable,

@@ -5,16 +5,20 @@
 // Lookup: a gather, bound by bytes (the rows that occur, once, and out).
 //
 // Gradient: no atomics, so that the sums have one order.  The ids are sorted
-// with their positions (stable, least significant digit first), the sorted
-// list is cut into chunks of equal length, and one CTA sums the rows of a
-// chunk, id by id.  An id that lies within one chunk is finished there; the
-// sums of one that spans several leave as partial rows, which a second kernel
-// adds in order.  Frequent ids so cost no more than others.
+// with their positions, the sorted list is cut into parts of equal length, and
+// one CTA sums the rows of a part, id by id.  An id that lies within one part is
+// finished there; the sums of one that spans several leave as partial rows,
+// which a second kernel adds in order.  Frequent ids so cost no more than others.
+// Rows of the table that no token names are zeroed beside the sums, each row
+// of the table being written once.  Bound by bytes: dout once, the table once.
 #include "common.cuh"
 #include "internal.h"
 #include "rows.cuh"
 
 namespace mb {
+
+__device__ unsigned int g_embedding_error = 0;
+
 namespace {
 
 // ---- lookup -------------------------------------------------------------------
@@ -89,9 +93,16 @@ int launch_lookup(const LookupParams &p, bool vec, cudaStream_t st) {
 }
 
 // ---- sort -----------------------------------------------------------------------
+// Stable, 8 bits at a time, least significant first.  Up to kTinyTokens tokens
+// one CTA runs all passes in shared memory; above that each pass counts the
+// digits of every tile and then moves the tile's items, whose places a CTA
+// finds from the counts itself while there are few tiles (kFewTiles), and from
+// their running sums, made by a kernel in between, when there are many.
 constexpr int kDigitBits = 8, kDigits = 1 << kDigitBits;
-constexpr int kSortThreads = 512, kSortItems = 8, kSortTile = kSortThreads * kSortItems;
+constexpr int kSortThreads = 256, kSortItems = 4, kSortTile = kSortThreads * kSortItems;
 constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kFewTiles = 64;
+constexpr int kTinyThreads = 1024, kTinyItems = 4, kTinyTokens = kTinyThreads * kTinyItems, kTinyWarps = kTinyThreads / 32;
 
 // Key of a token: its id, or `vocab` (behind all ids) for one outside the table.
 __device__ __forceinline__ uint32_t token_key(const void *ids, bool wide, int64_t t, uint32_t vocab) {
@@ -103,13 +114,115 @@ struct SortPass {
     const void *ids;  // first pass: the keys come from here; NULL: from keys_in, pos_in
     const uint32_t *keys_in, *pos_in;
     uint32_t *keys_out, *pos_out;
-    uint32_t *hist;  // [kDigits][tiles]: counts, then first places
+    uint32_t *hist;  // [tiles][kDigits] counts, or with many tiles [kDigits][tiles] first places
     uint32_t n, vocab;
-    int shift, tiles;
-    bool wide;
+    int shift, bits, tiles;
+    bool wide, few;
 };
 __device__ __forceinline__ uint32_t pass_key(const SortPass &p, uint32_t i) {
     return p.ids ? token_key(p.ids, p.wide, i, p.vocab) : p.keys_in[i];
+}
+
+// Place of each of a warp's items among the warp's items of the same digit
+// (items in the order k * 32 + lane; digit kDigits: no item); `count` [kDigits]
+// ends as the warp's numbers.  The lanes of one digit find each other by a match.
+template <int ITEMS, typename Digit>
+__device__ __forceinline__ void rank_in_warp(uint32_t *count, uint32_t (&rank)[ITEMS], Digit digit) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const uint32_t d = digit(k), same = __match_any_sync(0xffffffffu, d);
+        const uint32_t before = d < kDigits ? count[d] : 0;
+        rank[k] = before + __popc(same & ((1u << lane) - 1));
+        __syncwarp();
+        if (d < kDigits && lane == __ffs(same) - 1) count[d] = before + __popc(same);
+        __syncwarp();
+    }
+}
+// Exclusive sum over kDigits threads' values (the CTA's first kDigits threads; all call).
+__device__ __forceinline__ uint32_t exclusive_digits(uint32_t v, uint32_t *warp_sum) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t in = v;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, in, o);
+        if (lane >= o) in += u;
+    }
+    if (warp < kDigits / 32 && lane == 31) warp_sum[warp] = in;
+    __syncthreads();
+    uint32_t base = 0;
+    for (int w = 0; w < warp && w < kDigits / 32; ++w) base += warp_sum[w];
+    __syncthreads();
+    return base + in - v;
+}
+
+// All passes over at most kTinyTokens tokens.
+struct TinySmem {
+    uint32_t key[kTinyTokens], pos[kTinyTokens];
+    uint16_t count[kTinyWarps][kDigits];
+    uint32_t warp_sum[kDigits / 32];
+};
+__global__ void __launch_bounds__(kTinyThreads) sort_tiny_kernel(const SortPass p) {
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    TinySmem &sm = *reinterpret_cast<TinySmem *>(smem_raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int k = 0; k < kTinyItems; ++k) {
+        const uint32_t i = k * kTinyThreads + tid;
+        if (i < p.n) {
+            sm.key[i] = token_key(p.ids, p.wide, i, p.vocab);
+            sm.pos[i] = i;
+        }
+    }
+    for (int shift = 0; shift < p.bits; shift += kDigitBits) {
+        for (int d = tid; d < kTinyWarps * kDigits / 2; d += kTinyThreads) reinterpret_cast<uint32_t *>(sm.count)[d] = 0;
+        __syncthreads();
+        uint32_t key[kTinyItems], pos[kTinyItems], rank[kTinyItems];
+#pragma unroll
+        for (int k = 0; k < kTinyItems; ++k) {
+            const uint32_t i = warp * (32 * kTinyItems) + k * 32 + lane;
+            key[k] = i < p.n ? sm.key[i] : 0;
+            pos[k] = i < p.n ? sm.pos[i] : 0;
+        }
+        auto digit = [&](int k) {
+            const uint32_t i = warp * (32 * kTinyItems) + k * 32 + lane;
+            return i < p.n ? key[k] >> shift & (kDigits - 1) : (uint32_t)kDigits;
+        };
+#pragma unroll
+        for (int k = 0; k < kTinyItems; ++k) {
+            const uint32_t d = digit(k), same = __match_any_sync(0xffffffffu, d);
+            const uint32_t before = d < kDigits ? sm.count[warp][d] : 0;
+            rank[k] = before + __popc(same & ((1u << lane) - 1));
+            __syncwarp();
+            if (d < kDigits && lane == __ffs(same) - 1) sm.count[warp][d] = (uint16_t)(before + __popc(same));
+            __syncwarp();
+        }
+        __syncthreads();
+        uint32_t total = 0;
+        if (tid < kDigits)
+            for (int w = 0; w < kTinyWarps; ++w) total += sm.count[w][tid];
+        uint32_t run = exclusive_digits(total, sm.warp_sum);
+        if (tid < kDigits)
+            for (int w = 0; w < kTinyWarps; ++w) {
+                const uint32_t c = sm.count[w][tid];
+                sm.count[w][tid] = (uint16_t)run;
+                run += c;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kTinyItems; ++k) {
+            const uint32_t d = digit(k);
+            if (d < kDigits) {
+                const uint32_t to = sm.count[warp][d] + rank[k];
+                sm.key[to] = key[k];
+                sm.pos[to] = pos[k];
+            }
+        }
+        __syncthreads();
+    }
+    for (uint32_t i = tid; i < p.n; i += kTinyThreads) {
+        p.keys_out[i] = sm.key[i];
+        p.pos_out[i] = sm.pos[i];
+    }
 }
 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortPass p) {
@@ -123,7 +236,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortPass
         if (i < p.n) atomicAdd(&count[pass_key(p, i) >> p.shift & (kDigits - 1)], 1u);  // whole numbers: any order
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < kDigits; d += kSortThreads) p.hist[(size_t)d * p.tiles + blockIdx.x] = count[d];
+    for (int d = threadIdx.x; d < kDigits; d += kSortThreads)
+        p.hist[p.few ? (size_t)blockIdx.x * kDigits + d : (size_t)d * p.tiles + blockIdx.x] = count[d];
 }
 
 // Exclusive sums of `n` counts in place, one CTA.
@@ -172,12 +286,28 @@ __global__ void __launch_bounds__(1024) sort_sum_kernel(uint32_t *v, uint32_t n)
 }
 
 // Moves a tile's items to their places.  Warp w of the tile holds items
-// w * 32 * kSortItems + k * 32 + lane and counts its digits round by round (the
-// lanes of one digit find each other by a match), so equal digits keep their order.
+// w * 32 * kSortItems + k * 32 + lane, so equal digits keep their order.
 __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const SortPass p) {
+    static_assert(kSortThreads == kDigits, "a thread per digit");
     __shared__ uint32_t count[kSortWarps][kDigits];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int d = threadIdx.x; d < kSortWarps * kDigits; d += kSortThreads) count[d / kDigits][d % kDigits] = 0;
+    __shared__ uint32_t warp_sum[kDigits / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digit_of = threadIdx.x;
+    // first place of this tile's items of digit `digit_of`
+    uint32_t first = 0;
+    if (p.few) {
+        uint32_t before = 0, all = 0;
+#pragma unroll 8
+        for (int t = 0; t < p.tiles; ++t) {
+            const uint32_t c = p.hist[(size_t)t * kDigits + digit_of];
+            if (t < (int)blockIdx.x) before += c;
+            all += c;
+        }
+        first = exclusive_digits(all, warp_sum) + before;
+    } else {
+        first = p.hist[(size_t)digit_of * p.tiles + blockIdx.x];
+    }
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) count[w][digit_of] = 0;
     __syncthreads();
     const uint32_t base = blockIdx.x * (uint32_t)kSortTile + warp * (32 * kSortItems);
     uint32_t key[kSortItems], rank[kSortItems];
@@ -186,25 +316,15 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const SortPass 
         const uint32_t i = base + k * 32 + lane;
         key[k] = i < p.n ? pass_key(p, i) : 0;
     }
-#pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        const uint32_t i = base + k * 32 + lane;
-        const uint32_t d = i < p.n ? key[k] >> p.shift & (kDigits - 1) : kDigits;  // kDigits: no item
-        const uint32_t same = __match_any_sync(0xffffffffu, d);
-        const uint32_t before = d < kDigits ? count[warp][d] : 0;
-        rank[k] = before + __popc(same & ((1u << lane) - 1));
-        __syncwarp();
-        if (d < kDigits && lane == __ffs(same) - 1) count[warp][d] = before + __popc(same);
-        __syncwarp();
-    }
+    rank_in_warp<kSortItems>(count[warp], rank, [&](int k) {
+        return base + k * 32 + lane < p.n ? key[k] >> p.shift & (kDigits - 1) : (uint32_t)kDigits;
+    });
     __syncthreads();
-    for (int d = threadIdx.x; d < kDigits; d += kSortThreads) {
-        uint32_t run = p.hist[(size_t)d * p.tiles + blockIdx.x];
-        for (int w = 0; w < kSortWarps; ++w) {
-            const uint32_t c = count[w][d];
-            count[w][d] = run;
-            run += c;
-        }
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = count[w][digit_of];
+        count[w][digit_of] = first;
+        first += c;
     }
     __syncthreads();
 #pragma unroll
@@ -219,18 +339,23 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const SortPass 
 }
 
 // ---- sums -----------------------------------------------------------------------
-constexpr int kChunk = 16;       // sorted tokens per CTA
-constexpr int kSumRows = 8;      // rows a thread has in flight
-constexpr int kSumCtaThreads = 256;
+// The sorted list is cut into equal parts, one per CTA and about as many as fit
+// the GPU at once, so that an id that occurs often spans few of them.  Rows of
+// dout arrive through a ring in shared memory, fetched ahead by bulk copies.
+constexpr unsigned kErrEmbeddingTimeout = 512u;
+constexpr int kSumThreadsE = 256;
+constexpr int kSumStages = 8;
+constexpr int kZeroRows = 64;  // table rows that a CTA looks after
 
 struct SumParams {
     const uint32_t *keys, *pos;
     const void *dout;
     float *dtable;
-    float *part;  // [chunks][2][dim]: slot 0 an id begun in an earlier chunk, 1 one that goes on in the next
+    float *part;  // [parts][2][dim]: slot 0 an id begun in an earlier part, 1 one that goes on in the next
     int64_t dout_stride, table_stride;
-    uint32_t n, vocab;
-    int dim, chunks;
+    uint32_t n, vocab, len;  // len: sorted tokens per part
+    int dim, parts, cols, stages;  // cols: columns of a CTA
+    uint32_t stage;                // bytes of a row's place in the ring
     float scale;
     bool accumulate;
 };
@@ -245,57 +370,140 @@ __device__ __forceinline__ void put_row(const SumParams &p, uint32_t key, int c,
     store_n(to, v);
 }
 
-// blockIdx.x: chunk; blockIdx.y: block of columns.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kSumCtaThreads) embedding_sum_kernel(const SumParams p) {
-    __shared__ uint32_t key[kChunk + 2], pos[kChunk];  // key[1 + k]: token k of the chunk, around it its neighbours
-    const uint32_t first = blockIdx.x * (uint32_t)kChunk;
-    if (threadIdx.x < kChunk + 2) {
-        const uint32_t i = first + threadIdx.x - 1;  // wraps at -1: beyond n
-        key[threadIdx.x] = i < p.n ? p.keys[i] : p.vocab;
-    }
-    if (threadIdx.x < kChunk) pos[threadIdx.x] = first + threadIdx.x < p.n ? p.pos[first + threadIdx.x] : 0;
-    __syncthreads();
-    const int c = (blockIdx.y * kSumCtaThreads + threadIdx.x) * VEC;
-    if (c >= p.dim) return;
-    float sum[VEC] = {};
-    bool begun = key[0] == key[1] && first > 0;  // the current id begun in an earlier chunk
-#pragma unroll 1
-    for (int k0 = 0; k0 < kChunk; k0 += kSumRows) {
-        float v[kSumRows][VEC];
-#pragma unroll
-        for (int k = 0; k < kSumRows; ++k)
-            if (key[1 + k0 + k] < p.vocab)
-                load_n(static_cast<const T *>(p.dout) + (int64_t)pos[k0 + k] * p.dout_stride + c, v[k]);
-#pragma unroll
-        for (int k = 0; k < kSumRows; ++k) {
-            const uint32_t id = key[1 + k0 + k];
-            if (id >= p.vocab) return;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) sum[e] += v[k][e];
-            const bool last = k0 + k == kChunk - 1, ends = key[2 + k0 + k] != id;
-            if (ends || last) {
-                if (!begun && ends)
-                    put_row(p, id, c, sum);
-                else
-                    store_n(p.part + ((int64_t)blockIdx.x * 2 + (begun ? 0 : 1)) * p.dim + c, sum);
-                begun = false;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
-            }
+// Rows of the table that no token names become zero.
+__device__ void zero_rows(const SumParams &p, int64_t tile) {
+    __shared__ uint8_t present[kZeroRows];
+    const uint32_t v0 = (uint32_t)(tile * kZeroRows), v1 = (uint32_t)min((int64_t)p.vocab, (tile + 1) * kZeroRows);
+    if (v0 + threadIdx.x < v1) {
+        const uint32_t v = v0 + threadIdx.x;
+        uint32_t lo = 0, hi = p.n;  // the first sorted token with an id of v or more
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (p.keys[mid] < v)
+                lo = mid + 1;
+            else
+                hi = mid;
         }
+        present[threadIdx.x] = lo < p.n && p.keys[lo] == v;
+    }
+    __syncthreads();
+    const bool vec = p.dim % 4 == 0 && p.table_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.dtable) % 16 == 0;
+    for (uint32_t v = v0; v < v1; ++v) {
+        if (present[v - v0]) continue;
+        float *row = p.dtable + (int64_t)v * p.table_stride;
+        if (vec)
+            for (int c = threadIdx.x * 4; c < p.dim; c += kSumThreadsE * 4)
+                *reinterpret_cast<float4 *>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+        else
+            for (int c = threadIdx.x; c < p.dim; c += kSumThreadsE) row[c] = 0.f;
     }
 }
 
-// blockIdx.x: the chunk in which an id begins that goes on in the next ones.
+// blockIdx.x: part, and behind the parts tiles of the table to zero; blockIdx.y:
+// block of columns (the zeroing has one).  A thread has NV groups of VEC columns,
+// group g at column (g * threads + t) * VEC.
+template <typename T, int VEC, int NV>
+__global__ void __launch_bounds__(kSumThreadsE) embedding_sum_kernel(const SumParams p) {
+    if (blockIdx.x >= (unsigned)p.parts) {
+        if (blockIdx.y == 0) zero_rows(p, blockIdx.x - p.parts);
+        return;
+    }
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ uint64_t full[kSumStages];
+    __shared__ LostCopies lost;
+    const uint32_t first = blockIdx.x * p.len, end = min(p.n, first + p.len);
+    const int c0 = blockIdx.y * p.cols, cols = min(p.cols, p.dim - c0);
+    // a row's columns start at `from`; what precedes them in their 16 bytes is copied too
+    auto from = [&](uint32_t pos) {
+        return reinterpret_cast<const uint8_t *>(static_cast<const T *>(p.dout) + (int64_t)pos * p.dout_stride + c0);
+    };
+    auto fetch = [&](uint32_t pos, int s) {
+        const uint8_t *src = from(pos);
+        const uint32_t shift = (uint32_t)reinterpret_cast<uintptr_t>(src) & 15u;
+        const uint32_t bytes = (shift + cols * (uint32_t)sizeof(T) + 15) / 16 * 16;
+        mbar_arrive_expect_tx(&full[s], bytes);
+        bulk_load(ring + s * p.stage, src - shift, bytes, &full[s]);
+    };
+    // tokens outside the table are last: nothing behind the first of them counts
+    uint32_t live = end;
+    if (first < end && p.keys[end - 1] >= p.vocab) {
+        uint32_t lo = first, hi = end - 1;
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (p.keys[mid] < p.vocab)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        live = lo;
+    }
+    if (threadIdx.x == 0) {
+        lost = LostCopies{};
+        for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+        fence_mbar_init();
+        for (int s = 0; s < p.stages && first + s < live; ++s) fetch(p.pos[first + s], s);
+    }
+    __syncthreads();
+    if (first >= live) return;
+    // the next row to fetch, looked up a row ahead
+    uint32_t fetch_pos = first + p.stages < live ? p.pos[first + p.stages] : 0;
+    float sum[NV][VEC] = {};
+    uint32_t id = p.keys[first];
+    bool begun = first > 0 && p.keys[first - 1] == id;  // the current id begun in an earlier part
+    RingPlace at;
+    uint32_t next = first + 1 < p.n ? p.keys[first + 1] : p.vocab;
+    for (uint32_t i = first; i < live; ++i) {
+        const uint32_t after = i + 2 < p.n ? p.keys[i + 2] : p.vocab;  // on its way while the row is added
+        const uint32_t shift = VEC == 1 ? (uint32_t)reinterpret_cast<uintptr_t>(from(p.pos[i])) & 15u : 0u;
+        if (!await_copy(full, at.s, at.parity, &lost, kWaitNs)) atomicOr(&g_embedding_error, kErrEmbeddingTimeout);
+        const T *row = reinterpret_cast<const T *>(ring + at.s * p.stage + shift);
+#pragma unroll
+        for (int g = 0; g < NV; ++g) {
+            const int c = (g * kSumThreadsE + threadIdx.x) * VEC;
+            if (c < cols) {
+                float v[VEC];
+                load_n(row + c, v);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) sum[g][e] += v[e];
+            }
+        }
+        __syncthreads();  // the row's place is free
+        if (threadIdx.x == 0 && i + p.stages < live) {
+            if (!lost.flag) fetch(fetch_pos, at.s);
+            if (i + p.stages + 1 < live) fetch_pos = p.pos[i + p.stages + 1];
+        }
+        at.step(p.stages);
+        const bool ends = next != id;
+        if (ends || i + 1 == live) {
+#pragma unroll
+            for (int g = 0; g < NV; ++g) {
+                const int c = (g * kSumThreadsE + threadIdx.x) * VEC;
+                if (c < cols) {
+                    if (!begun && ends)
+                        put_row(p, id, c0 + c, sum[g]);
+                    else
+                        store_n(p.part + ((int64_t)blockIdx.x * 2 + (begun ? 0 : 1)) * p.dim + c0 + c, sum[g]);
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) sum[g][e] = 0.f;
+            }
+            begun = false;
+        }
+        id = next;
+        next = after;
+    }
+    drain_copies(full, p.stages, &lost, kWaitNs);
+}
+
+// blockIdx.x: the part in which an id begins that goes on in the next ones.
 template <int VEC>
-__global__ void __launch_bounds__(kSumCtaThreads) embedding_join_kernel(const SumParams p) {
-    const uint32_t first = blockIdx.x * (uint32_t)kChunk, end = first + kChunk;  // end: the next chunk's first
-    if (end >= p.n) return;
-    const uint32_t id = p.keys[end];
+__global__ void __launch_bounds__(kSumThreadsE) embedding_join_kernel(const SumParams p) {
+    const uint32_t first = blockIdx.x * p.len;
+    if (p.n - first <= p.len) return;  // the last part
+    const uint32_t end = first + p.len, id = p.keys[end];  // end: the next part's first
     if (id >= p.vocab || p.keys[end - 1] != id) return;
     if (first > 0 && p.keys[first - 1] == id) return;  // begun earlier
-    // one behind the id's last token
+    // the id's last token
     uint32_t lo = end, hi = p.n;
     while (lo + 1 < hi) {
         const uint32_t mid = lo + (hi - lo) / 2;
@@ -304,12 +512,12 @@ __global__ void __launch_bounds__(kSumCtaThreads) embedding_join_kernel(const Su
         else
             hi = mid;
     }
-    const int last = (int)(lo / kChunk);
-    const int c = (blockIdx.y * kSumCtaThreads + threadIdx.x) * VEC;
+    const int last = (int)(lo / p.len);
+    const int c = (blockIdx.y * kSumThreadsE + threadIdx.x) * VEC;
     if (c >= p.dim) return;
     float sum[VEC];
     load_n(p.part + ((int64_t)blockIdx.x * 2 + 1) * p.dim + c, sum);
-#pragma unroll 4
+#pragma unroll 8
     for (int k = blockIdx.x + 1; k <= last; ++k) {
         float v[VEC];
         load_n(p.part + (int64_t)k * 2 * p.dim + c, v);
@@ -319,28 +527,38 @@ __global__ void __launch_bounds__(kSumCtaThreads) embedding_join_kernel(const Su
     put_row(p, id, c, sum);
 }
 
-template <typename T>
-int launch_sums(const SumParams &p, bool vec, cudaStream_t st) {
-    const dim3 grid((unsigned)p.chunks, (unsigned)ceil_div(vec ? p.dim / 8 : p.dim, kSumCtaThreads));
-    if (vec) {
-        embedding_sum_kernel<T, 8><<<grid, kSumCtaThreads, 0, st>>>(p);
-        embedding_join_kernel<8><<<grid, kSumCtaThreads, 0, st>>>(p);
-    } else {
-        embedding_sum_kernel<T, 1><<<grid, kSumCtaThreads, 0, st>>>(p);
-        embedding_join_kernel<1><<<grid, kSumCtaThreads, 0, st>>>(p);
-    }
-    return launch_status("embedding_backward sum kernels");
+// Sorted tokens per part, and the parts.  Four CTAs an SM by shared memory.
+uint32_t part_length(int64_t n) { return (uint32_t)std::max<int64_t>(4, ceil_div64(n, 148 * 4)); }
+
+template <typename T, int VEC, int NV>
+int launch_sums(SumParams &p, cudaStream_t st) {
+    p.cols = kSumThreadsE * VEC * NV;
+    const int cols = std::min(p.cols, p.dim);
+    p.stage = (uint32_t)((cols * sizeof(T) + 30) / 128 * 128 + 128);
+    p.stages = (int)std::max<uint32_t>(2, std::min<uint32_t>(kSumStages, kRingBytes / 4 / p.stage));
+    auto kernel = embedding_sum_kernel<T, VEC, NV>;
+    if (allow_smem(kernel)) return -1;
+    const int64_t zero = p.accumulate ? 0 : ceil_div64(p.vocab, kZeroRows);
+    MB_CHECK_ARG(p.parts + zero <= 0x7fffffff, "embedding_backward: too many rows");
+    kernel<<<dim3((unsigned)(p.parts + zero), (unsigned)ceil_div(p.dim, p.cols)), kSumThreadsE,
+             (size_t)p.stage * p.stages, st>>>(p);
+    if (launch_status("embedding_backward sum kernel")) return -1;
+    if (p.parts == 1) return 0;
+    constexpr int JV = VEC == 1 ? 1 : 4;
+    embedding_join_kernel<JV><<<dim3((unsigned)p.parts, (unsigned)ceil_div(p.dim, kSumThreadsE * JV)), kSumThreadsE, 0,
+                                st>>>(p);
+    return launch_status("embedding_backward join kernel");
 }
 
 struct Layout {
     size_t keys[2], pos[2], hist, part, bytes;
-    int tiles, chunks;
+    int tiles, parts;
 };
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 Layout layout(int64_t n, int dim) {
     Layout l{};
     l.tiles = (int)ceil_div64(n, kSortTile);
-    l.chunks = (int)ceil_div64(n, kChunk);
+    l.parts = (int)ceil_div64(n, part_length(n));
     size_t at = 0;
     for (int k = 0; k < 2; ++k) {
         l.keys[k] = at;
@@ -351,7 +569,7 @@ Layout layout(int64_t n, int dim) {
     l.hist = at;
     at += up256((size_t)l.tiles * kDigits * 4);
     l.part = at;
-    at += up256((size_t)l.chunks * 2 * dim * 4);
+    at += up256((size_t)l.parts * 2 * dim * 4);
     l.bytes = at;
     return l;
 }
@@ -373,6 +591,16 @@ int check_embedding(const MambaEmbeddingArgs *a, const std::string &what) {
 }
 
 }  // namespace
+
+unsigned embedding_error_flags(bool clear) {
+    unsigned v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_embedding_error, sizeof(v)) != cudaSuccess) return ~0u;
+    if (clear && v) {
+        const unsigned z = 0;
+        cudaMemcpyToSymbol(g_embedding_error, &z, sizeof(z));
+    }
+    return v;
+}
 
 int embedding(const MambaEmbeddingArgs *a, cudaStream_t st) {
     if (check_embedding(a, "embedding")) return -1;
@@ -421,35 +649,47 @@ int embedding_backward(const MambaEmbeddingArgs *a, const void *dout, int64_t do
         MB_CHECK_ARG(ws && ws_bytes >= embedding_workspace_bytes(a) && aligned_to(ws, 16),
                      "embedding_backward: workspace too small or not 16-byte aligned");
     }
-    const size_t row = (size_t)a->dim * 4, pitch = a->vocab == 1 ? row : (size_t)dtable_stride * 4;
-    if (!accumulate) {
+    if (a->tokens == 0) {
+        if (accumulate) return 0;
+        const size_t row = (size_t)a->dim * 4, pitch = a->vocab == 1 ? row : (size_t)dtable_stride * 4;
         if (pitch == row)
             MB_CUDA_TRY(cudaMemsetAsync(dtable, 0, row * (size_t)a->vocab, st));
         else
             MB_CUDA_TRY(cudaMemset2DAsync(dtable, pitch, 0, row, (size_t)a->vocab, st));
+        return 0;
     }
-    if (a->tokens == 0) return 0;
     const Layout l = layout(a->tokens, a->dim);
     uint8_t *base = static_cast<uint8_t *>(ws);
     SortPass s{};
     s.n = (uint32_t)a->tokens;
     s.vocab = (uint32_t)a->vocab;
     s.tiles = l.tiles;
+    s.few = l.tiles <= kFewTiles;
     s.wide = a->id_bytes == 8;
     s.hist = reinterpret_cast<uint32_t *>(base + l.hist);
-    int bits = 1;
-    while (bits < 32 && (a->vocab >> bits) != 0) ++bits;  // keys are 0 .. vocab
-    int to = 0;
-    for (s.shift = 0; s.shift < bits; s.shift += kDigitBits, to ^= 1) {
-        s.ids = s.shift == 0 ? a->ids : nullptr;
-        s.keys_in = reinterpret_cast<uint32_t *>(base + l.keys[to ^ 1]);
-        s.pos_in = reinterpret_cast<uint32_t *>(base + l.pos[to ^ 1]);
-        s.keys_out = reinterpret_cast<uint32_t *>(base + l.keys[to]);
-        s.pos_out = reinterpret_cast<uint32_t *>(base + l.pos[to]);
-        sort_count_kernel<<<(unsigned)l.tiles, kSortThreads, 0, st>>>(s);
-        sort_sum_kernel<<<1, 1024, 0, st>>>(s.hist, (uint32_t)l.tiles * kDigits);
-        sort_move_kernel<<<(unsigned)l.tiles, kSortThreads, 0, st>>>(s);
-        if (launch_status("embedding_backward sort kernels")) return -1;
+    s.bits = 1;
+    while (s.bits < 32 && (a->vocab >> s.bits) != 0) ++s.bits;  // keys are 0 .. vocab
+    auto words = [&](size_t o) { return reinterpret_cast<uint32_t *>(base + o); };
+    if (a->tokens <= kTinyTokens) {
+        s.ids = a->ids;
+        s.keys_out = words(l.keys[0]);
+        s.pos_out = words(l.pos[0]);
+        if (allow_smem(sort_tiny_kernel)) return -1;
+        sort_tiny_kernel<<<1, kTinyThreads, sizeof(TinySmem), st>>>(s);
+        if (launch_status("embedding_backward sort kernel")) return -1;
+    } else {
+        int to = 0;
+        for (s.shift = 0; s.shift < s.bits; s.shift += kDigitBits, to ^= 1) {
+            s.ids = s.shift == 0 ? a->ids : nullptr;
+            s.keys_in = words(l.keys[to ^ 1]);
+            s.pos_in = words(l.pos[to ^ 1]);
+            s.keys_out = words(l.keys[to]);
+            s.pos_out = words(l.pos[to]);
+            sort_count_kernel<<<(unsigned)l.tiles, kSortThreads, 0, st>>>(s);
+            if (!s.few) sort_sum_kernel<<<1, 1024, 0, st>>>(s.hist, (uint32_t)l.tiles * kDigits);
+            sort_move_kernel<<<(unsigned)l.tiles, kSortThreads, 0, st>>>(s);
+            if (launch_status("embedding_backward sort kernels")) return -1;
+        }
     }
     SumParams p{};
     p.keys = s.keys_out;
@@ -462,12 +702,15 @@ int embedding_backward(const MambaEmbeddingArgs *a, const void *dout, int64_t do
     p.n = s.n;
     p.vocab = s.vocab;
     p.dim = a->dim;
-    p.chunks = l.chunks;
+    p.parts = l.parts;
+    p.len = part_length(a->tokens);
     p.scale = a->scale;
     p.accumulate = accumulate != 0;
     const bool vec = a->dim % 8 == 0 && aligned_to(dout, 16) && aligned_to(dtable, 16) && dtable_stride % 4 == 0 &&
                      (dout_stride * (int64_t)dtype_size(a->out_dtype)) % 16 == 0;
-    return a->out_dtype == MAMBA_F16 ? launch_sums<__half>(p, vec, st) : launch_sums<float>(p, vec, st);
+    // up to 2048 columns a CTA
+    if (a->out_dtype == MAMBA_F16) return vec ? launch_sums<__half, 8, 1>(p, st) : launch_sums<__half, 1, 8>(p, st);
+    return vec ? launch_sums<float, 4, 2>(p, st) : launch_sums<float, 1, 8>(p, st);
 }
 
 }  // namespace mb

@@ -89,6 +89,7 @@ int embedding(const MambaEmbeddingArgs *a, cudaStream_t st);
 size_t embedding_workspace_bytes(const MambaEmbeddingArgs *a);
 int embedding_backward(const MambaEmbeddingArgs *a, const void *dout, int64_t dout_stride, float *dtable,
                        int64_t dtable_stride, int accumulate, void *ws, size_t ws_bytes, cudaStream_t st);
+unsigned embedding_error_flags(bool clear);
 
 // dropout.cu
 int dropout(const MambaDropoutArgs *a, cudaStream_t st);

@@ -1268,10 +1268,11 @@ unsigned mamba_device_status(int clear) {
     const unsigned i8 = mb::linear_i8_error_flags(clear != 0);
     const unsigned norm = mb::block_norm_error_flags(clear != 0);
     const unsigned ln = mb::layer_norm_error_flags(clear != 0);
+    const unsigned emb = mb::embedding_error_flags(clear != 0);
     return (scan == ~0u || gemm == ~0u || lin == ~0u || proj == ~0u || step == ~0u || rec == ~0u || i8 == ~0u ||
-            norm == ~0u || ln == ~0u)
+            norm == ~0u || ln == ~0u || emb == ~0u)
                ? ~0u
-               : (scan | gemm | lin | proj | step | rec | i8 | norm | ln);
+               : (scan | gemm | lin | proj | step | rec | i8 | norm | ln | emb);
 }
 
 int mamba_selftest_bounded_wait(unsigned limit_us, void *stream) {
