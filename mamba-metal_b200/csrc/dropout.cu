@@ -46,22 +46,24 @@ __device__ __forceinline__ uint4 philox(uint64_t counter, uint64_t offset, uint6
 }
 
 constexpr int kDropThreads = 256;
-constexpr int kDropUnroll = 2;  // groups a thread has in flight
+constexpr int kDropElems = 16;  // elements a thread has in flight
 
-// Groups of 8 elements within a row (a contiguous tensor counts as one row).
+// Groups of VEC elements within a row (a contiguous tensor counts as one row):
+// 16 bytes of out.
 template <typename TX, typename TO, bool NONE>
 __global__ void __launch_bounds__(kDropThreads) dropout_vec_kernel(const DropoutParams p) {
+    constexpr int VEC = 16 / sizeof(TO), kDropUnroll = kDropElems / VEC;
     const uint64_t seed = p.state ? p.state[0] : p.seed, offset = p.offset + (p.state ? p.state[1] : 0);
-    const int64_t per_row = p.cols / 8, groups = p.rows * per_row;
+    const int64_t per_row = p.cols / VEC, groups = p.rows * per_row;
     int64_t g = (int64_t)blockIdx.x * (kDropThreads * kDropUnroll) + threadIdx.x;
-    float v[kDropUnroll][8], r[kDropUnroll][8];
+    float v[kDropUnroll][VEC], r[kDropUnroll][VEC];
     int64_t row[kDropUnroll], col[kDropUnroll];
 #pragma unroll
     for (int u = 0; u < kDropUnroll; ++u) {
         const int64_t at = g + u * kDropThreads;
         if (at < groups) {
             row[u] = p.rows == 1 ? 0 : at / per_row;
-            col[u] = (at - row[u] * per_row) * 8;
+            col[u] = (at - row[u] * per_row) * VEC;
             load_n(static_cast<const TX *>(p.x) + row[u] * p.sx + col[u], v[u]);
             if (p.res) load_n(p.res + row[u] * p.sr + col[u], r[u]);
         }
@@ -71,8 +73,8 @@ __global__ void __launch_bounds__(kDropThreads) dropout_vec_kernel(const Dropout
         const int64_t at = g + u * kDropThreads;
         if (at < groups) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint4 w = philox(2 * (uint64_t)at + h, offset, seed);
+            for (int h = 0; h < VEC / 4; ++h) {
+                const uint4 w = philox((uint64_t)at * (VEC / 4) + h, offset, seed);
                 const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -115,7 +117,7 @@ __global__ void __launch_bounds__(kDropThreads) dropout_any_kernel(const Dropout
 template <typename TX, typename TO, bool NONE>
 int launch_dropout(const DropoutParams &p, bool vec, cudaStream_t st) {
     const int64_t n = p.rows * p.cols;
-    const int64_t ctas = ceil_div64(n, vec ? 8 * kDropThreads * kDropUnroll : 4 * kDropThreads);
+    const int64_t ctas = ceil_div64(n, vec ? kDropElems * kDropThreads : 4 * kDropThreads);
     MB_CHECK_ARG(ctas <= 0x7fffffff, "dropout: too many elements");
     if (vec)
         dropout_vec_kernel<TX, TO, NONE><<<(unsigned)ctas, kDropThreads, 0, st>>>(p);

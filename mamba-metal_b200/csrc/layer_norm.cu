@@ -185,6 +185,11 @@ __global__ void __launch_bounds__(MAXT) layer_norm_bwd_kernel(const LayerNormGra
     if (RING) drain_copies(full, ring.stages, &lost, kWaitNs);
 }
 
+// Channels of a group with 16-byte accesses: 8 of FP16 rows, 4 where a row is
+// FP32 (32 bytes a thread would leave half of each access's sectors, or banks,
+// to the next).
+template <typename TX, typename TO> constexpr int kGroup = sizeof(TX) + sizeof(TO) == 4 ? 8 : 4;
+
 // Resident threads per SM of the ring kernels.
 constexpr int kLnThreads = 1024, kLnBwdThreads = 1024;
 
@@ -206,6 +211,7 @@ int ring_ln(const LayerNormParams &p, const RingRow<1> &r, int ctas, int threads
 }
 template <typename TX, typename TO>
 int launch_ln(const LayerNormParams &p, bool vec, cudaStream_t st) {
+    constexpr int V = kGroup<TX, TO>;
     RingRow<1> r{};
     if (p.cols <= 8192) {
         r.src[0] = p.x;
@@ -216,15 +222,15 @@ int launch_ln(const LayerNormParams &p, bool vec, cudaStream_t st) {
         int ctas = ln_ctas(threads, false);
         if (plan_ring<1>(r, p.rows, ctas)) {
             if (vec)
-                return one ? ring_ln<TX, TO, 8, 1>(p, r, ctas, threads, st) : ring_ln<TX, TO, 8, 2>(p, r, ctas, threads, st);
+                return one ? ring_ln<TX, TO, V, 8 / V>(p, r, ctas, threads, st) : ring_ln<TX, TO, V, 16 / V>(p, r, ctas, threads, st);
             return one ? ring_ln<TX, TO, 1, 8>(p, r, ctas, threads, st) : ring_ln<TX, TO, 1, 16>(p, r, ctas, threads, st);
         }
     }
     const unsigned grid = (unsigned)std::min<int64_t>(p.rows, 0x7fffffff);
     if (vec && p.cols <= 4096)
-        layer_norm_kernel<TX, TO, 8, 1, 512, false><<<grid, threads_for(p.cols, 8), 0, st>>>(p, r);
+        layer_norm_kernel<TX, TO, V, 8 / V, 512, false><<<grid, threads_for(p.cols, 8), 0, st>>>(p, r);
     else if (vec)
-        layer_norm_kernel<TX, TO, 8, 2, 1024, false><<<grid, threads_for(p.cols, 16), 0, st>>>(p, r);
+        layer_norm_kernel<TX, TO, V, 16 / V, 1024, false><<<grid, threads_for(p.cols, 16), 0, st>>>(p, r);
     else if (p.cols <= 4096)
         layer_norm_kernel<TX, TO, 1, 4, 1024, false><<<grid, threads_for(p.cols, 4), 0, st>>>(p, r);
     else
@@ -242,6 +248,7 @@ int ring_ln_bwd(const LayerNormGradParams &p, const RingRow<2> &r, unsigned grid
 // grid: CTAs to launch at most; set to those launched (rows of partial sums).
 template <typename TX, typename TO>
 int launch_ln_bwd(const LayerNormGradParams &p, bool vec, unsigned &grid, cudaStream_t st) {
+    constexpr int V = kGroup<TX, TO>;
     const int cols = p.cols;
     RingRow<2> r{};
     if (cols <= 8192) {
@@ -257,17 +264,17 @@ int launch_ln_bwd(const LayerNormGradParams &p, bool vec, unsigned &grid, cudaSt
         if (plan_ring<2>(r, p.rows, ctas)) {
             grid = std::min(grid, (unsigned)(ctas * device_sm_count()));
             if (vec)
-                return one ? ring_ln_bwd<TX, TO, 8, 1>(p, r, grid, threads, st)
-                           : ring_ln_bwd<TX, TO, 8, 2>(p, r, grid, threads, st);
+                return one ? ring_ln_bwd<TX, TO, V, 8 / V>(p, r, grid, threads, st)
+                           : ring_ln_bwd<TX, TO, V, 16 / V>(p, r, grid, threads, st);
             return one ? ring_ln_bwd<TX, TO, 1, 8>(p, r, grid, threads, st)
                        : ring_ln_bwd<TX, TO, 1, 16>(p, r, grid, threads, st);
         }
     }
     grid = std::min(grid, (unsigned)kDirectParts);
     if (vec && cols <= 4096)
-        layer_norm_bwd_kernel<TX, TO, 8, 1, 512, false><<<grid, threads_for(cols, 8), 0, st>>>(p, r);
+        layer_norm_bwd_kernel<TX, TO, V, 8 / V, 512, false><<<grid, threads_for(cols, 8), 0, st>>>(p, r);
     else if (vec)
-        layer_norm_bwd_kernel<TX, TO, 8, 2, 1024, false><<<grid, threads_for(cols, 16), 0, st>>>(p, r);
+        layer_norm_bwd_kernel<TX, TO, V, 16 / V, 1024, false><<<grid, threads_for(cols, 16), 0, st>>>(p, r);
     else if (cols <= 4096)
         layer_norm_bwd_kernel<TX, TO, 1, 4, 1024, false><<<grid, threads_for(cols, 4), 0, st>>>(p, r);
     else

@@ -17,7 +17,7 @@ namespace {
 constexpr int kMaxCols = 16384;
 constexpr int kDirectParts = 296;  // CTAs of the backward pass without a ring: few, so that their partial sums are
 
-// N consecutive elements as FP32; N = 8 by 16-byte accesses.
+// N consecutive elements as FP32; N = 8 by 16-byte accesses, N = 4 by 16 or 8 bytes.
 template <int N>
 __device__ __forceinline__ void load_n(const float *p, float (&v)[N]) {
     if constexpr (N == 1) {
@@ -37,6 +37,14 @@ template <int N>
 __device__ __forceinline__ void load_n(const __half *p, float (&v)[N]) {
     if constexpr (N == 1) {
         v[0] = __half2float(*p);
+    } else if constexpr (N == 4) {
+        const uint2 raw = *reinterpret_cast<const uint2 *>(p);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&raw.y));
+        v[0] = a.x;
+        v[1] = a.y;
+        v[2] = b.x;
+        v[3] = b.y;
     } else {
         const uint4 raw = *reinterpret_cast<const uint4 *>(p);
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -62,6 +70,10 @@ template <int N>
 __device__ __forceinline__ void store_n(__half *p, const float (&v)[N]) {
     if constexpr (N == 1) {
         *p = __float2half_rn(v[0]);
+    } else if constexpr (N == 4) {
+        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+        *reinterpret_cast<uint2 *>(p) =
+            make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
     } else {
         uint32_t w[4];
 #pragma unroll
