@@ -475,7 +475,7 @@ int block_norm_backward(const MambaBlockNormArgs *a, const MambaBlockNormGrads *
                      (g->dy_stride * (int64_t)es) % 16 == 0 && (!a->z || (g->dz_stride * (int64_t)es) % 16 == 0);
     if (a->dtype == MAMBA_F16 ? launch_bwd<__half>(p, vec, grid, st) : launch_bwd<float>(p, vec, grid, st)) return -1;
     if (!g->dw_post && !g->dw_pre) return 0;
-    column_sum_kernel<<<dim3((unsigned)ceil_div(a->cols, 32), 2), kSumThreads, 0, st>>>(
+    column_sum_kernel<><<<dim3((unsigned)ceil_div(a->cols, 32), 2), kSumThreads, 0, st>>>(
         p.part_post, p.part_pre, g->dw_post, g->dw_pre, (int)grid, a->cols);
     return launch_status("block_norm_backward sum kernel");
 }

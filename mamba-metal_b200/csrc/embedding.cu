@@ -83,7 +83,7 @@ int pow2_at_least(int v) {
 template <typename TT, typename TO>
 int launch_lookup(const LookupParams &p, bool vec, cudaStream_t st) {
     // 16 bytes of out a thread: FP32 rows written 32 bytes a thread leave half of each access's sectors empty
-    // (32768 x 2048 into FP32 71 us)
+    // (32768 x 2048 into FP32 71 us in place of 58)
     constexpr int VEC = 16 / sizeof(TO);
     const int tx = std::min(kLookupThreads, pow2_at_least(vec ? p.dim / VEC : p.dim)), ty = kLookupThreads / tx;
     const int64_t grid = ceil_div64(p.tokens, (int64_t)ty * kLookupTokens);
@@ -97,7 +97,9 @@ int launch_lookup(const LookupParams &p, bool vec, cudaStream_t st) {
 
 // ---- sort -----------------------------------------------------------------------
 // Stable, 8 bits at a time, least significant first.  Up to kTinyTokens tokens
-// one CTA runs all passes in shared memory; above that each pass counts the
+// one CTA runs all passes in shared memory, up to 8 times as many a cluster of 8
+// CTAs (32768 tokens, 16 bits: 18 us in one launch, by the kernels below 18 in
+// four); above that each pass counts the
 // digits of every tile and then moves the tile's items, whose places a CTA
 // finds from the counts itself while there are few tiles (kFewTiles), and from
 // their running sums, made by a kernel in between, when there are many.
@@ -129,8 +131,8 @@ __device__ __forceinline__ uint32_t pass_key(const SortPass &p, uint32_t i) {
 // Place of each of a warp's items among the warp's items of the same digit
 // (items in the order k * 32 + lane; digit kDigits: no item); `count` [kDigits]
 // ends as the warp's numbers.  The lanes of one digit find each other by a match.
-template <int ITEMS, typename Digit>
-__device__ __forceinline__ void rank_in_warp(uint32_t *count, uint32_t (&rank)[ITEMS], Digit digit) {
+template <int ITEMS, typename Count, typename Digit>
+__device__ __forceinline__ void rank_in_warp(Count *count, uint32_t (&rank)[ITEMS], Digit digit) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
@@ -138,7 +140,7 @@ __device__ __forceinline__ void rank_in_warp(uint32_t *count, uint32_t (&rank)[I
         const uint32_t before = d < kDigits ? count[d] : 0;
         rank[k] = before + __popc(same & ((1u << lane) - 1));
         __syncwarp();
-        if (d < kDigits && lane == __ffs(same) - 1) count[d] = before + __popc(same);
+        if (d < kDigits && lane == __ffs(same) - 1) count[d] = (Count)(before + __popc(same));
         __syncwarp();
     }
 }
@@ -159,51 +161,77 @@ __device__ __forceinline__ uint32_t exclusive_digits(uint32_t v, uint32_t *warp_
     return base + in - v;
 }
 
-// All passes over at most kTinyTokens tokens.
+// All passes over at most CTAS * kTinyTokens tokens, by one cluster.  CTA r holds
+// places r * kTinyTokens .. of the list in shared memory; in each pass the CTAs
+// tell each other their numbers of each digit and write their items to the
+// places' owners.
+template <int CTAS>
 struct TinySmem {
-    uint32_t key[kTinyTokens], pos[kTinyTokens];
+    uint64_t item[kTinyTokens];  // position, key above it
+    uint32_t total[CTAS][kDigits];
     uint16_t count[kTinyWarps][kDigits];
     uint32_t warp_sum[kDigits / 32];
 };
-__global__ void __launch_bounds__(kTinyThreads) sort_tiny_kernel(const SortPass p) {
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint64_t v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+template <int CTAS>
+__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kTinyThreads) sort_small_kernel(const SortPass p) {
+    static_assert(CTAS * kTinyTokens <= 65536, "places fit 16 bits");
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    TinySmem &sm = *reinterpret_cast<TinySmem *>(smem_raw);
+    TinySmem<CTAS> &sm = *reinterpret_cast<TinySmem<CTAS> *>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t self = CTAS > 1 ? cluster_ctarank() : 0, base = self * kTinyTokens;
+    uint32_t key[kTinyItems], pos[kTinyItems], rank[kTinyItems];
+#pragma unroll
     for (int k = 0; k < kTinyItems; ++k) {
-        const uint32_t i = k * kTinyThreads + tid;
-        if (i < p.n) {
-            sm.key[i] = token_key(p.ids, p.wide, i, p.vocab);
-            sm.pos[i] = i;
-        }
+        const uint32_t i = base + warp * (32 * kTinyItems) + k * 32 + lane;
+        key[k] = i < p.n ? token_key(p.ids, p.wide, i, p.vocab) : 0;
+        pos[k] = i;
     }
+    if (CTAS > 1) cluster_sync();  // every CTA has started: its shared memory may be written
     for (int shift = 0; shift < p.bits; shift += kDigitBits) {
+        if (shift > 0) {
+#pragma unroll
+            for (int k = 0; k < kTinyItems; ++k) {
+                const int i = warp * (32 * kTinyItems) + k * 32 + lane;
+                key[k] = (uint32_t)(sm.item[i] >> 32);
+                pos[k] = (uint32_t)sm.item[i];
+            }
+        }
         for (int d = tid; d < kTinyWarps * kDigits / 2; d += kTinyThreads) reinterpret_cast<uint32_t *>(sm.count)[d] = 0;
         __syncthreads();
-        uint32_t key[kTinyItems], pos[kTinyItems], rank[kTinyItems];
-#pragma unroll
-        for (int k = 0; k < kTinyItems; ++k) {
-            const uint32_t i = warp * (32 * kTinyItems) + k * 32 + lane;
-            key[k] = i < p.n ? sm.key[i] : 0;
-            pos[k] = i < p.n ? sm.pos[i] : 0;
-        }
         auto digit = [&](int k) {
-            const uint32_t i = warp * (32 * kTinyItems) + k * 32 + lane;
+            const uint32_t i = base + warp * (32 * kTinyItems) + k * 32 + lane;
             return i < p.n ? key[k] >> shift & (kDigits - 1) : (uint32_t)kDigits;
         };
-#pragma unroll
-        for (int k = 0; k < kTinyItems; ++k) {
-            const uint32_t d = digit(k), same = __match_any_sync(0xffffffffu, d);
-            const uint32_t before = d < kDigits ? sm.count[warp][d] : 0;
-            rank[k] = before + __popc(same & ((1u << lane) - 1));
-            __syncwarp();
-            if (d < kDigits && lane == __ffs(same) - 1) sm.count[warp][d] = (uint16_t)(before + __popc(same));
-            __syncwarp();
-        }
+        rank_in_warp<kTinyItems>(sm.count[warp], rank, digit);
         __syncthreads();
-        uint32_t total = 0;
-        if (tid < kDigits)
-            for (int w = 0; w < kTinyWarps; ++w) total += sm.count[w][tid];
-        uint32_t run = exclusive_digits(total, sm.warp_sum);
+        uint32_t all = 0, before = 0;
+        if (tid < kDigits) {
+            for (int w = 0; w < kTinyWarps; ++w) all += sm.count[w][tid];
+            if (CTAS > 1) {
+                const uint32_t at = smem_u32(&sm.total[self][tid]);
+#pragma unroll
+                for (int r = 0; r < CTAS; ++r) store_cluster(mapa_shared(at, r), all);
+            }
+        }
+        if (CTAS > 1) {
+            cluster_sync();  // also: every CTA has its items in registers
+            all = 0;
+            if (tid < kDigits) {
+#pragma unroll
+                for (int r = 0; r < CTAS; ++r) {
+                    const uint32_t v = sm.total[r][tid];
+                    if (r < (int)self) before += v;
+                    all += v;
+                }
+            }
+        }
+        uint32_t run = exclusive_digits(all, sm.warp_sum) + before;
         if (tid < kDigits)
             for (int w = 0; w < kTinyWarps; ++w) {
                 const uint32_t c = sm.count[w][tid];
@@ -216,15 +244,21 @@ __global__ void __launch_bounds__(kTinyThreads) sort_tiny_kernel(const SortPass 
             const uint32_t d = digit(k);
             if (d < kDigits) {
                 const uint32_t to = sm.count[warp][d] + rank[k];
-                sm.key[to] = key[k];
-                sm.pos[to] = pos[k];
+                const uint64_t item = (uint64_t)key[k] << 32 | pos[k];
+                if (CTAS > 1)
+                    store_cluster(mapa_shared(smem_u32(&sm.item[to % kTinyTokens]), to / kTinyTokens), item);
+                else
+                    sm.item[to] = item;
             }
         }
-        __syncthreads();
+        if (CTAS > 1)
+            cluster_sync();
+        else
+            __syncthreads();
     }
-    for (uint32_t i = tid; i < p.n; i += kTinyThreads) {
-        p.keys_out[i] = sm.key[i];
-        p.pos_out[i] = sm.pos[i];
+    for (uint32_t i = tid; i < kTinyTokens && base + i < p.n; i += kTinyThreads) {
+        p.keys_out[base + i] = (uint32_t)(sm.item[i] >> 32);
+        p.pos_out[base + i] = (uint32_t)sm.item[i];
     }
 }
 
@@ -339,6 +373,14 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(const SortPass 
             p.pos_out[to] = p.ids ? i : p.pos_in[i];
         }
     }
+}
+
+constexpr int kSmallCtas = 8;
+template <int CTAS>
+int launch_small(const SortPass &p, cudaStream_t st) {
+    if (allow_smem(sort_small_kernel<CTAS>)) return -1;
+    sort_small_kernel<CTAS><<<CTAS, kTinyThreads, sizeof(TinySmem<CTAS>), st>>>(p);
+    return launch_status("embedding_backward sort kernel");
 }
 
 // ---- sums -----------------------------------------------------------------------
@@ -506,13 +548,16 @@ __global__ void __launch_bounds__(kSumThreadsE) embedding_join_kernel(const SumP
     const uint32_t end = first + p.len, id = p.keys[end];  // end: the next part's first
     if (id >= p.vocab || p.keys[end - 1] != id) return;
     if (first > 0 && p.keys[first - 1] == id) return;  // begun earlier
-    int last = blockIdx.x + 1, beyond = p.parts;  // the last part that starts with the id
-    while (last + 1 < beyond) {
-        const int mid = last + (beyond - last) / 2;
-        if (p.keys[(uint32_t)mid * p.len] == id)
-            last = mid;
-        else
-            beyond = mid;
+    // the last part that starts with the id: each warp looks at 32 at once
+    int last = blockIdx.x + 1;
+    for (;;) {
+        const int part = last + 1 + (threadIdx.x & 31);
+        const uint32_t other = __ballot_sync(0xffffffffu, part >= p.parts || p.keys[(uint32_t)part * p.len] != id);
+        if (other) {
+            last += __ffs(other) - 1;
+            break;
+        }
+        last += 32;
     }
     const int c = (blockIdx.y * kSumThreadsE + threadIdx.x) * VEC;
     if (c >= p.dim) return;
@@ -671,13 +716,11 @@ int embedding_backward(const MambaEmbeddingArgs *a, const void *dout, int64_t do
     s.bits = 1;
     while (s.bits < 32 && (a->vocab >> s.bits) != 0) ++s.bits;  // keys are 0 .. vocab
     auto words = [&](size_t o) { return reinterpret_cast<uint32_t *>(base + o); };
-    if (a->tokens <= kTinyTokens) {
+    if (a->tokens <= kSmallCtas * kTinyTokens) {
         s.ids = a->ids;
         s.keys_out = words(l.keys[0]);
         s.pos_out = words(l.pos[0]);
-        if (allow_smem(sort_tiny_kernel)) return -1;
-        sort_tiny_kernel<<<1, kTinyThreads, sizeof(TinySmem), st>>>(s);
-        if (launch_status("embedding_backward sort kernel")) return -1;
+        if (a->tokens <= kTinyTokens ? launch_small<1>(s, st) : launch_small<kSmallCtas>(s, st)) return -1;
     } else {
         int to = 0;
         for (s.shift = 0; s.shift < s.bits; s.shift += kDigitBits, to ^= 1) {

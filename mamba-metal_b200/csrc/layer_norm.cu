@@ -6,8 +6,9 @@
 //
 // The deviation is a second sum over the row held in registers, not
 // mean(x^2) - mean^2, which cancels where the mean is large.  Bound by bytes:
-// each pass reads its rows once.  The rows come through the ring of rows.cuh
-// where there are many of them.
+// each pass reads its rows once.  With many rows the next one is loaded ahead:
+// into registers (forward), or through the ring of rows.cuh (backward, whose
+// registers hold the column sums, and rows that are not 16-byte aligned).
 #include "common.cuh"
 #include "internal.h"
 #include "rows.cuh"
@@ -102,6 +103,77 @@ __global__ void __launch_bounds__(MAXT) layer_norm_kernel(const LayerNormParams 
     if (RING) drain_copies(full, ring.stages, &lost, kWaitNs);
 }
 
+// VEC elements as loaded.
+template <typename T, int VEC> struct RawGroup;
+template <> struct RawGroup<float, 4> { using Type = uint4; };
+template <> struct RawGroup<__half, 4> { using Type = uint2; };
+template <> struct RawGroup<__half, 8> { using Type = uint4; };
+
+// The same for rows of 16-byte accesses, with the CTA's next row on its way in
+// registers while this one's sums are made.  32 channels a thread: one or two
+// warps for a row of 2048, whose barriers cost little.
+template <typename TX, typename TO, int VEC, int NV>
+__global__ void __launch_bounds__(512) layer_norm_ahead_kernel(const LayerNormParams p) {
+    using Raw = typename RawGroup<TX, VEC>::Type;
+    __shared__ float sm[64];
+    int turn = 0;
+    const float inv_cols = 1.f / (float)p.cols;
+    Raw raw[NV];
+    auto fetch = [&](int64_t row) {
+        const TX *x = static_cast<const TX *>(p.x) + row * p.sx;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * blockDim.x + threadIdx.x) * VEC;
+            if (c < p.cols) raw[j] = *reinterpret_cast<const Raw *>(x + c);
+        }
+    };
+    fetch(blockIdx.x);  // grid <= rows
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        float v[NV][VEC];
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * blockDim.x + threadIdx.x) * VEC;
+            if (c < p.cols) {
+                load_n(reinterpret_cast<const TX *>(&raw[j]), v[j]);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) s += v[j][k];
+            }
+        }
+        if (row + gridDim.x < p.rows) fetch(row + gridDim.x);
+        const float mean = block_sum(s, sm, turn) * inv_cols;
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * blockDim.x + threadIdx.x) * VEC;
+            if (c < p.cols) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    v[j][k] -= mean;
+                    ss = fmaf(v[j][k], v[j][k], ss);
+                }
+            }
+        }
+        const float rs = rsqrtf(block_sum(ss, sm, turn) * inv_cols + p.eps);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * blockDim.x + threadIdx.x) * VEC;
+            if (c < p.cols) {
+                float w[VEC], b[VEC];
+                load_weight(p.w, c, w);
+                if (p.b) load_n(p.b + c, b);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) w[k] = fmaf(v[j][k] * rs, w[k], p.b ? b[k] : 0.f);
+                store_n(static_cast<TO *>(p.out) + row * p.so + c, w);
+            }
+        }
+        if (threadIdx.x == 0) {
+            if (p.mean) p.mean[row] = mean;
+            if (p.rstd) p.rstd[row] = rs;
+        }
+    }
+}
+
 // Backward: CTA k walks rows k, k + CTAs, ... and keeps the column sums of its
 // rows in registers; they leave as one partial row per CTA.
 template <typename TX, typename TO, int VEC, int NV, int MAXT, bool RING>
@@ -190,21 +262,30 @@ __global__ void __launch_bounds__(MAXT) layer_norm_bwd_kernel(const LayerNormGra
 // to the next).
 template <typename TX, typename TO> constexpr int kGroup = sizeof(TX) + sizeof(TO) == 4 ? 8 : 4;
 
-// Resident threads per SM of the ring kernels.
-constexpr int kLnThreads = 1024, kLnBwdThreads = 1024;
+// Resident threads per SM of the ring kernels.  32768 x 2048 backward, FP32 to
+// FP16 and FP16 to FP16, 16 channels a thread: 1536 threads 118 and 84 us, 1024
+// 124 and 106; 8 channels a thread, 2048 threads 118 and 99, 1024 129; 32
+// channels a thread, 768 threads 178 and 142.
+constexpr int kLnThreads = 1024, kLnBwdThreads = 1536;
+constexpr int kLnBwdChannels = 16;  // channels a thread of the backward ring
+// Channels and resident threads per SM of the kernel that loads a row ahead.
+// Forward, FP32 to FP16 and FP16 to FP16: 71 and 61 us; 768 threads 88 and 73;
+// 64 channels a thread 137 and 63; through the ring, 8 channels a thread, 95 and 92.
+constexpr int kLnAheadChannels = 32, kLnAheadThreads = 1024;
+constexpr int kLnSumThreads = 1024;
 
 int ln_ctas(int threads, bool backward) {
     return backward ? std::min(16, ring_ctas(threads, kLnBwdThreads)) : ring_ctas(threads, kLnThreads);
 }
 // Rows of partial column sums of the backward pass at most.
 int64_t ln_parts(int64_t rows, int cols) {
-    const int ctas = ln_ctas(threads_for(cols, cols <= 4096 ? 8 : 16), true);
+    const int ctas = ln_ctas(threads_for(cols, kLnBwdChannels), true);
     return std::min<int64_t>(rows, std::max(kDirectParts, 148 * ctas));
 }
 
-template <typename TX, typename TO, int VEC, int NV>
+template <typename TX, typename TO, int NV>
 int ring_ln(const LayerNormParams &p, const RingRow<1> &r, int ctas, int threads, cudaStream_t st) {
-    auto kernel = layer_norm_kernel<TX, TO, VEC, NV, 512, true>;
+    auto kernel = layer_norm_kernel<TX, TO, 1, NV, 512, true>;
     if (allow_smem(kernel)) return -1;
     kernel<<<(unsigned)(ctas * device_sm_count()), threads, (size_t)r.stage * r.stages, st>>>(p, r);
     return launch_status("layer_norm kernel");
@@ -213,18 +294,22 @@ template <typename TX, typename TO>
 int launch_ln(const LayerNormParams &p, bool vec, cudaStream_t st) {
     constexpr int V = kGroup<TX, TO>;
     RingRow<1> r{};
-    if (p.cols <= 8192) {
+    if (vec && p.rows >= 2 * device_sm_count()) {  // with fewer rows nothing is ahead
+        const int threads = threads_for(p.cols, kLnAheadChannels);
+        const int ctas = std::min(32, kLnAheadThreads / threads);
+        const unsigned grid = (unsigned)std::min<int64_t>(p.rows, (int64_t)device_sm_count() * ctas);
+        layer_norm_ahead_kernel<TX, TO, V, kLnAheadChannels / V><<<grid, threads, 0, st>>>(p);
+        return launch_status("layer_norm kernel");
+    }
+    if (!vec && p.cols <= 8192) {
         r.src[0] = p.x;
         r.stride[0] = p.sx * (int64_t)sizeof(TX);
         r.bytes[0] = (uint32_t)(p.cols * sizeof(TX));
         const bool one = p.cols <= 4096;
         const int threads = threads_for(p.cols, one ? 8 : 16);
         int ctas = ln_ctas(threads, false);
-        if (plan_ring<1>(r, p.rows, ctas)) {
-            if (vec)
-                return one ? ring_ln<TX, TO, V, 8 / V>(p, r, ctas, threads, st) : ring_ln<TX, TO, V, 16 / V>(p, r, ctas, threads, st);
-            return one ? ring_ln<TX, TO, 1, 8>(p, r, ctas, threads, st) : ring_ln<TX, TO, 1, 16>(p, r, ctas, threads, st);
-        }
+        if (plan_ring<1>(r, p.rows, ctas))
+            return one ? ring_ln<TX, TO, 8>(p, r, ctas, threads, st) : ring_ln<TX, TO, 16>(p, r, ctas, threads, st);
     }
     const unsigned grid = (unsigned)std::min<int64_t>(p.rows, 0x7fffffff);
     if (vec && p.cols <= 4096)
@@ -258,16 +343,12 @@ int launch_ln_bwd(const LayerNormGradParams &p, bool vec, unsigned &grid, cudaSt
         r.stride[1] = p.sg * (int64_t)sizeof(TO);
         r.bytes[0] = (uint32_t)(cols * sizeof(TX));
         r.bytes[1] = (uint32_t)(cols * sizeof(TO));
-        const bool one = cols <= 4096;
-        const int threads = threads_for(cols, one ? 8 : 16);
+        const int threads = threads_for(cols, kLnBwdChannels);
         int ctas = ln_ctas(threads, true);
         if (plan_ring<2>(r, p.rows, ctas)) {
             grid = std::min(grid, (unsigned)(ctas * device_sm_count()));
-            if (vec)
-                return one ? ring_ln_bwd<TX, TO, V, 8 / V>(p, r, grid, threads, st)
-                           : ring_ln_bwd<TX, TO, V, 16 / V>(p, r, grid, threads, st);
-            return one ? ring_ln_bwd<TX, TO, 1, 8>(p, r, grid, threads, st)
-                       : ring_ln_bwd<TX, TO, 1, 16>(p, r, grid, threads, st);
+            return vec ? ring_ln_bwd<TX, TO, V, kLnBwdChannels / V>(p, r, grid, threads, st)
+                       : ring_ln_bwd<TX, TO, 1, kLnBwdChannels>(p, r, grid, threads, st);
         }
     }
     grid = std::min(grid, (unsigned)kDirectParts);
@@ -385,8 +466,8 @@ int layer_norm_backward(const MambaLayerNormArgs *a, const MambaLayerNormGrads *
                                        : launch_ln_bwd<float, float>(p, vec, grid, st);
     if (rc) return -1;
     if (!g->dw && !g->db) return 0;
-    column_sum_kernel<<<dim3((unsigned)ceil_div(a->cols, 32), 2), kSumThreads, 0, st>>>(p.part_w, p.part_b, g->dw, g->db,
-                                                                                       (int)grid, a->cols);
+    column_sum_kernel<kLnSumThreads><<<dim3((unsigned)ceil_div(a->cols, 32), 2), kLnSumThreads, 0, st>>>(
+        p.part_w, p.part_b, g->dw, g->db, (int)grid, a->cols);
     return launch_status("layer_norm_backward sum kernel");
 }
 

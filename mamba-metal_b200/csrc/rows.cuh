@@ -212,26 +212,27 @@ __device__ __forceinline__ void start_ring(const RingRow<N> &r, uint8_t *ring, u
     __syncthreads();
 }
 
-// Column sums of the partial rows, in a fixed order: warp w of a CTA adds
-// rows w, w + 8, ... of 32 columns, then the warps' sums are added in order.
+// Column sums of the partial rows, in a fixed order: warp w of a CTA of v adds
+// rows w, w + v, ... of 32 columns, then the warps' sums are added in order.
 // blockIdx.y: which of the two sums (NULL: not wanted).
 constexpr int kSumThreads = 256;
-__global__ void __launch_bounds__(kSumThreads)
+template <int THREADS = kSumThreads>
+__global__ void __launch_bounds__(THREADS)
     column_sum_kernel(const float *__restrict__ part0, const float *__restrict__ part1, float *__restrict__ sum0,
                       float *__restrict__ sum1, int parts, int cols) {
-    __shared__ float sm[kSumThreads / 32][32];
+    __shared__ float sm[THREADS / 32][32];
     const float *part = blockIdx.y ? part1 : part0;
     float *dw = blockIdx.y ? sum1 : sum0;
     if (!dw) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float s = 0.f;
     if (c < cols)
-        for (int k = warp; k < parts; k += kSumThreads / 32) s += part[(int64_t)k * cols + c];
+        for (int k = warp; k < parts; k += THREADS / 32) s += part[(int64_t)k * cols + c];
     sm[warp][lane] = s;
     __syncthreads();
     if (warp == 0 && c < cols) {
 #pragma unroll
-        for (int k = 1; k < kSumThreads / 32; ++k) s += sm[k][lane];
+        for (int k = 1; k < THREADS / 32; ++k) s += sm[k][lane];
         dw[c] = s;
     }
 }

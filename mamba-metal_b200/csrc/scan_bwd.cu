@@ -806,16 +806,16 @@ __global__ void __launch_bounds__(256) scan_bwd_sum_kernel(const ScanSumParams p
 
 // Tokens per chunk.  Passes 1 and 3 run 4 and 2 CTAs an SM, each as long as its
 // chunk and some tokens' worth of work around it, and pass 1 costs about 0.4 of
-// pass 3; several chunks add a tenth.  Taken: the number of chunks (of 16
-// tokens or more) for which the rounds of CTAs are shortest.
+// pass 3; several chunks add a tenth, and each a little to pass 2.  Taken: the
+// number of chunks for which the rounds of CTAs are shortest.
 int chunk_length(int64_t batch, int64_t L, int64_t dim) {
     const int64_t ctas = batch * ceil_div64(dim, kCh), slots = 148 * 2;
     int64_t best = 0;
     double least = 0;
-    for (int64_t n = 1; n <= 128 && n <= ceil_div64(L, 16); ++n) {
+    for (int64_t n = 1; n <= 128 && n <= ceil_div64(L, kT); ++n) {
         const int64_t chunk = ceil_div64(ceil_div64(L, n), kT) * kT, all = ctas * ceil_div64(L, chunk);
-        const double cost = (ceil_div64(all, slots) + 0.8 * ceil_div64(all, 2 * slots)) * (double)(chunk + 8) *
-                            (chunk < L ? 1.1 : 1.0);
+        double cost = (ceil_div64(all, slots) + 0.8 * ceil_div64(all, 2 * slots)) * (double)(chunk + 8);
+        if (chunk < L) cost = cost * 1.1 + 0.3 * n;
         if (best == 0 || cost < least) {
             best = chunk;
             least = cost;
