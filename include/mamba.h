@@ -173,6 +173,9 @@ int mamba_forward_device(MambaModel *m, const float *input, float *output, int b
 int mamba_step_device(MambaModel *m, MambaStateHandle *s, const float *token, float *out,
                       void *stream);
 
+/* CUDA device the model is bound to, or -1. */
+int mamba_model_device(const MambaModel *m);
+
 /* Batch of the state handle, or -1. */
 int mamba_state_batch(const MambaStateHandle *s);
 

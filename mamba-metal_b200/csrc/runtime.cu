@@ -1336,6 +1336,8 @@ int mamba_step_device(MambaModel *m, MambaStateHandle *s, const float *token, fl
     return mb::step_device(*m->rt, *s, token, out, static_cast<cudaStream_t>(stream)) ? -1 : 0;
 }
 
+int mamba_model_device(const MambaModel *m) { return m && m->rt ? m->rt->dev : -1; }
+
 int mamba_state_batch(const MambaStateHandle *s) { return s ? s->batch : -1; }
 
 int mamba_state_buffers(MambaStateHandle *s, int layer, float **conv_state, float **ssm_state) {

@@ -18,9 +18,11 @@ Reference interface mirrored (SNAPKITTYWEST/mamba-metal):
                    rmsnorm.metal)
 Without a counterpart in the reference: gated_recurrence (with its backward
 pass and single-token step), block_norm (with its backward pass),
-quantize_rows and linear_i8 (8-bit linear layer).  They take stream= (a torch
-stream or handle of the tensors' device) besides the arguments listed, and
-run, allocate and fill on it; a caller that uses their results on another
+quantize_rows and linear_i8 (8-bit linear layer); and for training,
+embedding, layer_norm and dropout (with their backward passes) and the
+backward passes of selective_scan and causal_conv1d.  They take stream= (a
+torch stream or handle of the tensors' device) besides the arguments listed,
+and run, allocate and fill on it; a caller that uses their results on another
 stream has to wait for it.
 
 No helper is an autograd function: results of tensors that require gradients
@@ -165,6 +167,7 @@ _PROTOTYPES = {
     "mamba_save_weights": (c_int, [c_void_p, c_void_p, c_size]),
     "mamba_forward_device": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "mamba_step_device": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mamba_model_device": (c_int, [c_void_p]),
     "mamba_state_batch": (c_int, [c_void_p]),
     "mamba_state_buffers": (c_int, [c_void_p, c_int, ctypes.POINTER(c_void_p),
                                     ctypes.POINTER(c_void_p)]),
@@ -413,6 +416,26 @@ class Model:
         stream handle; 0: the model's stream, behind the default stream's work so far."""
         _check(lib().mamba_forward_device(self._h, in_ptr, out_ptr, batch, L, stream),
                "mamba_forward_device")
+
+    def forward_tokens(self, tokens, table, scale=1.0):
+        """Token ids to hidden states on the device: embedding(tokens, table,
+        scale) in FP32 through mamba_forward_device, both on the current
+        stream.  tokens int32 or int64 [batch, L], table [vocab, d_model] F16
+        or F32, on the model's device.  Returns FP32 [batch, L, d_model].  As
+        for forward_device, calls on this model from other streams have to be
+        ordered by the caller."""
+        torch = _torch()
+        what = "Model.forward_tokens"
+        if tokens.dim() != 2 or table.dim() != 2 or table.shape[1] != self.cfg.d_model:
+            raise MambaError("%s: tokens must be [batch, L] and table [vocab, %d]" % (what, self.cfg.d_model))
+        if not tokens.is_cuda or tokens.device.index != self._lib.mamba_model_device(self._h):
+            raise MambaError("%s: tokens must be on the model's device" % what)
+        h = embedding(tokens, table, scale, out_dtype=torch.float32)
+        # handle 1 names the default stream; 0 would be the model's own
+        stream = torch.cuda.current_stream(tokens.device).cuda_stream or 1
+        if h.numel():
+            self.forward_device(h.data_ptr(), h.data_ptr(), h.shape[0], h.shape[1], stream)
+        return h
 
     def create_state(self, batch):
         return State(self, batch)
