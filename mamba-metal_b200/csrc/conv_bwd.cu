@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(kCbSumThreads)
     if (k == K ? !dbias : !dw) return;
     float s = 0.f;
     if (d < D)
+#pragma unroll 8
         for (int i = warp; i < parts; i += kCbSumThreads / 32) s += part[((int64_t)i * (K + 1) + k) * D + d];
     sm[warp][lane] = s;
     __syncthreads();
@@ -315,6 +316,9 @@ int causal_conv1d_backward(const MambaConvGradArgs *a, void *ws, size_t ws_bytes
     MB_CHECK_ARG(aligned(a->dy, es) && aligned(a->x, es) && aligned(a->dx, es) && aligned(a->w, 4) && aligned(a->bias, 4),
                  "causal_conv1d_backward: pointers must be aligned to their element type");
     MB_CHECK_ARG(a->dx != a->x && a->dx != a->dy, "causal_conv1d_backward: dx needs memory of its own");
+    MB_CHECK_ARG((a->batch == 1 || a->dx_stride[0] != 0) && (a->seqlen == 1 || a->dx_stride[1] != 0) &&
+                     (a->dim == 1 || a->dx_stride[2] != 0),
+                 "causal_conv1d_backward: the elements of dx overlap (strides)");
     MB_CHECK_ARG(ws && ws_bytes >= causal_conv1d_backward_workspace_bytes(a) && aligned(ws, 16),
                  "causal_conv1d_backward: workspace too small or not 16-byte aligned");
     ConvGradParams p{};

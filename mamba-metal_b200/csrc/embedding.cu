@@ -212,6 +212,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kTinyThreads) sor
         __syncthreads();
         uint32_t all = 0, before = 0;
         if (tid < kDigits) {
+#pragma unroll
             for (int w = 0; w < kTinyWarps; ++w) all += sm.count[w][tid];
             if (CTAS > 1) {
                 const uint32_t at = smem_u32(&sm.total[self][tid]);
@@ -232,12 +233,16 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(kTinyThreads) sor
             }
         }
         uint32_t run = exclusive_digits(all, sm.warp_sum) + before;
-        if (tid < kDigits)
+        if (tid < kDigits) {
+            uint16_t c[kTinyWarps];  // loads that wait for no store
+#pragma unroll
+            for (int w = 0; w < kTinyWarps; ++w) c[w] = sm.count[w][tid];
+#pragma unroll
             for (int w = 0; w < kTinyWarps; ++w) {
-                const uint32_t c = sm.count[w][tid];
                 sm.count[w][tid] = (uint16_t)run;
-                run += c;
+                run += c[w];
             }
+        }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < kTinyItems; ++k) {

@@ -130,16 +130,18 @@ __device__ __forceinline__ float2 step_2(float2 e, float2 a, float2 w, float2 K2
 }
 
 // (dt a - phi) / log2(e) from e, phi / log2(e) = e / A2 and dt ln 2.  The
-// difference cancels where |dt A| is small: there phi (x / (1 - e^-x) - 1) with
-// x = dt A, by x/2 + x^2/12 - x^4/720 + ... (the last term for FP32 only).
+// difference loses 2 d / x^2 of its value for an absolute error d of e, where x =
+// dt A: so below |x| = 0.4 (d = 6e-8: 8e-7; FP32 tensors, whose e has a relative
+// error, 0.25) phi (x / (1 - e^-x) - 1) by x/2 + x^2/12 - x^4/720 (the next term
+// is 7e-7 of the sum at 0.4).
 template <bool PRECISE>
 __device__ __forceinline__ float2 bend_2(float2 v, float2 e, float2 phi, float2 dt_ln2) {
     constexpr float c1 = 0.69314718055994531f, c2 = c1 * c1 / 12, c4 = -c1 * c1 * c1 * c1 / 720;
+    constexpr float near = (PRECISE ? 0.25f : 0.4f) * kLog2e;
     const float2 far = ffma2(phi, make2(-1.f), ffma2(dt_ln2, e, dt_ln2));
-    float2 s = ffma2(v, make2(c2), make2(c1 / 2));
-    if (PRECISE) s = ffma2(fmul2(fmul2(v, v), v), make2(c4), s);
+    float2 s = ffma2(fmul2(v, v), make2(c4), make2(c2));
+    s = ffma2(s, v, make2(c1 / 2));
     s = fmul2(fmul2(s, v), phi);
-    constexpr float near = PRECISE ? 4 * kNear : kNear;
     return make_float2(fabsf(v.x) < near ? s.x : far.x, fabsf(v.y) < near ? s.y : far.y);
 }
 
@@ -305,7 +307,8 @@ __device__ __forceinline__ Place place(const ScanGradParams &p) {
     return r;
 }
 
-// Pass 1.
+// Pass 1: 0.85 ms of the same call, at 17 instructions a state and token (issue
+// 0.53 a cycle); with its inputs fetched a round ahead (three CTAs an SM) 0.90.
 template <typename Tx, typename Td, typename Tb, bool MULTI>
 __global__ void __launch_bounds__(kCh, 4) scan_bwd_states_kernel(const ScanGradParams p) {
     constexpr bool PRECISE = sizeof(Tx) == 4;
@@ -418,8 +421,8 @@ __global__ void __launch_bounds__(256) scan_bwd_carry_kernel(const ScanGradParam
     A2 *= kLog2e;
     float *H = p.H + b * p.chunks * p.per + at, *G = p.G + b * p.chunks * p.per + at;
     const float *S = p.S + b * p.chunks * p.dim + d;
-    // 8 chunks' loads at a time: they do not wait for the stores between them
-    constexpr int kAhead = 8;
+    // 16 chunks' loads at a time: they do not wait for the stores between them
+    constexpr int kAhead = 16;
     float h = 0.f;
     for (int k0 = 0; k0 < p.chunks; k0 += kAhead) {
         float end[kAhead], sum[kAhead];
@@ -500,6 +503,13 @@ __device__ __forceinline__ void tmem_get(uint32_t at, float2 (&v)[4][2]) {
 // Pass 3.  The states before each of 8 tokens are 128 columns of tensor memory
 // (a thread's own lane), and with FP16 tensors the e of each token 128 more, so
 // that the reverse steps do not evaluate it again.
+//
+// Bound by issue slots: about 40 instructions a state and token, 18 of them
+// packed (which take two slots), at 0.5 instructions a cycle and scheduler; DRAM
+// 15%.  8 x 2048 x 4096 FP16: 2.24 ms with two CTAs an SM and 255 registers.
+// With the states in shared memory 2.8 ms; three CTAs, 168 registers and 128
+// columns 3.07; two CTAs without e 2.77; scalar operations 2.39; the next
+// token's values loaded from tensor memory during the sums over lanes 2.28.
 constexpr uint32_t kColumns = 2 * kT * kN;
 template <typename Tx, typename Td, typename Tb, bool MULTI>
 __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p) {
@@ -786,8 +796,10 @@ __global__ void __launch_bounds__(256) scan_bwd_sum_kernel(const ScanSumParams p
     const int64_t states = states_of(p.dim), cols = states + 2 * (int64_t)p.dim, row = sums_of(p.dim);
     const int64_t col = (int64_t)(blockIdx.x - p.bc_ctas) * 32 + lane;
     float s = 0.f;
-    if (col < cols)
+    if (col < cols) {
+#pragma unroll 8
         for (int k = warp; k < p.parts; k += 8) s += p.part_a[k * row + col];
+    }
     sm[warp][lane] = s;
     __syncthreads();
     if (warp != 0 || col >= cols) return;
@@ -807,12 +819,15 @@ __global__ void __launch_bounds__(256) scan_bwd_sum_kernel(const ScanSumParams p
 // Tokens per chunk.  Passes 1 and 3 run 4 and 2 CTAs an SM, each as long as its
 // chunk and some tokens' worth of work around it, and pass 1 costs about 0.4 of
 // pass 3; several chunks add a tenth, and each a little to pass 2.  Taken: the
-// number of chunks for which the rounds of CTAs are shortest.
+// number of chunks for which the rounds of CTAs are shortest (of 8 x 2048 x 4096
+// and 3 x 333 x 203, 9 and 42 chunks: 3.13 ms and 55 us; 5 and 11 took 3.33 and
+// 90).  At most 16384 tokens, about 13 ms: a CTA keeps half of its SM's tensor
+// memory as long.
 int chunk_length(int64_t batch, int64_t L, int64_t dim) {
-    const int64_t ctas = batch * ceil_div64(dim, kCh), slots = 148 * 2;
+    const int64_t ctas = batch * ceil_div64(dim, kCh), slots = 148 * 2, least_n = ceil_div64(L, 16384);
     int64_t best = 0;
     double least = 0;
-    for (int64_t n = 1; n <= 128 && n <= ceil_div64(L, kT); ++n) {
+    for (int64_t n = least_n; n <= least_n + 127 && n <= ceil_div64(L, kT); ++n) {
         const int64_t chunk = ceil_div64(ceil_div64(L, n), kT) * kT, all = ctas * ceil_div64(L, chunk);
         double cost = (ceil_div64(all, slots) + 0.8 * ceil_div64(all, 2 * slots)) * (double)(chunk + 8);
         if (chunk < L) cost = cost * 1.1 + 0.3 * n;
@@ -947,6 +962,14 @@ int selective_scan_backward(const MambaScanArgs *a, const MambaScanGrads *g, voi
     }
     MB_CHECK_ARG(ws && ws_bytes >= selective_scan_backward_workspace_bytes(a) && aligned(ws, 16),
                  "selective_scan_backward: workspace too small or not 16-byte aligned");
+    // an output's elements lie apart
+    auto apart = [&](const void *p, const int64_t *st3, int inner) {
+        return !p || ((a->batch == 1 || st3[0] != 0) && (a->seqlen == 1 || st3[1] != 0) && (inner == 1 || st3[2] != 0));
+    };
+    MB_CHECK_ARG(apart(g->dx, g->dx_stride, a->dim) && apart(g->ddelta, g->ddelta_stride, a->dim) &&
+                     (!a->z || apart(g->dz, g->dz_stride, a->dim)) && apart(g->dB, g->dB_stride, a->dstate) &&
+                     apart(g->dC, g->dC_stride, a->dstate),
+                 "selective_scan_backward: a gradient's elements overlap (strides)");
     const Layout l = layout(a);
     uint8_t *base = static_cast<uint8_t *>(ws);
     auto at = [&](size_t o) { return reinterpret_cast<float *>(base + o); };

@@ -1197,6 +1197,8 @@ def embedding_backward(dout, tokens, vocab, scale=1.0, dtable=None, accumulate=F
     o_dt = _float_dtype(dout.dtype, "dout", what)
     if dout.dim() < 1:
         raise MambaError("%s: dout must be [*tokens.shape, dim]" % what)
+    if vocab < 0:
+        raise MambaError("%s: negative vocab" % what)
     dim, rows = dout.shape[-1], dout.dim() == 2
     _check_tensor(dout, "dout", what, tokens.shape + (dim,), dout.dtype, tokens.device, rows)
     if dtable is not None:

@@ -39,9 +39,9 @@ def _dev(a):
     return None if a is None else torch.from_numpy(np.ascontiguousarray(a)).cuda()
 
 
-def _close(got, ref, mag, name, L, f16, terms=0):
+def _close(got, ref, mag, name, L, f16, terms=0, approx=2.0 ** -16):
     u = 2.0 ** -11 if got.dtype == F16 else 2.0 ** -24
-    d = 2.0 ** -24 * (64 + 8 * L + terms) + (2.0 ** -16 if f16 else 0.0)
+    d = 2.0 ** -24 * (64 + 8 * L + terms) + (approx if f16 else 0.0)
     got = got.double().cpu().numpy()
     assert got.shape == ref.shape and np.isfinite(got).all(), name
     err = np.abs(got - ref) - (u * np.abs(ref) + d * mag + 2.0 ** -25)
@@ -203,6 +203,40 @@ def test_scan_backward_special_A_and_steps(cuda, kind):
     v["A"][20:, 2] = np.linspace(-0.2, -20, 20)
     got = _scan_run({n: _dev(a) for n, a in v.items()})
     _scan_check(v, got, kind)
+
+
+@pytest.mark.parametrize("kind", KINDS[1:])
+@pytest.mark.parametrize("L", [1, 2])
+def test_scan_backward_dA_of_short_rows(cuda, kind, L):
+    """With no state before them dA is all (dt a - phi) / A, a difference that cancels twice.  Its relative errors:
+    1.9e-6 of e (two units of 2^-24 over 1/16), 8e-7 of the series or the difference, twice 4e-7 of dt: 2^-18."""
+    v = _scan_case(11 + L, 3, L, 300, 16, kind, carried=False)
+    got = _scan_run({n: _dev(a) for n, a in v.items()})
+    ref, mag = tr.scan_backward(v["dy"], v["x"], v["delta"], v["A"], v["B"], v["C"], v["D"], v["z"], v["dt_bias"])
+    _close(got[2], ref["dA"], mag["dA"], "dA", L, True, 3 * L, 2.0 ** -18)
+
+
+def test_scan_backward_long_sequence(cuda):
+    """Longer than one chunk may be; sampled against the same call in two halves, joined by the state and its
+    gradient (each half's own errors as above)."""
+    kind, L, half = (F32, F32, F32), 40000, 17000
+    v = _scan_case(12, 1, L, 5, 16, kind)
+    t = {n: _dev(a) for n, a in v.items()}
+    got = _scan_run(t)
+    a, b = ({k: (x[:, s].contiguous() if k in ("x", "dy", "z", "delta", "B", "C") else x) for k, x in t.items()}
+            for s in (slice(0, half), slice(half, L)))
+    _, mid = mb.selective_scan(a["x"], a["delta"], a["A"], a["B"], a["C"], D=a["D"], z=a["z"], dt_bias=a["dt_bias"],
+                               initial_state=a["initial_state"], return_final_state=True)
+    b["initial_state"] = mid
+    gb = _scan_run(b)
+    a["dfinal_state"] = gb[8]
+    ga = _scan_run(a)
+    for k, name in ((0, "dx"), (1, "ddelta"), (3, "dB"), (4, "dC"), (6, "dz")):
+        want = torch.cat([ga[k], gb[k]], 1)
+        assert (got[k] - want).abs().max() <= 1e-4 * want.abs().max(), name
+    for k, name in ((2, "dA"), (5, "dD"), (7, "ddt_bias")):
+        assert (got[k] - ga[k] - gb[k]).abs().max() <= 1e-4 * got[k].abs().max(), name
+    assert (got[8] - ga[8]).abs().max() <= 1e-4 * ga[8].abs().max()
 
 
 @pytest.mark.parametrize("kind", KINDS)

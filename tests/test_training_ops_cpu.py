@@ -141,7 +141,10 @@ def _refused(fn, text, *args):
 
 def _set(s, change):
     for k, v in change.items():
-        setattr(s, k, v)
+        if isinstance(v, tuple):
+            getattr(s, k)[:] = v
+        else:
+            setattr(s, k, v)
     return s
 
 
@@ -249,7 +252,8 @@ def _conv(**kw):
     (dict(K=9), "1..8"), (dict(dtype=2), "dtype"), (dict(seqlen=0x7fffffff), "long"), (dict(dy=None), "null"),
     (dict(x=None), "null"), (dict(w=None), "null"), (dict(dx=None), "null"), (dict(x=8194), "aligned"),
     (dict(dw=4098), "aligned"), (dict(bias=4098), "aligned"), (dict(dx=8192), "own"), (dict(dx=4096), "own"),
-    (dict(dw=28672), "own"), (dict(ws=None), "workspace"), (dict(ws=4104), "workspace"), (dict(short=1), "workspace")])
+    (dict(dw=28672), "own"), (dict(dx_stride=(0, 8, 1)), "overlap"), (dict(dx_stride=(40, 0, 1)), "overlap"),
+    (dict(dx_stride=(40, 8, 0)), "overlap"), (dict(ws=None), "workspace"), (dict(ws=4104), "workspace"), (dict(short=1), "workspace")])
 def test_conv_backward_refusals(change, text):
     change = dict(change)
     ws, short = change.pop("ws", 4096), change.pop("short", 0)
@@ -277,12 +281,17 @@ def _scan(**kw):
     (dict(dt_bias=4098), {}, "aligned"), ({}, dict(dA=4098), "aligned"), ({}, dict(dB=4098), "aligned"),
     (dict(initial_state=4098), {}, "aligned"), ({}, dict(dfinal_state=4098), "aligned"), ({}, dict(dx=4096), "inputs"),
     ({}, dict(dB=4096 * 3), "inputs"), ({}, dict(dinitial_state=4096 * 9), "inputs"), ({}, dict(dz=4096 * 13), "own"),
-    ({}, dict(dD=4096 * 18), "own"), ({}, dict(ws=None), "workspace"), ({}, dict(ws=4104), "workspace"),
+    ({}, dict(dD=4096 * 18), "own"), ({}, dict(dx_stride=(40, 0, 1)), "overlap"),
+    ({}, dict(ddelta_stride=(0, 8, 1)), "overlap"), ({}, dict(dz_stride=(40, 8, 0)), "overlap"),
+    ({}, dict(dB_stride=(20, 4, 0)), "overlap"), ({}, dict(dC_stride=(20, 0, 1)), "overlap"), ({}, dict(ws=None), "workspace"), ({}, dict(ws=4104), "workspace"),
     ({}, dict(short=1), "workspace")])
 def test_scan_backward_refusals(args, change, text):
     g, change = mb.MambaScanGrads(), dict(change)
     for k, (name, *_) in enumerate(mb.MambaScanGrads._fields_[:11]):
         setattr(g, name, 4096 * (11 + k))
+    for st in (g.dy_stride, g.dx_stride, g.ddelta_stride, g.dz_stride):
+        st[:] = (40, 8, 1)
+    g.dB_stride[:] = g.dC_stride[:] = (20, 4, 1)
     ws, short = change.pop("ws", 4096), change.pop("short", 0)
     need = mb.lib().mamba_selective_scan_backward_workspace(P(_scan()))
     assert need > 0
@@ -325,7 +334,7 @@ def test_binding_refuses_wrong_tensors():
                  lambda: mb.embedding(ids, x[0]), lambda: mb.embedding(ids.to(torch.int16), x),
                  lambda: mb.embedding(torch.zeros(6, dtype=torch.int64)[::2], x),
                  lambda: mb.embedding(ids, x, out=x[:2]), lambda: mb.embedding(ids, x, scale=1e300),
-                 lambda: mb.embedding_backward(x[:2], ids, 5), lambda: mb.embedding_backward(x.double(), ids, 5),
+                 lambda: mb.embedding_backward(x[:2], ids, 5), lambda: mb.embedding_backward(x.double(), ids, 5), lambda: mb.embedding_backward(x, ids, -1),
                  lambda: mb.embedding_backward(x, ids, 5, dtable=x), lambda: mb.embedding_backward(x, ids, 5,
                                                                                                   accumulate=True),
                  lambda: mb.embedding_backward(x, ids, 1 << 31, dtable=x),
