@@ -22,7 +22,9 @@ __device__ unsigned int g_embedding_error = 0;
 namespace {
 
 // ---- lookup -------------------------------------------------------------------
-constexpr int kLookupThreads = 256;
+// 32768 x 2048 FP16 into FP32 and into FP16: 128 threads and 4 tokens in flight
+// 53 and 32 us, 256 threads 58 and 44, 512 72 and 65, 8 tokens 68 and 44.
+constexpr int kLookupThreads = 128;
 constexpr int kLookupTokens = 4;  // tokens a thread has in flight
 
 __device__ __forceinline__ int64_t token_id(const void *ids, bool wide, int64_t t) {
@@ -40,20 +42,20 @@ struct LookupParams {
 };
 
 // Threads (x) cover a row in groups of VEC elements, (y) different tokens.
-template <typename TT, typename TO, int VEC>
+template <typename TT, typename TO, int VEC, int TOKENS>
 __global__ void __launch_bounds__(kLookupThreads) embedding_kernel(const LookupParams p) {
-    const int64_t t0 = (int64_t)blockIdx.x * (blockDim.y * kLookupTokens) + threadIdx.y;
-    int64_t id[kLookupTokens];
+    const int64_t t0 = (int64_t)blockIdx.x * (blockDim.y * TOKENS) + threadIdx.y;
+    int64_t id[TOKENS];
 #pragma unroll
-    for (int k = 0; k < kLookupTokens; ++k) {
+    for (int k = 0; k < TOKENS; ++k) {
         const int64_t t = t0 + k * blockDim.y;
         id[k] = t < p.tokens ? token_id(p.ids, p.wide, t) : -1;
         if (id[k] >= p.vocab) id[k] = -1;
     }
     for (int c = threadIdx.x * VEC; c < p.dim; c += blockDim.x * VEC) {
-        float v[kLookupTokens][VEC];
+        float v[TOKENS][VEC];
 #pragma unroll
-        for (int k = 0; k < kLookupTokens; ++k) {
+        for (int k = 0; k < TOKENS; ++k) {
             if (id[k] >= 0) {
                 load_n(static_cast<const TT *>(p.table) + id[k] * p.table_stride + c, v[k]);
             } else {
@@ -62,7 +64,7 @@ __global__ void __launch_bounds__(kLookupThreads) embedding_kernel(const LookupP
             }
         }
 #pragma unroll
-        for (int k = 0; k < kLookupTokens; ++k) {
+        for (int k = 0; k < TOKENS; ++k) {
             const int64_t t = t0 + k * blockDim.y;
             if (t >= p.tokens) break;
             if (id[k] >= 0) {
@@ -83,15 +85,22 @@ int pow2_at_least(int v) {
 template <typename TT, typename TO>
 int launch_lookup(const LookupParams &p, bool vec, cudaStream_t st) {
     // 16 bytes of out a thread: FP32 rows written 32 bytes a thread leave half of each access's sectors empty
-    // (32768 x 2048 into FP32 71 us in place of 58)
+    // (32768 x 2048 into FP32, 256 threads: 71 us in place of 58)
     constexpr int VEC = 16 / sizeof(TO);
     const int tx = std::min(kLookupThreads, pow2_at_least(vec ? p.dim / VEC : p.dim)), ty = kLookupThreads / tx;
-    const int64_t grid = ceil_div64(p.tokens, (int64_t)ty * kLookupTokens);
+    // few tokens: more CTAs instead (256 x 2560 2.5 us, 3.6 with 4 tokens each)
+    const bool few = p.tokens < (int64_t)ty * kLookupTokens * 2 * device_sm_count();
+    const int64_t grid = ceil_div64(p.tokens, (int64_t)ty * (few ? 1 : kLookupTokens));
     MB_CHECK_ARG(grid <= 0x7fffffff, "embedding: too many tokens");
-    if (vec)
-        embedding_kernel<TT, TO, VEC><<<(unsigned)grid, dim3(tx, ty), 0, st>>>(p);
+    const dim3 block(tx, ty);
+    if (vec && few)
+        embedding_kernel<TT, TO, VEC, 1><<<(unsigned)grid, block, 0, st>>>(p);
+    else if (vec)
+        embedding_kernel<TT, TO, VEC, kLookupTokens><<<(unsigned)grid, block, 0, st>>>(p);
+    else if (few)
+        embedding_kernel<TT, TO, 1, 1><<<(unsigned)grid, block, 0, st>>>(p);
     else
-        embedding_kernel<TT, TO, 1><<<(unsigned)grid, dim3(tx, ty), 0, st>>>(p);
+        embedding_kernel<TT, TO, 1, kLookupTokens><<<(unsigned)grid, block, 0, st>>>(p);
     return launch_status("embedding kernel");
 }
 
