@@ -231,7 +231,6 @@ __global__ void __launch_bounds__(kCbSumThreads)
     if (k == K ? !dbias : !dw) return;
     float s = 0.f;
     if (d < D)
-#pragma unroll 8
         for (int i = warp; i < parts; i += kCbSumThreads / 32) s += part[((int64_t)i * (K + 1) + k) * D + d];
     sm[warp][lane] = s;
     __syncthreads();
