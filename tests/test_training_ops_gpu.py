@@ -80,7 +80,8 @@ def _ln_check(x, w, b, g, f, grads, eps=1e-5):
 SHAPES = [(1, 1), (1, 8), (3, 7), (2, 64), (4, 264), (130, 1000), (9, 1001), (64, 2560), (3, 4096), (3, 4099),
           (2, 8192), (2, 8200), (2, 16384), (2, 12001),
           # enough rows for persistent CTAs with rows fetched ahead, aligned and not
-          (14500, 72), (7300, 264), (2000, 2048), (1000, 4096), (950, 8192), (14500, 71), (3700, 513), (950, 7001)]
+          (14500, 72), (7300, 264), (2000, 2048), (1000, 4096), (950, 8192), (14500, 71), (3700, 513), (950, 7001),
+          (300, 16384), (320, 12001), (297, 40), (295, 40)]
 
 
 @pytest.mark.parametrize("xt,ot", TYPES)
@@ -197,6 +198,30 @@ def test_embedding(cuda, T, vocab, dim, kind):
         _close(acc, ref + start, mag + np.abs(start), "accumulated", most)
         absent = np.setdiff1d(np.arange(vocab), ids)
         assert (_host(acc)[absent] == start[absent]).all() and (_host(dtable)[absent] == 0).all()
+
+
+@pytest.mark.parametrize("T,vocab,dim", [(32768, 70000, 8), (32769, 300, 16), (40000, 70000, 12), (65537, 1000, 8),
+                                         (150000, 66000, 4)])
+def test_embedding_many_tokens(cuda, T, vocab, dim):
+    """Each of the sort's ways (one cluster, few and many tiles, one to three passes), and lookups with several tokens
+    in flight."""
+    rng = np.random.default_rng(T)
+    ids = _ids(rng, T, vocab, "skew")
+    ids[rng.random(T) < 0.05] = -1
+    g = rng.standard_normal((T, dim)).astype(np.float32)
+    inside = ids >= 0
+    ref, mag = np.zeros((vocab, dim)), np.zeros((vocab, dim))
+    np.add.at(ref, ids[inside], g[inside].astype(np.float64))
+    np.add.at(mag, ids[inside], np.abs(g[inside].astype(np.float64)))
+    got = mb.embedding_backward(_dev(g), _dev(ids), vocab)
+    _close(got, ref, mag, "dtable", np.bincount(ids[inside]).max())
+    assert torch.equal(got, mb.embedding_backward(_dev(g), _dev(ids).int(), vocab))
+    wide = torch.randn((50, 2056 if T < 40000 else 1000), device="cuda")
+    tok = _dev(ids[:6000] % 51 - 1)
+    for dtype in (F16, F32):
+        out = mb.embedding(tok, wide.to(dtype), scale=0.5, out_dtype=F32)
+        want = torch.where((tok >= 0)[:, None], wide.to(dtype).float()[tok.clamp(min=0)] * 0.5, 0.0)
+        assert torch.equal(out, want)  # halving is exact
 
 
 def test_embedding_ids_beyond_32_bits(cuda):
