@@ -35,6 +35,10 @@ struct ConvGradParams {
 constexpr int kCbThreads = 128;
 constexpr int kCbRows = 4;  // rows of x and dy in flight
 
+// Channels a thread where rows allow it.  FP32: with 4 a thread needs 188
+// registers (8 x 4096 x 1000 115 us, with 2 93).
+template <typename T> constexpr int kWideChannels = sizeof(T) == 2 ? 4 : 2;
+
 // A row's VEC channels as loaded, and as pairs.
 template <typename T, int VEC> struct RowVec;
 template <typename T> struct RowVec<T, 1> {
@@ -55,18 +59,18 @@ template <> struct RowVec<__half, 4> {
     }
     static __device__ __forceinline__ uint2 zero() { return make_uint2(0u, 0u); }
 };
-template <> struct RowVec<float, 4> {
-    using Raw = float4;
-    static __device__ __forceinline__ void unpack(const float4 &r, float2 *f) {
-        f[0] = make_float2(r.x, r.y);
-        f[1] = make_float2(r.z, r.w);
-    }
-    static __device__ __forceinline__ float4 pack(const float2 *f) {
-        return make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
-    }
-    static __device__ __forceinline__ float4 zero() { return make_float4(0.f, 0.f, 0.f, 0.f); }
+template <> struct RowVec<__half, 2> {
+    using Raw = __half2;
+    static __device__ __forceinline__ void unpack(const __half2 &r, float2 *f) { f[0] = __half22float2(r); }
+    static __device__ __forceinline__ __half2 pack(const float2 *f) { return __float22half2_rn(f[0]); }
+    static __device__ __forceinline__ __half2 zero() { return __float2half2_rn(0.f); }
 };
-
+template <> struct RowVec<float, 2> {
+    using Raw = float2;
+    static __device__ __forceinline__ void unpack(const float2 &r, float2 *f) { f[0] = r; }
+    static __device__ __forceinline__ float2 pack(const float2 *f) { return f[0]; }
+    static __device__ __forceinline__ float2 zero() { return make_float2(0.f, 0.f); }
+};
 // SiLU'(v) = t (1 + v e t) with e = e^-v and t = 1 / (1 + e), for two values of
 // FP16 tensors (approximate exponential and reciprocal, 2^-22 each).  e ends at
 // 2^126, where t is the smallest normal number; a NaN stays one.
@@ -220,23 +224,23 @@ __global__ void __launch_bounds__(kCbThreads, sizeof(T) == 2 && K <= 4 ? 4 : 1) 
 }
 
 // dw and dbias from the partial rows, in a fixed order: warp v of a CTA adds
-// rows v, v + 8, ... of 32 channels and one tap, then the warps' sums are added
+// rows v, v + warps, ... of 32 channels and one tap, then the warps' sums are added
 // in order.
-constexpr int kCbSumThreads = 256;
-__global__ void __launch_bounds__(kCbSumThreads)
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS)
     conv1d_bwd_sum_kernel(const float *__restrict__ part, float *__restrict__ dw, float *__restrict__ dbias, int parts,
                           int K, int D) {
-    __shared__ float sm[kCbSumThreads / 32][32];
+    __shared__ float sm[THREADS / 32][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = blockIdx.x * 32 + lane, k = blockIdx.y;
     if (k == K ? !dbias : !dw) return;
     float s = 0.f;
     if (d < D)
-        for (int i = warp; i < parts; i += kCbSumThreads / 32) s += part[((int64_t)i * (K + 1) + k) * D + d];
+        for (int i = warp; i < parts; i += THREADS / 32) s += part[((int64_t)i * (K + 1) + k) * D + d];
     sm[warp][lane] = s;
     __syncthreads();
     if (warp == 0 && d < D) {
 #pragma unroll
-        for (int v = 1; v < kCbSumThreads / 32; ++v) s += sm[v][lane];
+        for (int v = 1; v < THREADS / 32; ++v) s += sm[v][lane];
         if (k == K)
             dbias[d] = s;
         else
@@ -252,18 +256,20 @@ int run_length(int64_t batch, int64_t L, int64_t D) {
 }
 
 template <typename T, int K>
-int launch_conv_bwd(ConvGradParams &p, bool vec, cudaStream_t st) {
-    p.blocks = ceil_div(p.D, kCbThreads * (vec ? 4 : 1));
+int launch_conv_bwd(ConvGradParams &p, int vec, cudaStream_t st) {
+    p.blocks = ceil_div(p.D, kCbThreads * vec);
     const int64_t grid = (int64_t)p.blocks * p.runs * p.batch;
     MB_CHECK_ARG(grid <= 0x7fffffff, "causal_conv1d_backward: too many elements");
-    if (vec)
-        conv1d_bwd_kernel<T, K, 4><<<(unsigned)grid, kCbThreads, 0, st>>>(p);
+    if (vec == kWideChannels<T>)
+        conv1d_bwd_kernel<T, K, kWideChannels<T>><<<(unsigned)grid, kCbThreads, 0, st>>>(p);
+    else if (vec == 2)
+        conv1d_bwd_kernel<T, K, 2><<<(unsigned)grid, kCbThreads, 0, st>>>(p);
     else
         conv1d_bwd_kernel<T, K, 1><<<(unsigned)grid, kCbThreads, 0, st>>>(p);
     return launch_status("causal_conv1d_backward kernel");
 }
 template <typename T>
-int launch_conv_bwd(ConvGradParams &p, int K, bool vec, cudaStream_t st) {
+int launch_conv_bwd(ConvGradParams &p, int K, int vec, cudaStream_t st) {
     switch (K) {
         case 1: return launch_conv_bwd<T, 1>(p, vec, st);
         case 2: return launch_conv_bwd<T, 2>(p, vec, st);
@@ -278,9 +284,9 @@ int launch_conv_bwd(ConvGradParams &p, int K, bool vec, cudaStream_t st) {
 
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-// Rows of 4 channels at a time: channels adjacent, every row start aligned.
-bool vector_rows(const void *v, const int64_t *s, int64_t es) {
-    return s[2] == 1 && aligned(v, (size_t)(4 * es)) && s[1] % 4 == 0 && s[0] % 4 == 0;
+// Rows of n channels at a time: channels adjacent, every row start aligned.
+bool vector_rows(const void *v, const int64_t *s, int64_t es, int n) {
+    return s[2] == 1 && aligned(v, (size_t)(n * es)) && s[1] % n == 0 && s[0] % n == 0;
 }
 
 int check(const MambaConvGradArgs *a) {
@@ -339,13 +345,20 @@ int causal_conv1d_backward(const MambaConvGradArgs *a, void *ws, size_t ws_bytes
     p.runs = ceil_div(p.L, p.run);
     p.silu = a->silu != 0;
     MB_CHECK_ARG((int64_t)p.runs * p.batch <= 0x7fffffff, "causal_conv1d_backward: too many elements");
-    const bool vec = p.D % 4 == 0 && vector_rows(a->x, p.sx, (int64_t)es) && vector_rows(a->dy, p.sdy, (int64_t)es) &&
-                     vector_rows(a->dx, p.sdx, (int64_t)es);
+    int vec = a->dtype == MAMBA_F16 ? kWideChannels<__half> : kWideChannels<float>;
+    while (vec > 1 && !(p.D % vec == 0 && vector_rows(a->x, p.sx, (int64_t)es, vec) &&
+                        vector_rows(a->dy, p.sdy, (int64_t)es, vec) && vector_rows(a->dx, p.sdx, (int64_t)es, vec)))
+        vec /= 2;
     if (a->dtype == MAMBA_F16 ? launch_conv_bwd<__half>(p, a->K, vec, st) : launch_conv_bwd<float>(p, a->K, vec, st))
         return -1;
     if (!a->dw && !a->dbias) return 0;
-    conv1d_bwd_sum_kernel<<<dim3((unsigned)ceil_div(p.D, 32), (unsigned)(a->K + 1)), kCbSumThreads, 0, st>>>(
-        p.part, a->dw, a->dbias, p.runs * p.batch, a->K, p.D);
+    // 32 warps to a CTA where that is one round of CTAs (777 channels, 282 rows 3.7 us, 5.2 with 8), else 8 (4096
+    // channels, 256 rows 8.5, with 32 15.8)
+    const dim3 grid((unsigned)ceil_div(p.D, 32), (unsigned)(a->K + 1));
+    if (grid.x * grid.y <= 2u * (unsigned)device_sm_count())
+        conv1d_bwd_sum_kernel<1024><<<grid, 1024, 0, st>>>(p.part, a->dw, a->dbias, p.runs * p.batch, a->K, p.D);
+    else
+        conv1d_bwd_sum_kernel<256><<<grid, 256, 0, st>>>(p.part, a->dw, a->dbias, p.runs * p.batch, a->K, p.D);
     return launch_status("causal_conv1d_backward sum kernel");
 }
 

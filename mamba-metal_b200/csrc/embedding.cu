@@ -82,26 +82,27 @@ int pow2_at_least(int v) {
     return p;
 }
 
-template <typename TT, typename TO>
-int launch_lookup(const LookupParams &p, bool vec, cudaStream_t st) {
-    // 16 bytes of out a thread: FP32 rows written 32 bytes a thread leave half of each access's sectors empty
-    // (32768 x 2048 into FP32, 256 threads: 71 us in place of 58)
-    constexpr int VEC = 16 / sizeof(TO);
-    const int tx = std::min(kLookupThreads, pow2_at_least(vec ? p.dim / VEC : p.dim)), ty = kLookupThreads / tx;
+template <typename TT, typename TO, int VEC>
+int launch_lookup(const LookupParams &p, cudaStream_t st) {
+    const int tx = std::min(kLookupThreads, pow2_at_least(p.dim / VEC)), ty = kLookupThreads / tx;
     // few tokens: more CTAs instead (256 x 2560 2.5 us, 3.6 with 4 tokens each)
     const bool few = p.tokens < (int64_t)ty * kLookupTokens * 2 * device_sm_count();
     const int64_t grid = ceil_div64(p.tokens, (int64_t)ty * (few ? 1 : kLookupTokens));
     MB_CHECK_ARG(grid <= 0x7fffffff, "embedding: too many tokens");
-    const dim3 block(tx, ty);
-    if (vec && few)
-        embedding_kernel<TT, TO, VEC, 1><<<(unsigned)grid, block, 0, st>>>(p);
-    else if (vec)
-        embedding_kernel<TT, TO, VEC, kLookupTokens><<<(unsigned)grid, block, 0, st>>>(p);
-    else if (few)
-        embedding_kernel<TT, TO, 1, 1><<<(unsigned)grid, block, 0, st>>>(p);
+    if (few)
+        embedding_kernel<TT, TO, VEC, 1><<<(unsigned)grid, dim3(tx, ty), 0, st>>>(p);
     else
-        embedding_kernel<TT, TO, 1, kLookupTokens><<<(unsigned)grid, block, 0, st>>>(p);
+        embedding_kernel<TT, TO, VEC, kLookupTokens><<<(unsigned)grid, dim3(tx, ty), 0, st>>>(p);
     return launch_status("embedding kernel");
+}
+
+// 16 bytes of out a thread: FP32 rows written 32 bytes a thread leave half of
+// each access's sectors empty (32768 x 2048 into FP32, 256 threads: 71 us in
+// place of 58).  Rows of an even width that are not 16-byte aligned: pairs.
+template <typename TT, typename TO>
+int launch_lookup(const LookupParams &p, bool vec, bool pairs, cudaStream_t st) {
+    if (vec) return launch_lookup<TT, TO, 16 / (int)sizeof(TO)>(p, st);
+    return pairs ? launch_lookup<TT, TO, 2>(p, st) : launch_lookup<TT, TO, 1>(p, st);
 }
 
 // ---- sort -----------------------------------------------------------------------
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__(kSumThreadsE) embedding_sum_kernel(const SumPa
     uint32_t next = first + 1 < p.n ? p.keys[first + 1] : p.vocab;
     for (uint32_t i = first; i < live; ++i) {
         const uint32_t after = i + 2 < p.n ? p.keys[i + 2] : p.vocab;  // on its way while the row is added
-        const uint32_t shift = VEC == 1 ? (uint32_t)reinterpret_cast<uintptr_t>(from(p.pos[i])) & 15u : 0u;
+        const uint32_t shift = VEC <= 2 ? (uint32_t)reinterpret_cast<uintptr_t>(from(p.pos[i])) & 15u : 0u;
         if (!await_copy(full, at.s, at.parity, &lost, kWaitNs)) atomicOr(&g_embedding_error, kErrEmbeddingTimeout);
         const T *row = reinterpret_cast<const T *>(ring + at.s * p.stage + shift);
 #pragma unroll
@@ -604,7 +605,7 @@ int launch_sums(SumParams &p, cudaStream_t st) {
              (size_t)p.stage * p.stages, st>>>(p);
     if (launch_status("embedding_backward sum kernel")) return -1;
     if (p.parts == 1) return 0;
-    constexpr int JV = VEC == 1 ? 1 : 4;
+    constexpr int JV = VEC <= 2 ? VEC : 4;
     embedding_join_kernel<JV><<<dim3((unsigned)p.parts, (unsigned)ceil_div(p.dim, kSumThreadsE * JV)), kSumThreadsE, 0,
                                 st>>>(p);
     return launch_status("embedding_backward join kernel");
@@ -684,10 +685,13 @@ int embedding(const MambaEmbeddingArgs *a, cudaStream_t st) {
     p.scale = a->scale;
     const bool vec = a->dim % 8 == 0 && aligned_to(a->table, 16) && aligned_to(a->out, 16) &&
                      (a->table_stride * et) % 16 == 0 && (a->out_stride * eo) % 16 == 0;
+    const bool pairs = a->dim % 2 == 0 && aligned_to(a->table, (size_t)(2 * et)) && aligned_to(a->out, (size_t)(2 * eo)) &&
+                       a->table_stride % 2 == 0 && a->out_stride % 2 == 0;
     if (a->table_dtype == MAMBA_F16)
-        return a->out_dtype == MAMBA_F16 ? launch_lookup<__half, __half>(p, vec, st)
-                                         : launch_lookup<__half, float>(p, vec, st);
-    return a->out_dtype == MAMBA_F16 ? launch_lookup<float, __half>(p, vec, st) : launch_lookup<float, float>(p, vec, st);
+        return a->out_dtype == MAMBA_F16 ? launch_lookup<__half, __half>(p, vec, pairs, st)
+                                         : launch_lookup<__half, float>(p, vec, pairs, st);
+    return a->out_dtype == MAMBA_F16 ? launch_lookup<float, __half>(p, vec, pairs, st)
+                                     : launch_lookup<float, float>(p, vec, pairs, st);
 }
 
 size_t embedding_workspace_bytes(const MambaEmbeddingArgs *a) {
@@ -766,9 +770,15 @@ int embedding_backward(const MambaEmbeddingArgs *a, const void *dout, int64_t do
     p.accumulate = accumulate != 0;
     const bool vec = a->dim % 8 == 0 && aligned_to(dout, 16) && aligned_to(dtable, 16) && dtable_stride % 4 == 0 &&
                      (dout_stride * (int64_t)dtype_size(a->out_dtype)) % 16 == 0;
+    const bool pairs = a->dim % 2 == 0 && aligned_to(dout, 2 * dtype_size(a->out_dtype)) && aligned_to(dtable, 8) &&
+                       dtable_stride % 2 == 0 && dout_stride % 2 == 0;
     // up to 2048 columns a CTA
-    if (a->out_dtype == MAMBA_F16) return vec ? launch_sums<__half, 8, 1>(p, st) : launch_sums<__half, 1, 8>(p, st);
-    return vec ? launch_sums<float, 4, 2>(p, st) : launch_sums<float, 1, 8>(p, st);
+    if (a->out_dtype == MAMBA_F16) {
+        if (vec) return launch_sums<__half, 8, 1>(p, st);
+        return pairs ? launch_sums<__half, 2, 4>(p, st) : launch_sums<__half, 1, 8>(p, st);
+    }
+    if (vec) return launch_sums<float, 4, 2>(p, st);
+    return pairs ? launch_sums<float, 2, 4>(p, st) : launch_sums<float, 1, 8>(p, st);
 }
 
 }  // namespace mb

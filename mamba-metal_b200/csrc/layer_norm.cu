@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(MAXT) layer_norm_kernel(const LayerNormParams 
     RingPlace at;
     if (RING) start_ring<1>(ring, smem, full, &lost, p.rows);
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const TX *x = RING ? reinterpret_cast<const TX *>(smem + at.s * ring.stage + (VEC == 1 ? ring.shift(0, row) : 0u))
+        const TX *x = RING ? reinterpret_cast<const TX *>(smem + at.s * ring.stage + (VEC <= 2 ? ring.shift(0, row) : 0u))
                            : static_cast<const TX *>(p.x) + row * p.sx;
         if (RING) await_row(full, at, &lost, &g_layer_norm_error);
         float v[NV][VEC];
@@ -105,11 +105,13 @@ __global__ void __launch_bounds__(MAXT) layer_norm_kernel(const LayerNormParams 
 
 // VEC elements as loaded.
 template <typename T, int VEC> struct RawGroup;
+template <> struct RawGroup<float, 2> { using Type = uint2; };
+template <> struct RawGroup<__half, 2> { using Type = uint32_t; };
 template <> struct RawGroup<float, 4> { using Type = uint4; };
 template <> struct RawGroup<__half, 4> { using Type = uint2; };
 template <> struct RawGroup<__half, 8> { using Type = uint4; };
 
-// The same for rows of 16-byte accesses, with the CTA's next row on its way in
+// The same for rows of 16-byte accesses, or of pairs, with the CTA's next row on its way in
 // registers while this one's sums are made.  32 channels a thread: one or two
 // warps for a row of 2048, whose barriers cost little.
 template <typename TX, typename TO, int VEC, int NV>
@@ -191,7 +193,7 @@ __global__ void __launch_bounds__(MAXT) layer_norm_bwd_kernel(const LayerNormGra
     float mean_next = p.mean[blockIdx.x], rs_next = p.rstd[blockIdx.x];  // grid <= rows
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const uint8_t *place = smem + at.s * ring.stage;
-        auto at_place = [&](int k) { return place + ring.offset[k] + (VEC == 1 ? ring.shift(k, row) : 0u); };
+        auto at_place = [&](int k) { return place + ring.offset[k] + (VEC <= 2 ? ring.shift(k, row) : 0u); };
         const TX *x = RING ? reinterpret_cast<const TX *>(at_place(0)) : static_cast<const TX *>(p.x) + row * p.sx;
         const TO *g = RING ? reinterpret_cast<const TO *>(at_place(1)) : static_cast<const TO *>(p.dout) + row * p.sg;
         // this row's statistics were loaded a row ago, the next row's are on their way
@@ -290,18 +292,32 @@ int ring_ln(const LayerNormParams &p, const RingRow<1> &r, int ctas, int threads
     kernel<<<(unsigned)(ctas * device_sm_count()), threads, (size_t)r.stage * r.stages, st>>>(p, r);
     return launch_status("layer_norm kernel");
 }
-template <typename TX, typename TO>
-int launch_ln(const LayerNormParams &p, bool vec, cudaStream_t st) {
-    constexpr int V = kGroup<TX, TO>;
-    RingRow<1> r{};
-    if (vec && p.rows >= 2 * device_sm_count()) {  // with fewer rows nothing is ahead
+// How a call's rows can be accessed: 16 bytes at a time, in pairs of channels
+// (every row of an even width), or one by one.
+enum Access { kSingle, kPairs, kWide };
+
+template <typename TX, typename TO, int V>
+int launch_ln_groups(const LayerNormParams &p, cudaStream_t st) {
+    if (p.rows >= 2 * device_sm_count()) {  // with fewer rows nothing is ahead
         const int threads = threads_for(p.cols, kLnAheadChannels);
         const int ctas = std::min(32, kLnAheadThreads / threads);
         const unsigned grid = (unsigned)std::min<int64_t>(p.rows, (int64_t)device_sm_count() * ctas);
         layer_norm_ahead_kernel<TX, TO, V, kLnAheadChannels / V><<<grid, threads, 0, st>>>(p);
-        return launch_status("layer_norm kernel");
+    } else if (p.cols <= 4096) {
+        layer_norm_kernel<TX, TO, V, 8 / V, 512, false>
+            <<<(unsigned)p.rows, threads_for(p.cols, 8), 0, st>>>(p, RingRow<1>{});
+    } else {
+        layer_norm_kernel<TX, TO, V, 16 / V, 1024, false>
+            <<<(unsigned)p.rows, threads_for(p.cols, 16), 0, st>>>(p, RingRow<1>{});
     }
-    if (!vec && p.cols <= 8192) {
+    return launch_status("layer_norm kernel");
+}
+template <typename TX, typename TO>
+int launch_ln(const LayerNormParams &p, Access access, cudaStream_t st) {
+    if (access == kWide) return launch_ln_groups<TX, TO, kGroup<TX, TO>>(p, st);
+    if (access == kPairs) return launch_ln_groups<TX, TO, 2>(p, st);
+    RingRow<1> r{};
+    if (p.cols <= 8192) {
         r.src[0] = p.x;
         r.stride[0] = p.sx * (int64_t)sizeof(TX);
         r.bytes[0] = (uint32_t)(p.cols * sizeof(TX));
@@ -312,11 +328,7 @@ int launch_ln(const LayerNormParams &p, bool vec, cudaStream_t st) {
             return one ? ring_ln<TX, TO, 8>(p, r, ctas, threads, st) : ring_ln<TX, TO, 16>(p, r, ctas, threads, st);
     }
     const unsigned grid = (unsigned)std::min<int64_t>(p.rows, 0x7fffffff);
-    if (vec && p.cols <= 4096)
-        layer_norm_kernel<TX, TO, V, 8 / V, 512, false><<<grid, threads_for(p.cols, 8), 0, st>>>(p, r);
-    else if (vec)
-        layer_norm_kernel<TX, TO, V, 16 / V, 1024, false><<<grid, threads_for(p.cols, 16), 0, st>>>(p, r);
-    else if (p.cols <= 4096)
+    if (p.cols <= 4096)
         layer_norm_kernel<TX, TO, 1, 4, 1024, false><<<grid, threads_for(p.cols, 4), 0, st>>>(p, r);
     else
         layer_norm_kernel<TX, TO, 1, 16, 1024, false><<<grid, threads_for(p.cols, 16), 0, st>>>(p, r);
@@ -332,7 +344,7 @@ int ring_ln_bwd(const LayerNormGradParams &p, const RingRow<2> &r, unsigned grid
 }
 // grid: CTAs to launch at most; set to those launched (rows of partial sums).
 template <typename TX, typename TO>
-int launch_ln_bwd(const LayerNormGradParams &p, bool vec, unsigned &grid, cudaStream_t st) {
+int launch_ln_bwd(const LayerNormGradParams &p, Access access, unsigned &grid, cudaStream_t st) {
     constexpr int V = kGroup<TX, TO>;
     const int cols = p.cols;
     RingRow<2> r{};
@@ -347,25 +359,35 @@ int launch_ln_bwd(const LayerNormGradParams &p, bool vec, unsigned &grid, cudaSt
         int ctas = ln_ctas(threads, true);
         if (plan_ring<2>(r, p.rows, ctas)) {
             grid = std::min(grid, (unsigned)(ctas * device_sm_count()));
-            return vec ? ring_ln_bwd<TX, TO, V, kLnBwdChannels / V>(p, r, grid, threads, st)
-                       : ring_ln_bwd<TX, TO, 1, kLnBwdChannels>(p, r, grid, threads, st);
+            if (access == kWide) return ring_ln_bwd<TX, TO, V, kLnBwdChannels / V>(p, r, grid, threads, st);
+            if (access == kPairs) return ring_ln_bwd<TX, TO, 2, kLnBwdChannels / 2>(p, r, grid, threads, st);
+            return ring_ln_bwd<TX, TO, 1, kLnBwdChannels>(p, r, grid, threads, st);
         }
     }
     grid = std::min(grid, (unsigned)kDirectParts);
-    if (vec && cols <= 4096)
-        layer_norm_bwd_kernel<TX, TO, V, 8 / V, 512, false><<<grid, threads_for(cols, 8), 0, st>>>(p, r);
-    else if (vec)
-        layer_norm_bwd_kernel<TX, TO, V, 16 / V, 1024, false><<<grid, threads_for(cols, 16), 0, st>>>(p, r);
+    const int eight = threads_for(cols, 8), sixteen = threads_for(cols, 16);
+    if (access == kWide && cols <= 4096)
+        layer_norm_bwd_kernel<TX, TO, V, 8 / V, 512, false><<<grid, eight, 0, st>>>(p, r);
+    else if (access == kWide)
+        layer_norm_bwd_kernel<TX, TO, V, 16 / V, 1024, false><<<grid, sixteen, 0, st>>>(p, r);
+    else if (access == kPairs && cols <= 4096)
+        layer_norm_bwd_kernel<TX, TO, 2, 4, 512, false><<<grid, eight, 0, st>>>(p, r);
+    else if (access == kPairs)
+        layer_norm_bwd_kernel<TX, TO, 2, 8, 1024, false><<<grid, sixteen, 0, st>>>(p, r);
     else if (cols <= 4096)
         layer_norm_bwd_kernel<TX, TO, 1, 4, 1024, false><<<grid, threads_for(cols, 4), 0, st>>>(p, r);
     else
-        layer_norm_bwd_kernel<TX, TO, 1, 16, 1024, false><<<grid, threads_for(cols, 16), 0, st>>>(p, r);
+        layer_norm_bwd_kernel<TX, TO, 1, 16, 1024, false><<<grid, sixteen, 0, st>>>(p, r);
     return launch_status("layer_norm_backward kernel");
 }
 
 bool float_dtype(int dt) { return dt == MAMBA_F32 || dt == MAMBA_F16; }
-bool aligned_rows(const void *p, int64_t stride, int dtype) {
-    return aligned_to(p, 16) && (stride * (int64_t)dtype_size(dtype)) % 16 == 0;
+// Every row starts on a boundary of `bytes`.
+bool aligned_rows(const void *p, int64_t stride, int dtype, int64_t bytes) {
+    return aligned_to(p, (size_t)bytes) && (stride * (int64_t)dtype_size(dtype)) % bytes == 0;
+}
+bool pair_rows(const void *p, int64_t stride, int dtype) {
+    return aligned_rows(p, stride, dtype, 2 * (int64_t)dtype_size(dtype));
 }
 
 int check_ln(const MambaLayerNormArgs *a, const std::string &what) {
@@ -404,12 +426,16 @@ int layer_norm(const MambaLayerNormArgs *a, cudaStream_t st) {
     p.eps = a->eps;
     p.sx = a->x_stride;
     p.so = a->out_stride;
-    // 16-byte accesses: 8 channels at a time, every row start aligned
-    const bool vec = a->cols % 8 == 0 && aligned_rows(a->x, a->x_stride, a->x_dtype) &&
-                     aligned_rows(a->out, a->out_stride, a->out_dtype) && aligned_to(a->w, 16) && aligned_to(a->b, 16);
+    Access access = kSingle;
+    if (a->cols % 8 == 0 && aligned_rows(a->x, a->x_stride, a->x_dtype, 16) &&
+        aligned_rows(a->out, a->out_stride, a->out_dtype, 16) && aligned_to(a->w, 16) && aligned_to(a->b, 16))
+        access = kWide;
+    else if (a->cols % 2 == 0 && pair_rows(a->x, a->x_stride, a->x_dtype) &&
+             pair_rows(a->out, a->out_stride, a->out_dtype) && aligned_to(a->w, 8) && aligned_to(a->b, 8))
+        access = kPairs;
     if (a->x_dtype == MAMBA_F16)
-        return a->out_dtype == MAMBA_F16 ? launch_ln<__half, __half>(p, vec, st) : launch_ln<__half, float>(p, vec, st);
-    return a->out_dtype == MAMBA_F16 ? launch_ln<float, __half>(p, vec, st) : launch_ln<float, float>(p, vec, st);
+        return a->out_dtype == MAMBA_F16 ? launch_ln<__half, __half>(p, access, st) : launch_ln<__half, float>(p, access, st);
+    return a->out_dtype == MAMBA_F16 ? launch_ln<float, __half>(p, access, st) : launch_ln<float, float>(p, access, st);
 }
 
 size_t layer_norm_workspace_bytes(const MambaLayerNormArgs *a) {
@@ -454,16 +480,22 @@ int layer_norm_backward(const MambaLayerNormArgs *a, const MambaLayerNormGrads *
     float *part = static_cast<float *>(ws);
     if (g->dw) p.part_w = part;
     if (g->db) p.part_b = part + ((int64_t)grid * a->cols + 3) / 4 * 4;  // grid is still the most
-    const bool vec = a->cols % 8 == 0 && aligned_rows(a->x, a->x_stride, a->x_dtype) &&
-                     aligned_rows(g->dout, g->dout_stride, a->out_dtype) &&
-                     aligned_rows(g->dx, g->dx_stride, a->x_dtype) && aligned_to(a->w, 16);
+    Access access = kSingle;
+    if (a->cols % 8 == 0 && aligned_rows(a->x, a->x_stride, a->x_dtype, 16) &&
+        aligned_rows(g->dout, g->dout_stride, a->out_dtype, 16) && aligned_rows(g->dx, g->dx_stride, a->x_dtype, 16) &&
+        aligned_to(a->w, 16))
+        access = kWide;
+    else if (a->cols % 2 == 0 && pair_rows(a->x, a->x_stride, a->x_dtype) &&
+             pair_rows(g->dout, g->dout_stride, a->out_dtype) && pair_rows(g->dx, g->dx_stride, a->x_dtype) &&
+             aligned_to(a->w, 8))
+        access = kPairs;
     int rc;
     if (a->x_dtype == MAMBA_F16)
-        rc = a->out_dtype == MAMBA_F16 ? launch_ln_bwd<__half, __half>(p, vec, grid, st)
-                                       : launch_ln_bwd<__half, float>(p, vec, grid, st);
+        rc = a->out_dtype == MAMBA_F16 ? launch_ln_bwd<__half, __half>(p, access, grid, st)
+                                       : launch_ln_bwd<__half, float>(p, access, grid, st);
     else
-        rc = a->out_dtype == MAMBA_F16 ? launch_ln_bwd<float, __half>(p, vec, grid, st)
-                                       : launch_ln_bwd<float, float>(p, vec, grid, st);
+        rc = a->out_dtype == MAMBA_F16 ? launch_ln_bwd<float, __half>(p, access, grid, st)
+                                       : launch_ln_bwd<float, float>(p, access, grid, st);
     if (rc) return -1;
     if (!g->dw && !g->db) return 0;
     column_sum_kernel<kLnSumThreads><<<dim3((unsigned)ceil_div(a->cols, 32), 2), kLnSumThreads, 0, st>>>(

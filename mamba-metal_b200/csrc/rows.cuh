@@ -17,11 +17,15 @@ namespace {
 constexpr int kMaxCols = 16384;
 constexpr int kDirectParts = 296;  // CTAs of the backward pass without a ring: few, so that their partial sums are
 
-// N consecutive elements as FP32; N = 8 by 16-byte accesses, N = 4 by 16 or 8 bytes.
+// N consecutive elements as FP32; N = 8 by 16-byte accesses, N = 4 and 2 by one of their size.
 template <int N>
 __device__ __forceinline__ void load_n(const float *p, float (&v)[N]) {
     if constexpr (N == 1) {
         v[0] = *p;
+    } else if constexpr (N == 2) {
+        const float2 q = *reinterpret_cast<const float2 *>(p);
+        v[0] = q.x;
+        v[1] = q.y;
     } else {
 #pragma unroll
         for (int k = 0; k < N; k += 4) {
@@ -37,6 +41,10 @@ template <int N>
 __device__ __forceinline__ void load_n(const __half *p, float (&v)[N]) {
     if constexpr (N == 1) {
         v[0] = __half2float(*p);
+    } else if constexpr (N == 2) {
+        const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(p));
+        v[0] = q.x;
+        v[1] = q.y;
     } else if constexpr (N == 4) {
         const uint2 raw = *reinterpret_cast<const uint2 *>(p);
         const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x));
@@ -60,6 +68,8 @@ template <int N>
 __device__ __forceinline__ void store_n(float *p, const float (&v)[N]) {
     if constexpr (N == 1) {
         *p = v[0];
+    } else if constexpr (N == 2) {
+        *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
     } else {
 #pragma unroll
         for (int k = 0; k < N; k += 4)
@@ -70,6 +80,8 @@ template <int N>
 __device__ __forceinline__ void store_n(__half *p, const float (&v)[N]) {
     if constexpr (N == 1) {
         *p = __float2half_rn(v[0]);
+    } else if constexpr (N == 2) {
+        *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(v[0], v[1]);
     } else if constexpr (N == 4) {
         const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
         *reinterpret_cast<uint2 *>(p) =
