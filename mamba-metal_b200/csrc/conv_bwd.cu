@@ -6,7 +6,7 @@
 //
 // Bound by bytes and, near them, by issue slots (about 30 a FP16 element, packed
 // operations counted twice): one pass over x and dy that writes dx.  8 x 4096 x
-// 4096 FP16, K 4, SiLU: 168 us for 805 MB with 4 channels a thread and 128
+// 4096 FP16, K 4, SiLU: 160-168 us for 805 MB with 4 channels a thread and 128
 // registers (four CTAs an SM); with 154 registers 182, 102 registers 244, 2
 // channels a thread 227, 8 rows in flight instead of 4 203.  A thread owns VEC
 // channels and a run of timesteps; the last K inputs and the last K p_t stay in
@@ -248,10 +248,12 @@ __global__ void __launch_bounds__(THREADS)
     }
 }
 
-// Timesteps per thread: 128, fewer where that leaves the GPU short of threads.
+// Timesteps per thread: 128, fewer where that leaves less than 256 threads an SM (8
+// x 4096 x 1000 FP16 and 1 x 4096 x 2048, with the sums of the partial rows: 56
+// and 21 us; for 512 threads 55 and 24, 1024 66 and 24).
 int run_length(int64_t batch, int64_t L, int64_t D) {
     int run = 128;
-    while (run > 16 && batch * ceil_div64(L, run) * ceil_div64(D, 4) < 148 * 1024) run /= 2;
+    while (run > 16 && batch * ceil_div64(L, run) * ceil_div64(D, 4) < 148 * 256) run /= 2;
     return run;
 }
 
