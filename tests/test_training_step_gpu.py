@@ -163,6 +163,29 @@ def test_two_streams_at_once(cuda):
                 assert (a[1][name] - b[1][name]).abs().max() <= 1e-5 * b[1][name].abs().max(), name
 
 
+def test_scan_gradients_beside_tensor_core_products(cuda):
+    """Both keep accumulators in tensor memory: calls on two streams wait for each other's columns, and give what they
+    give alone."""
+    g = torch.Generator(device="cpu").manual_seed(9)
+    r = lambda *s: torch.randn(s, generator=g).half().cuda()  # noqa: E731
+    xl, wl = r(4096, 1024), r(1024, 1024)
+    dy, x, z, delta, B, C = r(4, 256, 1024), r(4, 256, 1024), r(4, 256, 1024), r(4, 256, 1024), r(4, 256, 16), r(4, 256, 16)
+    A = -torch.arange(1, 17, device="cuda", dtype=torch.float32).repeat(1024, 1)
+    run = lambda: mb.selective_scan_backward(dy, x, delta, A, B, C, z=z)  # noqa: E731
+    want, want_l = run(), mb.linear(xl, wl)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(a):
+            got = [run() for _ in range(3)][-1]
+        with torch.cuda.stream(b):
+            got_l = [mb.linear(xl, wl) for _ in range(20)][-1]
+    torch.cuda.synchronize()
+    assert torch.equal(got_l, want_l)
+    assert all(p is q or torch.equal(p, q) for p, q in zip(got, want))
+    assert mb.device_status() == 0
+
+
 @pytest.mark.parametrize("side", [False, True])
 def test_model_forward_of_tokens(cuda, side):
     m = mb.Model(32, 16, 4, 2, 2, mb.F16)
