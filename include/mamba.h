@@ -266,9 +266,11 @@ int mamba_selective_scan(const MambaScanArgs *a, void *workspace, size_t workspa
  * and dinitial_state [batch, dim, dstate].  NULL: dB, dC, dA, dD, ddt_bias,
  * dinitial_state (not wanted).  All sums are FP32 in a fixed order: the same
  * bits on every call.  Strides in elements {batch, time, channel} ({batch,
- * time, state} for dB and dC).  FP16 tensors: exponentials and reciprocals are
- * approximate (2e-6).  Where |A| <= 1e-6 the gradients are those of the
- * zero-order hold's limit. Outputs must not overlap inputs or each other.  batch * seqlen * ceil(dim / 128) <= 2^31. */
+ * time, state} for dB and dC).  FP16 tensors: the exponentials e^(dt A) and the
+ * reciprocals are approximate (relative errors below 4e-7, of e^(dt A) also what
+ * rounding dt A to FP32 makes; 3e-6 of e^(dt A) - 1).  Where |A| <= 1e-6 the gradients are
+ * those of the zero-order hold's limit.  Outputs must not overlap inputs or each other.
+ * batch * seqlen * ceil(dim / 128) <= 2^31. */
 typedef struct MambaScanGrads {
     const void *dy;
     const float *dfinal_state;

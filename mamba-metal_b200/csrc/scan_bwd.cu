@@ -8,11 +8,13 @@
 //   dB = sum_d g phi x,            dC = sum_d q h_t
 //   ddelta = sigmoid(delta + dt_bias) sum_n g a (A h_{t-1} + w)
 //   dA = sum g (dt a h_{t-1} + w psi),   psi = (dt a - phi) / A
-// a - 1 is evaluated without cancellation (e): phi = e / A, and with FP16 tensors
-// e takes the place of a too: h_t = h + e (h + w / A), a g = g + e g.  Of A the
-// kernels keep A2 = A log2(e) and K2 = 1 / A2, with B log2(e) in place of B, so
-// that w / A = w2 K2.  dA is summed as A dA = sum r dt ln 2 h_{t-1} + g w2 (dt a
-// - phi) / log2(e) with r = g a A2.  A state with |A| < 1e-20 counts as 1e-20,
+// a - 1 is evaluated without cancellation (e): phi = e / A.  With FP16 tensors a
+// state and token has only e where |dt A| < 1/16 (h_t = h + e (h + w / A), a g =
+// g + e g) and only a elsewhere (h_t = a (h + w / A) - w / A): from the other of
+// the two, what a weak decay takes or a strong one leaves would be lost.  Of A
+// the kernels keep A2 = A log2(e) and K2 = 1 / A2, with B log2(e) in place of B,
+// so that w / A = w2 K2.  dA is summed as A dA = sum r dt ln 2 h_{t-1} + w2 g (dt
+// a - phi) / log2(e) with r = g a A2.  A state with |A| < 1e-20 counts as 1e-20,
 // where all of these are the limits.
 //
 // Three passes over time chunks:
@@ -82,13 +84,14 @@ __device__ __forceinline__ float clamp_nan(float v, float lo, float hi) {
 }
 
 // e = 2^v - 1, and a = 2^v, for two states.
-// FP16 tensors: one approximate exponential less 1, or where |dt A| is below
-// 1/16 the series to the fourth power (relative errors below 2e-6 and 2e-7);
-// a is left to the caller as 1 + e.
+// FP16 tensors: where |dt A| is below 1/16 (near) e by the series to the fourth
+// power (relative error 2e-7), elsewhere one approximate exponential a (2e-7;
+// that of a - 1 is up to 2e-6).  Either is returned in e.
 // FP32 tensors: v = j + f with j whole and |f| <= 1/2, 2^f - 1 = f q(f) with q
 // interpolating (2^f - 1) / f at the six Chebyshev nodes of [-1/2, 1/2]
 // (relative error 7e-8), a = 2^j (1 + f q), e = 2^j f q + (2^j - 1).
 constexpr float kNear = 0.0625f * 1.4426950408889634f;
+__device__ __forceinline__ bool is_near(float v) { return fabsf(v) < kNear; }
 template <bool PRECISE>
 __device__ __forceinline__ void exp2m1_2(float2 v, float2 &e, float2 &a) {
     if (PRECISE) {
@@ -109,39 +112,50 @@ __device__ __forceinline__ void exp2m1_2(float2 v, float2 &e, float2 &a) {
         return;
     }
     constexpr float c1 = 0.69314718055994531f, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
-    float2 far = make_float2(ex2_approx(v.x), ex2_approx(v.y));
-    far = fadd2(far, make2(-1.f));
+    const float2 far = make_float2(ex2_approx(v.x), ex2_approx(v.y));
     float2 s = ffma2(v, make2(c4), make2(c3));
     s = ffma2(s, v, make2(c2));
     s = ffma2(s, v, make2(c1));
     s = fmul2(s, v);
-    e = make_float2(fabsf(v.x) < kNear ? s.x : far.x, fabsf(v.y) < kNear ? s.y : far.y);
+    e = make_float2(is_near(v.x) ? s.x : far.x, is_near(v.y) ? s.y : far.y);
+}
+// (a - 1) K2 = phi / log2(e).
+template <bool PRECISE>
+__device__ __forceinline__ float2 phi_2(float2 v, float2 e, float2 K2) {
+    if (PRECISE) return fmul2(e, K2);
+    return ffma2(e, K2, make_float2(is_near(v.x) ? 0.f : -K2.x, is_near(v.y) ? 0.f : -K2.y));
 }
 
-// a x.  FP16 tensors: x + e x, which is off by 2^-24 |x| where a is small.
+// a x (FP16 tensors, near: x + e x).
 template <bool PRECISE>
-__device__ __forceinline__ float2 decay_2(float2 e, float2 a, float2 x) {
-    return PRECISE ? fmul2(a, x) : ffma2(e, x, x);
+__device__ __forceinline__ float2 decay_2(float2 v, float2 e, float2 a, float2 x) {
+    if (PRECISE) return fmul2(a, x);
+    return ffma2(e, x, make_float2(is_near(v.x) ? x.x : 0.f, is_near(v.y) ? x.y : 0.f));
 }
-// h_t = a h + phi w = h + e (h + w / A).
+// h_t = a h + phi w (FP16 tensors: a (h + w / A) - w / A, near h + e (h + w / A)).
 template <bool PRECISE>
-__device__ __forceinline__ float2 step_2(float2 e, float2 a, float2 w, float2 K2, float2 h) {
-    return PRECISE ? ffma2(fmul2(e, K2), w, fmul2(a, h)) : ffma2(e, ffma2(w, K2, h), h);
+__device__ __forceinline__ float2 step_2(float2 v, float2 e, float2 a, float2 w, float2 K2, float2 h) {
+    if (PRECISE) return ffma2(fmul2(e, K2), w, fmul2(a, h));
+    const float2 wk = fmul2(w, K2);
+    return ffma2(e, fadd2(h, wk), make_float2(is_near(v.x) ? h.x : -wk.x, is_near(v.y) ? h.y : -wk.y));
 }
 
-// (dt a - phi) / log2(e) from e, phi / log2(e) = e / A2 and dt ln 2.  The
-// difference loses 2 d / x^2 of its value for an absolute error d of e, where x =
-// dt A: so below |x| = 0.4 (d = 6e-8: 8e-7; FP32 tensors, whose e has a relative
-// error, 0.25) phi (x / (1 - e^-x) - 1) by x/2 + x^2/12 - x^4/720 (the next term
-// is 7e-7 of the sum at 0.4).
+// g (dt a - phi) / log2(e) from e, phi / log2(e) = (a - 1) / A2 and dt ln 2, and
+// from g a and g phi.  The difference loses 2 d / x^2 of its value for an absolute
+// error d of e, where x = dt A: so below |x| = 0.4 (d = 6e-8: 8e-7; FP32 tensors,
+// whose e has a relative error, 0.25) phi (x / (1 - e^-x) - 1) by x/2 + x^2/12 -
+// x^4/720 (the next term is 7e-7 of the sum at 0.4).  FP16 tensors: the roundings
+// of g a and g phi are 3e-7 of the difference at 0.4 each.
 template <bool PRECISE>
-__device__ __forceinline__ float2 bend_2(float2 v, float2 e, float2 phi, float2 dt_ln2) {
+__device__ __forceinline__ float2 bend_2(float2 v, float2 e, float2 phi, float2 dt_ln2, float2 g, float2 ga,
+                                         float2 gphi) {
     constexpr float c1 = 0.69314718055994531f, c2 = c1 * c1 / 12, c4 = -c1 * c1 * c1 * c1 / 720;
     constexpr float near = (PRECISE ? 0.25f : 0.4f) * kLog2e;
-    const float2 far = ffma2(phi, make2(-1.f), ffma2(dt_ln2, e, dt_ln2));
+    const float2 far = PRECISE ? fmul2(g, ffma2(phi, make2(-1.f), ffma2(dt_ln2, e, dt_ln2)))
+                               : ffma2(dt_ln2, ga, make_float2(-gphi.x, -gphi.y));
     float2 s = ffma2(fmul2(v, v), make2(c4), make2(c2));
     s = ffma2(s, v, make2(c1 / 2));
-    s = fmul2(fmul2(s, v), phi);
+    s = fmul2(fmul2(s, v), gphi);
     return make_float2(fabsf(v.x) < near ? s.x : far.x, fabsf(v.y) < near ? s.y : far.y);
 }
 
@@ -307,8 +321,8 @@ __device__ __forceinline__ Place place(const ScanGradParams &p) {
     return r;
 }
 
-// Pass 1: 0.85 ms of the same call, at 17 instructions a state and token (issue
-// 0.53 a cycle); with its inputs fetched a round ahead (three CTAs an SM) 0.90.
+// Pass 1: 0.82 ms of the call below; with its inputs fetched a round ahead (three
+// CTAs an SM) 0.05 more.
 template <typename Tx, typename Td, typename Tb, bool MULTI>
 __global__ void __launch_bounds__(kCh, 4) scan_bwd_states_kernel(const ScanGradParams p) {
     constexpr bool PRECISE = sizeof(Tx) == 4;
@@ -325,6 +339,7 @@ __global__ void __launch_bounds__(kCh, 4) scan_bwd_states_kernel(const ScanGradP
     float2 A2[4][2], K2[4][2], h[4][2], P[4][2], G[4][2];
     load_A(p, c4, n4, A2, K2);
     load_given(p, at.chunk == 0 ? p.h0 : nullptr, at.b, c4, n4, h);
+    float2 since[2] = {make2(0.f), make2(0.f)};  // sum of dt
     if (MULTI) {
 #pragma unroll
         for (int s = 0; s < 4; ++s)
@@ -378,6 +393,8 @@ __global__ void __launch_bounds__(kCh, 4) scan_bwd_states_kernel(const ScanGradP
                 const float4 q4 = *reinterpret_cast<const float4 *>(&qs[buf][k][l4]);
                 q2[0] = lo2(q4);
                 q2[1] = hi2(q4);
+                since[0] = fadd2(since[0], d2[0]);
+                since[1] = fadd2(since[1], d2[1]);
             }
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
@@ -385,10 +402,17 @@ __global__ void __launch_bounds__(kCh, 4) scan_bwd_states_kernel(const ScanGradP
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     float2 e, a;
-                    exp2m1_2<PRECISE>(fmul2(d2[i], A2[s][i]), e, a);
-                    h[s][i] = step_2<PRECISE>(e, a, fmul2(x2[i], lo2(bc)), K2[s][i], h[s][i]);
+                    const float2 v = fmul2(d2[i], A2[s][i]);
+                    exp2m1_2<PRECISE>(v, e, a);
+                    h[s][i] = step_2<PRECISE>(v, e, a, fmul2(x2[i], lo2(bc)), K2[s][i], h[s][i]);
                     if (MULTI) {
-                        P[s][i] = decay_2<PRECISE>(e, a, P[s][i]);
+                        // the decay since the chunk's start
+                        if (PRECISE) {
+                            P[s][i] = fmul2(a, P[s][i]);
+                        } else {  // as a product the 16 P would spill (890 us in place of 821)
+                            const float2 u = fmul2(since[i], A2[s][i]);
+                            P[s][i] = make_float2(ex2_approx(u.x), ex2_approx(u.y));
+                        }
                         G[s][i] = ffma2(P[s][i], fmul2(hi2(bc), q2[i]), G[s][i]);
                     }
                 }
@@ -500,17 +524,34 @@ __device__ __forceinline__ void tmem_get(uint32_t at, float2 (&v)[4][2]) {
         : "r"(at));
 }
 
+// 16 values each from 32 columns in a row.
+__device__ __forceinline__ void tmem_get(uint32_t at, float2 (&v)[4][2], float2 (&w)[4][2]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32"
+        " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+        " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0][0].x), "=f"(v[0][0].y), "=f"(v[0][1].x), "=f"(v[0][1].y), "=f"(v[1][0].x), "=f"(v[1][0].y),
+          "=f"(v[1][1].x), "=f"(v[1][1].y), "=f"(v[2][0].x), "=f"(v[2][0].y), "=f"(v[2][1].x), "=f"(v[2][1].y),
+          "=f"(v[3][0].x), "=f"(v[3][0].y), "=f"(v[3][1].x), "=f"(v[3][1].y), "=f"(w[0][0].x), "=f"(w[0][0].y),
+          "=f"(w[0][1].x), "=f"(w[0][1].y), "=f"(w[1][0].x), "=f"(w[1][0].y), "=f"(w[1][1].x), "=f"(w[1][1].y),
+          "=f"(w[2][0].x), "=f"(w[2][0].y), "=f"(w[2][1].x), "=f"(w[2][1].y), "=f"(w[3][0].x), "=f"(w[3][0].y),
+          "=f"(w[3][1].x), "=f"(w[3][1].y)
+        : "r"(at));
+}
+
 // Pass 3.  The states before each of 8 tokens are 128 columns of tensor memory
-// (a thread's own lane), and with FP16 tensors the e of each token 128 more, so
-// that the reverse steps do not evaluate it again.
+// (a thread's own lane), and with FP16 tensors the e or a of each token 128 more,
+// so that the reverse steps do not evaluate it again; there the state behind a
+// token is loaded too (the next one's), which costs less than to compute it.
 //
-// Bound by issue slots: about 40 instructions a state and token, 18 of them
-// packed (which take two slots), at 0.5 instructions a cycle and scheduler; DRAM
-// 15%.  8 x 2048 x 4096 FP16: 2.24 ms with two CTAs an SM and 255 registers.
-// With the states in shared memory 2.8 ms; three CTAs, 168 registers and 128
-// columns 3.07; two CTAs without e 2.77; scalar operations 2.39; the next
-// token's values loaded from tensor memory during the sums over lanes 2.28.
-constexpr uint32_t kColumns = 2 * kT * kN;
+// About 40 instructions a state and token, 18 of them packed (which take two
+// issue slots), at 0.5 instructions a cycle and scheduler; DRAM 15%.  8 x 2048 x
+// 4096 FP16: 2.29 ms with two CTAs an SM and 255 registers.  Measured when e
+// stood for a as well (2.24): the states in shared memory 2.8 ms; three CTAs, 168
+// registers and 128 columns 3.07; two CTAs without e 2.77; scalar operations
+// 2.39; the next token's values loaded during the sums over lanes 2.28.
+constexpr uint32_t kColumns = 2 * kT * kN, kSlot = 2 * kN;
 template <typename Tx, typename Td, typename Tb, bool MULTI>
 __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p) {
     constexpr bool PRECISE = sizeof(Tx) == 4, KEEP_E = !PRECISE;
@@ -617,8 +658,8 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
         }
 #pragma unroll
         for (int k = 0; k < kT; ++k) {
-            tmem_put(tmem + k * kN, h);
-            if (!KEEP_E && k + 1 == kT) break;
+            tmem_put(tmem + k * kSlot, h);
+            if (!KEEP_E && k + 1 == kT) break;  // FP16 tensors: h becomes the state behind the last token
             float2 ee[4][2];
             const float4 x4 = *reinterpret_cast<const float4 *>(&xs[k][l4]);
             const float4 d4 = *reinterpret_cast<const float4 *>(&dts[k][l4]);
@@ -629,12 +670,13 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     float2 e, a;
-                    exp2m1_2<PRECISE>(fmul2(d2[i], A2[s][i]), e, a);
+                    const float2 v = fmul2(d2[i], A2[s][i]);
+                    exp2m1_2<PRECISE>(v, e, a);
                     if (KEEP_E) ee[s][i] = e;
-                    h[s][i] = step_2<PRECISE>(e, a, fmul2(x2[i], B2), K2[s][i], h[s][i]);
+                    h[s][i] = step_2<PRECISE>(v, e, a, fmul2(x2[i], B2), K2[s][i], h[s][i]);
                 }
             }
-            if (KEEP_E) tmem_put(tmem + (kT + k) * kN, ee);
+            if (KEEP_E) tmem_put(tmem + k * kSlot + kN, ee);
         }
         tmem_wait_st();
 #pragma unroll 1
@@ -643,10 +685,8 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
             const float4 d4 = *reinterpret_cast<const float4 *>(&dts[k][l4]);
             const float4 q4 = *reinterpret_cast<const float4 *>(&qs[k][l4]);
             const float2 x2[2] = {lo2(x4), hi2(x4)}, d2[2] = {lo2(d4), hi2(d4)}, q2[2] = {lo2(q4), hi2(q4)};
-            float2 hp[4][2], y[2], dx[2], dd[2], dt_ln2[2];
-            float2 ee[4][2];
-            tmem_get(tmem + k * kN, hp);
-            if (KEEP_E) tmem_get(tmem + (kT + k) * kN, ee);
+            if (KEEP_E && k + 1 < kT) tmem_get(tmem + (k + 1) * kSlot, h);  // the state behind the token
+            float2 y[2], dx[2], dd[2], dt_ln2[2];
             float v8[8];  // dB of the 4 states, dC of them: sums over the 4 channels
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -655,10 +695,30 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
                 dd[i] = make2(0.f);
                 dt_ln2[i] = fmul2(d2[i], make2(kLn2));
             }
+            auto use_state = [&](int s, int i, float2 C2, float2 ht, float2 &dC) {
+                y[i] = ffma2(C2, ht, y[i]);
+                dC = i ? ffma2(q2[i], ht, dC) : fmul2(q2[i], ht);
+                g[s][i] = ffma2(C2, q2[i], g[s][i]);
+            };
+            if (KEEP_E) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const float2 C2 = reinterpret_cast<const float2 *>(&bc4[k][s * 4 + j])[1];
+                    float2 dC;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) use_state(s, i, C2, h[s][i], dC);
+                    v8[4 + s] = dC.x + dC.y;
+                }
+            }
+            float2 hp[4][2], ee[4][2];
+            if (KEEP_E)
+                tmem_get(tmem + k * kSlot, hp, ee);
+            else
+                tmem_get(tmem + k * kSlot, hp);
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 const float4 bc = bc4[k][s * 4 + j];
-                const float2 B2 = lo2(bc), C2 = hi2(bc);
+                const float2 B2 = lo2(bc);
                 float2 dB, dC;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -669,25 +729,22 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
                     else
                         exp2m1_2<PRECISE>(v, e, a);
                     const float2 w = fmul2(x2[i], B2);
+                    if (!KEEP_E) use_state(s, i, hi2(bc), step_2<PRECISE>(v, e, a, w, K2[s][i], hp[s][i]), dC);
+                    const float2 gt = g[s][i];
                     const float2 hw = ffma2(w, K2[s][i], hp[s][i]);  // h_{t-1} + B x / A
-                    const float2 ht = PRECISE ? step_2<PRECISE>(e, a, w, K2[s][i], hp[s][i])
-                                              : ffma2(e, hw, hp[s][i]);
-                    y[i] = ffma2(C2, ht, y[i]);
-                    dC = i ? ffma2(q2[i], ht, dC) : fmul2(q2[i], ht);
-                    const float2 gt = ffma2(C2, q2[i], g[s][i]);
-                    const float2 phi = fmul2(e, K2[s][i]), gphi = fmul2(gt, phi);
-                    const float2 ga = decay_2<PRECISE>(e, a, gt);
+                    const float2 ga = decay_2<PRECISE>(v, e, a, gt);
+                    const float2 phi = phi_2<PRECISE>(v, e, K2[s][i]), gphi = fmul2(gt, phi);
                     g[s][i] = ga;
                     dB = i ? ffma2(gphi, x2[i], dB) : fmul2(gphi, x2[i]);
                     dx[i] = ffma2(gphi, B2, dx[i]);
                     const float2 r = fmul2(ga, A2[s][i]);
                     dd[i] = ffma2(r, hw, dd[i]);
-                    const float2 bend = bend_2<PRECISE>(v, e, phi, dt_ln2[i]);
+                    const float2 bend = bend_2<PRECISE>(v, e, phi, dt_ln2[i], gt, ga, gphi);
                     dA[s][i] = ffma2(fmul2(r, dt_ln2[i]), hp[s][i], dA[s][i]);
-                    dA[s][i] = ffma2(fmul2(gt, w), bend, dA[s][i]);
+                    dA[s][i] = ffma2(w, bend, dA[s][i]);
                 }
                 v8[s] = dB.x + dB.y;
-                v8[4 + s] = dC.x + dC.y;
+                if (!KEEP_E) v8[4 + s] = dC.x + dC.y;
             }
             const float ys = quad_sum(y, j), dxs = quad_sum(dx, j), dds = quad_sum(dd, j);
             const float r = oct_sum(v8, lane);
