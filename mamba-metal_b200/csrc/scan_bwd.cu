@@ -551,10 +551,10 @@ __device__ __forceinline__ void tmem_get(uint32_t at, float2 (&v)[4][2], float2 
 // stood for a as well (2.24): the states in shared memory 2.8 ms; three CTAs, 168
 // registers and 128 columns 3.07; two CTAs without e 2.77; scalar operations
 // 2.39; the next token's values loaded during the sums over lanes 2.28.
-constexpr uint32_t kColumns = 2 * kT * kN, kSlot = 2 * kN;
 template <typename Tx, typename Td, typename Tb, bool MULTI>
 __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p) {
     constexpr bool PRECISE = sizeof(Tx) == 4, KEEP_E = !PRECISE;
+    constexpr uint32_t SLOT = KEEP_E ? 2 * kN : kN, COLUMNS = kT * SLOT;  // tensor-memory columns of a token, of all
     __shared__ __align__(16) float xs[kT][kCh];   // x, later dx
     __shared__ __align__(16) float dts[kT][kCh];  // dt, later the gradient of dt
     __shared__ __align__(16) float qs[kT][kCh];   // q, later sum_n C h + D x
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
     const int t_first = at.chunk * p.chunk, t_end = min(p.L, t_first + p.chunk);
     const int64_t chunk = (int64_t)at.b * p.chunks + at.chunk;
     if (warp == 0) {
-        tmem_alloc(&tmem_base, kColumns);
+        tmem_alloc(&tmem_base, COLUMNS);
         tmem_relinquish();
         tc_fence_before();
     }
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
         }
 #pragma unroll
         for (int k = 0; k < kT; ++k) {
-            tmem_put(tmem + k * kSlot, h);
+            tmem_put(tmem + k * SLOT, h);
             if (!KEEP_E && k + 1 == kT) break;  // FP16 tensors: h becomes the state behind the last token
             float2 ee[4][2];
             const float4 x4 = *reinterpret_cast<const float4 *>(&xs[k][l4]);
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
                     h[s][i] = step_2<PRECISE>(v, e, a, fmul2(x2[i], B2), K2[s][i], h[s][i]);
                 }
             }
-            if (KEEP_E) tmem_put(tmem + k * kSlot + kN, ee);
+            if (KEEP_E) tmem_put(tmem + k * SLOT + kN, ee);
         }
         tmem_wait_st();
 #pragma unroll 1
@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
             const float4 d4 = *reinterpret_cast<const float4 *>(&dts[k][l4]);
             const float4 q4 = *reinterpret_cast<const float4 *>(&qs[k][l4]);
             const float2 x2[2] = {lo2(x4), hi2(x4)}, d2[2] = {lo2(d4), hi2(d4)}, q2[2] = {lo2(q4), hi2(q4)};
-            if (KEEP_E && k + 1 < kT) tmem_get(tmem + (k + 1) * kSlot, h);  // the state behind the token
+            if (KEEP_E && k + 1 < kT) tmem_get(tmem + (k + 1) * SLOT, h);  // the state behind the token
             float2 y[2], dx[2], dd[2], dt_ln2[2];
             float v8[8];  // dB of the 4 states, dC of them: sums over the 4 channels
 #pragma unroll
@@ -712,9 +712,9 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
             }
             float2 hp[4][2], ee[4][2];
             if (KEEP_E)
-                tmem_get(tmem + k * kSlot, hp, ee);
+                tmem_get(tmem + k * SLOT, hp, ee);
             else
-                tmem_get(tmem + k * kSlot, hp);
+                tmem_get(tmem + k * SLOT, hp);
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 const float4 bc = bc4[k][s * 4 + j];
@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(kCh, 2) scan_bwd_kernel(const ScanGradParams p
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem_base, kColumns);
+    if (warp == 0) tmem_dealloc(tmem_base, COLUMNS);
 }
 
 struct ScanSumParams {

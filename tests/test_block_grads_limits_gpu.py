@@ -66,3 +66,29 @@ def test_steps_that_forget(cuda, b, L, D, N, kind):
         if not err.max() <= 0:  # a NaN too
             bad.append((k, err.max()))
     assert not bad, bad
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_beside_tensor_core_products(cuda, dtype):
+    """Two streams whose kernels both keep values in tensor memory, one of them with a round of CTAs that hold
+    their columns for 256 tokens: results as alone."""
+    g = torch.Generator(device="cpu").manual_seed(9)
+    r = lambda *s: torch.randn(s, generator=g).cuda()  # noqa: E731
+    xl, wl = r(4096, 1024).half(), r(1024, 1024).half()
+    b, L, D = 4, 512, 128 * 74
+    dy, x, z, delta = ((0.1 * r(b, L, 64)).to(dtype).repeat(1, 1, D // 64) for _ in range(4))
+    B, C = r(b, L, 16).to(dtype), r(b, L, 16).to(dtype)
+    A = -torch.arange(1, 17, device="cuda", dtype=torch.float32).repeat(D, 1)
+    run = lambda: mb.selective_scan_backward(dy, x, delta, A, B, C, z=z)  # noqa: E731
+    want, want_l = run(), mb.linear(xl, wl)
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(one):
+            got = run()
+        with torch.cuda.stream(two):
+            got_l = [mb.linear(xl, wl) for _ in range(20)][-1]
+    torch.cuda.synchronize()
+    assert torch.equal(got_l, want_l)
+    assert all(p is q or torch.equal(p, q) for p, q in zip(got, want))
+    assert mb.device_status() == 0
