@@ -125,6 +125,11 @@ unsigned mamba_device_status(int clear);
  * 7 and 8. */
 int mamba_selftest_bounded_wait(unsigned limit_us, void *stream);
 
+/* The same for the row waits of the layer norm (bit 8) and of the embedding's
+ * gradient (bit 9): both run out after limit_us microseconds (1..1000000) and
+ * are reported in mamba_device_status.  0 when both kernels ran, -1 otherwise. */
+int mamba_selftest_row_waits(unsigned limit_us, void *stream);
+
 /* dt_rank used for a config: ceil(d_model / 16). */
 int mamba_dt_rank(const MambaConfig *cfg);
 

@@ -459,6 +459,13 @@ __device__ void zero_rows(const SumParams &p, int64_t tile) {
     }
 }
 
+// Waits for the row at a place of the ring.  A wait that runs out is reported; the
+// CTA goes on, with wrong values.
+__device__ __forceinline__ void await_sum_row(uint64_t *full, const RingPlace &at, LostCopies *lost,
+                                              uint64_t limit_ns = kWaitNs) {
+    if (!await_copy(full, at.s, at.parity, lost, limit_ns)) atomicOr(&g_embedding_error, kErrEmbeddingTimeout);
+}
+
 // blockIdx.x: part, and behind the parts tiles of the table to zero; blockIdx.y:
 // block of columns (the zeroing has one).  A thread has NV groups of VEC columns,
 // group g at column (g * threads + t) * VEC.
@@ -515,7 +522,7 @@ __global__ void __launch_bounds__(kSumThreadsE) embedding_sum_kernel(const SumPa
     for (uint32_t i = first; i < live; ++i) {
         const uint32_t after = i + 2 < p.n ? p.keys[i + 2] : p.vocab;  // on its way while the row is added
         const uint32_t shift = VEC <= 2 ? (uint32_t)reinterpret_cast<uintptr_t>(from(p.pos[i])) & 15u : 0u;
-        if (!await_copy(full, at.s, at.parity, &lost, kWaitNs)) atomicOr(&g_embedding_error, kErrEmbeddingTimeout);
+        await_sum_row(full, at, &lost);
         const T *row = reinterpret_cast<const T *>(ring + at.s * p.stage + shift);
 #pragma unroll
         for (int g = 0; g < NV; ++g) {
@@ -635,6 +642,18 @@ Layout layout(int64_t n, int dim) {
     return l;
 }
 
+// A wait for a row that nothing fetches, through the kernel's own helpers.
+__global__ void embedding_wait_selftest_kernel(uint64_t limit_ns) {
+    __shared__ uint64_t full;
+    __shared__ LostCopies lost;
+    if (threadIdx.x != 0) return;
+    lost = LostCopies{};
+    mbar_init(&full, 1);
+    fence_mbar_init();
+    await_sum_row(&full, RingPlace{}, &lost, limit_ns);
+    drain_copies(&full, 1, &lost, limit_ns);
+}
+
 constexpr int64_t kMaxTokens = (int64_t)1 << 30;
 
 int check_embedding(const MambaEmbeddingArgs *a, const std::string &what) {
@@ -652,6 +671,11 @@ int check_embedding(const MambaEmbeddingArgs *a, const std::string &what) {
 }
 
 }  // namespace
+
+int embedding_wait_selftest(uint64_t limit_ns, cudaStream_t st) {
+    embedding_wait_selftest_kernel<<<1, 32, 0, st>>>(limit_ns);
+    return launch_status("embedding wait self-test kernel");
+}
 
 unsigned embedding_error_flags(bool clear) {
     unsigned v = 0;

@@ -83,6 +83,7 @@ int layer_norm(const MambaLayerNormArgs *a, cudaStream_t st);
 int layer_norm_backward(const MambaLayerNormArgs *a, const MambaLayerNormGrads *g, void *ws, size_t ws_bytes,
                         cudaStream_t st);
 unsigned layer_norm_error_flags(bool clear);
+int layer_norm_wait_selftest(uint64_t limit_ns, cudaStream_t st);
 
 // embedding.cu
 int embedding(const MambaEmbeddingArgs *a, cudaStream_t st);
@@ -90,6 +91,7 @@ size_t embedding_workspace_bytes(const MambaEmbeddingArgs *a);
 int embedding_backward(const MambaEmbeddingArgs *a, const void *dout, int64_t dout_stride, float *dtable,
                        int64_t dtable_stride, int accumulate, void *ws, size_t ws_bytes, cudaStream_t st);
 unsigned embedding_error_flags(bool clear);
+int embedding_wait_selftest(uint64_t limit_ns, cudaStream_t st);
 
 // dropout.cu
 int dropout(const MambaDropoutArgs *a, cudaStream_t st);

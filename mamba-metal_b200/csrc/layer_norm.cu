@@ -503,6 +503,27 @@ int layer_norm_backward(const MambaLayerNormArgs *a, const MambaLayerNormGrads *
     return launch_status("layer_norm_backward sum kernel");
 }
 
+namespace {
+
+// A wait for a row that nothing fetches, through the kernels' own helpers.
+__global__ void layer_norm_wait_selftest_kernel(uint64_t limit_ns) {
+    __shared__ uint64_t full;
+    __shared__ LostCopies lost;
+    if (threadIdx.x != 0) return;
+    lost = LostCopies{};
+    mbar_init(&full, 1);
+    fence_mbar_init();
+    await_row(&full, RingPlace{}, &lost, &g_layer_norm_error, limit_ns);
+    drain_copies(&full, 1, &lost, limit_ns);
+}
+
+}  // namespace
+
+int layer_norm_wait_selftest(uint64_t limit_ns, cudaStream_t st) {
+    layer_norm_wait_selftest_kernel<<<1, 32, 0, st>>>(limit_ns);
+    return launch_status("layer_norm wait self-test kernel");
+}
+
 unsigned layer_norm_error_flags(bool clear) {
     unsigned v = 0;
     if (cudaMemcpyFromSymbol(&v, g_layer_norm_error, sizeof(v)) != cudaSuccess) return ~0u;

@@ -1280,6 +1280,18 @@ int mamba_selftest_bounded_wait(unsigned limit_us, void *stream) {
     return mb::bounded_wait_selftest(limit_us, static_cast<cudaStream_t>(stream)) ? -1 : 0;
 }
 
+int mamba_selftest_row_waits(unsigned limit_us, void *stream) {
+    mb::clear_error();
+    return guarded([&] {
+        MB_CHECK_ARG(limit_us > 0 && limit_us <= 1000000u, "selftest_row_waits: limit must be in (0, 1 s]");
+        const uint64_t limit_ns = (uint64_t)limit_us * 1000ull;
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (mb::layer_norm_wait_selftest(limit_ns, st) || mb::embedding_wait_selftest(limit_ns, st)) return -1;
+        MB_CUDA_TRY(cudaStreamSynchronize(st));
+        return 0;
+    });
+}
+
 int mamba_dt_rank(const MambaConfig *cfg) { return cfg ? (cfg->d_model + 15) / 16 : -1; }
 
 size_t mamba_weights_blob_size(const MambaConfig *cfg) {
