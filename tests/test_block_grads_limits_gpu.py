@@ -68,6 +68,30 @@ def test_steps_that_forget(cuda, b, L, D, N, kind):
     assert not bad, bad
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_masked_steps(cuda, kind):
+    """A delta of -inf, of the type's lowest value and of 16000: steps of length zero, which pass the state and
+    its gradient on (dt = a - 1 = 0, nothing of delta's gradient), and steps that forget all of it."""
+    b, L, D, N = 2, 37, 70, 6
+    v = _inputs(1, b, L, D, N, kind)
+    v["delta"] = (np.float32(0.3) * (v["delta"].astype(np.float32) - 16)).astype(_np(kind[1]))
+    lowest = np.finfo(_np(kind[1])).min
+    v["delta"][0, 3:7], v["delta"][1, 30:], v["delta"][0, 20], v["delta"][1, 9] = -np.inf, -np.inf, lowest, 16000
+    ref, mag = tr.scan_backward(v["dy"], v["x"], np.maximum(v["delta"], -1e4), v["A"], v["B"], v["C"], v["D"], v["z"],
+                                None, v["initial_state"], v["dfinal_state"])
+    got = _run(v)
+    terms = {"dA": b * L, "dD": b * L, "dB": D, "dC": D}
+    for k, g in got.items():
+        if g is None:
+            continue
+        u, tiny = (2.0 ** -11, 2.0 ** -25) if g.dtype == F16 else (2.0 ** -24, 2.0 ** -100)
+        d = 2.0 ** -24 * (64 + 8 * L + terms.get(k, 0)) + 2.0 ** -16 + (2.0 ** -16 if kind[0] == F16 else 0)
+        err = np.abs(g.double().cpu().numpy() - ref[k]) - (u * np.abs(ref[k]) + d * mag[k] + tiny)
+        assert err.max() <= 0, (k, err.max())
+    ddelta = got["ddelta"]
+    assert (ddelta[0, 3:7] == 0).all() and (ddelta[1, 30:] == 0).all() and (ddelta[0, 20] == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_beside_tensor_core_products(cuda, dtype):
     """Two streams whose kernels both keep values in tensor memory, one of them with a round of CTAs that hold
