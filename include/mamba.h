@@ -292,8 +292,9 @@ typedef struct MambaScanGrads {
 } MambaScanGrads;
 
 /* Scratch bytes of the call (0 for invalid args): 16-byte aligned device
- * memory, about 8 bytes per token and channel (a state of 16 FP32 numbers
- * every 8 tokens).  Calls that share it must not overlap on the GPU. */
+ * memory, 8 to 10 bytes per token and channel (a state of 16 FP32 numbers
+ * every 8 tokens, whatever dstate is; nor does the time depend on dstate).
+ * Calls that share it must not overlap on the GPU. */
 size_t mamba_selective_scan_backward_workspace(const MambaScanArgs *a);
 int mamba_selective_scan_backward(const MambaScanArgs *a, const MambaScanGrads *g, void *workspace,
                                   size_t workspace_bytes, void *stream);

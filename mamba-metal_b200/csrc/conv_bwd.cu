@@ -4,11 +4,11 @@
 // p_t = dy_t SiLU'(pre_t) (dy_t without the activation):
 //   dx_t = sum_k w_k p_{t+K-1-k},  dw_k = sum_t p_t x_{t-K+1+k},  dbias = sum_t p_t
 //
-// Bound by bytes and, near them, by issue slots (about 30 a FP16 element, packed
-// operations counted twice): one pass over x and dy that writes dx.  8 x 4096 x
-// 4096 FP16, K 4, SiLU: 160-168 us for 805 MB with 4 channels a thread and 128
-// registers (four CTAs an SM); with 154 registers 182, 102 registers 244, 2
-// channels a thread 227, 8 rows in flight instead of 4 203.  A thread owns VEC
+// One pass over x and dy that writes dx.  8 x 4096 x 4096 FP16, K 4, SiLU: 160-168
+// us for 805 MB with 4 channels a thread and 128 registers (four CTAs an SM); with
+// 154 registers 182, 102 registers 244, 2 channels a thread 227, 8 rows in flight
+// instead of 4 203.  Neither bytes (DRAM 60%) nor issue slots (51%) are used up:
+// 16 warps an SM with 4 rows of x and dy each in flight wait for memory.  A thread owns VEC
 // channels and a run of timesteps; the last K inputs and the last K p_t stay in
 // registers, so a run reads K - 1 rows before it (of x) and behind it (of
 // both) again.  The sums of dw and dbias leave as one partial row per run and
@@ -36,7 +36,10 @@ constexpr int kCbThreads = 128;
 constexpr int kCbRows = 4;  // rows of x and dy in flight
 
 // Channels a thread where rows allow it.  FP32: with 4 a thread needs 188
-// registers (8 x 4096 x 1000 115 us, with 2 93).
+// registers (8 x 4096 x 1000 115 us, with 2 93).  FP16 with 5 to 8 taps, 188 to 228
+// registers: 8 x 4096 x 4096 219, 242, 264, 301 us, with 2 channels 221, 282, 292,
+// 302; 8 x 4096 x 1000 63, 71, 78, 90 and 58, 82, 85, 90; 1 x 4096 x 2048 20.7,
+// 25.4, 27.4, 35.7 and 18.7, 25.8, 27.5, 31.6.
 template <typename T> constexpr int kWideChannels = sizeof(T) == 2 ? 4 : 2;
 
 // A row's VEC channels as loaded, and as pairs.

@@ -112,7 +112,10 @@ int launch_lookup(const LookupParams &p, bool vec, bool pairs, cudaStream_t st) 
 // four); above that each pass counts the
 // digits of every tile and then moves the tile's items, whose places a CTA
 // finds from the counts itself while there are few tiles (kFewTiles), and from
-// their running sums, made by a kernel in between, when there are many.
+// their running sums, made by a kernel in between, when there are many.  That
+// kernel is one CTA, whose time grows with the tokens: two passes over 2^17, 2^18
+// and 2^20 tokens 28, 54 and 210 us, beside 126, 243 and 927 for the sums of rows
+// of 256.
 constexpr int kDigitBits = 8, kDigits = 1 << kDigitBits;
 constexpr int kSortThreads = 256, kSortItems = 4, kSortTile = kSortThreads * kSortItems;
 constexpr int kSortWarps = kSortThreads / 32;

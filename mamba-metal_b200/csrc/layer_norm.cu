@@ -271,8 +271,9 @@ template <typename TX, typename TO> constexpr int kGroup = sizeof(TX) + sizeof(T
 constexpr int kLnThreads = 1024, kLnBwdThreads = 1536;
 constexpr int kLnBwdChannels = 16;  // channels a thread of the backward ring
 // Channels and resident threads per SM of the kernel that loads a row ahead.
-// Forward, FP32 to FP16 and FP16 to FP16: 71 and 61 us; 768 threads 88 and 73;
-// 64 channels a thread 137 and 63; through the ring, 8 channels a thread, 95 and 92.
+// Forward, FP32 to FP16 and FP16 to FP16: 72 and 61 us (bytes alone 62 and 41); 768
+// threads 88 and 73; 64 channels a thread 137 and 63; through the ring, 8 channels a
+// thread, 95 and 92.
 constexpr int kLnAheadChannels = 32, kLnAheadThreads = 1024;
 constexpr int kLnSumThreads = 1024;
 

@@ -43,7 +43,7 @@ namespace {
 
 constexpr int kT = 8;        // tokens between checkpoints
 constexpr int kCh = 128;     // channels (and threads) per CTA
-constexpr int kN = 16;       // states, padded
+constexpr int kN = 16;       // states, padded: fewer cost the same (8 x 2048 x 4096 with 4 states 3.17 ms, 16 3.17)
 constexpr int kHalf = kT / 2;  // tokens that a thread stages, of two channels
 
 struct ScanGradParams {
@@ -545,9 +545,11 @@ __device__ __forceinline__ void tmem_get(uint32_t at, float2 (&v)[4][2], float2 
 // so that the reverse steps do not evaluate it again; there the state behind a
 // token is loaded too (the next one's), which costs less than to compute it.
 //
-// About 40 instructions a state and token, 18 of them packed (which take two
-// issue slots), at 0.5 instructions a cycle and scheduler; DRAM 15%.  8 x 2048 x
-// 4096 FP16: 2.29 ms with two CTAs an SM and 255 registers.  Measured when e
+// 42 instructions a state and token, about 18 of them packed (which take two issue
+// slots), at 0.51 instructions a cycle and scheduler with two warps each: FMA pipe
+// 46%, special functions 14%, DRAM 6%, none of them full; warps wait for the
+// fixed latency of what they issued last as often as they issue.  8 x 2048 x 4096
+// FP16: 2.29 ms with two CTAs an SM and 255 registers.  Measured when e
 // stood for a as well (2.24): the states in shared memory 2.8 ms; three CTAs, 168
 // registers and 128 columns 3.07; two CTAs without e 2.77; scalar operations
 // 2.39; the next token's values loaded during the sums over lanes 2.28.
@@ -878,7 +880,8 @@ __global__ void __launch_bounds__(256) scan_bwd_sum_kernel(const ScanSumParams p
 // pass 3; several chunks add a tenth, and each a little to pass 2.  Taken: the
 // number of chunks for which the rounds of CTAs are shortest (of 8 x 2048 x 4096
 // and 3 x 333 x 203, 9 and 42 chunks: 3.13 ms and 55 us; 5 and 11 took 3.33 and
-// 90).  At most 16384 tokens, about 13 ms: a CTA keeps half of its SM's tensor
+// 90).  At most 16384 tokens, about 21 ms with two CTAs an SM (FP16; chunks of 8192
+// tokens take 10.4): a CTA keeps a half (FP32 a quarter) of its SM's tensor
 // memory as long.
 int chunk_length(int64_t batch, int64_t L, int64_t dim) {
     const int64_t ctas = batch * ceil_div64(dim, kCh), slots = 148 * 2, least_n = ceil_div64(L, 16384);
